@@ -243,6 +243,19 @@ void ox_session_free(ox_session*);
 /* ≙ Session::upload. Host layout = interp::Tensor (crates/onyxia-ir/src/interp.rs:29-49). */
 ox_status ox_session_upload(ox_session*, int32_t dtype, const uint64_t* shape, int32_t rank,
                             const void* bytes, size_t nbytes, ox_tensor** out);
+/* The same from memory of the session's device (no counterpart in the reference): a copy of `nbytes` from
+ * `device_bytes`, which holds what the CUDA stream `stream` has enqueued up to this call (NULL: the legacy default
+ * stream). Nothing waits on the host; what is enqueued on `stream` later runs behind the copy, so the memory may be
+ * written or freed in that stream's order. */
+ox_status ox_session_upload_device(ox_session*, int32_t dtype, const uint64_t* shape, int32_t rank,
+                                   const void* device_bytes, size_t nbytes, void* stream, ox_tensor** out);
+/* Device address of a densely packed tensor, for kernels of the caller's own on the session's device (no counterpart
+ * in the reference). What is enqueued on `stream` after the call runs behind everything the session has enqueued so
+ * far. The address is good while a handle of the tensor is held; before the last one is released, and before the
+ * session is to read what `stream` has written there, ox_session_after_stream orders the session's later work behind
+ * `stream`. */
+ox_status ox_session_device_view(ox_session*, const ox_tensor*, void* stream, void** device_ptr);
+ox_status ox_session_after_stream(ox_session*, void* stream);
 /* ≙ Session::run: inputs matched by name against the module signature; all
  * module outputs are returned in signature order. `out_names[i]` points into
  * session-owned storage; `out_tensors[i]` are new handles the caller releases. */

@@ -113,6 +113,9 @@ SIGNATURES = {
     "ox_backend_prepare": (C.c_int32, [_P, _P, C.POINTER(_P)]),
     "ox_session_free": (None, [_P]),
     "ox_session_upload": (C.c_int32, [_P, C.c_int32, _u64p, C.c_int32, _P, C.c_size_t, C.POINTER(_P)]),
+    "ox_session_upload_device": (C.c_int32, [_P, C.c_int32, _u64p, C.c_int32, _P, C.c_size_t, _P, C.POINTER(_P)]),
+    "ox_session_device_view": (C.c_int32, [_P, _P, _P, C.POINTER(_P)]),
+    "ox_session_after_stream": (C.c_int32, [_P, _P]),
     "ox_session_run": (C.c_int32, [_P, C.POINTER(C.c_char_p), C.POINTER(_P), C.c_int32, C.POINTER(C.c_char_p),
                                    C.POINTER(_P), C.c_int32, _i32p]),
     "ox_session_num_outputs": (C.c_int32, [_P]),

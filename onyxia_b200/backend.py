@@ -9,13 +9,14 @@ There is no CPU path behind this class.
 from __future__ import annotations
 
 import ctypes as C
+import math
 from typing import Sequence
 
 import numpy as np
 
 from . import _ffi
 from ._ffi import check
-from .ir import HostTensor, Module
+from .ir import _NP, BF16, BOOL, I4, U4, HostTensor, Module, storage_bytes
 
 
 class DeviceTensor:
@@ -58,6 +59,30 @@ class DeviceTensor:
             self._h = None
 
 
+class DeviceView:
+    """Memory of a tensor as ``__cuda_array_interface__`` (``torch.as_tensor`` and others take it without a copy); bf16 as whole
+    numbers of 16 bits. The view keeps the tensor; when it goes, the session's later work is ordered behind the view's stream."""
+
+    def __init__(self, session: "CudaSession", t: DeviceTensor, stream: int):
+        dtype, shape = t.describe()
+        if dtype in (U4, I4):
+            raise ValueError("packed 4-bit values have no array interface")
+        self._tensor = t.clone()
+        ptr = C.c_void_p()
+        check(session._lib.ox_session_device_view(session._h, t.handle, C.c_void_p(int(stream)), C.byref(ptr)))
+        self._session, self._stream = session, int(stream)
+        kind = "<i2" if dtype == BF16 else "|b1" if dtype == BOOL else np.dtype(_NP[dtype]).str
+        self.__cuda_array_interface__ = {"shape": shape, "typestr": kind, "data": (ptr.value or 0, False), "version": 2, "strides": None}
+
+    def __del__(self):
+        session = getattr(self, "_session", None)
+        if session is not None and session._h:
+            try:
+                session._lib.ox_session_after_stream(session._h, C.c_void_p(self._stream))
+            except Exception:
+                pass
+
+
 class CudaSession:
     """≙ ``impl Session`` of the reference GPU backend (session.rs:510-649)."""
 
@@ -71,6 +96,19 @@ class CudaSession:
         check(self._lib.ox_session_upload(self._h, t.dtype, shape, len(t.shape), t.data.ctypes.data_as(C.c_void_p),
                                           t.data.size, C.byref(out)))
         return DeviceTensor(out)
+
+    def upload_device(self, dtype: int, shape, address: int, stream: int = 0) -> DeviceTensor:
+        """A copy of densely packed memory of the session's device, as the CUDA stream `stream` leaves it; nothing waits on the host."""
+        shape = tuple(int(n) for n in shape)
+        dims = (C.c_uint64 * max(len(shape), 1))(*shape)
+        out = C.c_void_p()
+        check(self._lib.ox_session_upload_device(self._h, dtype, dims, len(shape), C.c_void_p(int(address)), storage_bytes(dtype, math.prod(shape)),
+                                                 C.c_void_p(int(stream)), C.byref(out)))
+        return DeviceTensor(out)
+
+    def view(self, t: DeviceTensor, stream: int = 0) -> DeviceView:
+        """The tensor's memory for other code on the session's device, to be used in the order of the CUDA stream `stream`."""
+        return DeviceView(self, t, stream)
 
     def run(self, inputs) -> list:
         """inputs: dict or sequence of (name, DeviceTensor) → [(name, DeviceTensor)] in signature order."""

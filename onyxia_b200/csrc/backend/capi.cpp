@@ -102,6 +102,33 @@ ox_status ox_session_upload(ox_session* s, int32_t dtype, const uint64_t* shape,
     OX_CATCH
 }
 
+ox_status ox_session_upload_device(ox_session* s, int32_t dtype, const uint64_t* shape, int32_t rank, const void* device_bytes,
+                                   size_t nbytes, void* stream, ox_tensor** out) {
+    OX_TRY
+    if (dtype < 0 || dtype >= kNumDTypes) fail(ErrKind::DType, "unknown dtype code");
+    std::vector<int64_t> shp;
+    for (int i = 0; i < rank; i++) shp.push_back((int64_t)shape[i]);
+    auto t = std::make_unique<ox_tensor>();
+    t->t = s->s->upload_device((DType)dtype, shp, device_bytes, nbytes, (cudaStream_t)stream);
+    *out = t.release();
+    return OX_OK;
+    OX_CATCH
+}
+
+ox_status ox_session_device_view(ox_session* s, const ox_tensor* t, void* stream, void** device_ptr) {
+    OX_TRY
+    *device_ptr = s->s->device_view(t->t, (cudaStream_t)stream);
+    return OX_OK;
+    OX_CATCH
+}
+
+ox_status ox_session_after_stream(ox_session* s, void* stream) {
+    OX_TRY
+    s->s->after_stream((cudaStream_t)stream);
+    return OX_OK;
+    OX_CATCH
+}
+
 ox_status ox_session_run(ox_session* s, const char* const* names, ox_tensor* const* inputs, int32_t n_in,
                          const char** out_names, ox_tensor** out_tensors, int32_t out_cap, int32_t* n_out) {
     OX_TRY

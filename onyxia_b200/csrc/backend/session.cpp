@@ -161,6 +161,7 @@ Session::~Session() {
     }
     if (ev_t0_) cudaEventDestroy(ev_t0_);
     if (ev_t1_) cudaEventDestroy(ev_t1_);
+    if (ev_order_) cudaEventDestroy(ev_order_);
     if (stream_) cudaStreamDestroy(stream_);
 }
 
@@ -721,6 +722,49 @@ std::vector<DTensor> Session::upload_together(const std::vector<HostPart>& parts
     const DTensor all = upload(DType::U8, {(int64_t)total}, flat.data(), total);
     for (auto& t : out) t.buf = all.buf;
     return out;
+}
+
+// What is enqueued on `then` from now on runs behind what is on `first` by now.
+void Session::order(cudaStream_t first, cudaStream_t then) {
+    if (!ev_order_) OX_CUDA(cudaEventCreateWithFlags(&ev_order_, cudaEventDisableTiming));
+    OX_CUDA(cudaEventRecord(ev_order_, first));
+    OX_CUDA(cudaStreamWaitEvent(then, ev_order_, 0));
+}
+
+DTensor Session::upload_device(DType dtype, const std::vector<int64_t>& shape, const void* bytes, size_t nbytes, cudaStream_t stream) {
+    OX_CUDA(cudaSetDevice(device_));
+    DTensor t;
+    t.dtype = dtype;
+    t.shape = shape;
+    if (t.nbytes() != nbytes)
+        fail(ErrKind::Interp, "tensor data size mismatch: " + std::to_string(nbytes) + " bytes for " + dtype_name(dtype) +
+                                  " (expected " + std::to_string(t.nbytes()) + ")");
+    if (nbytes) {
+        cudaPointerAttributes at{};
+        const cudaError_t err = cudaPointerGetAttributes(&at, bytes);
+        if (err != cudaSuccess) cudaGetLastError();
+        if (err != cudaSuccess || (at.type != cudaMemoryTypeDevice && at.type != cudaMemoryTypeManaged) || (at.type == cudaMemoryTypeDevice && at.device != device_))
+            fail(ErrKind::Runtime, "the bytes are not memory of the session's device");
+    }
+    t.buf = pool_->alloc(nbytes ? nbytes : 1);
+    if (!nbytes) return t;
+    order(stream, stream_);
+    OX_CUDA(cudaMemcpyAsync(t.buf->ptr, bytes, nbytes, cudaMemcpyDeviceToDevice, stream_));
+    order(stream_, stream);
+    return t;
+}
+
+void* Session::device_view(const DTensor& t, cudaStream_t stream) {
+    OX_CUDA(cudaSetDevice(device_));
+    if (!t.buf) fail(ErrKind::Runtime, "not a device tensor of this backend");
+    if (t.cap && t.shape.size() == 4 && t.cap != t.shape[2]) fail(ErrKind::Shape, "a view needs a densely packed tensor");
+    order(stream_, stream);
+    return t.ptr();
+}
+
+void Session::after_stream(cudaStream_t stream) {
+    OX_CUDA(cudaSetDevice(device_));
+    order(stream, stream_);
 }
 
 DTensor Session::zeros(DType dtype, const std::vector<int64_t>& shape) {

@@ -102,6 +102,10 @@ public:
         size_t nbytes;
     };
     std::vector<DTensor> upload_together(const std::vector<HostPart>& parts);
+    // The session's device memory beside other streams of the device.
+    DTensor upload_device(DType dtype, const std::vector<int64_t>& shape, const void* bytes, size_t nbytes, cudaStream_t stream);
+    void* device_view(const DTensor& t, cudaStream_t stream);
+    void after_stream(cudaStream_t stream);
     // f32 values of a dense f32 or f16 tensor; `cap` and `written` count values.
     void download_f32(const DTensor& t, float* dst, size_t cap, size_t* written);
     void open_landing();  // what the first download_f32 of f16 values would make
@@ -225,6 +229,8 @@ private:
     bool err_pending_ = false;
     std::list<std::unique_ptr<Plan>> plans_;  // most recently used first
     cudaEvent_t ev_t0_ = nullptr, ev_t1_ = nullptr;
+    cudaEvent_t ev_order_ = nullptr;  // between streams: a wait takes the event as it was recorded last
+    void order(cudaStream_t first, cudaStream_t then);
     // pinned staging for small uploads
     static constexpr size_t kStageBytes = 64 * 1024;
     static constexpr unsigned kStageSlots = 16;

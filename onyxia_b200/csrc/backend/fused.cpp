@@ -612,6 +612,59 @@ void paged_kv_lower(FusedCtx& c) {
     oxk::emit_paged_kv_attention(c.em, d, c.ins[0], c.ins[1], d.append ? c.outs[1] : c.ins[2], d.append ? c.outs[2] : c.ins[3], c.ins[4], c.ins[5], c.outs[0]);
 }
 
+// ── onyxia.DifferentialAttention ──
+// proj, turns per position, keys, values, seqs, pages, lambda [, gain of the heads' norm ("head_norm")] → out, keys, values. "dim" is that of one map: a head's two
+// queries, and a key head's two keys, stand side by side. The other attributes are those of onyxia.PagedKVAttention.
+bool differential_accepts(const Module& m, const Node& n) {
+    const Attrs& a = n.composite.attrs;
+    const bool head_norm = a.int_or("head_norm", 0) != 0;
+    if (n.inputs.size() != 7u + head_norm || n.outputs.size() != 3) return false;
+    const int64_t H = a.int_or("heads", 0), G = a.int_or("kv_heads", 0), D = a.int_or("dim", 0), V = a.int_or("vdim", 0), R = a.int_or("rot_dims", 0);
+    if (H <= 0 || G <= 0 || D <= 0 || V <= 0 || H > 65535 || D > 8192 || V > 8192 || H % G != 0 || R < 0 || R > D || R % 2 != 0) return false;
+    if (a.int_or("window", 0) < 0 || a.int_or("window", 0) > INT32_MAX) return false;
+    for (const char* f : {"softcap", "epsilon", "head_epsilon"})
+        if (!(a.float_or(f, 0.0) >= 0.0) || !std::isfinite(a.float_or(f, 0.0))) return false;
+    if (!std::isfinite(a.float_or("scale", 1.0))) return false;
+    const TensorType &x = ty(m, n.inputs[0]), &turns = ty(m, n.inputs[1]), &keys = ty(m, n.inputs[2]), &values = ty(m, n.inputs[3]);
+    const TensorType &seqs = ty(m, n.inputs[4]), &pages = ty(m, n.inputs[5]), &out = ty(m, n.outputs[0]);
+    auto width = x.shape.size() == 2 ? x.shape[1].as_const() : std::nullopt;
+    if (!is_act(x.dtype) || !width) return false;
+    for (auto [name, cols] : {std::pair<const char*, int64_t>{"q_offset", H * 2 * D}, {"k_offset", G * 2 * D}, {"v_offset", G * V}})
+        if (a.int_or(name, 0) < 0 || a.int_or(name, 0) > (int64_t)*width - cols) return false;
+    if (!is_f32_vector(m, n.inputs[6], (uint64_t)H) || (head_norm && !is_f32_vector(m, n.inputs[7], (uint64_t)V))) return false;
+    if (turns.dtype != DType::F32 || turns.shape.size() != 2 || !is_const(turns.shape[0], 2) || (R > 0 && !is_const(turns.shape[1], R / 2))) return false;
+    for (auto [t, d] : {std::pair<const TensorType*, int64_t>{&keys, 2 * D}, {&values, V}})
+        if (t->dtype != x.dtype || t->shape.size() != 4 || !is_const(t->shape[1], G) || !t->shape[2].as_const() || !is_const(t->shape[3], d)) return false;
+    for (int i : {1, 2})
+        if (ty(m, n.outputs[i]).dtype != x.dtype || ty(m, n.outputs[i]).shape != ty(m, n.inputs[1 + i]).shape) return false;
+    const uint64_t page = *keys.shape[2].as_const();
+    if (page == 0 || page > (1u << 30) || (page & (page - 1)) != 0 || values.shape[0] != keys.shape[0] || values.shape[2] != keys.shape[2]) return false;
+    if (seqs.dtype != DType::I32 || seqs.shape.size() != 2 || !is_const(seqs.shape[1], 4)) return false;
+    if (pages.dtype != DType::I32 || pages.shape.size() != 2 || pages.shape[0] != seqs.shape[0]) return false;
+    return out.dtype == x.dtype && out.shape.size() == 2 && out.shape[0] == x.shape[0] && is_const(out.shape[1], H * V);
+}
+void differential_lower(FusedCtx& c) {
+    const Attrs& a = c.node.composite.attrs;
+    oxk::DifferentialDesc d{};
+    d.heads = a.int_("heads");
+    d.kv_heads = a.int_("kv_heads");
+    d.dim = a.int_("dim");
+    d.vdim = a.int_("vdim");
+    d.page = c.ins[2].shape[2];
+    d.q_off = a.int_or("q_offset", 0);
+    d.k_off = a.int_or("k_offset", 0);
+    d.v_off = a.int_or("v_offset", 0);
+    d.rot_dims = a.int_or("rot_dims", 0);
+    d.window = a.int_or("window", 0);
+    d.scale = a.float_or("scale", 1.0);
+    d.softcap = a.float_or("softcap", 0.0);
+    d.eps = a.float_or("epsilon", 1e-6);
+    d.norm = a.int_or("norm", 0) != 0;
+    d.sink = a.int_or("sink", 0) != 0;
+    d.head_eps = a.float_or("head_epsilon", 1e-6);
+    oxk::emit_differential(c.em, d, c.ins[0], c.ins[1], c.outs[1], c.outs[2], c.ins[4], c.ins[5], c.ins[6], a.int_or("head_norm", 0) != 0 ? &c.ins[7] : nullptr, c.outs[0]);
+}
+
 // ── onyxia.LatentAttention ──
 // queries in the latent space, queries, proj, norm weight, turns per position, pool, seqs, pages → out, pool
 bool latent_accepts(const Module& m, const Node& n) {
@@ -839,6 +892,7 @@ const KernelRegistry& standard_kernels() {
         r.add({"onyxia.GatedRecurrence", recurrence_accepts, recurrence_lower, {{1, 8}, {2, 9}}});
         r.add({"onyxia.PagedKVAttention", paged_kv_accepts, paged_kv_lower, {{1, 2}, {2, 3}}});
         r.add({"onyxia.SharedKVAttention", shared_kv_accepts, paged_kv_lower});
+        r.add({"onyxia.DifferentialAttention", differential_accepts, differential_lower, {{1, 2}, {2, 3}}});
         r.add({"onyxia.LightningAttention", lightning_accepts, lightning_lower, {{1, 2}}});
         r.add({"onyxia.GatedLinearAttention", gated_linear_accepts, gated_linear_lower, {{1, 2}}});
         r.add({"onyxia.GatedDeltaRule", delta_accepts, delta_lower, {{1, 4}, {2, 5}}});

@@ -454,6 +454,21 @@ struct PagedKvDesc {
 void emit_paged_kv_attention(Emitter&, const PagedKvDesc&, const TRef& proj, const TRef& turns, const TRef& keys, const TRef& values,
                              const TRef& seqs, const TRef& pages, const TRef& out);
 
+struct DifferentialDesc {
+    int64_t heads, kv_heads, dim, vdim, page;  // dim: of one map's query or key; page: a power of two
+    int64_t q_off, k_off, v_off;  // columns of the fused projection: head h's two queries from q_off + h · 2 · dim on, a key head's two keys likewise
+    int64_t rot_dims;             // leading dimensions of a query or key that rotate in two halves; 0: none
+    int64_t window;               // keys a position sees, itself among them; 0: all
+    double scale, softcap, eps;   // softcap 0: none
+    bool norm;                    // queries and keys divided by their root mean square over `dim` after the rotation
+    bool sink;                    // a score of 0 without a value in both softmax maps
+    double head_eps;              // of the norm of a head's result, where there is one
+};
+// Causal attention of the difference of two softmax maps over pools of keys [pages, kv_heads, page, 2 · dim] and values [pages, kv_heads, page, vdim].
+// `lambda` F32 [heads]: the second map's factor. `gain` F32 [vdim] or null: a head's result is divided by its root mean square and multiplied by it.
+void emit_differential(Emitter&, const DifferentialDesc&, const TRef& proj, const TRef& turns, const TRef& keys, const TRef& values, const TRef& seqs,
+                       const TRef& pages, const TRef& lambda, const TRef* gain, const TRef& out);
+
 // Attention whose keys and values are one latent per token that all heads share: key = (latent, rotated part), value =
 // latent. Queries come with their unrotated part already mapped into the latent space (`q_latent` [rows, heads · rank]) and with
 // their rotated part in `q` (head h's from column h · q_step + q_off on). The new latents are columns of `proj` from kv_off

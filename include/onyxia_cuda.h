@@ -323,7 +323,28 @@ ox_status ox_session_argmax_last(ox_session*, const ox_tensor* logits, ox_tensor
  * synchronising call. Returns an I64 tensor shaped like `logits` without its last axis. */
 ox_status ox_session_sample_last(ox_session*, const ox_tensor* logits, float temperature, int64_t top_k, float top_p,
                                  const float* uniform, size_t n_uniform, ox_tensor** out);
-/* The same argmax written into a tensor the caller already holds, without
+/* The rules of requests on the logits of their next tokens (no counterpart in the reference), one row of logits per
+ * request, in front of ox_session_argmax_last or ox_session_sample_last. In this order and in f32, for row r:
+ *   a token of its history:             l <- l > 0 ? l / repetition : l * repetition      (repetition > 0; 1: none)
+ *   said n > 0 times in the answer:     l <- l - n * frequency - presence                 (0: none)
+ *   the token's biases, added up in their order
+ *   not allowed by the row's mask:      l <- -infinity
+ * All tensors are densely packed; NULL stands for no such rule. `history`, `lengths` and `penalties` come together, as
+ * do `bias_ids` and `bias` (at most 4096 of a row; a token may be listed more than once). Tokens outside the
+ * vocabulary, lengths outside the history and masks that are not there are reported as OX_ERR_RUNTIME at the next
+ * synchronising call. A row whose mask allows nothing is all -infinity: sampling reports it, argmax takes the last index. */
+typedef struct ox_logit_rules {
+    const ox_tensor* history;   /* I32 [rows, width]: the prompt's tokens, then the answer's */
+    const ox_tensor* lengths;   /* I32 [rows, 2]: tokens of the prompt, tokens of both */
+    const ox_tensor* penalties; /* F32 [rows, 3]: repetition, frequency, presence */
+    const ox_tensor* bias_ids;  /* I32 [rows, n]; negative: none */
+    const ox_tensor* bias;      /* F32 [rows, n] */
+    const ox_tensor* masks;     /* U32 [n_masks, ceil(vocab / 32)]: a set bit allows a token, lowest bit first */
+    const ox_tensor* mask_of;   /* I32 [rows]: the row's mask, negative: none; NULL: row r has mask r */
+} ox_logit_rules;
+/* `logits`: F32 or F16. Returns an F32 tensor of the same shape. */
+ox_status ox_session_constrain_last(ox_session*, const ox_tensor* logits, const ox_logit_rules* rules, ox_tensor** out);
+/* The argmax of ox_session_argmax_last written into a tensor the caller already holds, without
  * allocating anything: no device allocation, no buffer from the session's pool,
  * no new tensor handle. One kernel is enqueued on the session's stream; its
  * scratch is a fixed array inside the library's device image. This entry point

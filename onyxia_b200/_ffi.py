@@ -68,6 +68,10 @@ class EngineToken(C.Structure):
     _fields_ = [("request", C.c_int64), ("token", C.c_int64), ("finished", C.c_int32)]
 
 
+class LogitRules(C.Structure):
+    _fields_ = [(name, C.c_void_p) for name in ("history", "lengths", "penalties", "bias_ids", "bias", "masks", "mask_of")]
+
+
 class KernelTiming(C.Structure):
     _fields_ = [("kernel", C.c_char_p), ("node", C.c_char_p), ("time_ns", C.c_uint64)]
 
@@ -135,6 +139,7 @@ SIGNATURES = {
     "ox_session_launch_count": (C.c_uint64, [_P]),
     "ox_session_plan_stats": (None, [_P, _u64p]),
     "ox_session_argmax_last": (C.c_int32, [_P, _P, C.POINTER(_P)]),
+    "ox_session_constrain_last": (C.c_int32, [_P, _P, C.POINTER(LogitRules), C.POINTER(_P)]),
     "ox_session_argmax_last_into": (C.c_int32, [_P, _P, _P]),
     "ox_session_sample_last": (C.c_int32, [_P, _P, C.c_float, C.c_int64, C.c_float, C.POINTER(C.c_float), C.c_size_t, C.POINTER(_P)]),
     "ox_llm_create": (C.c_int32, [_P, C.c_int64, C.POINTER(_P)]),

@@ -145,6 +145,17 @@ class CudaSession:
                                                u.ctypes.data_as(C.POINTER(C.c_float)), u.size, C.byref(out)))
         return DeviceTensor(out)
 
+    def constrain_last(self, logits: DeviceTensor, *, history: DeviceTensor | None = None, lengths: DeviceTensor | None = None,
+                       penalties: DeviceTensor | None = None, bias_ids: DeviceTensor | None = None, bias: DeviceTensor | None = None,
+                       masks: DeviceTensor | None = None, mask_of: DeviceTensor | None = None) -> DeviceTensor:
+        """Penalties for repeated tokens, biases and masks of allowed tokens on rows of logits, in front of `argmax_last` or `sample_last`
+        (``ox_session_constrain_last`` gives the operands' types and shapes): f32 logits of the same shape."""
+        operands = dict(history=history, lengths=lengths, penalties=penalties, bias_ids=bias_ids, bias=bias, masks=masks, mask_of=mask_of)
+        rules = _ffi.LogitRules(**{k: t.handle for k, t in operands.items() if t is not None})
+        out = C.c_void_p()
+        check(self._lib.ox_session_constrain_last(self._h, logits.handle, C.byref(rules), C.byref(out)))
+        return DeviceTensor(out)
+
     def argmax_last_into(self, t: DeviceTensor, out: DeviceTensor) -> None:
         """Argmax over the last axis written into `out` (I64, one element per row); allocates nothing."""
         check(self._lib.ox_session_argmax_last_into(self._h, t.handle, out.handle))

@@ -266,6 +266,19 @@ ox_status ox_session_sample_last(ox_session* s, const ox_tensor* logits, float t
     OX_CATCH
 }
 
+ox_status ox_session_constrain_last(ox_session* s, const ox_tensor* logits, const ox_logit_rules* rules, ox_tensor** out) {
+    OX_TRY
+    auto of = [](const ox_tensor* t) { return t ? &t->t : nullptr; };
+    oxrt::Rules r;
+    r.history = of(rules->history), r.lengths = of(rules->lengths), r.penalties = of(rules->penalties);
+    r.bias_ids = of(rules->bias_ids), r.bias = of(rules->bias), r.masks = of(rules->masks), r.mask_of = of(rules->mask_of);
+    auto t = std::make_unique<ox_tensor>();
+    t->t = s->s->constrain_last(logits->t, r);
+    *out = t.release();
+    return OX_OK;
+    OX_CATCH
+}
+
 ox_status ox_session_argmax_last_into(ox_session* s, const ox_tensor* logits, ox_tensor* out) {
     OX_TRY
     s->s->argmax_last_into(logits->t, out->t);

@@ -799,6 +799,9 @@ void Session::check_device_error() {
         case oxk::ERR_INT_POW_NEG: what = "integer pow with negative exponent"; break;
         case oxk::ERR_WAIT_TIMEOUT: what = "a bounded device-side wait gave up"; break;
         case oxk::ERR_SAMPLE_NO_FINITE: what = "All logits are NaN or Inf, cannot sample (row " + std::to_string(e.a) + ")"; break;
+        case oxk::ERR_RULES_TOKEN: what = "rules: token " + std::to_string(e.a) + " is not one of " + std::to_string(e.b); break;
+        case oxk::ERR_RULES_LENGTH: what = "rules: the lengths of row " + std::to_string(e.a) + " do not fit a history of " + std::to_string(e.b); break;
+        case oxk::ERR_RULES_MASK: what = "rules: mask " + std::to_string(e.a) + " is not one of " + std::to_string(e.b); break;
         default: what = "device error code " + std::to_string(e.code);
     }
     fail(ErrKind::Runtime, kind + " (node '" + node + "'): " + what);
@@ -944,6 +947,40 @@ DTensor Session::sample_last(const DTensor& logits, float temperature, long long
         for (auto& rl : r.relocs)
             if (rl.buf.slot == oxk::kSlotErr) rl.buf = Buf{3, rl.buf.off};
     launch_now(em, {logits.ptr(), out.ptr(), ud.ptr(), (void*)d_err_});
+    OX_CUDA(cudaMemcpyAsync(h_err_, d_err_, sizeof(oxk::ErrWord), cudaMemcpyDeviceToHost, stream_));
+    err_pending_ = true;
+    return out;
+}
+
+DTensor Session::constrain_last(const DTensor& logits, const Rules& rules) {
+    OX_CUDA(cudaSetDevice(device_));
+    check_rules(logits, rules);
+    DTensor out;
+    out.dtype = DType::F32;
+    out.shape = logits.shape;
+    out.buf = pool_->alloc(std::max<size_t>(out.nbytes(), 4));
+    oxk::Emitter em;
+    std::vector<void*> slots = {logits.ptr(), out.ptr(), (void*)d_err_};
+    auto slot = [&](const DTensor* t) {
+        if (!t) return Buf{oxk::kSlotNull, 0};
+        slots.push_back(t->ptr());
+        return Buf{(uint32_t)slots.size() - 1, 0};
+    };
+    oxk::LogitRules r;
+    const bool biased = rules.bias_ids && rules.bias_ids->shape[1] > 0;
+    r.history = slot(rules.history), r.lengths = slot(rules.lengths), r.penalties = slot(rules.penalties);
+    r.bias_ids = slot(biased ? rules.bias_ids : nullptr), r.bias = slot(biased ? rules.bias : nullptr);
+    r.masks = slot(rules.masks), r.mask_of = slot(rules.mask_of);
+    r.width = rules.history ? rules.history->shape[1] : 0;
+    r.n_bias = biased ? rules.bias_ids->shape[1] : 0;
+    r.n_masks = rules.masks ? rules.masks->shape[0] : 0;
+    r.aligned = reinterpret_cast<uintptr_t>(logits.ptr()) % (logits.dtype == DType::F32 ? 16 : 8) == 0;
+    TRef x{Buf{0, 0}, (int)logits.dtype, logits.shape, 0}, y{Buf{1, 0}, (int)DType::F32, out.shape, 0};
+    oxk::emit_logit_rules(em, x, y, r);
+    for (auto& rec : em.recs)
+        for (auto& rl : rec.relocs)
+            if (rl.buf.slot == oxk::kSlotErr) rl.buf = Buf{2, rl.buf.off};
+    launch_now(em, slots);
     OX_CUDA(cudaMemcpyAsync(h_err_, d_err_, sizeof(oxk::ErrWord), cudaMemcpyDeviceToHost, stream_));
     err_pending_ = true;
     return out;

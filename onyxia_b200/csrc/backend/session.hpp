@@ -4,6 +4,7 @@
 #include <list>
 
 #include "landing.hpp"
+#include "rules.hpp"
 #include "runtime.hpp"
 #include "../kernels/persist.hpp"
 
@@ -118,6 +119,7 @@ public:
     void download_async(const DTensor& t, void* pinned_dst);
     DTensor argmax_last(const DTensor& logits);
     DTensor sample_last(const DTensor& logits, float temperature, long long top_k, float top_p, const float* u, size_t n_u);
+    DTensor constrain_last(const DTensor& logits, const Rules& rules);
     void argmax_last_into(const DTensor& logits, const DTensor& out);
     void wait_idle();
     void timer_start();

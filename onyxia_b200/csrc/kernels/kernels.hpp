@@ -30,6 +30,9 @@ enum : int {
     ERR_SLICE_OOB = 5,
     ERR_WAIT_TIMEOUT = 6,
     ERR_SAMPLE_NO_FINITE = 7,
+    ERR_RULES_TOKEN = 8,
+    ERR_RULES_LENGTH = 9,
+    ERR_RULES_MASK = 10,
 };
 
 struct ErrWord {
@@ -251,6 +254,15 @@ struct GqaDesc {
 void emit_gqa(Emitter&, const GqaDesc&, const TRef& q, const TRef& k, const TRef& v, const TRef& past_k,
               const TRef& past_v, const TRef& seqlens, const TRef* cos, const TRef* sin, const TRef* bias,
               const TRef& out, const TRef& present_k, const TRef& present_v);
+
+// The rules of rows of logits (F32 or F16) on their way to the sampler; `out` F32. Without a history, biases or masks their buffers resolve to null.
+// `aligned`: the logits begin on a boundary of four.
+struct LogitRules {
+    Buf history, lengths, penalties, bias_ids, bias, masks, mask_of;
+    int64_t width = 0, n_bias = 0, n_masks = 0;
+    bool aligned = false;
+};
+void emit_logit_rules(Emitter&, const TRef& logits, const TRef& out, const LogitRules&);
 
 // The decode step (S = 1) over an in-place cache as one launch of thread-block
 // clusters; false when the shape is outside what that kernel handles. `t_size`

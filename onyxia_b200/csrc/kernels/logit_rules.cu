@@ -1,0 +1,164 @@
+// What a request's rules make of the logits of its next token, per row:
+//
+//   t in the row's history (prompt and answer):  l ← l > 0 ? l / repetition : l · repetition
+//   t said n > 0 times in the answer:            l ← l − n · frequency − presence
+//   biases of t:                                 l ← l + Σ, in the order they are listed
+//   t not in the row's mask:                     l ← −∞
+//
+// in f32, the result too (a half-precision logit times a penalty would be rounded again and could leave its range).
+//
+// A CTA takes a run of one row's vocabulary: it counts the row's history in shared memory (whole numbers: no order shows), streams the run and, last, writes the few
+// biased tokens again. The history is read once per run. Bound by the logits' bytes: read once, written once as f32.
+#include "common.cuh"
+#include "kernels.hpp"
+
+namespace oxk {
+
+namespace {
+
+constexpr int kRuleThreads = 256;
+
+struct RulesP {
+    const void* x;           // [rows, cols] logits
+    float* y;                // [rows, cols]
+    const int* history;      // [rows, width], or null
+    const int* lengths;      // [rows, 2]: tokens of the prompt, tokens of both
+    const float* penalties;  // [rows, 3]: repetition, frequency, presence
+    const int* bias_ids;     // [rows, n_bias], or null; negative: none
+    const float* bias;       // [rows, n_bias]
+    const unsigned* masks;   // [n_masks, words], or null
+    const int* mask_of;      // [rows], or null: row r has mask r; negative: none
+    ErrWord* err;
+    long long rows, cols;
+    int width, n_bias, n_masks, words, node;
+};
+
+// PER groups of four tokens per thread; VEC: rows begin on 16 bytes.
+template <int DT, int PER, bool VEC> __global__ void __launch_bounds__(kRuleThreads) constrain_rows(const RulesP p) {
+    constexpr int kRun = kRuleThreads * PER * 4;
+    __shared__ unsigned times[kRun];  // how often a token was said, the top bit: it is in the prompt
+    const long long row = blockIdx.y, c0 = (long long)blockIdx.x * kRun, base = row * p.cols;
+    const int tid = threadIdx.x, n = (int)min((long long)kRun, p.cols - c0);
+    auto token = [&](int i, int e) { return VEC ? (i * kRuleThreads + tid) * 4 + e : (i * 4 + e) * kRuleThreads + tid; };
+    float v[PER][4];
+#pragma unroll
+    for (int i = 0; i < PER; i++) {
+        if constexpr (VEC) {
+            const int c = token(i, 0);
+            if (c < n) {
+                if constexpr (DT == DT_F32) {
+                    const float4 f = *reinterpret_cast<const float4*>((const float*)p.x + base + c0 + c);
+                    v[i][0] = f.x, v[i][1] = f.y, v[i][2] = f.z, v[i][3] = f.w;
+                } else {
+                    const uint2 u = *reinterpret_cast<const uint2*>((const __half*)p.x + base + c0 + c);
+                    const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&u.x)), b = __half22float2(*reinterpret_cast<const __half2*>(&u.y));
+                    v[i][0] = a.x, v[i][1] = a.y, v[i][2] = b.x, v[i][3] = b.y;
+                }
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                if (token(i, e) < n) v[i][e] = ld<DT>(p.x, base + c0 + token(i, e));
+        }
+    }
+    float repetition = 1.f, frequency = 0.f, presence = 0.f;
+    if (p.history) {
+        for (int c = tid; c < kRun; c += kRuleThreads) times[c] = 0u;
+        int prompt = p.lengths[2 * row], total = p.lengths[2 * row + 1];
+        if (prompt < 0 || prompt > total || total > p.width) {
+            if (blockIdx.x == 0 && tid == 0) report(p.err, ERR_RULES_LENGTH, p.node, row, p.width);
+            total = max(0, min(total, p.width));
+            prompt = max(0, min(prompt, total));
+        }
+        repetition = p.penalties[3 * row], frequency = p.penalties[3 * row + 1], presence = p.penalties[3 * row + 2];
+        __syncthreads();
+        const int* h = p.history + row * p.width;
+        for (int i = tid; i < total; i += kRuleThreads) {
+            const int t = h[i];
+            const long long c = t - c0;
+            if (c >= 0 && c < n) {
+                if (i < prompt) atomicOr(&times[c], 0x80000000u);
+                else atomicAdd(&times[c], 1u);
+            } else if (blockIdx.x == 0 && (t < 0 || t >= p.cols)) {
+                report(p.err, ERR_RULES_TOKEN, p.node, t, p.cols);
+            }
+        }
+        __syncthreads();
+    }
+    auto penalised = [&](float l, unsigned said) {
+        if (said == 0u) return l;
+        l = l > 0.f ? l / repetition : l * repetition;
+        const unsigned k = said & 0x7FFFFFFFu;
+        return k ? l - (float)k * frequency - presence : l;
+    };
+    const unsigned* mask = nullptr;
+    if (p.masks) {
+        const int m = p.mask_of ? p.mask_of[row] : (int)row;
+        if (m < p.n_masks) mask = m >= 0 ? p.masks + (long long)m * p.words : nullptr;
+        else if (blockIdx.x == 0 && tid == 0) report(p.err, ERR_RULES_MASK, p.node, m, p.n_masks);
+    }
+    auto allowed = [&](long long t) { return !mask || (mask[t >> 5] >> (t & 31) & 1u); };
+#pragma unroll
+    for (int i = 0; i < PER; i++) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const int c = token(i, e);
+            if (c >= n) continue;
+            if (p.history) v[i][e] = penalised(v[i][e], times[c]);
+            if (!allowed(c0 + c)) v[i][e] = -INFINITY;
+            if (!VEC) p.y[base + c0 + c] = v[i][e];
+        }
+        if (VEC && token(i, 0) < n) *reinterpret_cast<float4*>(p.y + base + c0 + token(i, 0)) = make_float4(v[i][0], v[i][1], v[i][2], v[i][3]);
+    }
+    if (!p.bias_ids) return;
+    __syncthreads();  // behind the plain results
+    const int* ids = p.bias_ids + row * p.n_bias;
+    const float* bias = p.bias + row * p.n_bias;
+    for (int j = tid; j < p.n_bias; j += kRuleThreads) {
+        const int t = ids[j];
+        const long long c = t - c0;
+        if (t >= p.cols && blockIdx.x == 0) report(p.err, ERR_RULES_TOKEN, p.node, t, p.cols);
+        if (t < 0 || c < 0 || c >= n || !allowed(t)) continue;
+        float l = ld<DT>(p.x, base + t);
+        if (p.history) l = penalised(l, times[c]);
+        float more = 0.f;
+        bool first = true;  // a token that is listed again has the sum from its first place
+        for (int k = 0; k < p.n_bias; k++)
+            if (ids[k] == t) {
+                if (k < j) {
+                    first = false;
+                    break;
+                }
+                more += bias[k];
+            }
+        if (first) p.y[base + t] = l + more;
+    }
+}
+
+template <int DT> void emit_rules_of(Emitter& em, const RulesP& p, bool vec, std::initializer_list<std::pair<const void*, Buf>> ptrs) {
+    auto go = [&](void (*k)(const RulesP), int per) {
+        const long long run = (long long)kRuleThreads * per * 4;
+        em.launch(k, dim3((unsigned)((p.cols + run - 1) / run), (unsigned)p.rows), dim3(kRuleThreads), 0, p, ptrs, "constrain_rows");
+    };
+    vec ? go(constrain_rows<DT, 4, true>, 4) : go(constrain_rows<DT, 4, false>, 4);
+}
+
+}  // namespace
+
+void emit_logit_rules(Emitter& em, const TRef& logits, const TRef& out, const LogitRules& r) {
+    RulesP p{};
+    p.cols = logits.shape.back();
+    p.rows = p.cols ? logits.numel() / p.cols : 0;
+    if (p.rows == 0) return;
+    p.width = (int)r.width;
+    p.n_bias = (int)r.n_bias;
+    p.n_masks = (int)r.n_masks;
+    p.words = (int)((p.cols + 31) / 32);
+    p.node = em.node;
+    const std::initializer_list<std::pair<const void*, Buf>> ptrs = {{&p.x, logits.buf}, {&p.y, out.buf}, {&p.history, r.history}, {&p.lengths, r.lengths}, {&p.penalties, r.penalties},
+                                                                   {&p.bias_ids, r.bias_ids}, {&p.bias, r.bias}, {&p.masks, r.masks}, {&p.mask_of, r.mask_of}, {&p.err, Buf{kSlotErr, 0}}};
+    const bool vec = p.cols % 4 == 0 && r.aligned;
+    logits.dtype == DT_F32 ? emit_rules_of<DT_F32>(em, p, vec, ptrs) : emit_rules_of<DT_F16>(em, p, vec, ptrs);
+}
+
+}  // namespace oxk

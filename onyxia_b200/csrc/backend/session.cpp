@@ -802,6 +802,7 @@ void Session::check_device_error() {
         case oxk::ERR_RULES_TOKEN: what = "rules: token " + std::to_string(e.a) + " is not one of " + std::to_string(e.b); break;
         case oxk::ERR_RULES_LENGTH: what = "rules: the lengths of row " + std::to_string(e.a) + " do not fit a history of " + std::to_string(e.b); break;
         case oxk::ERR_RULES_MASK: what = "rules: mask " + std::to_string(e.a) + " is not one of " + std::to_string(e.b); break;
+        case oxk::ERR_BATCH_ROWS: what = "sequence " + std::to_string(e.a) + " has " + std::to_string(e.b) + " new tokens in a batch of no more rows than sequences"; break;
         default: what = "device error code " + std::to_string(e.code);
     }
     fail(ErrKind::Runtime, kind + " (node '" + node + "'): " + what);

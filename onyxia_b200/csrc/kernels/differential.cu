@@ -8,7 +8,10 @@
 // Queries and keys rotate and are normed as in paged_kv_attention.cu, each map by itself. A pool's key is the two maps' side by side.
 //
 //   differential_prepare   rotated, normed queries; the new keys and values go to the pools
+//   differential_decode    sequences with one new token: their keys split over CTAs and warps, all of the above in one launch
 //   differential_simt      any shape, f32 and bf16
+//
+// Decode reads min(past, window) · kv_heads · (2 · dim + vdim) · 2 bytes per sequence.
 #include "differential.cuh"
 
 namespace oxk {
@@ -44,7 +47,7 @@ template <typename T> __global__ void __launch_bounds__(kAnyKeys) differential_s
     pdl_enter();
     const int row = blockIdx.x, h = blockIdx.y, tid = threadIdx.x, s = find_seq(p.seqs, p.n_seqs, row);
     const SeqRow sq = load_seq(p.seqs, s);
-    if (row < sq.start || row >= sq.start + sq.len) return;
+    if (row < sq.start || row >= sq.start + sq.len || (sq.len == 1 && !p.singles)) return;
     const int pos = sq.past + row - sq.start, g = h / (p.heads / p.kv_heads);
     float *q = sm, *acc = sm + 2 * p.dim, *w = acc + 2 * p.vdim;
     for (int i = tid; i < 2 * p.dim; i += kAnyKeys) q[i] = to_f(((const T*)p.q)[((long long)row * p.heads + h) * 2 * p.dim + i]);
@@ -88,7 +91,318 @@ template <typename T> __global__ void __launch_bounds__(kAnyKeys) differential_s
     for (int i = tid; i < p.vdim; i += kAnyKeys) ((T*)p.out)[((long long)row * p.heads + h) * p.vdim + i] = from_f<T>(p.gain ? acc[i] * f * p.gain[i] : acc[i]);
 }
 
+// ───────────────────────────── single tokens ────────────────────────────
+constexpr int kDecWarps = 4, kDecThreads = kDecWarps * 32, kDecPages = 256, kDecHeads = 8, kDecKeys = 16;
+constexpr float kNoScore = -1e30f;  // below every score, and finite: differences stay numbers
+
+// DM, DV: dimensions of a map and of a value, padded
+template <int DM, int DV> struct DecSmem {
+    static constexpr int stages = DM <= 64 && DV <= 128 ? 3 : 2;
+    static constexpr int q_stride = DM * 2 + 16, k_stride = DM * 4 + 16, v_stride = DV * 2 + 16;
+    static constexpr int tile = kDecKeys * (k_stride + v_stride);  // keys, then values
+    static constexpr int q = 0;                                    // [map][high, low][8 heads]
+    static constexpr int kv = 4 * kDecHeads * q_stride;            // [warps][stages][tile]
+    static constexpr int ring = kDecWarps * stages * tile;
+    static constexpr int part = part_size(2 * kDecHeads, DV);      // floats of one partial result, rows [map][8 heads]
+    static constexpr int merge = kDecWarps * part * 4;             // reuses the ring after the last key
+    static constexpr int angle = kv + (ring > merge ? ring : merge);
+    static constexpr int total = angle + DM * 4;
+};
+
+// The difference of the two maps' results, from `n` partial results ([n][map][8 heads][DV + 2]: maximum, sum, accumulator), a warp per head.
+template <int DV> __device__ void merge_maps(const DiffP& p, const float* part, int n, int h0, int heads, bf16* out) {
+    constexpr int size = part_size(2 * kDecHeads, DV), C = (DV + 31) / 32;
+    const int lane = threadIdx.x & 31;
+    for (int r = threadIdx.x >> 5; r < heads; r += kDecWarps) {
+        float o[C] = {};
+#pragma unroll
+        for (int m = 0; m < 2; m++) {
+            // lane i weighs parts i and i + 32 (n ≤ 64); a part that saw no key has the maximum kNoScore, sum and values 0
+            const float* head = part + (m * kDecHeads + r) * (DV + 2);
+            float pm[2], pl[2];
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+                const bool in = k * 32 + lane < n;
+                pm[k] = in ? head[(long long)(k * 32 + lane) * size] : kNoScore;
+                pl[k] = in ? head[(long long)(k * 32 + lane) * size + 1] : 0.f;
+            }
+            float top = warp_max(fmaxf(pm[0], pm[1]));
+            if (p.sink) top = fmaxf(top, 0.f);
+            const float f0 = exp2f(pm[0] - top), f1 = exp2f(pm[1] - top);
+            const float l = warp_sum(fmaf(pl[0], f0, pl[1] * f1)) + (p.sink ? exp2f(-top) : 0.f);
+            const float f = m ? -p.lambda[h0 + r] / l : 1.f / l;
+#pragma unroll 4
+            for (int i = 0; i < n; i++) {
+                const float w = f * __shfl_sync(0xffffffffu, i < 32 ? f0 : f1, i & 31);
+#pragma unroll
+                for (int c = 0; c < C; c++)
+                    if (c * 32 + lane < DV) o[c] = fmaf(head[(long long)i * size + 2 + c * 32 + lane], w, o[c]);
+            }
+        }
+        float f = 1.f;
+        if (p.gain) {
+            float ss = 0.f;
+#pragma unroll
+            for (int c = 0; c < C; c++) ss = fmaf(o[c], o[c], ss);  // dimensions that are padding are 0
+            f = 1.f / sqrtf(warp_sum(ss) / (float)p.vdim + p.head_eps);
+        }
+#pragma unroll
+        for (int c = 0; c < C; c++) {
+            const int i = c * 32 + lane;
+            if (i < p.vdim) out[r * p.vdim + i] = __float2bfloat16_rn(p.gain ? o[c] * f * p.gain[i] : o[c]);
+        }
+    }
+}
+
+// Grid: (splits, kv_heads · groups of 8 query heads, sequences). Both maps of eight heads of one key head share each tile of 16 keys and values, which a warp copies for itself.
+template <int DM, int DV> __global__ void __launch_bounds__(kDecThreads) differential_decode(const DiffP p) {
+    extern __shared__ __align__(16) unsigned char smem[];
+    __shared__ unsigned arrived;
+    __shared__ int page_s[kDecPages];  // this CTA's pages, checked
+    using L = DecSmem<DM, DV>;
+    pdl_trigger();
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g8 = lane >> 2, t4 = lane & 3;
+    // no launch of a step writes the batch description or the keys and values of earlier steps: they may be read while the
+    // launches before this one finish
+    const int seq = blockIdx.z;
+    const SeqRow sq = load_seq(p.seqs, seq);
+    const int rep = p.heads / p.kv_heads, groups = (rep + kDecHeads - 1) / kDecHeads, g = blockIdx.y / groups, h0 = g * rep + (blockIdx.y % groups) * kDecHeads;
+    const int n_heads = min(kDecHeads, (g + 1) * rep - h0), pos = sq.past, dim = p.dim, vdim = p.vdim;
+    const bf16* x = (const bf16*)p.proj + (long long)sq.start * p.ld;
+    bf16 *keys = (bf16*)p.keys, *values = (bf16*)p.values;
+    const unsigned sm0 = smem_u32(smem);
+    float *cs = reinterpret_cast<float*>(smem + L::angle), *sn = cs + DM / 2;
+
+    // keys of this CTA: whole tiles of all four warps, so that a split never cuts a tile
+    constexpr int step = kDecKeys * kDecWarps;
+    const int low = first_key(p, pos), base = low / step, blocks = sq.len == 1 ? pos / step + 1 - base : 0;
+    const int b0 = base + (int)((long long)blocks * blockIdx.x / p.splits), b1 = base + (int)((long long)blocks * (blockIdx.x + 1) / p.splits);
+    const int lo = b0 * step, hi = min(b1 * step, pos + 1), from = max(lo, low);  // pages in front of the window may be anybody's
+    const int page0 = from >> p.shift, n_pages = from < hi ? ((hi - 1) >> p.shift) - page0 + 1 : 0;
+    for (int i = tid; i < min(n_pages, kDecPages); i += kDecThreads) page_s[i] = (int)page_of(p, seq, (page0 + i) << p.shift);
+    if (sq.len == 1) angles(p.turns, p.half, pos, cs, sn, tid, kDecThreads);
+    __syncthreads();
+    auto page_at = [&](int j) {
+        const int i = (j >> p.shift) - page0;
+        return i < kDecPages ? (long long)page_s[i] : page_of(p, seq, j);
+    };
+    const unsigned ring = sm0 + L::kv + warp * L::stages * L::tile;
+    const int first = lo + warp * kDecKeys, tiles = first < hi ? (hi - first + step - 1) / step : 0;
+    auto load_tile = [&](int i) {
+        const int j0 = first + i * step;
+        if (i < tiles) {
+            const unsigned dst = ring + (i % L::stages) * L::tile;
+            const bool inside = j0 >= from && j0 + kDecKeys <= hi, whole = (1 << p.shift) >= kDecKeys;  // a tile lies in one page
+            const long long row0 = whole && j0 + kDecKeys > from ? key_row(p, page_at(max(j0, from)), g, j0) : 0;
+            constexpr int k_ch = DM / 8, v_ch = DV / 8;
+            if (whole && inside && dim == DM && vdim == DV) {  // contiguous runs: a lane's copies are evenly spaced
+                const bf16 *k = keys + row0 * 2 * DM + lane * 8, *v = values + row0 * DV + lane * 8;
+#pragma unroll
+                for (int c = 0; c < kDecKeys * 2 * k_ch / 32; c++) {
+                    const int at = c * 32 + lane;
+                    cp_async16(dst + at / (2 * k_ch) * L::k_stride + at % (2 * k_ch) * 16, k + c * 256);
+                }
+#pragma unroll
+                for (int c = 0; c < kDecKeys * v_ch / 32; c++) {
+                    const int at = c * 32 + lane;
+                    cp_async16(dst + kDecKeys * L::k_stride + at / v_ch * L::v_stride + at % v_ch * 16, v + c * 256);
+                }
+                cp_async_commit();
+                return;
+            }
+            for (int c = lane; c < kDecKeys * (2 * k_ch + v_ch); c += 32) {
+                const int key = c / (2 * k_ch + v_ch), ch = c % (2 * k_ch + v_ch), j = j0 + key;
+                const bool in = j >= from && j < hi;
+                const long long row = !in ? 0 : whole ? row0 + key : key_row(p, page_at(j), g, j);
+                if (ch < 2 * k_ch) {
+                    const int m = ch / k_ch, d = ch % k_ch * 8;
+                    const bool live = in && d < dim;
+                    cp_async16(dst + key * L::k_stride + ch * 16, live ? keys + (row * 2 + m) * dim + d : keys, live);
+                } else {
+                    const int d = (ch - 2 * k_ch) * 8;
+                    const bool live = in && d < vdim;
+                    cp_async16(dst + kDecKeys * L::k_stride + key * L::v_stride + d * 2, live ? values + row * vdim + d : values, live);
+                }
+            }
+        }
+        cp_async_commit();
+    };
+    const bool newest = hi == pos + 1 && lo < hi;  // this CTA's keys include the new one
+    auto fill = [&]() {
+#pragma unroll
+        for (int i = 0; i < L::stages - 1; i++) load_tile(i);
+    };
+    if (!newest) fill();
+    pdl_wait();
+    if (sq.len != 1) {
+        if (p.only && sq.len > 1 && tid == 0) report(p.err, ERR_BATCH_ROWS, p.node, seq, sq.len);
+        return;
+    }
+    if (newest) {
+        // (where a key head has several groups of queries, each CTA that needs the new key writes it: the same bits)
+        const long long row = key_row(p, page_at(pos), g, pos);
+        if (warp < 2) {
+            const bf16* k = x + p.k_off + (g * 2 + warp) * dim;
+            const float f = map_factor(p, k);
+            for (int i = lane; i < dim; i += 32) keys[(row * 2 + warp) * dim + i] = __float2bfloat16_rn(rotated(p.half, 0, k, cs, sn, i) * f);
+        } else if (warp == 2) {
+            for (int i = lane; i < vdim; i += 32) values[row * vdim + i] = x[p.v_off + g * vdim + i];
+        }
+        __syncthreads();
+        fill();
+    }
+    for (int r = warp; r < 2 * kDecHeads; r += kDecWarps) {
+        const int m = r / kDecHeads, h = r % kDecHeads;
+        const bool live = h < n_heads;
+        const bf16* q = x + p.q_off + (long long)((live ? h0 + h : h0) * 2 + m) * dim;
+        const float f = map_factor(p, q);
+        for (int i = lane; i < DM; i += 32) {
+            const float v = live && i < dim ? rotated(p.half, 0, q, cs, sn, i) * f : 0.f;
+            const bf16 high = __float2bfloat16_rn(v);
+            bf16* to = reinterpret_cast<bf16*>(smem + L::q + (2 * m * kDecHeads + h) * L::q_stride) + i;
+            to[0] = high;
+            to[kDecHeads * L::q_stride / 2] = low_part(v, high);
+        }
+    }
+    __syncthreads();
+
+    // Keys are the rows of both products (S^T = K q^T, O^T = V^T P^T): a lane holds scores of keys g, g + 8 and heads 2t, 2t + 1.
+    float o[2][DV / 16][4];
+    float top[2][2], l[2][2];
+#pragma unroll
+    for (int m = 0; m < 2; m++) {
+        top[m][0] = top[m][1] = kNoScore;
+        l[m][0] = l[m][1] = 0.f;
+#pragma unroll
+        for (int n = 0; n < DV / 16; n++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) o[m][n][e] = 0.f;
+    }
+    for (int i = 0; i < tiles; i++) {
+        cp_async_wait<L::stages - 2>();
+        __syncwarp();
+        load_tile(i + L::stages - 1);  // the slot was read in the previous iteration
+        const unsigned ks = ring + (i % L::stages) * L::tile, vs = ks + kDecKeys * L::k_stride;
+        const int j0 = first + i * step;
+        float s[2][4];
+#pragma unroll
+        for (int m = 0; m < 2; m++) {
+#pragma unroll
+            for (int e = 0; e < 4; e++) s[m][e] = 0.f;
+#pragma unroll
+            for (int kk = 0; kk < DM / 32; kk++) {
+                unsigned high[4], low4[4];
+                const unsigned at = sm0 + L::q + (2 * m * kDecHeads + (lane & 7)) * L::q_stride + kk * 64 + (lane >> 3) * 16;
+                ldmatrix_x4(high, at);
+                ldmatrix_x4(low4, at + kDecHeads * L::q_stride);
+#pragma unroll
+                for (int half = 0; half < 2; half++) {
+                    unsigned ka[4];
+                    ldmatrix_x4(ka, ks + (lane & 15) * L::k_stride + m * DM * 2 + kk * 64 + half * 32 + (lane >> 4) * 16);
+                    mma_bf16(s[m], ka[0], ka[1], ka[2], ka[3], high[2 * half], high[2 * half + 1]);
+                    mma_bf16(s[m], ka[0], ka[1], ka[2], ka[3], low4[2 * half], low4[2 * half + 1]);
+                }
+            }
+        }
+        const bool edge = j0 + kDecKeys > hi || j0 < low;
+        bool moved = false;
+        float now[2][2];
+#pragma unroll
+        for (int m = 0; m < 2; m++) {
+            now[m][0] = top[m][0];
+            now[m][1] = top[m][1];
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const int j = j0 + g8 + 8 * (e >> 1);
+                s[m][e] = edge && (j >= hi || j < low) ? -INFINITY : score2(p, s[m][e]);
+                now[m][e & 1] = fmaxf(now[m][e & 1], s[m][e]);
+            }
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+#pragma unroll
+                for (int d = 4; d < 32; d <<= 1) now[m][e] = fmaxf(now[m][e], __shfl_xor_sync(0xffffffffu, now[m][e], d));
+                moved |= now[m][e] != top[m][e];
+            }
+        }
+        if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+            for (int m = 0; m < 2; m++)
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    const float keep = exp2f(top[m][e] - now[m][e]);
+                    top[m][e] = now[m][e];
+                    l[m][e] *= keep;
+#pragma unroll
+                    for (int n = 0; n < DV / 16; n++) {
+                        o[m][n][e] *= keep;
+                        o[m][n][e + 2] *= keep;
+                    }
+                }
+        }
+        unsigned pb[2][2];
+#pragma unroll
+        for (int m = 0; m < 2; m++)
+#pragma unroll
+            for (int r = 0; r < 2; r++) {
+                const float w0 = exp2f(s[m][2 * r] - top[m][0]), w1 = exp2f(s[m][2 * r + 1] - top[m][1]);
+                l[m][0] += w0;
+                l[m][1] += w1;
+                pb[m][r] = transpose8x8(pack_bf16(w0, w1));
+            }
+#pragma unroll
+        for (int n = 0; n < DV / 16; n++) {
+            unsigned va[4];
+            ldmatrix_x4_trans(va, vs + ((lane >> 4) * 8 + (lane & 7)) * L::v_stride + n * 32 + ((lane >> 3) & 1) * 16);
+#pragma unroll
+            for (int m = 0; m < 2; m++) mma_bf16(o[m][n], va[0], va[1], va[2], va[3], pb[m][0], pb[m][1]);
+        }
+        __syncwarp();
+    }
+    cp_async_wait<0>();
+    __syncthreads();  // the ring becomes the merge area
+    float* parts = reinterpret_cast<float*>(smem + L::kv);
+#pragma unroll
+    for (int m = 0; m < 2; m++)
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1) l[m][e] += __shfl_xor_sync(0xffffffffu, l[m][e], d);
+            float* to = parts + warp * L::part + (m * kDecHeads + t4 * 2 + e) * (DV + 2);
+            if (g8 == 0) {
+                to[0] = top[m][e];
+                to[1] = l[m][e];
+            }
+#pragma unroll
+            for (int n = 0; n < DV / 16; n++) {
+                to[2 + n * 16 + g8] = o[m][n][e];
+                to[2 + n * 16 + g8 + 8] = o[m][n][e + 2];
+            }
+        }
+    __syncthreads();
+    bf16* out = (bf16*)p.out + ((long long)sq.start * p.heads + h0) * vdim;
+    if (p.splits == 1) {
+        merge_maps<DV>(p, parts, kDecWarps, h0, n_heads, out);
+        return;
+    }
+    const long long cell = (long long)blockIdx.z * gridDim.y + blockIdx.y;
+    merge_parts<DV, 2 * kDecHeads, kDecWarps>(parts, kDecWarps, 2 * kDecHeads, vdim, 0.f, nullptr, p.part + (cell * p.splits + blockIdx.x) * L::part);
+    __threadfence();
+    __syncthreads();
+    if (tid == 0) arrived = atomicAdd(&p.counters[cell], 1u);
+    __syncthreads();
+    if (arrived != (unsigned)p.splits - 1) return;
+    __threadfence();
+    if (tid == 0) p.counters[cell] = 0;
+    merge_maps<DV>(p, p.part + cell * p.splits * L::part, p.splits, h0, n_heads, out);
+}
+
 using DiffKernel = void (*)(const DiffP);
+struct DecChoice {
+    DiffKernel kernel;
+    int smem, part;
+};
+template <int DM, int DV> DecChoice choice() { return {differential_decode<DM, DV>, DecSmem<DM, DV>::total, DecSmem<DM, DV>::part}; }
+template <int DM> DecChoice choice(int64_t vdim) { return vdim <= 64 ? choice<DM, 64>() : vdim <= 128 ? choice<DM, 128>() : choice<DM, 256>(); }
 
 }  // namespace
 
@@ -119,19 +433,50 @@ void emit_differential(Emitter& em, const DifferentialDesc& d, const TRef& proj,
     p.head_eps = (float)d.head_eps;
     p.norm = d.norm;
     p.sink = d.sink;
-    p.singles = 1;
+    p.cap2 = (float)(d.softcap * (double)kLog2e);
+    p.mul2 = (float)(d.softcap > 0 ? 2.0 * (double)kLog2e * d.scale / d.softcap : (double)kLog2e * d.scale);
+    p.splits = 1;
     const bool bf = proj.dtype == DT_BF16;
-    const Buf none{kSlotNull, 0}, q = em.scratch((size_t)rows * d.heads * 2 * d.dim * (bf ? 2 : 4));
-    auto launch = [&](DiffKernel k, dim3 grid, unsigned block, unsigned smem, const char* label) {
+    // 16-byte copies of key and value rows
+    const bool tc = bf && d.dim % 8 == 0 && d.vdim % 8 == 0 && d.dim <= 128 && d.vdim <= 256 && keys.buf.off % 16 == 0 && values.buf.off % 16 == 0 && n_seqs <= 65535;
+    p.only = tc && rows <= n_seqs;                     // every sequence has one new token, or none
+    p.singles = !tc || (!p.only && n_seqs == 1);       // a lone token with rows of nobody behind it
+    const Buf none{kSlotNull, 0}, q = p.only ? none : em.scratch((size_t)rows * d.heads * 2 * d.dim * (bf ? 2 : 4));
+    auto launch = [&](DiffKernel k, dim3 grid, unsigned block, unsigned smem, Buf part, const char* label) {
         em.launch(k, grid, dim3(block), smem, p,
                   {{&p.proj, proj.buf}, {&p.turns, turns.buf}, {&p.keys, keys.buf}, {&p.values, values.buf}, {&p.q, q}, {&p.out, out.buf}, {&p.seqs, seqs.buf}, {&p.table, pages.buf},
-                   {&p.lambda, lambda.buf}, {&p.gain, gain ? gain->buf : none}, {&p.err, Buf{kSlotErr, 0}}},
+                   {&p.lambda, lambda.buf}, {&p.gain, gain ? gain->buf : none}, {&p.part, part}, {&p.counters, Buf{kSlotCounters, 0}}, {&p.err, Buf{kSlotErr, 0}}},
                   label, /*pdl=*/true);
     };
-    launch(bf ? differential_prepare<bf16> : differential_prepare<float>, dim3((unsigned)rows), 128, (unsigned)(d.rot_dims * 4), "differential_prepare");
-    const DiffKernel k = bf ? differential_simt<bf16> : differential_simt<float>;
-    ensure_max_dynamic_smem((const void*)k, 220 * 1024);
-    launch(k, dim3((unsigned)rows, (unsigned)d.heads), kAnyKeys, (unsigned)((d.dim + d.vdim + kAnyKeys) * 8), "differential_simt");
+    if (!p.only) {
+        launch(bf ? differential_prepare<bf16> : differential_prepare<float>, dim3((unsigned)rows), 128, (unsigned)(d.rot_dims * 4), none, "differential_prepare");
+        const DiffKernel k = bf ? differential_simt<bf16> : differential_simt<float>;
+        ensure_max_dynamic_smem((const void*)k, 220 * 1024);
+        launch(k, dim3((unsigned)rows, (unsigned)d.heads), kAnyKeys, (unsigned)((d.dim + d.vdim + kAnyKeys) * 8), none, "differential_simt");
+    }
+    if (tc && (p.only || n_seqs > 1)) {
+        const DecChoice dc = d.dim <= 32 ? choice<32>(d.vdim) : d.dim <= 64 ? choice<64>(d.vdim) : choice<128>(d.vdim);
+        const int64_t groups = d.kv_heads * ((d.heads / d.kv_heads + kDecHeads - 1) / kDecHeads), cells = n_seqs * groups;
+        // splits of the most keys a sequence can see: whole waves of resident CTAs, each with a fixed cost worth about
+        // 160 keys, and the pieces have to be merged
+        const int64_t resident = std::max<int64_t>(1, std::min<int64_t>(3, 224 * 1024 / (dc.smem + 2560))), slots = resident * sm_count();
+        int64_t seen = (int64_t)p.width * d.page;
+        if (d.window > 0) seen = std::min<int64_t>(seen, d.window + 64);
+        int64_t splits = 1;
+        double best = 1e300;
+        for (int64_t sp = 1; sp <= 64 && sp * 64 <= std::max<int64_t>(seen, 64); sp++) {
+            const double us = (double)((cells * sp + slots - 1) / slots) * ((double)seen / sp + 160.0) + 4.0 * sp;
+            if (us < best) {
+                best = us;
+                splits = sp;
+            }
+        }
+        if (cells > (int64_t)kCounterWords) splits = 1;
+        p.splits = (int)splits;
+        const Buf part = splits > 1 ? em.scratch((size_t)cells * splits * dc.part * 4) : none;
+        ensure_max_dynamic_smem((const void*)dc.kernel, dc.smem);
+        launch(dc.kernel, dim3((unsigned)splits, (unsigned)groups, (unsigned)n_seqs), kDecThreads, (unsigned)dc.smem, part, "differential_decode");
+    }
 }
 
 }  // namespace oxk

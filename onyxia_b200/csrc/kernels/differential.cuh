@@ -14,15 +14,27 @@ struct DiffP {
     const int* table;            // [R, width]
     const float* lambda;         // [heads]
     const float* gain;           // [vdim], or null: results as they are
+    float* part;                 // partial results of single tokens
+    unsigned* counters;
     ErrWord* err;
     long long rows, ld, q_off, k_off, v_off;
-    int n_seqs, width, n_pages, shift /* log2 of the page */, heads, kv_heads, dim, vdim, half, window, node;
+    int n_seqs, width, n_pages, shift /* log2 of the page */, heads, kv_heads, dim, vdim, half, window, splits, node;
     float scale, cap, eps, head_eps;
+    float mul2, cap2;            // base 2: cap2 = 0: score2 = mul2 · q·k, otherwise cap2 · tanh with mul2 = 2 log2 e · scale / cap
     int norm, sink;
-    int singles;                 // prepare: also sequences with one new token
+    int singles;                 // sequences with one new token are for these kernels too
+    int only;                    // no sequence may have more than one
 };
 
 __device__ __forceinline__ int first_key(const DiffP& p, int pos) { return p.window > 0 ? max(0, pos - p.window + 1) : 0; }
+// log2 e · score of a dot product; tanh x = 1 − 2 / (1 + e^2x) is off by a few 1e-7 of the cap
+__device__ __forceinline__ float score2(const DiffP& p, float d) {
+    const float x = d * p.mul2;
+    return p.cap2 > 0.f ? p.cap2 - __fdividef(2.f * p.cap2, 1.f + exp2f(x)) : x;
+}
+// A query as the sum of two bf16. Rounded to one, it alone puts results 2.7e-3 from those of an f32 query (one token, 520 keys, scores of spread 1.5), more than the rounding
+// of the weights (1.1e-3) and of the results (1.7e-3) together.
+__device__ __forceinline__ bf16 low_part(float v, bf16 high) { return __float2bfloat16_rn(v - __bfloat162float(high)); }
 // 1 / root mean square of a map's query or key, by one warp
 template <typename T> __device__ __forceinline__ float map_factor(const DiffP& p, const T* x) {
     if (!p.norm) return 1.f;

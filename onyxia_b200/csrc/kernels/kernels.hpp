@@ -33,6 +33,7 @@ enum : int {
     ERR_RULES_TOKEN = 8,
     ERR_RULES_LENGTH = 9,
     ERR_RULES_MASK = 10,
+    ERR_BATCH_ROWS = 11,
 };
 
 struct ErrWord {

@@ -110,7 +110,7 @@ def test_long_ranges(kind):
 def test_rows_and_sequences_of_a_padded_batch(kind):
     """Rows behind the last sequence are left alone, and sequences without new tokens (behind all others) do nothing, to the pools neither."""
     f = Form(4, 2, 64, 128, 64)
-    for lengths, tail in (([(5, 3), (1, 70), (0, 10)], 9), ([(1, 3), (1, 70), (0, 10), (0, 0)], 1), ([(80, 0)], 70), ([(0, 5)], 3)):
+    for lengths, tail in (([(5, 3), (1, 70), (0, 10)], 9), ([(1, 3), (1, 70), (0, 10), (0, 0)], 1), ([(80, 0)], 70), ([(0, 5)], 3), ([(1, 70)], 4)):
         s, got = check(f, lengths, kind, tail=tail) if any(n for n, _ in lengths) else (None, None)
         s = s or util.step(f, lengths, tail=tail, round_to=stored(kind))
         session = cuda_backend().prepare(util.module(f, DTYPES[kind], s.lam, s.gain))
@@ -169,6 +169,14 @@ def test_a_page_that_is_none_is_reported(lengths, bad, kind):
     s.table[0, 1] = s.table[0, 0]
     dev["page_table"] = session.upload(HostTensor.from_numpy(s.table))
     session.download(session.run(dev)[0][1])
+
+
+def test_a_prompt_in_a_batch_of_no_more_rows_than_sequences_is_reported():
+    f = Form(4, 2, 64, 128, 64)
+    s = util.step(f, [(1, 3), (3, 5), (0, 0), (0, 0)])
+    session, _, outs = run(f, s, "bf16")
+    with pytest.raises(OnyxiaError, match="sequence 1 has 3 new tokens"):
+        session.download(outs["out"])
 
 
 def test_views_and_uploads_of_device_memory():

@@ -8,6 +8,7 @@
 // Queries and keys rotate and are normed as in paged_kv_attention.cu, each map by itself. A pool's key is the two maps' side by side.
 //
 //   differential_prepare   rotated, normed queries; the new keys and values go to the pools
+//   differential_prefill   sequences with several new tokens in bf16 (differential_prefill.cu)
 //   differential_decode    sequences with one new token: their keys split over CTAs and warps, all of the above in one launch
 //   differential_simt      any shape, f32 and bf16
 //
@@ -35,6 +36,17 @@ template <typename T> __global__ void __launch_bounds__(128) differential_prepar
         const T* src = k < 0 ? x + p.q_off + (long long)h * p.dim : x + p.k_off + (long long)k * p.dim;
         T* dst = k < 0 ? (T*)p.q + ((long long)row * p.heads * 2 + h) * p.dim : (T*)p.keys + (key_row(p, pg, k >> 1, pos) * 2 + (k & 1)) * p.dim;
         const float f = map_factor(p, src);
+        if constexpr (sizeof(T) == 2)
+            if (k < 0 && p.parts) {
+                bf16* to = (bf16*)p.q + ((long long)row * p.heads * 2 + h) * 2 * p.dim;
+                for (int i = lane; i < p.dim; i += 32) {
+                    const float v = rotated(p.half, 0, src, angle, angle + p.half, i) * f * p.mul2;
+                    const bf16 high = __float2bfloat16_rn(v);
+                    to[i] = high;
+                    to[p.dim + i] = low_part(v, high);
+                }
+                continue;
+            }
         for (int i = lane; i < p.dim; i += 32) dst[i] = from_f<T>(rotated(p.half, 0, src, angle, angle + p.half, i) * f);
     }
     for (int i = threadIdx.x; i < p.kv_heads * p.vdim; i += 128) ((T*)p.values)[key_row(p, pg, i / p.vdim, pos) * p.vdim + i % p.vdim] = x[p.v_off + i];
@@ -410,6 +422,7 @@ void emit_differential(Emitter& em, const DifferentialDesc& d, const TRef& proj,
                        const TRef& pages, const TRef& lambda, const TRef* gain, const TRef& out) {
     const int64_t rows = proj.shape[0], n_seqs = seqs.shape[0];
     if (rows == 0 || n_seqs == 0) return;
+    if (keys.shape[0] == 0) throw std::runtime_error("differential attention: new tokens, and pools without a page");
     DiffP p{};
     p.rows = rows;
     p.ld = proj.shape[1];
@@ -441,7 +454,9 @@ void emit_differential(Emitter& em, const DifferentialDesc& d, const TRef& proj,
     const bool tc = bf && d.dim % 8 == 0 && d.vdim % 8 == 0 && d.dim <= 128 && d.vdim <= 256 && keys.buf.off % 16 == 0 && values.buf.off % 16 == 0 && n_seqs <= 65535;
     p.only = tc && rows <= n_seqs;                     // every sequence has one new token, or none
     p.singles = !tc || (!p.only && n_seqs == 1);       // a lone token with rows of nobody behind it
-    const Buf none{kSlotNull, 0}, q = p.only ? none : em.scratch((size_t)rows * d.heads * 2 * d.dim * (bf ? 2 : 4));
+    const bool prefill = tc && !p.only && differential_prefill_fits(p, keys, values, out.buf.off);
+    p.parts = prefill;
+    const Buf none{kSlotNull, 0}, q = p.only ? none : em.scratch((size_t)rows * d.heads * 2 * d.dim * (bf && !prefill ? 2 : 4));
     auto launch = [&](DiffKernel k, dim3 grid, unsigned block, unsigned smem, Buf part, const char* label) {
         em.launch(k, grid, dim3(block), smem, p,
                   {{&p.proj, proj.buf}, {&p.turns, turns.buf}, {&p.keys, keys.buf}, {&p.values, values.buf}, {&p.q, q}, {&p.out, out.buf}, {&p.seqs, seqs.buf}, {&p.table, pages.buf},
@@ -450,9 +465,15 @@ void emit_differential(Emitter& em, const DifferentialDesc& d, const TRef& proj,
     };
     if (!p.only) {
         launch(bf ? differential_prepare<bf16> : differential_prepare<float>, dim3((unsigned)rows), 128, (unsigned)(d.rot_dims * 4), none, "differential_prepare");
-        const DiffKernel k = bf ? differential_simt<bf16> : differential_simt<float>;
-        ensure_max_dynamic_smem((const void*)k, 220 * 1024);
-        launch(k, dim3((unsigned)rows, (unsigned)d.heads), kAnyKeys, (unsigned)((d.dim + d.vdim + kAnyKeys) * 8), none, "differential_simt");
+        if (prefill) {
+            emit_differential_prefill(em, p, keys, values,
+                                      {{offsetof(DiffP, q), q}, {offsetof(DiffP, out), out.buf}, {offsetof(DiffP, seqs), seqs.buf}, {offsetof(DiffP, table), pages.buf},
+                                       {offsetof(DiffP, lambda), lambda.buf}, {offsetof(DiffP, gain), gain ? gain->buf : none}, {offsetof(DiffP, err), Buf{kSlotErr, 0}}});
+        } else {
+            const DiffKernel k = bf ? differential_simt<bf16> : differential_simt<float>;
+            ensure_max_dynamic_smem((const void*)k, 220 * 1024);
+            launch(k, dim3((unsigned)rows, (unsigned)d.heads), kAnyKeys, (unsigned)((d.dim + d.vdim + kAnyKeys) * 8), none, "differential_simt");
+        }
     }
     if (tc && (p.only || n_seqs > 1)) {
         const DecChoice dc = d.dim <= 32 ? choice<32>(d.vdim) : d.dim <= 64 ? choice<64>(d.vdim) : choice<128>(d.vdim);

@@ -8,7 +8,7 @@ struct DiffP {
     const void* proj;            // [rows, ld]
     const float* turns;          // [2, half]
     void *keys, *values;         // [pages, kv_heads, page, 2 · dim | vdim]
-    void* q;                     // [rows, heads · 2 · dim]: prepared queries
+    void* q;                     // prepared queries: [rows, heads, map, dim] of the pools' type, or, as the prefill kernel reads them, [rows, heads, map, high and low part, dim]
     void* out;                   // [rows, heads · vdim]
     const int* seqs;             // [R, 4]
     const int* table;            // [R, width]
@@ -23,6 +23,7 @@ struct DiffP {
     float mul2, cap2;            // base 2: cap2 = 0: score2 = mul2 · q·k, otherwise cap2 · tanh with mul2 = 2 log2 e · scale / cap
     int norm, sink;
     int singles;                 // sequences with one new token are for these kernels too
+    int parts;                   // prepare: queries in two parts, times mul2
     int only;                    // no sequence may have more than one
 };
 
@@ -45,5 +46,9 @@ template <typename T> __device__ __forceinline__ float map_factor(const DiffP& p
     }
     return 1.f / sqrtf(warp_sum(ss) / (float)p.dim + p.eps);
 }
+
+// Prompts on tcgen05 (differential_prefill.cu); queries come from `q` [rows, heads, map, high and low part, dim] in units of base 2; `ptrs`: fields of DiffP by their offset.
+bool differential_prefill_fits(const DiffP&, const TRef& keys, const TRef& values, int64_t out_off);
+void emit_differential_prefill(Emitter&, const DiffP&, const TRef& keys, const TRef& values, std::initializer_list<std::pair<size_t, Buf>> ptrs);
 
 }  // namespace oxk

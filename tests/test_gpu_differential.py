@@ -179,6 +179,22 @@ def test_a_prompt_in_a_batch_of_no_more_rows_than_sequences_is_reported():
         session.download(outs["out"])
 
 
+def test_nothing_to_do_and_nowhere_to_put_it():
+    f = Form(4, 2, 64, 128, 64)
+    s = util.step(f, [(2, 3)])
+    session = cuda_backend().prepare(util.module(f, ir.BF16, s.lam, s.gain))
+    dev = {k: session.upload(v) for k, v in util.feed(s, act("bf16")).items()}
+    none = dict(dev, proj=session.upload(HostTensor.bf16(s.proj[:0])))
+    assert session.run(none)[0][1].shape == (0, f.heads * f.vdim)
+    none = dict(dev, seq_info=session.upload(HostTensor.from_numpy(s.seqs[:0])), page_table=session.upload(HostTensor.from_numpy(s.table[:0])))
+    assert session.run(none)[0][1].shape == (2, f.heads * f.vdim)
+    none = {**dev, "pages.keys": session.upload(HostTensor.bf16(s.keys[:0])), "pages.values": session.upload(HostTensor.bf16(s.values[:0]))}
+    with pytest.raises(OnyxiaError, match="without a page"):
+        session.run(none)
+    want = util.reference(f, s)[0]
+    compare(session.download(session.run(dev)[0][1]).numpy(), want, "bf16", s)
+
+
 def test_views_and_uploads_of_device_memory():
     torch = pytest.importorskip("torch")
     f = Form(4, 2, 64, 128, 64)

@@ -27,7 +27,7 @@ template <typename T> __global__ void __launch_bounds__(128) differential_prepar
     const SeqRow sq = load_seq(p.seqs, s);
     const int pos = sq.past + row - sq.start;
     if (row < sq.start || row >= sq.start + sq.len || (sq.len == 1 && !p.singles)) return;
-    angles(p.turns, p.half, pos, angle, angle + p.half, threadIdx.x, 128);
+    quarter_angles(p, pos, angle, angle + p.half, threadIdx.x, 128);
     __syncthreads();
     const T* x = (const T*)p.proj + (long long)row * p.ld;
     const long long pg = page_of(p, s, pos);
@@ -50,6 +50,70 @@ template <typename T> __global__ void __launch_bounds__(128) differential_prepar
         for (int i = lane; i < p.dim; i += 32) dst[i] = from_f<T>(rotated(p.half, 0, src, angle, angle + p.half, i) * f);
     }
     for (int i = threadIdx.x; i < p.kv_heads * p.vdim; i += 128) ((T*)p.values)[key_row(p, pg, i / p.vdim, pos) * p.vdim + i % p.vdim] = x[p.v_off + i];
+}
+
+// The same in bf16 eight elements at a time, where heads, rotated halves and rows allow it: a unit is eight pairs that turn or eight elements that do not.
+__global__ void __launch_bounds__(128) differential_prepare8(const DiffP p) {
+    extern __shared__ float angle[];  // cos[half], sin[half], with norms [2 · (heads + kv_heads)] factors
+    pdl_enter();
+    const int row = blockIdx.x, s = find_seq(p.seqs, p.n_seqs, row), tid = threadIdx.x;
+    const SeqRow sq = load_seq(p.seqs, s);
+    const int pos = sq.past + row - sq.start, maps = 2 * (p.heads + p.kv_heads);
+    if (row < sq.start || row >= sq.start + sq.len || (sq.len == 1 && !p.singles)) return;
+    quarter_angles(p, pos, angle, angle + p.half, tid, 128);
+    const bf16* x = (const bf16*)p.proj + (long long)row * p.ld;
+    auto source = [&](int h) { return h < 2 * p.heads ? x + p.q_off + (long long)h * p.dim : x + p.k_off + (long long)(h - 2 * p.heads) * p.dim; };
+    float* factor = angle + 2 * p.half;
+    if (p.norm)
+        for (int h = tid >> 5; h < maps; h += 4) {
+            const float f = map_factor(p, source(h));
+            if ((tid & 31) == 0) factor[h] = f;
+        }
+    __syncthreads();
+    const long long pg = page_of(p, s, pos);
+    const int turned = p.half / 8, units = p.dim / 8 - turned;
+    auto put = [&](int h, int at, const float (&v)[8]) {
+        unsigned w[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) w[e] = pack_bf16(v[2 * e], v[2 * e + 1]);
+        const int k = h - 2 * p.heads;
+        bf16* to = k >= 0 ? (bf16*)p.keys + (key_row(p, pg, k >> 1, pos) * 2 + (k & 1)) * p.dim : (bf16*)p.q + ((long long)row * p.heads * 2 + h) * (1 + p.parts) * p.dim;
+        *reinterpret_cast<uint4*>(to + at) = make_uint4(w[0], w[1], w[2], w[3]);
+        if (k >= 0 || !p.parts) return;
+#pragma unroll
+        for (int e = 0; e < 4; e++) w[e] = pack_bf16(v[2 * e] - __uint_as_float(w[e] << 16), v[2 * e + 1] - __uint_as_float(w[e] & 0xFFFF0000u));
+        *reinterpret_cast<uint4*>(to + p.dim + at) = make_uint4(w[0], w[1], w[2], w[3]);
+    };
+    auto wide = [](uint4 u, float (&v)[8]) {
+        const unsigned w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int e = 0; e < 4; e++) v[2 * e] = __uint_as_float(w[e] << 16), v[2 * e + 1] = __uint_as_float(w[e] & 0xFFFF0000u);
+    };
+    for (int u = tid; u < maps * units; u += 128) {
+        const int h = u / units, i = u % units;
+        const bool turns = i < turned;
+        const int at = turns ? i * 8 : (i + turned) * 8;
+        const bf16* src = source(h) + at;
+        const float f = (p.norm ? factor[h] : 1.f) * (h < 2 * p.heads && p.parts ? p.mul2 : 1.f);
+        float a[8], b[8], o[8];
+        wide(*reinterpret_cast<const uint4*>(src), a);
+        if (!turns) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) o[e] = a[e] * f;
+            put(h, at, o);
+            continue;
+        }
+        wide(*reinterpret_cast<const uint4*>(src + p.half), b);
+        const float *c = angle + at, *n = c + p.half;
+#pragma unroll
+        for (int e = 0; e < 8; e++) o[e] = (a[e] * c[e] - b[e] * n[e]) * f;
+        put(h, at, o);
+#pragma unroll
+        for (int e = 0; e < 8; e++) o[e] = (b[e] * c[e] + a[e] * n[e]) * f;
+        put(h, at + p.half, o);
+    }
+    for (int u = tid; u < p.kv_heads * p.vdim / 8; u += 128)
+        *reinterpret_cast<uint4*>((bf16*)p.values + key_row(p, pg, u * 8 / p.vdim, pos) * p.vdim + u * 8 % p.vdim) = *reinterpret_cast<const uint4*>(x + p.v_off + u * 8);
 }
 
 // One CTA per (row, head); chunks of 128 keys, a thread per key, then a thread per value dimension.
@@ -192,7 +256,7 @@ template <int DM, int DV> __global__ void __launch_bounds__(kDecThreads) differe
     const int lo = b0 * step, hi = min(b1 * step, pos + 1), from = max(lo, low);  // pages in front of the window may be anybody's
     const int page0 = from >> p.shift, n_pages = from < hi ? ((hi - 1) >> p.shift) - page0 + 1 : 0;
     for (int i = tid; i < min(n_pages, kDecPages); i += kDecThreads) page_s[i] = (int)page_of(p, seq, (page0 + i) << p.shift);
-    if (sq.len == 1) angles(p.turns, p.half, pos, cs, sn, tid, kDecThreads);
+    if (sq.len == 1) quarter_angles(p, pos, cs, sn, tid, kDecThreads);
     __syncthreads();
     auto page_at = [&](int j) {
         const int i = (j >> p.shift) - page0;
@@ -356,10 +420,11 @@ template <int DM, int DV> __global__ void __launch_bounds__(kDecThreads) differe
         for (int m = 0; m < 2; m++)
 #pragma unroll
             for (int r = 0; r < 2; r++) {
-                const float w0 = exp2f(s[m][2 * r] - top[m][0]), w1 = exp2f(s[m][2 * r + 1] - top[m][1]);
-                l[m][0] += w0;
-                l[m][1] += w1;
-                pb[m][r] = transpose8x8(pack_bf16(w0, w1));
+                const unsigned w = pack_bf16(exp2f(s[m][2 * r] - top[m][0]), exp2f(s[m][2 * r + 1] - top[m][1]));
+                // the sums of the weights as they are multiplied: the rounding of a weight that stands out is in both
+                l[m][0] += __uint_as_float(w << 16);
+                l[m][1] += __uint_as_float(w & 0xFFFF0000u);
+                pb[m][r] = transpose8x8(w);
             }
 #pragma unroll
         for (int n = 0; n < DV / 16; n++) {
@@ -464,7 +529,9 @@ void emit_differential(Emitter& em, const DifferentialDesc& d, const TRef& proj,
                   label, /*pdl=*/true);
     };
     if (!p.only) {
-        launch(bf ? differential_prepare<bf16> : differential_prepare<float>, dim3((unsigned)rows), 128, (unsigned)(d.rot_dims * 4), none, "differential_prepare");
+        const bool by8 = tc && d.rot_dims % 16 == 0 && p.ld % 8 == 0 && d.q_off % 8 == 0 && d.k_off % 8 == 0 && d.v_off % 8 == 0 && proj.buf.off % 16 == 0 && d.heads <= 4096;
+        if (by8) launch(differential_prepare8, dim3((unsigned)rows), 128, (unsigned)((d.rot_dims + (d.norm ? 2 * (d.heads + d.kv_heads) : 0)) * 4), none, "differential_prepare");
+        else launch(bf ? differential_prepare<bf16> : differential_prepare<float>, dim3((unsigned)rows), 128, (unsigned)(d.rot_dims * 4), none, "differential_prepare");
         if (prefill) {
             emit_differential_prefill(em, p, keys, values,
                                       {{offsetof(DiffP, q), q}, {offsetof(DiffP, out), out.buf}, {offsetof(DiffP, seqs), seqs.buf}, {offsetof(DiffP, table), pages.buf},

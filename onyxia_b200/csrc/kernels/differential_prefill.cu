@@ -1,8 +1,8 @@
 // Prompts of differential attention in bf16 on tcgen05.
 //
-// A cluster of two CTAs owns 128 (token, head) rows of one key head, each CTA one of the two softmax maps: it walks over that map's keys 128 at a time. Queries come as the
-// sum of two bf16, base-2 units included, so scores need no factor: 8 · dim / 64 products of 128 × 128 make them, a thread per row caps, masks and weighs them, and for each
-// 64 keys 4 products of 128 × vdim add the weights' share of the values. Keys and values come by TMA, two tiles of keys and two halves of values on their way.
+// A cluster of two CTAs owns 128 (token, head) rows of one key head, each CTA one of the two softmax maps: it walks over that map's keys KEYS (64 or 128) at a time. Queries come as
+// the sum of two bf16, base-2 units included, so scores need no factor: dim / 8 products of 128 × KEYS × 16 make them, a thread per row caps, masks and weighs them, and for each
+// 64 keys 4 products of 128 × vdim × 16 add the weights' share of the values; the scores of the next keys are made under the weights of these. Keys and values come by TMA.
 // In the end each CTA sends the other half of its rows, divided by their sums, through the cluster's shared memory, and forms difference, norm and results of its own half.
 #include "differential.cuh"
 
@@ -10,9 +10,9 @@ namespace oxk {
 
 namespace {
 
-constexpr int kRows = 128, kKeys = 128, kPart = 64, kSoft = 128, kThreads = kSoft + 64;  // warps 0-3 softmax, 4 copies, 5 issues products
-constexpr unsigned kPanelQ = kRows * 128, kPanelK = kKeys * 128, kPanelV = kPart * 128;  // bytes: rows × 64 dimensions
-constexpr int kBarriers = 16;
+constexpr int kRows = 128, kPart = 64, kSoft = 128, kThreads = kSoft + 64;  // warps 0-3 softmax, 4 copies, 5 issues products
+constexpr unsigned kPanelQ = kRows * 128, kPanelV = kPart * 128;  // bytes: rows × 64 dimensions
+constexpr int kBarriers = 18;
 constexpr float kLazy = 8.f;  // how far (base 2) a row's scores may rise above the maximum that its weights are taken against
 
 struct PreP {
@@ -71,19 +71,36 @@ __device__ __forceinline__ void cluster_meet() {
     asm volatile("barrier.cluster.arrive.release;\n barrier.cluster.wait.acquire;" ::: "memory");
 }
 
-// TURNS: places for scores in tensor memory. One: 256 of its columns, two CTAs per SM, which work under each other's waits. Two: all columns, the next scores are made under the
-// weights of these.
-template <bool CAPPED, int TURNS> __global__ void __launch_bounds__(kThreads, 3 - TURNS) differential_prefill(const __grid_constant__ PreP pp) {
+// The pages of the copies to come, 32 at a time and the next 32 on their way: the table's answer to a single question takes as long as a copy.
+struct PagesAhead {
+    int first, now, next;
+    template <class Page> __device__ __forceinline__ PagesAhead(int from, Page&& page) : first(from), now(page(from)), next(page(from + 32)) {}
+    // of box i, which does not fall; all lanes ask the same
+    template <class Page> __device__ __forceinline__ int of(int i, Page&& page) {
+        if (i >= first + 32) {
+            first += 32;
+            now = next;
+            next = page(first + 32);
+        }
+        return __shfl_sync(0xffffffffu, now, i - first);
+    }
+};
+
+// KEYS 64: 256 columns of tensor memory (values of up to 128), two CTAs per SM, which work under each other's waits. 128: all columns.
+template <bool CAPPED, int KEYS> __global__ void __launch_bounds__(kThreads, KEYS == 64 ? 2 : 1) differential_prefill(const __grid_constant__ PreP pp) {
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     // (both CTAs of a cluster find the same place: their shared memory begins at the same address)
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     const DiffP& p = pp.kv;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, kp = pp.kp, vp = pp.vp, map = blockIdx.y & 1, g = blockIdx.y >> 1;
+    constexpr int kHalves = KEYS / kPart, kStagesV = 2 * kHalves > 3 ? 2 : 3;
+    constexpr unsigned kPanelK = KEYS * 128;
     const unsigned k_stage = kp * kPanelK, v_stage = vp * kPanelV;
-    const unsigned sq0 = smem_u32(smem), low0 = kp * kPanelQ, sk = sq0 + 2 * low0, sv = sk + 2 * k_stage, bars = sv + 2 * v_stage;
-    // barriers: keys there, free, values there, free, scores there, products added (two each), weights there (two halves of two)
-    const unsigned k_full = bars, k_free = bars + 16, v_full = bars + 32, v_free = bars + 48, s_full = bars + 64, o_done = bars + 80, w_full = bars + 96;
+    const unsigned sq0 = smem_u32(smem), low0 = kp * kPanelQ, sk = sq0 + 2 * low0, sv = sk + 2 * k_stage, bars = sv + kStagesV * v_stage;
+    // barriers: keys there, free (two each), values there, free (three), scores there, products added (two), weights there (two halves of two)
+    const unsigned k_full = bars, k_free = bars + 16, v_full = bars + 32, v_free = bars + 56, s_full = bars + 80, o_done = bars + 96, w_full = bars + 112;
     unsigned* tmem_slot = reinterpret_cast<unsigned*>(smem + (bars + kBarriers * 8 - sq0));
+    float* scales = reinterpret_cast<float*>(smem + (bars + kBarriers * 8 + 16 - sq0));  // [64]: what the norms divide by
     if (tid == 0) {
         for (int i = 0; i < kBarriers; i++) mbar_init(bars + i * 8, i >= kBarriers - 4 ? kSoft / 32 : 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -95,9 +112,9 @@ template <bool CAPPED, int TURNS> __global__ void __launch_bounds__(kThreads, 3 
     if (!locate_tile(p.seqs, p.n_seqs, (int)gridDim.x - 1 - (int)blockIdx.x, tq, &seq, &first, p.singles ? 1 : 2)) return;  // both CTAs of the cluster
     const SeqRow sq = load_seq(p.seqs, seq);
     const int n_tok = min(tq, sq.len - first), pos0 = sq.past + first, last = pos0 + n_tok - 1, low = first_key(p, pos0);
-    // Scores in TURNS turns of 128 columns, sums behind them; weights take the place of the scores that their thread has read. No more CTAs than have room in tensor memory may be on
+    // Scores in two turns of KEYS columns, sums behind them; weights take the place of the scores that their thread has read. No more CTAs than have room in tensor memory may be on
     // an SM at a time (differential_smem), or two clusters could wait for what the other one has.
-    constexpr unsigned cols = TURNS * 256;
+    constexpr unsigned cols = KEYS * 4;
     if (warp == 5) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(cols) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -116,8 +133,8 @@ template <bool CAPPED, int TURNS> __global__ void __launch_bounds__(kThreads, 3 
     __syncthreads();
     after_sync();
     pdl_trigger();  // the tensor memory is taken: nothing that starts now can keep it from this CTA
-    const unsigned tmem = *tmem_slot, t_sum = tmem + TURNS * kKeys;
-    const int kt0 = low / kKeys, n = last / kKeys + 1 - kt0;
+    const unsigned tmem = *tmem_slot, t_sum = tmem + 2 * KEYS;
+    const int kt0 = low / KEYS, n = last / KEYS + 1 - kt0;
     bool ok = true;
     // Waits until the products of tile i are in the sums. Tiles take turns at two barriers. Who has the scores of tile i knows the products of tile i - 2 and of all before it to be
     // done, so the barrier of tile i - 1 or i cannot be a round behind.
@@ -126,47 +143,54 @@ template <bool CAPPED, int TURNS> __global__ void __launch_bounds__(kThreads, 3 
     auto seen = [&](int j0, int h) { return j0 + h * kPart <= last && j0 + h * kPart + kPart > low; };
 
     if (warp == 4) {
+        // Copies of a page's keys each, where a page holds fewer than a half; those that nobody sees are left out. A tile's keys are asked for before the values of the tile before it.
+        const int box0 = max(low, kt0 * KEYS) / pp.box, box1 = last / pp.box;
+        auto page = [&](int i) { return i + lane <= box1 ? (int)page_of(p, seq, (i + lane) * pp.box) : 0; };
+        PagesAhead keys_pages(box0, page), values_pages(box0, page);
         RingAt keys_at, values_at;
         int halves = 0;
-        // copies of a page's keys each, where a page holds fewer than are wanted; those that nobody sees are left out
-        auto copy = [&](int kv, int j0, int keys, unsigned full, unsigned to, int panels, unsigned panel, int x) {
-            const int c0 = max(low - j0, 0) / pp.box, c1 = min((last - j0) / pp.box, keys / pp.box - 1);
-            if (elect_one() && ok) mbar_expect_tx(full, (unsigned)((c1 - c0 + 1) * pp.box * 128 * panels));
+        auto copy = [&](int kv, PagesAhead& pages, int j0, int keys, unsigned full, unsigned to, int panels, unsigned panel, int x) {
+            const int b0 = max(j0 / pp.box, box0), b1 = min((j0 + keys) / pp.box - 1, box1);
+            if (elect_one() && ok) mbar_expect_tx(full, (unsigned)((b1 - b0 + 1) * pp.box * 128 * panels));
             __syncwarp();
-            for (int b = c0; b <= c1; b++) {
-                const int j = j0 + b * pp.box, row = (int)key_row(p, page_of(p, seq, j), g, j);
+            for (int b = b0; b <= b1; b++) {
+                const int j = b * pp.box, row = (int)key_row(p, pages.of(b, page), g, j);
                 if (elect_one() && ok)
-                    for (int c = 0; c < panels; c++) tma_load_2d(to + c * panel + b * pp.box * 128, pp.maps[kv], x + c * 64, row, full);
+                    for (int c = 0; c < panels; c++) tma_load_2d(to + c * panel + (j - j0) * 128, pp.maps[kv], x + c * 64, row, full);
                 __syncwarp();
             }
         };
-        for (int i = 0; i < n && ok; i++) {
-            const int j0 = (kt0 + i) * kKeys;
-            if (i >= 2 && !mbar_wait(k_free + keys_at.s * 8, keys_at.parity ^ 1)) ok = false;
-            copy(0, j0, kKeys, k_full + keys_at.s * 8, sk + keys_at.s * k_stage, kp, kPanelK, map * p.dim);
+        auto copy_keys = [&](int i) {
+            if (i >= 2 && ok && !mbar_wait(k_free + keys_at.s * 8, keys_at.parity ^ 1)) ok = false;
+            copy(0, keys_pages, (kt0 + i) * KEYS, KEYS, k_full + keys_at.s * 8, sk + keys_at.s * k_stage, kp, kPanelK, map * p.dim);
             keys_at.next(2);
-            for (int h = 0; h < 2; h++) {
+        };
+        copy_keys(0);
+        for (int i = 0; i < n && ok; i++) {
+            if (i + 1 < n) copy_keys(i + 1);
+            const int j0 = (kt0 + i) * KEYS;
+            for (int h = 0; h < kHalves; h++) {
                 if (!seen(j0, h)) continue;
-                if (halves >= 2 && ok && !mbar_wait(v_free + values_at.s * 8, values_at.parity ^ 1)) ok = false;
-                copy(1, j0 + h * kPart, kPart, v_full + values_at.s * 8, sv + values_at.s * v_stage, vp, kPanelV, 0);
-                values_at.next(2);
+                if (halves >= kStagesV && ok && !mbar_wait(v_free + values_at.s * 8, values_at.parity ^ 1)) ok = false;
+                copy(1, values_pages, j0 + h * kPart, kPart, v_full + values_at.s * 8, sv + values_at.s * v_stage, vp, kPanelV, 0);
+                values_at.next(kStagesV);
                 halves++;
             }
             ok = __all_sync(0xffffffffu, ok);
         }
     } else if (warp == 5) {
         const unsigned base = (1u << 4) | (1u << 7) | (1u << 10) | (8u << 24);  // bf16 × bf16 → f32, M 128
-        const unsigned by_keys = base | ((kKeys >> 3) << 17), by_values = base | (1u << 16) | ((unsigned)(vp * 8) << 17);  // the values' wide axis is the result's
+        const unsigned by_keys = base | ((KEYS >> 3) << 17), by_values = base | (1u << 16) | ((unsigned)(vp * 8) << 17);  // the values' wide axis is the result's
         const unsigned long long dq = umma_kmajor_desc(sq0), dk = umma_kmajor_desc(sk), dv = umma_wide_desc(sv);
         RingAt keys_at, values_at;
         auto scores = [&](int i) {
             if (ok && !mbar_wait(k_full + keys_at.s * 8, keys_at.parity)) ok = false;
             // the products that read the weights in these scores' place have to be done
-            if (i >= TURNS && ok && !added(i - TURNS)) ok = false;
+            if (i >= 2 && ok && !added(i - 2)) ok = false;
             after_sync();
             if (elect_one() && ok) {
                 const unsigned long long k = dk + keys_at.s * (k_stage >> 4);
-                const unsigned to = tmem + (i % TURNS) * kKeys;
+                const unsigned to = tmem + (i & 1) * KEYS;
                 for (int e = 0; e < p.dim / 16; e++) {
                     const unsigned long long a = dq + (e >> 2) * (kPanelQ >> 4) + (e & 3) * 2, b = k + (e >> 2) * (kPanelK >> 4) + (e & 3) * 2;
                     umma_bf16(to, a, b, by_keys, e > 0);
@@ -181,9 +205,9 @@ template <bool CAPPED, int TURNS> __global__ void __launch_bounds__(kThreads, 3 
         scores(0);
         bool some = false;  // the sums hold something
         for (int i = 0; i < n; i++) {
-            if (TURNS == 2 && i + 1 < n) scores(i + 1);
-            const int j0 = (kt0 + i) * kKeys;
-            for (int h = 0; h < 2; h++) {
+            if (i + 1 < n) scores(i + 1);
+            const int j0 = (kt0 + i) * KEYS;
+            for (int h = 0; h < kHalves; h++) {
                 if (ok && !mbar_wait(w_full + (i & 1) * 16 + h * 8, (unsigned)(i >> 1) & 1)) ok = false;
                 if (!seen(j0, h)) continue;
                 if (ok && !mbar_wait(v_full + values_at.s * 8, values_at.parity)) ok = false;
@@ -192,16 +216,15 @@ template <bool CAPPED, int TURNS> __global__ void __launch_bounds__(kThreads, 3 
                     const unsigned long long v = dv + values_at.s * (v_stage >> 4);
 #pragma unroll
                     for (int e = 0; e < kPart / 16; e++)
-                        umma_weights(t_sum, tmem + (i % TURNS) * kKeys + h * (kPart / 2) + e * 8, v + e * 128, by_values, some || e > 0);
+                        umma_weights(t_sum, tmem + (i & 1) * KEYS + h * (kPart / 2) + e * 8, v + e * 128, by_values, some || e > 0);
                     umma_commit(v_free + values_at.s * 8);
                 }
                 __syncwarp();
                 some = true;
-                values_at.next(2);
+                values_at.next(kStagesV);
             }
             if (elect_one() && ok) umma_commit(o_done + (i & 1) * 8);
             __syncwarp();
-            if (TURNS == 1 && i + 1 < n) scores(i + 1);
         }
     }
     const int r = tid & (kRows - 1), tok = r / rep, head = g * rep + r % rep;
@@ -214,27 +237,27 @@ template <bool CAPPED, int TURNS> __global__ void __launch_bounds__(kThreads, 3 
         float m = -1e30f, l = 0.f;  // below every score, and finite: differences stay numbers
         RingAt values_at;
         for (int i = 0; i < n; i++) {
-            const int j0 = (kt0 + i) * kKeys;
-            const unsigned t_scores = tmem + lanes + (i % TURNS) * kKeys;
+            const int j0 = (kt0 + i) * KEYS;
+            const unsigned t_scores = tmem + lanes + (i & 1) * KEYS;
             if (ok && !mbar_wait(s_full + (i & 1) * 8, (unsigned)(i >> 1) & 1)) ok = false;
             after_sync();
-            unsigned v[4][32];
+            unsigned v[KEYS / 32][32];
 #pragma unroll
-            for (int c = 0; c < 4; c++) tmem_ld32(v[c], t_scores + c * 32);
+            for (int c = 0; c < KEYS / 32; c++) tmem_ld32(v[c], t_scores + c * 32);
             tmem_ld_wait();
             auto score = [&](int e) -> unsigned& { return v[e >> 5][e & 31]; };
             if (CAPPED) {
 #pragma unroll
-                for (int e = 0; e < kKeys; e++) score(e) = __float_as_uint(cap2 - __fdividef(2.f * cap2, 1.f + ex2(__uint_as_float(score(e)))));
+                for (int e = 0; e < KEYS; e++) score(e) = __float_as_uint(cap2 - __fdividef(2.f * cap2, 1.f + ex2(__uint_as_float(score(e)))));
             }
-            if (j0 + kKeys - 1 > pos0 || j0 < last_low) {
+            if (j0 + KEYS - 1 > pos0 || j0 < last_low) {
 #pragma unroll
-                for (int e = 0; e < kKeys; e++)
+                for (int e = 0; e < KEYS; e++)
                     if (j0 + e > pos || j0 + e < mine_low) score(e) = __float_as_uint(-INFINITY);
             }
             float top = __uint_as_float(score(0));
 #pragma unroll
-            for (int e = 1; e < kKeys; e++) top = fmaxf(top, __uint_as_float(score(e)));
+            for (int e = 1; e < KEYS; e++) top = fmaxf(top, __uint_as_float(score(e)));
             // Weights are taken against a maximum that may lie up to 2^8 behind: the sums are rarely taken anew, and bf16 holds 2^8 as well as 1.
             if (__any_sync(0xffffffffu, top > m + kLazy)) {
                 top = fmaxf(top, m);
@@ -256,7 +279,7 @@ template <bool CAPPED, int TURNS> __global__ void __launch_bounds__(kThreads, 3 
                 }
             }
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
+            for (int h = 0; h < kHalves; h++) {
                 if (seen(j0, h)) {
 #pragma unroll
                     for (int c = 0; c < 2; c++) {
@@ -281,7 +304,7 @@ template <bool CAPPED, int TURNS> __global__ void __launch_bounds__(kThreads, 3 
                         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     }
                     tmem_st_wait();
-                    values_at.next(2);
+                    values_at.next(kStagesV);
                 }
                 before_sync();
                 __syncwarp();
@@ -338,31 +361,37 @@ template <bool CAPPED, int TURNS> __global__ void __launch_bounds__(kThreads, 3 
                 *reinterpret_cast<float4*>(row + c + e) = o;
             }
         }
-        const float scale = p.gain ? 1.f / sqrtf(ss / (float)p.vdim + p.head_eps) : 1.f;
-        if (live && ok) {
-            bf16* out = (bf16*)p.out + ((sq.start + first + tok) * (long long)p.heads + head) * p.vdim;
-#pragma unroll 4
-            for (int c = 0; c < p.vdim; c += 8) {
-                float4 a = *reinterpret_cast<const float4*>(row + c), b = *reinterpret_cast<const float4*>(row + c + 4);
-                if (p.gain) {
-                    a.x *= scale * p.gain[c], a.y *= scale * p.gain[c + 1], a.z *= scale * p.gain[c + 2], a.w *= scale * p.gain[c + 3];
-                    b.x *= scale * p.gain[c + 4], b.y *= scale * p.gain[c + 5], b.z *= scale * p.gain[c + 6], b.w *= scale * p.gain[c + 7];
-                }
-                *reinterpret_cast<uint4*>(out + c) = make_uint4(pack_bf16(a.x, a.y), pack_bf16(a.z, a.w), pack_bf16(b.x, b.y), pack_bf16(b.z, b.w));
-            }
+        scales[r & 63] = p.gain ? 1.f / sqrtf(ss / (float)p.vdim + p.head_eps) : 1.f;
+    }
+    before_sync();
+    __syncthreads();
+    after_sync();
+    // a warp per row, sixteen bytes per lane
+    for (int u = lane; u < p.vdim / 8 && ok; u += 32) {
+        float gain[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) gain[e] = p.gain ? p.gain[u * 8 + e] : 1.f;
+        for (int i = warp; i < 64; i += kThreads / 32) {
+            const int at = map * 64 + i, t = at / rep;
+            if (t >= n_tok) break;
+            const float* row = reinterpret_cast<const float*>(smem) + i * stride + u * 8;
+            const float4 a = *reinterpret_cast<const float4*>(row), b = *reinterpret_cast<const float4*>(row + 4);
+            const float x = scales[i];
+            bf16* out = (bf16*)p.out + ((sq.start + first + t) * (long long)p.heads + g * rep + at % rep) * p.vdim;
+            *reinterpret_cast<uint4*>(out + u * 8) = make_uint4(pack_bf16(a.x * x * gain[0], a.y * x * gain[1]), pack_bf16(a.z * x * gain[2], a.w * x * gain[3]),
+                                                              pack_bf16(b.x * x * gain[4], b.y * x * gain[5]), pack_bf16(b.z * x * gain[6], b.w * x * gain[7]));
         }
     }
     if (!ok && lane == 0) report(p.err, ERR_WAIT_TIMEOUT, p.node, (long long)blockIdx.x, (long long)warp);
-    before_sync();
-    __syncthreads();
     if (warp == 5) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(cols) : "memory");
 }
 
-// One place for scores where two CTAs fit an SM.
-int differential_turns(int kp, int vp) { return kp == 1 && vp <= 2 ? 1 : 2; }
+// Two CTAs per SM where their shared and tensor memory allow it.
+int differential_keys(int kp, int vp) { return kp == 1 && vp <= 2 ? 64 : 128; }
 // No more CTAs share an SM than have room in its tensor memory: with 256 columns of 512 at most two (80 KB and more each), with all of them one (118 KB and more).
 int differential_smem(int kp, int vp) {
-    return std::max(1024 + kp * (int)(2 * kPanelQ + 2 * kPanelK) + vp * 2 * (int)kPanelV + kBarriers * 8 + 16, differential_turns(kp, vp) == 1 ? 80 * 1024 : 118 * 1024);
+    const int keys = differential_keys(kp, vp);
+    return std::max(1024 + kp * (int)(2 * kPanelQ + 2 * keys * 128) + vp * (keys == 64 ? 3 : 2) * (int)kPanelV + kBarriers * 8 + 16 + 256, keys == 64 ? 80 * 1024 : 118 * 1024);
 }
 
 }  // namespace
@@ -380,8 +409,8 @@ void emit_differential_prefill(Emitter& em, const DiffP& kv, const TRef& keys, c
     p.vp = (kv.vdim + 63) / 64;
     p.box = std::min(kPart, 1 << kv.shift);
     const int64_t tq = kRows / (kv.heads / kv.kv_heads), rows = (int64_t)kv.n_pages * kv.kv_heads << kv.shift;
-    void (*const k)(const PreP) = differential_turns(p.kp, p.vp) == 1 ? (kv.cap2 > 0.f ? differential_prefill<true, 1> : differential_prefill<false, 1>)
-                                                                       : (kv.cap2 > 0.f ? differential_prefill<true, 2> : differential_prefill<false, 2>);
+    void (*const k)(const PreP) = differential_keys(p.kp, p.vp) == 64 ? (kv.cap2 > 0.f ? differential_prefill<true, 64> : differential_prefill<false, 64>)
+                                                                     : (kv.cap2 > 0.f ? differential_prefill<true, 128> : differential_prefill<false, 128>);
     const int smem = differential_smem(p.kp, p.vp);
     ensure_max_dynamic_smem((const void*)k, 226 * 1024);
     LaunchRec& rec = em.launch(k, dim3((unsigned)((kv.rows + tq - 1) / tq + kv.n_seqs), (unsigned)kv.kv_heads * 2), dim3(kThreads), (unsigned)smem, p, {}, "differential_prefill", /*pdl=*/true);

@@ -1,8 +1,8 @@
 // Prompts of differential attention in bf16 on tcgen05.
 //
 // A cluster of two CTAs owns 128 (token, head) rows of one key head, each CTA one of the two softmax maps: it walks over that map's keys KEYS (64 or 128) at a time. Queries come as
-// the sum of two bf16, base-2 units included, so scores need no factor: dim / 8 products of 128 × KEYS × 16 make them, a thread per row caps, masks and weighs them, and for each
-// 64 keys 4 products of 128 × vdim × 16 add the weights' share of the values; the scores of the next keys are made under the weights of these. Keys and values come by TMA.
+// the sum of two bf16, base-2 units included, so scores need no factor: dim / 8 products of 128 × KEYS × 16 make them, a thread per row and 64 keys caps, masks and weighs them, and
+// 4 products of 128 × vdim × 16 add their weights' share of the values; the scores of the next keys are made under the weights of these. Keys and values come by TMA.
 // In the end each CTA sends the other half of its rows, divided by their sums, through the cluster's shared memory, and forms difference, norm and results of its own half.
 #include "differential.cuh"
 
@@ -10,15 +10,15 @@ namespace oxk {
 
 namespace {
 
-constexpr int kRows = 128, kPart = 64, kSoft = 128, kThreads = kSoft + 64;  // warps 0-3 softmax, 4 copies, 5 issues products
+constexpr int kRows = 128, kPart = 64;
 constexpr unsigned kPanelQ = kRows * 128, kPanelV = kPart * 128;  // bytes: rows × 64 dimensions
-constexpr int kBarriers = 18;
+constexpr int kBarriers = 20;
 constexpr float kLazy = 8.f;  // how far (base 2) a row's scores may rise above the maximum that its weights are taken against
 
 struct PreP {
     alignas(64) unsigned char maps[2][128];  // keys, values: [rows of the pool, 2 · dim | vdim]
     DiffP kv;
-    int kp, vp, box;  // panels of 64 dimensions, keys per copy
+    int kp, vp, box, inv;  // panels of 64 dimensions, keys per copy, 2^16 / heads of a key head, rounded up
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -87,22 +87,28 @@ struct PagesAhead {
 };
 
 // KEYS 64: 256 columns of tensor memory (values of up to 128), two CTAs per SM, which work under each other's waits. 128: all columns.
-template <bool CAPPED, int KEYS> __global__ void __launch_bounds__(kThreads, KEYS == 64 ? 2 : 1) differential_prefill(const __grid_constant__ PreP pp) {
+template <int KEYS> struct Shape {
+    static constexpr int halves = KEYS / kPart, soft = halves * kRows, threads = soft + 64;  // softmax warps, one of copies, one that issues products
+    static constexpr int keys = KEYS == 64 ? 3 : 2, values = KEYS == 64 ? 3 : 2;           // tiles of keys and halves of values on their way
+};
+template <bool CAPPED, int KEYS> __global__ void __launch_bounds__(Shape<KEYS>::threads, KEYS == 64 ? 2 : 1) differential_prefill(const __grid_constant__ PreP pp) {
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     // (both CTAs of a cluster find the same place: their shared memory begins at the same address)
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     const DiffP& p = pp.kv;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, kp = pp.kp, vp = pp.vp, map = blockIdx.y & 1, g = blockIdx.y >> 1;
-    constexpr int kHalves = KEYS / kPart, kStagesV = 2 * kHalves > 3 ? 2 : 3;
+    constexpr int kHalves = Shape<KEYS>::halves, kSoft = Shape<KEYS>::soft, kThreads = Shape<KEYS>::threads, kStagesK = Shape<KEYS>::keys, kStagesV = Shape<KEYS>::values;
+    constexpr int kCopies = kSoft / 32, kIssues = kCopies + 1;  // warps
     constexpr unsigned kPanelK = KEYS * 128;
     const unsigned k_stage = kp * kPanelK, v_stage = vp * kPanelV;
-    const unsigned sq0 = smem_u32(smem), low0 = kp * kPanelQ, sk = sq0 + 2 * low0, sv = sk + 2 * k_stage, bars = sv + kStagesV * v_stage;
-    // barriers: keys there, free (two each), values there, free (three), scores there, products added (two), weights there (two halves of two)
-    const unsigned k_full = bars, k_free = bars + 16, v_full = bars + 32, v_free = bars + 56, s_full = bars + 80, o_done = bars + 96, w_full = bars + 112;
+    const unsigned sq0 = smem_u32(smem), low0 = kp * kPanelQ, sk = sq0 + 2 * low0, sv = sk + kStagesK * k_stage, bars = sv + kStagesV * v_stage;
+    // barriers: keys there, free, values there, free (three each), scores there, products added (two each), weights there (two halves of two)
+    const unsigned k_full = bars, k_free = bars + 24, v_full = bars + 48, v_free = bars + 72, s_full = bars + 96, o_done = bars + 112, w_full = bars + 128;
     unsigned* tmem_slot = reinterpret_cast<unsigned*>(smem + (bars + kBarriers * 8 - sq0));
     float* scales = reinterpret_cast<float*>(smem + (bars + kBarriers * 8 + 16 - sq0));  // [64]: what the norms divide by
+    float* shared = scales + 64;  // [turn][half of the keys][row]: what the two threads of a row tell each other
     if (tid == 0) {
-        for (int i = 0; i < kBarriers; i++) mbar_init(bars + i * 8, i >= kBarriers - 4 ? kSoft / 32 : 1);
+        for (int i = 0; i < kBarriers; i++) mbar_init(bars + i * 8, i >= kBarriers - 4 ? kRows / 32 : 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     pdl_wait();
@@ -115,16 +121,22 @@ template <bool CAPPED, int KEYS> __global__ void __launch_bounds__(kThreads, KEY
     // Scores in two turns of KEYS columns, sums behind them; weights take the place of the scores that their thread has read. No more CTAs than have room in tensor memory may be on
     // an SM at a time (differential_smem), or two clusters could wait for what the other one has.
     constexpr unsigned cols = KEYS * 4;
-    if (warp == 5) {
+    if (warp == kIssues) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(cols) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    for (int i = tid; i < kRows * kp * 16; i += kThreads) {
-        const int r = i / (kp * 16), c = i % (kp * 16), part = c >= kp * 8, d = c - part * kp * 8, tok = r / rep, h = g * rep + r % rep;
-        const bool live = tok < n_tok && d * 8 < p.dim;
-        const bf16* src = (const bf16*)p.q;
-        cp_async16(sq0 + part * low0 + (d >> 3) * kPanelQ + r * 128 + (((d & 7) ^ (r & 7)) << 4),
-                   live ? src + ((((long long)(sq.start + first + tok) * p.heads + h) * 2 + map) * 2 + part) * p.dim + d * 8 : src, live);
+    const int inv = pp.inv;
+    auto token_of = [&](int row) { return row * inv >> 16; };  // row / rep
+    {
+        const int shift = kp + 2, chunks = 1 << (shift + 1), c = tid & (chunks - 1), part = c >> shift, d = c - (part << shift);  // kp is 1 or 2
+        const bf16* src = (const bf16*)p.q + ((((long long)(sq.start + first) * p.heads + g * rep) * 2 + map) * 2 + part) * p.dim + d * 8;
+        const unsigned to = sq0 + part * low0 + (d >> 3) * kPanelQ;
+#pragma unroll 4
+        for (int r = tid / chunks; r < kRows; r += kThreads / chunks) {
+            const int tok = token_of(r), h = r - tok * rep;
+            const bool live = tok < n_tok && d * 8 < p.dim;
+            cp_async16(to + r * 128 + (((d & 7) ^ (r & 7)) << 4), live ? src + ((long long)tok * p.heads + h) * 4 * p.dim : (const bf16*)p.q, live);
+        }
     }
     cp_async_commit();
     cp_async_wait<0>();
@@ -142,7 +154,7 @@ template <bool CAPPED, int KEYS> __global__ void __launch_bounds__(kThreads, KEY
     // Whether some row of the CTA may see keys of half h of the tile that begins at j0. Halves that nobody sees are neither copied nor multiplied.
     auto seen = [&](int j0, int h) { return j0 + h * kPart <= last && j0 + h * kPart + kPart > low; };
 
-    if (warp == 4) {
+    if (warp == kCopies) {
         // Copies of a page's keys each, where a page holds fewer than a half; those that nobody sees are left out. A tile's keys are asked for before the values of the tile before it.
         const int box0 = max(low, kt0 * KEYS) / pp.box, box1 = last / pp.box;
         auto page = [&](int i) { return i + lane <= box1 ? (int)page_of(p, seq, (i + lane) * pp.box) : 0; };
@@ -161,9 +173,9 @@ template <bool CAPPED, int KEYS> __global__ void __launch_bounds__(kThreads, KEY
             }
         };
         auto copy_keys = [&](int i) {
-            if (i >= 2 && ok && !mbar_wait(k_free + keys_at.s * 8, keys_at.parity ^ 1)) ok = false;
+            if (i >= kStagesK && ok && !mbar_wait(k_free + keys_at.s * 8, keys_at.parity ^ 1)) ok = false;
             copy(0, keys_pages, (kt0 + i) * KEYS, KEYS, k_full + keys_at.s * 8, sk + keys_at.s * k_stage, kp, kPanelK, map * p.dim);
-            keys_at.next(2);
+            keys_at.next(kStagesK);
         };
         copy_keys(0);
         for (int i = 0; i < n && ok; i++) {
@@ -178,7 +190,7 @@ template <bool CAPPED, int KEYS> __global__ void __launch_bounds__(kThreads, KEY
             }
             ok = __all_sync(0xffffffffu, ok);
         }
-    } else if (warp == 5) {
+    } else if (warp == kIssues) {
         const unsigned base = (1u << 4) | (1u << 7) | (1u << 10) | (8u << 24);  // bf16 × bf16 → f32, M 128
         const unsigned by_keys = base | ((KEYS >> 3) << 17), by_values = base | (1u << 16) | ((unsigned)(vp * 8) << 17);  // the values' wide axis is the result's
         const unsigned long long dq = umma_kmajor_desc(sq0), dk = umma_kmajor_desc(sk), dv = umma_wide_desc(sv);
@@ -200,7 +212,7 @@ template <bool CAPPED, int KEYS> __global__ void __launch_bounds__(kThreads, KEY
                 umma_commit(s_full + (i & 1) * 8);
             }
             __syncwarp();
-            keys_at.next(2);
+            keys_at.next(kStagesK);
         };
         scores(0);
         bool some = false;  // the sums hold something
@@ -227,48 +239,64 @@ template <bool CAPPED, int KEYS> __global__ void __launch_bounds__(kThreads, KEY
             __syncwarp();
         }
     }
-    const int r = tid & (kRows - 1), tok = r / rep, head = g * rep + r % rep;
+    const int r = tid & (kRows - 1), part = tid / kRows, tok = token_of(r), head = g * rep + r - tok * rep;  // thread `part` of a row has its keys of half `part`
     const unsigned lanes = (unsigned)((warp & 3) * 32) << 16;
-    const bool live = tok < n_tok;
+    // what both threads of a row know: by the two warps that share its rows
+    auto both = [&](int turn, float mine) {
+        float* at = shared + turn * 2 * kRows + r;
+        at[part * kRows] = mine;
+        asm volatile("bar.sync %0, 64;" ::"r"(1 + (warp & 3)) : "memory");
+        return at[(part ^ 1) * kRows];
+    };
     float f = 0.f;
-    if (warp < 4) {
-        const int pos = live ? pos0 + tok : last, mine_low = first_key(p, pos), last_low = first_key(p, last);  // rows without a token compute something harmless
+    if (warp < kCopies) {
+        const int pos = tok < n_tok ? pos0 + tok : last, mine_low = first_key(p, pos), last_low = first_key(p, last);  // rows without a token compute something harmless
         const float cap2 = p.cap2;
-        float m = -1e30f, l = 0.f;  // below every score, and finite: differences stay numbers
-        RingAt values_at;
+        float m = -1e30f, l = 0.f, l2 = 0.f;  // below every score, and finite: differences stay numbers
+        int halves = 0;                       // of the values, in front of this thread's
         for (int i = 0; i < n; i++) {
-            const int j0 = (kt0 + i) * KEYS;
+            const int j0 = (kt0 + i) * KEYS, j1 = j0 + part * kPart;
             const unsigned t_scores = tmem + lanes + (i & 1) * KEYS;
             if (ok && !mbar_wait(s_full + (i & 1) * 8, (unsigned)(i >> 1) & 1)) ok = false;
             after_sync();
-            unsigned v[KEYS / 32][32];
+            float s[kPart];
 #pragma unroll
-            for (int c = 0; c < KEYS / 32; c++) tmem_ld32(v[c], t_scores + c * 32);
+            for (int c = 0; c < 2; c++) {
+                unsigned v[32];
+                tmem_ld32(v, t_scores + part * kPart + c * 32);
+#pragma unroll
+                for (int e = 0; e < 32; e++) s[c * 32 + e] = __uint_as_float(v[e]);
+            }
             tmem_ld_wait();
-            auto score = [&](int e) -> unsigned& { return v[e >> 5][e & 31]; };
             if (CAPPED) {
 #pragma unroll
-                for (int e = 0; e < KEYS; e++) score(e) = __float_as_uint(cap2 - __fdividef(2.f * cap2, 1.f + ex2(__uint_as_float(score(e)))));
+                for (int e = 0; e < kPart; e++) s[e] = cap2 - __fdividef(2.f * cap2, 1.f + ex2(s[e]));
             }
-            if (j0 + KEYS - 1 > pos0 || j0 < last_low) {
+            if (j1 + kPart - 1 > pos0 || j1 < last_low) {
 #pragma unroll
-                for (int e = 0; e < KEYS; e++)
-                    if (j0 + e > pos || j0 + e < mine_low) score(e) = __float_as_uint(-INFINITY);
+                for (int e = 0; e < kPart; e++)
+                    if (j1 + e > pos || j1 + e < mine_low) s[e] = -INFINITY;
             }
-            float top = __uint_as_float(score(0));
+            float top = fmaxf(s[0], s[1]), top2 = fmaxf(s[2], s[3]);
 #pragma unroll
-            for (int e = 1; e < KEYS; e++) top = fmaxf(top, __uint_as_float(score(e)));
-            // Weights are taken against a maximum that may lie up to 2^8 behind: the sums are rarely taken anew, and bf16 holds 2^8 as well as 1.
+            for (int e = 4; e < kPart; e += 4) {
+                top = fmaxf(top, fmaxf(s[e], s[e + 1]));
+                top2 = fmaxf(top2, fmaxf(s[e + 2], s[e + 3]));
+            }
+            top = fmaxf(top, top2);
+            if (kHalves == 2) top = fmaxf(top, both(i & 1, top));
+            // Weights are taken against a maximum that may lie up to 2^8 behind: the sums are rarely taken anew, and bf16 holds 2^8 as well as 1. Both warps of a row see the same tops.
             if (__any_sync(0xffffffffu, top > m + kLazy)) {
                 top = fmaxf(top, m);
                 const float keep = ex2(m - top);
                 m = top;
                 l *= keep;
+                l2 *= keep;
                 if (i > 0) {
                     if (ok && !added(i - 1)) ok = false;
                     after_sync();
 #pragma unroll 1
-                    for (int c = 0; c < vp * 64; c += 16) {
+                    for (int c = part * 16; c < vp * 64; c += 16 * kHalves) {
                         unsigned o[16];
                         tmem_ld16(o, t_sum + lanes + c);
                         tmem_ld_wait();
@@ -278,39 +306,39 @@ template <bool CAPPED, int KEYS> __global__ void __launch_bounds__(kThreads, KEY
                     }
                 }
             }
+            const int before = kHalves == 2 && part == 1 && seen(j0, 0);  // the other half's values come first
+            if (seen(j0, part)) {
 #pragma unroll
-            for (int h = 0; h < kHalves; h++) {
-                if (seen(j0, h)) {
+                for (int c = 0; c < 2; c++) {
+                    unsigned w[16];
 #pragma unroll
-                    for (int c = 0; c < 2; c++) {
-                        unsigned w[16];
-#pragma unroll
-                        for (int e = 0; e < 16; e++) {
-                            const int at = h * kPart + c * 32 + 2 * e;
-                            w[e] = pack_bf16(ex2(__uint_as_float(score(at)) - m), ex2(__uint_as_float(score(at + 1)) - m));
-                            // the sum of the weights as they are multiplied: the rounding of a weight that stands out is in both
-                            l += __uint_as_float(w[e] << 16) + __uint_as_float(w[e] & 0xFFFF0000u);
-                        }
-                        tmem_st16(t_scores + h * (kPart / 2) + c * 16, w);
+                    for (int e = 0; e < 16; e++) {
+                        w[e] = pack_bf16(ex2(s[c * 32 + 2 * e] - m), ex2(s[c * 32 + 2 * e + 1] - m));
+                        // the sums of the weights as they are multiplied: the rounding of a weight that stands out is in both
+                        l += __uint_as_float(w[e] << 16);
+                        l2 += __uint_as_float(w[e] & 0xFFFF0000u);
                     }
-                    const int j1 = j0 + h * kPart;
-                    if (j1 + kPart - 1 > last || j1 < low) {  // what lies behind the last key or in front of the first may be no number, which a weight of 0 would not cancel
-                        if (ok && !mbar_wait(v_full + values_at.s * 8, values_at.parity)) ok = false;
-                        for (int u = tid; u < kPart * vp * 8; u += kSoft) {
-                            const int key = u & (kPart - 1), c = u / kPart;
-                            const unsigned to = sv + values_at.s * v_stage + (c >> 3) * kPanelV + key * 128 + (c & 7) * 16;
-                            if (j1 + key > last || j1 + key < low) asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(to), "r"(0) : "memory");
-                        }
-                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                    }
-                    tmem_st_wait();
-                    values_at.next(kStagesV);
+                    tmem_st16(t_scores + part * (kPart / 2) + c * 16, w);
                 }
-                before_sync();
-                __syncwarp();
-                if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(w_full + (i & 1) * 16 + h * 8) : "memory");
+                if (j1 + kPart - 1 > last || j1 < low) {  // what lies behind the last key or in front of the first may be no number, which a weight of 0 would not cancel
+                    const int at = halves + before, stage = at % kStagesV;
+                    if (ok && !mbar_wait(v_full + stage * 8, (unsigned)(at / kStagesV) & 1)) ok = false;
+                    for (int u = r; u < kPart * vp * 8; u += kRows) {
+                        const int key = u & (kPart - 1), c = u / kPart;
+                        const unsigned to = sv + stage * v_stage + (c >> 3) * kPanelV + key * 128 + (c & 7) * 16;
+                        if (j1 + key > last || j1 + key < low) asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(to), "r"(0) : "memory");
+                    }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                }
+                tmem_st_wait();
             }
+            before_sync();
+            __syncwarp();
+            if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(w_full + (i & 1) * 16 + part * 8) : "memory");
+            halves += seen(j0, 0) + (kHalves == 2 && seen(j0, 1));
         }
+        l += l2;
+        if (kHalves == 2) l += both(n & 1, l);
         if (ok && !added(n - 1)) ok = false;
         after_sync();
         f = 1.f / l;
@@ -325,11 +353,11 @@ template <bool CAPPED, int KEYS> __global__ void __launch_bounds__(kThreads, KEY
     const int stride = vp * 64 + 4;
     const unsigned mine = sq0 + (r & 63) * stride * 4;
     const bool keeps = (r >> 6) == map;  // CTA 0 has the first 64 rows
-    if (warp < 4 && !keeps) {
+    if (warp < kCopies && !keeps) {
         unsigned to;
         asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(mine), "r"(map ^ 1));
 #pragma unroll 1
-        for (int c = 0; c < vp * 64; c += 32) {
+        for (int c = part * 32; c < vp * 64; c += 32 * kHalves) {
             unsigned v[32];
             tmem_ld32(v, t_sum + lanes + c);
             tmem_ld_wait();
@@ -341,12 +369,12 @@ template <bool CAPPED, int KEYS> __global__ void __launch_bounds__(kThreads, KEY
         }
     }
     cluster_meet();
-    if (warp < 4 && keeps) {
+    if (warp < kCopies && keeps) {
         float* row = reinterpret_cast<float*>(smem + (mine - sq0));
         const float sign = map ? -1.f : 1.f;
         float ss = 0.f;
 #pragma unroll 1
-        for (int c = 0; c < vp * 64; c += 32) {
+        for (int c = part * 32; c < vp * 64; c += 32 * kHalves) {
             unsigned v[32];
             tmem_ld32(v, t_sum + lanes + c);
             tmem_ld_wait();
@@ -361,29 +389,33 @@ template <bool CAPPED, int KEYS> __global__ void __launch_bounds__(kThreads, KEY
                 *reinterpret_cast<float4*>(row + c + e) = o;
             }
         }
+        if (kHalves == 2) ss += both(0, ss);
         scales[r & 63] = p.gain ? 1.f / sqrtf(ss / (float)p.vdim + p.head_eps) : 1.f;
     }
     before_sync();
     __syncthreads();
     after_sync();
-    // a warp per row, sixteen bytes per lane
-    for (int u = lane; u < p.vdim / 8 && ok; u += 32) {
-        float gain[8];
+    // a row is written by neighbouring lanes, sixteen bytes each
+    const int wide = p.vdim / 8;
+    if (ok)
+        for (int c = tid % 32; c < wide; c += 32) {
+            float gain[8];
 #pragma unroll
-        for (int e = 0; e < 8; e++) gain[e] = p.gain ? p.gain[u * 8 + e] : 1.f;
-        for (int i = warp; i < 64; i += kThreads / 32) {
-            const int at = map * 64 + i, t = at / rep;
-            if (t >= n_tok) break;
-            const float* row = reinterpret_cast<const float*>(smem) + i * stride + u * 8;
-            const float4 a = *reinterpret_cast<const float4*>(row), b = *reinterpret_cast<const float4*>(row + 4);
-            const float x = scales[i];
-            bf16* out = (bf16*)p.out + ((sq.start + first + t) * (long long)p.heads + g * rep + at % rep) * p.vdim;
-            *reinterpret_cast<uint4*>(out + u * 8) = make_uint4(pack_bf16(a.x * x * gain[0], a.y * x * gain[1]), pack_bf16(a.z * x * gain[2], a.w * x * gain[3]),
-                                                              pack_bf16(b.x * x * gain[4], b.y * x * gain[5]), pack_bf16(b.z * x * gain[6], b.w * x * gain[7]));
+            for (int e = 0; e < 8; e++) gain[e] = p.gain ? p.gain[c * 8 + e] : 1.f;
+#pragma unroll 4
+            for (int i = warp; i < 64; i += kThreads / 32) {
+                const int at = map * 64 + i, t = token_of(at);
+                const float* row = reinterpret_cast<const float*>(smem) + i * stride + c * 8;
+                const float4 a = *reinterpret_cast<const float4*>(row), b = *reinterpret_cast<const float4*>(row + 4);
+                const float x = scales[i];
+                if (t < n_tok)
+                    *reinterpret_cast<uint4*>((bf16*)p.out + ((sq.start + first + t) * (long long)p.heads + g * rep + at - t * rep) * p.vdim + c * 8) =
+                        make_uint4(pack_bf16(a.x * x * gain[0], a.y * x * gain[1]), pack_bf16(a.z * x * gain[2], a.w * x * gain[3]), pack_bf16(b.x * x * gain[4], b.y * x * gain[5]),
+                                   pack_bf16(b.z * x * gain[6], b.w * x * gain[7]));
+            }
         }
-    }
     if (!ok && lane == 0) report(p.err, ERR_WAIT_TIMEOUT, p.node, (long long)blockIdx.x, (long long)warp);
-    if (warp == 5) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(cols) : "memory");
+    if (warp == kIssues) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(cols) : "memory");
 }
 
 // Two CTAs per SM where their shared and tensor memory allow it.
@@ -391,7 +423,8 @@ int differential_keys(int kp, int vp) { return kp == 1 && vp <= 2 ? 64 : 128; }
 // No more CTAs share an SM than have room in its tensor memory: with 256 columns of 512 at most two (80 KB and more each), with all of them one (118 KB and more).
 int differential_smem(int kp, int vp) {
     const int keys = differential_keys(kp, vp);
-    return std::max(1024 + kp * (int)(2 * kPanelQ + 2 * keys * 128) + vp * (keys == 64 ? 3 : 2) * (int)kPanelV + kBarriers * 8 + 16 + 256, keys == 64 ? 80 * 1024 : 118 * 1024);
+    const int kv = keys == 64 ? Shape<64>::keys * 64 * 128 * kp + Shape<64>::values * (int)kPanelV * vp : Shape<128>::keys * 128 * 128 * kp + Shape<128>::values * (int)kPanelV * vp;
+    return std::max(1024 + kp * 2 * (int)kPanelQ + kv + kBarriers * 8 + 16 + 256 + 4 * kRows * 4, keys == 64 ? 80 * 1024 : 118 * 1024);
 }
 
 }  // namespace
@@ -408,12 +441,13 @@ void emit_differential_prefill(Emitter& em, const DiffP& kv, const TRef& keys, c
     p.kp = (kv.dim + 63) / 64;
     p.vp = (kv.vdim + 63) / 64;
     p.box = std::min(kPart, 1 << kv.shift);
+    p.inv = (65536 + kv.heads / kv.kv_heads - 1) / (kv.heads / kv.kv_heads);
     const int64_t tq = kRows / (kv.heads / kv.kv_heads), rows = (int64_t)kv.n_pages * kv.kv_heads << kv.shift;
     void (*const k)(const PreP) = differential_keys(p.kp, p.vp) == 64 ? (kv.cap2 > 0.f ? differential_prefill<true, 64> : differential_prefill<false, 64>)
                                                                      : (kv.cap2 > 0.f ? differential_prefill<true, 128> : differential_prefill<false, 128>);
     const int smem = differential_smem(p.kp, p.vp);
     ensure_max_dynamic_smem((const void*)k, 226 * 1024);
-    LaunchRec& rec = em.launch(k, dim3((unsigned)((kv.rows + tq - 1) / tq + kv.n_seqs), (unsigned)kv.kv_heads * 2), dim3(kThreads), (unsigned)smem, p, {}, "differential_prefill", /*pdl=*/true);
+    LaunchRec& rec = em.launch(k, dim3((unsigned)((kv.rows + tq - 1) / tq + kv.n_seqs), (unsigned)kv.kv_heads * 2), dim3(differential_keys(p.kp, p.vp) == 64 ? Shape<64>::threads : Shape<128>::threads), (unsigned)smem, p, {}, "differential_prefill", /*pdl=*/true);
     rec.cluster = dim3(1, 2, 1);
     for (auto& pr : ptrs) rec.relocs.push_back(Reloc{(uint32_t)(offsetof(PreP, kv) + pr.first), pr.second});
     rec.tmaps.push_back(TmapReloc{(uint32_t)offsetof(PreP, maps), keys.buf, (uint64_t)kv.dim * 2, (uint64_t)rows, (uint64_t)kv.dim * 4, 64u, (uint32_t)p.box});

@@ -1,39 +1,116 @@
-// Prompts of differential attention in bf16 on tcgen05, maps of more than 64 dimensions or values of more than 128 (differential_pair.cu has the others).
+// Prompts of differential attention in bf16 on tcgen05.
 //
-// A cluster of two CTAs owns 128 (token, head) rows of one key head, each CTA one of the two softmax maps: it walks over that map's keys 128 at a time. Queries come as
-// the sum of two bf16, base-2 units included, so scores need no factor: dim / 8 products of 128 × 128 × 16 make them, a thread per row and 64 keys caps, masks and weighs them, and
-// 4 products of 128 × vdim × 16 add their weights' share of the values; the scores of the next keys are made under the weights of these. Keys and values come by TMA.
+// A cluster of two CTAs owns 128 (token, head) rows of one key head, each CTA one of the two softmax maps: it walks over that map's keys KEYS (64 or 128) at a time. Queries come as
+// the sum of two bf16, base-2 units included, so scores need no factor: dim / 8 products of 128 × KEYS × 16 make them, a thread per row and 64 keys caps, masks and weighs them, and
+// 4 products of 128 × vdim × 16 add their weights' share of the values. Keys and values come by TMA.
+// From the order to a product to the word that it is done it takes 400 cycles, more than most products themselves (N 64: 47, N 128: 62 each). So nothing waits for two in a row: scores have one
+// place, free as soon as they have been read, weights have two of their own, and the next scores are made, and the last weights multiplied, under the exponentials of these.
 // In the end each CTA sends the other half of its rows, divided by their sums, through the cluster's shared memory, and forms difference, norm and results of its own half.
-#include "differential_tc.cuh"
+#include "differential.cuh"
 
 namespace oxk {
 
 namespace {
 
-constexpr int kKeys = 128, kHalves = 2, kSoft = kHalves * kRows, kCopies = kSoft / 32, kIssues = kCopies + 1, kThreads = kSoft + 64;  // softmax warps, one of copies, one that issues products
-constexpr int kBarriers = 16;
-constexpr unsigned kPanelK = kKeys * 128;
+constexpr int kRows = 128, kPart = 64;
+constexpr unsigned kPanelQ = kRows * 128, kPanelV = kPart * 128;  // bytes: rows × 64 dimensions
+constexpr int kBarriers = 20;
+constexpr float kLazy = 8.f;  // how far (base 2) a row's scores may rise above the maximum that its weights are taken against
 
+struct PreP {
+    alignas(64) unsigned char maps[2][128];  // keys, values: [rows of the pool, 2 · dim | vdim]
+    DiffP kv;
+    int kp, vp, box, inv;  // panels of 64 dimensions, log2 of the keys per copy, 2^16 / heads of a key head, rounded up
+};
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// Rows of weights in tensor memory (two per column) × values, of which 64 stand side by side for a key.
+__device__ __forceinline__ void umma_weights(unsigned d, unsigned a, unsigned long long b, unsigned idesc, bool accumulate) {
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+        " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n}\n" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(accumulate ? 1u : 0u), "r"(0u)
+        : "memory");
+}
+// Shared-memory matrix descriptor, 128-byte swizzle, 64 elements of the wide axis side by side: groups of eight keys 1 024 bytes apart, the next 64
+// elements a panel further.
+__device__ __forceinline__ unsigned long long umma_wide_desc(unsigned smem_byte_addr) {
+    return (unsigned long long)((smem_byte_addr & 0x3FFFFu) >> 4) | ((unsigned long long)(kPanelV >> 4) << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
+}
+__device__ __forceinline__ void tmem_ld32(unsigned (&v)[32], unsigned from) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, "
+        "%21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]),
+          "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]),
+          "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]),
+          "=r"(v[30]), "=r"(v[31])
+        : "r"(from));
+}
+__device__ __forceinline__ void tmem_ld16(unsigned (&v)[16], unsigned from) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]),
+          "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+        : "r"(from));
+}
+__device__ __forceinline__ void tmem_st16(unsigned to, const unsigned (&v)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};\n" ::"r"(v[0]), "r"(v[1]), "r"(v[2]),
+        "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(to)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void before_sync() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void after_sync() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 // All threads of both CTAs. Every thread of a CTA that has a tile comes here, whatever its waits found.
 __device__ __forceinline__ void cluster_meet() {
     asm volatile("barrier.cluster.arrive.release;\n barrier.cluster.wait.acquire;" ::: "memory");
 }
 
-template <bool CAPPED> __global__ void __launch_bounds__(kThreads, 1) differential_prefill(const __grid_constant__ PreP pp) {
+// The pages of the copies to come, 32 at a time and the next 32 on their way: the table's answer to a single question takes as long as a copy.
+struct PagesAhead {
+    int first, now, next;
+    template <class Page> __device__ __forceinline__ PagesAhead(int from, Page&& page) : first(from), now(page(from)), next(page(from + 32)) {}
+    // of box i, which does not fall; all lanes ask the same
+    template <class Page> __device__ __forceinline__ int of(int i, Page&& page) {
+        if (i >= first + 32) {
+            first += 32;
+            now = next;
+            next = page(first + 32);
+        }
+        return __shfl_sync(0xffffffffu, now, i - first);
+    }
+};
+
+// KEYS 64: 256 columns of tensor memory (values of up to 128), two CTAs per SM, which work under each other's waits. 128: all columns.
+template <int KEYS> struct Shape {
+    static constexpr int halves = KEYS / kPart, soft = halves * kRows, threads = soft + 64;  // softmax warps, one of copies, one that issues products
+    static constexpr int keys = KEYS == 64 ? 3 : 2, values = KEYS == 64 ? 3 : 2;           // tiles of keys and halves of values on their way
+};
+template <bool CAPPED, int KEYS> __global__ void __launch_bounds__(Shape<KEYS>::threads, KEYS == 64 ? 2 : 1) differential_prefill(const __grid_constant__ PreP pp) {
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     // (both CTAs of a cluster find the same place: their shared memory begins at the same address)
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     const DiffP& p = pp.kv;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, kp = pp.kp, vp = pp.vp, map = blockIdx.y & 1, g = blockIdx.y >> 1;
+    constexpr int kHalves = Shape<KEYS>::halves, kSoft = Shape<KEYS>::soft, kThreads = Shape<KEYS>::threads, kStagesK = Shape<KEYS>::keys, kStagesV = Shape<KEYS>::values;
+    constexpr int kCopies = kSoft / 32, kIssues = kCopies + 1;  // warps
+    constexpr unsigned kPanelK = KEYS * 128;
     const unsigned k_stage = kp * kPanelK, v_stage = vp * kPanelV;
-    const unsigned sq0 = smem_u32(smem), low0 = kp * kPanelQ, sk = sq0 + 2 * low0, sv = sk + 2 * k_stage, bars = sv + 2 * v_stage;
-    // barriers: keys there, free, values there, free, scores there, products added (two each), weights there (two halves of two)
-    const unsigned k_full = bars, k_free = bars + 16, v_full = bars + 32, v_free = bars + 48, s_full = bars + 64, o_done = bars + 80, w_full = bars + 96;
+    const unsigned sq0 = smem_u32(smem), low0 = kp * kPanelQ, sk = sq0 + 2 * low0, sv = sk + kStagesK * k_stage, bars = sv + kStagesV * v_stage;
+    // barriers: keys there, free, values there, free (three each), scores there, read, products added (one, one and two), weights there (two halves of two)
+    const unsigned k_full = bars, k_free = bars + 24, v_full = bars + 48, v_free = bars + 72, s_full = bars + 96, s_free = bars + 104, o_done = bars + 112, w_full = bars + 128;
     unsigned* tmem_slot = reinterpret_cast<unsigned*>(smem + (bars + kBarriers * 8 - sq0));
     float* scales = reinterpret_cast<float*>(smem + (bars + kBarriers * 8 + 16 - sq0));  // [64]: what the norms divide by
     float* shared = scales + 64;  // [turn][half of the keys][row]: what the two threads of a row tell each other
     if (tid == 0) {
-        for (int i = 0; i < kBarriers; i++) mbar_init(bars + i * 8, i >= kBarriers - 4 ? kRows / 32 : 1);
+        for (int i = 0; i < kBarriers; i++) mbar_init(bars + i * 8, i == 13 ? kSoft / 32 : i >= kBarriers - 4 ? kRows / 32 : 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     pdl_wait();
@@ -43,9 +120,9 @@ template <bool CAPPED> __global__ void __launch_bounds__(kThreads, 1) differenti
     if (!locate_tile(p.seqs, p.n_seqs, (int)gridDim.x - 1 - (int)blockIdx.x, tq, &seq, &first, p.singles ? 1 : 2)) return;  // both CTAs of the cluster
     const SeqRow sq = load_seq(p.seqs, seq);
     const int n_tok = min(tq, sq.len - first), pos0 = sq.past + first, last = pos0 + n_tok - 1, low = first_key(p, pos0);
-    // Scores in two turns of 128 columns, sums behind them; weights take the place of the scores that their thread has read. One CTA at a time may be on an SM (cluster_smem), or two
-    // clusters could wait for tensor memory that the other one has.
-    constexpr unsigned cols = 512;
+    // Scores in KEYS columns, weights in two turns of half as many, sums behind them. No more CTAs than have room in tensor memory may be on an SM at a time
+    // (differential_smem), or two clusters could wait for what the other one has.
+    constexpr unsigned cols = KEYS * 4;
     if (warp == kIssues) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(cols) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -70,80 +147,86 @@ template <bool CAPPED> __global__ void __launch_bounds__(kThreads, 1) differenti
     __syncthreads();
     after_sync();
     pdl_trigger();  // the tensor memory is taken: nothing that starts now can keep it from this CTA
-    const unsigned tmem = *tmem_slot, t_sum = tmem + 2 * kKeys;
-    const int kt0 = low / kKeys, n = last / kKeys + 1 - kt0;
+    const unsigned tmem = *tmem_slot, t_sum = tmem + 2 * KEYS;
+    const int kt0 = low / KEYS, n = last / KEYS + 1 - kt0;
     bool ok = true;
-    // Waits until the products of tile i are in the sums. Tiles take turns at two barriers. Who has the scores of tile i knows the products of tile i - 2 and of all before it to be
-    // done, so the barrier of tile i - 1 or i cannot be a round behind.
+    // Waits until the products of tile i are in the sums. Tiles take turns at two barriers, and who asks has not let the products of tile i + 2 begin: the barrier cannot be a round
+    // ahead. Nor can it be two behind: each tile is asked for in its turn.
     auto added = [&](int i) { return mbar_wait(o_done + (i & 1) * 8, (unsigned)(i >> 1) & 1); };
     // Whether some row of the CTA may see keys of half h of the tile that begins at j0. Halves that nobody sees are neither copied nor multiplied.
     auto seen = [&](int j0, int h) { return j0 + h * kPart <= last && j0 + h * kPart + kPart > low; };
 
     if (warp == kCopies) {
         // Copies of a page's keys each, where a page holds fewer than a half; those that nobody sees are left out. A tile's keys are asked for before the values of the tile before it.
-        const int box0 = max(low, kt0 * kKeys) / pp.box, box1 = last / pp.box;
-        auto page = [&](int i) { return i + lane <= box1 ? (int)page_of(p, seq, (i + lane) * pp.box) : 0; };
+        const int box = pp.box, box0 = max(low, kt0 * KEYS) >> box, box1 = last >> box;
+        auto page = [&](int i) { return i + lane <= box1 ? (int)page_of(p, seq, (i + lane) << box) : 0; };
         PagesAhead keys_pages(box0, page), values_pages(box0, page);
         RingAt keys_at, values_at;
         int halves = 0;
-        auto copy = [&](int kv, PagesAhead& pages, int j0, int keys, unsigned full, unsigned to, int panels, unsigned panel, int x) {
-            const int b0 = max(j0 / pp.box, box0), b1 = min((j0 + keys) / pp.box - 1, box1);
-            if (elect_one() && ok) mbar_expect_tx(full, (unsigned)((b1 - b0 + 1) * pp.box * 128 * panels));
-            __syncwarp();
+        auto copy = [&](const unsigned char* map_of, PagesAhead& pages, int j0, int keys, unsigned full, unsigned to, int panels, unsigned panel, int x) {
+            const int b0 = max(j0 >> box, box0), b1 = min(((j0 + keys) >> box) - 1, box1);
             for (int b = b0; b <= b1; b++) {
-                const int j = b * pp.box, row = (int)key_row(p, pages.of(b, page), g, j);
-                if (elect_one() && ok)
-                    for (int c = 0; c < panels; c++) tma_load_2d(to + c * panel + (j - j0) * 128, pp.maps[kv], x + c * 64, row, full);
+                const int j = b << box, row = (int)key_row(p, pages.of(b, page), g, j);
+                const unsigned at = to + (j - j0) * 128;
+                if (elect_one() && ok) {
+                    if (b == b0) mbar_expect_tx(full, (unsigned)(((b1 - b0 + 1) << box) * 128 * panels));
+                    tma_load_2d(at, map_of, x, row, full);
+                    if (panels > 1) tma_load_2d(at + panel, map_of, x + 64, row, full);
+                    if (panels > 2) tma_load_2d(at + 2 * panel, map_of, x + 128, row, full);
+                    if (panels > 3) tma_load_2d(at + 3 * panel, map_of, x + 192, row, full);
+                }
                 __syncwarp();
             }
         };
         auto copy_keys = [&](int i) {
-            if (i >= 2 && ok && !mbar_wait(k_free + keys_at.s * 8, keys_at.parity ^ 1)) ok = false;
-            copy(0, keys_pages, (kt0 + i) * kKeys, kKeys, k_full + keys_at.s * 8, sk + keys_at.s * k_stage, kp, kPanelK, map * p.dim);
-            keys_at.next(2);
+            if (i >= kStagesK && ok && !mbar_wait(k_free + keys_at.s * 8, keys_at.parity ^ 1)) ok = false;
+            copy(pp.maps[0], keys_pages, (kt0 + i) * KEYS, KEYS, k_full + keys_at.s * 8, sk + keys_at.s * k_stage, kp, kPanelK, map * p.dim);
+            keys_at.next(kStagesK);
         };
         copy_keys(0);
         for (int i = 0; i < n && ok; i++) {
             if (i + 1 < n) copy_keys(i + 1);
-            const int j0 = (kt0 + i) * kKeys;
+            const int j0 = (kt0 + i) * KEYS;
             for (int h = 0; h < kHalves; h++) {
                 if (!seen(j0, h)) continue;
-                if (halves >= 2 && ok && !mbar_wait(v_free + values_at.s * 8, values_at.parity ^ 1)) ok = false;
-                copy(1, values_pages, j0 + h * kPart, kPart, v_full + values_at.s * 8, sv + values_at.s * v_stage, vp, kPanelV, 0);
-                values_at.next(2);
+                if (halves >= kStagesV && ok && !mbar_wait(v_free + values_at.s * 8, values_at.parity ^ 1)) ok = false;
+                copy(pp.maps[1], values_pages, j0 + h * kPart, kPart, v_full + values_at.s * 8, sv + values_at.s * v_stage, vp, kPanelV, 0);
+                values_at.next(kStagesV);
                 halves++;
             }
             ok = __all_sync(0xffffffffu, ok);
         }
     } else if (warp == kIssues) {
         const unsigned base = (1u << 4) | (1u << 7) | (1u << 10) | (8u << 24);  // bf16 × bf16 → f32, M 128
-        const unsigned by_keys = base | ((kKeys >> 3) << 17), by_values = base | (1u << 16) | ((unsigned)(vp * 8) << 17);  // the values' wide axis is the result's
+        const unsigned by_keys = base | ((KEYS >> 3) << 17), by_values = base | (1u << 16) | ((unsigned)(vp * 8) << 17);  // the values' wide axis is the result's
         const unsigned long long dq = umma_kmajor_desc(sq0), dk = umma_kmajor_desc(sk), dv = umma_wide_desc(sv);
         RingAt keys_at, values_at;
         auto scores = [&](int i) {
             if (ok && !mbar_wait(k_full + keys_at.s * 8, keys_at.parity)) ok = false;
-            // the products that read the weights in these scores' place have to be done
-            if (i >= 2 && ok && !added(i - 2)) ok = false;
+            if (i > 0 && ok && !mbar_wait(s_free, (unsigned)(i - 1) & 1)) ok = false;
             after_sync();
             if (elect_one() && ok) {
                 const unsigned long long k = dk + keys_at.s * (k_stage >> 4);
-                const unsigned to = tmem + (i & 1) * kKeys;
-                for (int e = 0; e < p.dim / 16; e++) {
-                    const unsigned long long a = dq + (e >> 2) * (kPanelQ >> 4) + (e & 3) * 2, b = k + (e >> 2) * (kPanelK >> 4) + (e & 3) * 2;
-                    umma_bf16(to, a, b, by_keys, e > 0);
-                    umma_bf16(to, a + (low0 >> 4), b, by_keys, true);
+                                for (int c = 0; c < kp; c++) {
+                    const unsigned long long a = dq + c * (kPanelQ >> 4), a2 = a + (low0 >> 4), b = k + c * (kPanelK >> 4);
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        if (c * 64 + e * 16 < p.dim) {
+                            umma_bf16(tmem, a + e * 2, b + e * 2, by_keys, c > 0 || e > 0);
+                            umma_bf16(tmem, a2 + e * 2, b + e * 2, by_keys, true);
+                        }
                 }
                 umma_commit(k_free + keys_at.s * 8);
-                umma_commit(s_full + (i & 1) * 8);
+                umma_commit(s_full);
             }
             __syncwarp();
-            keys_at.next(2);
+            keys_at.next(kStagesK);
         };
         scores(0);
         bool some = false;  // the sums hold something
         for (int i = 0; i < n; i++) {
             if (i + 1 < n) scores(i + 1);
-            const int j0 = (kt0 + i) * kKeys;
+            const int j0 = (kt0 + i) * KEYS;
             for (int h = 0; h < kHalves; h++) {
                 if (ok && !mbar_wait(w_full + (i & 1) * 16 + h * 8, (unsigned)(i >> 1) & 1)) ok = false;
                 if (!seen(j0, h)) continue;
@@ -153,12 +236,12 @@ template <bool CAPPED> __global__ void __launch_bounds__(kThreads, 1) differenti
                     const unsigned long long v = dv + values_at.s * (v_stage >> 4);
 #pragma unroll
                     for (int e = 0; e < kPart / 16; e++)
-                        umma_weights(t_sum, tmem + (i & 1) * kKeys + h * (kPart / 2) + e * 8, v + e * 128, by_values, some || e > 0);
+                        umma_weights(t_sum, tmem + KEYS + (i & 1) * (KEYS / 2) + h * (kPart / 2) + e * 8, v + e * 128, by_values, some || e > 0);
                     umma_commit(v_free + values_at.s * 8);
                 }
                 __syncwarp();
                 some = true;
-                values_at.next(2);
+                values_at.next(kStagesV);
             }
             if (elect_one() && ok) umma_commit(o_done + (i & 1) * 8);
             __syncwarp();
@@ -180,19 +263,21 @@ template <bool CAPPED> __global__ void __launch_bounds__(kThreads, 1) differenti
         float m = -1e30f, l = 0.f, l2 = 0.f;  // below every score, and finite: differences stay numbers
         int halves = 0;                       // of the values, in front of this thread's
         for (int i = 0; i < n; i++) {
-            const int j0 = (kt0 + i) * kKeys, j1 = j0 + part * kPart;
-            const unsigned t_scores = tmem + lanes + (i & 1) * kKeys;
-            if (ok && !mbar_wait(s_full + (i & 1) * 8, (unsigned)(i >> 1) & 1)) ok = false;
+            const int j0 = (kt0 + i) * KEYS, j1 = j0 + part * kPart;
+            if (ok && !mbar_wait(s_full, (unsigned)i & 1)) ok = false;
             after_sync();
             float s[kPart];
 #pragma unroll
             for (int c = 0; c < 2; c++) {
                 unsigned v[32];
-                tmem_ld32(v, t_scores + part * kPart + c * 32);
+                tmem_ld32(v, tmem + lanes + part * kPart + c * 32);
 #pragma unroll
                 for (int e = 0; e < 32; e++) s[c * 32 + e] = __uint_as_float(v[e]);
             }
             tmem_ld_wait();
+            before_sync();
+            __syncwarp();
+            if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(s_free) : "memory");
             if (CAPPED) {
 #pragma unroll
                 for (int e = 0; e < kPart; e++) s[e] = cap2 - __fdividef(2.f * cap2, 1.f + ex2(s[e]));
@@ -209,7 +294,7 @@ template <bool CAPPED> __global__ void __launch_bounds__(kThreads, 1) differenti
                 top2 = fmaxf(top2, fmaxf(s[e + 2], s[e + 3]));
             }
             top = fmaxf(top, top2);
-            top = fmaxf(top, both(i & 1, top));
+            if (kHalves == 2) top = fmaxf(top, both(i & 1, top));
             // Weights are taken against a maximum that may lie up to 2^8 behind: the sums are rarely taken anew, and bf16 holds 2^8 as well as 1. Both warps of a row see the same tops.
             if (__any_sync(0xffffffffu, top > m + kLazy)) {
                 top = fmaxf(top, m);
@@ -231,7 +316,9 @@ template <bool CAPPED> __global__ void __launch_bounds__(kThreads, 1) differenti
                     }
                 }
             }
-            const int before = part == 1 && seen(j0, 0);  // the other half's values come first
+            if (i >= 2 && ok && !added(i - 2)) ok = false;  // these weights' place
+            after_sync();
+            const int before = kHalves == 2 && part == 1 && seen(j0, 0);  // the other half's values come first
             if (seen(j0, part)) {
 #pragma unroll
                 for (int c = 0; c < 2; c++) {
@@ -243,11 +330,11 @@ template <bool CAPPED> __global__ void __launch_bounds__(kThreads, 1) differenti
                         l += __uint_as_float(w[e] << 16);
                         l2 += __uint_as_float(w[e] & 0xFFFF0000u);
                     }
-                    tmem_st16(t_scores + part * (kPart / 2) + c * 16, w);
+                    tmem_st16(tmem + lanes + KEYS + (i & 1) * (KEYS / 2) + part * (kPart / 2) + c * 16, w);
                 }
                 if (j1 + kPart - 1 > last || j1 < low) {  // what lies behind the last key or in front of the first may be no number, which a weight of 0 would not cancel
-                    const int at = halves + before, stage = at % 2;
-                    if (ok && !mbar_wait(v_full + stage * 8, (unsigned)(at / 2) & 1)) ok = false;
+                    const int at = halves + before, stage = at % kStagesV;
+                    if (ok && !mbar_wait(v_full + stage * 8, (unsigned)(at / kStagesV) & 1)) ok = false;
                     for (int u = r; u < kPart * vp * 8; u += kRows) {
                         const int key = u & (kPart - 1), c = u / kPart;
                         const unsigned to = sv + stage * v_stage + (c >> 3) * kPanelV + key * 128 + (c & 7) * 16;
@@ -260,10 +347,10 @@ template <bool CAPPED> __global__ void __launch_bounds__(kThreads, 1) differenti
             before_sync();
             __syncwarp();
             if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(w_full + (i & 1) * 16 + part * 8) : "memory");
-            halves += seen(j0, 0) + seen(j0, 1);
+            halves += seen(j0, 0) + (kHalves == 2 && seen(j0, 1));
         }
         l += l2;
-        l += both(n & 1, l);
+        if (kHalves == 2) l += both(n & 1, l);
         if (ok && !added(n - 1)) ok = false;
         after_sync();
         f = 1.f / l;
@@ -314,7 +401,7 @@ template <bool CAPPED> __global__ void __launch_bounds__(kThreads, 1) differenti
                 *reinterpret_cast<float4*>(row + c + e) = o;
             }
         }
-        ss += both(0, ss);
+        if (kHalves == 2) ss += both(0, ss);
         scales[r & 63] = p.gain ? 1.f / sqrtf(ss / (float)p.vdim + p.head_eps) : 1.f;
     }
     before_sync();
@@ -343,9 +430,13 @@ template <bool CAPPED> __global__ void __launch_bounds__(kThreads, 1) differenti
     if (warp == kIssues) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(cols) : "memory");
 }
 
-// More than half of what an SM has: one CTA at a time.
-int cluster_smem(int kp, int vp) {
-    return std::max(1024 + kp * 2 * (int)(kPanelQ + kPanelK) + vp * 2 * (int)kPanelV + kBarriers * 8 + 16 + 256 + 4 * kRows * 4, 118 * 1024);
+// Two CTAs per SM where their shared and tensor memory allow it.
+int differential_keys(int kp, int vp) { return kp == 1 && vp <= 2 ? 64 : 128; }
+// No more CTAs share an SM than have room in its tensor memory: with 256 columns of 512 at most two (80 KB and more each), with all of them one (118 KB and more).
+int differential_smem(int kp, int vp) {
+    const int keys = differential_keys(kp, vp);
+    const int kv = keys == 64 ? Shape<64>::keys * 64 * 128 * kp + Shape<64>::values * (int)kPanelV * vp : Shape<128>::keys * 128 * 128 * kp + Shape<128>::values * (int)kPanelV * vp;
+    return std::max(1024 + kp * 2 * (int)kPanelQ + kv + kBarriers * 8 + 16 + 256 + 4 * kRows * 4, keys == 64 ? 80 * 1024 : 118 * 1024);
 }
 
 }  // namespace
@@ -361,21 +452,18 @@ void emit_differential_prefill(Emitter& em, const DiffP& kv, const TRef& keys, c
     p.kv = kv;
     p.kp = (kv.dim + 63) / 64;
     p.vp = (kv.vdim + 63) / 64;
-    p.box = std::min(kPart, 1 << kv.shift);
+    p.box = std::min(6, kv.shift);
     p.inv = (65536 + kv.heads / kv.kv_heads - 1) / (kv.heads / kv.kv_heads);
     const int64_t tq = kRows / (kv.heads / kv.kv_heads), rows = (int64_t)kv.n_pages * kv.kv_heads << kv.shift;
-    const dim3 grid((unsigned)((kv.rows + tq - 1) / tq + kv.n_seqs), (unsigned)kv.kv_heads);
-    if (p.kp == 1 && p.vp <= 2) {
-        emit_differential_pair(em, p, grid);
-    } else {
-        void (*const k)(const PreP) = kv.cap2 > 0.f ? differential_prefill<true> : differential_prefill<false>;
-        ensure_max_dynamic_smem((const void*)k, 226 * 1024);
-        em.launch(k, dim3(grid.x, grid.y * 2), dim3(kThreads), (unsigned)cluster_smem(p.kp, p.vp), p, {}, "differential_prefill", /*pdl=*/true).cluster = dim3(1, 2, 1);
-    }
-    LaunchRec& rec = em.recs.back();
+    void (*const k)(const PreP) = differential_keys(p.kp, p.vp) == 64 ? (kv.cap2 > 0.f ? differential_prefill<true, 64> : differential_prefill<false, 64>)
+                                                                     : (kv.cap2 > 0.f ? differential_prefill<true, 128> : differential_prefill<false, 128>);
+    const int smem = differential_smem(p.kp, p.vp);
+    ensure_max_dynamic_smem((const void*)k, 226 * 1024);
+    LaunchRec& rec = em.launch(k, dim3((unsigned)((kv.rows + tq - 1) / tq + kv.n_seqs), (unsigned)kv.kv_heads * 2), dim3(differential_keys(p.kp, p.vp) == 64 ? Shape<64>::threads : Shape<128>::threads), (unsigned)smem, p, {}, "differential_prefill", /*pdl=*/true);
+    rec.cluster = dim3(1, 2, 1);
     for (auto& pr : ptrs) rec.relocs.push_back(Reloc{(uint32_t)(offsetof(PreP, kv) + pr.first), pr.second});
-    rec.tmaps.push_back(TmapReloc{(uint32_t)offsetof(PreP, maps), keys.buf, (uint64_t)kv.dim * 2, (uint64_t)rows, (uint64_t)kv.dim * 4, 64u, (uint32_t)p.box});
-    rec.tmaps.push_back(TmapReloc{(uint32_t)offsetof(PreP, maps) + 128, values.buf, (uint64_t)kv.vdim, (uint64_t)rows, (uint64_t)kv.vdim * 2, 64u, (uint32_t)p.box});
+    rec.tmaps.push_back(TmapReloc{(uint32_t)offsetof(PreP, maps), keys.buf, (uint64_t)kv.dim * 2, (uint64_t)rows, (uint64_t)kv.dim * 4, 64u, 1u << p.box});
+    rec.tmaps.push_back(TmapReloc{(uint32_t)offsetof(PreP, maps) + 128, values.buf, (uint64_t)kv.vdim, (uint64_t)rows, (uint64_t)kv.vdim * 2, 64u, 1u << p.box});
 }
 
 }  // namespace oxk

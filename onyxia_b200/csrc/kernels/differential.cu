@@ -21,13 +21,13 @@ namespace {
 
 // One CTA per row, one warp per query or key of a map.
 template <typename T> __global__ void __launch_bounds__(128) differential_prepare(const DiffP p) {
-    extern __shared__ float angle[];  // cos[half], sin[half]
+    extern __shared__ double angle[];  // cos[half], sin[half]
     pdl_enter();
     const int row = blockIdx.x, s = find_seq(p.seqs, p.n_seqs, row), lane = threadIdx.x & 31;
     const SeqRow sq = load_seq(p.seqs, s);
     const int pos = sq.past + row - sq.start;
     if (row < sq.start || row >= sq.start + sq.len || (sq.len == 1 && !p.singles)) return;
-    quarter_angles(p, pos, angle, angle + p.half, threadIdx.x, 128);
+    exact_angles(p, pos, angle, angle + p.half, threadIdx.x, 128);
     __syncthreads();
     const T* x = (const T*)p.proj + (long long)row * p.ld;
     const long long pg = page_of(p, s, pos);
@@ -40,30 +40,32 @@ template <typename T> __global__ void __launch_bounds__(128) differential_prepar
             if (k < 0 && p.parts) {
                 bf16* to = (bf16*)p.q + ((long long)row * p.heads * 2 + h) * 2 * p.dim;
                 for (int i = lane; i < p.dim; i += 32) {
-                    const float v = rotated(p.half, 0, src, angle, angle + p.half, i) * f * p.mul2;
+                    const float v = (float)turned(p, src, angle, angle + p.half, i) * f * p.mul2;
                     const bf16 high = __float2bfloat16_rn(v);
                     to[i] = high;
                     to[p.dim + i] = low_part(v, high);
                 }
                 continue;
             }
-        for (int i = lane; i < p.dim; i += 32) dst[i] = from_f<T>(rotated(p.half, 0, src, angle, angle + p.half, i) * f);
+        for (int i = lane; i < p.dim; i += 32) dst[i] = from_f<T>((float)(turned(p, src, angle, angle + p.half, i) * f));
     }
     for (int i = threadIdx.x; i < p.kv_heads * p.vdim; i += 128) ((T*)p.values)[key_row(p, pg, i / p.vdim, pos) * p.vdim + i % p.vdim] = x[p.v_off + i];
 }
 
 // The same in bf16 eight elements at a time, where heads, rotated halves and rows allow it: a unit is eight pairs that turn or eight elements that do not.
-__global__ void __launch_bounds__(128) differential_prepare8(const DiffP p) {
-    extern __shared__ float angle[];  // cos[half], sin[half], with norms [2 · (heads + kv_heads)] factors
+__global__ void __launch_bounds__(128, 8) differential_prepare8(const DiffP p) {
+    extern __shared__ double angle[];  // cos[half], sin[half], both again as f32 (for the queries), with norms [2 · (heads + kv_heads)] factors as f32
     pdl_enter();
     const int row = blockIdx.x, s = find_seq(p.seqs, p.n_seqs, row), tid = threadIdx.x;
     const SeqRow sq = load_seq(p.seqs, s);
     const int pos = sq.past + row - sq.start, maps = 2 * (p.heads + p.kv_heads);
     if (row < sq.start || row >= sq.start + sq.len || (sq.len == 1 && !p.singles)) return;
-    quarter_angles(p, pos, angle, angle + p.half, tid, 128);
+    float* short_angle = reinterpret_cast<float*>(angle + 2 * p.half);
+    exact_angles(p, pos, angle, angle + p.half, tid, 128);
+    for (int i = tid; i < p.half; i += 128) short_angle[i] = (float)angle[i], short_angle[p.half + i] = (float)angle[p.half + i];  // (its own)
     const bf16* x = (const bf16*)p.proj + (long long)row * p.ld;
     auto source = [&](int h) { return h < 2 * p.heads ? x + p.q_off + (long long)h * p.dim : x + p.k_off + (long long)(h - 2 * p.heads) * p.dim; };
-    float* factor = angle + 2 * p.half;
+    float* factor = short_angle + 2 * p.half;
     if (p.norm)
         for (int h = tid >> 5; h < maps; h += 4) {
             const float f = map_factor(p, source(h));
@@ -104,12 +106,22 @@ __global__ void __launch_bounds__(128) differential_prepare8(const DiffP p) {
             continue;
         }
         wide(*reinterpret_cast<const uint4*>(src + p.half), b);
-        const float *c = angle + at, *n = c + p.half;
+        if (h < 2 * p.heads) {
+            const float *c = short_angle + at, *n = c + p.half;
 #pragma unroll
-        for (int e = 0; e < 8; e++) o[e] = (a[e] * c[e] - b[e] * n[e]) * f;
+            for (int e = 0; e < 8; e++) o[e] = (a[e] * c[e] - b[e] * n[e]) * f;
+            put(h, at, o);
+#pragma unroll
+            for (int e = 0; e < 8; e++) o[e] = (b[e] * c[e] + a[e] * n[e]) * f;
+            put(h, at + p.half, o);
+            continue;
+        }
+        const double *c = angle + at, *n = c + p.half;
+#pragma unroll
+        for (int e = 0; e < 8; e++) o[e] = (float)(((double)a[e] * c[e] - (double)b[e] * n[e]) * f);
         put(h, at, o);
 #pragma unroll
-        for (int e = 0; e < 8; e++) o[e] = (b[e] * c[e] + a[e] * n[e]) * f;
+        for (int e = 0; e < 8; e++) o[e] = (float)(((double)b[e] * c[e] + (double)a[e] * n[e]) * f);
         put(h, at + p.half, o);
     }
     for (int u = tid; u < p.kv_heads * p.vdim / 8; u += 128)
@@ -182,7 +194,7 @@ template <int DM, int DV> struct DecSmem {
     static constexpr int part = part_size(2 * kDecHeads, DV);      // floats of one partial result, rows [map][8 heads]
     static constexpr int merge = kDecWarps * part * 4;             // reuses the ring after the last key
     static constexpr int angle = kv + (ring > merge ? ring : merge);
-    static constexpr int total = angle + DM * 4;
+    static constexpr int total = angle + DM * 8;
 };
 
 // The difference of the two maps' results, from `n` partial results ([n][map][8 heads][DV + 2]: maximum, sum, accumulator), a warp per head.
@@ -247,7 +259,7 @@ template <int DM, int DV> __global__ void __launch_bounds__(kDecThreads) differe
     const bf16* x = (const bf16*)p.proj + (long long)sq.start * p.ld;
     bf16 *keys = (bf16*)p.keys, *values = (bf16*)p.values;
     const unsigned sm0 = smem_u32(smem);
-    float *cs = reinterpret_cast<float*>(smem + L::angle), *sn = cs + DM / 2;
+    double *cs = reinterpret_cast<double*>(smem + L::angle), *sn = cs + DM / 2;
 
     // keys of this CTA: whole tiles of all four warps, so that a split never cuts a tile
     constexpr int step = kDecKeys * kDecWarps;
@@ -256,7 +268,7 @@ template <int DM, int DV> __global__ void __launch_bounds__(kDecThreads) differe
     const int lo = b0 * step, hi = min(b1 * step, pos + 1), from = max(lo, low);  // pages in front of the window may be anybody's
     const int page0 = from >> p.shift, n_pages = from < hi ? ((hi - 1) >> p.shift) - page0 + 1 : 0;
     for (int i = tid; i < min(n_pages, kDecPages); i += kDecThreads) page_s[i] = (int)page_of(p, seq, (page0 + i) << p.shift);
-    if (sq.len == 1) quarter_angles(p, pos, cs, sn, tid, kDecThreads);
+    if (sq.len == 1) exact_angles(p, pos, cs, sn, tid, kDecThreads);
     __syncthreads();
     auto page_at = [&](int j) {
         const int i = (j >> p.shift) - page0;
@@ -320,7 +332,7 @@ template <int DM, int DV> __global__ void __launch_bounds__(kDecThreads) differe
         if (warp < 2) {
             const bf16* k = x + p.k_off + (g * 2 + warp) * dim;
             const float f = map_factor(p, k);
-            for (int i = lane; i < dim; i += 32) keys[(row * 2 + warp) * dim + i] = __float2bfloat16_rn(rotated(p.half, 0, k, cs, sn, i) * f);
+            for (int i = lane; i < dim; i += 32) keys[(row * 2 + warp) * dim + i] = __float2bfloat16_rn((float)(turned(p, k, cs, sn, i) * f));
         } else if (warp == 2) {
             for (int i = lane; i < vdim; i += 32) values[row * vdim + i] = x[p.v_off + g * vdim + i];
         }
@@ -333,7 +345,7 @@ template <int DM, int DV> __global__ void __launch_bounds__(kDecThreads) differe
         const bf16* q = x + p.q_off + (long long)((live ? h0 + h : h0) * 2 + m) * dim;
         const float f = map_factor(p, q);
         for (int i = lane; i < DM; i += 32) {
-            const float v = live && i < dim ? rotated(p.half, 0, q, cs, sn, i) * f : 0.f;
+            const float v = live && i < dim ? (float)turned(p, q, cs, sn, i) * f : 0.f;
             const bf16 high = __float2bfloat16_rn(v);
             bf16* to = reinterpret_cast<bf16*>(smem + L::q + (2 * m * kDecHeads + h) * L::q_stride) + i;
             to[0] = high;
@@ -530,8 +542,12 @@ void emit_differential(Emitter& em, const DifferentialDesc& d, const TRef& proj,
     };
     if (!p.only) {
         const bool by8 = tc && d.rot_dims % 16 == 0 && p.ld % 8 == 0 && d.q_off % 8 == 0 && d.k_off % 8 == 0 && d.v_off % 8 == 0 && proj.buf.off % 16 == 0 && d.heads <= 4096;
-        if (by8) launch(differential_prepare8, dim3((unsigned)rows), 128, (unsigned)((d.rot_dims + (d.norm ? 2 * (d.heads + d.kv_heads) : 0)) * 4), none, "differential_prepare");
-        else launch(bf ? differential_prepare<bf16> : differential_prepare<float>, dim3((unsigned)rows), 128, (unsigned)(d.rot_dims * 4), none, "differential_prepare");
+        if (by8) launch(differential_prepare8, dim3((unsigned)rows), 128, (unsigned)(d.rot_dims * 12 + (d.norm ? 2 * (d.heads + d.kv_heads) : 0) * 4), none, "differential_prepare");
+        else {
+            const DiffKernel prepare = bf ? differential_prepare<bf16> : differential_prepare<float>;
+            ensure_max_dynamic_smem((const void*)prepare, 8192 * 8);
+            launch(prepare, dim3((unsigned)rows), 128, (unsigned)(d.rot_dims * 8), none, "differential_prepare");
+        }
         if (prefill) {
             emit_differential_prefill(em, p, keys, values,
                                       {{offsetof(DiffP, q), q}, {offsetof(DiffP, out), out.buf}, {offsetof(DiffP, seqs), seqs.buf}, {offsetof(DiffP, table), pages.buf},

@@ -33,17 +33,19 @@ __device__ __forceinline__ float score2(const DiffP& p, float d) {
     const float x = d * p.mul2;
     return p.cap2 > 0.f ? p.cap2 - __fdividef(2.f * p.cap2, 1.f + exp2f(x)) : x;
 }
-// Cosine and sine of every pair at a position, by `threads` threads. Turns are reduced to quarters in 64 bits: what is left of a quarter is small and loses little as f32, so
-// hardly more keys are stored a rounding off than with 64-bit angles (1.6 times as many with whole turns as f32).
-__device__ __forceinline__ void quarter_angles(const DiffP& p, int pos, float* cs, float* sn, int tid, int threads) {
+// Cosine and sine of every pair at a position, by `threads` threads, in 64 bits: a key is stored once and read for as long as its sequence lives, and in 64 bits it is the rounding of its
+// value (with whole turns as f32, 1.6 times as many keys are a rounding off as with f32 products of 64-bit angles).
+__device__ __forceinline__ void exact_angles(const DiffP& p, int pos, double* cs, double* sn, int tid, int threads) {
     for (int i = tid; i < p.half; i += threads) {
-        const double t = (double)pos * ((double)p.turns[i] + (double)p.turns[p.half + i]) * 4.0, whole = rint(t);
-        const int quarter = (int)((long long)whole & 3);
-        float s, c;
-        sincospif(0.5f * (float)(t - whole), &s, &c);
-        cs[i] = quarter == 0 ? c : quarter == 1 ? -s : quarter == 2 ? -c : s;
-        sn[i] = quarter == 0 ? s : quarter == 1 ? c : quarter == 2 ? -s : -c;
+        const double t = (double)pos * ((double)p.turns[i] + (double)p.turns[p.half + i]) * 2.0;
+        sincospi(t - 2.0 * rint(0.5 * t), sn + i, cs + i);
     }
+}
+// Dimension i of a query or key whose leading 2 · half dimensions turn, i with i + half.
+template <typename T> __device__ __forceinline__ double turned(const DiffP& p, const T* x, const double* cs, const double* sn, int i) {
+    const double v = (double)to_f(x[i]);
+    if (i >= 2 * p.half) return v;
+    return i < p.half ? v * cs[i] - (double)to_f(x[i + p.half]) * sn[i] : v * cs[i - p.half] + (double)to_f(x[i - p.half]) * sn[i - p.half];
 }
 // A query as the sum of two bf16. Rounded to one, it alone puts results 2.7e-3 from those of an f32 query (one token, 520 keys, scores of spread 1.5), more than the rounding
 // of the weights (1.1e-3) and of the results (1.7e-3) together.
@@ -57,6 +59,32 @@ template <typename T> __device__ __forceinline__ float map_factor(const DiffP& p
         ss = fmaf(v, v, ss);
     }
     return 1.f / sqrtf(warp_sum(ss) / (float)p.dim + p.eps);
+}
+
+// locate_tile, and the sequence that the tile belongs to: its row of the batch description comes with the count.
+__device__ __forceinline__ bool locate_rows(const int* seqs, int n_seqs, int tile, int tq, int least, int* seq, int* first, SeqRow* row) {
+    const int lane = threadIdx.x & 31;
+    int before = 0;
+    for (int r0 = 0; r0 < n_seqs; r0 += 32) {
+        const SeqRow mine = r0 + lane < n_seqs ? load_seq(seqs, r0 + lane) : SeqRow{0, 0, 0, 0};
+        const int n = mine.len >= least ? (mine.len + tq - 1) / tq : 0;
+        int inc = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, inc, o);
+            if (lane >= o) inc += v;
+        }
+        const unsigned hit = __ballot_sync(0xffffffffu, before + inc > tile);
+        if (hit) {
+            const int at = __ffs(hit) - 1;
+            *seq = r0 + at;
+            *first = (tile - before - (__shfl_sync(0xffffffffu, inc, at) - __shfl_sync(0xffffffffu, n, at))) * tq;
+            *row = SeqRow{__shfl_sync(0xffffffffu, mine.start, at), __shfl_sync(0xffffffffu, mine.len, at), __shfl_sync(0xffffffffu, mine.past, at), 0};
+            return true;
+        }
+        before += __shfl_sync(0xffffffffu, inc, 31);
+    }
+    return false;
 }
 
 // Prompts on tcgen05 (differential_prefill.cu); queries come from `q` [rows, heads, map, high and low part, dim] in units of base 2; `ptrs`: fields of DiffP by their offset.

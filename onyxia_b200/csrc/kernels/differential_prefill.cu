@@ -14,7 +14,7 @@ namespace {
 
 constexpr int kRows = 128, kPart = 64;
 constexpr unsigned kPanelQ = kRows * 128, kPanelV = kPart * 128;  // bytes: rows × 64 dimensions
-constexpr int kBarriers = 20;
+constexpr int kBarriers = 21;
 constexpr float kLazy = 8.f;  // how far (base 2) a row's scores may rise above the maximum that its weights are taken against
 
 struct PreP {
@@ -99,26 +99,26 @@ template <bool CAPPED, int KEYS> __global__ void __launch_bounds__(Shape<KEYS>::
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     const DiffP& p = pp.kv;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, kp = pp.kp, vp = pp.vp, map = blockIdx.y & 1, g = blockIdx.y >> 1;
-    constexpr int kHalves = Shape<KEYS>::halves, kSoft = Shape<KEYS>::soft, kThreads = Shape<KEYS>::threads, kStagesK = Shape<KEYS>::keys, kStagesV = Shape<KEYS>::values;
+    constexpr int kHalves = Shape<KEYS>::halves, kSoft = Shape<KEYS>::soft, kStagesK = Shape<KEYS>::keys, kStagesV = Shape<KEYS>::values;
     constexpr int kCopies = kSoft / 32, kIssues = kCopies + 1;  // warps
     constexpr unsigned kPanelK = KEYS * 128;
     const unsigned k_stage = kp * kPanelK, v_stage = vp * kPanelV;
     const unsigned sq0 = smem_u32(smem), low0 = kp * kPanelQ, sk = sq0 + 2 * low0, sv = sk + kStagesK * k_stage, bars = sv + kStagesV * v_stage;
-    // barriers: keys there, free, values there, free (three each), scores there, read, products added (one, one and two), weights there (two halves of two)
-    const unsigned k_full = bars, k_free = bars + 24, v_full = bars + 48, v_free = bars + 72, s_full = bars + 96, s_free = bars + 104, o_done = bars + 112, w_full = bars + 128;
+    // barriers: keys there, free, values there, free (three each), scores there, read, products added (one, one and two), weights there (two halves of two), queries there
+    const unsigned k_full = bars, k_free = bars + 24, v_full = bars + 48, v_free = bars + 72, s_full = bars + 96, s_free = bars + 104, o_done = bars + 112, w_full = bars + 128, q_full = bars + 160;
     unsigned* tmem_slot = reinterpret_cast<unsigned*>(smem + (bars + kBarriers * 8 - sq0));
-    float* scales = reinterpret_cast<float*>(smem + (bars + kBarriers * 8 + 16 - sq0));  // [64]: what the norms divide by
+    float* scales = reinterpret_cast<float*>(smem + (bars + kBarriers * 8 + 8 - sq0));  // [64]: what the norms divide by
     float* shared = scales + 64;  // [turn][half of the keys][row]: what the two threads of a row tell each other
     if (tid == 0) {
-        for (int i = 0; i < kBarriers; i++) mbar_init(bars + i * 8, i == 13 ? kSoft / 32 : i >= kBarriers - 4 ? kRows / 32 : 1);
+        for (int i = 0; i < kBarriers; i++) mbar_init(bars + i * 8, i == 13 ? kSoft / 32 : i == 20 ? kSoft : i >= 16 ? kRows / 32 : 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     pdl_wait();
     const int rep = p.heads / p.kv_heads, tq = kRows / rep;
     int seq, first;
+    SeqRow sq;
     // long rows first: the last tiles of a sequence see the most keys
-    if (!locate_tile(p.seqs, p.n_seqs, (int)gridDim.x - 1 - (int)blockIdx.x, tq, &seq, &first, p.singles ? 1 : 2)) return;  // both CTAs of the cluster
-    const SeqRow sq = load_seq(p.seqs, seq);
+    if (!locate_rows(p.seqs, p.n_seqs, (int)gridDim.x - 1 - (int)blockIdx.x, tq, p.singles ? 1 : 2, &seq, &first, &sq)) return;  // both CTAs of the cluster
     const int n_tok = min(tq, sq.len - first), pos0 = sq.past + first, last = pos0 + n_tok - 1, low = first_key(p, pos0);
     // Scores in KEYS columns, weights in two turns of half as many, sums behind them. No more CTAs than have room in tensor memory may be on an SM at a time
     // (differential_smem), or two clusters could wait for what the other one has.
@@ -129,20 +129,6 @@ template <bool CAPPED, int KEYS> __global__ void __launch_bounds__(Shape<KEYS>::
     }
     const int inv = pp.inv;
     auto token_of = [&](int row) { return row * inv >> 16; };  // row / rep
-    {
-        const int shift = kp + 2, chunks = 1 << (shift + 1), c = tid & (chunks - 1), part = c >> shift, d = c - (part << shift);  // kp is 1 or 2
-        const bf16* src = (const bf16*)p.q + ((((long long)(sq.start + first) * p.heads + g * rep) * 2 + map) * 2 + part) * p.dim + d * 8;
-        const unsigned to = sq0 + part * low0 + (d >> 3) * kPanelQ;
-#pragma unroll 4
-        for (int r = tid / chunks; r < kRows; r += kThreads / chunks) {
-            const int tok = token_of(r), h = r - tok * rep;
-            const bool live = tok < n_tok && d * 8 < p.dim;
-            cp_async16(to + r * 128 + (((d & 7) ^ (r & 7)) << 4), live ? src + ((long long)tok * p.heads + h) * 4 * p.dim : (const bf16*)p.q, live);
-        }
-    }
-    cp_async_commit();
-    cp_async_wait<0>();
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the tensor core reads them
     before_sync();
     __syncthreads();
     after_sync();
@@ -222,6 +208,7 @@ template <bool CAPPED, int KEYS> __global__ void __launch_bounds__(Shape<KEYS>::
             __syncwarp();
             keys_at.next(kStagesK);
         };
+        if (!mbar_wait(q_full, 0)) ok = false;
         scores(0);
         bool some = false;  // the sums hold something
         for (int i = 0; i < n; i++) {
@@ -246,6 +233,21 @@ template <bool CAPPED, int KEYS> __global__ void __launch_bounds__(Shape<KEYS>::
             if (elect_one() && ok) umma_commit(o_done + (i & 1) * 8);
             __syncwarp();
         }
+    }
+    if (warp < kCopies) {
+        const int shift = kp + 2, chunks = 1 << (shift + 1), c = tid & (chunks - 1), part = c >> shift, d = c - (part << shift);  // kp is 1 or 2
+        const bf16* src = (const bf16*)p.q + ((((long long)(sq.start + first) * p.heads + g * rep) * 2 + map) * 2 + part) * p.dim + d * 8;
+        const unsigned to = sq0 + part * low0 + (d >> 3) * kPanelQ;
+#pragma unroll 8
+        for (int row = tid / chunks; row < kRows; row += kSoft / chunks) {
+            const int t = token_of(row), h = row - t * rep;
+            const bool live = t < n_tok && d * 8 < p.dim;
+            cp_async16(to + row * 128 + (((d & 7) ^ (row & 7)) << 4), live ? src + ((long long)t * p.heads + h) * 4 * p.dim : (const bf16*)p.q, live);
+        }
+        cp_async_commit();
+        cp_async_wait<0>();
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the tensor core reads them
+        asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(q_full) : "memory");
     }
     const int r = tid & (kRows - 1), part = tid / kRows, tok = token_of(r), head = g * rep + r - tok * rep;  // thread `part` of a row has its keys of half `part`
     const unsigned lanes = (unsigned)((warp & 3) * 32) << 16;
@@ -368,7 +370,7 @@ template <bool CAPPED, int KEYS> __global__ void __launch_bounds__(Shape<KEYS>::
     if (warp < kCopies && !keeps) {
         unsigned to;
         asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(mine), "r"(map ^ 1));
-#pragma unroll 1
+#pragma unroll 2
         for (int c = part * 32; c < vp * 64; c += 32 * kHalves) {
             unsigned v[32];
             tmem_ld32(v, t_sum + lanes + c);
@@ -380,12 +382,17 @@ template <bool CAPPED, int KEYS> __global__ void __launch_bounds__(Shape<KEYS>::
                              : "memory");
         }
     }
+    // a row is written by neighbouring lanes, sixteen bytes each
+    const int wide = p.vdim > 128 ? 32 : 16, wc = (tid & (wide - 1)) * 8;
+    float gain[8];
+#pragma unroll
+    for (int e = 0; e < 8; e++) gain[e] = p.gain && wc < p.vdim ? p.gain[wc + e] : 1.f;
     cluster_meet();
     if (warp < kCopies && keeps) {
         float* row = reinterpret_cast<float*>(smem + (mine - sq0));
         const float sign = map ? -1.f : 1.f;
         float ss = 0.f;
-#pragma unroll 1
+#pragma unroll 2
         for (int c = part * 32; c < vp * 64; c += 32 * kHalves) {
             unsigned v[32];
             tmem_ld32(v, t_sum + lanes + c);
@@ -407,25 +414,19 @@ template <bool CAPPED, int KEYS> __global__ void __launch_bounds__(Shape<KEYS>::
     before_sync();
     __syncthreads();
     after_sync();
-    // a row is written by neighbouring lanes, sixteen bytes each
-    const int wide = p.vdim / 8;
-    if (ok)
-        for (int c = tid % 32; c < wide; c += 32) {
-            float gain[8];
-#pragma unroll
-            for (int e = 0; e < 8; e++) gain[e] = p.gain ? p.gain[c * 8 + e] : 1.f;
+    if (warp < kCopies && wc < p.vdim) {
 #pragma unroll 4
-            for (int i = warp; i < 64; i += kThreads / 32) {
-                const int at = map * 64 + i, t = token_of(at);
-                const float* row = reinterpret_cast<const float*>(smem) + i * stride + c * 8;
-                const float4 a = *reinterpret_cast<const float4*>(row), b = *reinterpret_cast<const float4*>(row + 4);
-                const float x = scales[i];
-                if (t < n_tok)
-                    *reinterpret_cast<uint4*>((bf16*)p.out + ((sq.start + first + t) * (long long)p.heads + g * rep + at - t * rep) * p.vdim + c * 8) =
-                        make_uint4(pack_bf16(a.x * x * gain[0], a.y * x * gain[1]), pack_bf16(a.z * x * gain[2], a.w * x * gain[3]), pack_bf16(b.x * x * gain[4], b.y * x * gain[5]),
-                                   pack_bf16(b.z * x * gain[6], b.w * x * gain[7]));
-            }
+        for (int i = tid / wide; i < 64; i += kSoft / wide) {
+            const int at = map * 64 + i, t = token_of(at);
+            const float* row = reinterpret_cast<const float*>(smem) + i * stride + wc;
+            const float4 a = *reinterpret_cast<const float4*>(row), b = *reinterpret_cast<const float4*>(row + 4);
+            const float x = scales[i];
+            if (t < n_tok && ok)
+                *reinterpret_cast<uint4*>((bf16*)p.out + ((sq.start + first + t) * (long long)p.heads + g * rep + at - t * rep) * p.vdim + wc) =
+                    make_uint4(pack_bf16(a.x * x * gain[0], a.y * x * gain[1]), pack_bf16(a.z * x * gain[2], a.w * x * gain[3]), pack_bf16(b.x * x * gain[4], b.y * x * gain[5]),
+                               pack_bf16(b.z * x * gain[6], b.w * x * gain[7]));
         }
+    }
     if (!ok && lane == 0) report(p.err, ERR_WAIT_TIMEOUT, p.node, (long long)blockIdx.x, (long long)warp);
     if (warp == kIssues) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(cols) : "memory");
 }

@@ -24,16 +24,19 @@ class DeviceTensor:
 
     def __init__(self, handle):
         self._h = handle
+        self._described = None
 
     @property
     def handle(self):
         return self._h
 
     def describe(self):
-        dt, rank = C.c_int32(), C.c_int32()
-        shape = (C.c_uint64 * 8)()
-        check(_ffi.cuda_lib().ox_tensor_describe(self._h, C.byref(dt), shape, 8, C.byref(rank)))
-        return dt.value, tuple(shape[i] for i in range(rank.value))
+        if self._described is None:  # a handle's type and shape stay what they are
+            dt, rank = C.c_int32(), C.c_int32()
+            shape = (C.c_uint64 * 8)()
+            check(_ffi.cuda_lib().ox_tensor_describe(self._h, C.byref(dt), shape, 8, C.byref(rank)))
+            self._described = dt.value, tuple(shape[i] for i in range(rank.value))
+        return self._described
 
     @property
     def dtype(self) -> int:
@@ -116,7 +119,7 @@ class CudaSession:
         n = len(items)
         names = (C.c_char_p * max(n, 1))(*[k.encode() for k, _ in items])
         handles = (C.c_void_p * max(n, 1))(*[t.handle for _, t in items])
-        cap = 4096
+        cap = max(self._lib.ox_session_num_outputs(self._h), 1)
         out_names = (C.c_char_p * cap)()
         out_tensors = (C.c_void_p * cap)()
         n_out = C.c_int32()

@@ -194,7 +194,8 @@ template <int DM, int DV> struct DecSmem {
     static constexpr int part = part_size(2 * kDecHeads, DV);      // floats of one partial result, rows [map][8 heads]
     static constexpr int merge = kDecWarps * part * 4;             // reuses the ring after the last key
     static constexpr int angle = kv + (ring > merge ? ring : merge);
-    static constexpr int total = angle + DM * 8;
+    static constexpr int raw = angle + DM * 12;                    // the token's queries of 8 heads, then its two keys, as they come
+    static constexpr int total = raw + 18 * DM * 2;
 };
 
 // The difference of the two maps' results, from `n` partial results ([n][map][8 heads][DV + 2]: maximum, sum, accumulator), a warp per head.
@@ -268,7 +269,11 @@ template <int DM, int DV> __global__ void __launch_bounds__(kDecThreads) differe
     const int lo = b0 * step, hi = min(b1 * step, pos + 1), from = max(lo, low);  // pages in front of the window may be anybody's
     const int page0 = from >> p.shift, n_pages = from < hi ? ((hi - 1) >> p.shift) - page0 + 1 : 0;
     for (int i = tid; i < min(n_pages, kDecPages); i += kDecThreads) page_s[i] = (int)page_of(p, seq, (page0 + i) << p.shift);
-    if (sq.len == 1) exact_angles(p, pos, cs, sn, tid, kDecThreads);
+    float *short_cs = reinterpret_cast<float*>(sn + DM / 2), *short_sn = short_cs + DM / 2;
+    if (sq.len == 1) {
+        exact_angles(p, pos, cs, sn, tid, kDecThreads);
+        for (int i = tid; i < p.half; i += kDecThreads) short_cs[i] = (float)cs[i], short_sn[i] = (float)sn[i];  // (its own)
+    }
     __syncthreads();
     auto page_at = [&](int j) {
         const int i = (j >> p.shift) - page0;
@@ -326,30 +331,48 @@ template <int DM, int DV> __global__ void __launch_bounds__(kDecThreads) differe
         if (p.only && sq.len > 1 && tid == 0) report(p.err, ERR_BATCH_ROWS, p.node, seq, sq.len);
         return;
     }
+    // all that comes from the projection at once
+    bf16* raw = reinterpret_cast<bf16*>(smem + L::raw);
+    const int q_rows = 2 * n_heads, raw_rows = q_rows + (newest ? 2 : 0);
+    const long long row = newest ? key_row(p, page_at(pos), g, pos) : 0;
+    auto source = [&](int r) { return r < q_rows ? x + p.q_off + (long long)(h0 * 2 + r) * dim : x + p.k_off + (long long)(g * 2 + r - q_rows) * dim; };
+    if (p.by8) {
+        const int chunks = dim / 8;
+        for (int u = tid; u < raw_rows * chunks; u += kDecThreads) {
+            const int r = u / chunks, c = u - r * chunks;
+            reinterpret_cast<uint4*>(raw)[r * (DM / 8) + c] = reinterpret_cast<const uint4*>(source(r))[c];
+        }
+        if (newest)
+            for (int u = tid; u < vdim / 8; u += kDecThreads) reinterpret_cast<uint4*>(values + row * vdim)[u] = reinterpret_cast<const uint4*>(x + p.v_off + (long long)g * vdim)[u];
+    } else {
+        for (int r = warp; r < raw_rows; r += kDecWarps)
+            for (int i = lane; i < dim; i += 32) raw[r * DM + i] = source(r)[i];
+        if (newest)
+            for (int i = tid; i < vdim; i += kDecThreads) values[row * vdim + i] = x[p.v_off + (long long)g * vdim + i];
+    }
+    __syncthreads();
     if (newest) {
         // (where a key head has several groups of queries, each CTA that needs the new key writes it: the same bits)
-        const long long row = key_row(p, page_at(pos), g, pos);
         if (warp < 2) {
-            const bf16* k = x + p.k_off + (g * 2 + warp) * dim;
+            const bf16* k = raw + (q_rows + warp) * DM;
             const float f = map_factor(p, k);
             for (int i = lane; i < dim; i += 32) keys[(row * 2 + warp) * dim + i] = __float2bfloat16_rn((float)(turned(p, k, cs, sn, i) * f));
-        } else if (warp == 2) {
-            for (int i = lane; i < vdim; i += 32) values[row * vdim + i] = x[p.v_off + g * vdim + i];
         }
         __syncthreads();
         fill();
     }
     for (int r = warp; r < 2 * kDecHeads; r += kDecWarps) {
-        const int m = r / kDecHeads, h = r % kDecHeads;
+        const int m = r & 1, h = r >> 1;
         const bool live = h < n_heads;
-        const bf16* q = x + p.q_off + (long long)((live ? h0 + h : h0) * 2 + m) * dim;
+        const bf16* q = raw + (live ? r : 0) * DM;
         const float f = map_factor(p, q);
+        bf16* to = reinterpret_cast<bf16*>(smem + L::q + (2 * m * kDecHeads + h) * L::q_stride);
+#pragma unroll
         for (int i = lane; i < DM; i += 32) {
-            const float v = live && i < dim ? (float)turned(p, q, cs, sn, i) * f : 0.f;
+            const float v = live && i < dim ? rotated(p.half, 0, q, short_cs, short_sn, i) * f : 0.f;
             const bf16 high = __float2bfloat16_rn(v);
-            bf16* to = reinterpret_cast<bf16*>(smem + L::q + (2 * m * kDecHeads + h) * L::q_stride) + i;
-            to[0] = high;
-            to[kDecHeads * L::q_stride / 2] = low_part(v, high);
+            to[i] = high;
+            to[kDecHeads * L::q_stride / 2 + i] = low_part(v, high);
         }
     }
     __syncthreads();
@@ -533,6 +556,7 @@ void emit_differential(Emitter& em, const DifferentialDesc& d, const TRef& proj,
     p.singles = !tc || (!p.only && n_seqs == 1);       // a lone token with rows of nobody behind it
     const bool prefill = tc && !p.only && differential_prefill_fits(p, keys, values, out.buf.off);
     p.parts = prefill;
+    p.by8 = p.ld % 8 == 0 && d.q_off % 8 == 0 && d.k_off % 8 == 0 && d.v_off % 8 == 0 && proj.buf.off % 16 == 0;
     const Buf none{kSlotNull, 0}, q = p.only ? none : em.scratch((size_t)rows * d.heads * 2 * d.dim * (bf && !prefill ? 2 : 4));
     auto launch = [&](DiffKernel k, dim3 grid, unsigned block, unsigned smem, Buf part, const char* label) {
         em.launch(k, grid, dim3(block), smem, p,
@@ -541,8 +565,7 @@ void emit_differential(Emitter& em, const DifferentialDesc& d, const TRef& proj,
                   label, /*pdl=*/true);
     };
     if (!p.only) {
-        const bool by8 = tc && d.rot_dims % 16 == 0 && p.ld % 8 == 0 && d.q_off % 8 == 0 && d.k_off % 8 == 0 && d.v_off % 8 == 0 && proj.buf.off % 16 == 0 && d.heads <= 4096;
-        if (by8) launch(differential_prepare8, dim3((unsigned)rows), 128, (unsigned)(d.rot_dims * 12 + (d.norm ? 2 * (d.heads + d.kv_heads) : 0) * 4), none, "differential_prepare");
+        if (tc && p.by8 && d.rot_dims % 16 == 0 && d.heads <= 4096) launch(differential_prepare8, dim3((unsigned)rows), 128, (unsigned)(d.rot_dims * 12 + (d.norm ? 2 * (d.heads + d.kv_heads) : 0) * 4), none, "differential_prepare");
         else {
             const DiffKernel prepare = bf ? differential_prepare<bf16> : differential_prepare<float>;
             ensure_max_dynamic_smem((const void*)prepare, 8192 * 8);

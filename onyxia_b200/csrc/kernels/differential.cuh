@@ -24,6 +24,7 @@ struct DiffP {
     int norm, sink;
     int singles;                 // sequences with one new token are for these kernels too
     int parts;                   // prepare: queries in two parts, times mul2
+    int by8;                     // the parts of a projection row begin on 16 bytes
     int only;                    // no sequence may have more than one
 };
 

@@ -203,30 +203,31 @@ template <int DV> __device__ void merge_maps(const DiffP& p, const float* part, 
     constexpr int size = part_size(2 * kDecHeads, DV), C = (DV + 31) / 32;
     const int lane = threadIdx.x & 31;
     for (int r = threadIdx.x >> 5; r < heads; r += kDecWarps) {
-        float o[C] = {};
+        float o[C] = {}, f0[2], f1[2];
+        const float* head[2] = {part + r * (DV + 2), part + (kDecHeads + r) * (DV + 2)};
 #pragma unroll
         for (int m = 0; m < 2; m++) {
             // lane i weighs parts i and i + 32 (n ≤ 64); a part that saw no key has the maximum kNoScore, sum and values 0
-            const float* head = part + (m * kDecHeads + r) * (DV + 2);
             float pm[2], pl[2];
 #pragma unroll
             for (int k = 0; k < 2; k++) {
                 const bool in = k * 32 + lane < n;
-                pm[k] = in ? head[(long long)(k * 32 + lane) * size] : kNoScore;
-                pl[k] = in ? head[(long long)(k * 32 + lane) * size + 1] : 0.f;
+                pm[k] = in ? head[m][(long long)(k * 32 + lane) * size] : kNoScore;
+                pl[k] = in ? head[m][(long long)(k * 32 + lane) * size + 1] : 0.f;
             }
             float top = warp_max(fmaxf(pm[0], pm[1]));
             if (p.sink) top = fmaxf(top, 0.f);
-            const float f0 = exp2f(pm[0] - top), f1 = exp2f(pm[1] - top);
-            const float l = warp_sum(fmaf(pl[0], f0, pl[1] * f1)) + (p.sink ? exp2f(-top) : 0.f);
+            f0[m] = exp2f(pm[0] - top), f1[m] = exp2f(pm[1] - top);
+            const float l = warp_sum(fmaf(pl[0], f0[m], pl[1] * f1[m])) + (p.sink ? exp2f(-top) : 0.f);
             const float f = m ? -p.lambda[h0 + r] / l : 1.f / l;
+            f0[m] *= f, f1[m] *= f;
+        }
 #pragma unroll 4
-            for (int i = 0; i < n; i++) {
-                const float w = f * __shfl_sync(0xffffffffu, i < 32 ? f0 : f1, i & 31);
+        for (int i = 0; i < n; i++) {
+            const float w0 = __shfl_sync(0xffffffffu, i < 32 ? f0[0] : f1[0], i & 31), w1 = __shfl_sync(0xffffffffu, i < 32 ? f0[1] : f1[1], i & 31);
 #pragma unroll
-                for (int c = 0; c < C; c++)
-                    if (c * 32 + lane < DV) o[c] = fmaf(head[(long long)i * size + 2 + c * 32 + lane], w, o[c]);
-            }
+            for (int c = 0; c < C; c++)
+                if (c * 32 + lane < DV) o[c] = fmaf(head[1][(long long)i * size + 2 + c * 32 + lane], w1, fmaf(head[0][(long long)i * size + 2 + c * 32 + lane], w0, o[c]));
         }
         float f = 1.f;
         if (p.gain) {
@@ -269,11 +270,10 @@ template <int DM, int DV> __global__ void __launch_bounds__(kDecThreads) differe
     const int lo = b0 * step, hi = min(b1 * step, pos + 1), from = max(lo, low);  // pages in front of the window may be anybody's
     const int page0 = from >> p.shift, n_pages = from < hi ? ((hi - 1) >> p.shift) - page0 + 1 : 0;
     for (int i = tid; i < min(n_pages, kDecPages); i += kDecThreads) page_s[i] = (int)page_of(p, seq, (page0 + i) << p.shift);
+    const bool newest = hi == pos + 1 && lo < hi;  // this CTA's keys include the new one
     float *short_cs = reinterpret_cast<float*>(sn + DM / 2), *short_sn = short_cs + DM / 2;
-    if (sq.len == 1) {
-        exact_angles(p, pos, cs, sn, tid, kDecThreads);
-        for (int i = tid; i < p.half; i += kDecThreads) short_cs[i] = (float)cs[i], short_sn[i] = (float)sn[i];  // (its own)
-    }
+    if (sq.len == 1 && warp < 2) short_angles(p, pos, short_cs, short_sn, tid, 64);
+    if (newest && warp >= 2) exact_angles(p, pos, cs, sn, tid - 64, 64);
     __syncthreads();
     auto page_at = [&](int j) {
         const int i = (j >> p.shift) - page0;
@@ -320,7 +320,6 @@ template <int DM, int DV> __global__ void __launch_bounds__(kDecThreads) differe
         }
         cp_async_commit();
     };
-    const bool newest = hi == pos + 1 && lo < hi;  // this CTA's keys include the new one
     auto fill = [&]() {
 #pragma unroll
         for (int i = 0; i < L::stages - 1; i++) load_tile(i);
@@ -353,27 +352,31 @@ template <int DM, int DV> __global__ void __launch_bounds__(kDecThreads) differe
     __syncthreads();
     if (newest) {
         // (where a key head has several groups of queries, each CTA that needs the new key writes it: the same bits)
-        if (warp < 2) {
-            const bf16* k = raw + (q_rows + warp) * DM;
-            const float f = map_factor(p, k);
-            for (int i = lane; i < dim; i += 32) keys[(row * 2 + warp) * dim + i] = __float2bfloat16_rn((float)(turned(p, k, cs, sn, i) * f));
-        }
+        const int m = warp >> 1;  // two warps per map
+        const bf16* k = raw + (q_rows + m) * DM;
+        const float f = map_factor(p, k);
+        for (int i = lane + (warp & 1) * 32; i < dim; i += 64) keys[(row * 2 + m) * dim + i] = __float2bfloat16_rn((float)(turned(p, k, cs, sn, i) * f));
         __syncthreads();
         fill();
     }
-    for (int r = warp; r < 2 * kDecHeads; r += kDecWarps) {
-        const int m = r & 1, h = r >> 1;
+    auto put = [&](bf16* to, int i, float v) {
+        const bf16 high = __float2bfloat16_rn(v);
+        to[i] = high;
+        to[kDecHeads * L::q_stride / 2 + i] = low_part(v, high);
+    };
+#pragma unroll
+    for (int k = 0; k < 2 * kDecHeads / kDecWarps; k++) {
+        const int r = k * kDecWarps + warp, m = r & 1, h = r >> 1;
         const bool live = h < n_heads;
         const bf16* q = raw + (live ? r : 0) * DM;
-        const float f = map_factor(p, q);
+        const float f = live ? map_factor(p, q) : 0.f;
         bf16* to = reinterpret_cast<bf16*>(smem + L::q + (2 * m * kDecHeads + h) * L::q_stride);
-#pragma unroll
-        for (int i = lane; i < DM; i += 32) {
-            const float v = live && i < dim ? rotated(p.half, 0, q, short_cs, short_sn, i) * f : 0.f;
-            const bf16 high = __float2bfloat16_rn(v);
-            to[i] = high;
-            to[kDecHeads * L::q_stride / 2 + i] = low_part(v, high);
+        for (int i = lane; i < p.half; i += 32) {
+            const float a = to_f(q[i]), b = to_f(q[i + p.half]), c = short_cs[i], n = short_sn[i];
+            put(to, i, live ? (a * c - b * n) * f : 0.f);
+            put(to, i + p.half, live ? (b * c + a * n) * f : 0.f);
         }
+        for (int i = 2 * p.half + lane; i < DM; i += 32) put(to, i, live && i < dim ? to_f(q[i]) * f : 0.f);
     }
     __syncthreads();
 
@@ -497,7 +500,8 @@ template <int DM, int DV> __global__ void __launch_bounds__(kDecThreads) differe
         return;
     }
     const long long cell = (long long)blockIdx.z * gridDim.y + blockIdx.y;
-    merge_parts<DV, 2 * kDecHeads, kDecWarps>(parts, kDecWarps, 2 * kDecHeads, vdim, 0.f, nullptr, p.part + (cell * p.splits + blockIdx.x) * L::part);
+    for (int m = 0; m < 2; m++)
+        merge_parts<DV, 2 * kDecHeads, kDecWarps>(parts + m * kDecHeads * (DV + 2), kDecWarps, n_heads, vdim, 0.f, nullptr, p.part + (cell * p.splits + blockIdx.x) * L::part + m * kDecHeads * (DV + 2));
     __threadfence();
     __syncthreads();
     if (tid == 0) arrived = atomicAdd(&p.counters[cell], 1u);

@@ -42,6 +42,17 @@ __device__ __forceinline__ void exact_angles(const DiffP& p, int pos, double* cs
         sincospi(t - 2.0 * rint(0.5 * t), sn + i, cs + i);
     }
 }
+// The same in 32 bits for queries, whose low part ends at 2^-18. Turns are reduced to quarters in 64 bits: what is left is small and loses little as f32.
+__device__ __forceinline__ void short_angles(const DiffP& p, int pos, float* cs, float* sn, int tid, int threads) {
+    for (int i = tid; i < p.half; i += threads) {
+        const double t = (double)pos * ((double)p.turns[i] + (double)p.turns[p.half + i]) * 4.0, whole = rint(t);
+        const int quarter = (int)((long long)whole & 3);
+        float s, c;
+        sincospif(0.5f * (float)(t - whole), &s, &c);
+        cs[i] = quarter == 0 ? c : quarter == 1 ? -s : quarter == 2 ? -c : s;
+        sn[i] = quarter == 0 ? s : quarter == 1 ? c : quarter == 2 ? -s : -c;
+    }
+}
 // Dimension i of a query or key whose leading 2 · half dimensions turn, i with i + half.
 template <typename T> __device__ __forceinline__ double turned(const DiffP& p, const T* x, const double* cs, const double* sn, int i) {
     const double v = (double)to_f(x[i]);

@@ -92,6 +92,7 @@ class CudaSession:
     def __init__(self, handle):
         self._h = handle
         self._lib = _ffi.cuda_lib()
+        self._num_outputs = max(self._lib.ox_session_num_outputs(handle), 1)
 
     def upload(self, t: HostTensor) -> DeviceTensor:
         shape = (C.c_uint64 * max(len(t.shape), 1))(*t.shape)
@@ -116,13 +117,10 @@ class CudaSession:
     def run(self, inputs) -> list:
         """inputs: dict or sequence of (name, DeviceTensor) → [(name, DeviceTensor)] in signature order."""
         items = list(inputs.items()) if isinstance(inputs, dict) else list(inputs)
-        n = len(items)
+        n, cap = len(items), self._num_outputs
         names = (C.c_char_p * max(n, 1))(*[k.encode() for k, _ in items])
-        handles = (C.c_void_p * max(n, 1))(*[t.handle for _, t in items])
-        cap = max(self._lib.ox_session_num_outputs(self._h), 1)
-        out_names = (C.c_char_p * cap)()
-        out_tensors = (C.c_void_p * cap)()
-        n_out = C.c_int32()
+        handles = (C.c_void_p * max(n, 1))(*[t._h for _, t in items])
+        out_names, out_tensors, n_out = (C.c_char_p * cap)(), (C.c_void_p * cap)(), C.c_int32()
         check(self._lib.ox_session_run(self._h, names, handles, n, out_names, out_tensors, cap, C.byref(n_out)))
         return [(out_names[i].decode(), DeviceTensor(C.c_void_p(out_tensors[i]))) for i in range(n_out.value)]
 

@@ -222,7 +222,7 @@ template <int DV> __device__ void merge_maps(const DiffP& p, const float* part, 
             const float f = m ? -p.lambda[h0 + r] / l : 1.f / l;
             f0[m] *= f, f1[m] *= f;
         }
-#pragma unroll 4
+#pragma unroll(DV <= 128 ? 8 : 4)
         for (int i = 0; i < n; i++) {
             const float w0 = __shfl_sync(0xffffffffu, i < 32 ? f0[0] : f1[0], i & 31), w1 = __shfl_sync(0xffffffffu, i < 32 ? f0[1] : f1[1], i & 31);
 #pragma unroll
@@ -285,41 +285,43 @@ template <int DM, int DV> __global__ void __launch_bounds__(kDecThreads) differe
         const int j0 = first + i * step;
         if (i < tiles) {
             const unsigned dst = ring + (i % L::stages) * L::tile;
-            const bool inside = j0 >= from && j0 + kDecKeys <= hi, whole = (1 << p.shift) >= kDecKeys;  // a tile lies in one page
+            const bool whole = (1 << p.shift) >= kDecKeys;  // a tile lies in one page
             const long long row0 = whole && j0 + kDecKeys > from ? key_row(p, page_at(max(j0, from)), g, j0) : 0;
-            constexpr int k_ch = DM / 8, v_ch = DV / 8;
-            if (whole && inside && dim == DM && vdim == DV) {  // contiguous runs: a lane's copies are evenly spaced
+            constexpr int k_ch = DM / 4, v_ch = DV / 8;  // 16-byte pieces of a key and of a value
+            if (whole && dim == DM && vdim == DV) {      // contiguous runs: a lane's copies are evenly spaced
                 const bf16 *k = keys + row0 * 2 * DM + lane * 8, *v = values + row0 * DV + lane * 8;
 #pragma unroll
-                for (int c = 0; c < kDecKeys * 2 * k_ch / 32; c++) {
-                    const int at = c * 32 + lane;
-                    cp_async16(dst + at / (2 * k_ch) * L::k_stride + at % (2 * k_ch) * 16, k + c * 256);
+                for (int c = 0; c < kDecKeys * k_ch / 32; c++) {
+                    const int at = c * 32 + lane, j = j0 + at / k_ch;
+                    const bool live = j >= from && j < hi;
+                    cp_async16(dst + at / k_ch * L::k_stride + at % k_ch * 16, live ? k + c * 256 : keys, live);
                 }
 #pragma unroll
                 for (int c = 0; c < kDecKeys * v_ch / 32; c++) {
-                    const int at = c * 32 + lane;
-                    cp_async16(dst + kDecKeys * L::k_stride + at / v_ch * L::v_stride + at % v_ch * 16, v + c * 256);
+                    const int at = c * 32 + lane, j = j0 + at / v_ch;
+                    const bool live = j >= from && j < hi;
+                    cp_async16(dst + kDecKeys * L::k_stride + at / v_ch * L::v_stride + at % v_ch * 16, live ? v + c * 256 : values, live);
                 }
-                cp_async_commit();
-                return;
-            }
-            for (int c = lane; c < kDecKeys * (2 * k_ch + v_ch); c += 32) {
-                const int key = c / (2 * k_ch + v_ch), ch = c % (2 * k_ch + v_ch), j = j0 + key;
-                const bool in = j >= from && j < hi;
-                const long long row = !in ? 0 : whole ? row0 + key : key_row(p, page_at(j), g, j);
-                if (ch < 2 * k_ch) {
-                    const int m = ch / k_ch, d = ch % k_ch * 8;
-                    const bool live = in && d < dim;
-                    cp_async16(dst + key * L::k_stride + ch * 16, live ? keys + (row * 2 + m) * dim + d : keys, live);
-                } else {
-                    const int d = (ch - 2 * k_ch) * 8;
-                    const bool live = in && d < vdim;
-                    cp_async16(dst + kDecKeys * L::k_stride + key * L::v_stride + d * 2, live ? values + row * vdim + d : values, live);
+            } else {  // key by key, a lane per piece (what is padding was cleared before)
+                const int pieces = dim / 8;
+                const bool has_k = lane < 2 * pieces, has_v = lane < vdim / 8;
+                const unsigned k_to = dst + lane * 16 + (lane >= pieces ? DM * 2 - dim * 2 : 0), v_to = dst + kDecKeys * L::k_stride + lane * 16;
+#pragma unroll 4
+                for (int key = 0; key < kDecKeys; key++) {
+                    const int j = j0 + key;
+                    const bool live = j >= from && j < hi;
+                    const long long row = !live ? 0 : whole ? row0 + key : key_row(p, page_at(j), g, j);
+                    if (has_k) cp_async16(k_to + key * L::k_stride, live ? keys + row * 2 * dim + lane * 8 : keys, live);
+                    if (has_v) cp_async16(v_to + key * L::v_stride, live ? values + row * vdim + lane * 8 : values, live);
                 }
             }
         }
         cp_async_commit();
     };
+    if (dim != DM || vdim != DV) {  // what is padding stays 0
+        for (int u = tid; u < kDecWarps * L::stages * L::tile / 16; u += kDecThreads) reinterpret_cast<uint4*>(smem + L::kv)[u] = make_uint4(0, 0, 0, 0);
+        __syncthreads();
+    }
     auto fill = [&]() {
 #pragma unroll
         for (int i = 0; i < L::stages - 1; i++) load_tile(i);

@@ -426,6 +426,12 @@ ox_status ox_engine_submit(ox_engine*, const int64_t* prompt, int32_t n_prompt, 
                            int64_t top_k, float top_p, uint64_t seed, int64_t* request);
 ox_status ox_engine_step(ox_engine*, int32_t token_budget, ox_engine_token* tokens, int32_t cap, int32_t* n_tokens);
 ox_status ox_engine_cancel(ox_engine*, int64_t request);
+/* Rules on the tokens that an unfinished request has still to generate, as ox_session_constrain_last applies them: its history is its prompt
+ * and what it has generated. Each call replaces what the one before it said. `allowed` has a bit per token of the vocabulary
+ * (ceil(vocab / 32) words, lowest bit first), at least one of them set; NULL allows all again. A grammar sets it before every step. */
+ox_status ox_engine_constrain(ox_engine*, int64_t request, float repetition, float frequency, float presence, const int32_t* bias_ids,
+                              const float* bias, int32_t n_bias);
+ox_status ox_engine_allow(ox_engine*, int64_t request, const uint32_t* allowed, size_t n_words);
 /* out: page size, free pages, free slots, live sequences, waiting requests, running requests, vocabulary size. */
 void ox_engine_stats(const ox_engine*, int64_t out[7]);
 

@@ -161,6 +161,8 @@ SIGNATURES = {
     "ox_engine_submit": (C.c_int32, [_P, C.POINTER(C.c_int64), C.c_int32, C.c_int32, C.c_int64, C.c_float, C.c_int64,
                                      C.c_float, C.c_uint64, C.POINTER(C.c_int64)]),
     "ox_engine_step": (C.c_int32, [_P, C.c_int32, C.POINTER(EngineToken), C.c_int32, _i32p]),
+    "ox_engine_constrain": (C.c_int32, [_P, C.c_int64, C.c_float, C.c_float, C.c_float, _i32p, C.POINTER(C.c_float), C.c_int32]),
+    "ox_engine_allow": (C.c_int32, [_P, C.c_int64, C.POINTER(C.c_uint32), C.c_size_t]),
     "ox_engine_cancel": (C.c_int32, [_P, C.c_int64]),
     "ox_engine_stats": (None, [_P, C.POINTER(C.c_int64)]),
     "ox_tp_unique_id": (C.c_int32, [C.c_char_p, C.POINTER(C.c_uint8)]),

@@ -2,6 +2,7 @@
 #include "engine.hpp"
 
 #include <algorithm>
+#include <cmath>
 #include <cstring>
 
 #include "../ir/module_api.hpp"
@@ -205,7 +206,85 @@ void Engine::cancel(int64_t request) {
         }
 }
 
-std::vector<int64_t> Engine::sample(const DTensor& logits, const std::vector<Request*>& rows) {
+Engine::Request& Engine::request_of(int64_t id) {
+    for (auto& r : waiting_)
+        if (r.id == id) return r;
+    for (auto& r : running_)
+        if (r.id == id) return r;
+    fail(ErrKind::Binding, "no unfinished request " + std::to_string(id));
+}
+
+void Engine::constrain(int64_t request, float repetition, float frequency, float presence, std::vector<int32_t> bias_ids, std::vector<float> bias) {
+    Request& r = request_of(request);
+    if (!(repetition > 0.f) || !std::isfinite(repetition)) fail(ErrKind::Attribute, "a repetition penalty is a factor above 0");
+    if (!std::isfinite(frequency) || !std::isfinite(presence)) fail(ErrKind::Attribute, "penalties must be finite");
+    if (bias_ids.size() != bias.size() || (int64_t)bias.size() > kMaxBiases) fail(ErrKind::Shape, "at most " + std::to_string(kMaxBiases) + " biases of a request");
+    for (size_t i = 0; i < bias.size(); i++) {
+        if (bias_ids[i] < 0 || bias_ids[i] >= vocab_) fail(ErrKind::Shape, "a bias of token " + std::to_string(bias_ids[i]) + ", which is not one of " + std::to_string(vocab_));
+        if (std::isnan(bias[i]) || bias[i] == INFINITY) fail(ErrKind::Attribute, "a bias is a number, or minus infinity");
+    }
+    r.rules.repetition = repetition, r.rules.frequency = frequency, r.rules.presence = presence;
+    r.rules.bias_ids = std::move(bias_ids), r.rules.bias = std::move(bias);
+}
+
+void Engine::allow(int64_t request, std::vector<uint32_t> allowed) {
+    Request& r = request_of(request);
+    if (!allowed.empty()) {
+        if ((int64_t)allowed.size() != (vocab_ + 31) / 32) fail(ErrKind::Shape, "a mask has a bit for each of " + std::to_string(vocab_) + " tokens");
+        if (vocab_ % 32) allowed.back() &= (1u << (vocab_ % 32)) - 1;
+        if (std::all_of(allowed.begin(), allowed.end(), [](uint32_t w) { return w == 0; })) fail(ErrKind::Shape, "the mask allows no token");
+    }
+    r.rules.allowed = std::move(allowed);
+}
+
+// The rows' logits under their requests' rules; those of a batch without any are left alone.
+DTensor Engine::constrained(const DTensor& logits, const std::vector<Request*>& rows) {
+    const size_t n = rows.size(), words = (size_t)(vocab_ + 31) / 32;
+    size_t longest = 0, biases = 0, masks = 0;
+    bool any = false;
+    for (const Request* r : rows) {
+        any = any || r->rules.any();
+        if (r->rules.history()) longest = std::max(longest, r->prompt.size() + r->answer.size());
+        biases = std::max(biases, r->rules.bias.size());
+        masks += !r->rules.allowed.empty();
+    }
+    if (!any) return logits;
+    std::vector<int32_t> history(n * longest), lengths(n * 2), bias_ids(n * biases, -1), mask_of(n, -1);
+    std::vector<float> penalties(n * 3), bias(n * biases);
+    std::vector<uint32_t> allowed;
+    allowed.reserve(masks * words);
+    for (size_t i = 0; i < n; i++) {
+        const Request& r = *rows[i];
+        if (r.rules.history()) {
+            lengths[2 * i] = (int32_t)r.prompt.size(), lengths[2 * i + 1] = (int32_t)(r.prompt.size() + r.answer.size());
+            auto at = history.begin() + (long)(i * longest);
+            std::transform(r.answer.begin(), r.answer.end(), std::transform(r.prompt.begin(), r.prompt.end(), at, [](int64_t t) { return (int32_t)t; }), [](int64_t t) { return (int32_t)t; });
+        }
+        penalties[3 * i] = r.rules.repetition, penalties[3 * i + 1] = r.rules.frequency, penalties[3 * i + 2] = r.rules.presence;
+        std::copy(r.rules.bias_ids.begin(), r.rules.bias_ids.end(), bias_ids.begin() + (long)(i * biases));
+        std::copy(r.rules.bias.begin(), r.rules.bias.end(), bias.begin() + (long)(i * biases));
+        if (!r.rules.allowed.empty()) {
+            mask_of[i] = (int32_t)(allowed.size() / words);
+            allowed.insert(allowed.end(), r.rules.allowed.begin(), r.rules.allowed.end());
+        }
+    }
+    const int64_t N = (int64_t)n;
+    const std::vector<DTensor> t = s_.upload_together({{DType::I32, {N, (int64_t)longest}, history.data(), history.size() * 4},
+                                                       {DType::I32, {N, 2}, lengths.data(), lengths.size() * 4},
+                                                       {DType::F32, {N, 3}, penalties.data(), penalties.size() * 4},
+                                                       {DType::I32, {N, (int64_t)biases}, bias_ids.data(), bias_ids.size() * 4},
+                                                       {DType::F32, {N, (int64_t)biases}, bias.data(), bias.size() * 4},
+                                                       {DType::U32, {(int64_t)masks, (int64_t)words}, allowed.data(), allowed.size() * 4},
+                                                       {DType::I32, {N}, mask_of.data(), mask_of.size() * 4}});
+    oxrt::Rules rules;
+    if (longest) rules.history = &t[0], rules.lengths = &t[1], rules.penalties = &t[2];
+    if (biases) rules.bias_ids = &t[3], rules.bias = &t[4];
+    if (masks) rules.masks = &t[5], rules.mask_of = &t[6];
+    return s_.constrain_last(logits, rules);
+}
+
+std::vector<int64_t> Engine::sample(const DTensor& unconstrained, const std::vector<Request*>& rows) {
+    const DTensor logits = constrained(unconstrained, rows);
     std::vector<int64_t> tokens(rows.size());
     const bool greedy = std::all_of(rows.begin(), rows.end(), [](Request* r) { return r->sampling.temperature < 1e-6f; });
     if (greedy) {
@@ -265,6 +344,7 @@ std::vector<Engine::Token> Engine::step(int32_t token_budget) {
     for (size_t i = 0; i < sampled.size(); i++) {
         Request& r = *sampled[i];
         r.last = tokens[i];
+        r.answer.push_back(tokens[i]);
         r.left--;
         out.push_back(Token{r.id, tokens[i], r.left == 0 || tokens[i] == r.eos});
     }
@@ -342,6 +422,22 @@ ox_status ox_engine_step(ox_engine* h, int32_t token_budget, ox_engine_token* to
     const auto got = h->e->step(token_budget);
     for (size_t i = 0; i < got.size(); i++) tokens[i] = ox_engine_token{got[i].request, got[i].token, got[i].finished ? 1 : 0};
     *n_tokens = (int32_t)got.size();
+    return OX_OK;
+    OX_CATCH
+}
+
+ox_status ox_engine_constrain(ox_engine* h, int64_t request, float repetition, float frequency, float presence, const int32_t* bias_ids, const float* bias,
+                              int32_t n_bias) {
+    OX_TRY
+    const size_t n = (size_t)std::max(n_bias, 0);
+    h->e->constrain(request, repetition, frequency, presence, std::vector<int32_t>(bias_ids, bias_ids + n), std::vector<float>(bias, bias + n));
+    return OX_OK;
+    OX_CATCH
+}
+
+ox_status ox_engine_allow(ox_engine* h, int64_t request, const uint32_t* allowed, size_t n_words) {
+    OX_TRY
+    h->e->allow(request, allowed ? std::vector<uint32_t>(allowed, allowed + n_words) : std::vector<uint32_t>());
     return OX_OK;
     OX_CATCH
 }

@@ -34,6 +34,15 @@ public:
         int64_t request, token;
         bool finished;
     };
+    // What a request asks of its tokens (rules.hpp); `allowed`: a bit per token, empty: all.
+    struct Rules {
+        float repetition = 1.f, frequency = 0.f, presence = 0.f;
+        std::vector<int32_t> bias_ids;
+        std::vector<float> bias;
+        std::vector<uint32_t> allowed;
+        bool history() const { return repetition != 1.f || frequency != 0.f || presence != 0.f; }
+        bool any() const { return history() || !bias_ids.empty() || !allowed.empty(); }
+    };
 
     // Room for `max_tokens` tokens (each sequence's count rounded up to whole pages) and `max_seqs` sequences.
     Engine(Session& s, int64_t max_tokens, int32_t max_seqs);
@@ -50,6 +59,9 @@ public:
     int64_t submit(std::vector<int64_t> prompt, int32_t max_new, int64_t eos, const Sampling& sampling);
     std::vector<Token> step(int32_t token_budget);
     void cancel(int64_t request);
+    // For the tokens that a submitted request has still to generate; each replaces what it was before.
+    void constrain(int64_t request, float repetition, float frequency, float presence, std::vector<int32_t> bias_ids, std::vector<float> bias);
+    void allow(int64_t request, std::vector<uint32_t> allowed);
 
     Session& session() { return s_; }
     int64_t page_size() const { return page_; }
@@ -68,7 +80,8 @@ private:
     };
     struct Request {
         int64_t id;
-        std::vector<int64_t> prompt;
+        std::vector<int64_t> prompt, answer;
+        Rules rules;
         size_t fed = 0;       // prompt tokens already run
         int64_t last = -1;    // the token to run next once the prompt is done
         int32_t left;         // tokens still to generate
@@ -79,6 +92,8 @@ private:
     };
     int64_t pages_for(int64_t tokens) const { return (tokens + page_ - 1) / page_; }
     std::vector<int64_t> sample(const DTensor& logits, const std::vector<Request*>& rows);
+    DTensor constrained(const DTensor& logits, const std::vector<Request*>& rows);
+    Request& request_of(int64_t id);
 
     Session& s_;
     int64_t page_ = 0, n_pages_ = 0, vocab_ = 0;

@@ -52,12 +52,46 @@ class Engine:
         check(self._lib.ox_engine_release(self._h, int(seq)))
 
     def submit(self, prompt, max_new: int, *, eos: int = -1, temperature: float = 0.0, top_k: int = 0, top_p: float = 1.0,
-               seed: int = 0) -> int:
+               seed: int = 0, repetition: float = 1.0, frequency: float = 0.0, presence: float = 0.0, bias: dict | None = None) -> int:
+        """`repetition` divides positive and multiplies negative logits of tokens in the prompt or the answer, `frequency` (times its count) and `presence` are taken
+        from those of the answer's tokens, `bias` adds to a token's logit."""
         words = _ffi.int_words("q", prompt)
         out = C.c_int64()
         check(self._lib.ox_engine_submit(self._h, C.cast(words.buffer_info()[0], C.POINTER(C.c_int64)), len(words), int(max_new), int(eos),
                                          float(temperature), int(top_k), float(top_p), int(seed) & (2 ** 64 - 1), C.byref(out)))
+        if repetition != 1.0 or frequency or presence or bias:
+            try:
+                self.constrain(out.value, repetition=repetition, frequency=frequency, presence=presence, bias=bias)
+            except Exception:
+                self.cancel(out.value)
+                raise
         return out.value
+
+    def constrain(self, request: int, *, repetition: float = 1.0, frequency: float = 0.0, presence: float = 0.0, bias: dict | None = None) -> None:
+        """The rules of :meth:`submit` for the tokens that a request has still to generate, in place of those it had."""
+        ids, values = np.array(list((bias or {}).keys()), dtype=np.int64), np.array(list((bias or {}).values()), dtype=np.float32)
+        if ids.size and (ids.min() < 0 or ids.max() > 2 ** 31 - 1):
+            raise ValueError(f"a bias of a token that is not one of {self.vocab}")
+        ids = ids.astype(np.int32)
+        check(self._lib.ox_engine_constrain(self._h, int(request), float(repetition), float(frequency), float(presence), ids.ctypes.data_as(C.POINTER(C.c_int32)),
+                                            values.ctypes.data_as(C.POINTER(C.c_float)), ids.size))
+
+    def allow(self, request: int, tokens=None) -> None:
+        """Only these tokens (ids, or a truth value per token of the vocabulary) from the request's next one on; None: all."""
+        if tokens is None:
+            check(self._lib.ox_engine_allow(self._h, int(request), None, 0))
+            return
+        tokens = np.asarray(tokens)
+        if tokens.dtype != np.bool_:
+            ids, tokens = tokens.astype(np.int64).reshape(-1), np.zeros(self.vocab, np.bool_)
+            if ids.size and (ids.min() < 0 or ids.max() >= self.vocab):
+                raise ValueError(f"a token that is not one of {self.vocab}")
+            tokens[ids] = True
+        if tokens.shape != (self.vocab,):
+            raise ValueError(f"a truth value per token is wanted, {self.vocab} of them")
+        bits = np.zeros(-(-self.vocab // 32) * 4, np.uint8)
+        bits[:-(-self.vocab // 8)] = np.packbits(tokens, bitorder="little")
+        check(self._lib.ox_engine_allow(self._h, int(request), bits.ctypes.data_as(C.POINTER(C.c_uint32)), bits.size // 4))
 
     def step(self, token_budget: int = 2048) -> list:
         """One scheduler step → [(request, token, finished)]."""
@@ -72,9 +106,9 @@ class Engine:
         check(self._lib.ox_engine_cancel(self._h, int(request)))
 
     def generate(self, prompts, max_new: int, *, token_budget: int = 2048, eos: int = -1, temperature: float = 0.0,
-                 top_k: int = 0, top_p: float = 1.0, seed: int = 0) -> list:
-        """Generated tokens of every prompt, batched continuously."""
-        ids = [self.submit(p, max_new, eos=eos, temperature=temperature, top_k=top_k, top_p=top_p, seed=seed + i)
+                 top_k: int = 0, top_p: float = 1.0, seed: int = 0, **rules) -> list:
+        """Generated tokens of every prompt, batched continuously. `rules`: those of :meth:`submit`."""
+        ids = [self.submit(p, max_new, eos=eos, temperature=temperature, top_k=top_k, top_p=top_p, seed=seed + i, **rules)
                for i, p in enumerate(prompts)]
         out = {i: [] for i in ids}
         while True:

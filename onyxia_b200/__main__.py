@@ -30,7 +30,11 @@ def generate(argv) -> int:
     ap.add_argument("--top-k", type=int, default=0)
     ap.add_argument("--top-p", type=float, default=1.0)
     ap.add_argument("--seed", type=int, default=0)
+    ap.add_argument("--repetition", type=float, default=1.0, help="what the logits of tokens seen before are divided by (negative ones: multiplied)")
+    ap.add_argument("--frequency", type=float, default=0.0, help="what a token's logit loses for every time it was generated")
+    ap.add_argument("--presence", type=float, default=0.0, help="what a token's logit loses once it was generated")
     a = ap.parse_args(argv)
+    rules = {k: getattr(a, k) for k, none in (("repetition", 1.0), ("frequency", 0.0), ("presence", 0.0)) if getattr(a, k) != none}
     from . import build
     build.ensure_built(oracle=False)
     from . import llm, models
@@ -40,7 +44,9 @@ def generate(argv) -> int:
     if "seq_info" in module.input_names():
         e = Engine(CudaBackend((0,)).prepare(module), a.max_tokens, a.max_seqs)
         outs = e.generate(a.prompt, a.max_new, token_budget=a.token_budget, eos=a.eos, temperature=a.temperature, top_k=a.top_k,
-                          top_p=a.top_p, seed=a.seed)
+                          top_p=a.top_p, seed=a.seed, **rules)
+    elif rules:
+        ap.error(f"--{next(iter(rules))} needs a module that the engine runs: this one has dense caches")
     else:  # a module with dense caches: one sequence after the other
         from .sampling import DeviceSampler, SamplingConfig
         s = llm.NativeLlmSession(CudaBackend((0,)), module, a.max_tokens)

@@ -8,7 +8,9 @@ followed by a mixture of experts.
 
 attention  grouped-query attention with biased projections: rotation of the leading dimensions of a head with all frequencies
            divided by a factor, queries and keys divided by their root mean square after it, capped scores, a window, a
-           sink of score 0 in the softmax. A layer may read the keys and values of an earlier one
+           sink of score 0 in the softmax. A layer may read the keys and values of an earlier one. Differential: a head has two
+           queries, its key head two keys, and the second softmax map, times a learned factor, is taken from the first; the
+           heads' results are divided by their root mean square
 lightning  linear attention with a matrix state per head that decays by a constant; the heads' results are normed
            together, gated and projected
 experts    the router's best few, weighted by the softmax over their logits; gated units with silu
@@ -45,6 +47,7 @@ class AttentionConfig:
     softcap: float = 0.0      # 0: none
     window: int = 0           # 0: all keys
     kv_from: int | None = None
+    lambda_init: float | None = None  # differential attention, `dim` that of one map: what the second map's factor begins with
 
 
 @dataclasses.dataclass
@@ -81,9 +84,13 @@ def _attention(i: int, m: dict, layers: list) -> AttentionConfig:
         raise ValueError(f"layer {i}: {a.rot_dims} of {a.dim} dimensions cannot rotate in pairs")
     if mask and a.window < 1:
         raise ValueError(f"layer {i}: a window of {a.window} tokens")
+    if m.get("differential") is not None:
+        a.lambda_init = float(m["differential"]["lambda_init"])
+        if a.kv_from is not None:
+            raise ValueError(f"layer {i}: differential attention reads keys of its own")
     if a.kv_from is not None:
         source = layers[a.kv_from].mixer if 0 <= a.kv_from < i else None
-        if not isinstance(source, AttentionConfig) or source.kv_from is not None:
+        if not isinstance(source, AttentionConfig) or source.kv_from is not None or source.lambda_init is not None:
             raise ValueError(f"layer {i}: layer {a.kv_from} has no keys of its own before it")
         if (source.kv_heads, source.dim, source.vdim) != (a.kv_heads, a.dim, a.vdim):
             raise ValueError(f"layer {i}: its keys and values differ in size from those of layer {a.kv_from}")
@@ -167,6 +174,9 @@ def build(cfg: KipizenConfig, w: Weights, dtype: int = ir.BF16) -> ir.Module:
     def matrix(name, rows, cols):
         return const(stored(name, rows, cols), dtype)
 
+    def maps(m):
+        return 1 if m.lambda_init is None else 2
+
     own_kv = [isinstance(l.mixer, AttentionConfig) and l.mixer.kv_from is None for l in cfg.layers]
     ids = b.input("input_ids", ir.I64, [N])
     seqs = b.input("seq_info", ir.I32, [R, 4])
@@ -178,7 +188,7 @@ def build(cfg: KipizenConfig, w: Weights, dtype: int = ir.BF16) -> ir.Module:
         if isinstance(m, LightningConfig):
             state[i] = (b.input(f"slots.{i}.state", ir.F32, [NS, m.heads, m.dim, m.vdim]),)
         elif own_kv[i]:
-            state[i] = (b.input(f"pages.{i}.keys", dtype, [NP, m.kv_heads, PAGE, m.dim]),
+            state[i] = (b.input(f"pages.{i}.keys", dtype, [NP, m.kv_heads, PAGE, maps(m) * m.dim]),
                         b.input(f"pages.{i}.values", dtype, [NP, m.kv_heads, PAGE, m.vdim]))
 
     # A sum that has not been formed yet: (residual or None, sublayer result, its factor). The norm that reads it forms it
@@ -196,7 +206,7 @@ def build(cfg: KipizenConfig, w: Weights, dtype: int = ir.BF16) -> ir.Module:
                            [(dt, [count, out]), (ir.F32, [count, H])])
 
     def attention(i, m, p, pend, norm):
-        q_n, k_n, v_n = m.heads * m.dim, m.kv_heads * m.dim, m.kv_heads * m.vdim
+        q_n, k_n, v_n = maps(m) * m.heads * m.dim, maps(m) * m.kv_heads * m.dim, m.kv_heads * m.vdim
         parts = [("q", q_n)] + ([("k", k_n), ("v", v_n)] if own_kv[i] else [])
         weight = np.concatenate([stored(f"{p}.mix.{n}", size, H) for n, size in parts])
         bias = np.concatenate([w.f32(f"{p}.mix.{n}.b") for n, _ in parts])
@@ -206,7 +216,21 @@ def build(cfg: KipizenConfig, w: Weights, dtype: int = ir.BF16) -> ir.Module:
         attrs = {"heads": m.heads, "kv_heads": m.kv_heads, "dim": m.dim, "vdim": m.vdim, "q_offset": 0, "rot_dims": m.rot_dims,
                  "window": m.window, "scale": float(m.scale), "softcap": float(m.softcap), "epsilon": float(cfg.eps), "norm": 1, "sink": 1}
         turns, out = const(turns_per_position(m.rot_dims, m.rot_base, m.rot_factor)), (dtype, [N, m.heads * m.vdim])
-        if own_kv[i]:
+        if m.lambda_init is not None:
+            lam = [w.f32(f"{p}.mix.lam.{n}").astype(np.float64) for n in ("q1", "k1", "q2", "k2")]
+            if any(v.shape != (m.dim,) for v in lam):
+                raise ValueError(f"layer {i}: the four vectors of the second map's factor have {m.dim} elements each")
+            factor = math.exp(lam[0] @ lam[1]) - math.exp(lam[2] @ lam[3]) + m.lambda_init
+            gain = w.f32(f"{p}.mix.head_norm")
+            if gain.shape != (m.vdim,):
+                raise ValueError(f"tensor '{p}.mix.head_norm' has shape {list(gain.shape)}, expected [{m.vdim}]")
+            b.set_loc(f"{p}.mix", "DifferentialAttention")
+            o, keys, values = b.composite(
+                "onyxia.DifferentialAttention", dict(attrs, k_offset=q_n, v_offset=q_n + k_n, head_norm=1, head_epsilon=float(cfg.eps)),
+                [proj, turns, *state[i], seqs, table, const(np.full(m.heads, factor, np.float32)), const(gain * np.float32(1.0 - m.lambda_init))],
+                [out, (dtype, [NP, m.kv_heads, PAGE, 2 * m.dim]), (dtype, [NP, m.kv_heads, PAGE, m.vdim])])
+            updated.extend([(f"pages.{i}.keys", keys), (f"pages.{i}.values", values)])
+        elif own_kv[i]:
             b.set_loc(f"{p}.mix", "PagedKVAttention")
             o, keys, values = b.composite(
                 "onyxia.PagedKVAttention", dict(attrs, k_offset=q_n, v_offset=q_n + k_n), [proj, turns, *state[i], seqs, table],
@@ -289,9 +313,13 @@ def tensor_shapes(cfg: KipizenConfig) -> dict:
             out.update({p + "mix.q": (qk, H), p + "mix.k": (qk, H), p + "mix.v": (vg, H), p + "mix.g": (vg, H), p + "mix.norm": (vg,),
                         p + "mix.o": (H, vg)})
         else:
-            sizes = [("q", m.heads * m.dim)]
+            n_maps = 1 if m.lambda_init is None else 2
+            sizes = [("q", n_maps * m.heads * m.dim)]
             if m.kv_from is None:
-                sizes += [("k", m.kv_heads * m.dim), ("v", m.kv_heads * m.vdim)]
+                sizes += [("k", n_maps * m.kv_heads * m.dim), ("v", m.kv_heads * m.vdim)]
+            if m.lambda_init is not None:
+                out.update({f"{p}mix.lam.{n}": (m.dim,) for n in ("q1", "k1", "q2", "k2")})
+                out[p + "mix.head_norm"] = (m.vdim,)
             for n, size in sizes:
                 out.update({f"{p}mix.{n}": (size, H), f"{p}mix.{n}.b": (size,)})
             out[p + "mix.o"] = (H, m.heads * m.vdim)
@@ -309,7 +337,9 @@ def random_weights(cfg: KipizenConfig, seed: int = 0) -> Weights:
     out = {}
     for name, shape in tensor_shapes(cfg).items():
         last, n = name.rsplit(".", 1)[-1], int(np.prod(shape))
-        if last in ("norm", "norm1", "norm2"):
+        if ".lam." in name:
+            a = 0.1 * rng.standard_normal(n, dtype=np.float32)
+        elif last in ("norm", "norm1", "norm2", "head_norm"):
             a = 1.0 + 0.05 * rng.standard_normal(n, dtype=np.float32)
         elif last == "b":
             a = 0.1 * rng.standard_normal(n, dtype=np.float32)

@@ -20,13 +20,75 @@ constexpr float kLazy = 8.f;  // how far (base 2) a row's scores may rise above 
 struct PreP {
     alignas(64) unsigned char maps[2][128];  // keys, values: [rows of the pool, 2 · dim | vdim]
     DiffP kv;
-    int kp, vp, box, inv;  // panels of 64 dimensions, log2 of the keys per copy, 2^16 / heads of a key head, rounded up
+    int kp, vp, box, inv, tiles;  // panels of 64 dimensions, log2 of the keys per copy, 2^16 / heads of a key head, rounded up, tiles of a key head
 };
 
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+// Two f32 side by side: one instruction adds or multiplies both.
+using f32x2 = unsigned long long;
+__device__ __forceinline__ f32x2 pair_of(float a, float b) {
+    f32x2 v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
+    return v;
+}
+__device__ __forceinline__ void apart(f32x2 v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+    f32x2 v;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
+    return v;
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+    f32x2 v;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
+    return v;
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+    f32x2 v;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(a), "l"(b), "l"(c));
+    return v;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float v;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(v) : "f"(a), "f"(b), "f"(c));
+    return v;
+}
+__device__ __forceinline__ float max_of(const float (&s)[kPart]) {
+    float a = s[0], b = s[1];
+#pragma unroll
+    for (int e = 2; e + 3 < kPart; e += 4) {
+        a = max3(a, s[e], s[e + 1]);
+        b = max3(b, s[e + 2], s[e + 3]);
+    }
+    return max3(a, b, fmaxf(s[kPart - 2], s[kPart - 1]));
+}
+// s with e^2x = 2^s becomes cap2 · tanh x. Where |x| of no row of the warp is above 1, which is where caps are meant to leave scores alone, tanh x / x is a polynomial in x² (the best of its
+// degree in relative error, 6e-7): eight products and sums, two elements each, instead of three turns of the unit that also makes the exponentials. A step of 128 keys took
+// 2 500 cycles for the cap with that unit alone, out of 4 450.
+__device__ __forceinline__ void cap_scores(float (&s)[kPart], float cap2) {
+    constexpr double k = 0.34657359027997264, k2 = k * k;  // x = k · s
+    constexpr double c[6] = {0.99999941, -0.33329042, 0.13281434, -0.05160567, 0.01674312, -0.00306706};
+    float most = 0.f;
+#pragma unroll
+    for (int e = 0; e < kPart; e += 2) most = max3(most, fabsf(s[e]), fabsf(s[e + 1]));
+    if (!__any_sync(0xffffffffu, most > (float)(1.0 / k))) {
+        const f32x2 q0 = pair_of((float)(c[0] * k) * cap2, (float)(c[0] * k) * cap2), q1 = pair_of((float)(c[1] * k * k2) * cap2, (float)(c[1] * k * k2) * cap2),
+                    q2 = pair_of((float)(c[2] * k * k2 * k2) * cap2, (float)(c[2] * k * k2 * k2) * cap2),
+                    q3 = pair_of((float)(c[3] * k * k2 * k2 * k2) * cap2, (float)(c[3] * k * k2 * k2 * k2) * cap2),
+                    q4 = pair_of((float)(c[4] * k * k2 * k2 * k2 * k2) * cap2, (float)(c[4] * k * k2 * k2 * k2 * k2) * cap2),
+                    q5 = pair_of((float)(c[5] * k * k2 * k2 * k2 * k2 * k2) * cap2, (float)(c[5] * k * k2 * k2 * k2 * k2 * k2) * cap2);
+#pragma unroll
+        for (int e = 0; e < kPart; e += 2) {
+            const f32x2 x = pair_of(s[e], s[e + 1]), u = mul2(x, x);
+            apart(mul2(x, fma2(u, fma2(u, fma2(u, fma2(u, fma2(u, q5, q4), q3), q2), q1), q0)), s[e], s[e + 1]);
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < kPart; e++) s[e] = cap2 - __fdividef(2.f * cap2, 1.f + ex2(s[e]));
+    }
 }
 // Rows of weights in tensor memory (two per column) × values, of which 64 stand side by side for a key.
 __device__ __forceinline__ void umma_weights(unsigned d, unsigned a, unsigned long long b, unsigned idesc, bool accumulate) {
@@ -98,7 +160,7 @@ template <bool CAPPED, int KEYS> __global__ void __launch_bounds__(Shape<KEYS>::
     // (both CTAs of a cluster find the same place: their shared memory begins at the same address)
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     const DiffP& p = pp.kv;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, kp = pp.kp, vp = pp.vp, map = blockIdx.y & 1, g = blockIdx.y >> 1;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, kp = pp.kp, vp = pp.vp, across = 2 * p.kv_heads, map = (int)blockIdx.x & 1, tile = (int)blockIdx.x / across, g = ((int)blockIdx.x - tile * across) >> 1;
     constexpr int kHalves = Shape<KEYS>::halves, kSoft = Shape<KEYS>::soft, kStagesK = Shape<KEYS>::keys, kStagesV = Shape<KEYS>::values;
     constexpr int kCopies = kSoft / 32, kIssues = kCopies + 1;  // warps
     constexpr unsigned kPanelK = KEYS * 128;
@@ -117,8 +179,8 @@ template <bool CAPPED, int KEYS> __global__ void __launch_bounds__(Shape<KEYS>::
     const int rep = p.heads / p.kv_heads, tq = kRows / rep;
     int seq, first;
     SeqRow sq;
-    // long rows first: the last tiles of a sequence see the most keys
-    if (!locate_rows(p.seqs, p.n_seqs, (int)gridDim.x - 1 - (int)blockIdx.x, tq, p.singles ? 1 : 2, &seq, &first, &sq)) return;  // both CTAs of the cluster
+    // long rows of all heads first: the last tiles of a sequence see the most keys
+    if (!locate_rows(p.seqs, p.n_seqs, pp.tiles - 1 - tile, tq, p.singles ? 1 : 2, &seq, &first, &sq)) return;  // both CTAs of the cluster
     const int n_tok = min(tq, sq.len - first), pos0 = sq.past + first, last = pos0 + n_tok - 1, low = first_key(p, pos0);
     // Scores in KEYS columns, weights in two turns of half as many, sums behind them. No more CTAs than have room in tensor memory may be on an SM at a time
     // (differential_smem), or two clusters could wait for what the other one has.
@@ -262,7 +324,8 @@ template <bool CAPPED, int KEYS> __global__ void __launch_bounds__(Shape<KEYS>::
     if (warp < kCopies) {
         const int pos = tok < n_tok ? pos0 + tok : last, mine_low = first_key(p, pos), last_low = first_key(p, last);  // rows without a token compute something harmless
         const float cap2 = p.cap2;
-        float m = -1e30f, l = 0.f, l2 = 0.f;  // below every score, and finite: differences stay numbers
+        float m = -1e30f;  // below every score, and finite: differences stay numbers
+        f32x2 l2 = pair_of(0.f, 0.f);  // the sum of even keys' weights and that of odd ones'
         int halves = 0;                       // of the values, in front of this thread's
         for (int i = 0; i < n; i++) {
             const int j0 = (kt0 + i) * KEYS, j1 = j0 + part * kPart;
@@ -280,30 +343,20 @@ template <bool CAPPED, int KEYS> __global__ void __launch_bounds__(Shape<KEYS>::
             before_sync();
             __syncwarp();
             if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(s_free) : "memory");
-            if (CAPPED) {
-#pragma unroll
-                for (int e = 0; e < kPart; e++) s[e] = cap2 - __fdividef(2.f * cap2, 1.f + ex2(s[e]));
-            }
+            if (CAPPED) cap_scores(s, cap2);
             if (j1 + kPart - 1 > pos0 || j1 < last_low) {
 #pragma unroll
                 for (int e = 0; e < kPart; e++)
                     if (j1 + e > pos || j1 + e < mine_low) s[e] = -INFINITY;
             }
-            float top = fmaxf(s[0], s[1]), top2 = fmaxf(s[2], s[3]);
-#pragma unroll
-            for (int e = 4; e < kPart; e += 4) {
-                top = fmaxf(top, fmaxf(s[e], s[e + 1]));
-                top2 = fmaxf(top2, fmaxf(s[e + 2], s[e + 3]));
-            }
-            top = fmaxf(top, top2);
+            float top = max_of(s);
             if (kHalves == 2) top = fmaxf(top, both(i & 1, top));
             // Weights are taken against a maximum that may lie up to 2^8 behind: the sums are rarely taken anew, and bf16 holds 2^8 as well as 1. Both warps of a row see the same tops.
             if (__any_sync(0xffffffffu, top > m + kLazy)) {
                 top = fmaxf(top, m);
                 const float keep = ex2(m - top);
                 m = top;
-                l *= keep;
-                l2 *= keep;
+                l2 = mul2(l2, pair_of(keep, keep));
                 if (i > 0) {
                     if (ok && !added(i - 1)) ok = false;
                     after_sync();
@@ -322,15 +375,17 @@ template <bool CAPPED, int KEYS> __global__ void __launch_bounds__(Shape<KEYS>::
             after_sync();
             const int before = kHalves == 2 && part == 1 && seen(j0, 0);  // the other half's values come first
             if (seen(j0, part)) {
+                const f32x2 behind = pair_of(-m, -m);
 #pragma unroll
                 for (int c = 0; c < 2; c++) {
                     unsigned w[16];
 #pragma unroll
                     for (int e = 0; e < 16; e++) {
-                        w[e] = pack_bf16(ex2(s[c * 32 + 2 * e] - m), ex2(s[c * 32 + 2 * e + 1] - m));
+                        float a, b;
+                        apart(add2(pair_of(s[c * 32 + 2 * e], s[c * 32 + 2 * e + 1]), behind), a, b);
+                        w[e] = pack_bf16(ex2(a), ex2(b));
                         // the sums of the weights as they are multiplied: the rounding of a weight that stands out is in both
-                        l += __uint_as_float(w[e] << 16);
-                        l2 += __uint_as_float(w[e] & 0xFFFF0000u);
+                        l2 = add2(l2, pair_of(__uint_as_float(w[e] << 16), __uint_as_float(w[e] & 0xFFFF0000u)));
                     }
                     tmem_st16(tmem + lanes + KEYS + (i & 1) * (KEYS / 2) + part * (kPart / 2) + c * 16, w);
                 }
@@ -351,7 +406,9 @@ template <bool CAPPED, int KEYS> __global__ void __launch_bounds__(Shape<KEYS>::
             if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(w_full + (i & 1) * 16 + part * 8) : "memory");
             halves += seen(j0, 0) + (kHalves == 2 && seen(j0, 1));
         }
-        l += l2;
+        float l, odd;
+        apart(l2, l, odd);
+        l += odd;
         if (kHalves == 2) l += both(n & 1, l);
         if (ok && !added(n - 1)) ok = false;
         after_sync();
@@ -443,8 +500,8 @@ int differential_smem(int kp, int vp) {
 }  // namespace
 
 bool differential_prefill_fits(const DiffP& p, const TRef& keys, const TRef& values, int64_t out_off) {
-    const int64_t rows = (int64_t)p.n_pages * p.kv_heads << p.shift;
-    return 1 << p.shift >= 8 && p.dim % 16 == 0 && p.dim <= 128 && p.vdim % 8 == 0 && p.vdim <= 256 && p.heads / p.kv_heads <= kRows && p.kv_heads <= 32767 && rows < INT32_MAX &&
+    const int64_t rows = (int64_t)p.n_pages * p.kv_heads << p.shift, rep = p.heads / p.kv_heads, tiles = rep <= kRows ? p.rows / (kRows / rep) + 1 + p.n_seqs : 0;
+    return 1 << p.shift >= 8 && p.dim % 16 == 0 && p.dim <= 128 && p.vdim % 8 == 0 && p.vdim <= 256 && rep <= kRows && tiles * 2 * p.kv_heads < INT32_MAX && rows < INT32_MAX &&
            keys.buf.off % 16 == 0 && values.buf.off % 16 == 0 && out_off % 16 == 0;
 }
 
@@ -456,12 +513,13 @@ void emit_differential_prefill(Emitter& em, const DiffP& kv, const TRef& keys, c
     p.box = std::min(6, kv.shift);
     p.inv = (65536 + kv.heads / kv.kv_heads - 1) / (kv.heads / kv.kv_heads);
     const int64_t tq = kRows / (kv.heads / kv.kv_heads), rows = (int64_t)kv.n_pages * kv.kv_heads << kv.shift;
+    p.tiles = (int)((kv.rows + tq - 1) / tq + kv.n_seqs);
     void (*const k)(const PreP) = differential_keys(p.kp, p.vp) == 64 ? (kv.cap2 > 0.f ? differential_prefill<true, 64> : differential_prefill<false, 64>)
                                                                      : (kv.cap2 > 0.f ? differential_prefill<true, 128> : differential_prefill<false, 128>);
     const int smem = differential_smem(p.kp, p.vp);
     ensure_max_dynamic_smem((const void*)k, 226 * 1024);
-    LaunchRec& rec = em.launch(k, dim3((unsigned)((kv.rows + tq - 1) / tq + kv.n_seqs), (unsigned)kv.kv_heads * 2), dim3(differential_keys(p.kp, p.vp) == 64 ? Shape<64>::threads : Shape<128>::threads), (unsigned)smem, p, {}, "differential_prefill", /*pdl=*/true);
-    rec.cluster = dim3(1, 2, 1);
+    LaunchRec& rec = em.launch(k, dim3((unsigned)p.tiles * (unsigned)kv.kv_heads * 2), dim3(differential_keys(p.kp, p.vp) == 64 ? Shape<64>::threads : Shape<128>::threads), (unsigned)smem, p, {}, "differential_prefill", /*pdl=*/true);
+    rec.cluster = dim3(2, 1, 1);
     for (auto& pr : ptrs) rec.relocs.push_back(Reloc{(uint32_t)(offsetof(PreP, kv) + pr.first), pr.second});
     rec.tmaps.push_back(TmapReloc{(uint32_t)offsetof(PreP, maps), keys.buf, (uint64_t)kv.dim * 2, (uint64_t)rows, (uint64_t)kv.dim * 4, 64u, 1u << p.box});
     rec.tmaps.push_back(TmapReloc{(uint32_t)offsetof(PreP, maps) + 128, values.buf, (uint64_t)kv.vdim, (uint64_t)rows, (uint64_t)kv.vdim * 2, 64u, 1u << p.box});

@@ -38,7 +38,7 @@ template <typename T> __global__ void __launch_bounds__(128) differential_prepar
         const float f = map_factor(p, src);
         if constexpr (sizeof(T) == 2)
             if (k < 0 && p.parts) {
-                bf16* to = (bf16*)p.q + ((long long)row * p.heads * 2 + h) * 2 * p.dim;
+                bf16* to = part_row(p, row, h);
                 for (int i = lane; i < p.dim; i += 32) {
                     const float v = (float)turned(p, src, angle, angle + p.half, i) * f * p.mul2;
                     const bf16 high = __float2bfloat16_rn(v);
@@ -52,18 +52,27 @@ template <typename T> __global__ void __launch_bounds__(128) differential_prepar
     for (int i = threadIdx.x; i < p.kv_heads * p.vdim; i += 128) ((T*)p.values)[key_row(p, pg, i / p.vdim, pos) * p.vdim + i % p.vdim] = x[p.v_off + i];
 }
 
-// The same in bf16 eight elements at a time, where heads, rotated halves and rows allow it: a unit is eight pairs that turn or eight elements that do not.
+// The same in bf16 eight elements at a time, where heads, rotated halves and rows allow it: a unit is eight pairs that turn or eight elements that do not. 4096 tokens with 64 queries and
+// 32 keys of 64 and 16 values of 128 (167 MB in and out): 40 us, with divisions by what only the host knows and nothing asked for before the angles 54; the kernel above 146.
 __global__ void __launch_bounds__(128, 8) differential_prepare8(const DiffP p) {
     extern __shared__ double angle[];  // cos[half], sin[half], both again as f32 (for the queries), with norms [2 · (heads + kv_heads)] factors as f32
     pdl_enter();
-    const int row = blockIdx.x, s = find_seq(p.seqs, p.n_seqs, row), tid = threadIdx.x;
+    const int row = blockIdx.x, tid = threadIdx.x;
+    // the row's queries, keys and values are on their way while its sequence is looked up and its angles are made
+    const bf16* x = (const bf16*)p.proj + (long long)row * p.ld;
+    auto fetch = [&](long long at, int n) {
+        for (int i = tid * 64; i < n; i += 128 * 64) asm volatile("prefetch.global.L1 [%0];" ::"l"(x + at + i) : "memory");
+    };
+    fetch(p.q_off, 2 * p.heads * p.dim);
+    fetch(p.k_off, 2 * p.kv_heads * p.dim);
+    fetch(p.v_off, p.kv_heads * p.vdim);
+    const int s = find_seq(p.seqs, p.n_seqs, row);
     const SeqRow sq = load_seq(p.seqs, s);
     const int pos = sq.past + row - sq.start, maps = 2 * (p.heads + p.kv_heads);
     if (row < sq.start || row >= sq.start + sq.len || (sq.len == 1 && !p.singles)) return;
     float* short_angle = reinterpret_cast<float*>(angle + 2 * p.half);
     exact_angles(p, pos, angle, angle + p.half, tid, 128);
     for (int i = tid; i < p.half; i += 128) short_angle[i] = (float)angle[i], short_angle[p.half + i] = (float)angle[p.half + i];  // (its own)
-    const bf16* x = (const bf16*)p.proj + (long long)row * p.ld;
     auto source = [&](int h) { return h < 2 * p.heads ? x + p.q_off + (long long)h * p.dim : x + p.k_off + (long long)(h - 2 * p.heads) * p.dim; };
     float* factor = short_angle + 2 * p.half;
     if (p.norm)
@@ -73,59 +82,75 @@ __global__ void __launch_bounds__(128, 8) differential_prepare8(const DiffP p) {
         }
     __syncthreads();
     const long long pg = page_of(p, s, pos);
-    const int turned = p.half / 8, units = p.dim / 8 - turned;
-    auto put = [&](int h, int at, const float (&v)[8]) {
-        unsigned w[4];
-#pragma unroll
-        for (int e = 0; e < 4; e++) w[e] = pack_bf16(v[2 * e], v[2 * e + 1]);
-        const int k = h - 2 * p.heads;
-        bf16* to = k >= 0 ? (bf16*)p.keys + (key_row(p, pg, k >> 1, pos) * 2 + (k & 1)) * p.dim : (bf16*)p.q + ((long long)row * p.heads * 2 + h) * (1 + p.parts) * p.dim;
-        *reinterpret_cast<uint4*>(to + at) = make_uint4(w[0], w[1], w[2], w[3]);
-        if (k >= 0 || !p.parts) return;
-#pragma unroll
-        for (int e = 0; e < 4; e++) w[e] = pack_bf16(v[2 * e] - __uint_as_float(w[e] << 16), v[2 * e + 1] - __uint_as_float(w[e] & 0xFFFF0000u));
-        *reinterpret_cast<uint4*>(to + p.dim + at) = make_uint4(w[0], w[1], w[2], w[3]);
-    };
+    const int turned = p.half / 8, units = p.dim / 8 - turned, lanes = p.vdim / 8;
+    const long long key0 = key_row(p, pg, 0, pos), page = 1ll << p.shift;
     auto wide = [](uint4 u, float (&v)[8]) {
         const unsigned w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
         for (int e = 0; e < 4; e++) v[2 * e] = __uint_as_float(w[e] << 16), v[2 * e + 1] = __uint_as_float(w[e] & 0xFFFF0000u);
     };
-    for (int u = tid; u < maps * units; u += 128) {
-        const int h = u / units, i = u % units;
+    auto put = [&](bf16* to, const float (&v)[8], bool parts) {
+        unsigned w[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) w[e] = pack_bf16(v[2 * e], v[2 * e + 1]);
+        *reinterpret_cast<uint4*>(to) = make_uint4(w[0], w[1], w[2], w[3]);
+        if (!parts) return;
+#pragma unroll
+        for (int e = 0; e < 4; e++) w[e] = pack_bf16(v[2 * e] - __uint_as_float(w[e] << 16), v[2 * e + 1] - __uint_as_float(w[e] & 0xFFFF0000u));
+        *reinterpret_cast<uint4*>(to + p.dim) = make_uint4(w[0], w[1], w[2], w[3]);
+    };
+    for (int u = tid; u < 2 * p.heads * units; u += 128) {
+        const int h = over(u, p.by_units), i = u - h * units;
         const bool turns = i < turned;
         const int at = turns ? i * 8 : (i + turned) * 8;
-        const bf16* src = source(h) + at;
-        const float f = (p.norm ? factor[h] : 1.f) * (h < 2 * p.heads && p.parts ? p.mul2 : 1.f);
+        const bf16* src = x + p.q_off + h * p.dim + at;
+        bf16* to = (p.parts ? part_row(p, row, h) : (bf16*)p.q + ((long long)row * p.heads * 2 + h) * p.dim) + at;
+        const float f = (p.norm ? factor[h] : 1.f) * (p.parts ? p.mul2 : 1.f);
         float a[8], b[8], o[8];
         wide(*reinterpret_cast<const uint4*>(src), a);
         if (!turns) {
 #pragma unroll
             for (int e = 0; e < 8; e++) o[e] = a[e] * f;
-            put(h, at, o);
+            put(to, o, p.parts);
             continue;
         }
         wide(*reinterpret_cast<const uint4*>(src + p.half), b);
-        if (h < 2 * p.heads) {
-            const float *c = short_angle + at, *n = c + p.half;
+        const float *c = short_angle + at, *n = c + p.half;
 #pragma unroll
-            for (int e = 0; e < 8; e++) o[e] = (a[e] * c[e] - b[e] * n[e]) * f;
-            put(h, at, o);
+        for (int e = 0; e < 8; e++) o[e] = (a[e] * c[e] - b[e] * n[e]) * f;
+        put(to, o, p.parts);
 #pragma unroll
-            for (int e = 0; e < 8; e++) o[e] = (b[e] * c[e] + a[e] * n[e]) * f;
-            put(h, at + p.half, o);
+        for (int e = 0; e < 8; e++) o[e] = (b[e] * c[e] + a[e] * n[e]) * f;
+        put(to + p.half, o, p.parts);
+    }
+    for (int u = tid; u < 2 * p.kv_heads * units; u += 128) {
+        const int k = over(u, p.by_units), i = u - k * units;
+        const bool turns = i < turned;
+        const int at = turns ? i * 8 : (i + turned) * 8;
+        const bf16* src = x + p.k_off + k * p.dim + at;
+        bf16* to = (bf16*)p.keys + ((key0 + (k >> 1) * page) * 2 + (k & 1)) * p.dim + at;
+        const float f = p.norm ? factor[2 * p.heads + k] : 1.f;
+        float a[8], b[8], o[8];
+        wide(*reinterpret_cast<const uint4*>(src), a);
+        if (!turns) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) o[e] = a[e] * f;
+            put(to, o, false);
             continue;
         }
+        wide(*reinterpret_cast<const uint4*>(src + p.half), b);
         const double *c = angle + at, *n = c + p.half;
 #pragma unroll
         for (int e = 0; e < 8; e++) o[e] = (float)(((double)a[e] * c[e] - (double)b[e] * n[e]) * f);
-        put(h, at, o);
+        put(to, o, false);
 #pragma unroll
         for (int e = 0; e < 8; e++) o[e] = (float)(((double)b[e] * c[e] + (double)a[e] * n[e]) * f);
-        put(h, at + p.half, o);
+        put(to + p.half, o, false);
     }
-    for (int u = tid; u < p.kv_heads * p.vdim / 8; u += 128)
-        *reinterpret_cast<uint4*>((bf16*)p.values + key_row(p, pg, u * 8 / p.vdim, pos) * p.vdim + u * 8 % p.vdim) = *reinterpret_cast<const uint4*>(x + p.v_off + u * 8);
+    for (int u = tid; u < p.kv_heads * lanes; u += 128) {
+        const int g = over(u, p.by_lanes);
+        *reinterpret_cast<uint4*>((bf16*)p.values + (key0 + g * page) * p.vdim + (u - g * lanes) * 8) = *reinterpret_cast<const uint4*>(x + p.v_off + u * 8);
+    }
 }
 
 // One CTA per (row, head); chunks of 128 keys, a thread per key, then a thread per value dimension.
@@ -562,6 +587,11 @@ void emit_differential(Emitter& em, const DifferentialDesc& d, const TRef& proj,
     p.singles = !tc || (!p.only && n_seqs == 1);       // a lone token with rows of nobody behind it
     const bool prefill = tc && !p.only && differential_prefill_fits(p, keys, values, out.buf.off);
     p.parts = prefill;
+    auto by = [](int64_t d) { return d > 1 ? (unsigned)(((1ull << 32) + d - 1) / d) : 0u; };
+    p.rep = d.heads / d.kv_heads;
+    p.by_rep = by(p.rep);
+    p.by_units = by(d.dim / 8 - d.rot_dims / 16);
+    p.by_lanes = by(d.vdim / 8);
     p.by8 = p.ld % 8 == 0 && d.q_off % 8 == 0 && d.k_off % 8 == 0 && d.v_off % 8 == 0 && proj.buf.off % 16 == 0;
     const Buf none{kSlotNull, 0}, q = p.only ? none : em.scratch((size_t)rows * d.heads * 2 * d.dim * (bf && !prefill ? 2 : 4));
     auto launch = [&](DiffKernel k, dim3 grid, unsigned block, unsigned smem, Buf part, const char* label) {

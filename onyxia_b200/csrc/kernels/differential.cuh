@@ -8,7 +8,7 @@ struct DiffP {
     const void* proj;            // [rows, ld]
     const float* turns;          // [2, half]
     void *keys, *values;         // [pages, kv_heads, page, 2 · dim | vdim]
-    void* q;                     // prepared queries: [rows, heads, map, dim] of the pools' type, or, as the prefill kernel reads them, [rows, heads, map, high and low part, dim]
+    void* q;                     // prepared queries: [rows, heads, map, dim] of the pools' type, or, as the prefill kernel copies them, [kv_heads, rows, heads of a key head, map, high and low part, dim]
     void* out;                   // [rows, heads · vdim]
     const int* seqs;             // [R, 4]
     const int* table;            // [R, width]
@@ -26,6 +26,8 @@ struct DiffP {
     int parts;                   // prepare: queries in two parts, times mul2
     int by8;                     // the parts of a projection row begin on 16 bytes
     int only;                    // no sequence may have more than one
+    int rep;                     // heads of a key head
+    unsigned by_rep, by_units, by_lanes;  // 2^32 / (heads of a key head, units of a query, sixteen bytes of a value), rounded up; 0: of one
 };
 
 __device__ __forceinline__ int first_key(const DiffP& p, int pos) { return p.window > 0 ? max(0, pos - p.window + 1) : 0; }
@@ -99,7 +101,15 @@ __device__ __forceinline__ bool locate_rows(const int* seqs, int n_seqs, int til
     return false;
 }
 
-// Prompts on tcgen05 (differential_prefill.cu); queries come from `q` [rows, heads, map, high and low part, dim] in units of base 2; `ptrs`: fields of DiffP by their offset.
+// n / d for n < 2^32 / d
+__device__ __forceinline__ int over(int n, unsigned by) { return by ? (int)__umulhi((unsigned)n, by) : n; }
+// Where the high part of query h (2 · head + map) of a row is, for the prefill kernel.
+__device__ __forceinline__ bf16* part_row(const DiffP& p, int row, int h) {
+    const int g = over(h >> 1, p.by_rep);
+    return (bf16*)p.q + ((((g * p.rows + row) * p.rep + (h >> 1) - g * p.rep) * 2 + (h & 1)) * 2) * p.dim;
+}
+
+// Prompts on tcgen05 (differential_prefill.cu); queries come from `q` (part_row) in units of base 2; `ptrs`: fields of DiffP by their offset.
 bool differential_prefill_fits(const DiffP&, const TRef& keys, const TRef& values, int64_t out_off);
 void emit_differential_prefill(Emitter&, const DiffP&, const TRef& keys, const TRef& values, std::initializer_list<std::pair<size_t, Buf>> ptrs);
 

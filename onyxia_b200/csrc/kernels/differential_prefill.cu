@@ -14,7 +14,7 @@ namespace {
 
 constexpr int kRows = 128, kPart = 64;
 constexpr unsigned kPanelQ = kRows * 128, kPanelV = kPart * 128;  // bytes: rows × 64 dimensions
-constexpr int kBarriers = 21;
+constexpr int kBarriers = 23;
 constexpr float kLazy = 8.f;  // how far (base 2) a row's scores may rise above the maximum that its weights are taken against
 
 struct PreP {
@@ -51,6 +51,10 @@ __device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
     asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(a), "l"(b), "l"(c));
     return v;
 }
+// Two bf16 side by side onto two sums in f32.
+__device__ __forceinline__ void add_bf16(float& a, float& b, unsigned w) {
+    asm("{\n .reg .b16 low, high;\n mov.b32 {low, high}, %2;\n add.f32.bf16 %0, low, %0;\n add.f32.bf16 %1, high, %1;\n}\n" : "+f"(a), "+f"(b) : "r"(w));
+}
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float v;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(v) : "f"(a), "f"(b), "f"(c));
@@ -65,26 +69,34 @@ __device__ __forceinline__ float max_of(const float (&s)[kPart]) {
     }
     return max3(a, b, fmaxf(s[kPart - 2], s[kPart - 1]));
 }
-// s with e^2x = 2^s becomes cap2 · tanh x. Where |x| of no row of the warp is above 1, which is where caps are meant to leave scores alone, tanh x / x is a polynomial in x² (the best of its
-// degree in relative error, 6e-7): eight products and sums, two elements each, instead of three turns of the unit that also makes the exponentials. A step of 128 keys took
-// 2 500 cycles for the cap with that unit alone, out of 4 450.
+// s with e^2x = 2^s, x = score / cap, becomes cap2 · tanh x. Caps are there for scores that stand out: while |x| of a warp's scores stays below 1/2, or 1, tanh x / x is a polynomial in x²
+// (the best of its degree in relative error, 6e-7), N + 2 instructions for two elements, where an
+// exponential and a reciprocal take sixteen cycles of the unit that also makes the weights: 1999 tokens behind 1000, 4 heads of 2 x 128, scores far below the cap, 58 us instead of 74.
+template <int N> __device__ __forceinline__ void cap_within(float (&s)[kPart], float cap2, const double (&c)[N + 1]) {
+    constexpr double k = 0.34657359027997264;  // x = k · s
+    f32x2 q[N + 1];
+    double power = k;
+#pragma unroll
+    for (int j = 0; j <= N; j++, power *= k * k) q[j] = pair_of((float)(c[j] * power) * cap2, (float)(c[j] * power) * cap2);
+#pragma unroll
+    for (int e = 0; e < kPart; e += 2) {
+        const f32x2 x = pair_of(s[e], s[e + 1]), u = mul2(x, x);
+        f32x2 y = q[N];
+#pragma unroll
+        for (int j = N - 1; j >= 0; j--) y = fma2(u, y, q[j]);
+        apart(mul2(x, y), s[e], s[e + 1]);
+    }
+}
 __device__ __forceinline__ void cap_scores(float (&s)[kPart], float cap2) {
-    constexpr double k = 0.34657359027997264, k2 = k * k;  // x = k · s
-    constexpr double c[6] = {0.99999941, -0.33329042, 0.13281434, -0.05160567, 0.01674312, -0.00306706};
     float most = 0.f;
 #pragma unroll
     for (int e = 0; e < kPart; e += 2) most = max3(most, fabsf(s[e]), fabsf(s[e + 1]));
-    if (!__any_sync(0xffffffffu, most > (float)(1.0 / k))) {
-        const f32x2 q0 = pair_of((float)(c[0] * k) * cap2, (float)(c[0] * k) * cap2), q1 = pair_of((float)(c[1] * k * k2) * cap2, (float)(c[1] * k * k2) * cap2),
-                    q2 = pair_of((float)(c[2] * k * k2 * k2) * cap2, (float)(c[2] * k * k2 * k2) * cap2),
-                    q3 = pair_of((float)(c[3] * k * k2 * k2 * k2) * cap2, (float)(c[3] * k * k2 * k2 * k2) * cap2),
-                    q4 = pair_of((float)(c[4] * k * k2 * k2 * k2 * k2) * cap2, (float)(c[4] * k * k2 * k2 * k2 * k2) * cap2),
-                    q5 = pair_of((float)(c[5] * k * k2 * k2 * k2 * k2 * k2) * cap2, (float)(c[5] * k * k2 * k2 * k2 * k2 * k2) * cap2);
-#pragma unroll
-        for (int e = 0; e < kPart; e += 2) {
-            const f32x2 x = pair_of(s[e], s[e + 1]), u = mul2(x, x);
-            apart(mul2(x, fma2(u, fma2(u, fma2(u, fma2(u, fma2(u, q5, q4), q3), q2), q1), q0)), s[e], s[e + 1]);
-        }
+    if (!__any_sync(0xffffffffu, most > 1.44269504f)) {  // |x| up to 1/2
+        constexpr double c[4] = {0.99999946, -0.33326318, 0.13190297, -0.04440223};
+        cap_within<3>(s, cap2, c);
+    } else if (!__any_sync(0xffffffffu, most > 2.88539008f)) {  // up to 1
+        constexpr double c[6] = {0.99999941, -0.33329042, 0.13281434, -0.05160567, 0.01674312, -0.00306706};
+        cap_within<5>(s, cap2, c);
     } else {
 #pragma unroll
         for (int e = 0; e < kPart; e++) s[e] = cap2 - __fdividef(2.f * cap2, 1.f + ex2(s[e]));
@@ -130,9 +142,13 @@ __device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void before_sync() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void after_sync() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-// All threads of both CTAs. Every thread of a CTA that has a tile comes here, whatever its waits found.
-__device__ __forceinline__ void cluster_meet() {
-    asm volatile("barrier.cluster.arrive.release;\n barrier.cluster.wait.acquire;" ::: "memory");
+// All threads of both CTAs, warps at a time. Every thread of a CTA that has a tile comes here, whatever its waits found.
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ unsigned of_cta(unsigned smem_byte_addr, unsigned cta) {
+    unsigned to;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(smem_byte_addr), "r"(cta));
+    return to;
 }
 
 // The pages of the copies to come, 32 at a time and the next 32 on their way: the table's answer to a single question takes as long as a copy.
@@ -166,15 +182,17 @@ template <bool CAPPED, int KEYS> __global__ void __launch_bounds__(Shape<KEYS>::
     constexpr unsigned kPanelK = KEYS * 128;
     const unsigned k_stage = kp * kPanelK, v_stage = vp * kPanelV;
     const unsigned sq0 = smem_u32(smem), low0 = kp * kPanelQ, sk = sq0 + 2 * low0, sv = sk + kStagesK * k_stage, bars = sv + kStagesV * v_stage;
-    // barriers: keys there, free, values there, free (three each), scores there, read, products added (one, one and two), weights there (two halves of two), queries there
-    const unsigned k_full = bars, k_free = bars + 24, v_full = bars + 48, v_free = bars + 72, s_full = bars + 96, s_free = bars + 104, o_done = bars + 112, w_full = bars + 128, q_full = bars + 160;
+    // barriers: keys there, free, values there, free (three each), scores there, read, products added (one, one and two), weights there (two halves of two), queries there, rows of the other CTA there (two warps')
+    const unsigned k_full = bars, k_free = bars + 24, v_full = bars + 48, v_free = bars + 72, s_full = bars + 96, s_free = bars + 104, o_done = bars + 112, w_full = bars + 128, q_full = bars + 160, r_full = bars + 168;
     unsigned* tmem_slot = reinterpret_cast<unsigned*>(smem + (bars + kBarriers * 8 - sq0));
     float* scales = reinterpret_cast<float*>(smem + (bars + kBarriers * 8 + 8 - sq0));  // [64]: what the norms divide by
     float* shared = scales + 64;  // [turn][half of the keys][row]: what the two threads of a row tell each other
     if (tid == 0) {
-        for (int i = 0; i < kBarriers; i++) mbar_init(bars + i * 8, i == 13 ? kSoft / 32 : i == 20 ? kSoft : i >= 16 ? kRows / 32 : 1);
+        for (int i = 0; i < kBarriers; i++) mbar_init(bars + i * 8, i == 13 ? kSoft / 32 : i == 20 ? kSoft : i >= 16 && i < 20 ? kRows / 32 : 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        for (int i = 0; i < 2; i++) mbar_expect_tx(r_full + i * 8, 32 * 256 * vp);
     }
+    if (tid < 2) asm volatile("prefetch.tensormap [%0];" ::"l"(pp.maps[tid]) : "memory");
     pdl_wait();
     const int rep = p.heads / p.kv_heads, tq = kRows / rep;
     int seq, first;
@@ -198,8 +216,8 @@ template <bool CAPPED, int KEYS> __global__ void __launch_bounds__(Shape<KEYS>::
     const unsigned tmem = *tmem_slot, t_sum = tmem + 2 * KEYS;
     const int kt0 = low / KEYS, n = last / KEYS + 1 - kt0;
     bool ok = true;
-    // Waits until the products of tile i are in the sums. Tiles take turns at two barriers, and who asks has not let the products of tile i + 2 begin: the barrier cannot be a round
-    // ahead. Nor can it be two behind: each tile is asked for in its turn.
+    // Waits until the products of tile i are in the sums. Tiles take turns at two barriers, and who asks has seen the scores of tile i + 1 (or i, the last) and not let the products of
+    // tile i + 2 begin. Products are done in the order of their issue, those of tile i − 1 in front of the scores of tile i + 1: the barrier is neither a round behind nor ahead.
     auto added = [&](int i) { return mbar_wait(o_done + (i & 1) * 8, (unsigned)(i >> 1) & 1); };
     // Whether some row of the CTA may see keys of half h of the tile that begins at j0. Halves that nobody sees are neither copied nor multiplied.
     auto seen = [&](int j0, int h) { return j0 + h * kPart <= last && j0 + h * kPart + kPart > low; };
@@ -298,13 +316,12 @@ template <bool CAPPED, int KEYS> __global__ void __launch_bounds__(Shape<KEYS>::
     }
     if (warp < kCopies) {
         const int shift = kp + 2, chunks = 1 << (shift + 1), c = tid & (chunks - 1), part = c >> shift, d = c - (part << shift);  // kp is 1 or 2
-        const bf16* src = (const bf16*)p.q + ((((long long)(sq.start + first) * p.heads + g * rep) * 2 + map) * 2 + part) * p.dim + d * 8;
+        const bf16* src = (const bf16*)p.q + (((g * p.rows + sq.start + first) * rep * 2 + map) * 2 + part) * p.dim + d * 8;
         const unsigned to = sq0 + part * low0 + (d >> 3) * kPanelQ;
 #pragma unroll 8
         for (int row = tid / chunks; row < kRows; row += kSoft / chunks) {
-            const int t = token_of(row), h = row - t * rep;
-            const bool live = t < n_tok && d * 8 < p.dim;
-            cp_async16(to + row * 128 + (((d & 7) ^ (row & 7)) << 4), live ? src + ((long long)t * p.heads + h) * 4 * p.dim : (const bf16*)p.q, live);
+            const bool live = row < n_tok * rep && d * 8 < p.dim;
+            cp_async16(to + row * 128 + (((d & 7) ^ (row & 7)) << 4), live ? src + row * 4 * p.dim : (const bf16*)p.q, live);
         }
         cp_async_commit();
         cp_async_wait<0>();
@@ -325,7 +342,7 @@ template <bool CAPPED, int KEYS> __global__ void __launch_bounds__(Shape<KEYS>::
         const int pos = tok < n_tok ? pos0 + tok : last, mine_low = first_key(p, pos), last_low = first_key(p, last);  // rows without a token compute something harmless
         const float cap2 = p.cap2;
         float m = -1e30f;  // below every score, and finite: differences stay numbers
-        f32x2 l2 = pair_of(0.f, 0.f);  // the sum of even keys' weights and that of odd ones'
+        float sums[4] = {};  // of every fourth key's weights each
         int halves = 0;                       // of the values, in front of this thread's
         for (int i = 0; i < n; i++) {
             const int j0 = (kt0 + i) * KEYS, j1 = j0 + part * kPart;
@@ -356,7 +373,8 @@ template <bool CAPPED, int KEYS> __global__ void __launch_bounds__(Shape<KEYS>::
                 top = fmaxf(top, m);
                 const float keep = ex2(m - top);
                 m = top;
-                l2 = mul2(l2, pair_of(keep, keep));
+#pragma unroll
+                for (int e = 0; e < 4; e++) sums[e] *= keep;
                 if (i > 0) {
                     if (ok && !added(i - 1)) ok = false;
                     after_sync();
@@ -371,9 +389,8 @@ template <bool CAPPED, int KEYS> __global__ void __launch_bounds__(Shape<KEYS>::
                     }
                 }
             }
-            if (i >= 2 && ok && !added(i - 2)) ok = false;  // these weights' place
-            after_sync();
             const int before = kHalves == 2 && part == 1 && seen(j0, 0);  // the other half's values come first
+            // (these weights' place is free: with the scores of tile i the products of tile i − 2 are done)
             if (seen(j0, part)) {
                 const f32x2 behind = pair_of(-m, -m);
 #pragma unroll
@@ -384,8 +401,9 @@ template <bool CAPPED, int KEYS> __global__ void __launch_bounds__(Shape<KEYS>::
                         float a, b;
                         apart(add2(pair_of(s[c * 32 + 2 * e], s[c * 32 + 2 * e + 1]), behind), a, b);
                         w[e] = pack_bf16(ex2(a), ex2(b));
-                        // the sums of the weights as they are multiplied: the rounding of a weight that stands out is in both
-                        l2 = add2(l2, pair_of(__uint_as_float(w[e] << 16), __uint_as_float(w[e] & 0xFFFF0000u)));
+                        // The sums of the weights as they are multiplied: the rounding of a weight that stands out is in both. Adding bf16 to f32 as they are, four sums at a time, 64 keys of
+                        // a row take 660 cycles, of which the exponentials need 512; unpacked, two sums, 900.
+                        add_bf16(sums[(e & 1) * 2], sums[(e & 1) * 2 + 1], w[e]);
                     }
                     tmem_st16(tmem + lanes + KEYS + (i & 1) * (KEYS / 2) + part * (kPart / 2) + c * 16, w);
                 }
@@ -406,9 +424,9 @@ template <bool CAPPED, int KEYS> __global__ void __launch_bounds__(Shape<KEYS>::
             if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(w_full + (i & 1) * 16 + part * 8) : "memory");
             halves += seen(j0, 0) + (kHalves == 2 && seen(j0, 1));
         }
-        float l, odd;
-        apart(l2, l, odd);
-        l += odd;
+        __syncwarp();
+        cluster_arrive();  // the last scores are there: nothing reads queries and keys any more
+        float l = (sums[0] + sums[1]) + (sums[2] + sums[3]);
         if (kHalves == 2) l += both(n & 1, l);
         if (ok && !added(n - 1)) ok = false;
         after_sync();
@@ -418,72 +436,97 @@ template <bool CAPPED, int KEYS> __global__ void __launch_bounds__(Shape<KEYS>::
             f = keep / (l * keep + ex2(-top));
         }
         if (map) f *= p.lambda[head];
+        __syncwarp();
+    } else {
+        cluster_arrive();
     }
-    // Copies and products of both CTAs are done: their places take the other CTA's rows, [64][vdim + 4] in f32.
-    cluster_meet();
-    const int stride = vp * 64 + 4;
-    const unsigned mine = sq0 + (r & 63) * stride * 4;
-    const bool keeps = (r >> 6) == map;  // CTA 0 has the first 64 rows
+    // A CTA's other 64 rows, [row][vp · 64] in f32, neighbouring rows' sixteen bytes in different banks, go where the other one's queries and keys were: 32 rows a copy, while both still
+    // have something to do.
+    cluster_wait();
+    const unsigned long_row = vp * 256, mine = (r & 63) * long_row;
+    auto place = [&](int row, int c) { return (unsigned)(((c >> 2) ^ (row & 7)) << 4); };  // of dimensions c … c + 3
+    const bool keeps = (r >> 6) == map;                                                    // CTA 0 has the first 64 rows
     if (warp < kCopies && !keeps) {
-        unsigned to;
-        asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(mine), "r"(map ^ 1));
-#pragma unroll 2
+#pragma unroll 1
         for (int c = part * 32; c < vp * 64; c += 32 * kHalves) {
             unsigned v[32];
             tmem_ld32(v, t_sum + lanes + c);
             tmem_ld_wait();
 #pragma unroll
             for (int e = 0; e < 32; e += 4)
-                asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(to + (c + e) * 4), "f"(__uint_as_float(v[e]) * f), "f"(__uint_as_float(v[e + 1]) * f),
+                asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(sv + mine + place(r, c + e)), "f"(__uint_as_float(v[e]) * f), "f"(__uint_as_float(v[e + 1]) * f),
                              "f"(__uint_as_float(v[e + 2]) * f), "f"(__uint_as_float(v[e + 3]) * f)
                              : "memory");
         }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        if (kHalves == 2)
+            asm volatile("bar.sync %0, 64;" ::"r"(1 + (warp & 3)) : "memory");
+        else
+            __syncwarp();
+        if (part == 0 && lane == 0)
+            asm volatile("cp.async.bulk.shared::cluster.shared::cta.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(of_cta(sq0 + mine, map ^ 1)), "r"(sv + mine), "r"(32 * long_row),
+                         "r"(of_cta(r_full + (warp & 1) * 8, map ^ 1))
+                         : "memory");
+        __syncwarp();
     }
     // a row is written by neighbouring lanes, sixteen bytes each
     const int wide = p.vdim > 128 ? 32 : 16, wc = (tid & (wide - 1)) * 8;
     float gain[8];
 #pragma unroll
     for (int e = 0; e < 8; e++) gain[e] = p.gain && wc < p.vdim ? p.gain[wc + e] : 1.f;
-    cluster_meet();
     if (warp < kCopies && keeps) {
-        float* row = reinterpret_cast<float*>(smem + (mine - sq0));
+        if (!mbar_wait(r_full + (warp & 1) * 8, 0)) ok = false;
         const float sign = map ? -1.f : 1.f;
         float ss = 0.f;
-#pragma unroll 2
+#pragma unroll 1
         for (int c = part * 32; c < vp * 64; c += 32 * kHalves) {
             unsigned v[32];
             tmem_ld32(v, t_sum + lanes + c);
+            float4 theirs[8];
+#pragma unroll
+            for (int e = 0; e < 32; e += 4) theirs[e / 4] = *reinterpret_cast<const float4*>(smem + mine + place(r, c + e));
             tmem_ld_wait();
 #pragma unroll
             for (int e = 0; e < 32; e += 4) {
-                float4 o = *reinterpret_cast<float4*>(row + c + e);
+                float4 o = theirs[e / 4];
                 o.x = (__uint_as_float(v[e]) * f - o.x) * sign;
                 o.y = (__uint_as_float(v[e + 1]) * f - o.y) * sign;
                 o.z = (__uint_as_float(v[e + 2]) * f - o.z) * sign;
                 o.w = (__uint_as_float(v[e + 3]) * f - o.w) * sign;
                 ss = fmaf(o.x, o.x, fmaf(o.y, o.y, fmaf(o.z, o.z, fmaf(o.w, o.w, ss))));  // dimensions that are padding are 0
-                *reinterpret_cast<float4*>(row + c + e) = o;
+                *reinterpret_cast<float4*>(smem + mine + place(r, c + e)) = o;
             }
         }
-        if (kHalves == 2) ss += both(0, ss);
+        if (kHalves == 2) ss += both((n + 1) & 1, ss);
         scales[r & 63] = p.gain ? 1.f / sqrtf(ss / (float)p.vdim + p.head_eps) : 1.f;
     }
     before_sync();
     __syncthreads();
     after_sync();
+    cluster_arrive();  // this CTA has what the other one sent
     if (warp < kCopies && wc < p.vdim) {
-#pragma unroll 4
-        for (int i = tid / wide; i < 64; i += kSoft / wide) {
-            const int at = map * 64 + i, t = token_of(at);
-            const float* row = reinterpret_cast<const float*>(smem) + i * stride + wc;
-            const float4 a = *reinterpret_cast<const float4*>(row), b = *reinterpret_cast<const float4*>(row + 4);
-            const float x = scales[i];
-            if (t < n_tok && ok)
-                *reinterpret_cast<uint4*>((bf16*)p.out + ((sq.start + first + t) * (long long)p.heads + g * rep + at - t * rep) * p.vdim + wc) =
-                    make_uint4(pack_bf16(a.x * x * gain[0], a.y * x * gain[1]), pack_bf16(a.z * x * gain[2], a.w * x * gain[3]), pack_bf16(b.x * x * gain[4], b.y * x * gain[5]),
-                               pack_bf16(b.z * x * gain[6], b.w * x * gain[7]));
+#pragma unroll 1
+        for (int i0 = tid / wide; i0 < 64; i0 += 4 * (kSoft / wide)) {
+            float4 a[4], b[4];
+#pragma unroll
+            for (int u = 0; u < 4; u++) {
+                const int i = i0 + u * (kSoft / wide);
+                a[u] = *reinterpret_cast<const float4*>(smem + i * long_row + place(i, wc));
+                b[u] = *reinterpret_cast<const float4*>(smem + i * long_row + place(i, wc + 4));
+            }
+#pragma unroll
+            for (int u = 0; u < 4; u++) {
+                const int i = i0 + u * (kSoft / wide), at = map * 64 + i, t = token_of(at);
+                const float x = scales[i];
+                if (t < n_tok && ok)
+                    *reinterpret_cast<uint4*>((bf16*)p.out + ((sq.start + first + t) * (long long)p.heads + g * rep + at - t * rep) * p.vdim + wc) =
+                        make_uint4(pack_bf16(a[u].x * x * gain[0], a[u].y * x * gain[1]), pack_bf16(a[u].z * x * gain[2], a[u].w * x * gain[3]),
+                                   pack_bf16(b[u].x * x * gain[4], b[u].y * x * gain[5]), pack_bf16(b[u].z * x * gain[6], b[u].w * x * gain[7]));
+            }
         }
     }
+    __syncwarp();
+    cluster_wait();  // no CTA leaves while its rows are on their way
     if (!ok && lane == 0) report(p.err, ERR_WAIT_TIMEOUT, p.node, (long long)blockIdx.x, (long long)warp);
     if (warp == kIssues) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(cols) : "memory");
 }

@@ -296,9 +296,6 @@ template <int DM, int DV> __global__ void __launch_bounds__(kDecThreads) differe
     const int page0 = from >> p.shift, n_pages = from < hi ? ((hi - 1) >> p.shift) - page0 + 1 : 0;
     for (int i = tid; i < min(n_pages, kDecPages); i += kDecThreads) page_s[i] = (int)page_of(p, seq, (page0 + i) << p.shift);
     const bool newest = hi == pos + 1 && lo < hi;  // this CTA's keys include the new one
-    float *short_cs = reinterpret_cast<float*>(sn + DM / 2), *short_sn = short_cs + DM / 2;
-    if (sq.len == 1 && warp < 2) short_angles(p, pos, short_cs, short_sn, tid, 64);
-    if (newest && warp >= 2) exact_angles(p, pos, cs, sn, tid - 64, 64);
     __syncthreads();
     auto page_at = [&](int j) {
         const int i = (j >> p.shift) - page0;
@@ -351,7 +348,12 @@ template <int DM, int DV> __global__ void __launch_bounds__(kDecThreads) differe
 #pragma unroll
         for (int i = 0; i < L::stages - 1; i++) load_tile(i);
     };
-    if (!newest) fill();
+    // The first tiles are on their way while the launch before this one ends, unless the new key is among them.
+    const bool late = newest && (pos - lo) / step < L::stages - 1;
+    if (!late) fill();
+    float *short_cs = reinterpret_cast<float*>(sn + DM / 2), *short_sn = short_cs + DM / 2;
+    if (sq.len == 1 && warp < 2) short_angles(p, pos, short_cs, short_sn, tid, 64);
+    if (newest && warp >= 2) exact_angles(p, pos, cs, sn, tid - 64, 64);
     pdl_wait();
     if (sq.len != 1) {
         if (p.only && sq.len > 1 && tid == 0) report(p.err, ERR_BATCH_ROWS, p.node, seq, sq.len);
@@ -384,7 +386,7 @@ template <int DM, int DV> __global__ void __launch_bounds__(kDecThreads) differe
         const float f = map_factor(p, k);
         for (int i = lane + (warp & 1) * 32; i < dim; i += 64) keys[(row * 2 + m) * dim + i] = __float2bfloat16_rn((float)(turned(p, k, cs, sn, i) * f));
         __syncthreads();
-        fill();
+        if (late) fill();
     }
     auto put = [&](bf16* to, int i, float v) {
         const bf16 high = __float2bfloat16_rn(v);
@@ -620,15 +622,16 @@ void emit_differential(Emitter& em, const DifferentialDesc& d, const TRef& proj,
     if (tc && (p.only || n_seqs > 1)) {
         const DecChoice dc = d.dim <= 32 ? choice<32>(d.vdim) : d.dim <= 64 ? choice<64>(d.vdim) : choice<128>(d.vdim);
         const int64_t groups = d.kv_heads * ((d.heads / d.kv_heads + kDecHeads - 1) / kDecHeads), cells = n_seqs * groups;
-        // splits of the most keys a sequence can see: whole waves of resident CTAs, each with a fixed cost worth about
-        // 160 keys, and the pieces have to be merged
+        // Splits of the most keys a sequence can see: whole waves of resident CTAs, and the pieces have to be merged. A CTA's beginning and end cost as much as 200 KB of keys and values
+        // (64 sequences behind 2047, 32 heads of 2 x 64 over 16, us for 1, 2, 4, 8 splits: 223, 246, 291, 369; four that see 4096 keys: 90, 60, 52, 58).
         const int64_t resident = std::max<int64_t>(1, std::min<int64_t>(3, 224 * 1024 / (dc.smem + 2560))), slots = resident * sm_count();
         int64_t seen = (int64_t)p.width * d.page;
         if (d.window > 0) seen = std::min<int64_t>(seen, d.window + 64);
         int64_t splits = 1;
+        const double fixed = 100.0 * 1024.0 / (2 * d.dim + d.vdim);
         double best = 1e300;
         for (int64_t sp = 1; sp <= 64 && sp * 64 <= std::max<int64_t>(seen, 64); sp++) {
-            const double us = (double)((cells * sp + slots - 1) / slots) * ((double)seen / sp + 160.0) + 4.0 * sp;
+            const double us = (double)((cells * sp + slots - 1) / slots) * ((double)seen / sp + fixed) + 4.0 * sp;
             if (us < best) {
                 best = us;
                 splits = sp;

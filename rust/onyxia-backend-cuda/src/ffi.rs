@@ -146,6 +146,17 @@ pub struct ox_engine_entry {
 }
 
 #[repr(C)]
+pub struct ox_logit_rules {
+    pub history: *const ox_tensor,
+    pub lengths: *const ox_tensor,
+    pub penalties: *const ox_tensor,
+    pub bias_ids: *const ox_tensor,
+    pub bias: *const ox_tensor,
+    pub masks: *const ox_tensor,
+    pub mask_of: *const ox_tensor,
+}
+
+#[repr(C)]
 pub struct ox_engine_token {
     pub request: i64,
     pub token: i64,
@@ -205,6 +216,11 @@ unsafe extern "C" {
     pub fn ox_session_argmax_last(s: *mut ox_session, logits: *const ox_tensor, out: *mut *mut ox_tensor) -> i32;
     pub fn ox_session_sample_last(s: *mut ox_session, logits: *const ox_tensor, temperature: f32, top_k: i64, top_p: f32,
                                   uniform: *const f32, n_uniform: usize, out: *mut *mut ox_tensor) -> i32;
+    pub fn ox_session_upload_device(s: *mut ox_session, dtype: i32, shape: *const u64, rank: i32, device_bytes: *const c_void, nbytes: usize,
+                                    stream: *mut c_void, out: *mut *mut ox_tensor) -> i32;
+    pub fn ox_session_device_view(s: *mut ox_session, t: *const ox_tensor, stream: *mut c_void, device_ptr: *mut *mut c_void) -> i32;
+    pub fn ox_session_after_stream(s: *mut ox_session, stream: *mut c_void) -> i32;
+    pub fn ox_session_constrain_last(s: *mut ox_session, logits: *const ox_tensor, rules: *const ox_logit_rules, out: *mut *mut ox_tensor) -> i32;
     pub fn ox_session_argmax_last_into(s: *mut ox_session, logits: *const ox_tensor, out: *mut ox_tensor) -> i32;
 
     pub fn ox_llm_create(s: *mut ox_session, max_seq_len: i64, out: *mut *mut ox_llm) -> i32;
@@ -228,5 +244,8 @@ unsafe extern "C" {
                             top_p: f32, seed: u64, request: *mut i64) -> i32;
     pub fn ox_engine_step(e: *mut ox_engine, token_budget: i32, tokens: *mut ox_engine_token, cap: i32, n_tokens: *mut i32) -> i32;
     pub fn ox_engine_cancel(e: *mut ox_engine, request: i64) -> i32;
+    pub fn ox_engine_constrain(e: *mut ox_engine, request: i64, repetition: f32, frequency: f32, presence: f32, bias_ids: *const i32,
+                               bias: *const f32, n_bias: i32) -> i32;
+    pub fn ox_engine_allow(e: *mut ox_engine, request: i64, allowed: *const u32, n_words: usize) -> i32;
     pub fn ox_engine_stats(e: *const ox_engine, out: *mut i64);
 }

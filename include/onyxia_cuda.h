@@ -253,7 +253,7 @@ ox_status ox_session_upload_device(ox_session*, int32_t dtype, const uint64_t* s
  * in the reference). What is enqueued on `stream` after the call runs behind everything the session has enqueued so
  * far. The address is good while a handle of the tensor is held; before the last one is released, and before the
  * session is to read what `stream` has written there, ox_session_after_stream orders the session's later work behind
- * `stream`. */
+ * `stream`. A stream that is being captured into a graph is refused by all three. */
 ox_status ox_session_device_view(ox_session*, const ox_tensor*, void* stream, void** device_ptr);
 ox_status ox_session_after_stream(ox_session*, void* stream);
 /* ≙ Session::run: inputs matched by name against the module signature; all
@@ -428,7 +428,8 @@ ox_status ox_engine_step(ox_engine*, int32_t token_budget, ox_engine_token* toke
 ox_status ox_engine_cancel(ox_engine*, int64_t request);
 /* Rules on the tokens that an unfinished request has still to generate, as ox_session_constrain_last applies them: its history is its prompt
  * and what it has generated. Each call replaces what the one before it said. `allowed` has a bit per token of the vocabulary
- * (ceil(vocab / 32) words, lowest bit first), at least one of them set; NULL allows all again. A grammar sets it before every step. */
+ * (ceil(vocab / 32) words, lowest bit first), at least one of them set; NULL allows all again. A grammar sets it before every step. Biases (each a number, or minus infinity) and
+ * allowed tokens have to leave one. */
 ox_status ox_engine_constrain(ox_engine*, int64_t request, float repetition, float frequency, float presence, const int32_t* bias_ids,
                               const float* bias, int32_t n_bias);
 ox_status ox_engine_allow(ox_engine*, int64_t request, const uint32_t* allowed, size_t n_words);

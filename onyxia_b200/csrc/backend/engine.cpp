@@ -214,6 +214,17 @@ Engine::Request& Engine::request_of(int64_t id) {
     fail(ErrKind::Binding, "no unfinished request " + std::to_string(id));
 }
 
+// Whether some token of `vocab` is allowed and has not minus infinity for its bias.
+static bool leaves_a_token(const Engine::Rules& r, int64_t vocab) {
+    std::vector<int32_t> barred;
+    for (size_t i = 0; i < r.bias.size(); i++)
+        if (r.bias[i] == -INFINITY && (r.allowed.empty() || (r.allowed[(size_t)r.bias_ids[i] / 32] >> (r.bias_ids[i] % 32) & 1u))) barred.push_back(r.bias_ids[i]);
+    std::sort(barred.begin(), barred.end());
+    int64_t left = r.allowed.empty() ? vocab : 0;
+    for (uint32_t w : r.allowed) left += __builtin_popcount(w);
+    return left > std::unique(barred.begin(), barred.end()) - barred.begin();
+}
+
 void Engine::constrain(int64_t request, float repetition, float frequency, float presence, std::vector<int32_t> bias_ids, std::vector<float> bias) {
     Request& r = request_of(request);
     if (!(repetition > 0.f) || !std::isfinite(repetition)) fail(ErrKind::Attribute, "a repetition penalty is a factor above 0");
@@ -223,8 +234,9 @@ void Engine::constrain(int64_t request, float repetition, float frequency, float
         if (bias_ids[i] < 0 || bias_ids[i] >= vocab_) fail(ErrKind::Shape, "a bias of token " + std::to_string(bias_ids[i]) + ", which is not one of " + std::to_string(vocab_));
         if (std::isnan(bias[i]) || bias[i] == INFINITY) fail(ErrKind::Attribute, "a bias is a number, or minus infinity");
     }
-    r.rules.repetition = repetition, r.rules.frequency = frequency, r.rules.presence = presence;
-    r.rules.bias_ids = std::move(bias_ids), r.rules.bias = std::move(bias);
+    Rules rules{repetition, frequency, presence, std::move(bias_ids), std::move(bias), r.rules.allowed};
+    if (!leaves_a_token(rules, vocab_)) fail(ErrKind::Shape, "the biases leave no token");
+    r.rules = std::move(rules);
 }
 
 void Engine::allow(int64_t request, std::vector<uint32_t> allowed) {
@@ -234,7 +246,11 @@ void Engine::allow(int64_t request, std::vector<uint32_t> allowed) {
         if (vocab_ % 32) allowed.back() &= (1u << (vocab_ % 32)) - 1;
         if (std::all_of(allowed.begin(), allowed.end(), [](uint32_t w) { return w == 0; })) fail(ErrKind::Shape, "the mask allows no token");
     }
-    r.rules.allowed = std::move(allowed);
+    allowed.swap(r.rules.allowed);
+    if (!leaves_a_token(r.rules, vocab_)) {
+        allowed.swap(r.rules.allowed);
+        fail(ErrKind::Shape, "the mask and the biases leave no token");
+    }
 }
 
 // The rows' logits under their requests' rules; those of a batch without any are left alone.
@@ -437,6 +453,7 @@ ox_status ox_engine_constrain(ox_engine* h, int64_t request, float repetition, f
 
 ox_status ox_engine_allow(ox_engine* h, int64_t request, const uint32_t* allowed, size_t n_words) {
     OX_TRY
+    if (allowed && n_words == 0) ox::fail(ox::ErrKind::Shape, "a mask of no words");
     h->e->allow(request, allowed ? std::vector<uint32_t>(allowed, allowed + n_words) : std::vector<uint32_t>());
     return OX_OK;
     OX_CATCH

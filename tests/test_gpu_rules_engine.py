@@ -137,6 +137,25 @@ def test_rules_that_are_refused():
             e.allow(r, bad)
     with pytest.raises(OnyxiaError, match="no unfinished request"):
         e.allow(r + 1, [3])
+    # biases and a mask that together leave nothing
+    bar = {t: -float("inf") for t in range(131)}
+    with pytest.raises(OnyxiaError, match="leave no token"):
+        e.constrain(r, bias=bar)
+    e.constrain(r, bias={t: -float("inf") for t in range(130)})
+    for bad in ([5], [5, 129]):
+        with pytest.raises(OnyxiaError, match="leave no token"):
+            e.allow(r, bad)
+    e.allow(r, [5, 130])
+    with pytest.raises(OnyxiaError, match="leave no token"):
+        e.constrain(r, bias={5: -float("inf"), 130: -float("inf")})
+    word = np.ones(5, np.uint32)
+    from onyxia_b200 import _ffi
+    import ctypes
+    assert _ffi.cuda_lib().ox_engine_allow(e._h, r, word.ctypes.data_as(ctypes.POINTER(ctypes.c_uint32)), 0) != 0
+    answer = []
+    while len(answer) < 3:
+        answer += [t for q, t, _ in e.step() if q == r]
+    assert answer == [130] * 3
     assert len(e.generate([tokens(4, 1)], 3)[0]) == 3  # and the engine goes on
     with pytest.raises(OnyxiaError, match="no unfinished request"):
         e.constrain(r, repetition=1.1)

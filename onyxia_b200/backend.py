@@ -64,7 +64,8 @@ class DeviceTensor:
 
 class DeviceView:
     """Memory of a tensor as ``__cuda_array_interface__`` (``torch.as_tensor`` and others take it without a copy); bf16 as whole
-    numbers of 16 bits. The view keeps the tensor; when it goes, the session's later work is ordered behind the view's stream."""
+    numbers of 16 bits. The view keeps the tensor; when it goes, the session's later work is ordered behind the view's stream, which has
+    to live as long."""
 
     def __init__(self, session: "CudaSession", t: DeviceTensor, stream: int):
         dtype, shape = t.describe()

@@ -624,7 +624,9 @@ bool differential_accepts(const Module& m, const Node& n) {
     if (a.int_or("window", 0) < 0 || a.int_or("window", 0) > INT32_MAX) return false;
     for (const char* f : {"softcap", "epsilon", "head_epsilon"})
         if (!(a.float_or(f, 0.0) >= 0.0) || !std::isfinite(a.float_or(f, 0.0))) return false;
-    if (!std::isfinite(a.float_or("scale", 1.0))) return false;
+    // (in f32, and in the quotient that scores are multiplied by, too)
+    const double scale = std::fabs(a.float_or("scale", 1.0)), cap = a.float_or("softcap", 0.0);
+    if (!(scale <= 1e30) || cap > 1e30 || (cap > 0.0 && scale > 1e30 * cap)) return false;
     const TensorType &x = ty(m, n.inputs[0]), &turns = ty(m, n.inputs[1]), &keys = ty(m, n.inputs[2]), &values = ty(m, n.inputs[3]);
     const TensorType &seqs = ty(m, n.inputs[4]), &pages = ty(m, n.inputs[5]), &out = ty(m, n.outputs[0]);
     auto width = x.shape.size() == 2 ? x.shape[1].as_const() : std::nullopt;

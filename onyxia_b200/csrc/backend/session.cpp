@@ -724,6 +724,16 @@ std::vector<DTensor> Session::upload_together(const std::vector<HostPart>& parts
     return out;
 }
 
+// The session's allocations and waits are not for a graph that a caller records.
+static void check_not_captured(cudaStream_t stream) {
+    cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+    if (cudaStreamIsCapturing(stream, &status) != cudaSuccess) {
+        cudaGetLastError();
+        fail(ErrKind::Runtime, "the stream is not one of this process's, or legacy while another one is captured");
+    }
+    if (status != cudaStreamCaptureStatusNone) fail(ErrKind::Runtime, "the stream is being captured into a graph");
+}
+
 // What is enqueued on `then` from now on runs behind what is on `first` by now.
 void Session::order(cudaStream_t first, cudaStream_t then) {
     if (!ev_order_) OX_CUDA(cudaEventCreateWithFlags(&ev_order_, cudaEventDisableTiming));
@@ -746,6 +756,7 @@ DTensor Session::upload_device(DType dtype, const std::vector<int64_t>& shape, c
         if (err != cudaSuccess || (at.type != cudaMemoryTypeDevice && at.type != cudaMemoryTypeManaged) || (at.type == cudaMemoryTypeDevice && at.device != device_))
             fail(ErrKind::Runtime, "the bytes are not memory of the session's device");
     }
+    check_not_captured(stream);
     t.buf = pool_->alloc(nbytes ? nbytes : 1);
     if (!nbytes) return t;
     order(stream, stream_);
@@ -758,12 +769,14 @@ void* Session::device_view(const DTensor& t, cudaStream_t stream) {
     OX_CUDA(cudaSetDevice(device_));
     if (!t.buf) fail(ErrKind::Runtime, "not a device tensor of this backend");
     if (t.cap && t.shape.size() == 4 && t.cap != t.shape[2]) fail(ErrKind::Shape, "a view needs a densely packed tensor");
+    check_not_captured(stream);
     order(stream_, stream);
     return t.ptr();
 }
 
 void Session::after_stream(cudaStream_t stream) {
     OX_CUDA(cudaSetDevice(device_));
+    check_not_captured(stream);
     order(stream, stream_);
 }
 
@@ -803,6 +816,7 @@ void Session::check_device_error() {
         case oxk::ERR_RULES_LENGTH: what = "rules: the lengths of row " + std::to_string(e.a) + " do not fit a history of " + std::to_string(e.b); break;
         case oxk::ERR_RULES_MASK: what = "rules: mask " + std::to_string(e.a) + " is not one of " + std::to_string(e.b); break;
         case oxk::ERR_BATCH_ROWS: what = "sequence " + std::to_string(e.a) + " has " + std::to_string(e.b) + " new tokens in a batch of no more rows than sequences"; break;
+        case oxk::ERR_BATCH_SEQ: what = "sequence " + std::to_string(e.a) + " does not lie in the rows of the batch, or its " + std::to_string(e.b) + " positions not in the page table"; break;
         default: what = "device error code " + std::to_string(e.code);
     }
     fail(ErrKind::Runtime, kind + " (node '" + node + "'): " + what);

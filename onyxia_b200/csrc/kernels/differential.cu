@@ -24,7 +24,8 @@ template <typename T> __global__ void __launch_bounds__(128) differential_prepar
     extern __shared__ double angle[];  // cos[half], sin[half]
     pdl_enter();
     const int row = blockIdx.x, s = find_seq(p.seqs, p.n_seqs, row), lane = threadIdx.x & 31;
-    const SeqRow sq = load_seq(p.seqs, s);
+    const SeqRow sq = checked_seq(p, s);
+    check_others(p, row, threadIdx.x, 128);
     const int pos = sq.past + row - sq.start;
     if (row < sq.start || row >= sq.start + sq.len || (sq.len == 1 && !p.singles)) return;
     exact_angles(p, pos, angle, angle + p.half, threadIdx.x, 128);
@@ -67,7 +68,8 @@ __global__ void __launch_bounds__(128, 8) differential_prepare8(const DiffP p) {
     fetch(p.k_off, 2 * p.kv_heads * p.dim);
     fetch(p.v_off, p.kv_heads * p.vdim);
     const int s = find_seq(p.seqs, p.n_seqs, row);
-    const SeqRow sq = load_seq(p.seqs, s);
+    const SeqRow sq = checked_seq(p, s);
+    check_others(p, row, tid, 128);
     const int pos = sq.past + row - sq.start, maps = 2 * (p.heads + p.kv_heads);
     if (row < sq.start || row >= sq.start + sq.len || (sq.len == 1 && !p.singles)) return;
     float* short_angle = reinterpret_cast<float*>(angle + 2 * p.half);
@@ -159,7 +161,7 @@ template <typename T> __global__ void __launch_bounds__(kAnyKeys) differential_s
     __shared__ float red[32];
     pdl_enter();
     const int row = blockIdx.x, h = blockIdx.y, tid = threadIdx.x, s = find_seq(p.seqs, p.n_seqs, row);
-    const SeqRow sq = load_seq(p.seqs, s);
+    const SeqRow sq = checked_seq(p, s);
     if (row < sq.start || row >= sq.start + sq.len || (sq.len == 1 && !p.singles)) return;
     const int pos = sq.past + row - sq.start, g = h / (p.heads / p.kv_heads);
     float *q = sm, *acc = sm + 2 * p.dim, *w = acc + 2 * p.vdim;
@@ -280,7 +282,7 @@ template <int DM, int DV> __global__ void __launch_bounds__(kDecThreads) differe
     // no launch of a step writes the batch description or the keys and values of earlier steps: they may be read while the
     // launches before this one finish
     const int seq = blockIdx.z;
-    const SeqRow sq = load_seq(p.seqs, seq);
+    const SeqRow sq = checked_seq(p, seq);
     const int rep = p.heads / p.kv_heads, groups = (rep + kDecHeads - 1) / kDecHeads, g = blockIdx.y / groups, h0 = g * rep + (blockIdx.y % groups) * kDecHeads;
     const int n_heads = min(kDecHeads, (g + 1) * rep - h0), pos = sq.past, dim = p.dim, vdim = p.vdim;
     const bf16* x = (const bf16*)p.proj + (long long)sq.start * p.ld;

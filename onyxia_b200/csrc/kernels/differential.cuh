@@ -30,6 +30,20 @@ struct DiffP {
     unsigned by_rep, by_units, by_lanes;  // 2^32 / (heads of a key head, units of a query, sixteen bytes of a value), rounded up; 0: of one
 };
 
+// Sequence r of the batch. One whose rows are not the batch's, or whose positions the page table has no place for, is reported and has no rows.
+__device__ __forceinline__ SeqRow checked_seq(const DiffP& p, int r) {
+    SeqRow s = load_seq(p.seqs, r);
+    if (s.len != 0 && (s.start < 0 || s.len < 0 || s.past < 0 || s.start + (long long)s.len > p.rows || s.past + (long long)s.len > (long long)p.width << p.shift)) {
+        report(p.err, ERR_BATCH_SEQ, p.node, r, s.past + (long long)s.len);
+        s.len = 0;
+    }
+    return s;
+}
+// By the CTA of the batch's first row: what is wrong with a sequence that no row belongs to.
+__device__ __forceinline__ void check_others(const DiffP& p, int row, int tid, int threads) {
+    if (row == 0)
+        for (int i = tid; i < p.n_seqs; i += threads) checked_seq(p, i);
+}
 __device__ __forceinline__ int first_key(const DiffP& p, int pos) { return p.window > 0 ? max(0, pos - p.window + 1) : 0; }
 // log2 e · score of a dot product; tanh x = 1 − 2 / (1 + e^2x) is off by a few 1e-7 of the cap
 __device__ __forceinline__ float score2(const DiffP& p, float d) {
@@ -76,11 +90,11 @@ template <typename T> __device__ __forceinline__ float map_factor(const DiffP& p
 }
 
 // locate_tile, and the sequence that the tile belongs to: its row of the batch description comes with the count.
-__device__ __forceinline__ bool locate_rows(const int* seqs, int n_seqs, int tile, int tq, int least, int* seq, int* first, SeqRow* row) {
+__device__ __forceinline__ bool locate_rows(const DiffP& p, int tile, int tq, int least, int* seq, int* first, SeqRow* row) {
     const int lane = threadIdx.x & 31;
     int before = 0;
-    for (int r0 = 0; r0 < n_seqs; r0 += 32) {
-        const SeqRow mine = r0 + lane < n_seqs ? load_seq(seqs, r0 + lane) : SeqRow{0, 0, 0, 0};
+    for (int r0 = 0; r0 < p.n_seqs; r0 += 32) {
+        const SeqRow mine = r0 + lane < p.n_seqs ? checked_seq(p, r0 + lane) : SeqRow{0, 0, 0, 0};
         const int n = mine.len >= least ? (mine.len + tq - 1) / tq : 0;
         int inc = n;
 #pragma unroll

@@ -198,7 +198,7 @@ template <bool CAPPED, int KEYS> __global__ void __launch_bounds__(Shape<KEYS>::
     int seq, first;
     SeqRow sq;
     // long rows of all heads first: the last tiles of a sequence see the most keys
-    if (!locate_rows(p.seqs, p.n_seqs, pp.tiles - 1 - tile, tq, p.singles ? 1 : 2, &seq, &first, &sq)) return;  // both CTAs of the cluster
+    if (!locate_rows(p, pp.tiles - 1 - tile, tq, p.singles ? 1 : 2, &seq, &first, &sq)) return;  // both CTAs of the cluster
     const int n_tok = min(tq, sq.len - first), pos0 = sq.past + first, last = pos0 + n_tok - 1, low = first_key(p, pos0);
     // Scores in KEYS columns, weights in two turns of half as many, sums behind them. No more CTAs than have room in tensor memory may be on an SM at a time
     // (differential_smem), or two clusters could wait for what the other one has.

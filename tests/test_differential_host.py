@@ -70,3 +70,9 @@ def test_forms_that_are_refused(takes, changed):
 
 def test_sizes_above_what_a_block_holds_are_refused(takes):
     assert takes(Form(1, 1, 8193, 8)) == 0 and takes(Form(1, 1, 8, 8200)) == 0 and takes(Form(65536, 1, 1, 1)) == 0
+
+
+@pytest.mark.parametrize("changed", [{"scale": 1e31}, {"scale": -1e31}, {"softcap": 1e31}, {"softcap": 1e-31}, {"scale": float("inf")}], ids=str)
+def test_factors_that_f32_cannot_hold_are_refused(takes, changed):
+    assert takes(F, **changed) == 0
+    assert takes(F, scale=1e-30, softcap=1e-30) == 1 and takes(F, scale=-1e30) == 1

@@ -8,6 +8,8 @@ sqrt(1 + λ²) / sqrt(1 + λ²) where they are independent and up to (1 + λ) / 
 spread is 1.5 · factor · dim^1/2 and what the rounding of queries and keys does to the weights grows with it: both bounds are times the ratio of the factors (16 for a factor of 2 over
 64 dimensions: scores of a spread of 24 are off by 1.1e-3 · sqrt 2 · 24 = 3.7e-2).
 """
+import dataclasses
+
 import numpy as np
 import pytest
 
@@ -223,3 +225,35 @@ def test_views_and_uploads_of_device_memory():
     assert empty.shape == (0, 3) and torch.as_tensor(session.view(empty), device="cuda").shape == (0, 3)
     with pytest.raises(ValueError, match="4-bit"):
         session.view(session.upload(HostTensor.packed_u4(np.arange(8) % 16, (8,))))
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("lengths,row", [([(1, 200), (1, 3)], (1, 1, 2 ** 30, 1)), ([(1, 200), (1, 3)], (2, 1, 3, 1)), ([(40, 60), (7, 3)], (-1, 7, 3, 1)), ([(40, 60), (7, 3)], (40, 8, 3, 1)),
+                                         ([(40, 60), (7, 3)], (40, 7, -1, 1)), ([(40, 60), (7, 3)], (40, -7, 3, 1)), ([(40, 60), (7, 3)], (40, 7, 2 ** 31 - 1, 1))], ids=str)
+def test_a_sequence_that_does_not_lie_in_the_batch_is_reported(lengths, row, kind):
+    f = Form(4, 2, 64, 128, 64)
+    s = util.step(f, lengths, round_to=stored(kind))
+    good = dataclasses.replace(s, seqs=s.seqs.copy())
+    s.seqs[1] = row
+    session = cuda_backend().prepare(util.module(f, DTYPES[kind], s.lam, s.gain))
+    dev = {k: session.upload(v) for k, v in util.feed(s, act(kind)).items()}
+    outs = session.run(dev)
+    with pytest.raises(OnyxiaError, match="sequence 1 does not lie in"):
+        session.download(outs[0][1])
+    dev = {k: session.upload(v) for k, v in util.feed(good, act(kind)).items()}
+    compare(session.download(session.run(dev)[0][1]).numpy(), util.reference(f, good, stored(kind))[0], kind, good)
+
+
+def test_streams_that_are_captured_are_refused():
+    torch = pytest.importorskip("torch")
+    session = cuda_backend().prepare(util.module(Form(4, 2, 64, 128, 64), ir.BF16, np.ones(4, np.float32), np.ones(128, np.float32)))
+    t, x, side = session.upload(HostTensor.from_numpy(np.arange(6, dtype=np.float32))), torch.ones(6, device="cuda"), torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side, capture_error_mode="relaxed"):
+        y = x + 1
+        for call in (lambda: session.upload_device(ir.F32, (6,), x.data_ptr(), side.cuda_stream), lambda: session.view(t, side.cuda_stream)):
+            with pytest.raises(OnyxiaError, match="captured"):
+                call()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert np.array_equal(y.cpu().numpy(), np.full(6, 2.0)) and np.array_equal(session.download(t).numpy(), np.arange(6))

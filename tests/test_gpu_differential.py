@@ -257,3 +257,20 @@ def test_streams_that_are_captured_are_refused():
     graph.replay()
     torch.cuda.synchronize()
     assert np.array_equal(y.cpu().numpy(), np.full(6, 2.0)) and np.array_equal(session.download(t).numpy(), np.arange(6))
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_more_sequences_and_heads_than_places(kind):
+    """More CTAs than run at a time: the last round's are cut into pieces."""
+    lengths = [(1, 40 + 67 * i % 500) for i in range(40)]
+    check(Form(16, 16, 32, 64, 16), lengths, kind)
+    check(Form(16, 16, 64, 128, 64, window=300), lengths[:30], kind, seed=1)
+    check(Form(9, 9, 128, 256, 32), lengths[:20], kind, seed=2)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("cap", [1.0, 4.0, 9.0, 100.0])
+def test_caps(cap, kind):
+    """Scores far above the cap, near it, at half of it and far below."""
+    for f in (Form(4, 2, 64, 128, 64, softcap=cap), Form(4, 1, 128, 256, 128, softcap=cap)):
+        check(f, [(100, 150), (1, 90)], kind)

@@ -5,7 +5,11 @@
 // 4 products of 128 × vdim × 16 add their weights' share of the values. Keys and values come by TMA.
 // From the order to a product to the word that it is done it takes 400 cycles, more than most products themselves (N 64: 47, N 128: 62 each). So nothing waits for two in a row: scores have one
 // place, free as soon as they have been read, weights have two of their own, and the next scores are made, and the last weights multiplied, under the exponentials of these.
-// In the end each CTA sends the other half of its rows, divided by their sums, through the cluster's shared memory, and forms difference, norm and results of its own half.
+// In the end each CTA stages the other half of its rows, divided by their sums, copies them into the other's shared memory, and forms difference, norm and results of its own half.
+//
+// Measured alone, L2 cold: 4096 tokens, 32 heads of 2 × 64 over 16, values of 128 (137 GFLOP) 289 us, 476 TFLOP/s, 950 with the queries' low part and a product of the values per map;
+// 2048, 16 over 4 60 us; 1999 capped behind 1000, 4 heads of 2 × 128 over one 60 us. A step of 64 keys takes 1 600 cycles with two CTAs per SM: products need 640 of an SM's 800, exponentials
+// 512; what bounds it is their order within a CTA, and a third CTA has no tensor memory. A tile's beginning and end take 16 000 cycles, half of them under the other CTA's steps.
 #include "differential.cuh"
 
 namespace oxk {
@@ -169,7 +173,7 @@ struct PagesAhead {
 // KEYS 64: 256 columns of tensor memory (values of up to 128), two CTAs per SM, which work under each other's waits. 128: all columns.
 template <int KEYS> struct Shape {
     static constexpr int halves = KEYS / kPart, soft = halves * kRows, threads = soft + 64;  // softmax warps, one of copies, one that issues products
-    static constexpr int keys = KEYS == 64 ? 3 : 2, values = KEYS == 64 ? 3 : 2;           // tiles of keys and halves of values on their way
+    static constexpr int keys = KEYS == 64 ? 3 : 2, values = KEYS == 64 ? 3 : 2;             // tiles of keys and halves of values on their way
 };
 template <bool CAPPED, int KEYS> __global__ void __launch_bounds__(Shape<KEYS>::threads, KEYS == 64 ? 2 : 1) differential_prefill(const __grid_constant__ PreP pp) {
     extern __shared__ __align__(1024) unsigned char smem_raw[];
@@ -182,7 +186,8 @@ template <bool CAPPED, int KEYS> __global__ void __launch_bounds__(Shape<KEYS>::
     constexpr unsigned kPanelK = KEYS * 128;
     const unsigned k_stage = kp * kPanelK, v_stage = vp * kPanelV;
     const unsigned sq0 = smem_u32(smem), low0 = kp * kPanelQ, sk = sq0 + 2 * low0, sv = sk + kStagesK * k_stage, bars = sv + kStagesV * v_stage;
-    // barriers: keys there, free, values there, free (three each), scores there, read, products added (one, one and two), weights there (two halves of two), queries there, rows of the other CTA there (two warps')
+    // barriers: keys there, free, values there, free (three each), scores there, read, products added (one, one and two), weights there (two halves of two), queries there, rows of the
+    // other CTA there (two warps')
     const unsigned k_full = bars, k_free = bars + 24, v_full = bars + 48, v_free = bars + 72, s_full = bars + 96, s_free = bars + 104, o_done = bars + 112, w_full = bars + 128, q_full = bars + 160, r_full = bars + 168;
     unsigned* tmem_slot = reinterpret_cast<unsigned*>(smem + (bars + kBarriers * 8 - sq0));
     float* scales = reinterpret_cast<float*>(smem + (bars + kBarriers * 8 + 8 - sq0));  // [64]: what the norms divide by
@@ -273,7 +278,7 @@ template <bool CAPPED, int KEYS> __global__ void __launch_bounds__(Shape<KEYS>::
             after_sync();
             if (elect_one() && ok) {
                 const unsigned long long k = dk + keys_at.s * (k_stage >> 4);
-                                for (int c = 0; c < kp; c++) {
+                for (int c = 0; c < kp; c++) {
                     const unsigned long long a = dq + c * (kPanelQ >> 4), a2 = a + (low0 >> 4), b = k + c * (kPanelK >> 4);
 #pragma unroll
                     for (int e = 0; e < 4; e++)
@@ -343,7 +348,7 @@ template <bool CAPPED, int KEYS> __global__ void __launch_bounds__(Shape<KEYS>::
         const float cap2 = p.cap2;
         float m = -1e30f;  // below every score, and finite: differences stay numbers
         float sums[4] = {};  // of every fourth key's weights each
-        int halves = 0;                       // of the values, in front of this thread's
+        int halves = 0;      // of the values, in front of this thread's
         for (int i = 0; i < n; i++) {
             const int j0 = (kt0 + i) * KEYS, j1 = j0 + part * kPart;
             if (ok && !mbar_wait(s_full, (unsigned)i & 1)) ok = false;
@@ -531,7 +536,7 @@ template <bool CAPPED, int KEYS> __global__ void __launch_bounds__(Shape<KEYS>::
     if (warp == kIssues) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(cols) : "memory");
 }
 
-// Two CTAs per SM where their shared and tensor memory allow it.
+// Two CTAs per SM where their shared and tensor memory allow it: 4096 tokens, 32 heads of 2 × 64 over 16 289 us, one CTA of 128 keys 426; 2048, 16 over 4 60 and 80.
 int differential_keys(int kp, int vp) { return kp == 1 && vp <= 2 ? 64 : 128; }
 // No more CTAs share an SM than have room in its tensor memory: with 256 columns of 512 at most two (80 KB and more each), with all of them one (118 KB and more).
 int differential_smem(int kp, int vp) {

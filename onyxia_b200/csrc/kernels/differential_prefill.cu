@@ -299,8 +299,10 @@ template <bool CAPPED, int KEYS> __global__ void __launch_bounds__(Shape<KEYS>::
         for (int i = 0; i < n; i++) {
             if (i + 1 < n) scores(i + 1);
             const int j0 = (kt0 + i) * KEYS;
-            for (int h = 0; h < kHalves; h++) {
+            // The threads of both halves before the products of either: where a row's maximum rises, each of its two threads scales every other sixteen columns of the sums, and products add to all of them.
+            for (int h = 0; h < kHalves; h++)
                 if (ok && !mbar_wait(w_full + (i & 1) * 16 + h * 8, (unsigned)(i >> 1) & 1)) ok = false;
+            for (int h = 0; h < kHalves; h++) {
                 if (!seen(j0, h)) continue;
                 if (ok && !mbar_wait(v_full + values_at.s * 8, values_at.parity)) ok = false;
                 after_sync();

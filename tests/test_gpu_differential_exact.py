@@ -1,0 +1,57 @@
+"""bf16 kernels of differential attention against what their roundings may cost (differential_exact.py).
+
+All results together are off by what they are due, give or take a tenth: over the thousands of (row, head) of each case the mean of squares is known to 2 %, and mantissas of exponentials of
+scores that spread over octaves, and of results, are spread as logarithms to a few percent. A query rounded once more would add 1.5 · 1.66e-3 to every score (a spread of 1.5), and with it
+sqrt((2 + 1.5²) / 2) = 1.46 times what is due at D = 1. Sums that miss a scaling, or the values of half a tile, are off by the order of the results.
+"""
+import numpy as np
+import pytest
+
+import differential_exact as exact
+import differential_util as util
+from differential_util import Form
+from gpu_util import cuda_backend
+from kipizen_util import to_bf16
+from onyxia_b200 import ir
+from onyxia_b200.ir import HostTensor
+
+pytestmark = pytest.mark.gpu
+
+DUE = 1.1
+# the second form's products are made by halves of a tile: maps above 64 or values above 128 dimensions
+NARROW, WIDE, WIDE_VALUES = Form(8, 2, 64, 128, 64), Form(4, 1, 128, 256, 128), Form(4, 2, 64, 192, 64)
+
+
+def results(f, s, runs=1):
+    session = cuda_backend().prepare(util.module(f, ir.BF16, s.lam, s.gain))
+    dev = {k: session.upload(v) for k, v in util.feed(s, HostTensor.bf16).items()}
+    return [session.download(session.run(dev)[0][1]).numpy() for _ in range(runs)]
+
+
+def rising(f, s, by):
+    """Keys grow along their sequences: every tile of keys brings rows a new maximum. Queries see them from their own side: all first dimensions are positive."""
+    q0, k0, _ = f.offsets
+    for i, (row, n, past, _) in enumerate(s.seqs):
+        for pos in range(past):
+            pg, off = s.table[i, pos // f.page], pos % f.page
+            for m in (0, 1):
+                s.keys[pg, :, off, m * f.dim] = by * pos / 64
+        for t in range(n):
+            for g in range(2 * f.kv_heads):
+                s.proj[row + t, k0 + g * f.dim] = by * (past + t) / 64
+    s.proj[:, q0:q0 + f.heads * 2 * f.dim:f.dim] = 1.0 / f.scale
+    s.keys, s.proj = to_bf16(s.keys), to_bf16(s.proj)
+
+
+@pytest.mark.parametrize("f", [NARROW, WIDE, WIDE_VALUES], ids=["narrow", "wide", "wide values"])
+@pytest.mark.parametrize("by", [0.05, 0.5, 3.0])
+def test_maxima_that_rise_with_every_tile(f, by):
+    """Sums are scaled again and again, by threads that share a row, in front of the products of either half of a tile."""
+    f = Form(f.heads, f.kv_heads, f.dim, f.vdim, 0)
+    s = util.step(f, [(700, 900), (130, 60)], 7)
+    rising(f, s, by)
+    first, *more = results(f, s, 6)
+    assert exact.share(f, s, first, to_bf16) <= DUE
+    live = np.concatenate([np.arange(r, r + n) for r, n, _, _ in s.seqs])
+    for again in more:
+        assert np.array_equal(again[live], first[live])

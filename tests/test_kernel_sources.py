@@ -16,3 +16,12 @@ def test_all_lanes_come_to_an_election(name):
     assert not re.findall(r"&& elect_one\(\)", text)
     left = re.findall(r"if \(([^\n]*mbar_wait[^\n]*)\) \{\s*ok = false;\s*break;", text)
     assert all("__all_sync" in condition for condition in left), left
+
+
+def test_products_of_a_tile_begin_behind_the_threads_of_all_its_halves():
+    """Where two threads share a row, each scales some columns of the row's sums, and products add to all of them: the issuing warp waits for both before it issues either half's."""
+    text = open(os.path.join(KERNELS, "differential_prefill.cu")).read()
+    issues = text[text.index("else if (warp == kIssues)"):text.index("umma_weights(t_sum")]
+    wait = issues.index("mbar_wait(w_full")
+    loops = [m.start() for m in re.finditer(r"for \(int h = 0; h < kHalves; h\+\+\)", issues)]
+    assert len(loops) == 2 and loops[0] < wait < loops[1]  # a loop of waits, then a loop of products

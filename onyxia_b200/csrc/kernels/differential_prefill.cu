@@ -416,6 +416,9 @@ template <bool CAPPED, int KEYS> __global__ void __launch_bounds__(Shape<KEYS>::
                 }
                 if (j1 + kPart - 1 > last || j1 < low) {  // what lies behind the last key or in front of the first may be no number, which a weight of 0 would not cancel
                     const int at = halves + before, stage = at % kStagesV;
+                    // The place's values before these have to be there, or the barrier's parity is that of the round before them. With three places they are of tile i − 3, whose products are done; with
+                    // two they are of tile i − 1, whose products may still wait for them.
+                    if (kHalves == 2 && i > 0 && ok && !added(i - 1)) ok = false;
                     if (ok && !mbar_wait(v_full + stage * 8, (unsigned)(at / kStagesV) & 1)) ok = false;
                     for (int u = r; u < kPart * vp * 8; u += kRows) {
                         const int key = u & (kPart - 1), c = u / kPart;

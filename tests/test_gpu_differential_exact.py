@@ -55,3 +55,22 @@ def test_maxima_that_rise_with_every_tile(f, by):
     live = np.concatenate([np.arange(r, r + n) for r, n, _, _ in s.seqs])
     for again in more:
         assert np.array_equal(again[live], first[live])
+
+
+@pytest.mark.parametrize("f", [NARROW, WIDE, WIDE_VALUES], ids=["narrow", "wide", "wide values"])
+@pytest.mark.parametrize("window", [0, 100])
+def test_a_tile_that_begins_and_ends_within_a_page_of_no_numbers(f, window):
+    """Prompts end in every part of a tile, and windows begin there; what lies behind the last key, and in front of the first, is NaN. Maxima stand still, so that nothing waits for products."""
+    f = Form(f.heads, f.kv_heads, f.dim, f.vdim, 0, window=window)
+    s = util.step(f, [(33, 128 * 3 + 1 + 13 * i) for i in range(12)] + [(200, 7), (90, 1200)], 11, spread=0.0)
+    if window:
+        for i, (_, _, past, _) in enumerate(s.seqs):
+            for pos in range(max(0, past - window + 1)):
+                s.keys[s.table[i, pos // f.page], :, pos % f.page] = s.values[s.table[i, pos // f.page], :, pos % f.page] = np.nan
+    first, *more = results(f, s, 6)
+    live = np.concatenate([np.arange(r, r + n) for r, n, _, _ in s.seqs])
+    assert np.isfinite(first[live]).all()
+    for again in more:
+        assert np.array_equal(again[live], first[live])
+    known = util.Step(s.proj, np.nan_to_num(s.keys), np.nan_to_num(s.values), s.seqs, s.table, s.lam, s.gain)  # (nothing times NaN is no number in the formulas)
+    assert exact.share(f, known, first, to_bf16) <= DUE

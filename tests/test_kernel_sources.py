@@ -25,3 +25,10 @@ def test_products_of_a_tile_begin_behind_the_threads_of_all_its_halves():
     wait = issues.index("mbar_wait(w_full")
     loops = [m.start() for m in re.finditer(r"for \(int h = 0; h < kHalves; h\+\+\)", issues)]
     assert len(loops) == 2 and loops[0] < wait < loops[1]  # a loop of waits, then a loop of products
+
+
+def test_values_behind_the_last_key_are_cleared_in_their_own_round():
+    """A wait by parity is good for the round before it is over: where two places hold one tile's values, those before them are waited for first."""
+    text = open(os.path.join(KERNELS, "differential_prefill.cu")).read()
+    clears = text[text.index("may be no number"):text.index("st.shared.v4.b32")]
+    assert 0 <= clears.find("kHalves == 2 && i > 0 && ok && !added(i - 1)") < clears.index("mbar_wait(v_full")

@@ -206,7 +206,7 @@ template <bool CAPPED, int KEYS> __global__ void __launch_bounds__(Shape<KEYS>::
     if (!locate_rows(p, pp.tiles - 1 - tile, tq, p.singles ? 1 : 2, &seq, &first, &sq)) return;  // both CTAs of the cluster
     const int n_tok = min(tq, sq.len - first), pos0 = sq.past + first, last = pos0 + n_tok - 1, low = first_key(p, pos0);
     // Scores in KEYS columns, weights in two turns of half as many, sums behind them. No more CTAs than have room in tensor memory may be on an SM at a time
-    // (differential_smem), or two clusters could wait for what the other one has.
+    // (differential_prefill_smem), or two clusters could wait for what the other one has.
     constexpr unsigned cols = KEYS * 4;
     if (warp == kIssues) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(cols) : "memory");
@@ -543,14 +543,18 @@ template <bool CAPPED, int KEYS> __global__ void __launch_bounds__(Shape<KEYS>::
 
 // Two CTAs per SM where their shared and tensor memory allow it: 4096 tokens, 32 heads of 2 × 64 over 16 289 us, one CTA of 128 keys 426; 2048, 16 over 4 60 and 80.
 int differential_keys(int kp, int vp) { return kp == 1 && vp <= 2 ? 64 : 128; }
-// No more CTAs share an SM than have room in its tensor memory: with 256 columns of 512 at most two (80 KB and more each), with all of them one (118 KB and more).
-int differential_smem(int kp, int vp) {
+}  // namespace
+
+// A CTA that has tensor memory waits for its neighbour, which may be waiting for some: so as many CTAs as share an SM, of either form and whatever their sizes (two sessions run on one
+// device), must have room in its tensor memory. Forms of 64 keys take 256 of 512 columns and 85 448 bytes at least: two share an SM (233 472 bytes, 1 024 of them the system's per CTA), three
+// do not. Forms of 128 keys take all columns, so they ask for as many bytes as keep the smallest of the others away (120 832 … 198 000 are their own). Kernels of single CTAs that hold tensor
+// memory end by themselves, and none of more than 256 columns is small enough to wait beside two CTAs that do not need it.
+int differential_prefill_columns(int kp, int vp) { return differential_keys(kp, vp) * 4; }
+int differential_prefill_smem(int kp, int vp) {
     const int keys = differential_keys(kp, vp);
     const int kv = keys == 64 ? Shape<64>::keys * 64 * 128 * kp + Shape<64>::values * (int)kPanelV * vp : Shape<128>::keys * 128 * 128 * kp + Shape<128>::values * (int)kPanelV * vp;
-    return std::max(1024 + kp * 2 * (int)kPanelQ + kv + kBarriers * 8 + 16 + 256 + 4 * kRows * 4, keys == 64 ? 80 * 1024 : 118 * 1024);
+    return std::max(1024 + kp * 2 * (int)kPanelQ + kv + kBarriers * 8 + 16 + 256 + 4 * kRows * 4, keys == 64 ? 80 * 1024 : 147 * 1024);
 }
-
-}  // namespace
 
 bool differential_prefill_fits(const DiffP& p, const TRef& keys, const TRef& values, int64_t out_off) {
     const int64_t rows = (int64_t)p.n_pages * p.kv_heads << p.shift, rep = p.heads / p.kv_heads, tiles = rep <= kRows ? p.rows / (kRows / rep) + 1 + p.n_seqs : 0;
@@ -569,7 +573,7 @@ void emit_differential_prefill(Emitter& em, const DiffP& kv, const TRef& keys, c
     p.tiles = (int)((kv.rows + tq - 1) / tq + kv.n_seqs);
     void (*const k)(const PreP) = differential_keys(p.kp, p.vp) == 64 ? (kv.cap2 > 0.f ? differential_prefill<true, 64> : differential_prefill<false, 64>)
                                                                      : (kv.cap2 > 0.f ? differential_prefill<true, 128> : differential_prefill<false, 128>);
-    const int smem = differential_smem(p.kp, p.vp);
+    const int smem = differential_prefill_smem(p.kp, p.vp);
     ensure_max_dynamic_smem((const void*)k, 226 * 1024);
     LaunchRec& rec = em.launch(k, dim3((unsigned)p.tiles * (unsigned)kv.kv_heads * 2), dim3(differential_keys(p.kp, p.vp) == 64 ? Shape<64>::threads : Shape<128>::threads), (unsigned)smem, p, {}, "differential_prefill", /*pdl=*/true);
     rec.cluster = dim3(2, 1, 1);

@@ -483,6 +483,9 @@ struct DifferentialDesc {
 // `lambda` F32 [heads]: the second map's factor. `gain` F32 [vdim] or null: a head's result is divided by its root mean square and multiplied by it.
 void emit_differential(Emitter&, const DifferentialDesc&, const TRef& proj, const TRef& turns, const TRef& keys, const TRef& values, const TRef& seqs,
                        const TRef& pages, const TRef& lambda, const TRef* gain, const TRef& out);
+// Bytes of shared memory and columns of tensor memory that a CTA of its prompt kernel takes, for maps and values of so many times 64 dimensions.
+int differential_prefill_smem(int kp, int vp);
+int differential_prefill_columns(int kp, int vp);
 
 // Attention whose keys and values are one latent per token that all heads share: key = (latent, rotated part), value =
 // latent. Queries come with their unrotated part already mapped into the latent space (`q_latent` [rows, heads · rank]) and with

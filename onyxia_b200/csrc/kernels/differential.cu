@@ -605,7 +605,8 @@ void emit_differential(Emitter& em, const DifferentialDesc& d, const TRef& proj,
                   label, /*pdl=*/true);
     };
     if (!p.only) {
-        if (tc && p.by8 && d.rot_dims % 16 == 0 && d.heads <= 4096) launch(differential_prepare8, dim3((unsigned)rows), 128, (unsigned)(d.rot_dims * 12 + (d.norm ? 2 * (d.heads + d.kv_heads) : 0) * 4), none, "differential_prepare");
+        const int64_t eight = d.rot_dims * 12 + (d.norm ? 2 * (d.heads + d.kv_heads) : 0) * 4;  // bytes that the kernel for eight at a time shares; a block may have 48 KB
+        if (tc && p.by8 && d.rot_dims % 16 == 0 && d.heads <= 4096 && eight <= 48 * 1024) launch(differential_prepare8, dim3((unsigned)rows), 128, (unsigned)eight, none, "differential_prepare");
         else {
             const DiffKernel prepare = bf ? differential_prepare<bf16> : differential_prepare<float>;
             ensure_max_dynamic_smem((const void*)prepare, 8192 * 8);

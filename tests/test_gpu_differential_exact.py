@@ -74,3 +74,10 @@ def test_a_tile_that_begins_and_ends_within_a_page_of_no_numbers(f, window):
         assert np.array_equal(again[live], first[live])
     known = util.Step(s.proj, np.nan_to_num(s.keys), np.nan_to_num(s.values), s.seqs, s.table, s.lam, s.gain)  # (nothing times NaN is no number in the formulas)
     assert exact.share(f, known, first, to_bf16) <= DUE
+
+
+def test_as_many_heads_as_fill_a_blocks_memory_with_factors():
+    """Normed queries and keys of 4096 heads and as many key heads: 64 KB of factors."""
+    f = Form(4096, 4096, 16, 16, 16, page=8, norm=1)
+    s = util.step(f, [(3, 9), (2, 0)], 3, spare=0)
+    assert exact.share(f, s, results(f, s)[0], to_bf16) <= DUE

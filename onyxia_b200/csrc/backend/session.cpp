@@ -815,7 +815,7 @@ void Session::check_device_error() {
         case oxk::ERR_RULES_TOKEN: what = "rules: token " + std::to_string(e.a) + " is not one of " + std::to_string(e.b); break;
         case oxk::ERR_RULES_LENGTH: what = "rules: the lengths of row " + std::to_string(e.a) + " do not fit a history of " + std::to_string(e.b); break;
         case oxk::ERR_RULES_MASK: what = "rules: mask " + std::to_string(e.a) + " is not one of " + std::to_string(e.b); break;
-        case oxk::ERR_BATCH_ROWS: what = "sequence " + std::to_string(e.a) + " has " + std::to_string(e.b) + " new tokens in a batch of no more rows than sequences"; break;
+        case oxk::ERR_BATCH_ROWS: what = "sequence " + std::to_string(e.a) + " has " + std::to_string(e.b) + " new tokens in a batch of as many rows as sequences"; break;
         case oxk::ERR_BATCH_SEQ: what = "sequence " + std::to_string(e.a) + " does not lie in the rows of the batch, or its " + std::to_string(e.b) + " positions not in the page table"; break;
         default: what = "device error code " + std::to_string(e.code);
     }

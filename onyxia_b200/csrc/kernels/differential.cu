@@ -11,6 +11,7 @@
 //   differential_prefill   sequences with several new tokens in bf16 (differential_prefill.cu)
 //   differential_decode    sequences with one new token: their keys split over CTAs and warps, all of the above in one launch
 //   differential_simt      any shape, f32 and bf16
+//   differential_several   sequences with several new tokens beside empty ones, in batches of fewer rows than sequences
 //
 // Decode reads min(past, window) · kv_heads · (2 · dim + vdim) · 2 bytes per sequence.
 #include "differential.cuh"
@@ -155,17 +156,10 @@ __global__ void __launch_bounds__(128, 8) differential_prepare8(const DiffP p) {
     }
 }
 
-// One CTA per (row, head); chunks of 128 keys, a thread per key, then a thread per value dimension.
-template <typename T> __global__ void __launch_bounds__(kAnyKeys) differential_simt(const DiffP p) {
-    extern __shared__ float sm[];  // q[2][dim], acc[2][vdim], w[2][128]
-    __shared__ float red[32];
-    pdl_enter();
-    const int row = blockIdx.x, h = blockIdx.y, tid = threadIdx.x, s = find_seq(p.seqs, p.n_seqs, row);
-    const SeqRow sq = checked_seq(p, s);
-    if (row < sq.start || row >= sq.start + sq.len || (sq.len == 1 && !p.singles)) return;
-    const int pos = sq.past + row - sq.start, g = h / (p.heads / p.kv_heads);
+// A row's head by 128 threads: chunks of 128 keys, a thread per key, then a thread per value dimension. `sm`: q[2][dim] (there), acc[2][vdim], w[2][128].
+template <typename T> __device__ __forceinline__ void attend_row(const DiffP& p, int s, int pos, int row, int h, float* sm, float* red) {
+    const int tid = threadIdx.x, g = h / (p.heads / p.kv_heads);
     float *q = sm, *acc = sm + 2 * p.dim, *w = acc + 2 * p.vdim;
-    for (int i = tid; i < 2 * p.dim; i += kAnyKeys) q[i] = to_f(((const T*)p.q)[((long long)row * p.heads + h) * 2 * p.dim + i]);
     for (int i = tid; i < 2 * p.vdim; i += kAnyKeys) acc[i] = 0.f;
     // a sink is a score of 0 that has no value; without one the sums begin below every score, at a number: differences stay numbers
     float m[2], l[2];
@@ -204,6 +198,60 @@ template <typename T> __global__ void __launch_bounds__(kAnyKeys) differential_s
     }
     const float f = p.gain ? 1.f / sqrtf(block_sum(ss, red) / (float)p.vdim + p.head_eps) : 1.f;
     for (int i = tid; i < p.vdim; i += kAnyKeys) ((T*)p.out)[((long long)row * p.heads + h) * p.vdim + i] = from_f<T>(p.gain ? acc[i] * f * p.gain[i] : acc[i]);
+}
+
+template <typename T> __global__ void __launch_bounds__(kAnyKeys) differential_simt(const DiffP p) {
+    extern __shared__ float sm[];
+    __shared__ float red[32];
+    pdl_enter();
+    const int row = blockIdx.x, h = blockIdx.y, s = find_seq(p.seqs, p.n_seqs, row);
+    const SeqRow sq = checked_seq(p, s);
+    if (row < sq.start || row >= sq.start + sq.len || (sq.len == 1 && !p.singles)) return;
+    for (int i = threadIdx.x; i < 2 * p.dim; i += kAnyKeys) sm[i] = to_f(((const T*)p.q)[((long long)row * p.heads + h) * 2 * p.dim + i]);
+    attend_row<T>(p, s, sq.past + row - sq.start, row, h, sm, red);
+}
+
+// The sequences of several new tokens in a batch of fewer rows than sequences, whose single tokens differential_decode takes: a CTA per key head and sequence stores the keys and values, then
+// goes through the rows. (64 sequences behind 2000, 16 heads of 2 x 64 over 4, four of
+// them without new tokens: 4 us of a call of 77; the launches for prompts in its place took 24.)
+__global__ void __launch_bounds__(kAnyKeys) differential_several(const DiffP p) {
+    extern __shared__ float sm[];  // what attend_row has, cosines and sines behind it
+    __shared__ float red[32];
+    pdl_enter();
+    const int g = blockIdx.x, seq = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, rep = p.heads / p.kv_heads;
+    const SeqRow sq = checked_seq(p, seq);
+    if (sq.len < 2) return;
+    double *cs = reinterpret_cast<double*>(sm + 2 * (p.dim + p.vdim + kAnyKeys)), *sn = cs + p.half;
+    bf16 *keys = (bf16*)p.keys, *values = (bf16*)p.values;
+    for (int t = 0; t < sq.len; t++) {
+        const int pos = sq.past + t;
+        const bf16* x = (const bf16*)p.proj + (long long)(sq.start + t) * p.ld;
+        const long long at = key_row(p, page_of(p, seq, pos), g, pos);
+        exact_angles(p, pos, cs, sn, tid, kAnyKeys);
+        __syncthreads();
+        if (warp < 2) {
+            const bf16* k = x + p.k_off + (long long)(g * 2 + warp) * p.dim;
+            const float f = map_factor(p, k);
+            for (int i = lane; i < p.dim; i += 32) keys[(at * 2 + warp) * p.dim + i] = __float2bfloat16_rn((float)(turned(p, k, cs, sn, i) * f));
+        }
+        for (int i = tid; i < p.vdim; i += kAnyKeys) values[at * p.vdim + i] = x[p.v_off + (long long)g * p.vdim + i];
+        __syncthreads();
+    }
+    for (int t = 0; t < sq.len; t++) {
+        const int pos = sq.past + t;
+        const bf16* x = (const bf16*)p.proj + (long long)(sq.start + t) * p.ld;
+        exact_angles(p, pos, cs, sn, tid, kAnyKeys);
+        for (int h = g * rep; h < (g + 1) * rep; h++) {
+            __syncthreads();
+            if (warp < 2) {
+                const bf16* q = x + p.q_off + (long long)(h * 2 + warp) * p.dim;
+                const float f = map_factor(p, q);
+                for (int i = lane; i < p.dim; i += 32) sm[warp * p.dim + i] = (float)(turned(p, q, cs, sn, i) * f);
+            }
+            attend_row<bf16>(p, seq, pos, sq.start + t, h, sm, red);
+        }
+        __syncthreads();
+    }
 }
 
 // ───────────────────────────── single tokens ────────────────────────────
@@ -358,7 +406,7 @@ template <int DM, int DV> __global__ void __launch_bounds__(kDecThreads) differe
     if (newest && warp >= 2) exact_angles(p, pos, cs, sn, tid - 64, 64);
     pdl_wait();
     if (sq.len != 1) {
-        if (p.only && sq.len > 1 && tid == 0) report(p.err, ERR_BATCH_ROWS, p.node, seq, sq.len);
+        if (p.only && sq.len > 1 && p.rows == p.n_seqs && tid == 0) report(p.err, ERR_BATCH_ROWS, p.node, seq, sq.len);
         return;
     }
     // all that comes from the projection at once
@@ -587,7 +635,7 @@ void emit_differential(Emitter& em, const DifferentialDesc& d, const TRef& proj,
     const bool bf = proj.dtype == DT_BF16;
     // 16-byte copies of key and value rows
     const bool tc = bf && d.dim % 8 == 0 && d.vdim % 8 == 0 && d.dim <= 128 && d.vdim <= 256 && keys.buf.off % 16 == 0 && values.buf.off % 16 == 0 && n_seqs <= 65535;
-    p.only = tc && rows <= n_seqs;                     // every sequence has one new token, or none
+    p.only = tc && rows <= n_seqs;                     // every sequence has one new token, or none; with fewer rows than sequences some may have more (differential_several)
     p.singles = !tc || (!p.only && n_seqs == 1);       // a lone token with rows of nobody behind it
     const bool prefill = tc && !p.only && differential_prefill_fits(p, keys, values, out.buf.off);
     p.parts = prefill;
@@ -622,6 +670,7 @@ void emit_differential(Emitter& em, const DifferentialDesc& d, const TRef& proj,
             launch(k, dim3((unsigned)rows, (unsigned)d.heads), kAnyKeys, (unsigned)((d.dim + d.vdim + kAnyKeys) * 8), none, "differential_simt");
         }
     }
+    if (p.only && rows > 1 && rows < n_seqs) launch(differential_several, dim3((unsigned)d.kv_heads, (unsigned)n_seqs), kAnyKeys, (unsigned)((d.dim + d.vdim + kAnyKeys) * 8 + d.rot_dims * 8), none, "differential_several");
     if (tc && (p.only || n_seqs > 1)) {
         const DecChoice dc = d.dim <= 32 ? choice<32>(d.vdim) : d.dim <= 64 ? choice<64>(d.vdim) : choice<128>(d.vdim);
         const int64_t groups = d.kv_heads * ((d.heads / d.kv_heads + kDecHeads - 1) / kDecHeads), cells = n_seqs * groups;

@@ -479,7 +479,7 @@ struct DifferentialDesc {
     double head_eps;              // of the norm of a head's result, where there is one
 };
 // Causal attention of the difference of two softmax maps over pools of keys [pages, kv_heads, page, 2 · dim] and values [pages, kv_heads, page, vdim].
-// Sequences stand in the order of their rows, those without new tokens behind the others; where the batch has no more rows than sequences, none has more than one.
+// Sequences stand in the order of their rows, those without new tokens behind the others; where the batch has as many rows as sequences, none has more than one (bf16: reported).
 // `lambda` F32 [heads]: the second map's factor. `gain` F32 [vdim] or null: a head's result is divided by its root mean square and multiplied by it.
 void emit_differential(Emitter&, const DifferentialDesc&, const TRef& proj, const TRef& turns, const TRef& keys, const TRef& values, const TRef& seqs,
                        const TRef& pages, const TRef& lambda, const TRef* gain, const TRef& out);

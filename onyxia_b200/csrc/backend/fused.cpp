@@ -3,6 +3,7 @@
 // `Backend::supports` reports; `accepts` narrows a kernel to the operand types
 // it implements, every other instance of the composite is legalised through
 // its decomposition.
+#include <algorithm>
 #include <cmath>
 
 #include "../kernels/common.cuh"
@@ -877,6 +878,17 @@ void emit_allreduce(Emitter& em, const TRef& x, const TRef& y) {
 
 namespace oxrt {
 
+bool may_begin_early(const FusedKernel& k, const Module& m, const Node& n) {
+    if (k.of_run.empty()) return true;
+    for (size_t i = 0; i < n.inputs.size(); i++) {
+        if (std::find(k.of_run.begin(), k.of_run.end(), (int)i) != k.of_run.end()) continue;
+        const auto* v = &m.values[n.inputs[i]];
+        while (v->origin.kind == Origin::Node && m.nodes[v->origin.id].is_prim && m.nodes[v->origin.id].prim.kind == PrimKind::Reshape) v = &m.values[m.nodes[v->origin.id].inputs[0]];  // (the same bytes)
+        if (v->origin.kind == Origin::Node) return false;
+    }
+    return true;
+}
+
 const KernelRegistry& standard_kernels() {
     static const KernelRegistry reg = [] {
         KernelRegistry r;
@@ -890,17 +902,17 @@ const KernelRegistry& standard_kernels() {
         r.add({"onyxia.AllReduce", allreduce_accepts, allreduce_lower});
         r.add({"onyxia.ResidualNorm", residual_norm_accepts, residual_norm_lower});
         r.add({"onyxia.Linear", linear_accepts, linear_lower});
-        r.add({"onyxia.PagedAttention", paged_accepts, paged_lower, {{1, 4}, {2, 5}}});
-        r.add({"onyxia.GatedRecurrence", recurrence_accepts, recurrence_lower, {{1, 8}, {2, 9}}});
-        r.add({"onyxia.PagedKVAttention", paged_kv_accepts, paged_kv_lower, {{1, 2}, {2, 3}}});
-        r.add({"onyxia.SharedKVAttention", shared_kv_accepts, paged_kv_lower});
-        r.add({"onyxia.DifferentialAttention", differential_accepts, differential_lower, {{1, 2}, {2, 3}}});
-        r.add({"onyxia.LightningAttention", lightning_accepts, lightning_lower, {{1, 2}}});
-        r.add({"onyxia.GatedLinearAttention", gated_linear_accepts, gated_linear_lower, {{1, 2}}});
-        r.add({"onyxia.GatedDeltaRule", delta_accepts, delta_lower, {{1, 4}, {2, 5}}});
+        r.add({"onyxia.PagedAttention", paged_accepts, paged_lower, {{1, 4}, {2, 5}}, {0}});
+        r.add({"onyxia.GatedRecurrence", recurrence_accepts, recurrence_lower, {{1, 8}, {2, 9}}, {0}});
+        r.add({"onyxia.PagedKVAttention", paged_kv_accepts, paged_kv_lower, {{1, 2}, {2, 3}}, {0}});
+        r.add({"onyxia.SharedKVAttention", shared_kv_accepts, paged_kv_lower, {}, {0, 2, 3}});
+        r.add({"onyxia.DifferentialAttention", differential_accepts, differential_lower, {{1, 2}, {2, 3}}, {0}});
+        r.add({"onyxia.LightningAttention", lightning_accepts, lightning_lower, {{1, 2}}, {0}});
+        r.add({"onyxia.GatedLinearAttention", gated_linear_accepts, gated_linear_lower, {{1, 2}}, {0, 1}});
+        r.add({"onyxia.GatedDeltaRule", delta_accepts, delta_lower, {{1, 4}, {2, 5}}, {0}});
         r.add({"onyxia.MixtureOfExperts", moe_accepts, moe_lower});
-        r.add({"onyxia.LatentAttention", latent_accepts, latent_lower, {{1, 5}}});
-        r.add({"onyxia.SelectiveScan", selective_accepts, selective_lower, {{1, 8}, {2, 9}}});
+        r.add({"onyxia.LatentAttention", latent_accepts, latent_lower, {{1, 5}}, {0, 1, 2}});
+        r.add({"onyxia.SelectiveScan", selective_accepts, selective_lower, {{1, 8}, {2, 9}}, {0}});
         return r;
     }();
     return reg;

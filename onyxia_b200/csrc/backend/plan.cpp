@@ -308,7 +308,10 @@ bool Session::lower_step(Plan& plan, oxk::Emitter& em, size_t step, Bindings& bi
             } else {
                 FusedCtx fc{em, node, ins, outs, (bool)kv_in_place[nid], false};
                 if (node.inputs.size() > 1) fc.weights_layout = interleaved_[node.inputs[1]];
+                const size_t before = em.recs.size();
                 info_[nid].fused->lower(fc);
+                if (!may_begin_early(*info_[nid].fused, m, node))
+                    for (size_t i = before; i < em.recs.size(); i++) em.recs[i].pdl = false;
                 plan.node_bucket[nid] = fc.bucket;
                 plan.node_bucket_step[nid] = fc.bucket_step;
             }

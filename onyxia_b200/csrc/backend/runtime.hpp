@@ -121,7 +121,11 @@ struct FusedKernel {
     // (result, operand) pairs of state tensors the kernel updates where they are: the result is a module output, the
     // operand a module input that nothing else reads, and a run hands the same buffer back.
     std::vector<std::pair<int, int>> in_place = {};
+    // Kernels that look at a batch before the launches in front of them have ended: the operands that they read behind their wait only. All others (batch description, page table, weights) have to be there
+    // before the run begins; where the module computes one, the node's launches are not begun early (may_begin_early). Empty: nothing is read in front of a wait but what is constant.
+    std::vector<int> of_run = {};
 };
+bool may_begin_early(const FusedKernel& k, const Module& m, const Node& n);
 
 // ≙ KernelRegistry / standard_kernels (fused.rs:43-86).
 class KernelRegistry {

@@ -327,8 +327,8 @@ template <int DM, int DV> __global__ void __launch_bounds__(kDecThreads) differe
     using L = DecSmem<DM, DV>;
     pdl_trigger();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g8 = lane >> 2, t4 = lane & 3;
-    // no launch of a step writes the batch description or the keys and values of earlier steps: they may be read while the
-    // launches before this one finish
+    // no launch of a step writes the batch description or the keys and values of earlier steps (where the module computes the
+    // former, this launch does not begin early): they may be read while the launches before this one finish
     const int seq = blockIdx.z;
     const SeqRow sq = checked_seq(p, seq);
     const int rep = p.heads / p.kv_heads, groups = (rep + kDecHeads - 1) / kDecHeads, g = blockIdx.y / groups, h0 = g * rep + (blockIdx.y % groups) * kDecHeads;

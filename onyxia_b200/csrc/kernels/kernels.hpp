@@ -107,7 +107,8 @@ struct LaunchRec {
     // Every such kernel triggers its own dependents at entry, so the section
     // before its wait may overlap not only the launch before it but several
     // earlier ones: it may read only memory that NO launch of the same run
-    // writes (constants, rows of a KV cache below the step's first new row).
+    // writes (constants, rows of a KV cache below the step's first new row; a batch description and a page table that are
+    // module inputs: where the module computes them, the session clears this).
     bool pdl = false;
     // Not a kernel of this library: a collective the session enqueues itself. The parameter bytes
     // are a CollP (with the usual pointer relocations); `func` is null.

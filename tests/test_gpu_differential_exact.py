@@ -7,6 +7,7 @@ sqrt((2 + 1.5²) / 2) = 1.46 times what is due at D = 1. Sums that miss a scalin
 import numpy as np
 import pytest
 
+import differential_computed
 import differential_exact as exact
 import differential_util as util
 from differential_util import Form
@@ -91,3 +92,28 @@ def test_batches_padded_with_sequences_without_new_tokens(f, lengths):
     """Fewer rows than sequences: sequences may have any number of new tokens. (As many rows as sequences say that each has one at most.)"""
     s = util.step(f, lengths, 5)
     assert exact.share(f, s, results(f, s)[0], to_bf16) <= DUE_FEW
+
+
+@pytest.mark.parametrize("maps", [2, 1], ids=["differential", "plain"])
+@pytest.mark.parametrize("computed", [("seq_info",), ("page_table",), ("turns",), ("reshaped",), ("seq_info", "page_table", "turns")], ids="+".join)
+def test_batches_and_angles_that_the_module_computes(computed, maps):
+    """The same bits as where they are inputs and constants, whether a run is launched one by one or replayed. The batch changes between runs."""
+    f = Form(16, 4, 64, 128, 64)
+    for lengths in ([(1, 700 + 50 * i) for i in range(20)], [(130, 40), (1, 900), (3, 60)]):
+        s = util.step(f, lengths, 3)
+        keys, values = s.keys[..., :maps * f.dim], s.values
+        want, got = [], []
+        for how, into in (((), want), (computed, got)):
+            session = cuda_backend().prepare(differential_computed.module(f, ir.BF16, s.lam, s.gain, how, maps))
+            feed = {"proj": session.upload(HostTensor.bf16(s.proj)), "pages.keys": session.upload(HostTensor.bf16(keys)), "pages.values": session.upload(HostTensor.bf16(values))}
+            for back in (0, 1, 5, 0, 2):
+                seqs = s.seqs.copy()
+                seqs[:, 2] = np.maximum(seqs[:, 2] - back, 0)
+                table = s.table[:, None] if "reshaped" in how else s.table
+                feed["seq_info"] = session.upload(HostTensor.from_numpy(seqs.astype(np.int64 if "seq_info" in how else np.int32)))
+                feed["page_table"] = session.upload(HostTensor.from_numpy(table.astype(np.int64 if "page_table" in how else np.int32)))
+                outs = dict(session.run(feed))
+                into.append([session.download(outs[n]).numpy() for n in ("out", "updated.pages.keys")])
+                feed["pages.keys"], feed["pages.values"] = outs["updated.pages.keys"], outs["updated.pages.values"]
+        for (a, k), (b, l) in zip(want, got):
+            assert np.array_equal(a, b) and np.array_equal(k, l, equal_nan=True)

@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+import threading
 from typing import Sequence
 
 import numpy as np
@@ -65,7 +66,8 @@ class DeviceTensor:
 class DeviceView:
     """Memory of a tensor as ``__cuda_array_interface__`` (``torch.as_tensor`` and others take it without a copy); bf16 as whole
     numbers of 16 bits. The view keeps the tensor; when it goes, the session's later work is ordered behind the view's stream, which has
-    to live as long."""
+    to live as long. Where it goes on another thread than the one that made it, the session does so at its next call. Where the stream
+    cannot be waited for (it is being captured), the tensor's memory stays the session's until it is closed."""
 
     def __init__(self, session: "CudaSession", t: DeviceTensor, stream: int):
         dtype, shape = t.describe()
@@ -74,26 +76,41 @@ class DeviceView:
         self._tensor = t.clone()
         ptr = C.c_void_p()
         check(session._lib.ox_session_device_view(session._h, t.handle, C.c_void_p(int(stream)), C.byref(ptr)))
-        self._session, self._stream = session, int(stream)
+        self._session, self._stream, self._thread = session, int(stream), threading.get_ident()
         kind = "<i2" if dtype == BF16 else "|b1" if dtype == BOOL else np.dtype(_NP[dtype]).str
         self.__cuda_array_interface__ = {"shape": shape, "typestr": kind, "data": (ptr.value or 0, False), "version": 2, "strides": None}
 
     def __del__(self):
         session = getattr(self, "_session", None)
-        if session is not None and session._h:
-            try:
-                session._lib.ox_session_after_stream(session._h, C.c_void_p(self._stream))
-            except Exception:
-                pass
+        if session is None or not session._open:
+            return
+        if threading.get_ident() == self._thread:
+            session._end_view(self._tensor, self._stream)
+        else:  # a session is for one thread at a time
+            session._dropped.append((self._tensor, self._stream))
 
 
 class CudaSession:
     """≙ ``impl Session`` of the reference GPU backend (session.rs:510-649)."""
 
     def __init__(self, handle):
-        self._h = handle
         self._lib = _ffi.cuda_lib()
+        self._open, self._dropped, self._kept = handle, [], []  # views that went on other threads; tensors of views whose stream could not be waited for
         self._num_outputs = max(self._lib.ox_session_num_outputs(handle), 1)
+
+    @property
+    def _h(self):
+        while self._dropped:
+            self._end_view(*self._dropped.pop())
+        return self._open
+
+    def _end_view(self, tensor, stream: int) -> None:
+        try:
+            ordered = self._lib.ox_session_after_stream(self._open, C.c_void_p(stream)) == 0
+        except Exception:
+            ordered = False
+        if not ordered:
+            self._kept.append(tensor)
 
     def upload(self, t: HostTensor) -> DeviceTensor:
         shape = (C.c_uint64 * max(len(t.shape), 1))(*t.shape)
@@ -205,8 +222,9 @@ class CudaSession:
 
     def close(self) -> None:
         if self._h:
-            self._lib.ox_session_free(self._h)
-            self._h = None
+            self._lib.ox_session_free(self._open)
+            self._open = None
+            self._kept.clear()
 
     def __del__(self):
         try:

@@ -10,7 +10,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
-import threading
+from threading import get_ident as _get_ident
 from typing import Sequence
 
 import numpy as np
@@ -76,15 +76,15 @@ class DeviceView:
         self._tensor = t.clone()
         ptr = C.c_void_p()
         check(session._lib.ox_session_device_view(session._h, t.handle, C.c_void_p(int(stream)), C.byref(ptr)))
-        self._session, self._stream, self._thread = session, int(stream), threading.get_ident()
+        self._session, self._stream, self._thread = session, int(stream), _get_ident()
         kind = "<i2" if dtype == BF16 else "|b1" if dtype == BOOL else np.dtype(_NP[dtype]).str
         self.__cuda_array_interface__ = {"shape": shape, "typestr": kind, "data": (ptr.value or 0, False), "version": 2, "strides": None}
 
-    def __del__(self):
+    def __del__(self, get_ident=_get_ident):  # (a module's names may be gone when the interpreter ends)
         session = getattr(self, "_session", None)
         if session is None or not session._open:
             return
-        if threading.get_ident() == self._thread:
+        if get_ident() == self._thread:
             session._end_view(self._tensor, self._stream)
         else:  # a session is for one thread at a time
             session._dropped.append((self._tensor, self._stream))
@@ -104,9 +104,9 @@ class CudaSession:
             self._end_view(*self._dropped.pop())
         return self._open
 
-    def _end_view(self, tensor, stream: int) -> None:
+    def _end_view(self, tensor, stream: int, pointer=C.c_void_p) -> None:
         try:
-            ordered = self._lib.ox_session_after_stream(self._open, C.c_void_p(stream)) == 0
+            ordered = self._lib.ox_session_after_stream(self._open, pointer(stream)) == 0
         except Exception:
             ordered = False
         if not ordered:

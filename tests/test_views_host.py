@@ -1,5 +1,8 @@
 """What becomes of a view's tensor and of its stream's order when the view goes, with a library that only takes notes."""
 import gc
+import os
+import subprocess
+import sys
 import threading
 
 import pytest
@@ -43,7 +46,7 @@ class Tensor:
         return Tensor()
 
     def __del__(self):
-        Tensor.released += 1
+        type(self).released += 1
 
 
 @pytest.fixture
@@ -99,3 +102,11 @@ def test_views_of_a_closed_session_ask_nothing_of_it(session):
     del v
     gc.collect()
     assert notes.calls[-1] == ("free",)
+
+
+def test_views_that_are_held_until_the_interpreter_ends_go_quietly():
+    here = os.path.dirname(os.path.abspath(__file__))
+    program = ("import sys\nimport test_views_host as t\nfrom onyxia_b200 import _ffi, backend\nnotes = t.Notes()\n_ffi.cuda_lib = lambda: notes\nsys.held = backend.CudaSession(1).view(t.Tensor(), 5)\n"
+               "held = backend.CudaSession(1).view(t.Tensor(), 5)\n")
+    r = subprocess.run([sys.executable, "-c", program], capture_output=True, text=True, env=dict(os.environ, PYTHONPATH=os.pathsep.join([here, os.path.dirname(here)])))
+    assert r.returncode == 0 and r.stderr == ""

@@ -367,8 +367,14 @@ template <bool CAPPED, int KEYS> __global__ void __launch_bounds__(Shape<KEYS>::
             before_sync();
             __syncwarp();
             if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(s_free) : "memory");
+            const bool edge = j1 + kPart - 1 > pos0 || j1 < last_low;
+            if (CAPPED && edge) {  // how a warp's scores are capped hangs on those that its rows see: the others may be anything
+#pragma unroll
+                for (int e = 0; e < kPart; e++)
+                    if (j1 + e > pos || j1 + e < mine_low) s[e] = 0.f;
+            }
             if (CAPPED) cap_scores(s, cap2);
-            if (j1 + kPart - 1 > pos0 || j1 < last_low) {
+            if (edge) {
 #pragma unroll
                 for (int e = 0; e < kPart; e++)
                     if (j1 + e > pos || j1 + e < mine_low) s[e] = -INFINITY;

@@ -117,3 +117,19 @@ def test_batches_and_angles_that_the_module_computes(computed, maps):
                 feed["pages.keys"], feed["pages.values"] = outs["updated.pages.keys"], outs["updated.pages.values"]
         for (a, k), (b, l) in zip(want, got):
             assert np.array_equal(a, b) and np.array_equal(k, l, equal_nan=True)
+
+
+@pytest.mark.parametrize("f", [NARROW, WIDE], ids=["narrow", "wide"])
+def test_what_lies_behind_the_last_key_changes_no_bit(f):
+    """Caps are a polynomial or an exponential by what a warp's scores are: those of keys that a row sees."""
+    f = Form(f.heads, f.kv_heads, f.dim, f.vdim, 0, softcap=4.0, window=150)
+    s = util.step(f, [(20, 40), (130, 100), (1, 70), (40, 300)], 13, spread=0.5)
+    outs = []
+    for behind in (0.0, 1.0, -300.0, 3e38, np.inf, np.nan):
+        keys = s.keys.copy()
+        keys[np.isnan(keys)] = behind
+        outs += results(f, util.Step(s.proj, to_bf16(keys), np.nan_to_num(s.values), s.seqs, s.table, s.lam, s.gain), 2)
+    assert exact.share(f, s, outs[0], to_bf16) <= DUE
+    live = np.concatenate([np.arange(r, r + n) for r, n, _, _ in s.seqs])
+    for other in outs[1:]:
+        assert np.array_equal(other[live], outs[0][live])

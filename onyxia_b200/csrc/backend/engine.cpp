@@ -272,9 +272,13 @@ DTensor Engine::constrained(const DTensor& logits, const std::vector<Request*>& 
     for (size_t i = 0; i < n; i++) {
         const Request& r = *rows[i];
         if (r.rules.history()) {
-            lengths[2 * i] = (int32_t)r.prompt.size(), lengths[2 * i + 1] = (int32_t)(r.prompt.size() + r.answer.size());
-            auto at = history.begin() + (long)(i * longest);
-            std::transform(r.answer.begin(), r.answer.end(), std::transform(r.prompt.begin(), r.prompt.end(), at, [](int64_t t) { return (int32_t)t; }), [](int64_t t) { return (int32_t)t; });
+            // (a prompt may hold tokens that have an embedding and no logit: nothing is to be penalised)
+            int32_t *const from = history.data() + i * longest, *at = from;
+            for (const std::vector<int64_t>* part : {&r.prompt, &r.answer}) {
+                for (int64_t t : *part)
+                    if (t >= 0 && t < vocab_) *at++ = (int32_t)t;
+                lengths[2 * i + (part == &r.answer)] = (int32_t)(at - from);
+            }
         }
         penalties[3 * i] = r.rules.repetition, penalties[3 * i + 1] = r.rules.frequency, penalties[3 * i + 2] = r.rules.presence;
         std::copy(r.rules.bias_ids.begin(), r.rules.bias_ids.end(), bias_ids.begin() + (long)(i * biases));

@@ -1,0 +1,59 @@
+"""Rules of requests and of rows where they meet other limits: tokens without a logit, biases that add up beyond f32, every place a number."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+from gpu_util import cuda_backend
+from onyxia_b200 import OnyxiaError, _ffi, ir
+from onyxia_b200.engine import Engine
+from onyxia_b200.ir import HostTensor
+
+pytestmark = pytest.mark.gpu
+
+VOCAB, MORE, WIDTH = 40, 9, 16
+
+
+def engine(max_seqs=4):
+    """Logits of `VOCAB` tokens, embeddings of `MORE` beyond them (places of a prompt that no answer has): each token's logits are those of its embedding alone."""
+    r = np.random.default_rng(0)
+    embed, head = r.standard_normal((VOCAB + MORE, WIDTH)).astype(np.float32), r.standard_normal((WIDTH, VOCAB)).astype(np.float32)
+    b = ir.GraphBuilder()
+    N, R, TW, W = b.sym("num_tokens"), b.sym("num_seqs"), b.sym("table_width"), b.sym("num_logits")
+    ids = b.input("input_ids", ir.I64, [N])
+    b.input("seq_info", ir.I32, [R, 4])
+    b.input("page_table", ir.I32, [R, TW])
+    rows = b.input("logit_rows", ir.I64, [W])
+    const = lambda a: b.constant(HostTensor.from_numpy(a))  # noqa: E731
+    b.output("logits", b.matmul(b.gather(b.gather(const(embed), ids, 0), rows, 0), const(head)))
+    return Engine(cuda_backend().prepare(b.finish()), 256, max_seqs), (embed @ head).astype(np.float64)
+
+
+def answer(e, request):
+    out = []
+    while e.stats()["waiting"] + e.stats()["running"]:
+        out += [t for q, t, _ in e.step() if q == request]
+    return out
+
+
+def expected(logits, prompt, n, repetition=1.0, frequency=0.0, presence=0.0):
+    said = []
+    for _ in range(n):
+        x = logits[(prompt + said)[-1]].copy()
+        for t in set(prompt + said):
+            if t < VOCAB:
+                x[t] = x[t] / repetition if x[t] > 0 else x[t] * repetition
+        for t in set(said):
+            x[t] -= said.count(t) * frequency + presence
+        said.append(int(np.argmax(x)))
+    return said
+
+
+@pytest.mark.parametrize("rules", [dict(repetition=1.9), dict(frequency=3.0), dict(repetition=1.3, presence=2.0)], ids=str)
+def test_tokens_of_a_prompt_that_have_no_logit_have_no_penalty(rules):
+    e, logits = engine()
+    prompt = [3, VOCAB, 7, VOCAB + MORE - 1, 7, VOCAB + 2]
+    assert answer(e, e.submit(prompt, 8)) == expected(logits, prompt, 8)
+    assert answer(e, e.submit(prompt, 8, **rules)) == expected(logits, prompt, 8, **rules) != expected(logits, prompt, 8)
+    only = [VOCAB, VOCAB + 1]
+    assert answer(e, e.submit(only, 8, **rules)) == expected(logits, only, 8, **rules)

@@ -428,8 +428,8 @@ ox_status ox_engine_step(ox_engine*, int32_t token_budget, ox_engine_token* toke
 ox_status ox_engine_cancel(ox_engine*, int64_t request);
 /* Rules on the tokens that an unfinished request has still to generate, as ox_session_constrain_last applies them: its history is its prompt
  * and what it has generated. Each call replaces what the one before it said. `allowed` has a bit per token of the vocabulary
- * (ceil(vocab / 32) words, lowest bit first), at least one of them set; NULL allows all again. A grammar sets it before every step. Biases (each a number, or minus infinity) and
- * allowed tokens have to leave one. */
+ * (ceil(vocab / 32) words, lowest bit first), at least one of them set; NULL allows all again. A grammar sets it before every step. Biases (each a number, or minus infinity;
+ * those of one token add up to no more than f32 holds) and allowed tokens have to leave one. */
 ox_status ox_engine_constrain(ox_engine*, int64_t request, float repetition, float frequency, float presence, const int32_t* bias_ids,
                               const float* bias, int32_t n_bias);
 ox_status ox_engine_allow(ox_engine*, int64_t request, const uint32_t* allowed, size_t n_words);

@@ -214,15 +214,26 @@ Engine::Request& Engine::request_of(int64_t id) {
     fail(ErrKind::Binding, "no unfinished request " + std::to_string(id));
 }
 
-// Whether some token of `vocab` is allowed and has not minus infinity for its bias.
+// What the biases of each token add up to, in their order and in f32 as the kernel does: (token, sum).
+static std::vector<std::pair<int32_t, float>> bias_sums(const Engine::Rules& r) {
+    std::vector<std::pair<int32_t, float>> sums;
+    for (size_t i = 0; i < r.bias.size(); i++) sums.emplace_back(r.bias_ids[i], r.bias[i]);
+    std::stable_sort(sums.begin(), sums.end(), [](const auto& a, const auto& b) { return a.first < b.first; });
+    size_t n = 0;
+    for (size_t i = 0; i < sums.size(); i++) {
+        if (n && sums[n - 1].first == sums[i].first) sums[n - 1].second += sums[i].second;
+        else sums[n++] = sums[i];
+    }
+    sums.resize(n);
+    return sums;
+}
+
+// Whether some token of `vocab` is allowed and has not minus infinity for its biases.
 static bool leaves_a_token(const Engine::Rules& r, int64_t vocab) {
-    std::vector<int32_t> barred;
-    for (size_t i = 0; i < r.bias.size(); i++)
-        if (r.bias[i] == -INFINITY && (r.allowed.empty() || (r.allowed[(size_t)r.bias_ids[i] / 32] >> (r.bias_ids[i] % 32) & 1u))) barred.push_back(r.bias_ids[i]);
-    std::sort(barred.begin(), barred.end());
     int64_t left = r.allowed.empty() ? vocab : 0;
     for (uint32_t w : r.allowed) left += __builtin_popcount(w);
-    return left > std::unique(barred.begin(), barred.end()) - barred.begin();
+    for (auto& [token, sum] : bias_sums(r)) left -= sum == -INFINITY && (r.allowed.empty() || (r.allowed[(size_t)token / 32] >> (token % 32) & 1u));
+    return left > 0;
 }
 
 void Engine::constrain(int64_t request, float repetition, float frequency, float presence, std::vector<int32_t> bias_ids, std::vector<float> bias) {
@@ -235,6 +246,8 @@ void Engine::constrain(int64_t request, float repetition, float frequency, float
         if (std::isnan(bias[i]) || bias[i] == INFINITY) fail(ErrKind::Attribute, "a bias is a number, or minus infinity");
     }
     Rules rules{repetition, frequency, presence, std::move(bias_ids), std::move(bias), r.rules.allowed};
+    for (auto& [token, sum] : bias_sums(rules))
+        if (sum == INFINITY) fail(ErrKind::Attribute, "the biases of token " + std::to_string(token) + " add up to more than f32 holds");
     if (!leaves_a_token(rules, vocab_)) fail(ErrKind::Shape, "the biases leave no token");
     r.rules = std::move(rules);
 }
@@ -449,7 +462,8 @@ ox_status ox_engine_step(ox_engine* h, int32_t token_budget, ox_engine_token* to
 ox_status ox_engine_constrain(ox_engine* h, int64_t request, float repetition, float frequency, float presence, const int32_t* bias_ids, const float* bias,
                               int32_t n_bias) {
     OX_TRY
-    const size_t n = (size_t)std::max(n_bias, 0);
+    if (n_bias < 0 || (n_bias > 0 && (!bias_ids || !bias))) ox::fail(ox::ErrKind::Shape, "biases without their tokens or values");
+    const size_t n = (size_t)n_bias;
     h->e->constrain(request, repetition, frequency, presence, std::vector<int32_t>(bias_ids, bias_ids + n), std::vector<float>(bias, bias + n));
     return OX_OK;
     OX_CATCH

@@ -57,3 +57,37 @@ def test_tokens_of_a_prompt_that_have_no_logit_have_no_penalty(rules):
     assert answer(e, e.submit(prompt, 8, **rules)) == expected(logits, prompt, 8, **rules) != expected(logits, prompt, 8)
     only = [VOCAB, VOCAB + 1]
     assert answer(e, e.submit(only, 8, **rules)) == expected(logits, only, 8, **rules)
+
+
+def constrain(e, request, ids, values, n=None):
+    ids, values = np.array(ids, np.int32), np.array(values, np.float32)
+    at = lambda a, kind: a.ctypes.data_as(C.POINTER(kind)) if a.size else None  # noqa: E731
+    _ffi.check(_ffi.cuda_lib().ox_engine_constrain(e._h, request, 1.0, 0.0, 0.0, at(ids, C.c_int32), at(values, C.c_float), len(ids) if n is None else n))
+
+
+def test_biases_that_add_up():
+    """A token may be listed more than once. What its biases add up to is a number, or minus infinity; minus infinity for all tokens is refused however it comes about."""
+    e, logits = engine()
+    big = float(np.finfo(np.float32).max)
+    r = e.submit([3], 2)
+    with pytest.raises(OnyxiaError, match="biases of token 5 add up"):
+        constrain(e, r, [5, 7, 5], [big, 1.0, big])
+    with pytest.raises(OnyxiaError, match="leave no token"):
+        constrain(e, r, list(range(VOCAB)) * 2, [-big] * VOCAB * 2)
+    constrain(e, r, list(range(VOCAB - 1)) * 2, [-big] * (VOCAB - 1) * 2)
+    with pytest.raises(OnyxiaError, match="leave no token"):
+        e.allow(r, [4, 5])
+    assert answer(e, r) == [VOCAB - 1] * 2
+    r = e.submit([3], 1)
+    constrain(e, r, [5, 5, 5], [big, -big, 100.0])
+    assert answer(e, r) == [5]
+
+
+def test_biases_without_tokens_or_values_are_refused_at_the_c_entry():
+    e, _ = engine()
+    r = e.submit([3], 1)
+    for ids, values, n in (([], [], 3), ([], [], -1), ([4], [], 1), ([], [1.0], 1)):
+        with pytest.raises(OnyxiaError, match="without their tokens or values"):
+            constrain(e, r, ids, values, n)
+    constrain(e, r, [], [], 0)
+    assert len(answer(e, r)) == 1

@@ -670,8 +670,21 @@ void Session::interleave_weights() {
     OX_CUDA(cudaStreamSynchronize(stream_));
 }
 
+// A caller's shape: one whose elements do not count up in 64 bits would be taken for a small one.
+static void check_extents(const std::vector<int64_t>& shape) {
+    uint64_t n = 1;
+    bool none = false;
+    for (int64_t d : shape) {
+        if (d < 0) fail(ErrKind::Shape, "a tensor's extent is not above 2^63 - 1");
+        none = none || d == 0;
+        if (!none && __builtin_mul_overflow(n, (uint64_t)d, &n)) n = UINT64_MAX;
+    }
+    if (!none && n > (uint64_t)INT64_MAX / 64) fail(ErrKind::Shape, "a tensor of more elements than memory can hold");
+}
+
 DTensor Session::upload(DType dtype, const std::vector<int64_t>& shape, const void* bytes, size_t nbytes) {
     OX_CUDA(cudaSetDevice(device_));
+    check_extents(shape);
     DTensor t;
     t.dtype = dtype;
     t.shape = shape;
@@ -743,6 +756,7 @@ void Session::order(cudaStream_t first, cudaStream_t then) {
 
 DTensor Session::upload_device(DType dtype, const std::vector<int64_t>& shape, const void* bytes, size_t nbytes, cudaStream_t stream) {
     OX_CUDA(cudaSetDevice(device_));
+    check_extents(shape);
     DTensor t;
     t.dtype = dtype;
     t.shape = shape;

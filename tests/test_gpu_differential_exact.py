@@ -133,3 +133,22 @@ def test_what_lies_behind_the_last_key_changes_no_bit(f):
     live = np.concatenate([np.arange(r, r + n) for r, n, _, _ in s.seqs])
     for other in outs[1:]:
         assert np.array_equal(other[live], outs[0][live])
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("lengths,tail", [([(0, 5)], 3), ([(0, 5), (0, 70), (0, 0)], 3), ([(0, 5), (0, 70), (0, 0)], 9), ([(2, 3), (0, 70), (0, 0)], 0), ([(2, 3), (0, 70), (0, 0)], 9)], ids=str)
+def test_sequences_without_new_tokens_leave_the_pools_alone(lengths, tail, kind):
+    """Rows of nobody behind them or not; the first run, and replayed ones."""
+    f = Form(4, 2, 64, 128, 64)
+    act = HostTensor.bf16 if kind == "bf16" else lambda a: HostTensor.from_numpy(np.asarray(a, np.float32))
+    s = util.step(f, lengths, tail=tail)
+    session = cuda_backend().prepare(util.module(f, ir.BF16 if kind == "bf16" else ir.F32, s.lam, s.gain))
+    dev = {k: session.upload(v) for k, v in util.feed(s, act).items()}
+    keys, values = util.reference(f, s, to_bf16 if kind == "bf16" else lambda a: np.asarray(a, np.float32))[1:]
+    for _ in range(3):
+        outs = dict(session.run(dev))
+        dev["pages.keys"], dev["pages.values"] = outs["updated.pages.keys"], outs["updated.pages.values"]
+        assert np.array_equal(session.download(dev["pages.values"]).numpy(), values.astype(np.float32), equal_nan=True)
+        got = session.download(dev["pages.keys"]).numpy()
+        old = ~np.isnan(s.keys)
+        assert np.array_equal(got[old], s.keys[old]) and np.array_equal(np.isnan(got), np.isnan(keys))

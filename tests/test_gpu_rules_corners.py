@@ -4,6 +4,7 @@ import ctypes as C
 import numpy as np
 import pytest
 
+import test_gpu_rules as plain
 from gpu_util import cuda_backend
 from onyxia_b200 import OnyxiaError, _ffi, ir
 from onyxia_b200.engine import Engine
@@ -91,3 +92,21 @@ def test_biases_without_tokens_or_values_are_refused_at_the_c_entry():
             constrain(e, r, ids, values, n)
     constrain(e, r, [], [], 0)
     assert len(answer(e, r)) == 1
+
+
+@pytest.mark.parametrize("dtype", [np.float32, np.float16])
+@pytest.mark.parametrize("rows,vocab", [(1, 1), (3, 33), (5, 4097), (3, 50021), (64, 8192)])
+def test_every_result_is_a_number_and_close(rows, vocab, dtype):
+    """Every place where the plain implementation has a number, those under rules among them: no NaN hides there. Tolerance: that of test_gpu_rules.py."""
+    r = np.random.default_rng(vocab)
+    x = (4.0 * r.standard_normal((rows, vocab))).astype(dtype)
+    b = ir.GraphBuilder()
+    b.output("one", b.const_f32([1.0], [1]))
+    session = cuda_backend().prepare(b.finish())
+    for width, n_bias, n_masks in ((0, 0, 0), (40, 7, 0), (700, 300, 3), (30, 0, 2), (0, 20, 0)):
+        more = plain.rules(rows, vocab, width, n_bias, n_masks, seed=rows)
+        got = session.download(session.constrain_last(session.upload(HostTensor.from_numpy(x)), **{k: session.upload(HostTensor.from_numpy(v)) for k, v in more.items()})).numpy()
+        want = plain.reference(x, **more)
+        assert not np.isnan(got).any() and np.array_equal(np.isfinite(got), np.isfinite(want))
+        there = np.isfinite(want)
+        assert np.max(np.abs(got[there] - want[there]), initial=0.0) <= plain.TOL

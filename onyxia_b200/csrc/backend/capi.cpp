@@ -268,6 +268,7 @@ ox_status ox_session_sample_last(ox_session* s, const ox_tensor* logits, float t
 
 ox_status ox_session_constrain_last(ox_session* s, const ox_tensor* logits, const ox_logit_rules* rules, ox_tensor** out) {
     OX_TRY
+    if (!logits || !rules) fail(ErrKind::Binding, "rules need logits, and a description of themselves");
     auto of = [](const ox_tensor* t) { return t ? &t->t : nullptr; };
     oxrt::Rules r;
     r.history = of(rules->history), r.lengths = of(rules->lengths), r.penalties = of(rules->penalties);

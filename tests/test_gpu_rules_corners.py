@@ -110,3 +110,14 @@ def test_every_result_is_a_number_and_close(rows, vocab, dtype):
         assert not np.isnan(got).any() and np.array_equal(np.isfinite(got), np.isfinite(want))
         there = np.isfinite(want)
         assert np.max(np.abs(got[there] - want[there]), initial=0.0) <= plain.TOL
+
+
+def test_null_logits_and_rules_are_refused_at_the_c_entry():
+    b = ir.GraphBuilder()
+    b.output("one", b.const_f32([1.0], [1]))
+    session, out = cuda_backend().prepare(b.finish()), C.c_void_p()
+    x, rules = session.upload(HostTensor.from_numpy(np.ones((1, 8), np.float32))), _ffi.LogitRules()
+    for logits, described in ((None, C.byref(rules)), (x.handle, None), (None, None)):
+        with pytest.raises(OnyxiaError, match="rules need logits"):
+            _ffi.check(_ffi.cuda_lib().ox_session_constrain_last(session._h, logits, described, C.byref(out)))
+    assert (session.download(session.constrain_last(x)).numpy() == 1.0).all()

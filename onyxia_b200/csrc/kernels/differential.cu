@@ -14,6 +14,8 @@
 //   differential_several   sequences with several new tokens beside empty ones, in batches of fewer rows than sequences
 //
 // Decode reads min(past, window) · kv_heads · (2 · dim + vdim) · 2 bytes per sequence.
+#include <cmath>
+
 #include "differential.cuh"
 
 namespace oxk {
@@ -320,7 +322,7 @@ template <int DV> __device__ void merge_maps(const DiffP& p, const float* part, 
 }
 
 // Grid: (splits, kv_heads · groups of 8 query heads, sequences). Both maps of eight heads of one key head share each tile of 16 keys and values, which a warp copies for itself.
-template <int DM, int DV> __global__ void __launch_bounds__(kDecThreads) differential_decode(const DiffP p) {
+template <int DM, int DV, bool LOW> __global__ void __launch_bounds__(kDecThreads) differential_decode(const DiffP p) {
     extern __shared__ __align__(16) unsigned char smem[];
     __shared__ unsigned arrived;
     __shared__ int page_s[kDecPages];  // this CTA's pages, checked
@@ -532,23 +534,29 @@ template <int DM, int DV> __global__ void __launch_bounds__(kDecThreads) differe
                     }
                 }
         }
-        unsigned pb[2][2];
+        unsigned pb[2][2], rest[2][2];
 #pragma unroll
         for (int m = 0; m < 2; m++)
 #pragma unroll
             for (int r = 0; r < 2; r++) {
-                const unsigned w = pack_bf16(exp2f(s[m][2 * r] - top[m][0]), exp2f(s[m][2 * r + 1] - top[m][1]));
+                const float w0 = exp2f(s[m][2 * r] - top[m][0]), w1 = exp2f(s[m][2 * r + 1] - top[m][1]);
+                const unsigned w = pack_bf16(w0, w1);
+                const float h0 = __uint_as_float(w << 16), h1 = __uint_as_float(w & 0xFFFF0000u);
                 // the sums of the weights as they are multiplied: the rounding of a weight that stands out is in both
-                l[m][0] += __uint_as_float(w << 16);
-                l[m][1] += __uint_as_float(w & 0xFFFF0000u);
+                l[m][0] += LOW ? w0 : h0;
+                l[m][1] += LOW ? w1 : h1;
                 pb[m][r] = transpose8x8(w);
+                if constexpr (LOW) rest[m][r] = transpose8x8(pack_bf16(w0 - h0, w1 - h1));
             }
 #pragma unroll
         for (int n = 0; n < DV / 16; n++) {
             unsigned va[4];
             ldmatrix_x4_trans(va, vs + ((lane >> 4) * 8 + (lane & 7)) * L::v_stride + n * 32 + ((lane >> 3) & 1) * 16);
 #pragma unroll
-            for (int m = 0; m < 2; m++) mma_bf16(o[m][n], va[0], va[1], va[2], va[3], pb[m][0], pb[m][1]);
+            for (int m = 0; m < 2; m++) {
+                mma_bf16(o[m][n], va[0], va[1], va[2], va[3], pb[m][0], pb[m][1]);
+                if constexpr (LOW) mma_bf16(o[m][n], va[0], va[1], va[2], va[3], rest[m][0], rest[m][1]);
+            }
         }
         __syncwarp();
     }
@@ -596,8 +604,8 @@ struct DecChoice {
     DiffKernel kernel;
     int smem, part;
 };
-template <int DM, int DV> DecChoice choice() { return {differential_decode<DM, DV>, DecSmem<DM, DV>::total, DecSmem<DM, DV>::part}; }
-template <int DM> DecChoice choice(int64_t vdim) { return vdim <= 64 ? choice<DM, 64>() : vdim <= 128 ? choice<DM, 128>() : choice<DM, 256>(); }
+template <int DM, int DV> DecChoice choice(bool low) { return {low ? differential_decode<DM, DV, true> : differential_decode<DM, DV, false>, DecSmem<DM, DV>::total, DecSmem<DM, DV>::part}; }
+template <int DM> DecChoice choice(int64_t vdim, bool low) { return vdim <= 64 ? choice<DM, 64>(low) : vdim <= 128 ? choice<DM, 128>(low) : choice<DM, 256>(low); }
 
 }  // namespace
 
@@ -639,6 +647,11 @@ void emit_differential(Emitter& em, const DifferentialDesc& d, const TRef& proj,
     p.singles = !tc || (!p.only && n_seqs == 1);       // a lone token with rows of nobody behind it
     const bool prefill = tc && !p.only && differential_prefill_fits(p, keys, values, out.buf.off);
     p.parts = prefill;
+    // Weights as the sum of two bf16 where scores are known not to spread: of queries and keys that are normed (their products spread by dim^1/2) or of a tight cap. Nearly equal weights of two maps cancel,
+    // their roundings do not. Off from 64-bit results with one bf16 → with two (1 500 keys): normed, scores of a spread of 1 2.5e-3 → 1.66e-3 (prompts), 2.3e-3 → 1.66e-3 (tokens), which is the results' own
+    // rounding; of 1.25 2.4e-3, of 2 2.2e-3, without a norm and of 1.5 2.3e-3; capped at 1 2.66e-3, at 2 2.64e-3. Time, one after the other: 4096 tokens, 32 heads of 2 x 64 over 16 393 → 475 us,
+    // normed 464 → 528; 2048, 16 over 4 79 → 86, normed 92 → 104; 1999 capped and normed behind 1000, 4 heads of 2 x 128 77 → 89; 64 tokens behind 2047, 32 over 16 212 → 224, other tokens 1 %.
+    p.low = (d.norm && std::fabs(d.scale) * std::sqrt((double)d.dim) <= 1.25) || (d.softcap > 0 && d.softcap <= 3.0);
     auto by = [](int64_t d) { return d > 1 ? (unsigned)(((1ull << 32) + d - 1) / d) : 0u; };
     p.rep = d.heads / d.kv_heads;
     p.by_rep = by(p.rep);
@@ -672,7 +685,7 @@ void emit_differential(Emitter& em, const DifferentialDesc& d, const TRef& proj,
     }
     if (p.only && rows > 1 && rows < n_seqs) launch(differential_several, dim3((unsigned)d.kv_heads, (unsigned)n_seqs), kAnyKeys, (unsigned)((d.dim + d.vdim + kAnyKeys) * 8 + d.rot_dims * 8), none, "differential_several");
     if (tc && (p.only || n_seqs > 1)) {
-        const DecChoice dc = d.dim <= 32 ? choice<32>(d.vdim) : d.dim <= 64 ? choice<64>(d.vdim) : choice<128>(d.vdim);
+        const DecChoice dc = d.dim <= 32 ? choice<32>(d.vdim, p.low) : d.dim <= 64 ? choice<64>(d.vdim, p.low) : choice<128>(d.vdim, p.low);
         const int64_t groups = d.kv_heads * ((d.heads / d.kv_heads + kDecHeads - 1) / kDecHeads), cells = n_seqs * groups;
         // Splits of the most keys a sequence can see: whole waves of resident CTAs, and the pieces have to be merged. A CTA's beginning and end cost as much as 200 KB of keys and values
         // (64 sequences behind 2047, 32 heads of 2 x 64 over 16, us for 1, 2, 4, 8 splits: 223, 246, 291, 369; four that see 4096 keys: 90, 60, 52, 58).

@@ -26,6 +26,7 @@ struct DiffP {
     int parts;                   // prepare: queries in two parts, times mul2
     int by8;                     // the parts of a projection row begin on 16 bytes
     int only;                    // no sequence may have more than one
+    int low;                     // weights are the sum of two bf16
     int rep;                     // heads of a key head
     unsigned by_rep, by_units, by_lanes;  // 2^32 / (heads of a key head, units of a query, sixteen bytes of a value), rounded up; 0: of one
 };

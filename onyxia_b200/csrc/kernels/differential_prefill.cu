@@ -10,6 +10,8 @@
 // Measured alone, L2 cold: 4096 tokens, 32 heads of 2 × 64 over 16, values of 128 (137 GFLOP) 289 us, 476 TFLOP/s, 950 with the queries' low part and a product of the values per map;
 // 2048, 16 over 4 60 us; 1999 capped behind 1000, 4 heads of 2 × 128 over one 60 us. A step of 64 keys takes 1 600 cycles with two CTAs per SM: products need 640 of an SM's 800, exponentials
 // 512; what bounds it is their order within a CTA, and a third CTA has no tensor memory. A tile's beginning and end take 16 000 cycles, half of them under the other CTA's steps.
+#include <type_traits>
+
 #include "differential.cuh"
 
 namespace oxk {
@@ -170,12 +172,13 @@ struct PagesAhead {
     }
 };
 
+// LOW: weights are the sum of two bf16 (emit_differential says where). Both are multiplied; their places are those of two turns, so a tile's are written behind the products of the tile before it.
 // KEYS 64: 256 columns of tensor memory (values of up to 128), two CTAs per SM, which work under each other's waits. 128: all columns.
 template <int KEYS> struct Shape {
     static constexpr int halves = KEYS / kPart, soft = halves * kRows, threads = soft + 64;  // softmax warps, one of copies, one that issues products
     static constexpr int keys = KEYS == 64 ? 3 : 2, values = KEYS == 64 ? 3 : 2;             // tiles of keys and halves of values on their way
 };
-template <bool CAPPED, int KEYS> __global__ void __launch_bounds__(Shape<KEYS>::threads, KEYS == 64 ? 2 : 1) differential_prefill(const __grid_constant__ PreP pp) {
+template <bool CAPPED, int KEYS, bool LOW> __global__ void __launch_bounds__(Shape<KEYS>::threads, KEYS == 64 ? 2 : 1) differential_prefill(const __grid_constant__ PreP pp) {
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     // (both CTAs of a cluster find the same place: their shared memory begins at the same address)
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
@@ -224,6 +227,8 @@ template <bool CAPPED, int KEYS> __global__ void __launch_bounds__(Shape<KEYS>::
     // Waits until the products of tile i are in the sums. Tiles take turns at two barriers, and who asks has seen the scores of tile i + 1 (or i, the last) and not let the products of
     // tile i + 2 begin. Products are done in the order of their issue, those of tile i − 1 in front of the scores of tile i + 1: the barrier is neither a round behind nor ahead.
     auto added = [&](int i) { return mbar_wait(o_done + (i & 1) * 8, (unsigned)(i >> 1) & 1); };
+    // Where the weights of half h of tile i are: two turns, or (LOW) one, whose low parts lie behind them.
+    auto weights_of = [&](int i, int h) { return tmem + KEYS + (LOW ? 0 : (i & 1) * (KEYS / 2)) + h * (kPart / 2); };
     // Whether some row of the CTA may see keys of half h of the tile that begins at j0. Halves that nobody sees are neither copied nor multiplied.
     auto seen = [&](int j0, int h) { return j0 + h * kPart <= last && j0 + h * kPart + kPart > low; };
 
@@ -309,8 +314,11 @@ template <bool CAPPED, int KEYS> __global__ void __launch_bounds__(Shape<KEYS>::
                 if (elect_one() && ok) {
                     const unsigned long long v = dv + values_at.s * (v_stage >> 4);
 #pragma unroll
-                    for (int e = 0; e < kPart / 16; e++)
-                        umma_weights(t_sum, tmem + KEYS + (i & 1) * (KEYS / 2) + h * (kPart / 2) + e * 8, v + e * 128, by_values, some || e > 0);
+                    for (int e = 0; e < kPart / 16; e++) umma_weights(t_sum, weights_of(i, h) + e * 8, v + e * 128, by_values, some || e > 0);
+                    if (LOW) {
+#pragma unroll
+                        for (int e = 0; e < kPart / 16; e++) umma_weights(t_sum, weights_of(i, h) + KEYS / 2 + e * 8, v + e * 128, by_values, true);
+                    }
                     umma_commit(v_free + values_at.s * 8);
                 }
                 __syncwarp();
@@ -383,9 +391,9 @@ template <bool CAPPED, int KEYS> __global__ void __launch_bounds__(Shape<KEYS>::
             if (kHalves == 2) top = fmaxf(top, both(i & 1, top));
             // Weights are taken against a maximum that may lie up to 2^8 behind, so that the sums are rarely taken anew. The largest weight is then rounded as the others are, where against the maximum itself
             // it is 1; the sums, of the weights as they are multiplied, are off with it, so a key that takes all weight costs nothing either way. Off from 64-bit results, behind → against the maximum
-            // itself: 2.31e-3 → 2.12e-3 (1500 keys, scores of a spread of 1.5; of 4: 1.90e-3 → 1.76e-3), 2.60e-3 → 2.49e-3 (normed, 2000 keys), 4.07e-3 → 4.16e-3 (scores nearly equal); the rounding of the
+            // itself: 2.31e-3 → 2.12e-3 (1500 keys, scores of a spread of 1.5; of 4: 1.90e-3 → 1.76e-3), 4.07e-3 → 4.16e-3 (scores nearly equal); the rounding of the
             // results alone is 1.66e-3. It would take 22 % of time (4096 tokens, 32 heads of 2 x 64 over 16; 2048, 16 over 4: 14 %; 1999 behind 1000, 4 heads of 2 x 128: 15 %).
-            // Both warps of a row see the same tops.
+            // (LOW: both parts of a weight are there either way.) Both warps of a row see the same tops.
             if (__any_sync(0xffffffffu, top > m + kLazy)) {
                 top = fmaxf(top, m);
                 const float keep = ex2(m - top);
@@ -410,19 +418,39 @@ template <bool CAPPED, int KEYS> __global__ void __launch_bounds__(Shape<KEYS>::
             // (these weights' place is free: with the scores of tile i the products of tile i − 2 are done)
             if (seen(j0, part)) {
                 const f32x2 behind = pair_of(-m, -m);
+                if constexpr (LOW) {
+                    unsigned w[32], rest[32];
 #pragma unroll
-                for (int c = 0; c < 2; c++) {
-                    unsigned w[16];
-#pragma unroll
-                    for (int e = 0; e < 16; e++) {
+                    for (int e = 0; e < 32; e++) {
                         float a, b;
-                        apart(add2(pair_of(s[c * 32 + 2 * e], s[c * 32 + 2 * e + 1]), behind), a, b);
-                        w[e] = pack_bf16(ex2(a), ex2(b));
-                        // The sums of the weights as they are multiplied: the rounding of a weight that stands out is in both. Adding bf16 to f32 as they are, four sums at a time, 64 keys of
-                        // a row take 660 cycles, of which the exponentials need 512; unpacked, two sums, 900.
-                        add_bf16(sums[(e & 1) * 2], sums[(e & 1) * 2 + 1], w[e]);
+                        apart(add2(pair_of(s[2 * e], s[2 * e + 1]), behind), a, b);
+                        a = ex2(a), b = ex2(b);
+                        w[e] = pack_bf16(a, b);
+                        rest[e] = pack_bf16(a - __uint_as_float(w[e] << 16), b - __uint_as_float(w[e] & 0xFFFF0000u));
+                        sums[(e & 1) * 2] += a, sums[(e & 1) * 2 + 1] += b;
                     }
-                    tmem_st16(tmem + lanes + KEYS + (i & 1) * (KEYS / 2) + part * (kPart / 2) + c * 16, w);
+                    if (i > 0 && ok && !added(i - 1)) ok = false;  // the last tile's weights have been multiplied
+                    after_sync();
+#pragma unroll
+                    for (int c = 0; c < 2; c++) {
+                        tmem_st16(weights_of(i, part) + lanes + c * 16, *reinterpret_cast<const unsigned(*)[16]>(w + c * 16));
+                        tmem_st16(weights_of(i, part) + lanes + KEYS / 2 + c * 16, *reinterpret_cast<const unsigned(*)[16]>(rest + c * 16));
+                    }
+                } else {
+#pragma unroll
+                    for (int c = 0; c < 2; c++) {
+                        unsigned w[16];
+#pragma unroll
+                        for (int e = 0; e < 16; e++) {
+                            float a, b;
+                            apart(add2(pair_of(s[c * 32 + 2 * e], s[c * 32 + 2 * e + 1]), behind), a, b);
+                            w[e] = pack_bf16(ex2(a), ex2(b));
+                            // The sums of the weights as they are multiplied: the rounding of a weight that stands out is in both. Adding bf16 to f32 as they are, four sums at a time, 64 keys of
+                            // a row take 660 cycles, of which the exponentials need 512; unpacked, two sums, 900.
+                            add_bf16(sums[(e & 1) * 2], sums[(e & 1) * 2 + 1], w[e]);
+                        }
+                        tmem_st16(weights_of(i, part) + lanes + c * 16, w);
+                    }
                 }
                 if (j1 + kPart - 1 > last || j1 < low) {  // what lies behind the last key or in front of the first may be no number, which a weight of 0 would not cancel
                     const int at = halves + before, stage = at % kStagesV;
@@ -581,8 +609,12 @@ void emit_differential_prefill(Emitter& em, const DiffP& kv, const TRef& keys, c
     p.inv = (65536 + kv.heads / kv.kv_heads - 1) / (kv.heads / kv.kv_heads);
     const int64_t tq = kRows / (kv.heads / kv.kv_heads), rows = (int64_t)kv.n_pages * kv.kv_heads << kv.shift;
     p.tiles = (int)((kv.rows + tq - 1) / tq + kv.n_seqs);
-    void (*const k)(const PreP) = differential_keys(p.kp, p.vp) == 64 ? (kv.cap2 > 0.f ? differential_prefill<true, 64> : differential_prefill<false, 64>)
-                                                                     : (kv.cap2 > 0.f ? differential_prefill<true, 128> : differential_prefill<false, 128>);
+    auto form = [&](auto capped, auto low) -> void (*)(const PreP) {
+        return differential_keys(p.kp, p.vp) == 64 ? differential_prefill<capped.value, 64, low.value> : differential_prefill<capped.value, 128, low.value>;
+    };
+    const std::true_type yes;
+    const std::false_type no;
+    void (*const k)(const PreP) = kv.cap2 > 0.f ? (kv.low ? form(yes, yes) : form(yes, no)) : (kv.low ? form(no, yes) : form(no, no));
     const int smem = differential_prefill_smem(p.kp, p.vp);
     ensure_max_dynamic_smem((const void*)k, 226 * 1024);
     LaunchRec& rec = em.launch(k, dim3((unsigned)p.tiles * (unsigned)kv.kv_heads * 2), dim3(differential_keys(p.kp, p.vp) == 64 ? Shape<64>::threads : Shape<128>::threads), (unsigned)smem, p, {}, "differential_prefill", /*pdl=*/true);

@@ -64,11 +64,13 @@ def exact(f, s, stored):
     return out, due
 
 
-def share(f, s, got, stored):
-    """Error of all results together as a share of what they are due: sqrt(mean of (error / result)²) over sqrt(mean of ROUNDING² (1 + D²)), over (row, head)."""
+def share(f, s, got, stored, two_parts=False):
+    """Error of all results together as a share of what they are due: sqrt(mean of (error / result)²) over sqrt(mean of ROUNDING² (1 + D²)), over (row, head). With weights in two bf16 (2^-17)
+    results are due their own rounding alone."""
     want, due = exact(f, s, stored)
     live = ~np.isnan(due[:, 0])
     got, want, due = got.reshape(want.shape)[live].astype(np.float64), want[live], due[live]
     assert np.isfinite(got).all()
     off = ((got - want) ** 2).mean(-1) / (want ** 2).mean(-1)
+    due = 0.0 * due if two_parts else due
     return float(np.sqrt(off.mean() / (ROUNDING ** 2 * (1.0 + due ** 2)).mean()))

@@ -152,3 +152,27 @@ def test_sequences_without_new_tokens_leave_the_pools_alone(lengths, tail, kind)
         got = session.download(dev["pages.keys"]).numpy()
         old = ~np.isnan(s.keys)
         assert np.array_equal(got[old], s.keys[old]) and np.array_equal(np.isnan(got), np.isnan(keys))
+
+
+@pytest.mark.parametrize("f", [NARROW, WIDE, WIDE_VALUES, Form(20, 2, 48, 96, 48)], ids=["narrow", "wide", "wide values", "many heads"])
+@pytest.mark.parametrize("more", [dict(norm=1), dict(norm=1, sink=1, softcap=30.0, window=700), dict(softcap=1.0), dict(softcap=3.0, sink=1)], ids=str)
+@pytest.mark.parametrize("lengths", [[(700, 900), (130, 60), (1, 400)], [(1, 1000 + 37 * i) for i in range(40)]], ids=["prompts", "tokens"])
+def test_scores_that_do_not_spread_cost_no_precision(f, more, lengths):
+    """Normed queries and keys, and tight caps: where maps of nearly equal weights are taken from each other, D is 1.2 and more, and results are off by their own rounding all the same."""
+    f = Form(f.heads, f.kv_heads, f.dim, f.vdim, f.rot_dims, **more)
+    s = util.step(f, lengths, 17)
+    assert exact.share(f, s, results(f, s)[0], to_bf16, two_parts=True) <= DUE
+
+
+@pytest.mark.parametrize("f", [NARROW, WIDE], ids=["narrow", "wide"])
+@pytest.mark.parametrize("by", [0.05, 3.0])
+def test_maxima_that_rise_with_weights_in_two_parts(f, by):
+    """The weights of a tile are written behind the products of the tile before it, the sums scaled in front of them."""
+    f = Form(f.heads, f.kv_heads, f.dim, f.vdim, 0, softcap=3.0)
+    s = util.step(f, [(700, 900), (130, 60)], 7)
+    rising(f, s, by)
+    first, *more = results(f, s, 6)
+    assert exact.share(f, s, first, to_bf16, two_parts=True) <= DUE
+    live = np.concatenate([np.arange(r, r + n) for r, n, _, _ in s.seqs])
+    for again in more:
+        assert np.array_equal(again[live], first[live])

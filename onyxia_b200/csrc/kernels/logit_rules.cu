@@ -7,8 +7,8 @@
 //
 // in f32, the result too (a half-precision logit times a penalty would be rounded again and could leave its range).
 //
-// A CTA takes a run of one row's vocabulary: it counts the row's history in shared memory (whole numbers: no order shows), streams the run and, last, writes the few
-// biased tokens again. The history is read once per run. Bound by the logits' bytes: read once, written once as f32.
+// A CTA takes a run of one row's vocabulary: it counts the row's history in shared memory (whole numbers: no order shows), adds up the biases of its tokens there, streams the run and, last, writes
+// the few biased tokens again. The history and the biased tokens are read once per run. Bound by the logits' bytes: read once, written once as f32.
 // 64 rows of 262144 with 2048 tokens of history, masks and biases each (134 MB): 30 us on top of a call of one row; 40 us where the history waits for its length and the mask is
 // asked for token by token. Runs of 8192 (half as many readings of the history, half as many CTAs per SM): 37.
 #include "common.cuh"
@@ -39,6 +39,7 @@ struct RulesP {
 template <int DT, int PER, bool VEC> __global__ void __launch_bounds__(kRuleThreads) constrain_rows(const RulesP p) {
     constexpr int kRun = kRuleThreads * PER * 4;
     __shared__ __align__(16) unsigned times[kRun];  // how often a token was said, the top bit: it is in the prompt
+    extern __shared__ float more[];                 // [kRun], where there are biases: what those of a biased token add up to
     const long long row = blockIdx.y, c0 = (long long)blockIdx.x * kRun, base = row * p.cols;
     const int tid = threadIdx.x, n = (int)min((long long)kRun, p.cols - c0);
     // everything that does not hang on something else is asked for at once
@@ -107,6 +108,35 @@ template <int DT, int PER, bool VEC> __global__ void __launch_bounds__(kRuleThre
         for (int i = kEarly * kRuleThreads + tid; i < total; i += kRuleThreads) count(i, h[i]);
         __syncthreads();
     }
+    const int* ids = p.bias_ids + row * p.n_bias;
+    if (p.bias_ids) {
+        // The sums of the biased tokens' biases, each in the order of the list: by one warp, 32 places at a time, those of one token one after the other by its first lane. 64 rows of 262144 with 300, 1000,
+        // 4096 biases, one call after the other: 64, 111, 333 us; where each listed token searches the list for its likes 172, 977, 11 907.
+        for (int j = tid; j < p.n_bias; j += kRuleThreads) {
+            const long long c = ids[j] - c0;
+            if (c >= 0 && c < n && ids[j] >= 0) more[c] = 0.f;
+        }
+        __syncthreads();
+        const float* bias = p.bias + row * p.n_bias;
+        if (tid < 32)
+            for (int j0 = 0; j0 < p.n_bias; j0 += 32) {
+                const int t = j0 + tid < p.n_bias ? ids[j0 + tid] : -1;
+                if (t >= p.cols && blockIdx.x == 0) report(p.err, ERR_RULES_TOKEN, p.node, t, p.cols);
+                const long long c = t - c0;
+                const bool mine = t >= 0 && c >= 0 && c < n;
+                if (!__any_sync(0xffffffffu, mine)) continue;
+                const float b = mine ? bias[j0 + tid] : 0.f;
+                const unsigned same = __match_any_sync(0xffffffffu, mine ? t : -1);
+                const bool first = mine && __ffs(same) == tid + 1;
+                float sum = first ? more[c] : 0.f;
+                for (int k = 0; k < 32; k++) {
+                    const float theirs = __shfl_sync(0xffffffffu, b, k);
+                    if (same >> k & 1u) sum += theirs;
+                }
+                if (first) more[c] = sum;
+                __syncwarp();
+            }
+    }
     auto penalised = [&](float l, unsigned said) {
         if (said == 0u) return l;
         l = l > 0.f ? l / repetition : l * repetition;
@@ -129,34 +159,21 @@ template <int DT, int PER, bool VEC> __global__ void __launch_bounds__(kRuleThre
         if (VEC && token(i, 0) < n) *reinterpret_cast<float4*>(p.y + base + c0 + token(i, 0)) = make_float4(v[i][0], v[i][1], v[i][2], v[i][3]);
     }
     if (!p.bias_ids) return;
-    __syncthreads();  // behind the plain results
-    const int* ids = p.bias_ids + row * p.n_bias;
-    const float* bias = p.bias + row * p.n_bias;
+    __syncthreads();  // behind the plain results, and the sums
     for (int j = tid; j < p.n_bias; j += kRuleThreads) {
         const int t = ids[j];
         const long long c = t - c0;
-        if (t >= p.cols && blockIdx.x == 0) report(p.err, ERR_RULES_TOKEN, p.node, t, p.cols);
         if (t < 0 || c < 0 || c >= n || !allowed(t)) continue;
         float l = ld<DT>(p.x, base + t);
         if (p.history) l = penalised(l, times[c]);
-        float more = 0.f;
-        bool first = true;  // a token that is listed again has the sum from its first place
-        for (int k = 0; k < p.n_bias; k++)
-            if (ids[k] == t) {
-                if (k < j) {
-                    first = false;
-                    break;
-                }
-                more += bias[k];
-            }
-        if (first) p.y[base + t] = l + more;
+        p.y[base + t] = l + more[c];  // (a token that is listed again gets the same)
     }
 }
 
 template <int DT> void emit_rules_of(Emitter& em, const RulesP& p, bool vec, std::initializer_list<std::pair<const void*, Buf>> ptrs) {
     auto go = [&](void (*k)(const RulesP), int per) {
         const long long run = (long long)kRuleThreads * per * 4;
-        em.launch(k, dim3((unsigned)((p.cols + run - 1) / run), (unsigned)p.rows), dim3(kRuleThreads), 0, p, ptrs, "constrain_rows");
+        em.launch(k, dim3((unsigned)((p.cols + run - 1) / run), (unsigned)p.rows), dim3(kRuleThreads), p.n_bias ? (unsigned)(run * 4) : 0u, p, ptrs, "constrain_rows");
     };
     vec ? go(constrain_rows<DT, 4, true>, 4) : go(constrain_rows<DT, 4, false>, 4);
 }

@@ -121,3 +121,28 @@ def test_null_logits_and_rules_are_refused_at_the_c_entry():
         with pytest.raises(OnyxiaError, match="rules need logits"):
             _ffi.check(_ffi.cuda_lib().ox_session_constrain_last(session._h, logits, described, C.byref(out)))
     assert (session.download(session.constrain_last(x)).numpy() == 1.0).all()
+
+
+@pytest.mark.parametrize("rows,vocab,n_bias", [(3, 4096, 4096), (2, 50021, 4096), (1, 262144, 1000), (3, 33, 200), (2, 4100, 31), (2, 4100, 33)])
+def test_biases_are_added_up_in_their_order(rows, vocab, n_bias):
+    """Bit by bit as one after the other in f32, tokens listed many times, near each other and far apart among them, biases of very different sizes; a zero that has no bias keeps its sign."""
+    r = np.random.default_rng(n_bias + vocab)
+    x = np.where(r.random((rows, vocab)) < 0.2, np.float32(-0.0), r.standard_normal((rows, vocab))).astype(np.float32)
+    few = r.integers(0, vocab, 5)
+    ids = np.where(r.random((rows, n_bias)) < 0.4, few[r.integers(0, 5, (rows, n_bias))], r.integers(0, vocab, (rows, n_bias))).astype(np.int32)
+    ids[r.random(ids.shape) < 0.1] = -1
+    bias = (r.standard_normal(ids.shape) * 10.0 ** r.integers(-4, 5, ids.shape)).astype(np.float32)
+    want = x.copy()
+    for i in range(rows):
+        sums = {}
+        for t, b in zip(ids[i].tolist(), bias[i]):
+            if t >= 0:
+                sums[t] = np.float32(sums.get(t, np.float32(0.0)) + b)
+        for t, s in sums.items():
+            want[i, t] = np.float32(x[i, t] + s)
+    b = ir.GraphBuilder()
+    b.output("one", b.const_f32([1.0], [1]))
+    session = cuda_backend().prepare(b.finish())
+    up = lambda a: session.upload(HostTensor.from_numpy(a))  # noqa: E731
+    got = session.download(session.constrain_last(up(x), bias_ids=up(ids), bias=up(bias))).numpy()
+    assert np.array_equal(got.view(np.uint32), want.view(np.uint32))

@@ -7,9 +7,10 @@
 // place, free as soon as they have been read, weights have two of their own, and the next scores are made, and the last weights multiplied, under the exponentials of these.
 // In the end each CTA stages the other half of its rows, divided by their sums, copies them into the other's shared memory, and forms difference, norm and results of its own half.
 //
-// Measured alone, L2 cold: 4096 tokens, 32 heads of 2 × 64 over 16, values of 128 (137 GFLOP) 289 us, 476 TFLOP/s, 950 with the queries' low part and a product of the values per map;
-// 2048, 16 over 4 60 us; 1999 capped behind 1000, 4 heads of 2 × 128 over one 60 us. A step of 64 keys takes 1 600 cycles with two CTAs per SM: products need 640 of an SM's 800, exponentials
-// 512; what bounds it is their order within a CTA, and a third CTA has no tensor memory. A tile's beginning and end take 16 000 cycles, half of them under the other CTA's steps.
+// Measured alone, L2 cold: 4096 tokens, 32 heads of 2 × 64 over 16, values of 128 (137 GFLOP) 289–305 us, 450–476 TFLOP/s, twice that with the queries' low part and a product of the values per map;
+// 2048, 16 over 4 60 us; 1999 capped and normed behind 1000, 4 heads of 2 × 128 over one, weights in two parts, 73 us (60 in one). A step of 64 keys takes 1 600 cycles with two CTAs per SM, of which both CTAs'
+// exponentials take 1 054 of their unit and both CTAs' products, one after the other, 1 280 (the tensor pipe counts as active for 47 % of the whole kernel: products of 64 columns do not fill it, and tiles begin and end);
+// what bounds it is their order within a CTA, and a third CTA has no tensor memory. A tile's beginning and end take 16 000 cycles, half of them under the other CTA's steps.
 #include <type_traits>
 
 #include "differential.cuh"

@@ -17,7 +17,7 @@ import numpy as np
 
 from . import _ffi
 from ._ffi import check
-from .ir import _NP, BF16, BOOL, I4, U4, HostTensor, Module, storage_bytes
+from .ir import _NP, BF16, HostTensor, Module, storage_bytes
 
 
 class DeviceTensor:
@@ -63,31 +63,41 @@ class DeviceTensor:
             self._h = None
 
 
+_ARRAY_TYPES = {**{dtype: np.dtype(kind).str for dtype, kind in _NP.items()}, BF16: "<i2"}
+
+
 class DeviceView:
     """Memory of a tensor as ``__cuda_array_interface__`` (``torch.as_tensor`` and others take it without a copy); bf16 as whole
     numbers of 16 bits. The view keeps the tensor; when it goes, the session's later work is ordered behind the view's stream, which has
     to live as long. Where it goes on another thread than the one that made it, the session does so at its next call. Where the stream
     cannot be waited for (it is being captured), the tensor's memory stays the session's until it is closed."""
 
+    _session = None  # until there is something to end
+
     def __init__(self, session: "CudaSession", t: DeviceTensor, stream: int):
         dtype, shape = t.describe()
-        if dtype in (U4, I4):
+        kind = _ARRAY_TYPES.get(dtype)
+        if kind is None:
             raise ValueError("packed 4-bit values have no array interface")
-        self._tensor = t.clone()
+        self._tensor, self._stream, self._thread = t.clone(), int(stream), _get_ident()
         ptr = C.c_void_p()
-        check(session._lib.ox_session_device_view(session._h, t.handle, C.c_void_p(int(stream)), C.byref(ptr)))
-        self._session, self._stream, self._thread = session, int(stream), _get_ident()
-        kind = "<i2" if dtype == BF16 else "|b1" if dtype == BOOL else np.dtype(_NP[dtype]).str
+        check(session._lib.ox_session_device_view(session._h, t.handle, self._stream, C.byref(ptr)))
+        self._session = session
         self.__cuda_array_interface__ = {"shape": shape, "typestr": kind, "data": (ptr.value or 0, False), "version": 2, "strides": None}
 
     def __del__(self, get_ident=_get_ident):  # (a module's names may be gone when the interpreter ends)
-        session = getattr(self, "_session", None)
+        session = self._session
         if session is None or not session._open:
             return
-        if get_ident() == self._thread:
-            session._end_view(self._tensor, self._stream)
-        else:  # a session is for one thread at a time
+        if get_ident() != self._thread:  # a session is for one thread at a time
             session._dropped.append((self._tensor, self._stream))
+            return
+        try:
+            ordered = session._after_stream(session._open, self._stream) == 0
+        except Exception:
+            ordered = False
+        if not ordered:
+            session._kept.append(self._tensor)
 
 
 class CudaSession:
@@ -96,21 +106,16 @@ class CudaSession:
     def __init__(self, handle):
         self._lib = _ffi.cuda_lib()
         self._open, self._dropped, self._kept = handle, [], []  # views that went on other threads; tensors of views whose stream could not be waited for
+        self._after_stream = self._lib.ox_session_after_stream
         self._num_outputs = max(self._lib.ox_session_num_outputs(handle), 1)
 
     @property
     def _h(self):
         while self._dropped:
-            self._end_view(*self._dropped.pop())
+            tensor, stream = self._dropped.pop()
+            if self._after_stream(self._open, stream) != 0:
+                self._kept.append(tensor)
         return self._open
-
-    def _end_view(self, tensor, stream: int, pointer=C.c_void_p) -> None:
-        try:
-            ordered = self._lib.ox_session_after_stream(self._open, pointer(stream)) == 0
-        except Exception:
-            ordered = False
-        if not ordered:
-            self._kept.append(tensor)
 
     def upload(self, t: HostTensor) -> DeviceTensor:
         shape = (C.c_uint64 * max(len(t.shape), 1))(*t.shape)

@@ -20,12 +20,12 @@ class Notes:
         return 1
 
     def ox_session_device_view(self, h, t, stream, ptr):
-        self.calls.append(("view", stream.value))
+        self.calls.append(("view", stream))
         return 0
 
     def ox_session_after_stream(self, h, stream):
-        self.calls.append(("after", stream.value, threading.get_ident()))
-        return 7 if stream.value in self.refuses else 0
+        self.calls.append(("after", stream, threading.get_ident()))
+        return 7 if stream in self.refuses else 0
 
     def ox_session_sync(self, h):
         self.calls.append(("sync",))
@@ -39,8 +39,11 @@ class Tensor:
     released = 0
     handle = None
 
+    def __init__(self, dtype=ir.F32):
+        self.dtype = dtype
+
     def describe(self):
-        return ir.F32, (2, 3)
+        return self.dtype, (2, 3)
 
     def clone(self):
         return Tensor()
@@ -93,6 +96,15 @@ def test_a_view_that_goes_on_another_thread_is_ended_by_the_sessions_next_call(s
     assert s._h == 1  # what every call begins with
     gc.collect()
     assert notes.calls[-1] == ("after", 5, threading.get_ident()) and Tensor.released == released + 1
+
+
+def test_the_types_that_arrays_know(session):
+    s, _ = session
+    for dtype, kind in ((ir.F32, "<f4"), (ir.F16, "<f2"), (ir.BF16, "<i2"), (ir.I64, "<i8"), (ir.I32, "<i4"), (ir.U32, "<u4"), (ir.U8, "|u1"), (ir.I8, "|i1"), (ir.BOOL, "|b1")):
+        assert s.view(Tensor(dtype)).__cuda_array_interface__["typestr"] == kind
+    for dtype in (ir.U4, ir.I4):
+        with pytest.raises(ValueError, match="4-bit"):
+            s.view(Tensor(dtype))
 
 
 def test_views_of_a_closed_session_ask_nothing_of_it(session):

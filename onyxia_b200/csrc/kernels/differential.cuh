@@ -25,7 +25,7 @@ struct DiffP {
     int singles;                 // sequences with one new token are for these kernels too
     int parts;                   // prepare: queries in two parts, times mul2
     int by8;                     // the parts of a projection row begin on 16 bytes
-    int only;                    // no sequence may have more than one
+    int only;                    // no rows for prompts: with as many rows as sequences none may have more than one new token, with fewer those are differential_several's
     int low;                     // weights are the sum of two bf16
     int rep;                     // heads of a key head
     unsigned by_rep, by_units, by_lanes;  // 2^32 / (heads of a key head, units of a query, sixteen bytes of a value), rounded up; 0: of one

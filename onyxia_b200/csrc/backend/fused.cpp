@@ -668,6 +668,107 @@ void differential_lower(FusedCtx& c) {
     oxk::emit_differential(c.em, d, c.ins[0], c.ins[1], c.outs[1], c.outs[2], c.ins[4], c.ins[5], c.ins[6], a.int_or("head_norm", 0) != 0 ? &c.ins[7] : nullptr, c.outs[0]);
 }
 
+// ── onyxia.PackedKVAttention / onyxia.SharedPackedKVAttention / onyxia.CacheWrite / onyxia.CacheRead ──
+// Keys and values in 4 bits (kernels/packed_cache.cuh). "factors": the last two operands are constants F32 [kv_heads] that keys and values are divided by before they are stored.
+//   PackedKVAttention        proj, turns per position, keys, values, seqs, pages [, factors × 2] → out, keys, values
+//   SharedPackedKVAttention  the same, to what another node has put into the pools → out
+//   CacheWrite               the same without queries → keys, values
+//   CacheRead                keys, values, places, pages [, factors × 2] → keys and values side by side
+// The other attributes are those of onyxia.PagedKVAttention.
+bool packed_sizes_fit(const Module& m, const Node& n, size_t pools) {
+    const Attrs& a = n.composite.attrs;
+    const int64_t G = a.int_or("kv_heads", 0), D = a.int_or("dim", 0), V = a.int_or("vdim", 0);
+    if (G <= 0 || G > 65535 || D <= 0 || V <= 0 || D > 8192 || V > 8192 || D % 16 != 0 || V % 16 != 0) return false;
+    const TensorType &keys = ty(m, n.inputs[pools]), &values = ty(m, n.inputs[pools + 1]);
+    for (auto [t, d] : {std::pair<const TensorType*, int64_t>{&keys, D}, {&values, V}})
+        if (t->dtype != DType::U8 || t->shape.size() != 4 || !is_const(t->shape[1], G) || !t->shape[2].as_const() || !is_const(t->shape[3], d / 16 * 9)) return false;
+    const uint64_t page = *keys.shape[2].as_const();
+    if (page < 16 || page > (1u << 20) || (page & (page - 1)) != 0 || values.shape[0] != keys.shape[0] || values.shape[2] != keys.shape[2]) return false;
+    const int64_t factors = a.int_or("factors", 0);
+    if (factors != 0 && factors != 1) return false;
+    for (size_t i = n.inputs.size() - 2 * (size_t)factors; i < n.inputs.size(); i++) {
+        if (!is_f32_vector(m, n.inputs[i], (uint64_t)G) || m.values[n.inputs[i]].origin.kind != Origin::Const) return false;
+        const uint8_t* bytes = m.consts.bytes(m.values[n.inputs[i]].origin.id);
+        for (int64_t g = 0; g < G; g++) {
+            float f;
+            std::memcpy(&f, bytes + g * 4, 4);
+            if (!(f >= 1e-30f && f <= 1e30f)) return false;
+        }
+    }
+    return true;
+}
+enum class PackedForm { Attend, Shared, Write };
+bool packed_fits(const Module& m, const Node& n, PackedForm form) {
+    const Attrs& a = n.composite.attrs;
+    const bool queries = form != PackedForm::Write, append = form != PackedForm::Shared;
+    if (n.inputs.size() != 6u + (a.int_or("factors", 0) != 0 ? 2 : 0) || n.outputs.size() != (size_t)queries + (append ? 2 : 0) || !packed_sizes_fit(m, n, 2)) return false;
+    const int64_t H = a.int_or("heads", 0), G = a.int_or("kv_heads", 0), D = a.int_or("dim", 0), V = a.int_or("vdim", 0), R = a.int_or("rot_dims", 0);
+    if ((queries && (H <= 0 || H > 65535 || H % G != 0)) || R < 0 || R > D || R % 2 != 0) return false;
+    if (a.int_or("window", 0) < 0 || a.int_or("window", 0) > INT32_MAX) return false;
+    for (const char* f : {"softcap", "epsilon"})
+        if (!(a.float_or(f, 0.0) >= 0.0) || !std::isfinite(a.float_or(f, 0.0))) return false;
+    // (in f32, and in the quotient that scores are multiplied by, too)
+    const double scale = std::fabs(a.float_or("scale", 1.0)), cap = a.float_or("softcap", 0.0);
+    if (!(scale <= 1e30) || cap > 1e30 || (cap > 0.0 && scale > 1e30 * cap)) return false;
+    const TensorType &x = ty(m, n.inputs[0]), &turns = ty(m, n.inputs[1]), &seqs = ty(m, n.inputs[4]), &pages = ty(m, n.inputs[5]);
+    auto width = x.shape.size() == 2 ? x.shape[1].as_const() : std::nullopt;
+    if (!is_act(x.dtype) || !width) return false;
+    auto inside = [&](const char* name, int64_t cols) { return a.int_or(name, 0) >= 0 && a.int_or(name, 0) <= (int64_t)*width - cols; };
+    if ((queries && !inside("q_offset", H * D)) || (append && (!inside("k_offset", G * D) || !inside("v_offset", G * V)))) return false;
+    if (turns.dtype != DType::F32 || turns.shape.size() != 2 || !is_const(turns.shape[0], 2) || (R > 0 && !is_const(turns.shape[1], R / 2))) return false;
+    if (seqs.dtype != DType::I32 || seqs.shape.size() != 2 || !is_const(seqs.shape[1], 4)) return false;
+    if (pages.dtype != DType::I32 || pages.shape.size() != 2 || pages.shape[0] != seqs.shape[0]) return false;
+    for (size_t i = 0; append && i < 2; i++) {
+        const TensorType &pool = ty(m, n.inputs[2 + i]), &updated = ty(m, n.outputs[(size_t)queries + i]);
+        if (updated.dtype != pool.dtype || updated.shape != pool.shape) return false;
+    }
+    if (!queries) return true;
+    const TensorType& out = ty(m, n.outputs[0]);
+    return out.dtype == x.dtype && out.shape.size() == 2 && out.shape[0] == x.shape[0] && is_const(out.shape[1], H * V);
+}
+bool packed_accepts(const Module& m, const Node& n) { return packed_fits(m, n, PackedForm::Attend); }
+bool shared_packed_accepts(const Module& m, const Node& n) { return packed_fits(m, n, PackedForm::Shared); }
+bool cache_write_accepts(const Module& m, const Node& n) { return packed_fits(m, n, PackedForm::Write); }
+oxk::PackedDesc packed_desc(FusedCtx& c, size_t pools) {
+    const Attrs& a = c.node.composite.attrs;
+    oxk::PackedDesc d{};
+    d.heads = a.int_or("heads", 0);
+    d.kv_heads = a.int_("kv_heads");
+    d.dim = a.int_("dim");
+    d.vdim = a.int_("vdim");
+    d.page = c.ins[pools].shape[2];
+    d.q_off = a.int_or("q_offset", 0);
+    d.k_off = a.int_or("k_offset", 0);
+    d.v_off = a.int_or("v_offset", 0);
+    d.rot_dims = a.int_or("rot_dims", 0);
+    d.window = a.int_or("window", 0);
+    d.scale = a.float_or("scale", 1.0);
+    d.softcap = a.float_or("softcap", 0.0);
+    d.eps = a.float_or("epsilon", 1e-6);
+    d.norm = a.int_or("norm", 0) != 0;
+    d.sink = a.int_or("sink", 0) != 0;
+    return d;
+}
+void packed_lower(FusedCtx& c) {
+    oxk::PackedDesc d = packed_desc(c, 2);
+    const bool queries = c.outs.size() != 2, factors = c.ins.size() == 8;
+    d.append = c.outs.size() > 1;
+    if (!queries) d.heads = 0;
+    oxk::emit_packed_attention(c.em, d, c.ins[0], c.ins[1], d.append ? c.outs[queries] : c.ins[2], d.append ? c.outs[queries + 1] : c.ins[3], c.ins[4], c.ins[5],
+                               factors ? &c.ins[6] : nullptr, factors ? &c.ins[7] : nullptr, queries ? &c.outs[0] : nullptr);
+}
+bool cache_read_accepts(const Module& m, const Node& n) {
+    const Attrs& a = n.composite.attrs;
+    if (n.inputs.size() != 4u + (a.int_or("factors", 0) != 0 ? 2 : 0) || n.outputs.size() != 1 || !packed_sizes_fit(m, n, 0)) return false;
+    const TensorType &places = ty(m, n.inputs[2]), &pages = ty(m, n.inputs[3]), &out = ty(m, n.outputs[0]);
+    if (places.dtype != DType::I32 || places.shape.size() != 2 || !is_const(places.shape[1], 2) || pages.dtype != DType::I32 || pages.shape.size() != 2) return false;
+    return is_act(out.dtype) && out.shape.size() == 2 && out.shape[0] == places.shape[0] && is_const(out.shape[1], a.int_("kv_heads") * (a.int_("dim") + a.int_("vdim")));
+}
+void cache_read_lower(FusedCtx& c) {
+    const bool factors = c.ins.size() == 6;
+    oxk::emit_packed_read(c.em, packed_desc(c, 0), c.ins[0], c.ins[1], c.ins[2], c.ins[3], factors ? &c.ins[4] : nullptr, factors ? &c.ins[5] : nullptr, c.outs[0]);
+}
+
 // ── onyxia.LatentAttention ──
 // queries in the latent space, queries, proj, norm weight, turns per position, pool, seqs, pages → out, pool
 bool latent_accepts(const Module& m, const Node& n) {
@@ -907,6 +1008,10 @@ const KernelRegistry& standard_kernels() {
         r.add({"onyxia.PagedKVAttention", paged_kv_accepts, paged_kv_lower, {{1, 2}, {2, 3}}, {0}});
         r.add({"onyxia.SharedKVAttention", shared_kv_accepts, paged_kv_lower, {}, {0, 2, 3}});
         r.add({"onyxia.DifferentialAttention", differential_accepts, differential_lower, {{1, 2}, {2, 3}}, {0}});
+        r.add({"onyxia.PackedKVAttention", packed_accepts, packed_lower, {{1, 2}, {2, 3}}, {0}});
+        r.add({"onyxia.SharedPackedKVAttention", shared_packed_accepts, packed_lower, {}, {0, 2, 3}});
+        r.add({"onyxia.CacheWrite", cache_write_accepts, packed_lower, {{0, 2}, {1, 3}}, {0}});
+        r.add({"onyxia.CacheRead", cache_read_accepts, cache_read_lower, {}, {0, 1}});
         r.add({"onyxia.LightningAttention", lightning_accepts, lightning_lower, {{1, 2}}, {0}});
         r.add({"onyxia.GatedLinearAttention", gated_linear_accepts, gated_linear_lower, {{1, 2}}, {0, 1}});
         r.add({"onyxia.GatedDeltaRule", delta_accepts, delta_lower, {{1, 4}, {2, 5}}, {0}});

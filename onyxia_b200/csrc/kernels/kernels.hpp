@@ -488,6 +488,24 @@ void emit_differential(Emitter&, const DifferentialDesc&, const TRef& proj, cons
 int differential_prefill_smem(int kp, int vp);
 int differential_prefill_columns(int kp, int vp);
 
+struct PackedDesc {
+    int64_t heads, kv_heads, dim, vdim, page;  // dim, vdim: multiples of 16; page: a power of two, 16 at least
+    int64_t q_off, k_off, v_off;  // columns of the fused projection
+    int64_t rot_dims;             // leading dimensions of a query or key that rotate in two halves; 0: none
+    int64_t window;               // keys a position sees, itself among them; 0: all
+    double scale, softcap, eps;   // softcap 0: none
+    bool norm;                    // queries and keys divided by their root mean square over `dim` after the rotation
+    bool sink;                    // a score of 0 without a value in the softmax
+    bool append;                  // the batch's keys and values go to the pools first
+};
+// Keys and values in 4 bits over pools U8 [pages, kv_heads, page, dim · 9 / 16] and [pages, kv_heads, page, vdim · 9 / 16] (packed_cache.cuh): a batch's own go there, and its
+// queries, where `out` is not null, attend to what the pools hold. Factors F32 [kv_heads] or null. Batches are described as for emit_differential.
+void emit_packed_attention(Emitter&, const PackedDesc&, const TRef& proj, const TRef& turns, const TRef& keys, const TRef& values, const TRef& seqs, const TRef& pages,
+                           const TRef* key_factors, const TRef* value_factors, const TRef* out);
+// `out` [rows, kv_heads · (dim + vdim)]: the keys, then the values, that the pools hold at `places` I32 [rows, 2] (row of the page table, position); zeros, and a report, where there is none.
+void emit_packed_read(Emitter&, const PackedDesc&, const TRef& keys, const TRef& values, const TRef& places, const TRef& pages, const TRef* key_factors, const TRef* value_factors,
+                      const TRef& out);
+
 // Attention whose keys and values are one latent per token that all heads share: key = (latent, rotated part), value =
 // latent. Queries come with their unrotated part already mapped into the latent space (`q_latent` [rows, heads · rank]) and with
 // their rotated part in `q` (head h's from column h · q_step + q_off on). The new latents are columns of `proj` from kv_off

@@ -1,0 +1,133 @@
+// Keys and values held in 4 bits: the format, and what the kernels that write, read and attend to it share.
+//
+// A pool is [pages, kv_heads, page, dim · 9 / 16] bytes. What a page holds of a head is one piece: first the codes of its keys (e2m1: 0, 0.5, 1, 1.5, 2, 3, 4, 6 and a sign; two in a
+// byte, the earlier dimension in the low half), dim / 2 bytes each, then their scales (e4m3), one per 16 dimensions. A value is code · scale · factor, with an f32 factor per head (1 where none are
+// given). code · scale has six significant bits at most and lies between 2^-10 and 2688: f16 holds it exactly, so matrix instructions multiply what is stored, not a rounding of it.
+//
+// Stored is, of y = x / factor in f32 and a = max |y| over 16 dimensions, scale = e4m3(a / 6) and code = e2m1(y / scale), both to the nearest, ties to even, at most 448 and 6. Where the
+// scale comes out as 0 so do the codes; where one of the 16 is no number the scale is none, and all 16 read as NaN.
+#pragma once
+#include "paged_util.cuh"
+
+namespace oxk {
+
+constexpr int kPack = 16;  // dimensions of a scale
+
+struct PackP {
+    const void* proj;            // [rows, ld]
+    const float* turns;          // [2, half]
+    unsigned char *keys, *values;  // [pages, kv_heads, page, dim | vdim times 9 / 16]
+    void* q;                     // prepared queries [rows, heads, dim], f32
+    void* out;                   // [rows, heads · vdim]
+    const int* seqs;             // [R, 4]
+    const int* table;            // [R, width]
+    const float *key_factors, *value_factors;  // [kv_heads], or null: 1
+    ErrWord* err;
+    long long rows, ld, q_off, k_off, v_off;
+    int n_seqs, width, n_pages, shift /* log2 of the page */, heads, kv_heads, dim, vdim, half, window, node;
+    float scale, cap;            // scores in natural units
+    double eps;
+    int norm, sink, append;
+    int singles;                 // sequences with one new token are for these kernels too
+};
+
+__device__ __forceinline__ float key_factor(const PackP& p, int g) { return p.key_factors ? p.key_factors[g] : 1.f; }
+__device__ __forceinline__ float value_factor(const PackP& p, int g) { return p.value_factors ? p.value_factors[g] : 1.f; }
+
+// Where page `pg` holds head g's codes and, behind them, scales, for keys or values of `dim` dimensions.
+template <class P> __device__ __forceinline__ unsigned char* held(const P& p, unsigned char* pool, long long pg, int g, int dim) {
+    return pool + ((pg * p.kv_heads + g) << p.shift) * (dim / kPack) * 9;
+}
+template <class P> __device__ __forceinline__ unsigned char* codes_of(const P& p, unsigned char* held, int pos, int dim) { return held + (pos & ((1 << p.shift) - 1)) * (dim / 2); }
+template <class P> __device__ __forceinline__ unsigned char* scales_of(const P& p, unsigned char* held, int pos, int dim) {
+    return held + ((dim / 2) << p.shift) + (pos & ((1 << p.shift) - 1)) * (dim / kPack);
+}
+
+// ── the format ──
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+// The scale of sixteen values whose largest magnitude is `a`, as it is stored.
+__device__ __forceinline__ unsigned scale_code(float a) {
+    unsigned short r;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(0.f), "f"(a / 6.f));
+    return r & 0xFFu;
+}
+__device__ __forceinline__ __half2 scales_f16(unsigned two) {
+    unsigned r;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"((unsigned short)two));
+    return *reinterpret_cast<__half2*>(&r);
+}
+__device__ __forceinline__ float scale_value(unsigned code) { return __low2float(scales_f16(code)); }
+// A value over its scale; 0 where that is 0 or no number.
+__device__ __forceinline__ float over_scale(float y, float scale) { return scale > 0.f ? y / scale : 0.f; }
+// Eight values over their scale as codes, the first one lowest.
+__device__ __forceinline__ unsigned codes8(const float (&r)[8]) {
+    unsigned v;
+    asm("{\n .reg .b8 a, b, c, d;\n"
+        " cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n cvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n cvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n"
+        " mov.b32 %0, {a, b, c, d};\n}\n"
+        : "=r"(v)
+        : "f"(r[0]), "f"(r[1]), "f"(r[2]), "f"(r[3]), "f"(r[4]), "f"(r[5]), "f"(r[6]), "f"(r[7]));
+    return v;
+}
+__device__ __forceinline__ unsigned code_of(float r) {
+    unsigned v;
+    asm("{\n .reg .b8 a, b;\n cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n mov.b32 %0, {a, a, a, a};\n}\n" : "=r"(v) : "f"(r), "f"(0.f));
+    return v & 15u;
+}
+// What the four bytes of a word stand for, two dimensions each, without their scale.
+__device__ __forceinline__ void units8(unsigned word, __half2 (&v)[4]) {
+    unsigned a, b, c, d;
+    asm("{\n .reg .b8 e, f, g, h;\n mov.b32 {e, f, g, h}, %4;\n"
+        " cvt.rn.f16x2.e2m1x2 %0, e;\n cvt.rn.f16x2.e2m1x2 %1, f;\n cvt.rn.f16x2.e2m1x2 %2, g;\n cvt.rn.f16x2.e2m1x2 %3, h;\n}\n"
+        : "=r"(a), "=r"(b), "=r"(c), "=r"(d)
+        : "r"(word));
+    v[0] = *reinterpret_cast<__half2*>(&a);
+    v[1] = *reinterpret_cast<__half2*>(&b);
+    v[2] = *reinterpret_cast<__half2*>(&c);
+    v[3] = *reinterpret_cast<__half2*>(&d);
+}
+
+// ── a batch step ──
+// Sequence r of the batch. One whose rows are not the batch's, or whose positions the page table has no place for, is reported and has no rows.
+template <class P> __device__ __forceinline__ SeqRow checked_seq(const P& p, int r) {
+    SeqRow s = load_seq(p.seqs, r);
+    if (s.len != 0 && (s.start < 0 || s.len < 0 || s.past < 0 || s.start + (long long)s.len > p.rows || s.past + (long long)s.len > (long long)p.width << p.shift)) {
+        report(p.err, ERR_BATCH_SEQ, p.node, r, s.past + (long long)s.len);
+        s.len = 0;
+    }
+    return s;
+}
+// By the CTA of the batch's first row: what is wrong with a sequence that no row belongs to.
+template <class P> __device__ __forceinline__ void check_others(const P& p, int row, int tid, int threads) {
+    if (row == 0)
+        for (int i = tid; i < p.n_seqs; i += threads) checked_seq(p, i);
+}
+template <class P> __device__ __forceinline__ int first_key(const P& p, int pos) { return p.window > 0 ? max(0, pos - p.window + 1) : 0; }
+// Cosine and sine of every pair at a position, by `threads` threads, in 64 bits: what one step stores is the rounding of the key itself, which any other way to compute it finds too.
+template <class P> __device__ __forceinline__ void exact_angles(const P& p, int pos, double* cs, double* sn, int tid, int threads) {
+    for (int i = tid; i < p.half; i += threads) {
+        const double t = (double)pos * ((double)p.turns[i] + (double)p.turns[p.half + i]) * 2.0;
+        sincospi(t - 2.0 * rint(0.5 * t), sn + i, cs + i);
+    }
+}
+// Dimension i of a query or key whose leading 2 · half dimensions turn, i with i + half.
+template <typename T> __device__ __forceinline__ double turned(int half, const T* x, const double* cs, const double* sn, int i) {
+    const double v = (double)to_f(x[i]);
+    if (i >= 2 * half) return v;
+    return i < half ? v * cs[i] - (double)to_f(x[i + half]) * sn[i] : v * cs[i - half] + (double)to_f(x[i - half]) * sn[i - half];
+}
+// 1 / root mean square of a query or key in 64 bits, by one warp
+template <typename T> __device__ __forceinline__ double norm_factor(const PackP& p, const T* x) {
+    if (!p.norm) return 1.0;
+    double ss = 0.0;
+    for (int i = threadIdx.x & 31; i < p.dim; i += 32) ss += (double)to_f(x[i]) * (double)to_f(x[i]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    return 1.0 / sqrt(ss / p.dim + p.eps);
+}
+
+}  // namespace oxk

@@ -7,6 +7,7 @@
 //
 //   packed_write   a batch's keys (rotated, normed) and values go to the pools; its queries, where there are any, are prepared
 //   packed_read    the keys and values of given places, side by side
+//   packed_decode  sequences with one new token in bf16, all of the above in one launch (packed_decode.cu)
 //   packed_simt    attention of any shape, f32 and bf16
 #include <cmath>
 
@@ -15,21 +16,6 @@
 namespace oxk {
 
 namespace {
-
-// `n` values of a head by one warp: codes and scales to where they are held. value(i): dimension i.
-template <class F> __device__ __forceinline__ void put_head(unsigned char* codes, unsigned char* scales, int n, float factor, F&& value) {
-    const int lane = threadIdx.x & 31;
-    for (int c = 0; c < n; c += 32) {
-        const int i = c + lane;
-        const float y = i < n ? value(i) / factor : 0.f;
-        float a = fabsf(y);
-#pragma unroll
-        for (int o = 8; o > 0; o >>= 1) a = max_nan(a, __shfl_xor_sync(0xffffffffu, a, o));
-        const unsigned s = scale_code(a), code = code_of(over_scale(y, scale_value(s))), next = __shfl_down_sync(0xffffffffu, code, 1);
-        if (i < n && lane % 2 == 0) codes[i / 2] = (unsigned char)(code | next << 4);
-        if (i < n && lane % kPack == 0) scales[i / kPack] = (unsigned char)s;
-    }
-}
 
 // One CTA per row, one warp per query, key or value of a head.
 template <typename T> __global__ void __launch_bounds__(128) packed_write(const PackP p) {
@@ -184,8 +170,6 @@ template <typename T> __global__ void __launch_bounds__(kAnyKeys) packed_simt(co
     for (int i = tid; i < p.vdim; i += kAnyKeys) ((T*)p.out)[((long long)row * p.heads + h) * p.vdim + i] = from_f<T>(acc[i] * f);
 }
 
-using PackKernel = void (*)(const PackP);
-
 }  // namespace
 
 void emit_packed_attention(Emitter& em, const PackedDesc& d, const TRef& proj, const TRef& turns, const TRef& keys, const TRef& values, const TRef& seqs, const TRef& pages,
@@ -217,22 +201,52 @@ void emit_packed_attention(Emitter& em, const PackedDesc& d, const TRef& proj, c
     p.norm = d.norm;
     p.sink = d.sink;
     p.append = d.append;
-    p.singles = 1;
-    const bool bf = proj.dtype == DT_BF16;
-    const Buf none{kSlotNull, 0}, q = out ? em.scratch((size_t)rows * d.heads * d.dim * 4) : none;
-    auto launch = [&](PackKernel k, dim3 grid, unsigned block, unsigned smem, const char* label) {
+    p.cap2 = (float)(d.softcap * (double)kLog2e);
+    p.mul2 = (float)(d.softcap > 0 ? 2.0 * (double)kLog2e * d.scale / d.softcap : (double)kLog2e * d.scale);
+    p.splits = 1;
+    const bool bf = proj.dtype == DT_BF16, tc = out && bf && d.dim <= 256 && d.vdim <= 256 && n_seqs <= 65535;
+    p.only = tc && rows == n_seqs;
+    p.singles = !tc;
+    const Buf none{kSlotNull, 0}, q = out && !p.only ? em.scratch((size_t)rows * d.heads * d.dim * 4) : none;
+    auto launch = [&](PackKernel k, dim3 grid, unsigned block, unsigned smem, Buf part, const char* label) {
         em.launch(k, grid, dim3(block), smem, p,
                   {{&p.proj, proj.buf}, {&p.turns, turns.buf}, {&p.keys, keys.buf}, {&p.values, values.buf}, {&p.q, q}, {&p.out, out ? out->buf : none}, {&p.seqs, seqs.buf}, {&p.table, pages.buf},
-                   {&p.key_factors, key_factors ? key_factors->buf : none}, {&p.value_factors, value_factors ? value_factors->buf : none}, {&p.err, Buf{kSlotErr, 0}}},
+                   {&p.key_factors, key_factors ? key_factors->buf : none}, {&p.value_factors, value_factors ? value_factors->buf : none}, {&p.part, part},
+                   {&p.counters, Buf{kSlotCounters, 0}}, {&p.err, Buf{kSlotErr, 0}}},
                   label, /*pdl=*/true);
     };
-    const PackKernel write = bf ? packed_write<bf16> : packed_write<float>;
-    ensure_max_dynamic_smem((const void*)write, 8192 * 8);
-    launch(write, dim3((unsigned)rows), 128, (unsigned)(d.rot_dims * 8), "packed_write");
-    if (!out) return;
-    const PackKernel k = bf ? packed_simt<bf16> : packed_simt<float>;
-    ensure_max_dynamic_smem((const void*)k, 220 * 1024);
-    launch(k, dim3((unsigned)rows, (unsigned)d.heads), kAnyKeys, (unsigned)((d.dim + d.vdim + kAnyKeys) * 4), "packed_simt");
+    if (!p.only) {
+        const PackKernel write = bf ? packed_write<bf16> : packed_write<float>;
+        ensure_max_dynamic_smem((const void*)write, 8192 * 8);
+        launch(write, dim3((unsigned)rows), 128, (unsigned)(d.rot_dims * 8), none, "packed_write");
+        if (!out) return;
+        const PackKernel k = bf ? packed_simt<bf16> : packed_simt<float>;
+        ensure_max_dynamic_smem((const void*)k, 220 * 1024);
+        launch(k, dim3((unsigned)rows, (unsigned)d.heads), kAnyKeys, (unsigned)((d.dim + d.vdim + kAnyKeys) * 4), none, "packed_simt");
+    }
+    if (tc) {
+        const PackedDecode dc = packed_decode_of(d.dim, d.vdim);
+        const int64_t groups = d.kv_heads * ((d.heads / d.kv_heads + dc.heads - 1) / dc.heads), cells = n_seqs * groups;
+        // Splits of the most keys a sequence can see: whole waves of resident CTAs, each with a beginning and an end, and the pieces have to be merged.
+        const int64_t slots = (int64_t)dc.resident * sm_count();
+        int64_t seen = (int64_t)p.width * d.page;
+        if (d.window > 0) seen = std::min<int64_t>(seen, d.window + dc.step);
+        int64_t splits = 1;
+        const double fixed = 64.0 * 1024.0 / (d.dim + d.vdim);
+        double best = 1e300;
+        for (int64_t sp = 1; sp <= 64 && sp * dc.step <= std::max<int64_t>(seen, dc.step); sp++) {
+            const double us = (double)((cells * sp + slots - 1) / slots) * ((double)seen / sp + fixed) + 4.0 * sp;
+            if (us < best) {
+                best = us;
+                splits = sp;
+            }
+        }
+        if (cells > (int64_t)kCounterWords) splits = 1;
+        p.splits = (int)splits;
+        const Buf part = splits > 1 ? em.scratch((size_t)cells * splits * dc.part * 4) : none;
+        ensure_max_dynamic_smem((const void*)dc.kernel, dc.smem);
+        launch(dc.kernel, dim3((unsigned)splits, (unsigned)groups, (unsigned)n_seqs), 128, (unsigned)dc.smem, part, "packed_decode");
+    }
 }
 
 void emit_packed_read(Emitter& em, const PackedDesc& d, const TRef& keys, const TRef& values, const TRef& places, const TRef& pages, const TRef* key_factors, const TRef* value_factors,

@@ -22,13 +22,17 @@ struct PackP {
     const int* seqs;             // [R, 4]
     const int* table;            // [R, width]
     const float *key_factors, *value_factors;  // [kv_heads], or null: 1
+    float* part;                 // partial results of single tokens
+    unsigned* counters;
     ErrWord* err;
     long long rows, ld, q_off, k_off, v_off;
-    int n_seqs, width, n_pages, shift /* log2 of the page */, heads, kv_heads, dim, vdim, half, window, node;
+    int n_seqs, width, n_pages, shift /* log2 of the page */, heads, kv_heads, dim, vdim, half, window, splits, node;
     float scale, cap;            // scores in natural units
+    float mul2, cap2;            // base 2: cap2 = 0: score2 = mul2 · q·k, otherwise cap2 · tanh with mul2 = 2 log2 e · scale / cap
     double eps;
     int norm, sink, append;
     int singles;                 // sequences with one new token are for these kernels too
+    int only;                    // no rows for prompts: as many rows as sequences, none of which may have more than one new token
 };
 
 __device__ __forceinline__ float key_factor(const PackP& p, int g) { return p.key_factors ? p.key_factors[g] : 1.f; }
@@ -129,5 +133,29 @@ template <typename T> __device__ __forceinline__ double norm_factor(const PackP&
     for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
     return 1.0 / sqrt(ss / p.dim + p.eps);
 }
+
+// `n` values of a head by one warp: codes and scales to where they are held. value(i): dimension i.
+template <class F> __device__ __forceinline__ void put_head(unsigned char* codes, unsigned char* scales, int n, float factor, F&& value) {
+    const int lane = threadIdx.x & 31;
+    for (int c = 0; c < n; c += 32) {
+        const int i = c + lane;
+        const float y = i < n ? value(i) / factor : 0.f;
+        float a = fabsf(y);
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) a = max_nan(a, __shfl_xor_sync(0xffffffffu, a, o));
+        const unsigned s = scale_code(a), code = code_of(over_scale(y, scale_value(s))), next = __shfl_down_sync(0xffffffffu, code, 1);
+        if (i < n && lane % 2 == 0) codes[i / 2] = (unsigned char)(code | next << 4);
+        if (i < n && lane % kPack == 0) scales[i / kPack] = (unsigned char)s;
+    }
+}
+
+// Single tokens in bf16 (packed_decode.cu), keys and values of 256 dimensions at most.
+using PackKernel = void (*)(const PackP);
+struct PackedDecode {
+    PackKernel kernel;
+    int smem, part;          // bytes; floats of a partial result
+    int resident, heads, step;  // CTAs of an SM; query heads and keys that a CTA takes at a time
+};
+PackedDecode packed_decode_of(int64_t dim, int64_t vdim);
 
 }  // namespace oxk

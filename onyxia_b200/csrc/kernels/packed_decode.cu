@@ -1,0 +1,348 @@
+// Single tokens over keys and values in 4 bits: sequences with one new token, their keys split over CTAs and warps, rotation, norms, storing and joining in one launch.
+//
+// A warp takes 16 keys at a time straight from the pools into registers, as both products' rows: S^T = K q^T, O^T = V^T P^T (`mma.sync`, f16). The order of a contraction is free, so a lane
+// holds for S the whole blocks of 16 dimensions of two keys, whose codes become f16 and are multiplied by their scale (exactly), and for O^T the same run of dimensions of four keys: pairs of keys
+// come together by swapping halves of bytes.
+#include <cmath>
+
+#include "packed_cache.cuh"
+
+namespace oxk {
+
+namespace {
+
+constexpr int kWarps = 4, kThreads = kWarps * 32, kPages = 256, kHeads = 8, kKeys = 16;
+constexpr float kNone = -1e30f;  // below every score, and finite: differences stay numbers
+
+__device__ __forceinline__ void mma_f16(float (&c)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ unsigned bits(__half2 v) { return *reinterpret_cast<unsigned*>(&v); }
+
+// KS: blocks of 16 dimensions of a key per lane (64 · KS dimensions at most); VC: bytes of codes of a value per lane (16 · VC dimensions at most)
+template <int KS, int VC> struct Smem {
+    static constexpr int dk = 64 * KS, dv = 16 * VC;
+    static constexpr int q_stride = dk * 2 + 16;
+    static constexpr int q = 0;                                   // [8 heads] f16
+    static constexpr int part = part_size(kHeads, dv);            // floats of one partial result
+    static constexpr int parts = q + kHeads * q_stride;           // [warps][part]
+    static constexpr int angle = (parts + kWarps * part * 4 + 7) / 8 * 8;  // cosines and sines in 64 bits, and in 32
+    static constexpr int total = angle + dk * 12;
+};
+
+// What a lane holds of 16 keys and values.
+template <int KS, int VC> struct Tile {
+    uint2 key[2][KS];
+    unsigned key_scale[2];   // KS bytes
+    unsigned value[4][VC / 4];
+    unsigned value_scale[4];  // one byte, or two
+};
+
+// Grid: (splits, kv_heads · groups of 8 query heads, sequences).
+template <int KS, int VC, int RESIDENT> __global__ void __launch_bounds__(kThreads, RESIDENT) packed_decode(const PackP p) {
+    extern __shared__ __align__(16) unsigned char smem[];
+    __shared__ unsigned arrived;
+    __shared__ int page_s[kPages];  // this CTA's pages, checked
+    __shared__ float factor_s[kHeads];
+    using L = Smem<KS, VC>;
+    pdl_trigger();
+    if (!p.append) pdl_wait();  // another node of the step may have written any of the keys
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g8 = lane >> 2, t4 = lane & 3;
+    // no launch of a step writes the batch description or the keys and values of earlier steps (where the module computes the
+    // former, this launch does not begin early): they may be read while the launches before this one finish
+    const int seq = blockIdx.z;
+    const SeqRow sq = checked_seq(p, seq);
+    const int rep = p.heads / p.kv_heads, groups = (rep + kHeads - 1) / kHeads, g = blockIdx.y / groups, h0 = g * rep + (blockIdx.y % groups) * kHeads;
+    const int n_heads = min(kHeads, (g + 1) * rep - h0), pos = sq.past, dim = p.dim, vdim = p.vdim;
+
+    // keys of this CTA: whole tiles of all four warps, so that a split never cuts a tile
+    constexpr int step = kKeys * kWarps;
+    const int low = first_key(p, pos), base = low / step, blocks = sq.len == 1 ? pos / step + 1 - base : 0;
+    const int b0 = base + (int)((long long)blocks * blockIdx.x / p.splits), b1 = base + (int)((long long)blocks * (blockIdx.x + 1) / p.splits);
+    const int lo = b0 * step, hi = min(b1 * step, pos + 1), from = max(lo, low);  // pages in front of the window may be anybody's
+    const int page0 = from >> p.shift, n_pages = from < hi ? ((hi - 1) >> p.shift) - page0 + 1 : 0;
+    for (int i = tid; i < min(n_pages, kPages); i += kThreads) page_s[i] = (int)page_of(p, seq, (page0 + i) << p.shift);
+    const bool newest = hi == pos + 1 && lo < hi;  // this CTA's keys include the new one
+    __syncthreads();
+    auto page_at = [&](int j) {
+        const int i = (j >> p.shift) - page0;
+        return i < kPages ? (long long)page_s[i] : page_of(p, seq, j);
+    };
+    const int first = lo + warp * kKeys, tiles = first < hi ? (hi - first + step - 1) / step : 0;
+    const bool whole_k = dim == L::dk, whole_v = vdim == L::dv;
+    auto load = [&](int i, Tile<KS, VC>& t) {
+        const int j0 = first + i * step;
+        if (i >= tiles || j0 + kKeys <= from) return;  // (keys in front of the window are not looked at)
+        const long long pg = page_at(max(j0, from));
+        const int off = j0 & ((1 << p.shift) - 1);
+        const unsigned char* k = held(p, p.keys, pg, g, dim);
+        const unsigned char* ks = k + ((dim / 2) << p.shift);
+#pragma unroll
+        for (int r = 0; r < 2; r++) {
+            const int at = off + g8 + 8 * r;
+            const unsigned char *codes = k + at * (dim / 2) + t4 * KS * 8, *scales = ks + at * (dim / kPack) + t4 * KS;
+            if (whole_k) {
+                if constexpr (KS == 1) {
+                    t.key[r][0] = *reinterpret_cast<const uint2*>(codes);
+                    t.key_scale[r] = *scales;
+                } else {
+#pragma unroll
+                    for (int c = 0; c < KS; c += 2) {
+                        const uint4 v = reinterpret_cast<const uint4*>(codes)[c / 2];
+                        t.key[r][c] = make_uint2(v.x, v.y);
+                        t.key[r][c + 1] = make_uint2(v.z, v.w);
+                    }
+                    t.key_scale[r] = KS == 2 ? *reinterpret_cast<const unsigned short*>(scales) : *reinterpret_cast<const unsigned*>(scales);
+                }
+            } else {
+                t.key_scale[r] = 0;
+#pragma unroll
+                for (int c = 0; c < KS; c++) {
+                    const bool in = t4 * KS + c < dim / kPack;
+                    t.key[r][c] = in ? reinterpret_cast<const uint2*>(codes)[c] : make_uint2(0, 0);
+                    t.key_scale[r] |= in ? (unsigned)scales[c] << (8 * c) : 0u;
+                }
+            }
+        }
+        const unsigned char* v = held(p, p.values, pg, g, vdim);
+        const unsigned char* vs = v + ((vdim / 2) << p.shift);
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const int at = off + 2 * t4 + (e & 1) + 8 * (e >> 1);
+            const unsigned char *codes = v + at * (vdim / 2) + g8 * VC, *scales = vs + at * (vdim / kPack);
+            if constexpr (VC == 4) {
+                const bool in = g8 * VC < vdim / 2;
+                t.value[e][0] = in ? *reinterpret_cast<const unsigned*>(codes) : 0u;
+                t.value_scale[e] = in ? scales[g8 / 2] : 0u;
+            } else if constexpr (VC == 8) {
+                const bool in = g8 * VC < vdim / 2;
+                const uint2 w = in ? *reinterpret_cast<const uint2*>(codes) : make_uint2(0, 0);
+                t.value[e][0] = w.x;
+                t.value[e][1] = w.y;
+                t.value_scale[e] = in ? scales[g8] : 0u;
+            } else if (whole_v) {
+                const uint4 w = *reinterpret_cast<const uint4*>(codes);
+                t.value[e][0] = w.x;
+                t.value[e][1] = w.y;
+                t.value[e][2] = w.z;
+                t.value[e][3] = w.w;
+                t.value_scale[e] = reinterpret_cast<const unsigned short*>(scales)[g8];
+            } else {
+                t.value_scale[e] = 0;
+#pragma unroll
+                for (int c = 0; c < 2; c++) {
+                    const bool in = g8 * VC + c * 8 < vdim / 2;
+                    const uint2 w = in ? reinterpret_cast<const uint2*>(codes)[c] : make_uint2(0, 0);
+                    t.value[e][2 * c] = w.x;
+                    t.value[e][2 * c + 1] = w.y;
+                    t.value_scale[e] |= in ? (unsigned)scales[2 * g8 + c] << (8 * c) : 0u;
+                }
+            }
+        }
+    };
+    Tile<KS, VC> ahead[2];
+    // The first tiles are on their way while the launch before this one ends, unless the new key is among them.
+    const bool late = newest && p.append && (pos - lo) / step < 2;
+    if (!late) load(0, ahead[0]), load(1, ahead[1]);
+    double *cs = reinterpret_cast<double*>(smem + L::angle), *sn = cs + L::dk / 2;
+    float *short_cs = reinterpret_cast<float*>(sn + L::dk / 2), *short_sn = short_cs + L::dk / 2;
+    if (sq.len == 1) {
+        exact_angles(p, pos, cs, sn, tid, kThreads);
+        for (int i = tid; i < p.half; i += kThreads) short_cs[i] = (float)cs[i], short_sn[i] = (float)sn[i];  // (its own)
+    }
+    pdl_wait();
+    if (sq.len != 1) {
+        if (p.only && sq.len > 1 && tid == 0) report(p.err, ERR_BATCH_ROWS, p.node, seq, sq.len);
+        return;
+    }
+    const bf16* x = (const bf16*)p.proj + (long long)sq.start * p.ld;
+    __syncthreads();
+    if (newest && p.append) {
+        // (where a key head has several groups of queries, each CTA that needs the new key stores it: the same bits)
+        if (warp == 0) {
+            const bf16* src = x + p.k_off + (long long)g * dim;
+            unsigned char* to = held(p, p.keys, page_at(pos), g, dim);
+            const double f = norm_factor(p, src);
+            put_head(codes_of(p, to, pos, dim), scales_of(p, to, pos, dim), dim, key_factor(p, g),
+                     [&](int i) { return __bfloat162float(__float2bfloat16_rn((float)(turned(p.half, src, cs, sn, i) * f))); });
+        } else if (warp == 1) {
+            const bf16* src = x + p.v_off + (long long)g * vdim;
+            unsigned char* to = held(p, p.values, page_at(pos), g, vdim);
+            put_head(codes_of(p, to, pos, vdim), scales_of(p, to, pos, vdim), vdim, value_factor(p, g), [&](int i) { return __bfloat162float(src[i]); });
+        }
+        __syncthreads();
+        if (late) load(0, ahead[0]), load(1, ahead[1]);
+    }
+    // Queries as f16, times the power of two that puts their largest element next to 1: none is too large, and what is rounded is 2^-12 of an element.
+    for (int r = warp; r < kHeads; r += kWarps) {
+        __half* to = reinterpret_cast<__half*>(smem + L::q + r * L::q_stride);
+        const bool live = r < n_heads;
+        const bf16* q = x + p.q_off + (long long)(h0 + (live ? r : 0)) * dim;
+        const float f = (float)norm_factor(p, q);
+        auto value = [&](int i) {
+            const float v = to_f(q[i]);
+            if (i >= 2 * p.half) return v * f;
+            return (i < p.half ? v * short_cs[i] - to_f(q[i + p.half]) * short_sn[i] : v * short_cs[i - p.half] + to_f(q[i - p.half]) * short_sn[i - p.half]) * f;
+        };
+        float top = 0.f;
+        for (int i = lane; i < dim; i += 32) top = fmaxf(top, fabsf(value(i)));
+        const int e = min(max((int)(__float_as_uint(warp_max(top)) >> 23), 1), 253);
+        const float down = __uint_as_float((unsigned)(254 - e) << 23);
+        for (int i = lane; i < L::dk; i += 32) to[i] = __float2half_rn(live && i < dim ? value(i) * down : 0.f);
+        if (lane == 0) factor_s[r] = p.mul2 * __uint_as_float((unsigned)e << 23) * key_factor(p, g);
+    }
+    __syncthreads();
+    unsigned q[KS][8];
+#pragma unroll
+    for (int c = 0; c < KS; c++)
+#pragma unroll
+        for (int half = 0; half < 2; half++) {
+            const uint4 v = *reinterpret_cast<const uint4*>(smem + L::q + g8 * L::q_stride + (t4 * KS + c) * 32 + half * 16);
+            q[c][4 * half] = v.x;
+            q[c][4 * half + 1] = v.y;
+            q[c][4 * half + 2] = v.z;
+            q[c][4 * half + 3] = v.w;
+        }
+    const float mul[2] = {factor_s[2 * t4], factor_s[2 * t4 + 1]};
+
+    // a lane holds scores of keys g8, g8 + 8 and heads 2 · t4, 2 · t4 + 1, and results of dimensions 2 · VC · g8 + 2i, + 1 of these heads
+    float o[VC][4], top[2] = {kNone, kNone}, l[2] = {0.f, 0.f};
+#pragma unroll
+    for (int n = 0; n < VC; n++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) o[n][e] = 0.f;
+    auto attend = [&](int i, Tile<KS, VC>& t) {
+        const int j0 = first + i * step;
+        if (j0 + kKeys <= from) return;
+        float s[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < KS; c++) {
+            const unsigned two = (t.key_scale[0] >> (8 * c) & 0xFFu) | (t.key_scale[1] >> (8 * c) & 0xFFu) << 8;
+            const __half2 both = scales_f16(two), s0 = __low2half2(both), s1 = __high2half2(both);
+#pragma unroll
+            for (int w = 0; w < 2; w++) {
+                __half2 a[4], b[4];
+                units8(w ? t.key[0][c].y : t.key[0][c].x, a);
+                units8(w ? t.key[1][c].y : t.key[1][c].x, b);
+#pragma unroll
+                for (int e = 0; e < 4; e += 2)
+                    mma_f16(s, bits(__hmul2(a[e], s0)), bits(__hmul2(b[e], s1)), bits(__hmul2(a[e + 1], s0)), bits(__hmul2(b[e + 1], s1)), q[c][4 * w + e], q[c][4 * w + e + 1]);
+            }
+        }
+        const bool edge = j0 + kKeys > hi || j0 < low;
+        bool above = false;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const int j = j0 + g8 + 8 * (e >> 1);
+            float v = s[e] * mul[e & 1];
+            if (p.cap2 > 0.f) v = p.cap2 - __fdividef(2.f * p.cap2, 1.f + exp2f(v));
+            s[e] = edge && (j >= hi || j < low) ? -INFINITY : v;
+            above |= s[e] > top[e & 1] + 8.f;
+        }
+        // Weights are taken against a maximum that the largest score is up to 8 above: f16 holds 2^8 as exactly as 1, and 2^-22 of the largest weight with all its bits.
+        if (__any_sync(0xffffffffu, above)) {
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                float now = fmaxf(top[e], fmaxf(s[e], s[e + 2]));
+#pragma unroll
+                for (int d = 4; d < 32; d <<= 1) now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, d));
+                const float keep = exp2f(top[e] - now);
+                top[e] = now;
+                l[e] *= keep;
+#pragma unroll
+                for (int n = 0; n < VC; n++) {
+                    o[n][e] *= keep;
+                    o[n][e + 2] *= keep;
+                }
+            }
+        }
+        unsigned pb[2];
+#pragma unroll
+        for (int r = 0; r < 2; r++) {
+            const __half2 w = __floats2half2_rn(exp2f(s[2 * r] - top[0]), exp2f(s[2 * r + 1] - top[1]));
+            // the sums of the weights as they are multiplied: the rounding of a weight that stands out is in both
+            l[0] += __low2float(w);
+            l[1] += __high2float(w);
+            pb[r] = transpose8x8(bits(w));
+        }
+        if (edge) {  // what lies behind the last key may be no number, which a weight of 0 would not cancel: its scale would be none
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const int j = j0 + 2 * t4 + (e & 1) + 8 * (e >> 1);
+                if (j >= hi || j < low) t.value_scale[e] = 0;
+            }
+        }
+#pragma unroll
+        for (int b = 0; b < (VC + 7) / 8; b++) {
+            const __half2 s01 = scales_f16((t.value_scale[0] >> (8 * b) & 0xFFu) | (t.value_scale[1] >> (8 * b) & 0xFFu) << 8);
+            const __half2 s23 = scales_f16((t.value_scale[2] >> (8 * b) & 0xFFu) | (t.value_scale[3] >> (8 * b) & 0xFFu) << 8);
+#pragma unroll
+            for (int w = 2 * b; w < 2 * b + (VC < 8 ? 1 : 2); w++) {
+                // pairs of keys in a byte: the earlier dimension of each byte, then the later one
+                constexpr unsigned kLow = 0x0F0F0F0Fu;
+                __half2 a[4], c[4], d[4], f[4];
+                units8((t.value[0][w] & kLow) | (t.value[1][w] << 4 & ~kLow), a);
+                units8((t.value[0][w] >> 4 & kLow) | (t.value[1][w] & ~kLow), c);
+                units8((t.value[2][w] & kLow) | (t.value[3][w] << 4 & ~kLow), d);
+                units8((t.value[2][w] >> 4 & kLow) | (t.value[3][w] & ~kLow), f);
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    mma_f16(o[4 * w + e], bits(__hmul2(a[e], s01)), bits(__hmul2(c[e], s01)), bits(__hmul2(d[e], s23)), bits(__hmul2(f[e], s23)), pb[0], pb[1]);
+            }
+        }
+    };
+    for (int i = 0; i < tiles; i += 2) {
+        attend(i, ahead[0]);
+        load(i + 2, ahead[0]);
+        if (i + 1 < tiles) attend(i + 1, ahead[1]);
+        load(i + 3, ahead[1]);
+    }
+    float* parts = reinterpret_cast<float*>(smem + L::parts);
+#pragma unroll
+    for (int e = 0; e < 2; e++) {
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) l[e] += __shfl_xor_sync(0xffffffffu, l[e], d);
+        float* to = parts + warp * L::part + (t4 * 2 + e) * (L::dv + 2);
+        if (g8 == 0) {
+            to[0] = top[e];
+            to[1] = l[e];
+        }
+#pragma unroll
+        for (int n = 0; n < VC; n++) {
+            to[2 + g8 * 2 * VC + 2 * n] = o[n][e];
+            to[2 + g8 * 2 * VC + 2 * n + 1] = o[n][e + 2];
+        }
+    }
+    __syncthreads();
+    bf16* out = (bf16*)p.out + ((long long)sq.start * p.heads + h0) * vdim;
+    auto scale = [&](int) { return value_factor(p, g); };
+    auto sink = [&](int) { return p.sink ? 0.f : -INFINITY; };
+    if (p.splits == 1) {
+        merge_parts<L::dv, kHeads, kWarps>(parts, kWarps, n_heads, vdim, scale, out, nullptr, sink);
+        return;
+    }
+    const long long cell = (long long)blockIdx.z * gridDim.y + blockIdx.y;
+    merge_parts<L::dv, kHeads, kWarps>(parts, kWarps, n_heads, vdim, 0.f, nullptr, p.part + (cell * p.splits + blockIdx.x) * L::part);
+    __threadfence();
+    __syncthreads();
+    if (tid == 0) arrived = atomicAdd(&p.counters[cell], 1u);
+    __syncthreads();
+    if (arrived != (unsigned)p.splits - 1) return;
+    __threadfence();
+    if (tid == 0) p.counters[cell] = 0;
+    merge_parts<L::dv, kHeads, kWarps>(p.part + cell * p.splits * L::part, p.splits, n_heads, vdim, scale, out, nullptr, sink);
+}
+
+template <int KS, int VC> PackedDecode choice() {
+    constexpr int resident = KS <= 2 && VC <= 8 ? 3 : 2;
+    return {packed_decode<KS, VC, resident>, Smem<KS, VC>::total, Smem<KS, VC>::part, resident, kHeads, kKeys * kWarps};
+}
+template <int KS> PackedDecode choice(int64_t vdim) { return vdim <= 64 ? choice<KS, 4>() : vdim <= 128 ? choice<KS, 8>() : choice<KS, 16>(); }
+
+}  // namespace
+
+PackedDecode packed_decode_of(int64_t dim, int64_t vdim) { return dim <= 64 ? choice<1>(vdim) : dim <= 128 ? choice<2>(vdim) : choice<4>(vdim); }
+
+}  // namespace oxk

@@ -267,6 +267,16 @@ def test_a_place_that_is_none_is_reported_and_reads_as_zeros(bad, kind):
     assert np.array_equal(got[[0, 2]], want) and not got[1].any()
 
 
+def test_a_prompt_in_a_batch_of_as_many_rows_as_sequences():
+    """Taken in f32; in bf16 such a batch is one of single tokens, and a sequence of more is reported."""
+    f = Form(4, 2, 64, 128, 64)
+    check(f, [(3, 3), (1, 5), (0, 0), (0, 0)], "f32")
+    s = util.step(f, [(3, 3), (1, 5), (0, 0), (0, 0)])
+    session, _, outs = run(f, s, "bf16")
+    with pytest.raises(OnyxiaError, match="sequence 0 has 3 new tokens"):
+        session.download(outs["out"])
+
+
 @BOTH
 @pytest.mark.parametrize("form", ["attend", "write", "read"])
 def test_nothing_to_do_and_nowhere_to_put_it(form, kind):

@@ -8,6 +8,7 @@
 //   packed_write   a batch's keys (rotated, normed) and values go to the pools; its queries, where there are any, are prepared
 //   packed_read    the keys and values of given places, side by side
 //   packed_decode  sequences with one new token in bf16, all of the above in one launch (packed_decode.cu)
+//   packed_prefill sequences with several new tokens in bf16 (packed_prefill.cu)
 //   packed_simt    attention of any shape, f32 and bf16
 #include <cmath>
 
@@ -34,9 +35,19 @@ template <typename T> __global__ void __launch_bounds__(128) packed_write(const 
         const int g = h - p.heads;
         if (g < 0) {
             const T* src = x + p.q_off + (long long)h * p.dim;
-            float* q = (float*)p.q + ((long long)row * p.heads + h) * p.dim;
+            const long long at = (long long)row * p.heads + h;
             const double f = norm_factor(p, src);
-            for (int i = lane; i < p.dim; i += 32) q[i] = (float)(turned(p.half, src, angle, angle + p.half, i) * f);
+            auto value = [&](int i) { return (float)(turned(p.half, src, angle, angle + p.half, i) * f); };
+            if (p.q_mul) {
+                float top = 0.f;
+                for (int i = lane; i < p.dim; i += 32) top = fmaxf(top, fabsf(value(i)));
+                const int e = query_exponent(warp_max(top));
+                __half* q = (__half*)p.q + at * p.dim;
+                for (int i = lane; i < p.dim; i += 32) q[i] = __float2half_rn(value(i) * power_down(e));
+                if (lane == 0) p.q_mul[at] = p.mul2 * power_up(e) * key_factor(p, h / (p.heads / p.kv_heads));
+            } else {
+                for (int i = lane; i < p.dim; i += 32) ((float*)p.q)[at * p.dim + i] = value(i);
+            }
         } else if (g < p.kv_heads) {
             const T* src = x + p.k_off + (long long)g * p.dim;
             unsigned char* to = held(p, p.keys, pg, g, p.dim);
@@ -206,12 +217,13 @@ void emit_packed_attention(Emitter& em, const PackedDesc& d, const TRef& proj, c
     p.splits = 1;
     const bool bf = proj.dtype == DT_BF16, tc = out && bf && d.dim <= 256 && d.vdim <= 256 && n_seqs <= 65535;
     p.only = tc && rows == n_seqs;
-    p.singles = !tc;
-    const Buf none{kSlotNull, 0}, q = out && !p.only ? em.scratch((size_t)rows * d.heads * d.dim * 4) : none;
+    const bool prefill = tc && !p.only && d.heads / d.kv_heads <= 128 && out->buf.off % 16 == 0;
+    p.singles = !tc || (!p.only && n_seqs == 1);  // a lone token with rows of nobody behind it
+    const Buf none{kSlotNull, 0}, q = out && !p.only ? em.scratch((size_t)rows * d.heads * d.dim * (prefill ? 2 : 4)) : none, q_mul = prefill ? em.scratch((size_t)rows * d.heads * 4) : none;
     auto launch = [&](PackKernel k, dim3 grid, unsigned block, unsigned smem, Buf part, const char* label) {
         em.launch(k, grid, dim3(block), smem, p,
-                  {{&p.proj, proj.buf}, {&p.turns, turns.buf}, {&p.keys, keys.buf}, {&p.values, values.buf}, {&p.q, q}, {&p.out, out ? out->buf : none}, {&p.seqs, seqs.buf}, {&p.table, pages.buf},
-                   {&p.key_factors, key_factors ? key_factors->buf : none}, {&p.value_factors, value_factors ? value_factors->buf : none}, {&p.part, part},
+                  {{&p.proj, proj.buf}, {&p.turns, turns.buf}, {&p.keys, keys.buf}, {&p.values, values.buf}, {&p.q, q}, {&p.q_mul, q_mul}, {&p.out, out ? out->buf : none}, {&p.seqs, seqs.buf},
+                   {&p.table, pages.buf}, {&p.key_factors, key_factors ? key_factors->buf : none}, {&p.value_factors, value_factors ? value_factors->buf : none}, {&p.part, part},
                    {&p.counters, Buf{kSlotCounters, 0}}, {&p.err, Buf{kSlotErr, 0}}},
                   label, /*pdl=*/true);
     };
@@ -220,11 +232,19 @@ void emit_packed_attention(Emitter& em, const PackedDesc& d, const TRef& proj, c
         ensure_max_dynamic_smem((const void*)write, 8192 * 8);
         launch(write, dim3((unsigned)rows), 128, (unsigned)(d.rot_dims * 8), none, "packed_write");
         if (!out) return;
-        const PackKernel k = bf ? packed_simt<bf16> : packed_simt<float>;
-        ensure_max_dynamic_smem((const void*)k, 220 * 1024);
-        launch(k, dim3((unsigned)rows, (unsigned)d.heads), kAnyKeys, (unsigned)((d.dim + d.vdim + kAnyKeys) * 4), none, "packed_simt");
+        if (prefill) {
+            const int64_t rep = d.heads / d.kv_heads;
+            const PackedPrefill pf = packed_prefill_of(d.dim, d.vdim, rows, d.kv_heads, rep);
+            const int64_t tq = pf.rows / rep;
+            ensure_max_dynamic_smem((const void*)pf.kernel, pf.smem);
+            launch(pf.kernel, dim3((unsigned)((rows + tq - 1) / tq + n_seqs), (unsigned)d.kv_heads), (unsigned)pf.threads, (unsigned)pf.smem, none, "packed_prefill");
+        } else {
+            const PackKernel k = bf ? packed_simt<bf16> : packed_simt<float>;
+            ensure_max_dynamic_smem((const void*)k, 220 * 1024);
+            launch(k, dim3((unsigned)rows, (unsigned)d.heads), kAnyKeys, (unsigned)((d.dim + d.vdim + kAnyKeys) * 4), none, "packed_simt");
+        }
     }
-    if (tc) {
+    if (tc && (p.only || n_seqs > 1)) {
         const PackedDecode dc = packed_decode_of(d.dim, d.vdim);
         const int64_t groups = d.kv_heads * ((d.heads / d.kv_heads + dc.heads - 1) / dc.heads), cells = n_seqs * groups;
         // Splits of the most keys a sequence can see: whole waves of resident CTAs, each with a beginning and an end, and the pieces have to be merged.

@@ -17,7 +17,8 @@ struct PackP {
     const void* proj;            // [rows, ld]
     const float* turns;          // [2, half]
     unsigned char *keys, *values;  // [pages, kv_heads, page, dim | vdim times 9 / 16]
-    void* q;                     // prepared queries [rows, heads, dim], f32
+    void* q;                     // prepared queries [rows, heads, dim]: f32, or f16 for the prompt kernel
+    float* q_mul;                // [rows, heads]: what products with f16 queries are multiplied by, in base 2
     void* out;                   // [rows, heads · vdim]
     const int* seqs;             // [R, 4]
     const int* table;            // [R, width]
@@ -110,6 +111,31 @@ template <class P> __device__ __forceinline__ void check_others(const P& p, int 
     if (row == 0)
         for (int i = tid; i < p.n_seqs; i += threads) checked_seq(p, i);
 }
+// The tile of `tq` tokens a CTA works on, counted over the sequences with `least` new tokens and more, and the sequence that it belongs to.
+template <class P> __device__ __forceinline__ bool locate_rows(const P& p, int tile, int tq, int least, int* seq, int* first, SeqRow* row) {
+    const int lane = threadIdx.x & 31;
+    int before = 0;
+    for (int r0 = 0; r0 < p.n_seqs; r0 += 32) {
+        const SeqRow mine = r0 + lane < p.n_seqs ? checked_seq(p, r0 + lane) : SeqRow{0, 0, 0, 0};
+        const int n = mine.len >= least ? (mine.len + tq - 1) / tq : 0;
+        int inc = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, inc, o);
+            if (lane >= o) inc += v;
+        }
+        const unsigned hit = __ballot_sync(0xffffffffu, before + inc > tile);
+        if (hit) {
+            const int at = __ffs(hit) - 1;
+            *seq = r0 + at;
+            *first = (tile - before - (__shfl_sync(0xffffffffu, inc, at) - __shfl_sync(0xffffffffu, n, at))) * tq;
+            *row = SeqRow{__shfl_sync(0xffffffffu, mine.start, at), __shfl_sync(0xffffffffu, mine.len, at), __shfl_sync(0xffffffffu, mine.past, at), 0};
+            return true;
+        }
+        before += __shfl_sync(0xffffffffu, inc, 31);
+    }
+    return false;
+}
 template <class P> __device__ __forceinline__ int first_key(const P& p, int pos) { return p.window > 0 ? max(0, pos - p.window + 1) : 0; }
 // Cosine and sine of every pair at a position, by `threads` threads, in 64 bits: what one step stores is the rounding of the key itself, which any other way to compute it finds too.
 template <class P> __device__ __forceinline__ void exact_angles(const P& p, int pos, double* cs, double* sn, int tid, int threads) {
@@ -134,6 +160,10 @@ template <typename T> __device__ __forceinline__ double norm_factor(const PackP&
     return 1.0 / sqrt(ss / p.dim + p.eps);
 }
 
+// The power of two that brings the largest element of a query, `top`, next to 1, as its exponent field: queries are f16 times it, so that none is too large and what is rounded is 2^-12 of an element.
+__device__ __forceinline__ int query_exponent(float top) { return min(max((int)(__float_as_uint(top) >> 23), 1), 253); }
+__device__ __forceinline__ float power_down(int e) { return __uint_as_float((unsigned)(254 - e) << 23); }
+__device__ __forceinline__ float power_up(int e) { return __uint_as_float((unsigned)e << 23); }
 // `n` values of a head by one warp: codes and scales to where they are held. value(i): dimension i.
 template <class F> __device__ __forceinline__ void put_head(unsigned char* codes, unsigned char* scales, int n, float factor, F&& value) {
     const int lane = threadIdx.x & 31;
@@ -157,5 +187,11 @@ struct PackedDecode {
     int resident, heads, step;  // CTAs of an SM; query heads and keys that a CTA takes at a time
 };
 PackedDecode packed_decode_of(int64_t dim, int64_t vdim);
+// Prompts in bf16 (packed_prefill.cu), keys and values of 256 dimensions at most, 128 query heads of a key head at most.
+struct PackedPrefill {
+    PackKernel kernel;
+    int smem, rows, threads;  // bytes; (token, head) rows of a CTA
+};
+PackedPrefill packed_prefill_of(int64_t dim, int64_t vdim, int64_t rows, int64_t kv_heads, int64_t rep);
 
 }  // namespace oxk

@@ -175,7 +175,6 @@ template <int KS, int VC, int RESIDENT> __global__ void __launch_bounds__(kThrea
         __syncthreads();
         if (late) load(0, ahead[0]), load(1, ahead[1]);
     }
-    // Queries as f16, times the power of two that puts their largest element next to 1: none is too large, and what is rounded is 2^-12 of an element.
     for (int r = warp; r < kHeads; r += kWarps) {
         __half* to = reinterpret_cast<__half*>(smem + L::q + r * L::q_stride);
         const bool live = r < n_heads;
@@ -188,10 +187,10 @@ template <int KS, int VC, int RESIDENT> __global__ void __launch_bounds__(kThrea
         };
         float top = 0.f;
         for (int i = lane; i < dim; i += 32) top = fmaxf(top, fabsf(value(i)));
-        const int e = min(max((int)(__float_as_uint(warp_max(top)) >> 23), 1), 253);
-        const float down = __uint_as_float((unsigned)(254 - e) << 23);
+        const int e = query_exponent(warp_max(top));
+        const float down = power_down(e);
         for (int i = lane; i < L::dk; i += 32) to[i] = __float2half_rn(live && i < dim ? value(i) * down : 0.f);
-        if (lane == 0) factor_s[r] = p.mul2 * __uint_as_float((unsigned)e << 23) * key_factor(p, g);
+        if (lane == 0) factor_s[r] = p.mul2 * power_up(e) * key_factor(p, g);
     }
     __syncthreads();
     unsigned q[KS][8];

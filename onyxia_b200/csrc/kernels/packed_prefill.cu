@@ -1,0 +1,349 @@
+// Prompts over keys and values in 4 bits on tcgen05: scores and sums of values in tensor memory.
+//
+// A CTA owns one or two tiles of 128 (token, head) rows of one key head and walks over their keys. Four warps turn codes into f16 in shared memory (exactly: packed_cache.cuh), a stage ahead of the
+// products; one warp issues these; a thread per row masks and weighs scores. Two tiles take turns at the tensor core and share what is unpacked; one tile has two turns of scores.
+#include "packed_cache.cuh"
+
+namespace oxk {
+
+namespace {
+
+constexpr int kRows = 128, kUnpack = 128, kStages = 2;
+constexpr unsigned kPanelQ = kRows * 128;  // bytes: rows × 64 dimensions
+constexpr float kNone = -1e30f;            // below every score, and finite: differences stay numbers
+
+__device__ __forceinline__ unsigned bits(__half2 v) { return *reinterpret_cast<unsigned*>(&v); }
+
+// Bytes of codes per key and thread: 64 at most, in pieces of 8
+constexpr int kPieces = 8;
+struct Held {
+    uint2 codes[kPieces];
+    unsigned char scales[kPieces];
+};
+
+template <int KEYS, int TILES> __global__ void __launch_bounds__(TILES * kRows + kUnpack + 32, TILES == 1 ? 2 : 1) packed_prefill(const PackP p) {
+    extern __shared__ __align__(1024) unsigned char smem_raw[];
+    unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    constexpr int kSoft = TILES * kRows, kThreads = kSoft + kUnpack + 32, kSoftWarps = kSoft / 32, kIssues = kSoftWarps + kUnpack / 32;
+    constexpr unsigned kPanel = KEYS * 128;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, kp = (p.dim + 63) / 64, vp = (p.vdim + 63) / 64;
+    const unsigned k_stage = kp * kPanel, v_stage = vp * kPanel;
+    const unsigned sq0 = smem_u32(smem), sk = sq0 + TILES * kp * kPanelQ, sv = sk + kStages * k_stage, bars = sv + kStages * v_stage;
+    // barriers: keys there, free, values there, free, scores there, weights there, sums (two each)
+    const unsigned k_full = bars, k_free = bars + 16, v_full = bars + 32, v_free = bars + 48, s_full = bars + 64, w_full = bars + 80, o_done = bars + 96;
+    unsigned* tmem_slot = reinterpret_cast<unsigned*>(smem + (bars + 112 - sq0));
+    if (tid == 0) {
+        for (int i = 0; i < 14; i++) mbar_init(bars + i * 8, i < 2 || i == 4 || i == 5 ? kUnpack / 32 : i == 10 || i == 11 ? kRows / 32 : 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    pdl_wait();
+    const int rep = p.heads / p.kv_heads, tq = kSoft / rep, g = blockIdx.y;
+    int seq, first;
+    // long rows first: the last tiles of a sequence see the most keys
+    SeqRow sq;
+    if (!locate_rows(p, (int)gridDim.x - 1 - (int)blockIdx.x, tq, p.singles ? 1 : 2, &seq, &first, &sq)) return;
+    const int n_tok = min(tq, sq.len - first), pos0 = sq.past + first, last = pos0 + n_tok - 1;
+    const unsigned cols = TILES == 1 && vp <= 2 ? 256 : 512;
+    if (warp == kIssues) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(cols) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    const __half* queries = (const __half*)p.q;
+    for (int i = tid; i < kSoft * kp * 8; i += kThreads) {
+        const int r = i / (kp * 8), c = i % (kp * 8), tok = r / rep, h = g * rep + r % rep;
+        const bool live = tok < n_tok && c * 8 < p.dim;
+        cp_async16(sq0 + (r / kRows * kp + (c >> 3)) * kPanelQ + r % kRows * 128 + (((c & 7) ^ (r & 7)) << 4),
+                   live ? queries + ((long long)(sq.start + first + tok) * p.heads + h) * p.dim + c * 8 : queries, live);
+    }
+    cp_async_commit();
+    // dimensions that are padding are 0 in every stage
+    auto clear = [&](unsigned base, int panels, int dim) {
+        const int from = dim / 8, n = panels * 8 - from;
+        for (int i = tid; i < kStages * KEYS * n; i += kThreads) {
+            const int c = from + i % n, key = i / n % KEYS, s = i / n / KEYS;
+            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(base + (s * panels + (c >> 3)) * kPanel + key * 128 + (((c & 7) ^ (key & 7)) << 4)), "r"(0) : "memory");
+        }
+    };
+    if (p.dim % 64) clear(sk, kp, p.dim);
+    if (p.vdim % 64) clear(sv, vp, p.vdim);
+    cp_async_wait<0>();
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the tensor core reads them
+    before_sync();
+    __syncthreads();
+    after_sync();
+    pdl_trigger();  // the tensor memory is taken: nothing that starts now can keep it from this CTA
+    const unsigned tmem = *tmem_slot, t_sum = tmem + 2 * KEYS;  // two turns, or tiles, of scores; weights take their place
+    const int lowest = first_key(p, pos0), kt0 = lowest / KEYS, n = last / KEYS + 1 - kt0;
+    bool ok = true;
+
+    if (warp >= kSoftWarps && warp < kIssues) {
+        // A thread has a key, or half of one.
+        constexpr int kShare = kUnpack / KEYS;
+        const int u = tid - kSoft, key = u % KEYS, part = u / KEYS;
+        auto load = [&](int i, Held& t, unsigned char* pool, int dim) {
+            const int j = (kt0 + i) * KEYS + key, blocks = dim / kPack;
+            const bool live = i < n && j >= lowest && j <= last;  // pages in front of the window may be anybody's
+            unsigned char* from = live ? held(p, pool, page_of(p, seq, j), g, dim) : pool;
+            const uint2* codes = reinterpret_cast<const uint2*>(codes_of(p, from, j, dim));
+            const unsigned char* scales = scales_of(p, from, j, dim);
+#pragma unroll
+            for (int b = 0; b < kPieces; b++) {
+                const int at = b * kShare + part;
+                const bool in = live && at < blocks;
+                t.codes[b] = in ? codes[at] : make_uint2(0, 0);
+                t.scales[b] = in ? scales[at] : 0;
+            }
+        };
+        auto put = [&](const Held& t, unsigned base, int dim) {
+#pragma unroll
+            for (int b = 0; b < kPieces; b++) {
+                const int at = b * kShare + part;
+                if (at * kPack >= dim) break;
+                const __half2 s = __low2half2(scales_f16(t.scales[b]));
+#pragma unroll
+                for (int w = 0; w < 2; w++) {
+                    __half2 v[4];
+                    units8(w ? t.codes[b].y : t.codes[b].x, v);
+                    const int c = at * 2 + w;
+                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(base + (c >> 3) * kPanel + key * 128 + (((c & 7) ^ (key & 7)) << 4)), "r"(bits(__hmul2(v[0], s))),
+                                 "r"(bits(__hmul2(v[1], s))), "r"(bits(__hmul2(v[2], s))), "r"(bits(__hmul2(v[3], s)))
+                                 : "memory");
+                }
+            }
+        };
+        auto tell = [&](unsigned bar) {
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+        };
+        Held k, v;
+        load(0, k, p.keys, p.dim);
+        load(0, v, p.values, p.vdim);
+        RingAt at;
+        for (int i = 0; i < n; i++) {
+            if (i >= kStages && ok && !mbar_wait(k_free + at.s * 8, at.parity ^ 1)) ok = false;
+            put(k, sk + at.s * k_stage, p.dim);
+            tell(k_full + at.s * 8);
+            load(i + 1, k, p.keys, p.dim);
+            if (i >= kStages && ok && !mbar_wait(v_free + at.s * 8, at.parity ^ 1)) ok = false;
+            put(v, sv + at.s * v_stage, p.vdim);
+            tell(v_full + at.s * 8);
+            load(i + 1, v, p.values, p.vdim);
+            at.next(kStages);
+        }
+    } else if (warp == kIssues) {
+        const unsigned base = (1u << 4) | (8u << 24);  // f16 × f16 → f32, M 128
+        const unsigned by_keys = base | ((KEYS >> 3) << 17), by_values = base | (1u << 16) | ((unsigned)(vp * 8) << 17);  // the values' wide axis is the result's
+        const unsigned long long dq = umma_kmajor_desc(sq0), dk = umma_kmajor_desc(sk);
+        // as umma_wide_desc, panels of KEYS keys
+        const unsigned long long dv = (unsigned long long)((sv & 0x3FFFFu) >> 4) | ((unsigned long long)(kPanel >> 4) << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
+        // scores of a tile and stage to a place; who waits has asked for the keys
+        auto scores = [&](int tile, unsigned stage, unsigned place) {
+            const unsigned long long k = dk + stage * (k_stage >> 4), q = dq + tile * (kp * kPanelQ >> 4);
+            for (int c = 0; c < kp; c++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) umma_bf16(tmem + place * KEYS, q + c * (kPanelQ >> 4) + e * 2, k + c * (kPanel >> 4) + e * 2, by_keys, c > 0 || e > 0);
+        };
+        auto sums = [&](unsigned place, unsigned stage, unsigned to, bool more) {
+            const unsigned long long v = dv + stage * (v_stage >> 4);
+#pragma unroll
+            for (int e = 0; e < KEYS / 16; e++) umma_weights(to, tmem + place * KEYS + e * 8, v + e * 128, by_values, more || e > 0);
+        };
+        RingAt ahead, at;  // stages of keys, of values
+        auto keys_there = [&] {
+            if (ok && !mbar_wait(k_full + ahead.s * 8, ahead.parity)) ok = false;
+            after_sync();
+        };
+        if constexpr (TILES == 2) {
+            keys_there();
+            if (elect_one() && ok) {
+                scores(0, 0, 0);
+                umma_commit(s_full);
+                scores(1, 0, 1);
+                umma_commit(k_free);
+                umma_commit(s_full + 8);
+            }
+            __syncwarp();
+            ahead.next(kStages);
+            for (int i = 0; i < n; i++) {
+                if (ok && !mbar_wait(v_full + at.s * 8, at.parity)) ok = false;
+#pragma unroll
+                for (int tile = 0; tile < 2; tile++) {
+                    if (ok && !mbar_wait(w_full + tile * 8, i & 1)) ok = false;
+                    after_sync();
+                    if (elect_one() && ok) {
+                        sums(tile, at.s, t_sum + tile * 128, i > 0);
+                        if (tile == 1) umma_commit(v_free + at.s * 8);
+                        umma_commit(o_done + tile * 8);
+                    }
+                    __syncwarp();
+                    if (i + 1 == n) continue;
+                    if (tile == 0) keys_there();
+                    if (elect_one() && ok) {  // the tile's weights are read before its scores take their place: products go in order
+                        scores(tile, ahead.s, tile);
+                        if (tile == 1) umma_commit(k_free + ahead.s * 8);
+                        umma_commit(s_full + tile * 8);
+                    }
+                    __syncwarp();
+                }
+                ahead.next(kStages);
+                at.next(kStages);
+            }
+        } else {
+            RingAt turn_ahead, turn;
+            auto next_scores = [&] {
+                keys_there();
+                if (elect_one() && ok) {
+                    scores(0, ahead.s, turn_ahead.s);
+                    umma_commit(k_free + ahead.s * 8);
+                    umma_commit(s_full + turn_ahead.s * 8);
+                }
+                __syncwarp();
+                ahead.next(kStages);
+                turn_ahead.next(2);
+            };
+            next_scores();
+            for (int i = 0; i < n; i++) {
+                if (i + 1 < n) next_scores();  // the products that read this place's weights were issued before
+                if (ok && !mbar_wait(w_full + turn.s * 8, turn.parity)) ok = false;
+                if (ok && !mbar_wait(v_full + at.s * 8, at.parity)) ok = false;
+                after_sync();
+                if (elect_one() && ok) {
+                    sums(turn.s, at.s, t_sum, i > 0);
+                    umma_commit(v_free + at.s * 8);
+                    umma_commit(o_done + turn.s * 8);
+                }
+                __syncwarp();
+                at.next(kStages);
+                turn.next(2);
+            }
+        }
+    } else {
+        const int tile = warp / 4, r = tid, tok = r / rep, head = g * rep + r % rep;
+        const bool live = tok < n_tok;
+        const int pos = live ? pos0 + tok : last, low = first_key(p, pos), last_low = first_key(p, last);  // rows without a token compute something harmless
+        const long long token = sq.start + first + tok;
+        const float mul = live ? p.q_mul[token * p.heads + head] : 0.f, cap2 = p.cap2;
+        const unsigned lanes = (unsigned)((warp & 3) * 32) << 16, sum = t_sum + lanes + (TILES == 2 ? tile * 128 : 0);
+        float m = kNone, l = 0.f;
+        RingAt at;
+        if (TILES == 2) at.s = tile;
+        for (int i = 0; i < n; i++) {
+            const int j0 = (kt0 + i) * KEYS;
+            if (ok && !mbar_wait(s_full + at.s * 8, at.parity)) ok = false;
+            after_sync();
+            const unsigned place = tmem + lanes + at.s * KEYS;
+            const bool edge = j0 + KEYS - 1 > pos0 || j0 < last_low;
+            // 32 scores in base 2, the hidden ones below all
+            auto scores = [&](int c, float (&s)[32]) {
+                unsigned v[32];
+                tmem_ld32(v, place + c);
+                tmem_ld_wait();
+#pragma unroll
+                for (int e = 0; e < 32; e++) {
+                    const float x = __uint_as_float(v[e]) * mul;
+                    s[e] = cap2 > 0.f ? cap2 - __fdividef(2.f * cap2, 1.f + exp2f(x)) : x;
+                    if (edge && (j0 + c + e > pos || j0 + c + e < low)) s[e] = -INFINITY;
+                }
+            };
+            float top = -INFINITY;
+#pragma unroll
+            for (int c = 0; c < KEYS; c += 32) {
+                float s[32];
+                scores(c, s);
+#pragma unroll
+                for (int e = 0; e < 32; e++) top = fmaxf(top, s[e]);
+            }
+            // Weights are taken against a maximum that the largest score is up to 8 above: f16 holds 2^8 as exactly as 1.
+            if (__any_sync(0xffffffffu, top > m + 8.f)) {
+                const float now = fmaxf(m, top), keep = exp2f(m - now);
+                m = now;
+                l *= keep;
+                if (i > 0) {
+                    // the sums of the tile before: with two tiles these scores were made behind them
+                    if (TILES == 1 && ok && !mbar_wait(o_done + ((i - 1) & 1) * 8, (unsigned)((i - 1) >> 1) & 1)) ok = false;
+                    after_sync();
+#pragma unroll 1
+                    for (int c = 0; c < vp * 64; c += 16) {
+                        unsigned v[16];
+                        tmem_ld16(v, sum + c);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int e = 0; e < 16; e++) v[e] = __float_as_uint(__uint_as_float(v[e]) * keep);
+                        tmem_st16(sum + c, v);
+                    }
+                }
+            }
+#pragma unroll
+            for (int c = 0; c < KEYS; c += 32) {
+                float s[32];
+                scores(c, s);
+                unsigned w[16];
+#pragma unroll
+                for (int e = 0; e < 16; e++) {
+                    const float a = exp2f(s[2 * e] - m), b = exp2f(s[2 * e + 1] - m);
+                    l += a + b;
+                    w[e] = bits(__floats2half2_rn(a, b));
+                }
+                tmem_st16(place + c / 2, w);  // where scores were that this thread has read twice
+            }
+            tmem_st_wait();
+            before_sync();
+            __syncwarp();
+            if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(w_full + at.s * 8) : "memory");
+            if (TILES == 2) at.parity ^= 1;
+            else at.next(2);
+        }
+        if (TILES == 2) {
+            if (ok && !mbar_wait(o_done + tile * 8, (unsigned)(n - 1) & 1)) ok = false;
+        } else {
+            if (ok && !mbar_wait(o_done + ((n - 1) & 1) * 8, (unsigned)((n - 1) >> 1) & 1)) ok = false;
+        }
+        after_sync();
+        float f = value_factor(p, g) / l;
+        if (p.sink) {
+            const float top = fmaxf(m, 0.f), keep = exp2f(m - top);
+            f = value_factor(p, g) * keep / (l * keep + exp2f(-top));
+        }
+        bf16* out = (bf16*)p.out + (token * p.heads + head) * p.vdim;
+#pragma unroll 1
+        for (int c = 0; c < vp * 64; c += 32) {
+            unsigned v[32];
+            tmem_ld32(v, sum + c);
+            tmem_ld_wait();
+            if (live && ok) {
+#pragma unroll
+                for (int e = 0; e < 32; e += 8)
+                    if (c + e < p.vdim) {
+                        uint4 q;
+                        q.x = pack_bf16(__uint_as_float(v[e]) * f, __uint_as_float(v[e + 1]) * f);
+                        q.y = pack_bf16(__uint_as_float(v[e + 2]) * f, __uint_as_float(v[e + 3]) * f);
+                        q.z = pack_bf16(__uint_as_float(v[e + 4]) * f, __uint_as_float(v[e + 5]) * f);
+                        q.w = pack_bf16(__uint_as_float(v[e + 6]) * f, __uint_as_float(v[e + 7]) * f);
+                        *reinterpret_cast<uint4*>(out + c + e) = q;
+                    }
+            }
+            __syncwarp();
+        }
+    }
+    if (!ok && lane == 0) report(p.err, ERR_WAIT_TIMEOUT, p.node, (long long)blockIdx.x, (long long)warp);
+    before_sync();
+    __syncthreads();
+    if (warp == kIssues) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(cols) : "memory");
+}
+
+// With 512 columns of tensor memory a CTA has its SM alone.
+int smem_of(int dim, int vdim, int keys, int tiles) {
+    const int kp = (dim + 63) / 64, vp = (vdim + 63) / 64, bytes = 1024 + tiles * kp * (int)kPanelQ + kStages * (kp + vp) * keys * 128 + 128;
+    return tiles == 2 || vp > 2 ? std::max(bytes, 120 * 1024) : bytes;
+}
+
+}  // namespace
+
+PackedPrefill packed_prefill_of(int64_t dim, int64_t vdim, int64_t rows, int64_t kv_heads, int64_t rep) {
+    const bool two = dim <= 128 && vdim <= 128 && (rows * rep + 2 * kRows - 1) / (2 * kRows) * kv_heads >= 2 * sm_count();
+    if (two) return {packed_prefill<128, 2>, smem_of((int)dim, (int)vdim, 128, 2), 2 * kRows, 2 * kRows + kUnpack + 32};
+    return {packed_prefill<64, 1>, smem_of((int)dim, (int)vdim, 64, 1), kRows, kRows + kUnpack + 32};
+}
+
+}  // namespace oxk

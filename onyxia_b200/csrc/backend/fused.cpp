@@ -678,7 +678,7 @@ void differential_lower(FusedCtx& c) {
 bool packed_sizes_fit(const Module& m, const Node& n, size_t pools) {
     const Attrs& a = n.composite.attrs;
     const int64_t G = a.int_or("kv_heads", 0), D = a.int_or("dim", 0), V = a.int_or("vdim", 0);
-    if (G <= 0 || G > 65535 || D <= 0 || V <= 0 || D > 8192 || V > 8192 || D % 16 != 0 || V % 16 != 0) return false;
+    if (G <= 0 || G > 65535 || D <= 0 || V <= 0 || D > 8192 || V > 8192 || D % 16 != 0 || V % 16 != 0 || G * (D + V) > 1 << 22) return false;
     const TensorType &keys = ty(m, n.inputs[pools]), &values = ty(m, n.inputs[pools + 1]);
     for (auto [t, d] : {std::pair<const TensorType*, int64_t>{&keys, D}, {&values, V}})
         if (t->dtype != DType::U8 || t->shape.size() != 4 || !is_const(t->shape[1], G) || !t->shape[2].as_const() || !is_const(t->shape[3], d / 16 * 9)) return false;
@@ -703,7 +703,7 @@ bool packed_fits(const Module& m, const Node& n, PackedForm form) {
     const bool queries = form != PackedForm::Write, append = form != PackedForm::Shared;
     if (n.inputs.size() != 6u + (a.int_or("factors", 0) != 0 ? 2 : 0) || n.outputs.size() != (size_t)queries + (append ? 2 : 0) || !packed_sizes_fit(m, n, 2)) return false;
     const int64_t H = a.int_or("heads", 0), G = a.int_or("kv_heads", 0), D = a.int_or("dim", 0), V = a.int_or("vdim", 0), R = a.int_or("rot_dims", 0);
-    if ((queries && (H <= 0 || H > 65535 || H % G != 0)) || R < 0 || R > D || R % 2 != 0) return false;
+    if ((queries && (H <= 0 || H > 65535 || H % G != 0 || H * std::max(D, V) > 1 << 22)) || R < 0 || R > D || R % 2 != 0) return false;
     if (a.int_or("window", 0) < 0 || a.int_or("window", 0) > INT32_MAX) return false;
     for (const char* f : {"softcap", "epsilon"})
         if (!(a.float_or(f, 0.0) >= 0.0) || !std::isfinite(a.float_or(f, 0.0))) return false;

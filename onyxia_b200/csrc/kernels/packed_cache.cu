@@ -62,6 +62,146 @@ template <typename T> __global__ void __launch_bounds__(128) packed_write(const 
     }
 }
 
+// The same in bf16 eight elements at a time, where heads, rotated halves and rows allow it: a unit is eight pairs that turn or eight elements that do not, two neighbours share their scales.
+__global__ void __launch_bounds__(128, 8) packed_write8(const PackP p) {
+    // cos[half], sin[half], norms of keys [kv_heads] in 64 bits; both angles as f32, norms of queries [heads], with queries as f16 their largest elements [heads]
+    extern __shared__ double angle[];
+    pdl_enter();
+    const int row = blockIdx.x, tid = threadIdx.x;
+    // the row's queries, keys and values are on their way while its sequence is looked up and its angles are made
+    const bf16* x = (const bf16*)p.proj + (long long)row * p.ld;
+    auto fetch = [&](long long at, int n) {
+        for (int i = tid * 64; i < n; i += 128 * 64) asm volatile("prefetch.global.L1 [%0];" ::"l"(x + at + i) : "memory");
+    };
+    fetch(p.q_off, p.heads * p.dim);
+    if (p.append) fetch(p.k_off, p.kv_heads * p.dim), fetch(p.v_off, p.kv_heads * p.vdim);
+    const int s = find_seq(p.seqs, p.n_seqs, row);
+    const SeqRow sq = checked_seq(p, s);
+    check_others(p, row, tid, 128);
+    const int pos = sq.past + row - sq.start, kv = p.append ? p.kv_heads : 0;
+    if (row < sq.start || row >= sq.start + sq.len || (sq.len == 1 && !p.singles)) return;
+    double* key_norm = angle + 2 * p.half;
+    float *short_angle = reinterpret_cast<float*>(key_norm + p.kv_heads), *query_norm = short_angle + 2 * p.half;
+    unsigned* query_top = reinterpret_cast<unsigned*>(query_norm + p.heads);
+    exact_angles(p, pos, angle, angle + p.half, tid, 128);
+    for (int i = tid; i < p.half; i += 128) short_angle[i] = (float)angle[i], short_angle[p.half + i] = (float)angle[p.half + i];  // (its own)
+    const int turned = p.half / 8, units = p.dim / 8 - turned, runs = p.vdim / 8;
+    if (p.norm)
+        for (int h = tid >> 5; h < p.heads + kv; h += 4) {
+            const double f = norm_factor(p, x + (h < p.heads ? p.q_off + (long long)h * p.dim : p.k_off + (long long)(h - p.heads) * p.dim));
+            if ((tid & 31) == 0) (h < p.heads ? (void)(query_norm[h] = (float)f) : (void)(key_norm[h - p.heads] = f));
+        }
+    auto wide = [](const bf16* from, float (&v)[8]) {
+        const uint4 u = *reinterpret_cast<const uint4*>(from);
+        const unsigned w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int e = 0; e < 4; e++) v[2 * e] = __uint_as_float(w[e] << 16), v[2 * e + 1] = __uint_as_float(w[e] & 0xFFFF0000u);
+    };
+    if (p.q_mul) {  // a rotation makes no element larger than sqrt 2 times the largest
+        for (int h = tid; h < p.heads; h += 128) query_top[h] = 0;
+        __syncthreads();
+        for (int u = tid; u < p.heads * (p.dim / 8); u += 128) {
+            float a[8], top = 0.f;
+            wide(x + p.q_off + u * 8, a);
+#pragma unroll
+            for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(a[e]));
+            atomicMax(query_top + u * 8 / p.dim, __float_as_uint(top));
+        }
+    }
+    __syncthreads();
+    for (int u = tid; u < p.heads * units; u += 128) {
+        const int h = over(u, p.by_units), i = u - h * units;
+        const bool turns = i < turned;
+        const int at = turns ? i * 8 : (i + turned) * 8;
+        const bf16* src = x + p.q_off + h * p.dim + at;
+        const long long to = ((long long)row * p.heads + h) * p.dim + at;
+        float f = p.norm ? query_norm[h] : 1.f;
+        if (p.q_mul) {
+            const int e = query_exponent(__uint_as_float(query_top[h]) * f);
+            f *= power_down(e);
+            if (i == 0) p.q_mul[(long long)row * p.heads + h] = p.mul2 * power_up(e) * key_factor(p, over(h, p.by_rep));
+        }
+        auto put = [&](long long at, const float (&v)[8]) {
+            if (p.q_mul) {
+                unsigned w[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const __half2 two = __floats2half2_rn(v[2 * e], v[2 * e + 1]);
+                    w[e] = *reinterpret_cast<const unsigned*>(&two);
+                }
+                *reinterpret_cast<uint4*>((__half*)p.q + at) = make_uint4(w[0], w[1], w[2], w[3]);
+            } else {
+                float4* q = reinterpret_cast<float4*>((float*)p.q + at);
+                q[0] = make_float4(v[0], v[1], v[2], v[3]);
+                q[1] = make_float4(v[4], v[5], v[6], v[7]);
+            }
+        };
+        float a[8], b[8], o[8];
+        wide(src, a);
+        if (!turns) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) o[e] = a[e] * f;
+            put(to, o);
+            continue;
+        }
+        wide(src + p.half, b);
+        const float *c = short_angle + at, *n = c + p.half;
+#pragma unroll
+        for (int e = 0; e < 8; e++) o[e] = (a[e] * c[e] - b[e] * n[e]) * f;
+        put(to, o);
+#pragma unroll
+        for (int e = 0; e < 8; e++) o[e] = (b[e] * c[e] + a[e] * n[e]) * f;
+        put(to + p.half, o);
+    }
+    if (!p.append) return;
+    const long long pg = page_of(p, s, pos);
+    // eight dimensions from `at` on; the lane next to this one has the other eight of their scale
+    auto store = [&](unsigned char* to, int dim, int at, float (&v)[8], float factor, bool in) {
+        float a = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            if (factor != 1.f) v[e] /= factor;
+            a = max_nan(a, fabsf(v[e]));
+        }
+        const unsigned code = scale_code(max_nan(a, __shfl_xor_sync(0xffffffffu, a, 1)));
+        const float scale = scale_value(code);
+#pragma unroll
+        for (int e = 0; e < 8; e++) v[e] = over_scale(v[e], scale);
+        if (!in) return;
+        *reinterpret_cast<unsigned*>(codes_of(p, to, pos, dim) + at / 2) = codes8(v);
+        if (at % kPack == 0) scales_of(p, to, pos, dim)[at / kPack] = (unsigned char)code;
+    };
+    for (int u0 = 0; u0 < kv * units; u0 += 128) {
+        const bool in = u0 + tid < kv * units;
+        const int u = in ? u0 + tid : tid & 1, g = over(u, p.by_units), i = u - g * units;
+        const bool turns = i < turned;
+        const int at = turns ? i * 8 : (i + turned) * 8;
+        const bf16* src = x + p.k_off + g * p.dim + at;
+        unsigned char* to = held(p, p.keys, pg, g, p.dim);
+        const double f = p.norm ? key_norm[g] : 1.0;
+        const float factor = key_factor(p, g);
+        float a[8], b[8], o[8];
+        wide(src, a);
+        if (turns) wide(src + p.half, b);
+        const double *c = angle + (turns ? at : 0), *n = c + p.half;
+        auto rounded = [](double v) { return __bfloat162float(__float2bfloat16_rn((float)v)); };
+#pragma unroll
+        for (int e = 0; e < 8; e++) o[e] = rounded((turns ? (double)a[e] * c[e] - (double)b[e] * n[e] : (double)a[e]) * f);
+        store(to, p.dim, at, o, factor, in);
+        if (turned == 0) continue;  // (all lanes alike)
+#pragma unroll
+        for (int e = 0; e < 8; e++) o[e] = turns ? rounded(((double)b[e] * c[e] + (double)a[e] * n[e]) * f) : 0.f;
+        store(to, p.dim, at + p.half, o, factor, in && turns);
+    }
+    for (int u0 = 0; u0 < kv * runs; u0 += 128) {
+        const bool in = u0 + tid < kv * runs;
+        const int u = in ? u0 + tid : tid & 1, g = over(u, p.by_runs), at = (u - g * runs) * 8;
+        float a[8];
+        wide(x + p.v_off + u * 8, a);
+        store(held(p, p.values, pg, g, p.vdim), p.vdim, at, a, value_factor(p, g), in);
+    }
+}
+
 // ── reading back ──
 struct ReadP {
     unsigned char *keys, *values;
@@ -72,43 +212,67 @@ struct ReadP {
     ErrWord* err;
     long long rows;
     int n_seqs, width, n_pages, shift, kv_heads, dim, vdim, node;
+    int per;                              // places of a CTA
+    unsigned by_all, by_key, by_value;    // for over(): blocks of 16 dimensions of a place, of a key, of a value
 };
+constexpr int kReadThreads = 256, kReadRows = 64;
 
-// A CTA per place, a thread per sixteen dimensions.
-template <typename T> __global__ void __launch_bounds__(128) packed_read(const ReadP p) {
+// A CTA has a run of places, a thread sixteen dimensions at a time.
+template <typename T> __global__ void __launch_bounds__(kReadThreads) packed_read(const ReadP p) {
+    __shared__ int page_s[kReadRows], pos_s[kReadRows];
     pdl_enter();
-    const long long row = blockIdx.x;
-    const int seq = p.places[2 * row], pos = p.places[2 * row + 1], keys = p.kv_heads * p.dim / kPack, values = p.kv_heads * p.vdim / kPack;
-    long long pg = -1;
-    if ((unsigned)seq >= (unsigned)p.n_seqs || pos < 0) report(p.err, ERR_GATHER_OOB, p.node, seq < 0 || seq >= p.n_seqs ? seq : pos, p.n_seqs);
-    else {
-        const int i = pos >> p.shift;
-        const int at = i < p.width ? p.table[(long long)seq * p.width + i] : -1;
-        if ((unsigned)at >= (unsigned)p.n_pages) report(p.err, ERR_GATHER_OOB, p.node, at, p.n_pages);
-        else pg = at;
+    const long long row0 = (long long)blockIdx.x * p.per;
+    const int rows = (int)min((long long)p.per, p.rows - row0), keys = p.kv_heads * (p.dim / kPack), all = keys + p.kv_heads * (p.vdim / kPack);
+    for (int r = threadIdx.x; r < rows; r += kReadThreads) {
+        const int2 at = reinterpret_cast<const int2*>(p.places)[row0 + r];
+        int pg = -1;
+        if ((unsigned)at.x >= (unsigned)p.n_seqs || at.y < 0) report(p.err, ERR_GATHER_OOB, p.node, (unsigned)at.x >= (unsigned)p.n_seqs ? at.x : at.y, p.n_seqs);
+        else {
+            const int i = at.y >> p.shift, given = i < p.width ? p.table[(long long)at.x * p.width + i] : -1;
+            if ((unsigned)given >= (unsigned)p.n_pages) report(p.err, ERR_GATHER_OOB, p.node, given, p.n_pages);
+            else pg = given;
+        }
+        page_s[r] = pg;
+        pos_s[r] = at.y;
     }
-    T* out = (T*)p.out + row * (keys + values) * kPack;
-    for (int u = threadIdx.x; u < keys + values; u += 128) {
-        const bool of_key = u < keys;
-        const int dim = of_key ? p.dim : p.vdim, v = of_key ? u : u - keys, g = v / (dim / kPack), b = v % (dim / kPack);
-        float x[kPack];
-        if (pg < 0) {
-            for (int i = 0; i < kPack; i++) x[i] = 0.f;
-        } else {
+    __syncthreads();
+    T* out = (T*)p.out + row0 * all * kPack;
+#pragma unroll 4
+    for (int u = threadIdx.x; u < rows * all; u += kReadThreads) {
+        const int r = over(u, p.by_all), v = u - r * all, pg = page_s[r], pos = pos_s[r];
+        const bool of_key = v < keys;
+        const int dim = of_key ? p.dim : p.vdim, w = of_key ? v : v - keys, g = over(w, of_key ? p.by_key : p.by_value), b = w - g * (dim / kPack);
+        uint2 codes = make_uint2(0, 0);
+        unsigned scale = 0;
+        float f = 1.f;
+        if (pg >= 0) {
             unsigned char* from = held(p, of_key ? p.keys : p.values, pg, g, dim);
+            codes = reinterpret_cast<const uint2*>(codes_of(p, from, pos, dim))[b];
+            scale = scales_of(p, from, pos, dim)[b];
             const float* factors = of_key ? p.key_factors : p.value_factors;
-            const float f = factors ? factors[g] : 1.f, s = scale_value(scales_of(p, from, pos, dim)[b]);
-            const uint2 w = reinterpret_cast<const uint2*>(codes_of(p, from, pos, dim))[b];
+            if (factors) f = factors[g];
+        }
+        const __half2 s = __low2half2(scales_f16(scale));
+        uint4* to = reinterpret_cast<uint4*>(out + (long long)u * kPack);
 #pragma unroll
-            for (int k = 0; k < 2; k++) {
-                __half2 h[4];
-                units8(k ? w.y : w.x, h);
+        for (int k = 0; k < 2; k++) {
+            __half2 h[4];
+            units8(k ? codes.y : codes.x, h);
+            float2 x[4];
 #pragma unroll
-                for (int e = 0; e < 4; e++) x[k * 8 + 2 * e] = __low2float(h[e]) * s * f, x[k * 8 + 2 * e + 1] = __high2float(h[e]) * s * f;
+            for (int e = 0; e < 4; e++) {
+                x[e] = __half22float2(__hmul2(h[e], s));  // exact
+                x[e].x *= f;
+                x[e].y *= f;
+            }
+            if constexpr (sizeof(T) == 2) {
+                to[k] = make_uint4(pack_bf16(x[0].x, x[0].y), pack_bf16(x[1].x, x[1].y), pack_bf16(x[2].x, x[2].y), pack_bf16(x[3].x, x[3].y));
+            } else {
+                auto four = [](float2 a, float2 b) { return make_uint4(__float_as_uint(a.x), __float_as_uint(a.y), __float_as_uint(b.x), __float_as_uint(b.y)); };
+                to[2 * k] = four(x[0], x[1]);
+                to[2 * k + 1] = four(x[2], x[3]);
             }
         }
-#pragma unroll
-        for (int i = 0; i < kPack; i++) out[u * kPack + i] = from_f<T>(x[i]);
     }
 }
 
@@ -215,6 +379,9 @@ void emit_packed_attention(Emitter& em, const PackedDesc& d, const TRef& proj, c
     p.cap2 = (float)(d.softcap * (double)kLog2e);
     p.mul2 = (float)(d.softcap > 0 ? 2.0 * (double)kLog2e * d.scale / d.softcap : (double)kLog2e * d.scale);
     p.splits = 1;
+    p.by_rep = by_of(d.heads ? d.heads / d.kv_heads : 1);
+    p.by_units = by_of(d.dim / 8 - d.rot_dims / 16);
+    p.by_runs = by_of(d.vdim / 8);
     const bool bf = proj.dtype == DT_BF16, tc = out && bf && d.dim <= 256 && d.vdim <= 256 && n_seqs <= 65535;
     p.only = tc && rows == n_seqs;
     const bool prefill = tc && !p.only && d.heads / d.kv_heads <= 128 && out->buf.off % 16 == 0;
@@ -228,9 +395,16 @@ void emit_packed_attention(Emitter& em, const PackedDesc& d, const TRef& proj, c
                   label, /*pdl=*/true);
     };
     if (!p.only) {
-        const PackKernel write = bf ? packed_write<bf16> : packed_write<float>;
-        ensure_max_dynamic_smem((const void*)write, 8192 * 8);
-        launch(write, dim3((unsigned)rows), 128, (unsigned)(d.rot_dims * 8), none, "packed_write");
+        // bytes that the kernel for eight at a time shares; a block may have 48 KB
+        const int64_t eight = d.rot_dims * 12 + d.kv_heads * 8 + d.heads * 8;
+        const bool by8 = p.ld % 8 == 0 && d.q_off % 8 == 0 && d.k_off % 8 == 0 && d.v_off % 8 == 0 && proj.buf.off % 16 == 0;
+        if (bf && by8 && d.rot_dims % 32 == 0 && eight <= 48 * 1024) {
+            launch(packed_write8, dim3((unsigned)rows), 128, (unsigned)eight, none, "packed_write");
+        } else {
+            const PackKernel write = bf ? packed_write<bf16> : packed_write<float>;
+            ensure_max_dynamic_smem((const void*)write, 8192 * 8);
+            launch(write, dim3((unsigned)rows), 128, (unsigned)(d.rot_dims * 8), none, "packed_write");
+        }
         if (!out) return;
         if (prefill) {
             const int64_t rep = d.heads / d.kv_heads;
@@ -284,8 +458,14 @@ void emit_packed_read(Emitter& em, const PackedDesc& d, const TRef& keys, const 
     p.dim = (int)d.dim;
     p.vdim = (int)d.vdim;
     p.node = em.node;
+    const int64_t blocks = d.kv_heads * (d.dim + d.vdim) / kPack;
+    p.by_all = by_of(blocks);
+    p.by_key = by_of(d.dim / kPack);
+    p.by_value = by_of(d.vdim / kPack);
+    // eight blocks a thread, fewer where that leaves SMs without a CTA
+    p.per = (int)std::max<int64_t>(1, std::min<int64_t>({kReadRows, 8 * kReadThreads / blocks, (rows + 2 * sm_count() - 1) / (2 * sm_count())}));
     const Buf none{kSlotNull, 0};
-    em.launch(out.dtype == DT_BF16 ? packed_read<bf16> : packed_read<float>, dim3((unsigned)rows), dim3(128), 0, p,
+    em.launch(out.dtype == DT_BF16 ? packed_read<bf16> : packed_read<float>, dim3((unsigned)((rows + p.per - 1) / p.per)), dim3(kReadThreads), 0, p,
               {{&p.keys, keys.buf}, {&p.values, values.buf}, {&p.places, places.buf}, {&p.table, pages.buf}, {&p.out, out.buf}, {&p.key_factors, key_factors ? key_factors->buf : none},
                {&p.value_factors, value_factors ? value_factors->buf : none}, {&p.err, Buf{kSlotErr, 0}}},
               "packed_read", /*pdl=*/true);

@@ -33,8 +33,13 @@ struct PackP {
     double eps;
     int norm, sink, append;
     int singles;                 // sequences with one new token are for these kernels too
+    unsigned by_rep, by_units, by_runs;  // for over(): heads of a key head, units of eight pairs or dimensions of a query or key, runs of eight dimensions of a value
     int only;                    // no rows for prompts: as many rows as sequences, none of which may have more than one new token
 };
+
+// n / d for n < 2^32 / d: `by` is by_of(d)
+__device__ __forceinline__ int over(int n, unsigned by) { return by ? (int)__umulhi((unsigned)n, by) : n; }
+inline unsigned by_of(int64_t d) { return d > 1 ? (unsigned)(((1ull << 32) + d - 1) / d) : 0u; }
 
 __device__ __forceinline__ float key_factor(const PackP& p, int g) { return p.key_factors ? p.key_factors[g] : 1.f; }
 __device__ __forceinline__ float value_factor(const PackP& p, int g) { return p.value_factors ? p.value_factors[g] : 1.f; }

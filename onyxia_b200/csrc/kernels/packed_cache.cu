@@ -157,16 +157,23 @@ __global__ void __launch_bounds__(128, 8) packed_write8(const PackP p) {
     const long long pg = page_of(p, s, pos);
     // eight dimensions from `at` on; the lane next to this one has the other eight of their scale
     auto store = [&](unsigned char* to, int dim, int at, float (&v)[8], float factor, bool in) {
+        const bool plain = factor == 1.f;
+        if (!plain)
+#pragma unroll
+            for (int e = 0; e < 8; e++) v[e] /= factor;
         float a = 0.f;
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-            if (factor != 1.f) v[e] /= factor;
-            a = max_nan(a, fabsf(v[e]));
-        }
+        for (int e = 0; e < 8; e++) a = max_nan(a, fabsf(v[e]));
         const unsigned code = scale_code(max_nan(a, __shfl_xor_sync(0xffffffffu, a, 1)));
-        const float scale = scale_value(code);
+        const float scale = scale_value(code), by = scale > 0.f ? 1.f / scale : 0.f;
+        // (an infinite value over a scale that is none would be no number)
+        if (plain && scale > 0.f) {
 #pragma unroll
-        for (int e = 0; e < 8; e++) v[e] = over_scale(v[e], scale);
+            for (int e = 0; e < 8; e++) v[e] = near_scale(v[e], by);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; e++) v[e] = over_scale(v[e], scale);
+        }
         if (!in) return;
         *reinterpret_cast<unsigned*>(codes_of(p, to, pos, dim) + at / 2) = codes8(v);
         if (at % kPack == 0) scales_of(p, to, pos, dim)[at / kPack] = (unsigned char)code;
@@ -183,14 +190,42 @@ __global__ void __launch_bounds__(128, 8) packed_write8(const PackP p) {
         float a[8], b[8], o[8];
         wide(src, a);
         if (turns) wide(src + p.half, b);
-        const double *c = angle + (turns ? at : 0), *n = c + p.half;
-        auto rounded = [](double v) { return __bfloat162float(__float2bfloat16_rn((float)v)); };
+        // In 32 bits a key is off by less than 2^-21 of its pair; where that leaves open which bf16 it is, and for what is no number, 64 bits say. (One element of 4000.)
+        auto rounded = [&](float (&v)[8], const float (&size)[8], auto&& exact) {
+            unsigned open = 0;
 #pragma unroll
-        for (int e = 0; e < 8; e++) o[e] = rounded((turns ? (double)a[e] * c[e] - (double)b[e] * n[e] : (double)a[e]) * f);
+            for (int e = 0; e < 8; e += 2) {
+                const unsigned less = pack_bf16(v[e] - size[e] * 0x1p-21f, v[e + 1] - size[e + 1] * 0x1p-21f), more = pack_bf16(v[e] + size[e] * 0x1p-21f, v[e + 1] + size[e + 1] * 0x1p-21f);
+                open |= less ^ more;
+                v[e] = __uint_as_float(less << 16);
+                v[e + 1] = __uint_as_float(less & 0xFFFF0000u);
+            }
+            if (open)
+#pragma unroll
+                for (int e = 0; e < 8; e++) v[e] = __bfloat162float(__float2bfloat16_rn((float)exact(e)));
+        };
+        float size[8];
+        const float short_f = (float)f;
+        if (turns) {
+            const double *c = angle + at, *n = c + p.half;
+            const float *sc = short_angle + at, *sn = sc + p.half;
+#pragma unroll
+            for (int e = 0; e < 8; e++) size[e] = (fabsf(a[e]) + fabsf(b[e])) * short_f, o[e] = (a[e] * sc[e] - b[e] * sn[e]) * short_f;
+            rounded(o, size, [&](int e) { return ((double)to_f(src[e]) * c[e] - (double)to_f(src[e + p.half]) * n[e]) * f; });
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; e++) size[e] = p.norm ? fabsf(a[e]) * short_f : 0.f, o[e] = a[e] * short_f;
+            rounded(o, size, [&](int e) { return (double)to_f(src[e]) * f; });
+        }
         store(to, p.dim, at, o, factor, in);
         if (turned == 0) continue;  // (all lanes alike)
+        if (turns) {
+            const double *c = angle + at, *n = c + p.half;
+            const float *sc = short_angle + at, *sn = sc + p.half;
 #pragma unroll
-        for (int e = 0; e < 8; e++) o[e] = turns ? rounded(((double)b[e] * c[e] + (double)a[e] * n[e]) * f) : 0.f;
+            for (int e = 0; e < 8; e++) o[e] = (b[e] * sc[e] + a[e] * sn[e]) * short_f;
+            rounded(o, size, [&](int e) { return ((double)to_f(src[e + p.half]) * c[e] + (double)to_f(src[e]) * n[e]) * f; });
+        }
         store(to, p.dim, at + p.half, o, factor, in && turns);
     }
     for (int u0 = 0; u0 < kv * runs; u0 += 128) {

@@ -5,7 +5,7 @@
 // given). code · scale has six significant bits at most and lies between 2^-10 and 2688: f16 holds it exactly, so matrix instructions multiply what is stored, not a rounding of it.
 //
 // Stored is, of y = x / factor in f32 and a = max |y| over 16 dimensions, scale = e4m3(a / 6) and code = e2m1(y / scale), both to the nearest, ties to even, at most 448 and 6. Where the
-// scale comes out as 0 so do the codes; where one of the 16 is no number the scale is none, and all 16 read as NaN.
+// scale comes out as 0 so do the codes; where one of the 16 is no number the scale is none, and all 16 read as NaN. The code of 0 has no sign.
 #pragma once
 #include "paged_util.cuh"
 
@@ -73,6 +73,10 @@ __device__ __forceinline__ __half2 scales_f16(unsigned two) {
 __device__ __forceinline__ float scale_value(unsigned code) { return __low2float(scales_f16(code)); }
 // A value over its scale; 0 where that is 0 or no number.
 __device__ __forceinline__ float over_scale(float y, float scale) { return scale > 0.f ? y / scale : 0.f; }
+// The same for a value of eight significant bits (bf16), by the scale's reciprocal `by`: y / scale is halfway between two codes (a multiple of 1/4 up to 5), or 2^-10 away from it and more. The sum
+// with 3072 rounds to a multiple of 2^-12: what is halfway comes out so, the rest stays on its side.
+__device__ __forceinline__ float near_scale(float y, float by) { return __fadd_rn(__fmaf_rn(y, by, 3072.f), -3072.f); }
+__device__ __forceinline__ unsigned without_signs_of_0(unsigned codes) { return codes & (0x77777777u | (((codes & 0x77777777u) + 0x77777777u) & 0x88888888u)); }
 // Eight values over their scale as codes, the first one lowest.
 __device__ __forceinline__ unsigned codes8(const float (&r)[8]) {
     unsigned v;
@@ -81,12 +85,13 @@ __device__ __forceinline__ unsigned codes8(const float (&r)[8]) {
         " mov.b32 %0, {a, b, c, d};\n}\n"
         : "=r"(v)
         : "f"(r[0]), "f"(r[1]), "f"(r[2]), "f"(r[3]), "f"(r[4]), "f"(r[5]), "f"(r[6]), "f"(r[7]));
-    return v;
+    return without_signs_of_0(v);
 }
 __device__ __forceinline__ unsigned code_of(float r) {
     unsigned v;
     asm("{\n .reg .b8 a, b;\n cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n mov.b32 %0, {a, a, a, a};\n}\n" : "=r"(v) : "f"(r), "f"(0.f));
-    return v & 15u;
+    v &= 15u;
+    return v == 8u ? 0u : v;
 }
 // What the four bytes of a word stand for, two dimensions each, without their scale.
 __device__ __forceinline__ void units8(unsigned word, __half2 (&v)[4]) {

@@ -79,7 +79,8 @@ def packed(x, factor):
     s = SCALES[scales][..., None]
     with np.errstate(divide="ignore", invalid="ignore"):
         r = np.where(s > 0, np.abs(y) / s, 0.0)
-    codes = nearest(np.minimum(r, 6.0), MAGNITUDES) + np.where((np.signbit(y)) & (s > 0), 8, 0)
+    codes = nearest(np.minimum(r, 6.0), MAGNITUDES)
+    codes += np.where((y < 0) & (codes > 0), 8, 0)  # 0 has no sign
     return codes.reshape(x.shape).astype(np.uint8), np.where(bad, 127, scales).astype(np.uint8)
 
 

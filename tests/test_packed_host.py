@@ -118,7 +118,7 @@ def test_the_nearest_code_and_of_two_the_even_one():
     # a largest magnitude of 6 has the scale 1: halfway between two codes is the even one's
     codes, scales = one(6.0, 0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, -0.25, -5.0, 0.26, 4.99, 5.01, -0.0)
     assert util.scale_values(scales).tolist() == [[[1.0]]]
-    assert codes[0, 0, :14].tolist() == [7, 0, 2, 2, 4, 4, 6, 6, 8, 14, 1, 6, 7, 8]
+    assert codes[0, 0, :14].tolist() == [7, 0, 2, 2, 4, 4, 6, 6, 0, 14, 1, 6, 7, 0]
     # scales: the largest, the least, what is too small for one
     assert one(2688.0)[1].item() == one(1e30)[1].item() == one(np.inf)[1].item() == 126 and one(6 * 2.0 ** -9)[1].item() == 1
     codes, scales = one(6 * 2.0 ** -10, -1e-9)

@@ -40,8 +40,14 @@ template <int KS, int VC> struct Tile {
     unsigned value_scale[4];  // one byte, or two
 };
 
-// Grid: (splits, kv_heads · groups of 8 query heads, sequences).
-template <int KS, int VC, int RESIDENT> __global__ void __launch_bounds__(kThreads, RESIDENT) packed_decode(const PackP p) {
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// Grid: (splits, kv_heads · groups of 8 query heads, sequences). WHOLE: keys have 64 · KS dimensions and values 16 · VC.
+template <int KS, int VC, bool WHOLE, int RESIDENT> __global__ void __launch_bounds__(kThreads, RESIDENT) packed_decode(const PackP p) {
     extern __shared__ __align__(16) unsigned char smem[];
     __shared__ unsigned arrived;
     __shared__ int page_s[kPages];  // this CTA's pages, checked
@@ -55,7 +61,7 @@ template <int KS, int VC, int RESIDENT> __global__ void __launch_bounds__(kThrea
     const int seq = blockIdx.z;
     const SeqRow sq = checked_seq(p, seq);
     const int rep = p.heads / p.kv_heads, groups = (rep + kHeads - 1) / kHeads, g = blockIdx.y / groups, h0 = g * rep + (blockIdx.y % groups) * kHeads;
-    const int n_heads = min(kHeads, (g + 1) * rep - h0), pos = sq.past, dim = p.dim, vdim = p.vdim;
+    const int n_heads = min(kHeads, (g + 1) * rep - h0), pos = sq.past, dim = WHOLE ? 64 * KS : p.dim, vdim = WHOLE ? 16 * VC : p.vdim;
 
     // keys of this CTA: whole tiles of all four warps, so that a split never cuts a tile
     constexpr int step = kKeys * kWarps;
@@ -71,81 +77,87 @@ template <int KS, int VC, int RESIDENT> __global__ void __launch_bounds__(kThrea
         return i < kPages ? (long long)page_s[i] : page_of(p, seq, j);
     };
     const int first = lo + warp * kKeys, tiles = first < hi ? (hi - first + step - 1) / step : 0;
-    const bool whole_k = dim == L::dk, whole_v = vdim == L::dv;
+    // a page's bytes, and where this lane's part of a tile at the page's front is
+    const long long key_page = ((long long)p.kv_heads << p.shift) * (dim / kPack) * 9, value_page = ((long long)p.kv_heads << p.shift) * (vdim / kPack) * 9;
+    const unsigned char *keys0 = held(p, p.keys, 0, g, dim), *values0 = held(p, p.values, 0, g, vdim);
+    const int key_scales = (dim / 2) << p.shift, value_scales = (vdim / 2) << p.shift;
+    // The first tiles come to the L2 cache while the launch before this one ends.
+    if (lane < 8 && lane / 4 < tiles && first + (lane / 4) * step + kKeys > from) {
+        const int j0 = first + lane / 4 * step, off = j0 & ((1 << p.shift) - 1);
+        const long long pg = page_at(max(j0, from));
+        const unsigned char* at = lane & 2 ? values0 + pg * value_page : keys0 + pg * key_page;
+        const int d = lane & 2 ? vdim : dim, per = lane & 1 ? d / kPack : d / 2;
+        asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(at + (lane & 1 ? (d / 2) << p.shift : 0) + off * per), "r"(kKeys * per) : "memory");
+    }
     auto load = [&](int i, Tile<KS, VC>& t) {
         const int j0 = first + i * step;
         if (i >= tiles || j0 + kKeys <= from) return;  // (keys in front of the window are not looked at)
         const long long pg = page_at(max(j0, from));
         const int off = j0 & ((1 << p.shift) - 1);
-        const unsigned char* k = held(p, p.keys, pg, g, dim);
-        const unsigned char* ks = k + ((dim / 2) << p.shift);
+        const unsigned char* k = keys0 + pg * key_page;
+        const unsigned char *codes = k + (off + g8) * (dim / 2) + t4 * KS * 8, *scales = k + (key_scales + (off + g8) * (dim / kPack) + t4 * KS);
 #pragma unroll
         for (int r = 0; r < 2; r++) {
-            const int at = off + g8 + 8 * r;
-            const unsigned char *codes = k + at * (dim / 2) + t4 * KS * 8, *scales = ks + at * (dim / kPack) + t4 * KS;
-            if (whole_k) {
+            const unsigned char *c8 = codes + r * 8 * (dim / 2), *s8 = scales + r * 8 * (dim / kPack);
+            if constexpr (WHOLE) {
                 if constexpr (KS == 1) {
-                    t.key[r][0] = *reinterpret_cast<const uint2*>(codes);
-                    t.key_scale[r] = *scales;
+                    t.key[r][0] = *reinterpret_cast<const uint2*>(c8);
+                    t.key_scale[r] = *s8;
                 } else {
 #pragma unroll
                     for (int c = 0; c < KS; c += 2) {
-                        const uint4 v = reinterpret_cast<const uint4*>(codes)[c / 2];
+                        const uint4 v = reinterpret_cast<const uint4*>(c8)[c / 2];
                         t.key[r][c] = make_uint2(v.x, v.y);
                         t.key[r][c + 1] = make_uint2(v.z, v.w);
                     }
-                    t.key_scale[r] = KS == 2 ? *reinterpret_cast<const unsigned short*>(scales) : *reinterpret_cast<const unsigned*>(scales);
+                    t.key_scale[r] = KS == 2 ? *reinterpret_cast<const unsigned short*>(s8) : *reinterpret_cast<const unsigned*>(s8);
                 }
             } else {
                 t.key_scale[r] = 0;
 #pragma unroll
                 for (int c = 0; c < KS; c++) {
                     const bool in = t4 * KS + c < dim / kPack;
-                    t.key[r][c] = in ? reinterpret_cast<const uint2*>(codes)[c] : make_uint2(0, 0);
-                    t.key_scale[r] |= in ? (unsigned)scales[c] << (8 * c) : 0u;
+                    t.key[r][c] = in ? reinterpret_cast<const uint2*>(c8)[c] : make_uint2(0, 0);
+                    t.key_scale[r] |= in ? (unsigned)s8[c] << (8 * c) : 0u;
                 }
             }
         }
-        const unsigned char* v = held(p, p.values, pg, g, vdim);
-        const unsigned char* vs = v + ((vdim / 2) << p.shift);
+        const unsigned char* v = values0 + pg * value_page;
+        const unsigned char *value_codes = v + (off + 2 * t4) * (vdim / 2) + g8 * VC, *value_scale = v + (value_scales + (off + 2 * t4) * (vdim / kPack) + (VC == 4 ? g8 / 2 : g8 * (VC / 8)));
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-            const int at = off + 2 * t4 + (e & 1) + 8 * (e >> 1);
-            const unsigned char *codes = v + at * (vdim / 2) + g8 * VC, *scales = vs + at * (vdim / kPack);
-            if constexpr (VC == 4) {
-                const bool in = g8 * VC < vdim / 2;
-                t.value[e][0] = in ? *reinterpret_cast<const unsigned*>(codes) : 0u;
-                t.value_scale[e] = in ? scales[g8 / 2] : 0u;
-            } else if constexpr (VC == 8) {
-                const bool in = g8 * VC < vdim / 2;
-                const uint2 w = in ? *reinterpret_cast<const uint2*>(codes) : make_uint2(0, 0);
-                t.value[e][0] = w.x;
-                t.value[e][1] = w.y;
-                t.value_scale[e] = in ? scales[g8] : 0u;
-            } else if (whole_v) {
-                const uint4 w = *reinterpret_cast<const uint4*>(codes);
+            const int row = (e & 1) + 8 * (e >> 1);
+            const unsigned char *c8 = value_codes + row * (vdim / 2), *s8 = value_scale + row * (vdim / kPack);
+            if constexpr (VC < 16) {
+                const bool in = WHOLE || g8 * VC < vdim / 2;
+                if constexpr (VC == 4) {
+                    t.value[e][0] = in ? *reinterpret_cast<const unsigned*>(c8) : 0u;
+                } else {
+                    const uint2 w = in ? *reinterpret_cast<const uint2*>(c8) : make_uint2(0, 0);
+                    t.value[e][0] = w.x;
+                    t.value[e][1] = w.y;
+                }
+                t.value_scale[e] = in ? *s8 : 0u;
+            } else if constexpr (WHOLE) {
+                const uint4 w = *reinterpret_cast<const uint4*>(c8);
                 t.value[e][0] = w.x;
                 t.value[e][1] = w.y;
                 t.value[e][2] = w.z;
                 t.value[e][3] = w.w;
-                t.value_scale[e] = reinterpret_cast<const unsigned short*>(scales)[g8];
+                t.value_scale[e] = *reinterpret_cast<const unsigned short*>(s8);
             } else {
                 t.value_scale[e] = 0;
 #pragma unroll
                 for (int c = 0; c < 2; c++) {
                     const bool in = g8 * VC + c * 8 < vdim / 2;
-                    const uint2 w = in ? reinterpret_cast<const uint2*>(codes)[c] : make_uint2(0, 0);
+                    const uint2 w = in ? reinterpret_cast<const uint2*>(c8)[c] : make_uint2(0, 0);
                     t.value[e][2 * c] = w.x;
                     t.value[e][2 * c + 1] = w.y;
-                    t.value_scale[e] |= in ? (unsigned)scales[2 * g8 + c] << (8 * c) : 0u;
+                    t.value_scale[e] |= in ? (unsigned)s8[c] << (8 * c) : 0u;
                 }
             }
         }
     };
-    Tile<KS, VC> ahead[2];
-    // The first tiles are on their way while the launch before this one ends, unless the new key is among them.
-    const bool late = newest && p.append && (pos - lo) / step < 2;
-    if (!late) load(0, ahead[0]), load(1, ahead[1]);
     double *cs = reinterpret_cast<double*>(smem + L::angle), *sn = cs + L::dk / 2;
     float *short_cs = reinterpret_cast<float*>(sn + L::dk / 2), *short_sn = short_cs + L::dk / 2;
     if (sq.len == 1) {
@@ -172,8 +184,6 @@ template <int KS, int VC, int RESIDENT> __global__ void __launch_bounds__(kThrea
             unsigned char* to = held(p, p.values, page_at(pos), g, vdim);
             put_head(codes_of(p, to, pos, vdim), scales_of(p, to, pos, vdim), vdim, value_factor(p, g), [&](int i) { return __bfloat162float(src[i]); });
         }
-        __syncthreads();
-        if (late) load(0, ahead[0]), load(1, ahead[1]);
     }
     for (int r = warp; r < kHeads; r += kWarps) {
         __half* to = reinterpret_cast<__half*>(smem + L::q + r * L::q_stride);
@@ -193,6 +203,9 @@ template <int KS, int VC, int RESIDENT> __global__ void __launch_bounds__(kThrea
         if (lane == 0) factor_s[r] = p.mul2 * power_up(e) * key_factor(p, g);
     }
     __syncthreads();
+    Tile<KS, VC> ahead[2];
+    load(0, ahead[0]);
+    load(1, ahead[1]);
     unsigned q[KS][8];
 #pragma unroll
     for (int c = 0; c < KS; c++)
@@ -207,7 +220,7 @@ template <int KS, int VC, int RESIDENT> __global__ void __launch_bounds__(kThrea
     const float mul[2] = {factor_s[2 * t4], factor_s[2 * t4 + 1]};
 
     // a lane holds scores of keys g8, g8 + 8 and heads 2 · t4, 2 · t4 + 1, and results of dimensions 2 · VC · g8 + 2i, + 1 of these heads
-    float o[VC][4], top[2] = {kNone, kNone}, l[2] = {0.f, 0.f};
+    float o[VC][4], top[2] = {kNone, kNone}, most[2] = {kNone, kNone}, l[2] = {0.f, 0.f};
 #pragma unroll
     for (int n = 0; n < VC; n++)
 #pragma unroll
@@ -218,8 +231,7 @@ template <int KS, int VC, int RESIDENT> __global__ void __launch_bounds__(kThrea
         float s[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int c = 0; c < KS; c++) {
-            const unsigned two = (t.key_scale[0] >> (8 * c) & 0xFFu) | (t.key_scale[1] >> (8 * c) & 0xFFu) << 8;
-            const __half2 both = scales_f16(two), s0 = __low2half2(both), s1 = __high2half2(both);
+            const __half2 both = scales_f16(__byte_perm(t.key_scale[0], t.key_scale[1], c | (4 + c) << 4)), s0 = __low2half2(both), s1 = __high2half2(both);
 #pragma unroll
             for (int w = 0; w < 2; w++) {
                 __half2 a[4], b[4];
@@ -231,15 +243,21 @@ template <int KS, int VC, int RESIDENT> __global__ void __launch_bounds__(kThrea
             }
         }
         const bool edge = j0 + kKeys > hi || j0 < low;
-        bool above = false;
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-            const int j = j0 + g8 + 8 * (e >> 1);
-            float v = s[e] * mul[e & 1];
-            if (p.cap2 > 0.f) v = p.cap2 - __fdividef(2.f * p.cap2, 1.f + exp2f(v));
-            s[e] = edge && (j >= hi || j < low) ? -INFINITY : v;
-            above |= s[e] > top[e & 1] + 8.f;
+        for (int e = 0; e < 4; e++) s[e] *= mul[e & 1];
+        if (p.cap2 > 0.f)
+#pragma unroll
+            for (int e = 0; e < 4; e++) s[e] = p.cap2 - __fdividef(2.f * p.cap2, 1.f + exp2_fast(s[e]));
+        if (edge) {
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const int j = j0 + g8 + 8 * (e >> 1), k = j0 + 2 * t4 + (e & 1) + 8 * (e >> 1);
+                if (j >= hi || j < low) s[e] = -INFINITY;
+                // what lies behind the last key may be no number, which a weight of 0 would not cancel: its scale would be none
+                if (k >= hi || k < low) t.value_scale[e] = 0;
+            }
         }
+        const bool above = s[0] > most[0] || s[1] > most[1] || s[2] > most[0] || s[3] > most[1];
         // Weights are taken against a maximum that the largest score is up to 8 above: f16 holds 2^8 as exactly as 1, and 2^-22 of the largest weight with all its bits.
         if (__any_sync(0xffffffffu, above)) {
 #pragma unroll
@@ -247,8 +265,9 @@ template <int KS, int VC, int RESIDENT> __global__ void __launch_bounds__(kThrea
                 float now = fmaxf(top[e], fmaxf(s[e], s[e + 2]));
 #pragma unroll
                 for (int d = 4; d < 32; d <<= 1) now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, d));
-                const float keep = exp2f(top[e] - now);
+                const float keep = exp2_fast(top[e] - now);
                 top[e] = now;
+                most[e] = now + 8.f;
                 l[e] *= keep;
 #pragma unroll
                 for (int n = 0; n < VC; n++) {
@@ -260,23 +279,15 @@ template <int KS, int VC, int RESIDENT> __global__ void __launch_bounds__(kThrea
         unsigned pb[2];
 #pragma unroll
         for (int r = 0; r < 2; r++) {
-            const __half2 w = __floats2half2_rn(exp2f(s[2 * r] - top[0]), exp2f(s[2 * r + 1] - top[1]));
+            const __half2 w = __floats2half2_rn(exp2_fast(s[2 * r] - top[0]), exp2_fast(s[2 * r + 1] - top[1]));
             // the sums of the weights as they are multiplied: the rounding of a weight that stands out is in both
             l[0] += __low2float(w);
             l[1] += __high2float(w);
             pb[r] = transpose8x8(bits(w));
         }
-        if (edge) {  // what lies behind the last key may be no number, which a weight of 0 would not cancel: its scale would be none
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const int j = j0 + 2 * t4 + (e & 1) + 8 * (e >> 1);
-                if (j >= hi || j < low) t.value_scale[e] = 0;
-            }
-        }
 #pragma unroll
         for (int b = 0; b < (VC + 7) / 8; b++) {
-            const __half2 s01 = scales_f16((t.value_scale[0] >> (8 * b) & 0xFFu) | (t.value_scale[1] >> (8 * b) & 0xFFu) << 8);
-            const __half2 s23 = scales_f16((t.value_scale[2] >> (8 * b) & 0xFFu) | (t.value_scale[3] >> (8 * b) & 0xFFu) << 8);
+            const __half2 s01 = scales_f16(__byte_perm(t.value_scale[0], t.value_scale[1], b | (4 + b) << 4)), s23 = scales_f16(__byte_perm(t.value_scale[2], t.value_scale[3], b | (4 + b) << 4));
 #pragma unroll
             for (int w = 2 * b; w < 2 * b + (VC < 8 ? 1 : 2); w++) {
                 // pairs of keys in a byte: the earlier dimension of each byte, then the later one
@@ -334,14 +345,16 @@ template <int KS, int VC, int RESIDENT> __global__ void __launch_bounds__(kThrea
     merge_parts<L::dv, kHeads, kWarps>(p.part + cell * p.splits * L::part, p.splits, n_heads, vdim, scale, out, nullptr, sink);
 }
 
-template <int KS, int VC> PackedDecode choice() {
-    constexpr int resident = KS <= 2 && VC <= 8 ? 3 : 2;
-    return {packed_decode<KS, VC, resident>, Smem<KS, VC>::total, Smem<KS, VC>::part, resident, kHeads, kKeys * kWarps};
+template <int KS, int VC> PackedDecode choice(bool whole) {
+    constexpr int resident = KS <= 2 && VC <= 8 ? 4 : 2;
+    return {whole ? packed_decode<KS, VC, true, resident> : packed_decode<KS, VC, false, resident>, Smem<KS, VC>::total, Smem<KS, VC>::part, resident, kHeads, kKeys * kWarps};
 }
-template <int KS> PackedDecode choice(int64_t vdim) { return vdim <= 64 ? choice<KS, 4>() : vdim <= 128 ? choice<KS, 8>() : choice<KS, 16>(); }
+template <int KS> PackedDecode choice(int64_t dim, int64_t vdim) {
+    return vdim <= 64 ? choice<KS, 4>(dim == 64 * KS && vdim == 64) : vdim <= 128 ? choice<KS, 8>(dim == 64 * KS && vdim == 128) : choice<KS, 16>(dim == 64 * KS && vdim == 256);
+}
 
 }  // namespace
 
-PackedDecode packed_decode_of(int64_t dim, int64_t vdim) { return dim <= 64 ? choice<1>(vdim) : dim <= 128 ? choice<2>(vdim) : choice<4>(vdim); }
+PackedDecode packed_decode_of(int64_t dim, int64_t vdim) { return dim <= 64 ? choice<1>(dim, vdim) : dim <= 128 ? choice<2>(dim, vdim) : choice<4>(dim, vdim); }
 
 }  // namespace oxk

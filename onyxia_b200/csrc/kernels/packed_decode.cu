@@ -1,8 +1,8 @@
 // Single tokens over keys and values in 4 bits: sequences with one new token, their keys split over CTAs and warps, rotation, norms, storing and joining in one launch.
 //
-// A warp takes 16 keys at a time straight from the pools into registers, as both products' rows: S^T = K q^T, O^T = V^T P^T (`mma.sync`, f16). The order of a contraction is free, so a lane
-// holds for S the whole blocks of 16 dimensions of two keys, whose codes become f16 and are multiplied by their scale (exactly), and for O^T the same run of dimensions of four keys: pairs of keys
-// come together by swapping halves of bytes.
+// A warp copies 32 keys and values at a time for itself (bulk copies: what a page holds of them is four runs of bytes) and takes 16 of them as both products' rows: S^T = K q^T, O^T = V^T P^T
+// (`mma.sync`, f16). The order of a contraction is free, so a lane holds for S the whole blocks of 16 dimensions of two keys, whose codes become f16 and are multiplied by their scale (exactly), and
+// for O^T the same run of dimensions of four keys: pairs of keys come together by swapping halves of bytes.
 #include <cmath>
 
 #include "packed_cache.cuh"
@@ -11,7 +11,7 @@ namespace oxk {
 
 namespace {
 
-constexpr int kWarps = 4, kThreads = kWarps * 32, kPages = 256, kHeads = 8, kKeys = 16;
+constexpr int kWarps = 4, kThreads = kWarps * 32, kPages = 256, kHeads = 8, kKeys = 16, kTile = 2 * kKeys, kStages = 3;
 constexpr float kNone = -1e30f;  // below every score, and finite: differences stay numbers
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
@@ -25,19 +25,13 @@ __device__ __forceinline__ unsigned bits(__half2 v) { return *reinterpret_cast<u
 template <int KS, int VC> struct Smem {
     static constexpr int dk = 64 * KS, dv = 16 * VC;
     static constexpr int q_stride = dk * 2 + 16;
-    static constexpr int q = 0;                                   // [8 heads] f16
     static constexpr int part = part_size(kHeads, dv);            // floats of one partial result
-    static constexpr int parts = q + kHeads * q_stride;           // [warps][part]
-    static constexpr int angle = (parts + kWarps * part * 4 + 7) / 8 * 8;  // cosines and sines in 64 bits, and in 32
-    static constexpr int total = angle + dk * 12;
-};
-
-// What a lane holds of 16 keys and values.
-template <int KS, int VC> struct Tile {
-    uint2 key[2][KS];
-    unsigned key_scale[2];   // KS bytes
-    unsigned value[4][VC / 4];
-    unsigned value_scale[4];  // one byte, or two
+    static constexpr int stage = kTile * (dk + dv) / kPack * 9;   // codes of keys, scales, codes of values, scales
+    static constexpr int rings = kStages * kWarps * stage, parts = kWarps * part * 4;  // [stages][warps][stage]; partial results take their place
+    // before the last stage is filled: queries [8 heads] f16, cosines and sines in 64 bits, and in 32
+    static constexpr int q = (kStages - 1) * kWarps * stage, angle = q + kHeads * q_stride;
+    static constexpr int total = rings > parts ? rings : parts;
+    static_assert(angle + dk * 12 <= rings && angle % 16 == 0, "queries and angles fit the last stage");
 };
 
 __device__ __forceinline__ float exp2_fast(float x) {
@@ -52,6 +46,7 @@ template <int KS, int VC, bool WHOLE, int RESIDENT> __global__ void __launch_bou
     __shared__ unsigned arrived;
     __shared__ int page_s[kPages];  // this CTA's pages, checked
     __shared__ float factor_s[kHeads];
+    __shared__ __align__(8) unsigned long long full_s[kWarps * kStages];
     using L = Smem<KS, VC>;
     pdl_trigger();
     if (!p.append) pdl_wait();  // another node of the step may have written any of the keys
@@ -64,100 +59,53 @@ template <int KS, int VC, bool WHOLE, int RESIDENT> __global__ void __launch_bou
     const int n_heads = min(kHeads, (g + 1) * rep - h0), pos = sq.past, dim = WHOLE ? 64 * KS : p.dim, vdim = WHOLE ? 16 * VC : p.vdim;
 
     // keys of this CTA: whole tiles of all four warps, so that a split never cuts a tile
-    constexpr int step = kKeys * kWarps;
+    constexpr int step = kTile * kWarps;
     const int low = first_key(p, pos), base = low / step, blocks = sq.len == 1 ? pos / step + 1 - base : 0;
     const int b0 = base + (int)((long long)blocks * blockIdx.x / p.splits), b1 = base + (int)((long long)blocks * (blockIdx.x + 1) / p.splits);
     const int lo = b0 * step, hi = min(b1 * step, pos + 1), from = max(lo, low);  // pages in front of the window may be anybody's
     const int page0 = from >> p.shift, n_pages = from < hi ? ((hi - 1) >> p.shift) - page0 + 1 : 0;
     for (int i = tid; i < min(n_pages, kPages); i += kThreads) page_s[i] = (int)page_of(p, seq, (page0 + i) << p.shift);
     const bool newest = hi == pos + 1 && lo < hi;  // this CTA's keys include the new one
+    if (tid < kWarps * kStages) mbar_init(smem_u32(full_s + tid), 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     __syncthreads();
     auto page_at = [&](int j) {
         const int i = (j >> p.shift) - page0;
         return i < kPages ? (long long)page_s[i] : page_of(p, seq, j);
     };
-    const int first = lo + warp * kKeys, tiles = first < hi ? (hi - first + step - 1) / step : 0;
-    // a page's bytes, and where this lane's part of a tile at the page's front is
+    const int first = lo + warp * kTile, tiles = first < hi ? (hi - first + step - 1) / step : 0;
     const long long key_page = ((long long)p.kv_heads << p.shift) * (dim / kPack) * 9, value_page = ((long long)p.kv_heads << p.shift) * (vdim / kPack) * 9;
     const unsigned char *keys0 = held(p, p.keys, 0, g, dim), *values0 = held(p, p.values, 0, g, vdim);
-    const int key_scales = (dim / 2) << p.shift, value_scales = (vdim / 2) << p.shift;
-    // The first tiles come to the L2 cache while the launch before this one ends.
-    if (lane < 8 && lane / 4 < tiles && first + (lane / 4) * step + kKeys > from) {
-        const int j0 = first + lane / 4 * step, off = j0 & ((1 << p.shift) - 1);
-        const long long pg = page_at(max(j0, from));
-        const unsigned char* at = lane & 2 ? values0 + pg * value_page : keys0 + pg * key_page;
-        const int d = lane & 2 ? vdim : dim, per = lane & 1 ? d / kPack : d / 2;
-        asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(at + (lane & 1 ? (d / 2) << p.shift : 0) + off * per), "r"(kKeys * per) : "memory");
-    }
-    auto load = [&](int i, Tile<KS, VC>& t) {
-        const int j0 = first + i * step;
-        if (i >= tiles || j0 + kKeys <= from) return;  // (keys in front of the window are not looked at)
-        const long long pg = page_at(max(j0, from));
-        const int off = j0 & ((1 << p.shift) - 1);
-        const unsigned char* k = keys0 + pg * key_page;
-        const unsigned char *codes = k + (off + g8) * (dim / 2) + t4 * KS * 8, *scales = k + (key_scales + (off + g8) * (dim / kPack) + t4 * KS);
-#pragma unroll
-        for (int r = 0; r < 2; r++) {
-            const unsigned char *c8 = codes + r * 8 * (dim / 2), *s8 = scales + r * 8 * (dim / kPack);
-            if constexpr (WHOLE) {
-                if constexpr (KS == 1) {
-                    t.key[r][0] = *reinterpret_cast<const uint2*>(c8);
-                    t.key_scale[r] = *s8;
-                } else {
-#pragma unroll
-                    for (int c = 0; c < KS; c += 2) {
-                        const uint4 v = reinterpret_cast<const uint4*>(c8)[c / 2];
-                        t.key[r][c] = make_uint2(v.x, v.y);
-                        t.key[r][c + 1] = make_uint2(v.z, v.w);
-                    }
-                    t.key_scale[r] = KS == 2 ? *reinterpret_cast<const unsigned short*>(s8) : *reinterpret_cast<const unsigned*>(s8);
-                }
-            } else {
-                t.key_scale[r] = 0;
-#pragma unroll
-                for (int c = 0; c < KS; c++) {
-                    const bool in = t4 * KS + c < dim / kPack;
-                    t.key[r][c] = in ? reinterpret_cast<const uint2*>(c8)[c] : make_uint2(0, 0);
-                    t.key_scale[r] |= in ? (unsigned)s8[c] << (8 * c) : 0u;
-                }
-            }
-        }
-        const unsigned char* v = values0 + pg * value_page;
-        const unsigned char *value_codes = v + (off + 2 * t4) * (vdim / 2) + g8 * VC, *value_scale = v + (value_scales + (off + 2 * t4) * (vdim / kPack) + (VC == 4 ? g8 / 2 : g8 * (VC / 8)));
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-            const int row = (e & 1) + 8 * (e >> 1);
-            const unsigned char *c8 = value_codes + row * (vdim / 2), *s8 = value_scale + row * (vdim / kPack);
-            if constexpr (VC < 16) {
-                const bool in = WHOLE || g8 * VC < vdim / 2;
-                if constexpr (VC == 4) {
-                    t.value[e][0] = in ? *reinterpret_cast<const unsigned*>(c8) : 0u;
-                } else {
-                    const uint2 w = in ? *reinterpret_cast<const uint2*>(c8) : make_uint2(0, 0);
-                    t.value[e][0] = w.x;
-                    t.value[e][1] = w.y;
-                }
-                t.value_scale[e] = in ? *s8 : 0u;
-            } else if constexpr (WHOLE) {
-                const uint4 w = *reinterpret_cast<const uint4*>(c8);
-                t.value[e][0] = w.x;
-                t.value[e][1] = w.y;
-                t.value[e][2] = w.z;
-                t.value[e][3] = w.w;
-                t.value_scale[e] = *reinterpret_cast<const unsigned short*>(s8);
-            } else {
-                t.value_scale[e] = 0;
-#pragma unroll
-                for (int c = 0; c < 2; c++) {
-                    const bool in = g8 * VC + c * 8 < vdim / 2;
-                    const uint2 w = in ? reinterpret_cast<const uint2*>(c8)[c] : make_uint2(0, 0);
-                    t.value[e][2 * c] = w.x;
-                    t.value[e][2 * c + 1] = w.y;
-                    t.value_scale[e] |= in ? (unsigned)s8[c] << (8 * c) : 0u;
-                }
-            }
+    // a stage: what a page holds of the tile's keys and values, run behind run
+    const int key_scales = kTile * (dim / 2), value_codes = key_scales + kTile * (dim / kPack), value_scales = value_codes + kTile * (vdim / 2);
+    const unsigned ring = smem_u32(smem) + warp * L::stage, full = smem_u32(full_s + warp * kStages);
+    // By lane 0. Tiles lie in one page, or their halves in one each; what lies beyond the keys of this CTA may be on no page.
+    auto copy = [&](int i, unsigned s) {
+        if (i >= tiles || lane != 0) return;
+        const int j0 = first + i * step, whole = (1 << p.shift) >= kTile, n = whole ? kTile : kKeys;
+        const unsigned to = ring + s * kWarps * L::stage, bar = full + s * 8;
+        const int a = max(j0, from) & ~(n - 1), b = min(hi, j0 + kTile);  // whole runs from a on, before b
+        mbar_expect_tx(bar, a < b ? (unsigned)((b - a + n - 1) / n * n * ((dim + vdim) / kPack) * 9) : 0u);
+        for (int j = a; j < b; j += n) {
+            const long long pg = page_at(max(j, from));
+            const int off = j & ((1 << p.shift) - 1), at = j - j0;
+            const unsigned char *k = keys0 + pg * key_page, *v = values0 + pg * value_page;
+            auto run = [&](int dst, const unsigned char* src, int bytes) {
+                asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(to + dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+            };
+            run(at * (dim / 2), k + off * (dim / 2), n * (dim / 2));
+            run(key_scales + at * (dim / kPack), k + ((dim / 2) << p.shift) + off * (dim / kPack), n * (dim / kPack));
+            run(value_codes + at * (vdim / 2), v + off * (vdim / 2), n * (vdim / 2));
+            run(value_scales + at * (vdim / kPack), v + ((vdim / 2) << p.shift) + off * (vdim / kPack), n * (vdim / kPack));
         }
     };
+    // The first tiles are on their way while the launch before this one ends, unless the new key is among them.
+    const bool late = newest && p.append && (pos - lo) / step < kStages - 1;
+    auto fill = [&](int i, int end) {
+#pragma unroll 1
+        for (; i < end; i++) copy(i, i);
+    };
+    if (!late) fill(0, kStages - 1);
     double *cs = reinterpret_cast<double*>(smem + L::angle), *sn = cs + L::dk / 2;
     float *short_cs = reinterpret_cast<float*>(sn + L::dk / 2), *short_sn = short_cs + L::dk / 2;
     if (sq.len == 1) {
@@ -203,9 +151,6 @@ template <int KS, int VC, bool WHOLE, int RESIDENT> __global__ void __launch_bou
         if (lane == 0) factor_s[r] = p.mul2 * power_up(e) * key_factor(p, g);
     }
     __syncthreads();
-    Tile<KS, VC> ahead[2];
-    load(0, ahead[0]);
-    load(1, ahead[1]);
     unsigned q[KS][8];
 #pragma unroll
     for (int c = 0; c < KS; c++)
@@ -217,6 +162,9 @@ template <int KS, int VC, bool WHOLE, int RESIDENT> __global__ void __launch_bou
             q[c][4 * half + 2] = v.z;
             q[c][4 * half + 3] = v.w;
         }
+    asm volatile("fence.proxy.async;" ::: "memory");  // copies read the new key, and take the queries' place
+    __syncthreads();
+    fill(late ? 0 : kStages - 1, kStages);
     const float mul[2] = {factor_s[2 * t4], factor_s[2 * t4 + 1]};
 
     // a lane holds scores of keys g8, g8 + 8 and heads 2 · t4, 2 · t4 + 1, and results of dimensions 2 · VC · g8 + 2i, + 1 of these heads
@@ -225,18 +173,85 @@ template <int KS, int VC, bool WHOLE, int RESIDENT> __global__ void __launch_bou
     for (int n = 0; n < VC; n++)
 #pragma unroll
         for (int e = 0; e < 4; e++) o[n][e] = 0.f;
-    auto attend = [&](int i, Tile<KS, VC>& t) {
-        const int j0 = first + i * step;
-        if (j0 + kKeys <= from) return;
+    bool ok = true;
+    RingAt at;
+#pragma unroll 1
+    for (int i = 0; i < tiles; i++, at.next(kStages)) {
+      if (ok && !mbar_wait(full + at.s * 8, at.parity)) ok = false;
+      const unsigned char* stage = smem + (at.s * kWarps + warp) * L::stage;
+#pragma unroll 1
+      for (int half = 0; half < 2; half++) {
+        const int j0 = first + i * step + half * kKeys;
+        if (j0 + kKeys <= from || j0 >= hi) continue;
+        uint2 key[2][KS];
+        unsigned key_scale[2], value[4][VC / 4], value_scale[4];  // KS bytes; one byte, or two
+#pragma unroll
+        for (int r = 0; r < 2; r++) {
+            const int row = half * kKeys + g8 + 8 * r;
+            const unsigned char *codes = stage + row * (dim / 2) + t4 * KS * 8, *scales = stage + key_scales + row * (dim / kPack) + t4 * KS;
+            if constexpr (WHOLE && KS == 1) {
+                key[r][0] = *reinterpret_cast<const uint2*>(codes);
+                key_scale[r] = *scales;
+            } else if constexpr (WHOLE) {
+#pragma unroll
+                for (int c = 0; c < KS; c += 2) {
+                    const uint4 v = reinterpret_cast<const uint4*>(codes)[c / 2];
+                    key[r][c] = make_uint2(v.x, v.y);
+                    key[r][c + 1] = make_uint2(v.z, v.w);
+                }
+                key_scale[r] = KS == 2 ? *reinterpret_cast<const unsigned short*>(scales) : *reinterpret_cast<const unsigned*>(scales);
+            } else {
+                key_scale[r] = 0;
+#pragma unroll
+                for (int c = 0; c < KS; c++) {
+                    const bool in = t4 * KS + c < dim / kPack;
+                    key[r][c] = in ? reinterpret_cast<const uint2*>(codes)[c] : make_uint2(0, 0);
+                    key_scale[r] |= in ? (unsigned)scales[c] << (8 * c) : 0u;
+                }
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const int row = half * kKeys + 2 * t4 + (e & 1) + 8 * (e >> 1);
+            const unsigned char *codes = stage + value_codes + row * (vdim / 2) + g8 * VC, *scales = stage + value_scales + row * (vdim / kPack) + (VC == 4 ? g8 / 2 : g8 * (VC / 8));
+            if constexpr (VC < 16) {
+                const bool in = WHOLE || g8 * VC < vdim / 2;
+                if constexpr (VC == 4) {
+                    value[e][0] = in ? *reinterpret_cast<const unsigned*>(codes) : 0u;
+                } else {
+                    const uint2 w = in ? *reinterpret_cast<const uint2*>(codes) : make_uint2(0, 0);
+                    value[e][0] = w.x;
+                    value[e][1] = w.y;
+                }
+                value_scale[e] = in ? *scales : 0u;
+            } else if constexpr (WHOLE) {
+                const uint4 w = *reinterpret_cast<const uint4*>(codes);
+                value[e][0] = w.x;
+                value[e][1] = w.y;
+                value[e][2] = w.z;
+                value[e][3] = w.w;
+                value_scale[e] = *reinterpret_cast<const unsigned short*>(scales);
+            } else {
+                value_scale[e] = 0;
+#pragma unroll
+                for (int c = 0; c < 2; c++) {
+                    const bool in = g8 * VC + c * 8 < vdim / 2;
+                    const uint2 w = in ? reinterpret_cast<const uint2*>(codes)[c] : make_uint2(0, 0);
+                    value[e][2 * c] = w.x;
+                    value[e][2 * c + 1] = w.y;
+                    value_scale[e] |= in ? (unsigned)scales[c] << (8 * c) : 0u;
+                }
+            }
+        }
         float s[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int c = 0; c < KS; c++) {
-            const __half2 both = scales_f16(__byte_perm(t.key_scale[0], t.key_scale[1], c | (4 + c) << 4)), s0 = __low2half2(both), s1 = __high2half2(both);
+            const __half2 both = scales_f16(__byte_perm(key_scale[0], key_scale[1], c | (4 + c) << 4)), s0 = __low2half2(both), s1 = __high2half2(both);
 #pragma unroll
             for (int w = 0; w < 2; w++) {
                 __half2 a[4], b[4];
-                units8(w ? t.key[0][c].y : t.key[0][c].x, a);
-                units8(w ? t.key[1][c].y : t.key[1][c].x, b);
+                units8(w ? key[0][c].y : key[0][c].x, a);
+                units8(w ? key[1][c].y : key[1][c].x, b);
 #pragma unroll
                 for (int e = 0; e < 4; e += 2)
                     mma_f16(s, bits(__hmul2(a[e], s0)), bits(__hmul2(b[e], s1)), bits(__hmul2(a[e + 1], s0)), bits(__hmul2(b[e + 1], s1)), q[c][4 * w + e], q[c][4 * w + e + 1]);
@@ -254,7 +269,7 @@ template <int KS, int VC, bool WHOLE, int RESIDENT> __global__ void __launch_bou
                 const int j = j0 + g8 + 8 * (e >> 1), k = j0 + 2 * t4 + (e & 1) + 8 * (e >> 1);
                 if (j >= hi || j < low) s[e] = -INFINITY;
                 // what lies behind the last key may be no number, which a weight of 0 would not cancel: its scale would be none
-                if (k >= hi || k < low) t.value_scale[e] = 0;
+                if (k >= hi || k < low) value_scale[e] = 0;
             }
         }
         const bool above = s[0] > most[0] || s[1] > most[1] || s[2] > most[0] || s[3] > most[1];
@@ -287,29 +302,28 @@ template <int KS, int VC, bool WHOLE, int RESIDENT> __global__ void __launch_bou
         }
 #pragma unroll
         for (int b = 0; b < (VC + 7) / 8; b++) {
-            const __half2 s01 = scales_f16(__byte_perm(t.value_scale[0], t.value_scale[1], b | (4 + b) << 4)), s23 = scales_f16(__byte_perm(t.value_scale[2], t.value_scale[3], b | (4 + b) << 4));
+            const __half2 s01 = scales_f16(__byte_perm(value_scale[0], value_scale[1], b | (4 + b) << 4)), s23 = scales_f16(__byte_perm(value_scale[2], value_scale[3], b | (4 + b) << 4));
 #pragma unroll
             for (int w = 2 * b; w < 2 * b + (VC < 8 ? 1 : 2); w++) {
                 // pairs of keys in a byte: the earlier dimension of each byte, then the later one
                 constexpr unsigned kLow = 0x0F0F0F0Fu;
                 __half2 a[4], c[4], d[4], f[4];
-                units8((t.value[0][w] & kLow) | (t.value[1][w] << 4 & ~kLow), a);
-                units8((t.value[0][w] >> 4 & kLow) | (t.value[1][w] & ~kLow), c);
-                units8((t.value[2][w] & kLow) | (t.value[3][w] << 4 & ~kLow), d);
-                units8((t.value[2][w] >> 4 & kLow) | (t.value[3][w] & ~kLow), f);
+                units8((value[0][w] & kLow) | (value[1][w] << 4 & ~kLow), a);
+                units8((value[0][w] >> 4 & kLow) | (value[1][w] & ~kLow), c);
+                units8((value[2][w] & kLow) | (value[3][w] << 4 & ~kLow), d);
+                units8((value[2][w] >> 4 & kLow) | (value[3][w] & ~kLow), f);
 #pragma unroll
                 for (int e = 0; e < 4; e++)
                     mma_f16(o[4 * w + e], bits(__hmul2(a[e], s01)), bits(__hmul2(c[e], s01)), bits(__hmul2(d[e], s23)), bits(__hmul2(f[e], s23)), pb[0], pb[1]);
             }
         }
-    };
-    for (int i = 0; i < tiles; i += 2) {
-        attend(i, ahead[0]);
-        load(i + 2, ahead[0]);
-        if (i + 1 < tiles) attend(i + 1, ahead[1]);
-        load(i + 3, ahead[1]);
+      }
+      __syncwarp();
+      copy(i + kStages, at.s);
     }
-    float* parts = reinterpret_cast<float*>(smem + L::parts);
+    if (!ok && lane == 0) report(p.err, ERR_WAIT_TIMEOUT, p.node, (long long)blockIdx.x, (long long)warp);
+    __syncthreads();  // the rings become the place of partial results
+    float* parts = reinterpret_cast<float*>(smem);
 #pragma unroll
     for (int e = 0; e < 2; e++) {
 #pragma unroll
@@ -347,7 +361,7 @@ template <int KS, int VC, bool WHOLE, int RESIDENT> __global__ void __launch_bou
 
 template <int KS, int VC> PackedDecode choice(bool whole) {
     constexpr int resident = KS <= 2 && VC <= 8 ? 4 : 2;
-    return {whole ? packed_decode<KS, VC, true, resident> : packed_decode<KS, VC, false, resident>, Smem<KS, VC>::total, Smem<KS, VC>::part, resident, kHeads, kKeys * kWarps};
+    return {whole ? packed_decode<KS, VC, true, resident> : packed_decode<KS, VC, false, resident>, Smem<KS, VC>::total, Smem<KS, VC>::part, resident, kHeads, kTile * kWarps};
 }
 template <int KS> PackedDecode choice(int64_t dim, int64_t vdim) {
     return vdim <= 64 ? choice<KS, 4>(dim == 64 * KS && vdim == 64) : vdim <= 128 ? choice<KS, 8>(dim == 64 * KS && vdim == 128) : choice<KS, 16>(dim == 64 * KS && vdim == 256);

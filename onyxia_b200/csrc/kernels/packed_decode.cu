@@ -79,24 +79,38 @@ template <int KS, int VC, bool WHOLE, int RESIDENT> __global__ void __launch_bou
     // a stage: what a page holds of the tile's keys and values, run behind run
     const int key_scales = kTile * (dim / 2), value_codes = key_scales + kTile * (dim / kPack), value_scales = value_codes + kTile * (vdim / 2);
     const unsigned ring = smem_u32(smem) + warp * L::stage, full = smem_u32(full_s + warp * kStages);
-    // By lane 0. Tiles lie in one page, or their halves in one each; what lies beyond the keys of this CTA may be on no page.
+    // Tiles lie in one page, or their halves in one each; what lies beyond the keys of this CTA may be on no page.
+    const bool whole_tiles = (1 << p.shift) >= kTile;
     auto copy = [&](int i, unsigned s) {
         if (i >= tiles || lane != 0) return;
-        const int j0 = first + i * step, whole = (1 << p.shift) >= kTile, n = whole ? kTile : kKeys;
+        const int j0 = first + i * step;
         const unsigned to = ring + s * kWarps * L::stage, bar = full + s * 8;
-        const int a = max(j0, from) & ~(n - 1), b = min(hi, j0 + kTile);  // whole runs from a on, before b
-        mbar_expect_tx(bar, a < b ? (unsigned)((b - a + n - 1) / n * n * ((dim + vdim) / kPack) * 9) : 0u);
-        for (int j = a; j < b; j += n) {
+        // keys from j on, which stand `at` keys behind the tile's first
+        auto runs = [&](int j, int at, int n) {
             const long long pg = page_at(max(j, from));
-            const int off = j & ((1 << p.shift) - 1), at = j - j0;
+            const int off = j & ((1 << p.shift) - 1);
             const unsigned char *k = keys0 + pg * key_page, *v = values0 + pg * value_page;
             auto run = [&](int dst, const unsigned char* src, int bytes) {
                 asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(to + dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
             };
             run(at * (dim / 2), k + off * (dim / 2), n * (dim / 2));
-            run(key_scales + at * (dim / kPack), k + ((dim / 2) << p.shift) + off * (dim / kPack), n * (dim / kPack));
+            run(key_scales + at * (dim / kPack), k + (((dim / 2) << p.shift) + off * (dim / kPack)), n * (dim / kPack));
             run(value_codes + at * (vdim / 2), v + off * (vdim / 2), n * (vdim / 2));
-            run(value_scales + at * (vdim / kPack), v + ((vdim / 2) << p.shift) + off * (vdim / kPack), n * (vdim / kPack));
+            run(value_scales + at * (vdim / kPack), v + (((vdim / 2) << p.shift) + off * (vdim / kPack)), n * (vdim / kPack));
+        };
+        const int half_bytes = kKeys * ((dim + vdim) / kPack) * 9;
+        if (whole_tiles) {
+            if (j0 + kTile > from) {
+                mbar_expect_tx(bar, 2 * half_bytes);
+                runs(j0, 0, kTile);
+            } else {
+                mbar_expect_tx(bar, 0);
+            }
+        } else {
+            const bool one = j0 + kKeys > from && j0 < hi, two = j0 + kTile > from && j0 + kKeys < hi;
+            mbar_expect_tx(bar, (one + two) * half_bytes);
+            if (one) runs(j0, 0, kKeys);
+            if (two) runs(j0 + kKeys, kKeys, kKeys);
         }
     };
     // The first tiles are on their way while the launch before this one ends, unless the new key is among them.
@@ -179,7 +193,7 @@ template <int KS, int VC, bool WHOLE, int RESIDENT> __global__ void __launch_bou
     for (int i = 0; i < tiles; i++, at.next(kStages)) {
       if (ok && !mbar_wait(full + at.s * 8, at.parity)) ok = false;
       const unsigned char* stage = smem + (at.s * kWarps + warp) * L::stage;
-#pragma unroll 1
+#pragma unroll
       for (int half = 0; half < 2; half++) {
         const int j0 = first + i * step + half * kKeys;
         if (j0 + kKeys <= from || j0 >= hi) continue;

@@ -43,8 +43,8 @@ template <typename T> __global__ void __launch_bounds__(128) packed_write(const 
                 for (int i = lane; i < p.dim; i += 32) top = fmaxf(top, fabsf(value(i)));
                 const int e = query_exponent(warp_max(top));
                 __half* q = (__half*)p.q + at * p.dim;
-                for (int i = lane; i < p.dim; i += 32) q[i] = __float2half_rn(value(i) * power_down(e));
-                if (lane == 0) p.q_mul[at] = p.mul2 * power_up(e) * key_factor(p, h / (p.heads / p.kv_heads));
+                for (int i = lane; i < p.dim; i += 32) q[i] = __float2half_rn(copysignf(1.f, p.mul2) * value(i) * power_down(e));
+                if (lane == 0) p.q_mul[at] = fabsf(p.mul2) * power_up(e) * key_factor(p, h / (p.heads / p.kv_heads));
             } else {
                 for (int i = lane; i < p.dim; i += 32) ((float*)p.q)[at * p.dim + i] = value(i);
             }
@@ -118,8 +118,8 @@ __global__ void __launch_bounds__(128, 8) packed_write8(const PackP p) {
         float f = p.norm ? query_norm[h] : 1.f;
         if (p.q_mul) {
             const int e = query_exponent(__uint_as_float(query_top[h]) * f);
-            f *= power_down(e);
-            if (i == 0) p.q_mul[(long long)row * p.heads + h] = p.mul2 * power_up(e) * key_factor(p, over(h, p.by_rep));
+            f *= copysignf(power_down(e), p.mul2);
+            if (i == 0) p.q_mul[(long long)row * p.heads + h] = fabsf(p.mul2) * power_up(e) * key_factor(p, over(h, p.by_rep));
         }
         auto put = [&](long long at, const float (&v)[8]) {
             if (p.q_mul) {
@@ -443,7 +443,7 @@ void emit_packed_attention(Emitter& em, const PackedDesc& d, const TRef& proj, c
         if (!out) return;
         if (prefill) {
             const int64_t rep = d.heads / d.kv_heads;
-            const PackedPrefill pf = packed_prefill_of(d.dim, d.vdim, rows, d.kv_heads, rep);
+            const PackedPrefill pf = packed_prefill_of(d.dim, d.vdim, rows, d.kv_heads, rep, d.softcap > 0);
             const int64_t tq = pf.rows / rep;
             ensure_max_dynamic_smem((const void*)pf.kernel, pf.smem);
             launch(pf.kernel, dim3((unsigned)((rows + tq - 1) / tq + n_seqs), (unsigned)d.kv_heads), (unsigned)pf.threads, (unsigned)pf.smem, none, "packed_prefill");

@@ -18,7 +18,7 @@ struct PackP {
     const float* turns;          // [2, half]
     unsigned char *keys, *values;  // [pages, kv_heads, page, dim | vdim times 9 / 16]
     void* q;                     // prepared queries [rows, heads, dim]: f32, or f16 for the prompt kernel
-    float* q_mul;                // [rows, heads]: what products with f16 queries are multiplied by, in base 2
+    float* q_mul;                // [rows, heads]: what products with f16 queries are multiplied by, in base 2; the sign of `mul2` is in the queries
     void* out;                   // [rows, heads · vdim]
     const int* seqs;             // [R, 4]
     const int* table;            // [R, width]
@@ -202,6 +202,6 @@ struct PackedPrefill {
     PackKernel kernel;
     int smem, rows, threads;  // bytes; (token, head) rows of a CTA
 };
-PackedPrefill packed_prefill_of(int64_t dim, int64_t vdim, int64_t rows, int64_t kv_heads, int64_t rep);
+PackedPrefill packed_prefill_of(int64_t dim, int64_t vdim, int64_t rows, int64_t kv_heads, int64_t rep, bool capped);
 
 }  // namespace oxk

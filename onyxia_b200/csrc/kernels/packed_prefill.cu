@@ -21,7 +21,13 @@ struct Held {
     unsigned char scales[kPieces];
 };
 
-template <int KEYS, int TILES> __global__ void __launch_bounds__(TILES * kRows + kUnpack + 32, TILES == 1 ? 2 : 1) packed_prefill(const PackP p) {
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+template <int KEYS, int TILES, bool CAPPED> __global__ void __launch_bounds__(TILES * kRows + kUnpack + 32, TILES == 1 ? 2 : 1) packed_prefill(const PackP p) {
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     constexpr int kSoft = TILES * kRows, kThreads = kSoft + kUnpack + 32, kSoftWarps = kSoft / 32, kIssues = kSoftWarps + kUnpack / 32;
@@ -234,29 +240,40 @@ template <int KEYS, int TILES> __global__ void __launch_bounds__(TILES * kRows +
             after_sync();
             const unsigned place = tmem + lanes + at.s * KEYS;
             const bool edge = j0 + KEYS - 1 > pos0 || j0 < last_low;
-            // 32 scores in base 2, the hidden ones below all
-            auto scores = [&](int c, float (&s)[32]) {
-                unsigned v[32];
-                tmem_ld32(v, place + c);
-                tmem_ld_wait();
+            // In base 2. Factors are positive (a negative one is in the queries): the largest score is that of the largest product.
+            auto score = [&](float d) {
+                const float x = d * mul;
+                return CAPPED ? cap2 - __fdividef(2.f * cap2, 1.f + exp2_fast(x)) : x;
+            };
+            auto hidden = [&](int j) { return j > pos || j < low; };
+            // 32 products at a time, the next ones on their way
+            auto each = [&](auto&& take) {
+                unsigned v[2][32];
+                tmem_ld32(v[0], place);
 #pragma unroll
-                for (int e = 0; e < 32; e++) {
-                    const float x = __uint_as_float(v[e]) * mul;
-                    s[e] = cap2 > 0.f ? cap2 - __fdividef(2.f * cap2, 1.f + exp2f(x)) : x;
-                    if (edge && (j0 + c + e > pos || j0 + c + e < low)) s[e] = -INFINITY;
+                for (int c = 0; c < KEYS / 32; c++) {
+                    tmem_ld_wait();
+                    if (c + 1 < KEYS / 32) tmem_ld32(v[(c + 1) & 1], place + (c + 1) * 32);
+                    take(c * 32, v[c & 1]);
                 }
             };
             float top = -INFINITY;
+            if (edge) {
+                each([&](int c, const unsigned (&v)[32]) {
 #pragma unroll
-            for (int c = 0; c < KEYS; c += 32) {
-                float s[32];
-                scores(c, s);
+                    for (int e = 0; e < 32; e++) top = fmaxf(top, hidden(j0 + c + e) ? -INFINITY : __uint_as_float(v[e]));
+                });
+                if (top != -INFINITY) top = score(top);
+            } else {
+                each([&](int c, const unsigned (&v)[32]) {
 #pragma unroll
-                for (int e = 0; e < 32; e++) top = fmaxf(top, s[e]);
+                    for (int e = 0; e < 32; e += 2) top = fmaxf(fmaxf(top, __uint_as_float(v[e])), __uint_as_float(v[e + 1]));
+                });
+                top = score(top);
             }
             // Weights are taken against a maximum that the largest score is up to 8 above: f16 holds 2^8 as exactly as 1.
             if (__any_sync(0xffffffffu, top > m + 8.f)) {
-                const float now = fmaxf(m, top), keep = exp2f(m - now);
+                const float now = fmaxf(m, top), keep = exp2_fast(m - now);
                 m = now;
                 l *= keep;
                 if (i > 0) {
@@ -274,19 +291,24 @@ template <int KEYS, int TILES> __global__ void __launch_bounds__(TILES * kRows +
                     }
                 }
             }
-#pragma unroll
-            for (int c = 0; c < KEYS; c += 32) {
-                float s[32];
-                scores(c, s);
+            each([&](int c, const unsigned (&v)[32]) {
                 unsigned w[16];
 #pragma unroll
-                for (int e = 0; e < 16; e++) {
-                    const float a = exp2f(s[2 * e] - m), b = exp2f(s[2 * e + 1] - m);
+                for (int e = 0; e < 32; e += 2) {
+                    float a, b;
+                    if (CAPPED) a = score(__uint_as_float(v[e])) - m, b = score(__uint_as_float(v[e + 1])) - m;
+                    else a = __fmaf_rn(__uint_as_float(v[e]), mul, -m), b = __fmaf_rn(__uint_as_float(v[e + 1]), mul, -m);
+                    a = exp2_fast(a);
+                    b = exp2_fast(b);
+                    if (edge) {
+                        if (hidden(j0 + c + e)) a = 0.f;
+                        if (hidden(j0 + c + e + 1)) b = 0.f;
+                    }
                     l += a + b;
-                    w[e] = bits(__floats2half2_rn(a, b));
+                    w[e / 2] = bits(__floats2half2_rn(a, b));
                 }
                 tmem_st16(place + c / 2, w);  // where scores were that this thread has read twice
-            }
+            });
             tmem_st_wait();
             before_sync();
             __syncwarp();
@@ -340,10 +362,10 @@ int smem_of(int dim, int vdim, int keys, int tiles) {
 
 }  // namespace
 
-PackedPrefill packed_prefill_of(int64_t dim, int64_t vdim, int64_t rows, int64_t kv_heads, int64_t rep) {
+PackedPrefill packed_prefill_of(int64_t dim, int64_t vdim, int64_t rows, int64_t kv_heads, int64_t rep, bool capped) {
     const bool two = dim <= 128 && vdim <= 128 && (rows * rep + 2 * kRows - 1) / (2 * kRows) * kv_heads >= 2 * sm_count();
-    if (two) return {packed_prefill<128, 2>, smem_of((int)dim, (int)vdim, 128, 2), 2 * kRows, 2 * kRows + kUnpack + 32};
-    return {packed_prefill<64, 1>, smem_of((int)dim, (int)vdim, 64, 1), kRows, kRows + kUnpack + 32};
+    if (two) return {capped ? packed_prefill<128, 2, true> : packed_prefill<128, 2, false>, smem_of((int)dim, (int)vdim, 128, 2), 2 * kRows, 2 * kRows + kUnpack + 32};
+    return {capped ? packed_prefill<64, 1, true> : packed_prefill<64, 1, false>, smem_of((int)dim, (int)vdim, 64, 1), kRows, kRows + kUnpack + 32};
 }
 
 }  // namespace oxk

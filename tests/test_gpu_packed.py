@@ -66,7 +66,7 @@ def check(f, lengths, kind, seed=0, form="attend", **more):
     for name, want in zip(("updated.pages.keys", "updated.pages.values"), pools):
         assert name not in got or np.array_equal(got[name], want)
     if "out" in got:
-        compare(got["out"], util.reference(f, s, pools), kind, s, 1.5 * f.scale * f.dim ** 0.5 * (0.7 if f.norm else 1.0))
+        compare(got["out"], util.reference(f, s, pools), kind, s, 1.5 * abs(f.scale) * f.dim ** 0.5)
     return s, got
 
 
@@ -94,7 +94,8 @@ def test_page_sizes(page, kind):
 
 @BOTH
 @pytest.mark.parametrize("more", [dict(window=1), dict(window=17), dict(window=64), dict(window=100, sink=1), dict(softcap=5.0), dict(sink=1), dict(norm=1), dict(factors=1),
-                                  dict(softcap=20.0, sink=1, norm=1, window=90, factors=1), dict(scale=0.25)], ids=str)
+                                  dict(softcap=20.0, sink=1, norm=1, window=90, factors=1), dict(scale=0.25), dict(scale=-0.125),
+                                  dict(scale=-0.125, softcap=3.0)], ids=str)
 def test_scores(more, kind):
     f = Form(4, 2, 64, 128, 64, **more)
     check(f, [(150, 0), (1, 200), (20, 130), (1, 0), (1, 64)], kind)

@@ -86,10 +86,15 @@ template <int KEYS, int TILES, bool CAPPED> __global__ void __launch_bounds__(TI
         // A thread has a key, or half of one.
         constexpr int kShare = kUnpack / KEYS;
         const int u = tid - kSoft, key = u % KEYS, part = u / KEYS;
-        auto load = [&](int i, Held& t, unsigned char* pool, int dim) {
+        // the page of this thread's key of step i; none where the key is not there: pages in front of the window may be anybody's
+        auto page = [&](int i) {
+            const int j = (kt0 + i) * KEYS + key;
+            return i < n && j >= lowest && j <= last ? page_of(p, seq, j) : -1ll;
+        };
+        auto load = [&](int i, long long pg, Held& t, unsigned char* pool, int dim) {
             const int j = (kt0 + i) * KEYS + key, blocks = dim / kPack;
-            const bool live = i < n && j >= lowest && j <= last;  // pages in front of the window may be anybody's
-            unsigned char* from = live ? held(p, pool, page_of(p, seq, j), g, dim) : pool;
+            const bool live = pg >= 0;
+            unsigned char* from = live ? held(p, pool, pg, g, dim) : pool;
             const uint2* codes = reinterpret_cast<const uint2*>(codes_of(p, from, j, dim));
             const unsigned char* scales = scales_of(p, from, j, dim);
 #pragma unroll
@@ -123,18 +128,21 @@ template <int KEYS, int TILES, bool CAPPED> __global__ void __launch_bounds__(TI
             if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
         };
         Held k, v;
-        load(0, k, p.keys, p.dim);
-        load(0, v, p.values, p.vdim);
+        long long pg = page(0);
+        load(0, pg, k, p.keys, p.dim);
+        load(0, pg, v, p.values, p.vdim);
+        pg = page(1);
         RingAt at;
         for (int i = 0; i < n; i++) {
             if (i >= kStages && ok && !mbar_wait(k_free + at.s * 8, at.parity ^ 1)) ok = false;
             put(k, sk + at.s * k_stage, p.dim);
             tell(k_full + at.s * 8);
-            load(i + 1, k, p.keys, p.dim);
+            load(i + 1, pg, k, p.keys, p.dim);
             if (i >= kStages && ok && !mbar_wait(v_free + at.s * 8, at.parity ^ 1)) ok = false;
             put(v, sv + at.s * v_stage, p.vdim);
             tell(v_full + at.s * 8);
-            load(i + 1, v, p.values, p.vdim);
+            load(i + 1, pg, v, p.values, p.vdim);
+            pg = page(i + 2);
             at.next(kStages);
         }
     } else if (warp == kIssues) {
@@ -291,24 +299,22 @@ template <int KEYS, int TILES, bool CAPPED> __global__ void __launch_bounds__(TI
                     }
                 }
             }
-            each([&](int c, const unsigned (&v)[32]) {
+            auto weigh = [&](int c, const unsigned (&v)[32], auto&& shown) {
                 unsigned w[16];
 #pragma unroll
                 for (int e = 0; e < 32; e += 2) {
                     float a, b;
                     if (CAPPED) a = score(__uint_as_float(v[e])) - m, b = score(__uint_as_float(v[e + 1])) - m;
                     else a = __fmaf_rn(__uint_as_float(v[e]), mul, -m), b = __fmaf_rn(__uint_as_float(v[e + 1]), mul, -m);
-                    a = exp2_fast(a);
-                    b = exp2_fast(b);
-                    if (edge) {
-                        if (hidden(j0 + c + e)) a = 0.f;
-                        if (hidden(j0 + c + e + 1)) b = 0.f;
-                    }
+                    a = exp2_fast(shown(a, j0 + c + e));
+                    b = exp2_fast(shown(b, j0 + c + e + 1));
                     l += a + b;
                     w[e / 2] = bits(__floats2half2_rn(a, b));
                 }
                 tmem_st16(place + c / 2, w);  // where scores were that this thread has read twice
-            });
+            };
+            if (edge) each([&](int c, const unsigned (&v)[32]) { weigh(c, v, [&](float x, int j) { return hidden(j) ? -INFINITY : x; }); });
+            else each([&](int c, const unsigned (&v)[32]) { weigh(c, v, [](float x, int) { return x; }); });
             tmem_st_wait();
             before_sync();
             __syncwarp();

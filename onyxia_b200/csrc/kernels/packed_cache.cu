@@ -446,7 +446,7 @@ void emit_packed_attention(Emitter& em, const PackedDesc& d, const TRef& proj, c
             const PackedPrefill pf = packed_prefill_of(d.dim, d.vdim, rows, d.kv_heads, rep, d.softcap > 0);
             const int64_t tq = pf.rows / rep;
             ensure_max_dynamic_smem((const void*)pf.kernel, pf.smem);
-            launch(pf.kernel, dim3((unsigned)((rows + tq - 1) / tq + n_seqs), (unsigned)d.kv_heads), (unsigned)pf.threads, (unsigned)pf.smem, none, "packed_prefill");
+            launch(pf.kernel, dim3((unsigned)(((rows + tq - 1) / tq + n_seqs) * d.kv_heads)), (unsigned)pf.threads, (unsigned)pf.smem, none, "packed_prefill");
         } else {
             const PackKernel k = bf ? packed_simt<bf16> : packed_simt<float>;
             ensure_max_dynamic_smem((const void*)k, 220 * 1024);

@@ -43,11 +43,11 @@ template <int KEYS, int TILES, bool CAPPED> __global__ void __launch_bounds__(TI
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     pdl_wait();
-    const int rep = p.heads / p.kv_heads, tq = kSoft / rep, g = blockIdx.y;
+    const int rep = p.heads / p.kv_heads, tq = kSoft / rep, g = blockIdx.x % p.kv_heads;
     int seq, first;
-    // long rows first: the last tiles of a sequence see the most keys
+    // long rows first, of all heads: the last tiles of a sequence see the most keys
     SeqRow sq;
-    if (!locate_rows(p, (int)gridDim.x - 1 - (int)blockIdx.x, tq, p.singles ? 1 : 2, &seq, &first, &sq)) return;
+    if (!locate_rows(p, (int)((gridDim.x - 1 - blockIdx.x) / p.kv_heads), tq, p.singles ? 1 : 2, &seq, &first, &sq)) return;
     const int n_tok = min(tq, sq.len - first), pos0 = sq.past + first, last = pos0 + n_tok - 1;
     const unsigned cols = TILES == 1 && vp <= 2 ? 256 : 512;
     if (warp == kIssues) {
@@ -239,7 +239,7 @@ template <int KEYS, int TILES, bool CAPPED> __global__ void __launch_bounds__(TI
         const long long token = sq.start + first + tok;
         const float mul = live ? p.q_mul[token * p.heads + head] : 0.f, cap2 = p.cap2;
         const unsigned lanes = (unsigned)((warp & 3) * 32) << 16, sum = t_sum + lanes + (TILES == 2 ? tile * 128 : 0);
-        float m = kNone, l = 0.f;
+        float m = kNone, l = 0.f, sums[4];
         RingAt at;
         if (TILES == 2) at.s = tile;
         for (int i = 0; i < n; i++) {
@@ -299,6 +299,8 @@ template <int KEYS, int TILES, bool CAPPED> __global__ void __launch_bounds__(TI
                     }
                 }
             }
+#pragma unroll
+            for (int e = 0; e < 4; e++) sums[e] = 0.f;
             auto weigh = [&](int c, const unsigned (&v)[32], auto&& shown) {
                 unsigned w[16];
 #pragma unroll
@@ -308,13 +310,15 @@ template <int KEYS, int TILES, bool CAPPED> __global__ void __launch_bounds__(TI
                     else a = __fmaf_rn(__uint_as_float(v[e]), mul, -m), b = __fmaf_rn(__uint_as_float(v[e + 1]), mul, -m);
                     a = exp2_fast(shown(a, j0 + c + e));
                     b = exp2_fast(shown(b, j0 + c + e + 1));
-                    l += a + b;
+                    sums[e / 2 % 2] += a;
+                    sums[2 + e / 2 % 2] += b;
                     w[e / 2] = bits(__floats2half2_rn(a, b));
                 }
                 tmem_st16(place + c / 2, w);  // where scores were that this thread has read twice
             };
             if (edge) each([&](int c, const unsigned (&v)[32]) { weigh(c, v, [&](float x, int j) { return hidden(j) ? -INFINITY : x; }); });
             else each([&](int c, const unsigned (&v)[32]) { weigh(c, v, [](float x, int) { return x; }); });
+            l += (sums[0] + sums[1]) + (sums[2] + sums[3]);
             tmem_st_wait();
             before_sync();
             __syncwarp();

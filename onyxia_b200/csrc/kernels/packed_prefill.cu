@@ -1,15 +1,16 @@
 // Prompts over keys and values in 4 bits on tcgen05: scores and sums of values in tensor memory.
 //
 // A CTA owns one or two tiles of 128 (token, head) rows of one key head and walks over their keys. Four warps turn codes into f16 in shared memory (exactly: packed_cache.cuh), a stage ahead of the
-// products; one warp issues these; a thread per row masks and weighs scores. Two tiles take turns at the tensor core and share what is unpacked; one tile has two turns of scores.
+// products; one warp issues these; a thread per row masks and weighs scores, 64 keys at a time. The next 64 keys' scores are made meanwhile: a tile has two turns of them. Two tiles share what is
+// unpacked.
 #include "packed_cache.cuh"
 
 namespace oxk {
 
 namespace {
 
-constexpr int kRows = 128, kUnpack = 128, kStages = 2;
-constexpr unsigned kPanelQ = kRows * 128;  // bytes: rows × 64 dimensions
+constexpr int kRows = 128, kUnpack = 128, kStages = 2, kKeys = 64;
+constexpr unsigned kPanelQ = kRows * 128, kPanel = kKeys * 128;  // bytes: rows, or keys, × 64 dimensions
 constexpr float kNone = -1e30f;            // below every score, and finite: differences stay numbers
 
 __device__ __forceinline__ unsigned bits(__half2 v) { return *reinterpret_cast<unsigned*>(&v); }
@@ -27,19 +28,18 @@ __device__ __forceinline__ float exp2_fast(float x) {
     return y;
 }
 
-template <int KEYS, int TILES, bool CAPPED> __global__ void __launch_bounds__(TILES * kRows + kUnpack + 32, TILES == 1 ? 2 : 1) packed_prefill(const PackP p) {
+template <int TILES, bool CAPPED> __global__ void __launch_bounds__(TILES * kRows + kUnpack + 32, TILES == 1 ? 2 : 1) packed_prefill(const PackP p) {
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     constexpr int kSoft = TILES * kRows, kThreads = kSoft + kUnpack + 32, kSoftWarps = kSoft / 32, kIssues = kSoftWarps + kUnpack / 32;
-    constexpr unsigned kPanel = KEYS * 128;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, kp = (p.dim + 63) / 64, vp = (p.vdim + 63) / 64;
     const unsigned k_stage = kp * kPanel, v_stage = vp * kPanel;
     const unsigned sq0 = smem_u32(smem), sk = sq0 + TILES * kp * kPanelQ, sv = sk + kStages * k_stage, bars = sv + kStages * v_stage;
-    // barriers: keys there, free, values there, free, scores there, weights there, sums (two each)
-    const unsigned k_full = bars, k_free = bars + 16, v_full = bars + 32, v_free = bars + 48, s_full = bars + 64, w_full = bars + 80, o_done = bars + 96;
-    unsigned* tmem_slot = reinterpret_cast<unsigned*>(smem + (bars + 112 - sq0));
+    // barriers: keys there, free, values there, free (one per stage), scores there, weights there, sums (two per tile, by turns)
+    const unsigned k_full = bars, k_free = k_full + kStages * 8, v_full = k_free + kStages * 8, v_free = v_full + kStages * 8, s_full = v_free + kStages * 8, w_full = s_full + 32, o_done = w_full + 32;
+    unsigned* tmem_slot = reinterpret_cast<unsigned*>(smem + (o_done + 32 - sq0));
     if (tid == 0) {
-        for (int i = 0; i < 14; i++) mbar_init(bars + i * 8, i < 2 || i == 4 || i == 5 ? kUnpack / 32 : i == 10 || i == 11 ? kRows / 32 : 1);
+        for (unsigned b = bars; b < o_done + 32; b += 8) mbar_init(b, (b >= k_full && b < k_free) || (b >= v_full && b < v_free) ? kUnpack / 32 : b >= w_full && b < o_done ? kRows / 32 : 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     pdl_wait();
@@ -65,8 +65,8 @@ template <int KEYS, int TILES, bool CAPPED> __global__ void __launch_bounds__(TI
     // dimensions that are padding are 0 in every stage
     auto clear = [&](unsigned base, int panels, int dim) {
         const int from = dim / 8, n = panels * 8 - from;
-        for (int i = tid; i < kStages * KEYS * n; i += kThreads) {
-            const int c = from + i % n, key = i / n % KEYS, s = i / n / KEYS;
+        for (int i = tid; i < kStages * kKeys * n; i += kThreads) {
+            const int c = from + i % n, key = i / n % kKeys, s = i / n / kKeys;
             asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(base + (s * panels + (c >> 3)) * kPanel + key * 128 + (((c & 7) ^ (key & 7)) << 4)), "r"(0) : "memory");
         }
     };
@@ -78,21 +78,21 @@ template <int KEYS, int TILES, bool CAPPED> __global__ void __launch_bounds__(TI
     __syncthreads();
     after_sync();
     pdl_trigger();  // the tensor memory is taken: nothing that starts now can keep it from this CTA
-    const unsigned tmem = *tmem_slot, t_sum = tmem + 2 * KEYS;  // two turns, or tiles, of scores; weights take their place
-    const int lowest = first_key(p, pos0), kt0 = lowest / KEYS, n = last / KEYS + 1 - kt0;
+    const unsigned tmem = *tmem_slot, t_sum = tmem + TILES * 2 * kKeys;  // two turns of scores of each tile; weights take their place
+    const int lowest = first_key(p, pos0), kt0 = lowest / kKeys, n = last / kKeys + 1 - kt0;
     bool ok = true;
 
     if (warp >= kSoftWarps && warp < kIssues) {
         // A thread has a key, or half of one.
-        constexpr int kShare = kUnpack / KEYS;
-        const int u = tid - kSoft, key = u % KEYS, part = u / KEYS;
+        constexpr int kShare = kUnpack / kKeys;
+        const int u = tid - kSoft, key = u % kKeys, part = u / kKeys;
         // the page of this thread's key of step i; none where the key is not there: pages in front of the window may be anybody's
         auto page = [&](int i) {
-            const int j = (kt0 + i) * KEYS + key;
+            const int j = (kt0 + i) * kKeys + key;
             return i < n && j >= lowest && j <= last ? page_of(p, seq, j) : -1ll;
         };
         auto load = [&](int i, long long pg, Held& t, unsigned char* pool, int dim) {
-            const int j = (kt0 + i) * KEYS + key, blocks = dim / kPack;
+            const int j = (kt0 + i) * kKeys + key, blocks = dim / kPack;
             const bool live = pg >= 0;
             unsigned char* from = live ? held(p, pool, pg, g, dim) : pool;
             const uint2* codes = reinterpret_cast<const uint2*>(codes_of(p, from, j, dim));
@@ -147,107 +147,66 @@ template <int KEYS, int TILES, bool CAPPED> __global__ void __launch_bounds__(TI
         }
     } else if (warp == kIssues) {
         const unsigned base = (1u << 4) | (8u << 24);  // f16 × f16 → f32, M 128
-        const unsigned by_keys = base | ((KEYS >> 3) << 17), by_values = base | (1u << 16) | ((unsigned)(vp * 8) << 17);  // the values' wide axis is the result's
-        const unsigned long long dq = umma_kmajor_desc(sq0), dk = umma_kmajor_desc(sk);
-        // as umma_wide_desc, panels of KEYS keys
-        const unsigned long long dv = (unsigned long long)((sv & 0x3FFFFu) >> 4) | ((unsigned long long)(kPanel >> 4) << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
-        // scores of a tile and stage to a place; who waits has asked for the keys
-        auto scores = [&](int tile, unsigned stage, unsigned place) {
-            const unsigned long long k = dk + stage * (k_stage >> 4), q = dq + tile * (kp * kPanelQ >> 4);
-            for (int c = 0; c < kp; c++)
-#pragma unroll
-                for (int e = 0; e < 4; e++) umma_bf16(tmem + place * KEYS, q + c * (kPanelQ >> 4) + e * 2, k + c * (kPanel >> 4) + e * 2, by_keys, c > 0 || e > 0);
-        };
-        auto sums = [&](unsigned place, unsigned stage, unsigned to, bool more) {
-            const unsigned long long v = dv + stage * (v_stage >> 4);
-#pragma unroll
-            for (int e = 0; e < KEYS / 16; e++) umma_weights(to, tmem + place * KEYS + e * 8, v + e * 128, by_values, more || e > 0);
-        };
+        const unsigned by_keys = base | ((kKeys >> 3) << 17), by_values = base | (1u << 16) | ((unsigned)(vp * 8) << 17);  // the values' wide axis is the result's
+        const unsigned long long dq = umma_kmajor_desc(sq0), dk = umma_kmajor_desc(sk), dv = umma_wide_desc(sv);
         RingAt ahead, at;  // stages of keys, of values
-        auto keys_there = [&] {
+        unsigned turn_ahead = 0, turn = 0, parity = 0;
+        auto next_scores = [&] {
             if (ok && !mbar_wait(k_full + ahead.s * 8, ahead.parity)) ok = false;
             after_sync();
-        };
-        if constexpr (TILES == 2) {
-            keys_there();
             if (elect_one() && ok) {
-                scores(0, 0, 0);
-                umma_commit(s_full);
-                scores(1, 0, 1);
-                umma_commit(k_free);
-                umma_commit(s_full + 8);
+                const unsigned long long k = dk + ahead.s * (k_stage >> 4);
+#pragma unroll
+                for (int tile = 0; tile < TILES; tile++) {
+                    const unsigned long long q = dq + tile * (kp * kPanelQ >> 4);
+                    for (int c = 0; c < kp; c++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++)
+                            umma_bf16(tmem + (2 * tile + turn_ahead) * kKeys, q + c * (kPanelQ >> 4) + e * 2, k + c * (kPanel >> 4) + e * 2, by_keys, c > 0 || e > 0);
+                    if (tile == TILES - 1) umma_commit(k_free + ahead.s * 8);
+                    umma_commit(s_full + (2 * tile + turn_ahead) * 8);
+                }
             }
             __syncwarp();
             ahead.next(kStages);
-            for (int i = 0; i < n; i++) {
-                if (ok && !mbar_wait(v_full + at.s * 8, at.parity)) ok = false;
+            turn_ahead ^= 1;
+        };
+        next_scores();
+        for (int i = 0; i < n; i++) {
+            if (i + 1 < n) next_scores();  // the products that read the weights in this place were issued before
+            if (ok && !mbar_wait(v_full + at.s * 8, at.parity)) ok = false;
 #pragma unroll
-                for (int tile = 0; tile < 2; tile++) {
-                    if (ok && !mbar_wait(w_full + tile * 8, i & 1)) ok = false;
-                    after_sync();
-                    if (elect_one() && ok) {
-                        sums(tile, at.s, t_sum + tile * 128, i > 0);
-                        if (tile == 1) umma_commit(v_free + at.s * 8);
-                        umma_commit(o_done + tile * 8);
-                    }
-                    __syncwarp();
-                    if (i + 1 == n) continue;
-                    if (tile == 0) keys_there();
-                    if (elect_one() && ok) {  // the tile's weights are read before its scores take their place: products go in order
-                        scores(tile, ahead.s, tile);
-                        if (tile == 1) umma_commit(k_free + ahead.s * 8);
-                        umma_commit(s_full + tile * 8);
-                    }
-                    __syncwarp();
-                }
-                ahead.next(kStages);
-                at.next(kStages);
-            }
-        } else {
-            RingAt turn_ahead, turn;
-            auto next_scores = [&] {
-                keys_there();
-                if (elect_one() && ok) {
-                    scores(0, ahead.s, turn_ahead.s);
-                    umma_commit(k_free + ahead.s * 8);
-                    umma_commit(s_full + turn_ahead.s * 8);
-                }
-                __syncwarp();
-                ahead.next(kStages);
-                turn_ahead.next(2);
-            };
-            next_scores();
-            for (int i = 0; i < n; i++) {
-                if (i + 1 < n) next_scores();  // the products that read this place's weights were issued before
-                if (ok && !mbar_wait(w_full + turn.s * 8, turn.parity)) ok = false;
-                if (ok && !mbar_wait(v_full + at.s * 8, at.parity)) ok = false;
+            for (int tile = 0; tile < TILES; tile++) {
+                if (ok && !mbar_wait(w_full + (2 * tile + turn) * 8, parity)) ok = false;
                 after_sync();
                 if (elect_one() && ok) {
-                    sums(turn.s, at.s, t_sum, i > 0);
-                    umma_commit(v_free + at.s * 8);
-                    umma_commit(o_done + turn.s * 8);
+                    const unsigned long long v = dv + at.s * (v_stage >> 4);
+#pragma unroll
+                    for (int e = 0; e < kKeys / 16; e++) umma_weights(t_sum + tile * 128, tmem + (2 * tile + turn) * kKeys + e * 8, v + e * 128, by_values, i > 0 || e > 0);
+                    if (tile == TILES - 1) umma_commit(v_free + at.s * 8);
+                    umma_commit(o_done + (2 * tile + turn) * 8);
                 }
                 __syncwarp();
-                at.next(kStages);
-                turn.next(2);
             }
+            at.next(kStages);
+            parity ^= turn;
+            turn ^= 1;
         }
     } else {
         const int tile = warp / 4, r = tid, tok = r / rep, head = g * rep + r % rep;
         const bool live = tok < n_tok;
         const int pos = live ? pos0 + tok : last, low = first_key(p, pos), last_low = first_key(p, last);  // rows without a token compute something harmless
-        const long long token = sq.start + first + tok;
-        const float mul = live ? p.q_mul[token * p.heads + head] : 0.f, cap2 = p.cap2;
-        const unsigned lanes = (unsigned)((warp & 3) * 32) << 16, sum = t_sum + lanes + (TILES == 2 ? tile * 128 : 0);
+        const float mul = live ? p.q_mul[(long long)(sq.start + first + tok) * p.heads + head] : 0.f, cap2 = p.cap2;
+        const unsigned lanes = (unsigned)((warp & 3) * 32) << 16, sum = t_sum + lanes + tile * 128;
         float m = kNone, l = 0.f, sums[4];
+        const float factor = value_factor(p, g);
         RingAt at;
-        if (TILES == 2) at.s = tile;
         for (int i = 0; i < n; i++) {
-            const int j0 = (kt0 + i) * KEYS;
-            if (ok && !mbar_wait(s_full + at.s * 8, at.parity)) ok = false;
+            const int j0 = (kt0 + i) * kKeys;
+            if (ok && !mbar_wait(s_full + (2 * tile + at.s) * 8, at.parity)) ok = false;
             after_sync();
-            const unsigned place = tmem + lanes + at.s * KEYS;
-            const bool edge = j0 + KEYS - 1 > pos0 || j0 < last_low;
+            const unsigned place = tmem + lanes + (2 * tile + at.s) * kKeys;
+            const bool edge = j0 + kKeys - 1 > pos0 || j0 < last_low;
             // In base 2. Factors are positive (a negative one is in the queries): the largest score is that of the largest product.
             auto score = [&](float d) {
                 const float x = d * mul;
@@ -259,9 +218,9 @@ template <int KEYS, int TILES, bool CAPPED> __global__ void __launch_bounds__(TI
                 unsigned v[2][32];
                 tmem_ld32(v[0], place);
 #pragma unroll
-                for (int c = 0; c < KEYS / 32; c++) {
+                for (int c = 0; c < kKeys / 32; c++) {
                     tmem_ld_wait();
-                    if (c + 1 < KEYS / 32) tmem_ld32(v[(c + 1) & 1], place + (c + 1) * 32);
+                    if (c + 1 < kKeys / 32) tmem_ld32(v[(c + 1) & 1], place + (c + 1) * 32);
                     take(c * 32, v[c & 1]);
                 }
             };
@@ -285,8 +244,7 @@ template <int KEYS, int TILES, bool CAPPED> __global__ void __launch_bounds__(TI
                 m = now;
                 l *= keep;
                 if (i > 0) {
-                    // the sums of the tile before: with two tiles these scores were made behind them
-                    if (TILES == 1 && ok && !mbar_wait(o_done + ((i - 1) & 1) * 8, (unsigned)((i - 1) >> 1) & 1)) ok = false;
+                    if (ok && !mbar_wait(o_done + (2 * tile + ((i - 1) & 1)) * 8, (unsigned)((i - 1) >> 1) & 1)) ok = false;
                     after_sync();
 #pragma unroll 1
                     for (int c = 0; c < vp * 64; c += 16) {
@@ -322,38 +280,40 @@ template <int KEYS, int TILES, bool CAPPED> __global__ void __launch_bounds__(TI
             tmem_st_wait();
             before_sync();
             __syncwarp();
-            if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(w_full + at.s * 8) : "memory");
-            if (TILES == 2) at.parity ^= 1;
-            else at.next(2);
+            if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(w_full + (2 * tile + at.s) * 8) : "memory");
+            at.next(2);
         }
-        if (TILES == 2) {
-            if (ok && !mbar_wait(o_done + tile * 8, (unsigned)(n - 1) & 1)) ok = false;
-        } else {
-            if (ok && !mbar_wait(o_done + ((n - 1) & 1) * 8, (unsigned)((n - 1) >> 1) & 1)) ok = false;
-        }
+        if (ok && !mbar_wait(o_done + (2 * tile + ((n - 1) & 1)) * 8, (unsigned)((n - 1) >> 1) & 1)) ok = false;
         after_sync();
-        float f = value_factor(p, g) / l;
+        float f = factor / l;
         if (p.sink) {
-            const float top = fmaxf(m, 0.f), keep = exp2f(m - top);
-            f = value_factor(p, g) * keep / (l * keep + exp2f(-top));
+            const float top = fmaxf(m, 0.f), keep = exp2_fast(m - top);
+            f = factor * keep / (l * keep + exp2_fast(-top));
         }
-        bf16* out = (bf16*)p.out + (token * p.heads + head) * p.vdim;
+        // 64 dimensions of 32 rows at a time by way of shared memory, where the queries were, so that eight lanes write a row's 128 bytes
+        unsigned char* mine = smem + tile * kp * kPanelQ + (warp & 3) * 32 * 128;
 #pragma unroll 1
-        for (int c = 0; c < vp * 64; c += 32) {
-            unsigned v[32];
-            tmem_ld32(v, sum + c);
+        for (int c = 0; c < vp * 64; c += 64) {
+            unsigned v[2][32];
+            tmem_ld32(v[0], sum + c);
+            tmem_ld32(v[1], sum + c + 32);
             tmem_ld_wait();
-            if (live && ok) {
 #pragma unroll
-                for (int e = 0; e < 32; e += 8)
-                    if (c + e < p.vdim) {
-                        uint4 q;
-                        q.x = pack_bf16(__uint_as_float(v[e]) * f, __uint_as_float(v[e + 1]) * f);
-                        q.y = pack_bf16(__uint_as_float(v[e + 2]) * f, __uint_as_float(v[e + 3]) * f);
-                        q.z = pack_bf16(__uint_as_float(v[e + 4]) * f, __uint_as_float(v[e + 5]) * f);
-                        q.w = pack_bf16(__uint_as_float(v[e + 6]) * f, __uint_as_float(v[e + 7]) * f);
-                        *reinterpret_cast<uint4*>(out + c + e) = q;
-                    }
+            for (int e = 0; e < 8; e++) {
+                const unsigned* x = v[e / 4] + e % 4 * 8;
+                uint4 q;
+                q.x = pack_bf16(__uint_as_float(x[0]) * f, __uint_as_float(x[1]) * f);
+                q.y = pack_bf16(__uint_as_float(x[2]) * f, __uint_as_float(x[3]) * f);
+                q.z = pack_bf16(__uint_as_float(x[4]) * f, __uint_as_float(x[5]) * f);
+                q.w = pack_bf16(__uint_as_float(x[6]) * f, __uint_as_float(x[7]) * f);
+                *reinterpret_cast<uint4*>(mine + lane * 128 + ((e ^ (lane & 7)) << 4)) = q;
+            }
+            __syncwarp();
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const int row = e * 4 + lane / 8, at = lane % 8, R = tid - lane + row, t = R / rep, h = g * rep + R % rep;
+                if (t < n_tok && ok && c + at * 8 < p.vdim)
+                    *reinterpret_cast<uint4*>((bf16*)p.out + ((long long)(sq.start + first + t) * p.heads + h) * p.vdim + c + at * 8) = *reinterpret_cast<const uint4*>(mine + row * 128 + ((at ^ (row & 7)) << 4));
             }
             __syncwarp();
         }
@@ -365,8 +325,8 @@ template <int KEYS, int TILES, bool CAPPED> __global__ void __launch_bounds__(TI
 }
 
 // With 512 columns of tensor memory a CTA has its SM alone.
-int smem_of(int dim, int vdim, int keys, int tiles) {
-    const int kp = (dim + 63) / 64, vp = (vdim + 63) / 64, bytes = 1024 + tiles * kp * (int)kPanelQ + kStages * (kp + vp) * keys * 128 + 128;
+int smem_of(int dim, int vdim, int tiles) {
+    const int kp = (dim + 63) / 64, vp = (vdim + 63) / 64, bytes = 1024 + tiles * kp * (int)kPanelQ + kStages * (kp + vp) * (int)kPanel + 256;
     return tiles == 2 || vp > 2 ? std::max(bytes, 120 * 1024) : bytes;
 }
 
@@ -374,8 +334,8 @@ int smem_of(int dim, int vdim, int keys, int tiles) {
 
 PackedPrefill packed_prefill_of(int64_t dim, int64_t vdim, int64_t rows, int64_t kv_heads, int64_t rep, bool capped) {
     const bool two = dim <= 128 && vdim <= 128 && (rows * rep + 2 * kRows - 1) / (2 * kRows) * kv_heads >= 2 * sm_count();
-    if (two) return {capped ? packed_prefill<128, 2, true> : packed_prefill<128, 2, false>, smem_of((int)dim, (int)vdim, 128, 2), 2 * kRows, 2 * kRows + kUnpack + 32};
-    return {capped ? packed_prefill<64, 1, true> : packed_prefill<64, 1, false>, smem_of((int)dim, (int)vdim, 64, 1), kRows, kRows + kUnpack + 32};
+    if (two) return {capped ? packed_prefill<2, true> : packed_prefill<2, false>, smem_of((int)dim, (int)vdim, 2), 2 * kRows, 2 * kRows + kUnpack + 32};
+    return {capped ? packed_prefill<1, true> : packed_prefill<1, false>, smem_of((int)dim, (int)vdim, 1), kRows, kRows + kUnpack + 32};
 }
 
 }  // namespace oxk

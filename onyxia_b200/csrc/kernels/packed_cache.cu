@@ -417,6 +417,8 @@ void emit_packed_attention(Emitter& em, const PackedDesc& d, const TRef& proj, c
     p.by_rep = by_of(d.heads ? d.heads / d.kv_heads : 1);
     p.by_units = by_of(d.dim / 8 - d.rot_dims / 16);
     p.by_runs = by_of(d.vdim / 8);
+    p.by_key = by_of(d.dim / kPack);
+    p.by_value = by_of(d.vdim / kPack);
     const bool bf = proj.dtype == DT_BF16, tc = out && bf && d.dim <= 256 && d.vdim <= 256 && n_seqs <= 65535;
     p.only = tc && rows == n_seqs;
     const bool prefill = tc && !p.only && d.heads / d.kv_heads <= 128 && out->buf.off % 16 == 0;
@@ -445,6 +447,7 @@ void emit_packed_attention(Emitter& em, const PackedDesc& d, const TRef& proj, c
             const int64_t rep = d.heads / d.kv_heads;
             const PackedPrefill pf = packed_prefill_of(d.dim, d.vdim, rows, d.kv_heads, rep, d.softcap > 0);
             const int64_t tq = pf.rows / rep;
+            p.raw_slots = pf.slots;
             ensure_max_dynamic_smem((const void*)pf.kernel, pf.smem);
             launch(pf.kernel, dim3((unsigned)(((rows + tq - 1) / tq + n_seqs) * d.kv_heads)), (unsigned)pf.threads, (unsigned)pf.smem, none, "packed_prefill");
         } else {

@@ -34,6 +34,8 @@ struct PackP {
     int norm, sink, append;
     int singles;                 // sequences with one new token are for these kernels too
     unsigned by_rep, by_units, by_runs;  // for over(): heads of a key head, units of eight pairs or dimensions of a query or key, runs of eight dimensions of a value
+    unsigned by_key, by_value;   // the same: scales of a key, of a value
+    int raw_slots;               // prompts: copies of 64 keys or values under way
     int only;                    // no rows for prompts: as many rows as sequences, none of which may have more than one new token
 };
 
@@ -200,7 +202,7 @@ PackedDecode packed_decode_of(int64_t dim, int64_t vdim);
 // Prompts in bf16 (packed_prefill.cu), keys and values of 256 dimensions at most, 128 query heads of a key head at most.
 struct PackedPrefill {
     PackKernel kernel;
-    int smem, rows, threads;  // bytes; (token, head) rows of a CTA
+    int smem, rows, threads, slots;  // bytes; (token, head) rows of a CTA; copies of 64 keys or values under way
 };
 PackedPrefill packed_prefill_of(int64_t dim, int64_t vdim, int64_t rows, int64_t kv_heads, int64_t rep, bool capped);
 

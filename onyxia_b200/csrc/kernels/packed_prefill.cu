@@ -1,7 +1,7 @@
 // Prompts over keys and values in 4 bits on tcgen05: scores and sums of values in tensor memory.
 //
-// A CTA owns one or two tiles of 128 (token, head) rows of one key head and walks over their keys. Four warps turn codes into f16 in shared memory (exactly: packed_cache.cuh), a stage ahead of the
-// products; one warp issues these; a thread per row masks and weighs scores, 64 keys at a time. The next 64 keys' scores are made meanwhile: a tile has two turns of them. Two tiles share what is
+// A CTA owns one or two tiles of 128 (token, head) rows of one key head and walks over their keys, 64 at a time. One warp copies what the pages hold of them, several steps ahead; four warps turn
+// codes into f16 (exactly: packed_cache.cuh), a step ahead of the products; one warp issues these; a thread per row masks and weighs scores. The next 64 keys' scores are made meanwhile: a tile has two turns of them. Two tiles share what is
 // unpacked.
 #include "packed_cache.cuh"
 
@@ -9,18 +9,11 @@ namespace oxk {
 
 namespace {
 
-constexpr int kRows = 128, kUnpack = 128, kStages = 2, kKeys = 64;
+constexpr int kRows = 128, kUnpack = 128, kStages = 2, kKeys = 64, kSlots = 8;
 constexpr unsigned kPanelQ = kRows * 128, kPanel = kKeys * 128;  // bytes: rows, or keys, × 64 dimensions
 constexpr float kNone = -1e30f;            // below every score, and finite: differences stay numbers
 
 __device__ __forceinline__ unsigned bits(__half2 v) { return *reinterpret_cast<unsigned*>(&v); }
-
-// Bytes of codes per key and thread: 64 at most, in pieces of 8
-constexpr int kPieces = 8;
-struct Held {
-    uint2 codes[kPieces];
-    unsigned char scales[kPieces];
-};
 
 __device__ __forceinline__ float exp2_fast(float x) {
     float y;
@@ -28,18 +21,18 @@ __device__ __forceinline__ float exp2_fast(float x) {
     return y;
 }
 
-template <int TILES, bool CAPPED> __global__ void __launch_bounds__(TILES * kRows + kUnpack + 32, TILES == 1 ? 2 : 1) packed_prefill(const PackP p) {
+template <int TILES, bool CAPPED> __global__ void __launch_bounds__(TILES * kRows + kUnpack + 64, TILES == 1 ? 2 : 1) packed_prefill(const PackP p) {
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-    constexpr int kSoft = TILES * kRows, kThreads = kSoft + kUnpack + 32, kSoftWarps = kSoft / 32, kIssues = kSoftWarps + kUnpack / 32;
+    constexpr int kSoft = TILES * kRows, kThreads = kSoft + kUnpack + 64, kSoftWarps = kSoft / 32, kIssues = kSoftWarps + kUnpack / 32, kCopies = kIssues + 1;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, kp = (p.dim + 63) / 64, vp = (p.vdim + 63) / 64;
     const unsigned k_stage = kp * kPanel, v_stage = vp * kPanel;
-    const unsigned sq0 = smem_u32(smem), sk = sq0 + TILES * kp * kPanelQ, sv = sk + kStages * k_stage, bars = sv + kStages * v_stage;
-    // barriers: keys there, free, values there, free (one per stage), scores there, weights there, sums (two per tile, by turns)
-    const unsigned k_full = bars, k_free = k_full + kStages * 8, v_full = k_free + kStages * 8, v_free = v_full + kStages * 8, s_full = v_free + kStages * 8, w_full = s_full + 32, o_done = w_full + 32;
-    unsigned* tmem_slot = reinterpret_cast<unsigned*>(smem + (o_done + 32 - sq0));
+    const unsigned sq0 = smem_u32(smem), sk = sq0 + TILES * kp * kPanelQ, sv = sk + kStages * k_stage, raw = sv + kStages * v_stage, slot = kKeys * max(p.dim, p.vdim) / kPack * 9, bars = raw + p.raw_slots * slot;
+    // barriers: keys there, free, values there, free (one per stage), scores there, weights there, sums (two per tile, by turns), copies there, free (one per slot, keys and values by turns)
+    const unsigned k_full = bars, k_free = k_full + kStages * 8, v_full = k_free + kStages * 8, v_free = v_full + kStages * 8, s_full = v_free + kStages * 8, w_full = s_full + 32, o_done = w_full + 32, raw_full = o_done + 32, raw_free = raw_full + kSlots * 8;
+    unsigned* tmem_slot = reinterpret_cast<unsigned*>(smem + (raw_free + kSlots * 8 - sq0));
     if (tid == 0) {
-        for (unsigned b = bars; b < o_done + 32; b += 8) mbar_init(b, (b >= k_full && b < k_free) || (b >= v_full && b < v_free) ? kUnpack / 32 : b >= w_full && b < o_done ? kRows / 32 : 1);
+        for (unsigned b = bars; b < raw_free + kSlots * 8; b += 8) mbar_init(b, (b >= k_full && b < k_free) || (b >= v_full && b < v_free) || b >= raw_free ? kUnpack / 32 : b >= w_full && b < o_done ? kRows / 32 : 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     pdl_wait();
@@ -54,12 +47,15 @@ template <int TILES, bool CAPPED> __global__ void __launch_bounds__(TILES * kRow
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(cols) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    const __half* queries = (const __half*)p.q;
-    for (int i = tid; i < kSoft * kp * 8; i += kThreads) {
-        const int r = i / (kp * 8), c = i % (kp * 8), tok = r / rep, h = g * rep + r % rep;
-        const bool live = tok < n_tok && c * 8 < p.dim;
-        cp_async16(sq0 + (r / kRows * kp + (c >> 3)) * kPanelQ + r % kRows * 128 + (((c & 7) ^ (r & 7)) << 4),
-                   live ? queries + ((long long)(sq.start + first + tok) * p.heads + h) * p.dim + c * 8 : queries, live);
+    // eight lanes a row's 128 bytes
+    for (int r = warp * 4 + lane / 8; r < kSoft; r += kThreads / 8) {
+        const int tok = over(r, p.by_rep), h = g * rep + r - tok * rep;
+        const __half* row = (const __half*)p.q + ((long long)(sq.start + first + tok) * p.heads + h) * p.dim;
+        for (int c = 0; c < kp; c++) {
+            const int at = c * 64 + lane % 8 * 8;
+            const bool live = tok < n_tok && at < p.dim;
+            cp_async16(sq0 + (r / kRows * kp + c) * kPanelQ + r % kRows * 128 + ((lane % 8 ^ (r & 7)) << 4), live ? row + at : (const __half*)p.q, live);
+        }
     }
     cp_async_commit();
     // dimensions that are padding are 0 in every stage
@@ -83,67 +79,80 @@ template <int TILES, bool CAPPED> __global__ void __launch_bounds__(TILES * kRow
     bool ok = true;
 
     if (warp >= kSoftWarps && warp < kIssues) {
-        // A thread has a key, or half of one.
-        constexpr int kShare = kUnpack / kKeys;
-        const int u = tid - kSoft, key = u % kKeys, part = u / kKeys;
-        // the page of this thread's key of step i; none where the key is not there: pages in front of the window may be anybody's
-        auto page = [&](int i) {
-            const int j = (kt0 + i) * kKeys + key;
-            return i < n && j >= lowest && j <= last ? page_of(p, seq, j) : -1ll;
-        };
-        auto load = [&](int i, long long pg, Held& t, unsigned char* pool, int dim) {
-            const int j = (kt0 + i) * kKeys + key, blocks = dim / kPack;
-            const bool live = pg >= 0;
-            unsigned char* from = live ? held(p, pool, pg, g, dim) : pool;
-            const uint2* codes = reinterpret_cast<const uint2*>(codes_of(p, from, j, dim));
-            const unsigned char* scales = scales_of(p, from, j, dim);
+        // A thread has sixteen dimensions of a key at a time.
+        const int u0 = tid - kSoft;
+        auto put = [&](unsigned from, unsigned base, int i, int dim, unsigned by) {
+            const int j0 = (kt0 + i) * kKeys, blocks = dim / kPack, whole = j0 >= lowest && j0 + kKeys - 1 <= last;
+            const unsigned scales = from + kKeys * (dim / 2);
+#pragma unroll 4
+            for (int u = u0; u < kKeys * blocks; u += kUnpack) {
+                const int key = over(u, by), b = u - key * blocks;
+                unsigned x, y, code;
+                asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(x), "=r"(y) : "r"(from + u * 8));
+                asm volatile("ld.shared.u8 %0, [%1];" : "=r"(code) : "r"(scales + u));
+                // keys that are not there are 0: what was copied in their place, or not, may be no number
+                if (!whole && (j0 + key < lowest || j0 + key > last)) code = 0;
+                const __half2 s = __low2half2(scales_f16(code));
+                // (the first 64 dimensions' lanes begin with the even eighths, the next with the odd ones: eight lanes write 128 bytes in different banks)
+                const unsigned flip = b >> 2 & 1, to = base + (b >> 2) * kPanel + key * 128;
 #pragma unroll
-            for (int b = 0; b < kPieces; b++) {
-                const int at = b * kShare + part;
-                const bool in = live && at < blocks;
-                t.codes[b] = in ? codes[at] : make_uint2(0, 0);
-                t.scales[b] = in ? scales[at] : 0;
-            }
-        };
-        auto put = [&](const Held& t, unsigned base, int dim) {
-#pragma unroll
-            for (int b = 0; b < kPieces; b++) {
-                const int at = b * kShare + part;
-                if (at * kPack >= dim) break;
-                const __half2 s = __low2half2(scales_f16(t.scales[b]));
-#pragma unroll
-                for (int w = 0; w < 2; w++) {
+                for (unsigned w = 0; w < 2; w++) {
+                    const unsigned odd = w ^ flip, c = (b & 3) * 2 + odd;
                     __half2 v[4];
-                    units8(w ? t.codes[b].y : t.codes[b].x, v);
-                    const int c = at * 2 + w;
-                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(base + (c >> 3) * kPanel + key * 128 + (((c & 7) ^ (key & 7)) << 4)), "r"(bits(__hmul2(v[0], s))),
-                                 "r"(bits(__hmul2(v[1], s))), "r"(bits(__hmul2(v[2], s))), "r"(bits(__hmul2(v[3], s)))
+                    units8(odd ? y : x, v);
+                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to + ((c ^ (key & 7)) << 4)), "r"(bits(__hmul2(v[0], s))), "r"(bits(__hmul2(v[1], s))),
+                                 "r"(bits(__hmul2(v[2], s))), "r"(bits(__hmul2(v[3], s)))
                                  : "memory");
                 }
             }
         };
-        auto tell = [&](unsigned bar) {
+        auto tell = [&](unsigned there, unsigned free) {
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
-            if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+            if (lane == 0) {
+                asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(there) : "memory");
+                asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(free) : "memory");
+            }
         };
-        Held k, v;
-        long long pg = page(0);
-        load(0, pg, k, p.keys, p.dim);
-        load(0, pg, v, p.values, p.vdim);
-        pg = page(1);
-        RingAt at;
+        RingAt at, in;
         for (int i = 0; i < n; i++) {
+            if (ok && !mbar_wait(raw_full + in.s * 8, in.parity)) ok = false;
             if (i >= kStages && ok && !mbar_wait(k_free + at.s * 8, at.parity ^ 1)) ok = false;
-            put(k, sk + at.s * k_stage, p.dim);
-            tell(k_full + at.s * 8);
-            load(i + 1, pg, k, p.keys, p.dim);
+            put(raw + in.s * slot, sk + at.s * k_stage, i, p.dim, p.by_key);
+            tell(k_full + at.s * 8, raw_free + in.s * 8);
+            in.next(p.raw_slots);
+            if (ok && !mbar_wait(raw_full + in.s * 8, in.parity)) ok = false;
             if (i >= kStages && ok && !mbar_wait(v_free + at.s * 8, at.parity ^ 1)) ok = false;
-            put(v, sv + at.s * v_stage, p.vdim);
-            tell(v_full + at.s * 8);
-            load(i + 1, pg, v, p.values, p.vdim);
-            pg = page(i + 2);
+            put(raw + in.s * slot, sv + at.s * v_stage, i, p.vdim, p.by_value);
+            tell(v_full + at.s * 8, raw_free + in.s * 8);
+            in.next(p.raw_slots);
             at.next(kStages);
+        }
+    } else if (warp == kCopies) {
+        // What a page holds of 64 keys are two runs of bytes, of smaller pages' two each; pages in front of the window may be anybody's, and behind the last key there may be none.
+        const int run = min(kKeys, 1 << p.shift);
+        RingAt in;
+        for (int i = 0; i < 2 * n; i++) {
+            const int j0 = (kt0 + i / 2) * kKeys, d = i & 1 ? p.vdim : p.dim, a = max(j0, lowest) & ~(run - 1), b = min(last + 1, j0 + kKeys);
+            unsigned char* pool = i & 1 ? p.values : p.keys;
+            if (i >= p.raw_slots && ok && !mbar_wait(raw_free + in.s * 8, in.parity ^ 1)) ok = false;
+            const unsigned bar = raw_full + in.s * 8, to = raw + in.s * slot;
+            if (elect_one() && ok) {
+                const int runs = (b - a + run - 1) >> (p.shift < 6 ? p.shift : 6);
+                mbar_expect_tx(bar, runs * run * (d / kPack) * 9);
+                for (int j = a; j < b; j += run) {
+                    const unsigned char* from = held(p, pool, page_of(p, seq, j), g, d);
+                    const int off = j & ((1 << p.shift) - 1);
+                    auto copy = [&](unsigned dst, const unsigned char* src, int bytes) {
+                        asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+                    };
+                    copy(to + (j - j0) * (d / 2), from + off * (d / 2), run * (d / 2));
+                    copy(to + kKeys * (d / 2) + (j - j0) * (d / kPack), from + (((d / 2) << p.shift) + off * (d / kPack)), run * (d / kPack));
+                }
+            }
+            __syncwarp();
+            ok = __all_sync(0xffffffffu, ok);
+            in.next(p.raw_slots);
         }
     } else if (warp == kIssues) {
         const unsigned base = (1u << 4) | (8u << 24);  // f16 × f16 → f32, M 128
@@ -193,7 +202,7 @@ template <int TILES, bool CAPPED> __global__ void __launch_bounds__(TILES * kRow
             turn ^= 1;
         }
     } else {
-        const int tile = warp / 4, r = tid, tok = r / rep, head = g * rep + r % rep;
+        const int tile = warp / 4, tok = over(tid, p.by_rep), head = g * rep + tid - tok * rep;
         const bool live = tok < n_tok;
         const int pos = live ? pos0 + tok : last, low = first_key(p, pos), last_low = first_key(p, last);  // rows without a token compute something harmless
         const float mul = live ? p.q_mul[(long long)(sq.start + first + tok) * p.heads + head] : 0.f, cap2 = p.cap2;
@@ -311,7 +320,7 @@ template <int TILES, bool CAPPED> __global__ void __launch_bounds__(TILES * kRow
             __syncwarp();
 #pragma unroll
             for (int e = 0; e < 8; e++) {
-                const int row = e * 4 + lane / 8, at = lane % 8, R = tid - lane + row, t = R / rep, h = g * rep + R % rep;
+                const int row = e * 4 + lane / 8, at = lane % 8, R = tid - lane + row, t = over(R, p.by_rep), h = g * rep + R - t * rep;
                 if (t < n_tok && ok && c + at * 8 < p.vdim)
                     *reinterpret_cast<uint4*>((bf16*)p.out + ((long long)(sq.start + first + t) * p.heads + h) * p.vdim + c + at * 8) = *reinterpret_cast<const uint4*>(mine + row * 128 + ((at ^ (row & 7)) << 4));
             }
@@ -324,18 +333,22 @@ template <int TILES, bool CAPPED> __global__ void __launch_bounds__(TILES * kRow
     if (warp == kIssues) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(cols) : "memory");
 }
 
-// With 512 columns of tensor memory a CTA has its SM alone.
+// Bytes without the slots of copies
 int smem_of(int dim, int vdim, int tiles) {
-    const int kp = (dim + 63) / 64, vp = (vdim + 63) / 64, bytes = 1024 + tiles * kp * (int)kPanelQ + kStages * (kp + vp) * (int)kPanel + 256;
-    return tiles == 2 || vp > 2 ? std::max(bytes, 120 * 1024) : bytes;
+    const int kp = (dim + 63) / 64, vp = (vdim + 63) / 64;
+    return 1024 + tiles * kp * (int)kPanelQ + kStages * (kp + vp) * (int)kPanel + (4 * kStages + 12 + 2 * kSlots) * 8 + 16;
 }
 
 }  // namespace
 
 PackedPrefill packed_prefill_of(int64_t dim, int64_t vdim, int64_t rows, int64_t kv_heads, int64_t rep, bool capped) {
-    const bool two = dim <= 128 && vdim <= 128 && (rows * rep + 2 * kRows - 1) / (2 * kRows) * kv_heads >= 2 * sm_count();
-    if (two) return {capped ? packed_prefill<2, true> : packed_prefill<2, false>, smem_of((int)dim, (int)vdim, 2), 2 * kRows, 2 * kRows + kUnpack + 32};
-    return {capped ? packed_prefill<1, true> : packed_prefill<1, false>, smem_of((int)dim, (int)vdim, 1), kRows, kRows + kUnpack + 32};
+    const int tiles = dim <= 128 && vdim <= 128 && (rows * rep + 2 * kRows - 1) / (2 * kRows) * kv_heads >= 2 * sm_count() ? 2 : 1;
+    const PackKernel k = tiles == 2 ? (capped ? packed_prefill<2, true> : packed_prefill<2, false>) : capped ? packed_prefill<1, true> : packed_prefill<1, false>;
+    // With 512 columns of tensor memory a CTA has its SM alone, with 256 it shares it with one other.
+    const bool alone = tiles == 2 || vdim > 128;
+    const int fixed = smem_of((int)dim, (int)vdim, tiles), slot = kKeys * (int)std::max(dim, vdim) / kPack * 9, room = (alone || fixed + 2 * slot > 112 * 1024 ? 226 : 112) * 1024;
+    const int slots = std::min(kSlots, (room - fixed) / slot), smem = fixed + slots * slot;
+    return {k, alone ? std::max(smem, 120 * 1024) : smem, tiles * kRows, tiles * kRows + kUnpack + 64, slots};
 }
 
 }  // namespace oxk

@@ -4,6 +4,7 @@
 // (`mma.sync`, f16). The order of a contraction is free, so a lane holds for S the whole blocks of 16 dimensions of two keys, whose codes become f16 and are multiplied by their scale (exactly), and
 // for O^T the same run of dimensions of four keys: pairs of keys come together by swapping halves of bytes.
 #include <cmath>
+#include <type_traits>
 
 #include "packed_cache.cuh"
 
@@ -82,7 +83,7 @@ template <int KS, int VC, bool WHOLE, int RESIDENT> __global__ void __launch_bou
     // Tiles lie in one page, or their halves in one each; what lies beyond the keys of this CTA may be on no page.
     const bool whole_tiles = (1 << p.shift) >= kTile;
     auto copy = [&](int i, unsigned s) {
-        if (i >= tiles || lane != 0) return;
+        if (i >= tiles || !elect_one()) return;
         const int j0 = first + i * step;
         const unsigned to = ring + s * kWarps * L::stage, bar = full + s * 8;
         // keys from j on, which stand `at` keys behind the tile's first
@@ -160,9 +161,9 @@ template <int KS, int VC, bool WHOLE, int RESIDENT> __global__ void __launch_bou
         float top = 0.f;
         for (int i = lane; i < dim; i += 32) top = fmaxf(top, fabsf(value(i)));
         const int e = query_exponent(warp_max(top));
-        const float down = power_down(e);
-        for (int i = lane; i < L::dk; i += 32) to[i] = __float2half_rn(live && i < dim ? value(i) * down : 0.f);
-        if (lane == 0) factor_s[r] = p.mul2 * power_up(e) * key_factor(p, g);
+        const float down = copysignf(power_down(e), p.mul2);
+        for (int i = lane; i < L::dk; i += 32) to[i] = __float2half_rn(live && p.mul2 != 0.f && i < dim ? value(i) * down : 0.f);
+        if (lane == 0) factor_s[r] = (p.mul2 != 0.f ? fabsf(p.mul2) : 1.f) * power_up(e) * key_factor(p, g);
     }
     __syncthreads();
     unsigned q[KS][8];
@@ -179,125 +180,92 @@ template <int KS, int VC, bool WHOLE, int RESIDENT> __global__ void __launch_bou
     asm volatile("fence.proxy.async;" ::: "memory");  // copies read the new key, and take the queries' place
     __syncthreads();
     fill(late ? 0 : kStages - 1, kStages);
-    const float mul[2] = {factor_s[2 * t4], factor_s[2 * t4 + 1]};
-
     // a lane holds scores of keys g8, g8 + 8 and heads 2 · t4, 2 · t4 + 1, and results of dimensions 2 · VC · g8 + 2i, + 1 of these heads
-    float o[VC][4], top[2] = {kNone, kNone}, most[2] = {kNone, kNone}, l[2] = {0.f, 0.f};
+    const float mul[2] = {factor_s[2 * t4], factor_s[2 * t4 + 1]};
+    const bool capped = p.cap2 > 0.f;
+    const float weigh[2] = {capped ? 1.f : mul[0], capped ? 1.f : mul[1]}, back[2] = {1.f / weigh[0], 1.f / weigh[1]};
+    // `most`: what a score may be until the weights are taken against another maximum, before it is multiplied; `l`: sums of the weights, by a product with ones
+    float o[VC][4], l[4] = {0.f, 0.f, 0.f, 0.f}, top[2] = {kNone, kNone}, most[2] = {kNone, kNone};
 #pragma unroll
     for (int n = 0; n < VC; n++)
 #pragma unroll
         for (int e = 0; e < 4; e++) o[n][e] = 0.f;
-    bool ok = true;
-    RingAt at;
-#pragma unroll 1
-    for (int i = 0; i < tiles; i++, at.next(kStages)) {
-      if (ok && !mbar_wait(full + at.s * 8, at.parity)) ok = false;
-      const unsigned char* stage = smem + (at.s * kWarps + warp) * L::stage;
+    auto attend = [&](auto edge, int j0, const unsigned char* stage) {
+        float s[2][4];
 #pragma unroll
-      for (int half = 0; half < 2; half++) {
-        const int j0 = first + i * step + half * kKeys;
-        if (j0 + kKeys <= from || j0 >= hi) continue;
-        uint2 key[2][KS];
-        unsigned key_scale[2], value[4][VC / 4], value_scale[4];  // KS bytes; one byte, or two
+        for (int half = 0; half < 2; half++) {
+            uint2 key[2][KS];
+            unsigned key_scale[2];  // KS bytes
 #pragma unroll
-        for (int r = 0; r < 2; r++) {
-            const int row = half * kKeys + g8 + 8 * r;
-            const unsigned char *codes = stage + row * (dim / 2) + t4 * KS * 8, *scales = stage + key_scales + row * (dim / kPack) + t4 * KS;
-            if constexpr (WHOLE && KS == 1) {
-                key[r][0] = *reinterpret_cast<const uint2*>(codes);
-                key_scale[r] = *scales;
-            } else if constexpr (WHOLE) {
+            for (int r = 0; r < 2; r++) {
+                const int row = half * kKeys + g8 + 8 * r;
+                const unsigned char *codes = stage + row * (dim / 2) + t4 * KS * 8, *scales = stage + key_scales + row * (dim / kPack) + t4 * KS;
+                if constexpr (WHOLE && KS == 1) {
+                    key[r][0] = *reinterpret_cast<const uint2*>(codes);
+                    key_scale[r] = *scales;
+                } else if constexpr (WHOLE) {
 #pragma unroll
-                for (int c = 0; c < KS; c += 2) {
-                    const uint4 v = reinterpret_cast<const uint4*>(codes)[c / 2];
-                    key[r][c] = make_uint2(v.x, v.y);
-                    key[r][c + 1] = make_uint2(v.z, v.w);
-                }
-                key_scale[r] = KS == 2 ? *reinterpret_cast<const unsigned short*>(scales) : *reinterpret_cast<const unsigned*>(scales);
-            } else {
-                key_scale[r] = 0;
-#pragma unroll
-                for (int c = 0; c < KS; c++) {
-                    const bool in = t4 * KS + c < dim / kPack;
-                    key[r][c] = in ? reinterpret_cast<const uint2*>(codes)[c] : make_uint2(0, 0);
-                    key_scale[r] |= in ? (unsigned)scales[c] << (8 * c) : 0u;
-                }
-            }
-        }
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-            const int row = half * kKeys + 2 * t4 + (e & 1) + 8 * (e >> 1);
-            const unsigned char *codes = stage + value_codes + row * (vdim / 2) + g8 * VC, *scales = stage + value_scales + row * (vdim / kPack) + (VC == 4 ? g8 / 2 : g8 * (VC / 8));
-            if constexpr (VC < 16) {
-                const bool in = WHOLE || g8 * VC < vdim / 2;
-                if constexpr (VC == 4) {
-                    value[e][0] = in ? *reinterpret_cast<const unsigned*>(codes) : 0u;
+                    for (int c = 0; c < KS; c += 2) {
+                        const uint4 v = reinterpret_cast<const uint4*>(codes)[c / 2];
+                        key[r][c] = make_uint2(v.x, v.y);
+                        key[r][c + 1] = make_uint2(v.z, v.w);
+                    }
+                    key_scale[r] = KS == 2 ? *reinterpret_cast<const unsigned short*>(scales) : *reinterpret_cast<const unsigned*>(scales);
                 } else {
-                    const uint2 w = in ? *reinterpret_cast<const uint2*>(codes) : make_uint2(0, 0);
-                    value[e][0] = w.x;
-                    value[e][1] = w.y;
-                }
-                value_scale[e] = in ? *scales : 0u;
-            } else if constexpr (WHOLE) {
-                const uint4 w = *reinterpret_cast<const uint4*>(codes);
-                value[e][0] = w.x;
-                value[e][1] = w.y;
-                value[e][2] = w.z;
-                value[e][3] = w.w;
-                value_scale[e] = *reinterpret_cast<const unsigned short*>(scales);
-            } else {
-                value_scale[e] = 0;
+                    key_scale[r] = 0;
 #pragma unroll
-                for (int c = 0; c < 2; c++) {
-                    const bool in = g8 * VC + c * 8 < vdim / 2;
-                    const uint2 w = in ? reinterpret_cast<const uint2*>(codes)[c] : make_uint2(0, 0);
-                    value[e][2 * c] = w.x;
-                    value[e][2 * c + 1] = w.y;
-                    value_scale[e] |= in ? (unsigned)scales[c] << (8 * c) : 0u;
+                    for (int c = 0; c < KS; c++) {
+                        const bool in = t4 * KS + c < dim / kPack;
+                        key[r][c] = in ? reinterpret_cast<const uint2*>(codes)[c] : make_uint2(0, 0);
+                        key_scale[r] |= in ? (unsigned)scales[c] << (8 * c) : 0u;
+                    }
                 }
             }
-        }
-        float s[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int c = 0; c < KS; c++) {
-            const __half2 both = scales_f16(__byte_perm(key_scale[0], key_scale[1], c | (4 + c) << 4)), s0 = __low2half2(both), s1 = __high2half2(both);
+            for (int e = 0; e < 4; e++) s[half][e] = 0.f;
 #pragma unroll
-            for (int w = 0; w < 2; w++) {
-                __half2 a[4], b[4];
-                units8(w ? key[0][c].y : key[0][c].x, a);
-                units8(w ? key[1][c].y : key[1][c].x, b);
+            for (int c = 0; c < KS; c++) {
+                const __half2 both = scales_f16(__byte_perm(key_scale[0], key_scale[1], c | (4 + c) << 4)), s0 = __low2half2(both), s1 = __high2half2(both);
 #pragma unroll
-                for (int e = 0; e < 4; e += 2)
-                    mma_f16(s, bits(__hmul2(a[e], s0)), bits(__hmul2(b[e], s1)), bits(__hmul2(a[e + 1], s0)), bits(__hmul2(b[e + 1], s1)), q[c][4 * w + e], q[c][4 * w + e + 1]);
+                for (int w = 0; w < 2; w++) {
+                    __half2 a[4], b[4];
+                    units8(w ? key[0][c].y : key[0][c].x, a);
+                    units8(w ? key[1][c].y : key[1][c].x, b);
+#pragma unroll
+                    for (int e = 0; e < 4; e += 2)
+                        mma_f16(s[half], bits(__hmul2(a[e], s0)), bits(__hmul2(b[e], s1)), bits(__hmul2(a[e + 1], s0)), bits(__hmul2(b[e + 1], s1)), q[c][4 * w + e], q[c][4 * w + e + 1]);
+                }
             }
         }
-        const bool edge = j0 + kKeys > hi || j0 < low;
+        bool above = false;
 #pragma unroll
-        for (int e = 0; e < 4; e++) s[e] *= mul[e & 1];
-        if (p.cap2 > 0.f)
+        for (int half = 0; half < 2; half++) {
+            if (capped)
 #pragma unroll
-            for (int e = 0; e < 4; e++) s[e] = p.cap2 - __fdividef(2.f * p.cap2, 1.f + exp2_fast(s[e]));
-        if (edge) {
+                for (int e = 0; e < 4; e++) s[half][e] = p.cap2 - __fdividef(2.f * p.cap2, 1.f + exp2_fast(s[half][e] * mul[e & 1]));
+            if constexpr (edge) {
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const int j = j0 + g8 + 8 * (e >> 1), k = j0 + 2 * t4 + (e & 1) + 8 * (e >> 1);
-                if (j >= hi || j < low) s[e] = -INFINITY;
-                // what lies behind the last key may be no number, which a weight of 0 would not cancel: its scale would be none
-                if (k >= hi || k < low) value_scale[e] = 0;
+                for (int e = 0; e < 4; e++) {
+                    const int j = j0 + half * kKeys + g8 + 8 * (e >> 1);
+                    if (j >= hi || j < low) s[half][e] = -INFINITY;
+                }
             }
+#pragma unroll
+            for (int e = 0; e < 4; e++) above |= s[half][e] > most[e & 1];
         }
-        const bool above = s[0] > most[0] || s[1] > most[1] || s[2] > most[0] || s[3] > most[1];
         // Weights are taken against a maximum that the largest score is up to 8 above: f16 holds 2^8 as exactly as 1, and 2^-22 of the largest weight with all its bits.
         if (__any_sync(0xffffffffu, above)) {
 #pragma unroll
             for (int e = 0; e < 2; e++) {
-                float now = fmaxf(top[e], fmaxf(s[e], s[e + 2]));
+                float now = fmaxf(fmaxf(s[0][e], s[0][e + 2]), fmaxf(s[1][e], s[1][e + 2]));
 #pragma unroll
                 for (int d = 4; d < 32; d <<= 1) now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, d));
+                now = now > -INFINITY ? fmaxf(top[e], now * weigh[e]) : top[e];
                 const float keep = exp2_fast(top[e] - now);
                 top[e] = now;
-                most[e] = now + 8.f;
+                most[e] = now > kNone ? (now + 8.f) * back[e] : kNone;
                 l[e] *= keep;
+                l[e + 2] *= keep;
 #pragma unroll
                 for (int n = 0; n < VC; n++) {
                     o[n][e] *= keep;
@@ -305,43 +273,90 @@ template <int KS, int VC, bool WHOLE, int RESIDENT> __global__ void __launch_bou
                 }
             }
         }
-        unsigned pb[2];
 #pragma unroll
-        for (int r = 0; r < 2; r++) {
-            const __half2 w = __floats2half2_rn(exp2_fast(s[2 * r] - top[0]), exp2_fast(s[2 * r + 1] - top[1]));
-            // the sums of the weights as they are multiplied: the rounding of a weight that stands out is in both
-            l[0] += __low2float(w);
-            l[1] += __high2float(w);
-            pb[r] = transpose8x8(bits(w));
-        }
+        for (int half = 0; half < 2; half++) {
+            unsigned pb[2];
 #pragma unroll
-        for (int b = 0; b < (VC + 7) / 8; b++) {
-            const __half2 s01 = scales_f16(__byte_perm(value_scale[0], value_scale[1], b | (4 + b) << 4)), s23 = scales_f16(__byte_perm(value_scale[2], value_scale[3], b | (4 + b) << 4));
+            for (int r = 0; r < 2; r++) {
+                const float w0 = exp2_fast(__fmaf_rn(s[half][2 * r], weigh[0], -top[0])), w1 = exp2_fast(__fmaf_rn(s[half][2 * r + 1], weigh[1], -top[1]));
+                pb[r] = transpose8x8(bits(__floats2half2_rn(w0, w1)));
+            }
+            constexpr unsigned kOnes = 0x3C003C00u;
+            mma_f16(l, kOnes, kOnes, kOnes, kOnes, pb[0], pb[1]);
+            unsigned value[4][VC / 4], value_scale[4];  // one byte, or two
 #pragma unroll
-            for (int w = 2 * b; w < 2 * b + (VC < 8 ? 1 : 2); w++) {
-                // pairs of keys in a byte: the earlier dimension of each byte, then the later one
-                constexpr unsigned kLow = 0x0F0F0F0Fu;
-                __half2 a[4], c[4], d[4], f[4];
-                units8((value[0][w] & kLow) | (value[1][w] << 4 & ~kLow), a);
-                units8((value[0][w] >> 4 & kLow) | (value[1][w] & ~kLow), c);
-                units8((value[2][w] & kLow) | (value[3][w] << 4 & ~kLow), d);
-                units8((value[2][w] >> 4 & kLow) | (value[3][w] & ~kLow), f);
+            for (int e = 0; e < 4; e++) {
+                const int row = half * kKeys + 2 * t4 + (e & 1) + 8 * (e >> 1);
+                const unsigned char *codes = stage + value_codes + row * (vdim / 2) + g8 * VC, *scales = stage + value_scales + row * (vdim / kPack) + (VC == 4 ? g8 / 2 : g8 * (VC / 8));
+                if constexpr (VC < 16) {
+                    const bool in = WHOLE || g8 * VC < vdim / 2;
+                    if constexpr (VC == 4) {
+                        value[e][0] = in ? *reinterpret_cast<const unsigned*>(codes) : 0u;
+                    } else {
+                        const uint2 w = in ? *reinterpret_cast<const uint2*>(codes) : make_uint2(0, 0);
+                        value[e][0] = w.x;
+                        value[e][1] = w.y;
+                    }
+                    value_scale[e] = in ? *scales : 0u;
+                } else if constexpr (WHOLE) {
+                    const uint4 w = *reinterpret_cast<const uint4*>(codes);
+                    value[e][0] = w.x;
+                    value[e][1] = w.y;
+                    value[e][2] = w.z;
+                    value[e][3] = w.w;
+                    value_scale[e] = *reinterpret_cast<const unsigned short*>(scales);
+                } else {
+                    value_scale[e] = 0;
 #pragma unroll
-                for (int e = 0; e < 4; e++)
-                    mma_f16(o[4 * w + e], bits(__hmul2(a[e], s01)), bits(__hmul2(c[e], s01)), bits(__hmul2(d[e], s23)), bits(__hmul2(f[e], s23)), pb[0], pb[1]);
+                    for (int c = 0; c < 2; c++) {
+                        const bool in = g8 * VC + c * 8 < vdim / 2;
+                        const uint2 w = in ? reinterpret_cast<const uint2*>(codes)[c] : make_uint2(0, 0);
+                        value[e][2 * c] = w.x;
+                        value[e][2 * c + 1] = w.y;
+                        value_scale[e] |= in ? (unsigned)scales[c] << (8 * c) : 0u;
+                    }
+                }
+                // what lies beyond the keys may be no number, which a weight of 0 would not cancel: its scale would be none
+                if constexpr (edge)
+                    if (j0 + row >= hi || j0 + row < low) value_scale[e] = 0;
+            }
+#pragma unroll
+            for (int b = 0; b < (VC + 7) / 8; b++) {
+                const __half2 s01 = scales_f16(__byte_perm(value_scale[0], value_scale[1], b | (4 + b) << 4)), s23 = scales_f16(__byte_perm(value_scale[2], value_scale[3], b | (4 + b) << 4));
+#pragma unroll
+                for (int w = 2 * b; w < 2 * b + (VC < 8 ? 1 : 2); w++) {
+                    // pairs of keys in a byte: the earlier dimension of each byte, then the later one
+                    constexpr unsigned kLow = 0x0F0F0F0Fu;
+                    __half2 a[4], c[4], d[4], f[4];
+                    units8((value[0][w] & kLow) | (value[1][w] << 4 & ~kLow), a);
+                    units8((value[0][w] >> 4 & kLow) | (value[1][w] & ~kLow), c);
+                    units8((value[2][w] & kLow) | (value[3][w] << 4 & ~kLow), d);
+                    units8((value[2][w] >> 4 & kLow) | (value[3][w] & ~kLow), f);
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        mma_f16(o[4 * w + e], bits(__hmul2(a[e], s01)), bits(__hmul2(c[e], s01)), bits(__hmul2(d[e], s23)), bits(__hmul2(f[e], s23)), pb[0], pb[1]);
+                }
             }
         }
-      }
-      __syncwarp();
-      copy(i + kStages, at.s);
+    };
+    bool ok = true;
+    RingAt at;
+#pragma unroll 1
+    for (int i = 0; i < tiles; i++, at.next(kStages)) {
+        if (ok && !mbar_wait(full + at.s * 8, at.parity)) ok = false;
+        const int j0 = first + i * step;
+        const unsigned char* stage = smem + (at.s * kWarps + warp) * L::stage;
+        if (j0 + kTile > hi || j0 < low) attend(std::true_type{}, j0, stage);
+        else attend(std::false_type{}, j0, stage);
+        __syncwarp();
+        copy(i + kStages, at.s);
+        __syncwarp();
     }
     if (!ok && lane == 0) report(p.err, ERR_WAIT_TIMEOUT, p.node, (long long)blockIdx.x, (long long)warp);
     __syncthreads();  // the rings become the place of partial results
     float* parts = reinterpret_cast<float*>(smem);
 #pragma unroll
     for (int e = 0; e < 2; e++) {
-#pragma unroll
-        for (int d = 4; d < 32; d <<= 1) l[e] += __shfl_xor_sync(0xffffffffu, l[e], d);
         float* to = parts + warp * L::part + (t4 * 2 + e) * (L::dv + 2);
         if (g8 == 0) {
             to[0] = top[e];

@@ -95,7 +95,7 @@ def test_page_sizes(page, kind):
 @BOTH
 @pytest.mark.parametrize("more", [dict(window=1), dict(window=17), dict(window=64), dict(window=100, sink=1), dict(softcap=5.0), dict(sink=1), dict(norm=1), dict(factors=1),
                                   dict(softcap=20.0, sink=1, norm=1, window=90, factors=1), dict(scale=0.25), dict(scale=-0.125),
-                                  dict(scale=-0.125, softcap=3.0)], ids=str)
+                                  dict(scale=-0.125, softcap=3.0), dict(scale=1e-30, window=70)], ids=str)
 def test_scores(more, kind):
     f = Form(4, 2, 64, 128, 64, **more)
     check(f, [(150, 0), (1, 200), (20, 130), (1, 0), (1, 64)], kind)

@@ -16,7 +16,7 @@ constexpr int kWarps = 4, kThreads = kWarps * 32, kPages = 256, kHeads = 8, kKey
 constexpr float kNone = -1e30f;  // below every score, and finite: differences stay numbers
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
@@ -191,52 +191,58 @@ template <int KS, int VC, bool WHOLE, int RESIDENT> __global__ void __launch_bou
 #pragma unroll
         for (int e = 0; e < 4; e++) o[n][e] = 0.f;
     auto attend = [&](auto edge, int j0, const unsigned char* stage) {
-        float s[2][4];
+        // (the two halves in turn, each in two sums: a product does not wait for the one before it)
+        uint2 key[2][2][KS];
+        unsigned key_scale[2][2];  // KS bytes
 #pragma unroll
-        for (int half = 0; half < 2; half++) {
-            uint2 key[2][KS];
-            unsigned key_scale[2];  // KS bytes
+        for (int half = 0; half < 2; half++)
 #pragma unroll
             for (int r = 0; r < 2; r++) {
                 const int row = half * kKeys + g8 + 8 * r;
                 const unsigned char *codes = stage + row * (dim / 2) + t4 * KS * 8, *scales = stage + key_scales + row * (dim / kPack) + t4 * KS;
                 if constexpr (WHOLE && KS == 1) {
-                    key[r][0] = *reinterpret_cast<const uint2*>(codes);
-                    key_scale[r] = *scales;
+                    key[half][r][0] = *reinterpret_cast<const uint2*>(codes);
+                    key_scale[half][r] = *scales;
                 } else if constexpr (WHOLE) {
 #pragma unroll
                     for (int c = 0; c < KS; c += 2) {
                         const uint4 v = reinterpret_cast<const uint4*>(codes)[c / 2];
-                        key[r][c] = make_uint2(v.x, v.y);
-                        key[r][c + 1] = make_uint2(v.z, v.w);
+                        key[half][r][c] = make_uint2(v.x, v.y);
+                        key[half][r][c + 1] = make_uint2(v.z, v.w);
                     }
-                    key_scale[r] = KS == 2 ? *reinterpret_cast<const unsigned short*>(scales) : *reinterpret_cast<const unsigned*>(scales);
+                    key_scale[half][r] = KS == 2 ? *reinterpret_cast<const unsigned short*>(scales) : *reinterpret_cast<const unsigned*>(scales);
                 } else {
-                    key_scale[r] = 0;
+                    key_scale[half][r] = 0;
 #pragma unroll
                     for (int c = 0; c < KS; c++) {
                         const bool in = t4 * KS + c < dim / kPack;
-                        key[r][c] = in ? reinterpret_cast<const uint2*>(codes)[c] : make_uint2(0, 0);
-                        key_scale[r] |= in ? (unsigned)scales[c] << (8 * c) : 0u;
+                        key[half][r][c] = in ? reinterpret_cast<const uint2*>(codes)[c] : make_uint2(0, 0);
+                        key_scale[half][r] |= in ? (unsigned)scales[c] << (8 * c) : 0u;
                     }
                 }
             }
+        float s[2][4], more[2][4];
 #pragma unroll
-            for (int e = 0; e < 4; e++) s[half][e] = 0.f;
+        for (int half = 0; half < 2; half++)
 #pragma unroll
-            for (int c = 0; c < KS; c++) {
-                const __half2 both = scales_f16(__byte_perm(key_scale[0], key_scale[1], c | (4 + c) << 4)), s0 = __low2half2(both), s1 = __high2half2(both);
+            for (int e = 0; e < 4; e++) s[half][e] = more[half][e] = 0.f;
 #pragma unroll
-                for (int w = 0; w < 2; w++) {
+        for (int c = 0; c < KS; c++)
+#pragma unroll
+            for (int w = 0; w < 2; w++)
+#pragma unroll
+                for (int half = 0; half < 2; half++) {
+                    const __half2 both = scales_f16(__byte_perm(key_scale[half][0], key_scale[half][1], c | (4 + c) << 4)), s0 = __low2half2(both), s1 = __high2half2(both);
                     __half2 a[4], b[4];
-                    units8(w ? key[0][c].y : key[0][c].x, a);
-                    units8(w ? key[1][c].y : key[1][c].x, b);
-#pragma unroll
-                    for (int e = 0; e < 4; e += 2)
-                        mma_f16(s[half], bits(__hmul2(a[e], s0)), bits(__hmul2(b[e], s1)), bits(__hmul2(a[e + 1], s0)), bits(__hmul2(b[e + 1], s1)), q[c][4 * w + e], q[c][4 * w + e + 1]);
+                    units8(w ? key[half][0][c].y : key[half][0][c].x, a);
+                    units8(w ? key[half][1][c].y : key[half][1][c].x, b);
+                    mma_f16(s[half], bits(__hmul2(a[0], s0)), bits(__hmul2(b[0], s1)), bits(__hmul2(a[1], s0)), bits(__hmul2(b[1], s1)), q[c][4 * w], q[c][4 * w + 1]);
+                    mma_f16(more[half], bits(__hmul2(a[2], s0)), bits(__hmul2(b[2], s1)), bits(__hmul2(a[3], s0)), bits(__hmul2(b[3], s1)), q[c][4 * w + 2], q[c][4 * w + 3]);
                 }
-            }
-        }
+#pragma unroll
+        for (int half = 0; half < 2; half++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) s[half][e] += more[half][e];
         bool above = false;
 #pragma unroll
         for (int half = 0; half < 2; half++) {

@@ -413,7 +413,6 @@ void emit_packed_attention(Emitter& em, const PackedDesc& d, const TRef& proj, c
     p.append = d.append;
     p.cap2 = (float)(d.softcap * (double)kLog2e);
     p.mul2 = (float)(d.softcap > 0 ? 2.0 * (double)kLog2e * d.scale / d.softcap : (double)kLog2e * d.scale);
-    p.splits = 1;
     p.by_rep = by_of(d.heads ? d.heads / d.kv_heads : 1);
     p.by_units = by_of(d.dim / 8 - d.rot_dims / 16);
     p.by_runs = by_of(d.vdim / 8);
@@ -459,25 +458,12 @@ void emit_packed_attention(Emitter& em, const PackedDesc& d, const TRef& proj, c
     if (tc && (p.only || n_seqs > 1)) {
         const PackedDecode dc = packed_decode_of(d.dim, d.vdim);
         const int64_t groups = d.kv_heads * ((d.heads / d.kv_heads + dc.heads - 1) / dc.heads), cells = n_seqs * groups;
-        // Splits of the most keys a sequence can see: whole waves of resident CTAs, each with a beginning and an end, and the pieces have to be merged.
-        const int64_t slots = (int64_t)dc.resident * sm_count();
-        int64_t seen = (int64_t)p.width * d.page;
-        if (d.window > 0) seen = std::min<int64_t>(seen, d.window + dc.step);
-        int64_t splits = 1;
-        const double fixed = 64.0 * 1024.0 / (d.dim + d.vdim);
-        double best = 1e300;
-        for (int64_t sp = 1; sp <= 64 && sp * dc.step <= std::max<int64_t>(seen, dc.step); sp++) {
-            const double us = (double)((cells * sp + slots - 1) / slots) * ((double)seen / sp + fixed) + 4.0 * sp;
-            if (us < best) {
-                best = us;
-                splits = sp;
-            }
-        }
-        if (cells > (int64_t)kCounterWords) splits = 1;
-        p.splits = (int)splits;
-        const Buf part = splits > 1 ? em.scratch((size_t)cells * splits * dc.part * 4) : none;
+        // As many CTAs as there is room for share the keys of all sequences evenly, but for cells without a counter each.
+        const int64_t blocks = ((int64_t)p.width * d.page + dc.step - 1) / dc.step + 1, ctas = cells > (int64_t)kCounterWords ? cells : std::min<int64_t>((int64_t)dc.resident * sm_count(), cells * blocks);
+        p.cells = cells > (int64_t)kCounterWords ? (int)cells : 0;
+        const Buf part = p.cells ? none : em.scratch((size_t)ctas * 2 * dc.part * 4);
         ensure_max_dynamic_smem((const void*)dc.kernel, dc.smem);
-        launch(dc.kernel, dim3((unsigned)splits, (unsigned)groups, (unsigned)n_seqs), 128, (unsigned)dc.smem, part, "packed_decode");
+        launch(dc.kernel, dim3((unsigned)ctas), 128, (unsigned)dc.smem, part, "packed_decode");
     }
 }
 

@@ -27,7 +27,7 @@ struct PackP {
     unsigned* counters;
     ErrWord* err;
     long long rows, ld, q_off, k_off, v_off;
-    int n_seqs, width, n_pages, shift /* log2 of the page */, heads, kv_heads, dim, vdim, half, window, splits, node;
+    int n_seqs, width, n_pages, shift /* log2 of the page */, heads, kv_heads, dim, vdim, half, window, node;
     float scale, cap;            // scores in natural units
     float mul2, cap2;            // base 2: cap2 = 0: score2 = mul2 · q·k, otherwise cap2 · tanh with mul2 = 2 log2 e · scale / cap
     double eps;
@@ -35,6 +35,7 @@ struct PackP {
     int singles;                 // sequences with one new token are for these kernels too
     unsigned by_rep, by_units, by_runs;  // for over(): heads of a key head, units of eight pairs or dimensions of a query or key, runs of eight dimensions of a value
     unsigned by_key, by_value;   // the same: scales of a key, of a value
+    int cells;                   // single tokens: a CTA per sequence and group, of which there are so many; 0: CTAs share them evenly
     int raw_slots;               // prompts: copies of 64 keys or values under way
     int only;                    // no rows for prompts: as many rows as sequences, none of which may have more than one new token
 };

@@ -418,6 +418,7 @@ void emit_packed_attention(Emitter& em, const PackedDesc& d, const TRef& proj, c
     p.by_runs = by_of(d.vdim / 8);
     p.by_key = by_of(d.dim / kPack);
     p.by_value = by_of(d.vdim / kPack);
+    p.by_eighths = by_of(d.dim / 8);
     const bool bf = proj.dtype == DT_BF16, tc = out && bf && d.dim <= 256 && d.vdim <= 256 && n_seqs <= 65535;
     p.only = tc && rows == n_seqs;
     const bool prefill = tc && !p.only && d.heads / d.kv_heads <= 128 && out->buf.off % 16 == 0;
@@ -430,11 +431,11 @@ void emit_packed_attention(Emitter& em, const PackedDesc& d, const TRef& proj, c
                    {&p.counters, Buf{kSlotCounters, 0}}, {&p.err, Buf{kSlotErr, 0}}},
                   label, /*pdl=*/true);
     };
+    p.by8 = p.ld % 8 == 0 && d.q_off % 8 == 0 && d.k_off % 8 == 0 && d.v_off % 8 == 0 && proj.buf.off % 16 == 0;
     if (!p.only) {
         // bytes that the kernel for eight at a time shares; a block may have 48 KB
         const int64_t eight = d.rot_dims * 12 + d.kv_heads * 8 + d.heads * 8;
-        const bool by8 = p.ld % 8 == 0 && d.q_off % 8 == 0 && d.k_off % 8 == 0 && d.v_off % 8 == 0 && proj.buf.off % 16 == 0;
-        if (bf && by8 && d.rot_dims % 32 == 0 && eight <= 48 * 1024) {
+        if (bf && p.by8 && d.rot_dims % 32 == 0 && eight <= 48 * 1024) {
             launch(packed_write8, dim3((unsigned)rows), 128, (unsigned)eight, none, "packed_write");
         } else {
             const PackKernel write = bf ? packed_write<bf16> : packed_write<float>;

@@ -34,7 +34,8 @@ struct PackP {
     int norm, sink, append;
     int singles;                 // sequences with one new token are for these kernels too
     unsigned by_rep, by_units, by_runs;  // for over(): heads of a key head, units of eight pairs or dimensions of a query or key, runs of eight dimensions of a value
-    unsigned by_key, by_value;   // the same: scales of a key, of a value
+    unsigned by_key, by_value, by_eighths;  // the same: scales of a key, of a value, runs of eight dimensions of a key
+    int by8;                     // the parts of a projection row begin on 16 bytes
     int cells;                   // single tokens: a CTA per sequence and group, of which there are so many; 0: CTAs share them evenly
     int raw_slots;               // prompts: copies of 64 keys or values under way
     int only;                    // no rows for prompts: as many rows as sequences, none of which may have more than one new token
@@ -157,6 +158,17 @@ template <class P> __device__ __forceinline__ void exact_angles(const P& p, int 
         sincospi(t - 2.0 * rint(0.5 * t), sn + i, cs + i);
     }
 }
+// The same in 32 bits for queries, which f16 holds to 2^-12. Turns are reduced to quarters in 64 bits: what is left is small and loses little as f32.
+template <class P> __device__ __forceinline__ void short_angles(const P& p, int pos, float* cs, float* sn, int tid, int threads) {
+    for (int i = tid; i < p.half; i += threads) {
+        const double t = (double)pos * ((double)p.turns[i] + (double)p.turns[p.half + i]) * 4.0, whole = rint(t);
+        const int quarter = (int)((long long)whole & 3);
+        float s, c;
+        sincospif(0.5f * (float)(t - whole), &s, &c);
+        cs[i] = quarter == 0 ? c : quarter == 1 ? -s : quarter == 2 ? -c : s;
+        sn[i] = quarter == 0 ? s : quarter == 1 ? c : quarter == 2 ? -s : -c;
+    }
+}
 // Dimension i of a query or key whose leading 2 · half dimensions turn, i with i + half.
 template <typename T> __device__ __forceinline__ double turned(int half, const T* x, const double* cs, const double* sn, int i) {
     const double v = (double)to_f(x[i]);
@@ -177,19 +189,19 @@ template <typename T> __device__ __forceinline__ double norm_factor(const PackP&
 __device__ __forceinline__ int query_exponent(float top) { return min(max((int)(__float_as_uint(top) >> 23), 1), 253); }
 __device__ __forceinline__ float power_down(int e) { return __uint_as_float((unsigned)(254 - e) << 23); }
 __device__ __forceinline__ float power_up(int e) { return __uint_as_float((unsigned)e << 23); }
-// `n` values of a head by one warp: codes and scales to where they are held. value(i): dimension i.
-template <class F> __device__ __forceinline__ void put_head(unsigned char* codes, unsigned char* scales, int n, float factor, F&& value) {
-    const int lane = threadIdx.x & 31;
-    for (int c = 0; c < n; c += 32) {
-        const int i = c + lane;
-        const float y = i < n ? value(i) / factor : 0.f;
-        float a = fabsf(y);
+// 32 values of a head by one warp, the lane's `value` dimension c + lane: codes and scales to where they are held. Values from n on are nobody's.
+__device__ __forceinline__ void put_32(unsigned char* codes, unsigned char* scales, int c, int n, float factor, float value) {
+    const int lane = threadIdx.x & 31, i = c + lane;
+    const float y = i < n ? value / factor : 0.f;
+    float a = fabsf(y);
 #pragma unroll
-        for (int o = 8; o > 0; o >>= 1) a = max_nan(a, __shfl_xor_sync(0xffffffffu, a, o));
-        const unsigned s = scale_code(a), code = code_of(over_scale(y, scale_value(s))), next = __shfl_down_sync(0xffffffffu, code, 1);
-        if (i < n && lane % 2 == 0) codes[i / 2] = (unsigned char)(code | next << 4);
-        if (i < n && lane % kPack == 0) scales[i / kPack] = (unsigned char)s;
-    }
+    for (int o = 8; o > 0; o >>= 1) a = max_nan(a, __shfl_xor_sync(0xffffffffu, a, o));
+    const unsigned s = scale_code(a), code = code_of(over_scale(y, scale_value(s))), next = __shfl_down_sync(0xffffffffu, code, 1);
+    if (i < n && lane % 2 == 0) codes[i / 2] = (unsigned char)(code | next << 4);
+    if (i < n && lane % kPack == 0) scales[i / kPack] = (unsigned char)s;
+}
+template <class F> __device__ __forceinline__ void put_head(unsigned char* codes, unsigned char* scales, int n, float factor, F&& value) {
+    for (int c = 0; c < n; c += 32) put_32(codes, scales, c, n, factor, c + (int)(threadIdx.x & 31) < n ? value(c + (int)(threadIdx.x & 31)) : 0.f);
 }
 
 // Single tokens in bf16 (packed_decode.cu), keys and values of 256 dimensions at most.

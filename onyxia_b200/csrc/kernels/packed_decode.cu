@@ -29,10 +29,10 @@ template <int KS, int VC> struct Smem {
     static constexpr int part = part_size(kHeads, dv);            // floats of one partial result
     static constexpr int stage = kTile * (dk + dv) / kPack * 9;   // codes of keys, scales, codes of values, scales
     static constexpr int rings = kStages * kWarps * stage, parts = kWarps * part * 4;  // [stages][warps][stage]; partial results take their place
-    // before the last stage is filled: queries [8 heads] f16, cosines and sines in 64 bits, and in 32
-    static constexpr int q = (kStages - 1) * kWarps * stage, angle = q + kHeads * q_stride;
+    // before the last stage is filled: queries [8 heads] f16, cosines and sines in 64 bits, and in 32, and what comes from the projection: queries of 8 heads, the key, the value
+    static constexpr int q = (kStages - 1) * kWarps * stage, angle = q + kHeads * q_stride, raw = angle + dk * 12;
     static constexpr int total = rings > parts ? rings : parts;
-    static_assert(angle + dk * 12 <= rings && angle % 16 == 0, "queries and angles fit the last stage");
+    static_assert(raw + (kHeads + 1) * dk * 2 + dv * 2 <= rings && angle % 16 == 0 && raw % 16 == 0, "all of it fits the last stage");
 };
 
 __device__ __forceinline__ float exp2_fast(float x) {
@@ -42,10 +42,6 @@ __device__ __forceinline__ float exp2_fast(float x) {
 }
 
 // What single tokens have to go through: blocks of 128 keys of every sequence and group of query heads (a cell), cell behind cell.
-struct Work {
-    long long total;  // blocks
-    int most;         // of one cell
-};
 template <class P> __device__ __forceinline__ int blocks_of(const P& p, const SeqRow& s) {
     return s.len == 1 ? s.past / (kTile * kWarps) + 1 - first_key(p, s.past) / (kTile * kWarps) : 0;
 }
@@ -107,22 +103,19 @@ template <int KS, int VC, bool WHOLE, int RESIDENT> __global__ void __launch_bou
     // no launch of a step writes the batch description or the keys and values of earlier steps (where the module computes the
     // former, this launch does not begin early): they may be read while the launches before this one finish
     const int rep = p.heads / p.kv_heads, groups = (rep + kHeads - 1) / kHeads, n_groups = p.kv_heads * groups, dim = WHOLE ? 64 * KS : p.dim, vdim = WHOLE ? 16 * VC : p.vdim;
-    Work all{0, 0};
+    long long total = 0;  // blocks
+    int longest = 0;      // of one cell
+#pragma unroll 4
     for (int r0 = 0; r0 < p.n_seqs; r0 += 32) {
         const SeqRow s = r0 + lane < p.n_seqs ? checked_seq(p, r0 + lane) : SeqRow{0, 0, 0, 0};
         if (p.only && s.len > 1 && blockIdx.x == 0 && warp == 0) report(p.err, ERR_BATCH_ROWS, p.node, r0 + lane, s.len);
-        long long sum = blocks_of(p, s);
-        int top = (int)sum;
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            sum += __shfl_xor_sync(0xffffffffu, sum, o);
-            top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-        }
-        all.total += sum * n_groups;
-        all.most = max(all.most, top);
+        const int n = blocks_of(p, s);
+        total += (long long)__reduce_add_sync(0xffffffffu, n) * n_groups;
+        longest = max(longest, __reduce_max_sync(0xffffffffu, n));
     }
     // 64 parts of a cell at most; without room for a counter per cell a CTA has the cells of one sequence and group
-    const long long each = max((all.total + gridDim.x - 1) / gridDim.x, (long long)(all.most + 61) / 62), u0 = blockIdx.x * each, u_end = min(u0 + each, all.total);
+    const long long share = total >> 31 ? (total + gridDim.x - 1) / gridDim.x : ((unsigned)total + gridDim.x - 1) / gridDim.x;
+    const long long each = max(share, (long long)((longest + 61) / 62)), u0 = blockIdx.x * each, u_end = min(u0 + each, total);
     int seq = 0, group = 0, begin = 0;  // where this CTA begins: sequence, group, block
     SeqRow sq{0, 0, 0, 0};
     if (p.cells) {
@@ -131,25 +124,25 @@ template <int KS, int VC, bool WHOLE, int RESIDENT> __global__ void __launch_bou
         long long before = 0;
         for (int r0 = 0;; r0 += 32) {
             const SeqRow s = r0 + lane < p.n_seqs ? checked_seq(p, r0 + lane) : SeqRow{0, 0, 0, 0};
-            const long long mine = (long long)blocks_of(p, s) * n_groups;
-            long long inc = mine;
+            const int n = blocks_of(p, s);
+            const long long chunk = (long long)__reduce_add_sync(0xffffffffu, n) * n_groups;
+            if (before + chunk <= u0) {
+                before += chunk;
+                continue;
+            }
+            int inc = n;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
-                const long long v = __shfl_up_sync(0xffffffffu, inc, o);
+                const int v = __shfl_up_sync(0xffffffffu, inc, o);
                 if (lane >= o) inc += v;
             }
-            const unsigned hit = __ballot_sync(0xffffffffu, before + inc > u0);
-            if (hit) {
-                const int at = __ffs(hit) - 1;
-                const long long in = u0 - before - (__shfl_sync(0xffffffffu, inc, at) - __shfl_sync(0xffffffffu, mine, at));
-                seq = r0 + at;
-                sq = SeqRow{__shfl_sync(0xffffffffu, s.start, at), __shfl_sync(0xffffffffu, s.len, at), __shfl_sync(0xffffffffu, s.past, at), 0};
-                const int n = blocks_of(p, sq);
-                group = (int)(in / n);
-                begin = (int)(in % n);
-                break;
-            }
-            before += __shfl_sync(0xffffffffu, inc, 31);
+            const int at = __ffs(__ballot_sync(0xffffffffu, before + (long long)inc * n_groups > u0)) - 1, blocks = __shfl_sync(0xffffffffu, n, at);
+            const long long in = u0 - before - (long long)(__shfl_sync(0xffffffffu, inc, at) - blocks) * n_groups;
+            seq = r0 + at;
+            sq = SeqRow{__shfl_sync(0xffffffffu, s.start, at), __shfl_sync(0xffffffffu, s.len, at), __shfl_sync(0xffffffffu, s.past, at), 0};
+            group = (int)(in / blocks);
+            begin = (int)(in - (long long)group * blocks);
+            break;
         }
     }
     if (tid < kWarps * kStages) mbar_init(smem_u32(full_s + tid), 1);
@@ -218,40 +211,68 @@ template <int KS, int VC, bool WHOLE, int RESIDENT> __global__ void __launch_bou
         if (!late) fill(0, kStages - 1);
         double *cs = reinterpret_cast<double*>(smem + L::angle), *sn = cs + L::dk / 2;
         float *short_cs = reinterpret_cast<float*>(sn + L::dk / 2), *short_sn = short_cs + L::dk / 2;
-        exact_angles(p, pos, cs, sn, tid, kThreads);
-        for (int i = tid; i < p.half; i += kThreads) short_cs[i] = (float)cs[i], short_sn[i] = (float)sn[i];  // (its own)
+        const bool stores = newest && p.append;
+        if (warp < 2) short_angles(p, pos, short_cs, short_sn, tid, 64);
+        else if (stores) exact_angles(p, pos, cs, sn, tid - 64, 64);
         if (u == u0) pdl_wait();
+        // all that comes from the projection at once
         const bf16* x = (const bf16*)p.proj + (long long)sq.start * p.ld;
+        bf16 *raw = reinterpret_cast<bf16*>(smem + L::raw), *raw_key = raw + kHeads * L::dk, *raw_value = raw_key + L::dk;
+        const bf16 *from_q = x + p.q_off + (long long)h0 * dim, *from_k = x + p.k_off + (long long)g * dim, *from_v = x + p.v_off + (long long)g * vdim;
+        if (p.by8) {
+            const int chunks = dim / 8;
+            for (int c = tid; c < n_heads * chunks; c += kThreads) {
+                const int r = over(c, p.by_eighths);
+                *reinterpret_cast<uint4*>(raw + r * L::dk + (c - r * chunks) * 8) = *reinterpret_cast<const uint4*>(from_q + c * 8);
+            }
+            if (stores) {
+                for (int c = tid; c < chunks; c += kThreads) *reinterpret_cast<uint4*>(raw_key + c * 8) = *reinterpret_cast<const uint4*>(from_k + c * 8);
+                for (int c = kThreads - 1 - tid; c < vdim / 8; c += kThreads) *reinterpret_cast<uint4*>(raw_value + c * 8) = *reinterpret_cast<const uint4*>(from_v + c * 8);
+            }
+        } else {
+            for (int r = warp; r < n_heads; r += kWarps)
+                for (int i = lane; i < dim; i += 32) raw[r * L::dk + i] = from_q[r * dim + i];
+            for (int i = tid; stores && i < dim; i += kThreads) raw_key[i] = from_k[i];
+            for (int i = tid; stores && i < vdim; i += kThreads) raw_value[i] = from_v[i];
+        }
         __syncthreads();
-        if (newest && p.append) {
+        if (stores) {
             // (where a key head has several groups of queries, each CTA that needs the new key stores it: the same bits)
-            if (warp == 0) {
-                const bf16* src = x + p.k_off + (long long)g * dim;
-                unsigned char* to = held(p, p.keys, page_at(pos), g, dim);
-                const double f = norm_factor(p, src);
-                put_head(codes_of(p, to, pos, dim), scales_of(p, to, pos, dim), dim, key_factor(p, g),
-                         [&](int i) { return __bfloat162float(__float2bfloat16_rn((float)(turned(p.half, src, cs, sn, i) * f))); });
-            } else if (warp == 1) {
-                const bf16* src = x + p.v_off + (long long)g * vdim;
-                unsigned char* to = held(p, p.values, page_at(pos), g, vdim);
-                put_head(codes_of(p, to, pos, vdim), scales_of(p, to, pos, vdim), vdim, value_factor(p, g), [&](int i) { return __bfloat162float(src[i]); });
+            const bool key = warp < 2;
+            const int d = key ? dim : vdim;
+            unsigned char *to = held(p, key ? p.keys : p.values, page_at(pos), g, d), *codes = codes_of(p, to, pos, d), *scales = scales_of(p, to, pos, d);
+            const float factor = key ? key_factor(p, g) : value_factor(p, g);
+            const double f = key ? norm_factor(p, raw_key) : 1.0;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const int c = j * 64 + (warp & 1) * 32, i = c + lane;
+                if (c >= d) break;
+                const float v = i >= d ? 0.f : key ? __bfloat162float(__float2bfloat16_rn((float)(turned(p.half, raw_key, cs, sn, i) * f))) : __bfloat162float(raw_value[i]);
+                put_32(codes, scales, c, d, factor, v);
             }
         }
+#pragma unroll
         for (int r = warp; r < kHeads; r += kWarps) {
             __half* to = reinterpret_cast<__half*>(smem + L::q + r * L::q_stride);
             const bool live = r < n_heads;
-            const bf16* q = x + p.q_off + (long long)(h0 + (live ? r : 0)) * dim;
-            const float f = (float)norm_factor(p, q);
-            auto value = [&](int i) {
-                const float v = to_f(q[i]);
-                if (i >= 2 * p.half) return v * f;
-                return (i < p.half ? v * short_cs[i] - to_f(q[i + p.half]) * short_sn[i] : v * short_cs[i - p.half] + to_f(q[i - p.half]) * short_sn[i - p.half]) * f;
-            };
-            float top = 0.f;
-            for (int i = lane; i < dim; i += 32) top = fmaxf(top, fabsf(value(i)));
-            const int e = query_exponent(warp_max(top));
+            const bf16* from = raw + (live ? r : 0) * L::dk;
+            const float f = (float)norm_factor(p, from);
+            float v[L::dk / 32], most = 0.f;
+#pragma unroll
+            for (int j = 0; j < L::dk / 32; j++) {
+                const int i = j * 32 + lane;
+                v[j] = 0.f;
+                if (i < dim) {
+                    const float a = to_f(from[i]);
+                    v[j] = i >= 2 * p.half ? a : i < p.half ? a * short_cs[i] - to_f(from[i + p.half]) * short_sn[i] : a * short_cs[i - p.half] + to_f(from[i - p.half]) * short_sn[i - p.half];
+                }
+                v[j] *= f;
+                most = fmaxf(most, fabsf(v[j]));
+            }
+            const int e = query_exponent(warp_max(most));
             const float down = copysignf(power_down(e), p.mul2);
-            for (int i = lane; i < L::dk; i += 32) to[i] = __float2half_rn(live && p.mul2 != 0.f && i < dim ? value(i) * down : 0.f);
+#pragma unroll
+            for (int j = 0; j < L::dk / 32; j++) to[j * 32 + lane] = __float2half_rn(live && p.mul2 != 0.f ? v[j] * down : 0.f);
             if (lane == 0) factor_s[r] = (p.mul2 != 0.f ? fabsf(p.mul2) : 1.f) * power_up(e) * key_factor(p, g);
         }
         __syncthreads();
@@ -266,7 +287,9 @@ template <int KS, int VC, bool WHOLE, int RESIDENT> __global__ void __launch_bou
                 q[c][4 * half + 2] = v.z;
                 q[c][4 * half + 3] = v.w;
             }
-        asm volatile("fence.proxy.async;" ::: "memory");  // copies read the new key, and take the queries' place
+        // copies read the new key, and take the queries' place
+        if (stores) asm volatile("fence.proxy.async;" ::: "memory");
+        else asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncthreads();
         fill(late ? 0 : kStages - 1, kStages);
         // a lane holds scores of keys g8, g8 + 8 and heads 2 · t4, 2 · t4 + 1, and results of dimensions 2 · VC · g8 + 2i, + 1 of these heads
@@ -475,13 +498,15 @@ template <int KS, int VC, bool WHOLE, int RESIDENT> __global__ void __launch_bou
             const int a = (int)(cell0 / each), n = (int)((cell0 + n_blocks - 1) / each) - a + 1, late_first = cell0 != a * each;
             auto place = [&](int k) { return p.part + (2ll * (a + k) + (k == 0 ? late_first : 0)) * L::part; };
             join_parts<L::dv>(p, own, kWarps, n_heads, vdim, 0.f, nullptr, place((int)blockIdx.x - a));
-            __threadfence();
             __syncthreads();
             unsigned* counter = p.counters + (long long)seq * n_groups + group;
-            if (tid == 0) arrived = atomicAdd(counter, 1u);
+            if (tid == 0) {  // what the others have written is written before this, and read behind it
+                __threadfence();
+                arrived = atomicAdd(counter, 1u);
+                __threadfence();
+            }
             __syncthreads();
             if (arrived == (unsigned)n - 1) {
-                __threadfence();
                 if (tid == 0) *counter = 0;
                 join_parts<L::dv>(p, place, n, n_heads, vdim, factor, out, nullptr);
             }

@@ -115,7 +115,19 @@ template <int KS, int VC, bool WHOLE, int RESIDENT> __global__ void __launch_bou
     }
     // 64 parts of a cell at most; without room for a counter per cell a CTA has the cells of one sequence and group
     const long long share = total >> 31 ? (total + gridDim.x - 1) / gridDim.x : ((unsigned)total + gridDim.x - 1) / gridDim.x;
-    const long long each = max(share, (long long)((longest + 61) / 62)), u0 = blockIdx.x * each, u_end = min(u0 + each, total);
+    long long each = max(share, (long long)((longest + 61) / 62));
+    // A second cell costs a CTA as much as four to five blocks: where a few more blocks leave every CTA in one cell, cells are filled up to a multiple of them.
+    bool filled = false;
+    if ((long long)p.n_seqs * n_groups <= gridDim.x)
+        for (int more = 0; more < 5 && !filled; more++) {
+            int pieces = 0;
+            for (int r0 = 0; r0 < p.n_seqs; r0 += 32)
+                pieces += __reduce_add_sync(0xffffffffu, r0 + lane < p.n_seqs ? (blocks_of(p, checked_seq(p, r0 + lane)) + (int)each + more - 1) / ((int)each + more) : 0);
+            filled = pieces * n_groups <= (int)gridDim.x;
+            if (filled) total = pieces * n_groups * (each += more);
+        }
+    auto room = [&](int n) { return filled ? (n + (int)each - 1) / (int)each * (int)each : n; };
+    const long long u0 = blockIdx.x * each, u_end = min(u0 + each, total);
     int seq = 0, group = 0, begin = 0;  // where this CTA begins: sequence, group, block
     SeqRow sq{0, 0, 0, 0};
     if (p.cells) {
@@ -124,7 +136,7 @@ template <int KS, int VC, bool WHOLE, int RESIDENT> __global__ void __launch_bou
         long long before = 0;
         for (int r0 = 0;; r0 += 32) {
             const SeqRow s = r0 + lane < p.n_seqs ? checked_seq(p, r0 + lane) : SeqRow{0, 0, 0, 0};
-            const int n = blocks_of(p, s);
+            const int n = room(blocks_of(p, s));
             const long long chunk = (long long)__reduce_add_sync(0xffffffffu, n) * n_groups;
             if (before + chunk <= u0) {
                 before += chunk;
@@ -149,15 +161,22 @@ template <int KS, int VC, bool WHOLE, int RESIDENT> __global__ void __launch_bou
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     bool ok = true;
     unsigned rounds = 0;  // parities of the stages' barriers
-    long long u = u0, left = p.cells ? blocks_of(p, sq) : u_end - u0;
+    long long u = u0, left = p.cells ? blocks_of(p, sq) : filled ? min(each, (long long)blocks_of(p, sq) - begin) : u_end - u0;
     if (left <= 0) return pdl_wait();
+    // turns per position of two pairs, by the first two warps
+    double turns[2];
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+        const int i = tid + k * 64;
+        turns[k] = warp < 2 && i < p.half ? (double)p.turns[i] + (double)p.turns[p.half + i] : 0.0;
+    }
     while (true) {
         const int g = group / groups, h0 = g * rep + (group % groups) * kHeads, n_heads = min(kHeads, (g + 1) * rep - h0), pos = sq.past, n_blocks = blocks_of(p, sq);
         const int count = (int)min((long long)(n_blocks - begin), left), low = first_key(p, pos), lo = (low / step + begin) * step, hi = min(lo + count * step, pos + 1);
         const int from = max(lo, low), page0 = from >> p.shift, n_pages = ((hi - 1) >> p.shift) - page0 + 1;  // pages in front of the window may be anybody's
         for (int i = tid; i < min(n_pages, kPages); i += kThreads) page_s[i] = (int)page_of(p, seq, (page0 + i) << p.shift);
         const bool newest = begin + count == n_blocks;  // these keys include the new one
-        __syncthreads();
+        if (u == u0) __syncthreads();
         auto page_at = [&](int j) {
             const int i = (j >> p.shift) - page0;
             return i < kPages ? (long long)page_s[i] : page_of(p, seq, j);
@@ -208,12 +227,15 @@ template <int KS, int VC, bool WHOLE, int RESIDENT> __global__ void __launch_bou
 #pragma unroll 1
             for (; i < end; i++) copy(i, i);
         };
-        if (!late) fill(0, kStages - 1);
+        if (u == u0 && !late) fill(0, kStages - 1);
         double *cs = reinterpret_cast<double*>(smem + L::angle), *sn = cs + L::dk / 2;
         float *short_cs = reinterpret_cast<float*>(sn + L::dk / 2), *short_sn = short_cs + L::dk / 2;
         const bool stores = newest && p.append;
-        if (warp < 2) short_angles(p, pos, short_cs, short_sn, tid, 64);
-        else if (stores) exact_angles(p, pos, cs, sn, tid - 64, 64);
+        if (warp < 2) {
+#pragma unroll
+            for (int k = 0; k < 2; k++)
+                if (tid + k * 64 < p.half) short_angle(pos, turns[k], short_cs + tid + k * 64, short_sn + tid + k * 64);
+        } else if (stores) exact_angles(p, pos, cs, sn, tid - 64, 64);
         if (u == u0) pdl_wait();
         // all that comes from the projection at once
         const bf16* x = (const bf16*)p.proj + (long long)sq.start * p.ld;
@@ -236,6 +258,7 @@ template <int KS, int VC, bool WHOLE, int RESIDENT> __global__ void __launch_bou
             for (int i = tid; stores && i < vdim; i += kThreads) raw_value[i] = from_v[i];
         }
         __syncthreads();
+        if (u != u0 && !late) fill(0, kStages - 1);
         if (stores) {
             // (where a key head has several groups of queries, each CTA that needs the new key stores it: the same bits)
             const bool key = warp < 2;
@@ -254,8 +277,13 @@ template <int KS, int VC, bool WHOLE, int RESIDENT> __global__ void __launch_bou
 #pragma unroll
         for (int r = warp; r < kHeads; r += kWarps) {
             __half* to = reinterpret_cast<__half*>(smem + L::q + r * L::q_stride);
-            const bool live = r < n_heads;
-            const bf16* from = raw + (live ? r : 0) * L::dk;
+            if (r >= n_heads) {  // nobody's: nothing
+#pragma unroll
+                for (int j = 0; j < L::dk / 32; j++) to[j * 32 + lane] = __float2half_rn(0.f);
+                if (lane == 0) factor_s[r] = 1.f;
+                continue;
+            }
+            const bf16* from = raw + r * L::dk;
             const float f = (float)norm_factor(p, from);
             float v[L::dk / 32], most = 0.f;
 #pragma unroll
@@ -272,7 +300,7 @@ template <int KS, int VC, bool WHOLE, int RESIDENT> __global__ void __launch_bou
             const int e = query_exponent(warp_max(most));
             const float down = copysignf(power_down(e), p.mul2);
 #pragma unroll
-            for (int j = 0; j < L::dk / 32; j++) to[j * 32 + lane] = __float2half_rn(live && p.mul2 != 0.f ? v[j] * down : 0.f);
+            for (int j = 0; j < L::dk / 32; j++) to[j * 32 + lane] = __float2half_rn(p.mul2 != 0.f ? v[j] * down : 0.f);
             if (lane == 0) factor_s[r] = (p.mul2 != 0.f ? fabsf(p.mul2) : 1.f) * power_up(e) * key_factor(p, g);
         }
         __syncthreads();

@@ -459,10 +459,13 @@ void emit_packed_attention(Emitter& em, const PackedDesc& d, const TRef& proj, c
     if (tc && (p.only || n_seqs > 1)) {
         const PackedDecode dc = packed_decode_of(d.dim, d.vdim);
         const int64_t groups = d.kv_heads * ((d.heads / d.kv_heads + dc.heads - 1) / dc.heads), cells = n_seqs * groups;
-        // As many CTAs as there is room for share the keys of all sequences evenly, but for cells without a counter each.
-        const int64_t blocks = ((int64_t)p.width * d.page + dc.step - 1) / dc.step + 1, ctas = cells > (int64_t)kCounterWords ? cells : std::min<int64_t>((int64_t)dc.resident * sm_count(), cells * blocks);
-        p.cells = cells > (int64_t)kCounterWords ? (int)cells : 0;
-        const Buf part = p.cells ? none : em.scratch((size_t)ctas * 2 * dc.part * 4);
+        // Pieces of the same number for every cell leave nobody a second one, which costs as much as a dozen blocks of 128 keys. With more cells than places, or places that would stay empty, CTAs share
+        // all blocks evenly, but for cells without a counter each.
+        const int64_t places = (int64_t)dc.resident * sm_count(), blocks = ((int64_t)p.width * d.page + dc.step - 1) / dc.step + 1;
+        const int64_t pieces = std::min<int64_t>({places / cells, blocks, dc.pieces});
+        p.pieces = (int)(cells > (int64_t)kCounterWords ? 1 : pieces * cells * 5 >= places * 4 || pieces == blocks || pieces == dc.pieces ? pieces : 0);
+        const int64_t ctas = p.pieces ? cells * p.pieces : std::min(places, cells * blocks);
+        const Buf part = p.pieces == 1 ? none : em.scratch((size_t)ctas * 2 * dc.part * 4);
         ensure_max_dynamic_smem((const void*)dc.kernel, dc.smem);
         launch(dc.kernel, dim3((unsigned)ctas), 128, (unsigned)dc.smem, part, "packed_decode");
     }

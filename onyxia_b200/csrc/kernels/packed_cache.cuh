@@ -36,7 +36,7 @@ struct PackP {
     unsigned by_rep, by_units, by_runs;  // for over(): heads of a key head, units of eight pairs or dimensions of a query or key, runs of eight dimensions of a value
     unsigned by_key, by_value, by_eighths;  // the same: scales of a key, of a value, runs of eight dimensions of a key
     int by8;                     // the parts of a projection row begin on 16 bytes
-    int cells;                   // single tokens: a CTA per sequence and group, of which there are so many; 0: CTAs share them evenly
+    int pieces;                  // single tokens: CTAs per sequence and group of query heads; 0: CTAs share them all evenly
     int raw_slots;               // prompts: copies of 64 keys or values under way
     int only;                    // no rows for prompts: as many rows as sequences, none of which may have more than one new token
 };
@@ -207,7 +207,7 @@ using PackKernel = void (*)(const PackP);
 struct PackedDecode {
     PackKernel kernel;
     int smem, part;          // bytes; floats of a partial result
-    int resident, heads, step;  // CTAs of an SM; query heads and keys that a CTA takes at a time
+    int resident, heads, step, pieces;  // CTAs of an SM; query heads and keys that a CTA takes at a time; the most CTAs that may share a sequence
 };
 PackedDecode packed_decode_of(int64_t dim, int64_t vdim);
 // Prompts in bf16 (packed_prefill.cu), keys and values of 256 dimensions at most, 128 query heads of a key head at most.

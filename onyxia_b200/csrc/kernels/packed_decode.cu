@@ -12,7 +12,7 @@ namespace oxk {
 
 namespace {
 
-constexpr int kWarps = 4, kThreads = kWarps * 32, kPages = 256, kHeads = 8, kKeys = 16, kTile = 2 * kKeys, kStages = 3;
+constexpr int kWarps = 4, kThreads = kWarps * 32, kPages = 256, kHeads = 8, kKeys = 16, kTile = 2 * kKeys, kStages = 3, kMostParts = 64;
 constexpr float kNone = -1e30f;  // below every score, and finite: differences stay numbers
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
@@ -87,8 +87,8 @@ template <int DV, class At> __device__ __forceinline__ void join_parts(const Pac
     }
 }
 
-// Every CTA goes through the same number of blocks: cells that no CTA has alone are joined by the last of those that share one. (With a grid of cells and splits, 64 sequences behind 4096 to 8191 keys
-// and rounds that the last CTAs leave half empty: %ROUNDS%.) WHOLE: keys have 64 · KS dimensions and values 16 · VC.
+// CTAs have a piece of a cell each where there is room for all cells at once (emit_packed_attention), otherwise the same share of the blocks of all cells: cells that no CTA has alone are joined by the
+// last of those that have a part. WHOLE: keys have 64 · KS dimensions and values 16 · VC.
 template <int KS, int VC, bool WHOLE, int RESIDENT> __global__ void __launch_bounds__(kThreads, RESIDENT) packed_decode(const PackP p) {
     extern __shared__ __align__(16) unsigned char smem[];
     __shared__ unsigned arrived;
@@ -103,40 +103,36 @@ template <int KS, int VC, bool WHOLE, int RESIDENT> __global__ void __launch_bou
     // no launch of a step writes the batch description or the keys and values of earlier steps (where the module computes the
     // former, this launch does not begin early): they may be read while the launches before this one finish
     const int rep = p.heads / p.kv_heads, groups = (rep + kHeads - 1) / kHeads, n_groups = p.kv_heads * groups, dim = WHOLE ? 64 * KS : p.dim, vdim = WHOLE ? 16 * VC : p.vdim;
-    long long total = 0;  // blocks
-    int longest = 0;      // of one cell
-#pragma unroll 4
-    for (int r0 = 0; r0 < p.n_seqs; r0 += 32) {
-        const SeqRow s = r0 + lane < p.n_seqs ? checked_seq(p, r0 + lane) : SeqRow{0, 0, 0, 0};
-        if (p.only && s.len > 1 && blockIdx.x == 0 && warp == 0) report(p.err, ERR_BATCH_ROWS, p.node, r0 + lane, s.len);
-        const int n = blocks_of(p, s);
-        total += (long long)__reduce_add_sync(0xffffffffu, n) * n_groups;
-        longest = max(longest, __reduce_max_sync(0xffffffffu, n));
-    }
-    // 64 parts of a cell at most; without room for a counter per cell a CTA has the cells of one sequence and group
-    const long long share = total >> 31 ? (total + gridDim.x - 1) / gridDim.x : ((unsigned)total + gridDim.x - 1) / gridDim.x;
-    long long each = max(share, (long long)((longest + 61) / 62));
-    // A second cell costs a CTA as much as four to five blocks: where a few more blocks leave every CTA in one cell, cells are filled up to a multiple of them.
-    bool filled = false;
-    if ((long long)p.n_seqs * n_groups <= gridDim.x)
-        for (int more = 0; more < 5 && !filled; more++) {
-            int pieces = 0;
-            for (int r0 = 0; r0 < p.n_seqs; r0 += 32)
-                pieces += __reduce_add_sync(0xffffffffu, r0 + lane < p.n_seqs ? (blocks_of(p, checked_seq(p, r0 + lane)) + (int)each + more - 1) / ((int)each + more) : 0);
-            filled = pieces * n_groups <= (int)gridDim.x;
-            if (filled) total = pieces * n_groups * (each += more);
-        }
-    auto room = [&](int n) { return filled ? (n + (int)each - 1) / (int)each * (int)each : n; };
-    const long long u0 = blockIdx.x * each, u_end = min(u0 + each, total);
-    int seq = 0, group = 0, begin = 0;  // where this CTA begins: sequence, group, block
+    long long each = 0, u0 = 0, left = 0;  // blocks: a CTA's share, where it begins counted over all cells, what it has to do
+    int seq = 0, group = 0, begin = 0;     // where it begins: sequence, group, block
     SeqRow sq{0, 0, 0, 0};
-    if (p.cells) {
-        if (blockIdx.x < (unsigned)p.cells) seq = blockIdx.x / n_groups, group = blockIdx.x % n_groups, sq = checked_seq(p, seq);
-    } else if (u0 < u_end) {
-        long long before = 0;
-        for (int r0 = 0;; r0 += 32) {
+    if (p.pieces) {
+        const int cell = blockIdx.x / p.pieces, piece = blockIdx.x - cell * p.pieces;
+        seq = cell / n_groups;
+        group = cell - seq * n_groups;
+        sq = checked_seq(p, seq);
+        if (p.only && sq.len > 1 && tid == 0) report(p.err, ERR_BATCH_ROWS, p.node, seq, sq.len);
+        const int n = blocks_of(p, sq), of = min(n, p.pieces);
+        if (piece < of) begin = (int)((long long)n * piece / of), left = (int)((long long)n * (piece + 1) / of) - begin;
+    } else {
+        long long total = 0;
+        int longest = 0;  // cell
+#pragma unroll 4
+        for (int r0 = 0; r0 < p.n_seqs; r0 += 32) {
             const SeqRow s = r0 + lane < p.n_seqs ? checked_seq(p, r0 + lane) : SeqRow{0, 0, 0, 0};
-            const int n = room(blocks_of(p, s));
+            if (p.only && s.len > 1 && blockIdx.x == 0 && warp == 0) report(p.err, ERR_BATCH_ROWS, p.node, r0 + lane, s.len);
+            const int n = blocks_of(p, s);
+            total += (long long)__reduce_add_sync(0xffffffffu, n) * n_groups;
+            longest = max(longest, __reduce_max_sync(0xffffffffu, n));
+        }
+        const long long share = total >> 31 ? (total + gridDim.x - 1) / gridDim.x : ((unsigned)total + gridDim.x - 1) / gridDim.x;
+        each = max(share, (long long)((longest + kMostParts - 2) / (kMostParts - 2)));
+        u0 = blockIdx.x * each;
+        left = min(each, total - u0);
+        long long before = 0;
+        for (int r0 = 0; left > 0; r0 += 32) {
+            const SeqRow s = r0 + lane < p.n_seqs ? checked_seq(p, r0 + lane) : SeqRow{0, 0, 0, 0};
+            const int n = blocks_of(p, s);
             const long long chunk = (long long)__reduce_add_sync(0xffffffffu, n) * n_groups;
             if (before + chunk <= u0) {
                 before += chunk;
@@ -152,7 +148,7 @@ template <int KS, int VC, bool WHOLE, int RESIDENT> __global__ void __launch_bou
             const long long in = u0 - before - (long long)(__shfl_sync(0xffffffffu, inc, at) - blocks) * n_groups;
             seq = r0 + at;
             sq = SeqRow{__shfl_sync(0xffffffffu, s.start, at), __shfl_sync(0xffffffffu, s.len, at), __shfl_sync(0xffffffffu, s.past, at), 0};
-            group = (int)(in / blocks);
+            group = in >> 31 ? (int)(in / blocks) : (int)((unsigned)in / (unsigned)blocks);
             begin = (int)(in - (long long)group * blocks);
             break;
         }
@@ -161,7 +157,7 @@ template <int KS, int VC, bool WHOLE, int RESIDENT> __global__ void __launch_bou
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     bool ok = true;
     unsigned rounds = 0;  // parities of the stages' barriers
-    long long u = u0, left = p.cells ? blocks_of(p, sq) : filled ? min(each, (long long)blocks_of(p, sq) - begin) : u_end - u0;
+    long long u = u0;
     if (left <= 0) return pdl_wait();
     // turns per position of two pairs, by the first two warps
     double turns[2];
@@ -521,10 +517,12 @@ template <int KS, int VC, bool WHOLE, int RESIDENT> __global__ void __launch_bou
         if (count == n_blocks) {
             join_parts<L::dv>(p, own, kWarps, n_heads, vdim, factor, out, nullptr);
         } else {
-            // A CTA's first block has the place 2 · CTA, what it ends with 2 · CTA + 1. The cell's parts are those of the CTAs from the one that has its first block on.
+            // Pieces of a cell stand one behind the other. Shares: a CTA's first block has the place 2 · CTA, what it ends with 2 · CTA + 1; a cell's parts are those of the CTAs from the one that has its
+            // first block on.
             const long long cell0 = u - begin;
-            const int a = (int)(cell0 / each), n = (int)((cell0 + n_blocks - 1) / each) - a + 1, late_first = cell0 != a * each;
-            auto place = [&](int k) { return p.part + (2ll * (a + k) + (k == 0 ? late_first : 0)) * L::part; };
+            const int a = p.pieces ? blockIdx.x / p.pieces * p.pieces : (int)(cell0 / each), n = p.pieces ? min(n_blocks, p.pieces) : (int)((cell0 + n_blocks - 1) / each) - a + 1;
+            const int step_of = p.pieces ? 1 : 2, late_first = !p.pieces && cell0 != a * each;
+            auto place = [&](int k) { return p.part + ((long long)step_of * (a + k) + (k == 0 ? late_first : 0)) * L::part; };
             join_parts<L::dv>(p, own, kWarps, n_heads, vdim, 0.f, nullptr, place((int)blockIdx.x - a));
             __syncthreads();
             unsigned* counter = p.counters + (long long)seq * n_groups + group;
@@ -556,7 +554,7 @@ template <int KS, int VC, bool WHOLE, int RESIDENT> __global__ void __launch_bou
 
 template <int KS, int VC> PackedDecode choice(bool whole) {
     constexpr int resident = KS <= 2 && VC <= 8 ? 4 : 2;
-    return {whole ? packed_decode<KS, VC, true, resident> : packed_decode<KS, VC, false, resident>, Smem<KS, VC>::total, Smem<KS, VC>::part, resident, kHeads, kTile * kWarps};
+    return {whole ? packed_decode<KS, VC, true, resident> : packed_decode<KS, VC, false, resident>, Smem<KS, VC>::total, Smem<KS, VC>::part, resident, kHeads, kTile * kWarps, kMostParts - 2};
 }
 template <int KS> PackedDecode choice(int64_t dim, int64_t vdim) {
     return vdim <= 64 ? choice<KS, 4>(dim == 64 * KS && vdim == 64) : vdim <= 128 ? choice<KS, 8>(dim == 64 * KS && vdim == 128) : choice<KS, 16>(dim == 64 * KS && vdim == 256);

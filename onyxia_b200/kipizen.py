@@ -10,7 +10,8 @@ attention  grouped-query attention with biased projections: rotation of the lead
            divided by a factor, queries and keys divided by their root mean square after it, capped scores, a window, a
            sink of score 0 in the softmax. A layer may read the keys and values of an earlier one. Differential: a head has two
            queries, its key head two keys, and the second softmax map, times a learned factor, is taken from the first; the
-           heads' results are divided by their root mean square
+           heads' results are divided by their root mean square. Keys and values may be held in 4 bits ("cache": "e2m1"), for
+           the layers that read them too: 4.5 bits a value with its share of a scale, instead of the module's type
 lightning  linear attention with a matrix state per head that decays by a constant; the heads' results are normed
            together, gated and projected
 experts    the router's best few, weighted by the softmax over their logits; gated units with silu
@@ -48,6 +49,7 @@ class AttentionConfig:
     window: int = 0           # 0: all keys
     kv_from: int | None = None
     lambda_init: float | None = None  # differential attention, `dim` that of one map: what the second map's factor begins with
+    packed: bool = False      # keys and values are held in 4 bits
 
 
 @dataclasses.dataclass
@@ -88,12 +90,21 @@ def _attention(i: int, m: dict, layers: list) -> AttentionConfig:
         a.lambda_init = float(m["differential"]["lambda_init"])
         if a.kv_from is not None:
             raise ValueError(f"layer {i}: differential attention reads keys of its own")
+    if m.get("cache") is not None:
+        if m["cache"] != "e2m1":
+            raise ValueError(f"layer {i}: unknown cache type {m['cache']!r}")
+        if a.kv_from is not None or a.lambda_init is not None:
+            raise ValueError(f"layer {i}: a cache in 4 bits belongs to keys and values of the layer's own, one key per head")
+        if a.dim % 16 or a.vdim % 16:
+            raise ValueError(f"layer {i}: a cache in 4 bits has a scale per 16 dimensions; {a.dim} and {a.vdim} are not multiples of it")
+        a.packed = True
     if a.kv_from is not None:
         source = layers[a.kv_from].mixer if 0 <= a.kv_from < i else None
         if not isinstance(source, AttentionConfig) or source.kv_from is not None or source.lambda_init is not None:
             raise ValueError(f"layer {i}: layer {a.kv_from} has no keys of its own before it")
         if (source.kv_heads, source.dim, source.vdim) != (a.kv_heads, a.dim, a.vdim):
             raise ValueError(f"layer {i}: its keys and values differ in size from those of layer {a.kv_from}")
+        a.packed = source.packed
     return a
 
 
@@ -177,6 +188,9 @@ def build(cfg: KipizenConfig, w: Weights, dtype: int = ir.BF16) -> ir.Module:
     def maps(m):
         return 1 if m.lambda_init is None else 2
 
+    def pool(m, d):
+        return (ir.U8, [NP, m.kv_heads, PAGE, d // 16 * 9]) if m.packed else (dtype, [NP, m.kv_heads, PAGE, d])
+
     own_kv = [isinstance(l.mixer, AttentionConfig) and l.mixer.kv_from is None for l in cfg.layers]
     ids = b.input("input_ids", ir.I64, [N])
     seqs = b.input("seq_info", ir.I32, [R, 4])
@@ -188,8 +202,7 @@ def build(cfg: KipizenConfig, w: Weights, dtype: int = ir.BF16) -> ir.Module:
         if isinstance(m, LightningConfig):
             state[i] = (b.input(f"slots.{i}.state", ir.F32, [NS, m.heads, m.dim, m.vdim]),)
         elif own_kv[i]:
-            state[i] = (b.input(f"pages.{i}.keys", dtype, [NP, m.kv_heads, PAGE, maps(m) * m.dim]),
-                        b.input(f"pages.{i}.values", dtype, [NP, m.kv_heads, PAGE, m.vdim]))
+            state[i] = (b.input(f"pages.{i}.keys", *pool(m, maps(m) * m.dim)), b.input(f"pages.{i}.values", *pool(m, m.vdim)))
 
     # A sum that has not been formed yet: (residual or None, sublayer result, its factor). The norm that reads it forms it
     # and leaves the new residual.
@@ -231,15 +244,16 @@ def build(cfg: KipizenConfig, w: Weights, dtype: int = ir.BF16) -> ir.Module:
                 [out, (dtype, [NP, m.kv_heads, PAGE, 2 * m.dim]), (dtype, [NP, m.kv_heads, PAGE, m.vdim])])
             updated.extend([(f"pages.{i}.keys", keys), (f"pages.{i}.values", values)])
         elif own_kv[i]:
-            b.set_loc(f"{p}.mix", "PagedKVAttention")
-            o, keys, values = b.composite(
-                "onyxia.PagedKVAttention", dict(attrs, k_offset=q_n, v_offset=q_n + k_n), [proj, turns, *state[i], seqs, table],
-                [out, (dtype, [NP, m.kv_heads, PAGE, m.dim]), (dtype, [NP, m.kv_heads, PAGE, m.vdim])])
+            kind = "PackedKVAttention" if m.packed else "PagedKVAttention"
+            b.set_loc(f"{p}.mix", kind)
+            o, keys, values = b.composite("onyxia." + kind, dict(attrs, k_offset=q_n, v_offset=q_n + k_n), [proj, turns, *state[i], seqs, table],
+                                          [out, pool(m, m.dim), pool(m, m.vdim)])
             pools[i] = (keys, values)
             updated.extend([(f"pages.{i}.keys", keys), (f"pages.{i}.values", values)])
         else:
-            b.set_loc(f"{p}.mix", "SharedKVAttention")
-            o = b.composite("onyxia.SharedKVAttention", attrs, [proj, turns, *pools[m.kv_from], seqs, table], [out])[0]
+            kind = "SharedPackedKVAttention" if m.packed else "SharedKVAttention"
+            b.set_loc(f"{p}.mix", kind)
+            o = b.composite("onyxia." + kind, attrs, [proj, turns, *pools[m.kv_from], seqs, table], [out])[0]
         b.set_loc(f"{p}.mix.out", "Linear")
         return x, b.composite("onyxia.Linear", {}, [o, matrix(f"{p}.mix.o", H, m.heads * m.vdim)], [(ir.F32, [N, H])])[0]
 

@@ -62,34 +62,35 @@ template <typename T> __global__ void __launch_bounds__(128) packed_write(const 
     }
 }
 
-// The same in bf16 eight elements at a time, where heads, rotated halves and rows allow it: a unit is eight pairs that turn or eight elements that do not, two neighbours share their scales.
-__global__ void __launch_bounds__(128, 8) packed_write8(const PackP p) {
-    // cos[half], sin[half], norms of keys [kv_heads] in 64 bits; both angles as f32, norms of queries [heads], with queries as f16 their largest elements [heads]
-    extern __shared__ double angle[];
+// The same in bf16 eight elements at a time, where heads, rotated halves and rows allow it: a unit is eight pairs that turn (all of them, ALL) or eight elements that do not, two neighbours share their
+// scales. Angles, and keys where that says which bf16 they are, in 32 bits.
+template <bool ALL, bool NORM> __global__ void __launch_bounds__(128, 8) packed_write8(const PackP p) {
+    extern __shared__ __align__(16) float cs[];  // cosines [half], sines [half], norms of keys [kv_heads] in 64 bits, of queries [heads], with queries as f16 their largest elements [heads]
     pdl_enter();
     const int row = blockIdx.x, tid = threadIdx.x;
     // the row's queries, keys and values are on their way while its sequence is looked up and its angles are made
     const bf16* x = (const bf16*)p.proj + (long long)row * p.ld;
-    auto fetch = [&](long long at, int n) {
-        for (int i = tid * 64; i < n; i += 128 * 64) asm volatile("prefetch.global.L1 [%0];" ::"l"(x + at + i) : "memory");
+    const bf16 *from_q = x + p.q_off, *from_k = x + p.k_off, *from_v = x + p.v_off;
+    auto fetch = [&](const bf16* from, int n) {
+        for (int i = tid * 64; i < n; i += 128 * 64) asm volatile("prefetch.global.L1 [%0];" ::"l"(from + i) : "memory");
     };
-    fetch(p.q_off, p.heads * p.dim);
-    if (p.append) fetch(p.k_off, p.kv_heads * p.dim), fetch(p.v_off, p.kv_heads * p.vdim);
+    fetch(from_q, p.heads * p.dim);
+    if (p.append) fetch(from_k, p.kv_heads * p.dim), fetch(from_v, p.kv_heads * p.vdim);
     const int s = find_seq(p.seqs, p.n_seqs, row);
     const SeqRow sq = checked_seq(p, s);
     check_others(p, row, tid, 128);
-    const int pos = sq.past + row - sq.start, kv = p.append ? p.kv_heads : 0;
+    const int pos = sq.past + row - sq.start, kv = p.append ? p.kv_heads : 0, half = p.half;
     if (row < sq.start || row >= sq.start + sq.len || (sq.len == 1 && !p.singles)) return;
-    double* key_norm = angle + 2 * p.half;
-    float *short_angle = reinterpret_cast<float*>(key_norm + p.kv_heads), *query_norm = short_angle + 2 * p.half;
+    float* sn = cs + half;
+    double* norms = reinterpret_cast<double*>(sn + half);
+    float* query_norm = reinterpret_cast<float*>(norms + p.kv_heads);
     unsigned* query_top = reinterpret_cast<unsigned*>(query_norm + p.heads);
-    exact_angles(p, pos, angle, angle + p.half, tid, 128);
-    for (int i = tid; i < p.half; i += 128) short_angle[i] = (float)angle[i], short_angle[p.half + i] = (float)angle[p.half + i];  // (its own)
-    const int turned = p.half / 8, units = p.dim / 8 - turned, runs = p.vdim / 8;
-    if (p.norm)
+    for (int i = tid; i < half; i += 128) short_angle(pos, (double)p.turns[i] + (double)p.turns[half + i], cs + i, sn + i);
+    const int turned = half / 8, units = p.dim / 8 - turned, runs = p.vdim / 8, eighths = p.dim / 8;
+    if (NORM)
         for (int h = tid >> 5; h < p.heads + kv; h += 4) {
-            const double f = norm_factor(p, x + (h < p.heads ? p.q_off + (long long)h * p.dim : p.k_off + (long long)(h - p.heads) * p.dim));
-            if ((tid & 31) == 0) (h < p.heads ? (void)(query_norm[h] = (float)f) : (void)(key_norm[h - p.heads] = f));
+            const double f = norm_factor(p, h < p.heads ? from_q + h * p.dim : from_k + (h - p.heads) * p.dim);
+            if ((tid & 31) == 0) (h < p.heads ? (void)(query_norm[h] = (float)f) : (void)(norms[h - p.heads] = f));
         }
     auto wide = [](const bf16* from, float (&v)[8]) {
         const uint4 u = *reinterpret_cast<const uint4*>(from);
@@ -97,25 +98,24 @@ __global__ void __launch_bounds__(128, 8) packed_write8(const PackP p) {
 #pragma unroll
         for (int e = 0; e < 4; e++) v[2 * e] = __uint_as_float(w[e] << 16), v[2 * e + 1] = __uint_as_float(w[e] & 0xFFFF0000u);
     };
-    if (p.q_mul) {  // a rotation makes no element larger than sqrt 2 times the largest
+    if (p.q_mul) {  // (a rotation makes no element larger than sqrt 2 times the largest)
         for (int h = tid; h < p.heads; h += 128) query_top[h] = 0;
         __syncthreads();
-        for (int u = tid; u < p.heads * (p.dim / 8); u += 128) {
-            float a[8], top = 0.f;
-            wide(x + p.q_off + u * 8, a);
-#pragma unroll
-            for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(a[e]));
-            atomicMax(query_top + u * 8 / p.dim, __float_as_uint(top));
+        for (int u = tid; u < p.heads * eighths; u += 128) {
+            const uint4 v = *reinterpret_cast<const uint4*>(from_q + u * 8);
+            auto most = [](unsigned a, unsigned b) { return __vmaxu2(a & 0x7FFF7FFFu, b & 0x7FFF7FFFu); };  // magnitudes are ordered as their bits
+            const unsigned m = __vmaxu2(most(v.x, v.y), most(v.z, v.w));
+            atomicMax(query_top + over(u, p.by_eighths), max(m << 16, m & 0xFFFF0000u));
         }
     }
     __syncthreads();
     for (int u = tid; u < p.heads * units; u += 128) {
         const int h = over(u, p.by_units), i = u - h * units;
-        const bool turns = i < turned;
+        const bool turns = ALL || i < turned;
         const int at = turns ? i * 8 : (i + turned) * 8;
-        const bf16* src = x + p.q_off + h * p.dim + at;
+        const bf16* src = from_q + h * p.dim + at;
         const long long to = ((long long)row * p.heads + h) * p.dim + at;
-        float f = p.norm ? query_norm[h] : 1.f;
+        float f = NORM ? query_norm[h] : 1.f;
         if (p.q_mul) {
             const int e = query_exponent(__uint_as_float(query_top[h]) * f);
             f *= copysignf(power_down(e), p.mul2);
@@ -138,23 +138,27 @@ __global__ void __launch_bounds__(128, 8) packed_write8(const PackP p) {
         };
         float a[8], b[8], o[8];
         wide(src, a);
-        if (!turns) {
 #pragma unroll
-            for (int e = 0; e < 8; e++) o[e] = a[e] * f;
-            put(to, o);
+        for (int e = 0; e < 8; e++) a[e] *= f;
+        if (!turns) {
+            put(to, a);
             continue;
         }
-        wide(src + p.half, b);
-        const float *c = short_angle + at, *n = c + p.half;
+        wide(src + half, b);
+        const float4 *c4 = reinterpret_cast<const float4*>(cs + at), *n4 = reinterpret_cast<const float4*>(sn + at);
+        const float4 c0 = c4[0], c1 = c4[1], n0 = n4[0], n1 = n4[1];
+        const float c[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w}, n[8] = {n0.x, n0.y, n0.z, n0.w, n1.x, n1.y, n1.z, n1.w};
 #pragma unroll
-        for (int e = 0; e < 8; e++) o[e] = (a[e] * c[e] - b[e] * n[e]) * f;
+        for (int e = 0; e < 8; e++) b[e] *= f, o[e] = a[e] * c[e] - b[e] * n[e];
         put(to, o);
 #pragma unroll
-        for (int e = 0; e < 8; e++) o[e] = (b[e] * c[e] + a[e] * n[e]) * f;
-        put(to + p.half, o);
+        for (int e = 0; e < 8; e++) o[e] = b[e] * c[e] + a[e] * n[e];
+        put(to + half, o);
     }
     if (!p.append) return;
     const long long pg = page_of(p, s, pos);
+    const int off = pos & ((1 << p.shift) - 1), key_head = (p.dim / kPack * 9) << p.shift, value_head = (p.vdim / kPack * 9) << p.shift;
+    unsigned char *keys = p.keys + pg * p.kv_heads * key_head, *values = p.values + pg * p.kv_heads * value_head;
     // eight dimensions from `at` on; the lane next to this one has the other eight of their scale
     auto store = [&](unsigned char* to, int dim, int at, float (&v)[8], float factor, bool in) {
         const bool plain = factor == 1.f;
@@ -165,9 +169,10 @@ __global__ void __launch_bounds__(128, 8) packed_write8(const PackP p) {
 #pragma unroll
         for (int e = 0; e < 8; e++) a = max_nan(a, fabsf(v[e]));
         const unsigned code = scale_code(max_nan(a, __shfl_xor_sync(0xffffffffu, a, 1)));
-        const float scale = scale_value(code), by = scale > 0.f ? 1.f / scale : 0.f;
+        const float scale = scale_value(code);
         // (an infinite value over a scale that is none would be no number)
         if (plain && scale > 0.f) {
+            const float by = __frcp_rn(scale);
 #pragma unroll
             for (int e = 0; e < 8; e++) v[e] = near_scale(v[e], by);
         } else {
@@ -175,65 +180,87 @@ __global__ void __launch_bounds__(128, 8) packed_write8(const PackP p) {
             for (int e = 0; e < 8; e++) v[e] = over_scale(v[e], scale);
         }
         if (!in) return;
-        *reinterpret_cast<unsigned*>(codes_of(p, to, pos, dim) + at / 2) = codes8(v);
-        if (at % kPack == 0) scales_of(p, to, pos, dim)[at / kPack] = (unsigned char)code;
+        *reinterpret_cast<unsigned*>(to + (off * dim + at) / 2) = codes8(v);
+        if (at % kPack == 0) to[((dim / 2) << p.shift) + (off * dim + at) / kPack] = (unsigned char)code;
     };
     for (int u0 = 0; u0 < kv * units; u0 += 128) {
         const bool in = u0 + tid < kv * units;
         const int u = in ? u0 + tid : tid & 1, g = over(u, p.by_units), i = u - g * units;
-        const bool turns = i < turned;
+        const bool turns = ALL || i < turned;
         const int at = turns ? i * 8 : (i + turned) * 8;
-        const bf16* src = x + p.k_off + g * p.dim + at;
-        unsigned char* to = held(p, p.keys, pg, g, p.dim);
-        const double f = p.norm ? key_norm[g] : 1.0;
-        const float factor = key_factor(p, g);
-        float a[8], b[8], o[8];
+        const bf16* src = from_k + g * p.dim + at;
+        unsigned char* to = keys + g * key_head;
+        const double f = NORM ? norms[g] : 1.0;
+        const float factor = key_factor(p, g), short_f = (float)f;
+        float a[8], b[8], second[8] = {}, size[8];
         wide(src, a);
-        if (turns) wide(src + p.half, b);
         // In 32 bits a key is off by less than 2^-21 of its pair; where that leaves open which bf16 it is, and for what is no number, 64 bits say. (One element of 4000.)
-        auto rounded = [&](float (&v)[8], const float (&size)[8], auto&& exact) {
+        auto rounded = [&](float (&v)[8], auto&& exact) {
             unsigned open = 0;
 #pragma unroll
             for (int e = 0; e < 8; e += 2) {
-                const unsigned less = pack_bf16(v[e] - size[e] * 0x1p-21f, v[e + 1] - size[e + 1] * 0x1p-21f), more = pack_bf16(v[e] + size[e] * 0x1p-21f, v[e + 1] + size[e + 1] * 0x1p-21f);
-                open |= less ^ more;
+                const unsigned less = pack_bf16(__fmaf_rn(size[e], -0x1p-21f, v[e]), __fmaf_rn(size[e + 1], -0x1p-21f, v[e + 1]));
+                const unsigned more = pack_bf16(__fmaf_rn(size[e], 0x1p-21f, v[e]), __fmaf_rn(size[e + 1], 0x1p-21f, v[e + 1]));
+                const unsigned other = less ^ more;
+                open |= (other & 0xFFFFu ? 1u << e : 0u) | (other >> 16 ? 2u << e : 0u);
                 v[e] = __uint_as_float(less << 16);
                 v[e + 1] = __uint_as_float(less & 0xFFFF0000u);
             }
-            if (open)
+            if (open) {
+#pragma unroll 1
+                for (int e = 0; e < 8; e++) {
+                    if (!(open >> e & 1)) continue;
+                    const float w = __bfloat162float(__float2bfloat16_rn((float)exact(e)));
 #pragma unroll
-                for (int e = 0; e < 8; e++) v[e] = __bfloat162float(__float2bfloat16_rn((float)exact(e)));
+                    for (int k = 0; k < 8; k++)
+                        if (k == e) v[k] = w;
+                }
+            }
         };
-        float size[8];
-        const float short_f = (float)f;
+        auto turn = [&](int e, double* c, double* n) {
+            const double t = (double)pos * ((double)p.turns[at + e] + (double)p.turns[half + at + e]) * 2.0;
+            sincospi(t - 2.0 * rint(0.5 * t), n, c);
+        };
         if (turns) {
-            const double *c = angle + at, *n = c + p.half;
-            const float *sc = short_angle + at, *sn = sc + p.half;
+            wide(src + half, b);
+            const float4 *c4 = reinterpret_cast<const float4*>(cs + at), *n4 = reinterpret_cast<const float4*>(sn + at);
+            const float4 c0 = c4[0], c1 = c4[1], n0 = n4[0], n1 = n4[1];
+            const float c[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w}, n[8] = {n0.x, n0.y, n0.z, n0.w, n1.x, n1.y, n1.z, n1.w};
+            if (NORM)
 #pragma unroll
-            for (int e = 0; e < 8; e++) size[e] = (fabsf(a[e]) + fabsf(b[e])) * short_f, o[e] = (a[e] * sc[e] - b[e] * sn[e]) * short_f;
-            rounded(o, size, [&](int e) { return ((double)to_f(src[e]) * c[e] - (double)to_f(src[e + p.half]) * n[e]) * f; });
-        } else {
+                for (int e = 0; e < 8; e++) a[e] *= short_f, b[e] *= short_f;
 #pragma unroll
-            for (int e = 0; e < 8; e++) size[e] = p.norm ? fabsf(a[e]) * short_f : 0.f, o[e] = a[e] * short_f;
-            rounded(o, size, [&](int e) { return (double)to_f(src[e]) * f; });
+            for (int e = 0; e < 8; e++) {
+                const float first = a[e] * c[e] - b[e] * n[e];
+                size[e] = fabsf(a[e]) + fabsf(b[e]);
+                second[e] = b[e] * c[e] + a[e] * n[e];
+                a[e] = first;
+            }
+            rounded(a, [&](int e) {
+                double ec, en;
+                turn(e, &ec, &en);
+                return ((double)to_f(src[e]) * ec - (double)to_f(src[e + half]) * en) * f;
+            });
+            rounded(second, [&](int e) {
+                double ec, en;
+                turn(e, &ec, &en);
+                return ((double)to_f(src[e + half]) * ec + (double)to_f(src[e]) * en) * f;
+            });
+        } else if (NORM) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) size[e] = fabsf(a[e]) * short_f, a[e] *= short_f;
+            rounded(a, [&](int e) { return (double)to_f(src[e]) * f; });
         }
-        store(to, p.dim, at, o, factor, in);
-        if (turned == 0) continue;  // (all lanes alike)
-        if (turns) {
-            const double *c = angle + at, *n = c + p.half;
-            const float *sc = short_angle + at, *sn = sc + p.half;
-#pragma unroll
-            for (int e = 0; e < 8; e++) o[e] = (b[e] * sc[e] + a[e] * sn[e]) * short_f;
-            rounded(o, size, [&](int e) { return ((double)to_f(src[e + p.half]) * c[e] + (double)to_f(src[e]) * n[e]) * f; });
-        }
-        store(to, p.dim, at + p.half, o, factor, in && turns);
+        // (all lanes come)
+        store(to, p.dim, at, a, factor, in);
+        if (ALL || turned > 0) store(to, p.dim, at + half, second, factor, in && turns);
     }
     for (int u0 = 0; u0 < kv * runs; u0 += 128) {
         const bool in = u0 + tid < kv * runs;
         const int u = in ? u0 + tid : tid & 1, g = over(u, p.by_runs), at = (u - g * runs) * 8;
         float a[8];
-        wide(x + p.v_off + u * 8, a);
-        store(held(p, p.values, pg, g, p.vdim), p.vdim, at, a, value_factor(p, g), in);
+        wide(from_v + u * 8, a);
+        store(values + g * value_head, p.vdim, at, a, value_factor(p, g), in);
     }
 }
 
@@ -433,10 +460,12 @@ void emit_packed_attention(Emitter& em, const PackedDesc& d, const TRef& proj, c
     };
     p.by8 = p.ld % 8 == 0 && d.q_off % 8 == 0 && d.k_off % 8 == 0 && d.v_off % 8 == 0 && proj.buf.off % 16 == 0;
     if (!p.only) {
-        // bytes that the kernel for eight at a time shares; a block may have 48 KB
-        const int64_t eight = d.rot_dims * 12 + d.kv_heads * 8 + d.heads * 8;
-        if (bf && p.by8 && d.rot_dims % 32 == 0 && eight <= 48 * 1024) {
-            launch(packed_write8, dim3((unsigned)rows), 128, (unsigned)eight, none, "packed_write");
+        // bytes that the kernel for eight at a time shares, of which a block may have 48 KB; it counts a page's bytes in 32 bits
+        const int64_t eight = d.kv_heads * 8 + d.rot_dims * 4 + d.heads * 8;
+        if (bf && p.by8 && d.rot_dims % 32 == 0 && eight <= 48 * 1024 && d.kv_heads * d.page * std::max(d.dim, d.vdim) < (int64_t)1 << 31) {
+            const bool turns = d.rot_dims == d.dim;
+            launch(d.norm ? (turns ? packed_write8<true, true> : packed_write8<false, true>) : turns ? packed_write8<true, false> : packed_write8<false, false>, dim3((unsigned)rows), 128, (unsigned)eight,
+                   none, "packed_write");
         } else {
             const PackKernel write = bf ? packed_write<bf16> : packed_write<float>;
             ensure_max_dynamic_smem((const void*)write, 8192 * 8);

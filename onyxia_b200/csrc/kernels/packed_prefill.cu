@@ -3,6 +3,8 @@
 // A CTA owns one or two tiles of 128 (token, head) rows of one key head and walks over their keys, 64 at a time. One warp copies what the pages hold of them, several steps ahead; four warps turn
 // codes into f16 (exactly: packed_cache.cuh), a step ahead of the products; one warp issues these; a thread per row masks and weighs scores. The next 64 keys' scores are made meanwhile: a tile has two turns of them. Two tiles share what is
 // unpacked.
+#include <type_traits>
+
 #include "packed_cache.cuh"
 
 namespace oxk {
@@ -11,6 +13,7 @@ namespace {
 
 constexpr int kRows = 128, kUnpack = 128, kStages = 2, kKeys = 64, kSlots = 8;
 constexpr unsigned kPanelQ = kRows * 128, kPanel = kKeys * 128;  // bytes: rows, or keys, × 64 dimensions
+constexpr float kTwiceLog2e = 2.f * kLog2e;
 constexpr float kNone = -1e30f;            // below every score, and finite: differences stay numbers
 
 __device__ __forceinline__ unsigned bits(__half2 v) { return *reinterpret_cast<unsigned*>(&v); }
@@ -205,7 +208,7 @@ template <int TILES, bool CAPPED> __global__ void __launch_bounds__(TILES * kRow
         const int tile = warp / 4, tok = over(tid, p.by_rep), head = g * rep + tid - tok * rep;
         const bool live = tok < n_tok;
         const int pos = live ? pos0 + tok : last, low = first_key(p, pos), last_low = first_key(p, last);  // rows without a token compute something harmless
-        const float mul = live ? p.q_mul[(long long)(sq.start + first + tok) * p.heads + head] : 0.f, cap2 = p.cap2;
+        const float mul = live ? p.q_mul[(long long)(sq.start + first + tok) * p.heads + head] : 0.f, cap2 = p.cap2, by_cap = mul * (1.f / kTwiceLog2e), series1 = cap2 * (-1.f / 3.f), series2 = cap2 * (2.f / 15.f), series3 = cap2 * (-17.f / 315.f);
         const unsigned lanes = (unsigned)((warp & 3) * 32) << 16, sum = t_sum + lanes + tile * 128;
         float m = kNone, l = 0.f, sums[4];
         const float factor = value_factor(p, g);
@@ -216,6 +219,7 @@ template <int TILES, bool CAPPED> __global__ void __launch_bounds__(TILES * kRow
             after_sync();
             const unsigned place = tmem + lanes + (2 * tile + at.s) * kKeys;
             const bool edge = j0 + kKeys - 1 > pos0 || j0 < last_low;
+            bool near = false;
             // In base 2. Factors are positive (a negative one is in the queries): the largest score is that of the largest product.
             auto score = [&](float d) {
                 const float x = d * mul;
@@ -233,7 +237,7 @@ template <int TILES, bool CAPPED> __global__ void __launch_bounds__(TILES * kRow
                     take(c * 32, v[c & 1]);
                 }
             };
-            float top = -INFINITY;
+            float top = -INFINITY, least = INFINITY;
             if (edge) {
                 each([&](int c, const unsigned (&v)[32]) {
 #pragma unroll
@@ -243,8 +247,13 @@ template <int TILES, bool CAPPED> __global__ void __launch_bounds__(TILES * kRow
             } else {
                 each([&](int c, const unsigned (&v)[32]) {
 #pragma unroll
-                    for (int e = 0; e < 32; e += 2) top = fmaxf(fmaxf(top, __uint_as_float(v[e])), __uint_as_float(v[e + 1]));
+                    for (int e = 0; e < 32; e += 2) {
+                        top = fmaxf(fmaxf(top, __uint_as_float(v[e])), __uint_as_float(v[e + 1]));
+                        if (CAPPED) least = fminf(fminf(least, __uint_as_float(v[e])), __uint_as_float(v[e + 1]));
+                    }
                 });
+                // tanh u = u (1 - u²/3 + 2u⁴/15 - 17u⁶/315 + 62u⁸/2835 - ...): where no score that the warp's rows see is beyond a quarter of the cap, what is left out is 4e-7 of it.
+                if (CAPPED) near = __all_sync(0xffffffffu, fmaxf(fabsf(top), fabsf(least)) * mul <= 0.25f * kTwiceLog2e);
                 top = score(top);
             }
             // Weights are taken against a maximum that the largest score is up to 8 above: f16 holds 2^8 as exactly as 1.
@@ -268,12 +277,17 @@ template <int TILES, bool CAPPED> __global__ void __launch_bounds__(TILES * kRow
             }
 #pragma unroll
             for (int e = 0; e < 4; e++) sums[e] = 0.f;
-            auto weigh = [&](int c, const unsigned (&v)[32], auto&& shown) {
+            auto near_score = [&](float d) {
+                const float u = d * by_cap, z = u * u;
+                return __fmaf_rn(u, __fmaf_rn(__fmaf_rn(__fmaf_rn(series3, z, series2), z, series1), z, cap2), -m);
+            };
+            auto weigh = [&](int c, const unsigned (&v)[32], auto series, auto&& shown) {
                 unsigned w[16];
 #pragma unroll
                 for (int e = 0; e < 32; e += 2) {
                     float a, b;
-                    if (CAPPED) a = score(__uint_as_float(v[e])) - m, b = score(__uint_as_float(v[e + 1])) - m;
+                    if constexpr (CAPPED && series) a = near_score(__uint_as_float(v[e])), b = near_score(__uint_as_float(v[e + 1]));
+                    else if (CAPPED) a = score(__uint_as_float(v[e])) - m, b = score(__uint_as_float(v[e + 1])) - m;
                     else a = __fmaf_rn(__uint_as_float(v[e]), mul, -m), b = __fmaf_rn(__uint_as_float(v[e + 1]), mul, -m);
                     a = exp2_fast(shown(a, j0 + c + e));
                     b = exp2_fast(shown(b, j0 + c + e + 1));
@@ -283,8 +297,10 @@ template <int TILES, bool CAPPED> __global__ void __launch_bounds__(TILES * kRow
                 }
                 tmem_st16(place + c / 2, w);  // where scores were that this thread has read twice
             };
-            if (edge) each([&](int c, const unsigned (&v)[32]) { weigh(c, v, [&](float x, int j) { return hidden(j) ? -INFINITY : x; }); });
-            else each([&](int c, const unsigned (&v)[32]) { weigh(c, v, [](float x, int) { return x; }); });
+            auto plainly = [](float x, int) { return x; };
+            if (edge) each([&](int c, const unsigned (&v)[32]) { weigh(c, v, std::false_type{}, [&](float x, int j) { return hidden(j) ? -INFINITY : x; }); });
+            else if (CAPPED && near) each([&](int c, const unsigned (&v)[32]) { weigh(c, v, std::true_type{}, plainly); });
+            else each([&](int c, const unsigned (&v)[32]) { weigh(c, v, std::false_type{}, plainly); });
             l += (sums[0] + sums[1]) + (sums[2] + sums[3]);
             tmem_st_wait();
             before_sync();

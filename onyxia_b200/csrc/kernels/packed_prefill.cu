@@ -85,27 +85,37 @@ template <int TILES, bool CAPPED> __global__ void __launch_bounds__(TILES * kRow
         // A thread has sixteen dimensions of a key at a time.
         const int u0 = tid - kSoft;
         auto put = [&](unsigned from, unsigned base, int i, int dim, unsigned by) {
-            const int j0 = (kt0 + i) * kKeys, blocks = dim / kPack, whole = j0 >= lowest && j0 + kKeys - 1 <= last;
+            const int j0 = (kt0 + i) * kKeys, blocks = dim / kPack;
+            const bool whole = j0 >= lowest && j0 + kKeys - 1 <= last;
             const unsigned scales = from + kKeys * (dim / 2);
-#pragma unroll 4
-            for (int u = u0; u < kKeys * blocks; u += kUnpack) {
-                const int key = over(u, by), b = u - key * blocks;
+            // Sixteen dimensions of a key. (The first 64 dimensions' lanes begin with the even eighths, the next with the odd ones: eight lanes write 128 bytes in different banks.)
+            auto unit = [&](unsigned codes, unsigned scale, unsigned to0, unsigned to1, unsigned first, int key) {
                 unsigned x, y, code;
-                asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(x), "=r"(y) : "r"(from + u * 8));
-                asm volatile("ld.shared.u8 %0, [%1];" : "=r"(code) : "r"(scales + u));
+                asm volatile("ld.shared.b32 %0, [%1];" : "=r"(x) : "r"(codes + first));
+                asm volatile("ld.shared.b32 %0, [%1];" : "=r"(y) : "r"(codes + (first ^ 4)));
+                asm volatile("ld.shared.u8 %0, [%1];" : "=r"(code) : "r"(scale));
                 // keys that are not there are 0: what was copied in their place, or not, may be no number
                 if (!whole && (j0 + key < lowest || j0 + key > last)) code = 0;
                 const __half2 s = __low2half2(scales_f16(code));
-                // (the first 64 dimensions' lanes begin with the even eighths, the next with the odd ones: eight lanes write 128 bytes in different banks)
-                const unsigned flip = b >> 2 & 1, to = base + (b >> 2) * kPanel + key * 128;
-#pragma unroll
-                for (unsigned w = 0; w < 2; w++) {
-                    const unsigned odd = w ^ flip, c = (b & 3) * 2 + odd;
-                    __half2 v[4];
-                    units8(odd ? y : x, v);
-                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to + ((c ^ (key & 7)) << 4)), "r"(bits(__hmul2(v[0], s))), "r"(bits(__hmul2(v[1], s))),
-                                 "r"(bits(__hmul2(v[2], s))), "r"(bits(__hmul2(v[3], s)))
-                                 : "memory");
+                __half2 v[4], w[4];
+                units8(x, v);
+                units8(y, w);
+                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to0), "r"(bits(__hmul2(v[0], s))), "r"(bits(__hmul2(v[1], s))), "r"(bits(__hmul2(v[2], s))), "r"(bits(__hmul2(v[3], s)))
+                             : "memory");
+                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to1), "r"(bits(__hmul2(w[0], s))), "r"(bits(__hmul2(w[1], s))), "r"(bits(__hmul2(w[2], s))), "r"(bits(__hmul2(w[3], s)))
+                             : "memory");
+            };
+            if ((blocks & blocks - 1) == 0) {  // a thread's units are the same dimensions of keys that lie a multiple of eight apart
+                const int b = u0 & blocks - 1, key0 = over(u0, by), keys = over(kUnpack, by);
+                const unsigned flip = b >> 2 & 1, c = (b & 3) * 2 + flip, row = base + (b >> 2) * kPanel + key0 * 128, to0 = row + ((c ^ (key0 & 7)) << 4), to1 = row + ((c ^ 1 ^ (key0 & 7)) << 4);
+#pragma unroll 4
+                for (int k = 0; k + key0 < kKeys; k += keys) unit(from + (u0 + k * blocks) * 8, scales + u0 + k * blocks, to0 + k * 128, to1 + k * 128, flip * 4, k + key0);
+            } else {
+#pragma unroll 2
+                for (int u = u0; u < kKeys * blocks; u += kUnpack) {
+                    const int key = over(u, by), b = u - key * blocks;
+                    const unsigned flip = b >> 2 & 1, c = (b & 3) * 2 + flip, row = base + (b >> 2) * kPanel + key * 128;
+                    unit(from + u * 8, scales + u, row + ((c ^ (key & 7)) << 4), row + ((c ^ 1 ^ (key & 7)) << 4), flip * 4, key);
                 }
             }
         };

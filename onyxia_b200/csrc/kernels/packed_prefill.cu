@@ -236,15 +236,26 @@ template <int TILES, bool CAPPED> __global__ void __launch_bounds__(TILES * kRow
                 return CAPPED ? cap2 - __fdividef(2.f * cap2, 1.f + exp2_fast(x)) : x;
             };
             auto hidden = [&](int j) { return j > pos || j < low; };
-            // 32 products at a time, the next ones on their way
-            auto each = [&](auto&& take) {
-                unsigned v[2][32];
-                tmem_ld32(v[0], place);
+            // 32 products at a time. Two tiles' threads have the registers to keep them all; otherwise they are read twice, the next ones on their way.
+            unsigned all[TILES == 2 ? kKeys : 64];
+            if constexpr (TILES == 2) {
 #pragma unroll
-                for (int c = 0; c < kKeys / 32; c++) {
-                    tmem_ld_wait();
-                    if (c + 1 < kKeys / 32) tmem_ld32(v[(c + 1) & 1], place + (c + 1) * 32);
-                    take(c * 32, v[c & 1]);
+                for (int c = 0; c < kKeys; c += 32) tmem_ld32(*reinterpret_cast<unsigned(*)[32]>(all + c), place + c);
+                tmem_ld_wait();
+            }
+            auto each = [&](auto&& take) {
+                if constexpr (TILES == 2) {
+#pragma unroll
+                    for (int c = 0; c < kKeys; c += 32) take(c, *reinterpret_cast<const unsigned(*)[32]>(all + c));
+                } else {
+                    unsigned(&v)[2][32] = *reinterpret_cast<unsigned(*)[2][32]>(all);
+                    tmem_ld32(v[0], place);
+#pragma unroll
+                    for (int c = 0; c < kKeys / 32; c++) {
+                        tmem_ld_wait();
+                        if (c + 1 < kKeys / 32) tmem_ld32(v[(c + 1) & 1], place + (c + 1) * 32);
+                        take(c * 32, v[c & 1]);
+                    }
                 }
             };
             float top = -INFINITY, least = INFINITY;

@@ -683,7 +683,7 @@ bool packed_sizes_fit(const Module& m, const Node& n, size_t pools) {
     for (auto [t, d] : {std::pair<const TensorType*, int64_t>{&keys, D}, {&values, V}})
         if (t->dtype != DType::U8 || t->shape.size() != 4 || !is_const(t->shape[1], G) || !t->shape[2].as_const() || !is_const(t->shape[3], d / 16 * 9)) return false;
     const uint64_t page = *keys.shape[2].as_const();
-    if (page < 16 || page > (1u << 20) || (page & (page - 1)) != 0 || values.shape[0] != keys.shape[0] || values.shape[2] != keys.shape[2]) return false;
+    if (page < 16 || page > (1u << 20) || (page & (page - 1)) != 0 || page * (uint64_t)std::max(D, V) > 1u << 30 || values.shape[0] != keys.shape[0] || values.shape[2] != keys.shape[2]) return false;
     const int64_t factors = a.int_or("factors", 0);
     if (factors != 0 && factors != 1) return false;
     for (size_t i = n.inputs.size() - 2 * (size_t)factors; i < n.inputs.size(); i++) {

@@ -446,9 +446,9 @@ void emit_packed_attention(Emitter& em, const PackedDesc& d, const TRef& proj, c
     p.by_key = by_of(d.dim / kPack);
     p.by_value = by_of(d.vdim / kPack);
     p.by_eighths = by_of(d.dim / 8);
-    const bool bf = proj.dtype == DT_BF16, tc = out && bf && d.dim <= 256 && d.vdim <= 256 && n_seqs <= 65535;
+    const bool bf = proj.dtype == DT_BF16, tc = out && bf && d.dim <= 256 && d.vdim <= 256 && n_seqs <= 65535 && n_seqs * d.heads <= INT32_MAX;
     p.only = tc && rows == n_seqs;
-    const bool prefill = tc && !p.only && d.heads / d.kv_heads <= 128 && out->buf.off % 16 == 0;
+    const bool prefill = tc && !p.only && d.heads / d.kv_heads <= 128 && out->buf.off % 16 == 0 && rows * d.heads / 64 + n_seqs * d.kv_heads <= INT32_MAX;
     p.singles = !tc || (!p.only && n_seqs == 1);  // a lone token with rows of nobody behind it
     const Buf none{kSlotNull, 0}, q = out && !p.only ? em.scratch((size_t)rows * d.heads * d.dim * (prefill ? 2 : 4)) : none, q_mul = prefill ? em.scratch((size_t)rows * d.heads * 4) : none;
     auto launch = [&](PackKernel k, dim3 grid, unsigned block, unsigned smem, Buf part, const char* label) {

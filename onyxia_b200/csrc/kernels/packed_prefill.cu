@@ -34,6 +34,7 @@ template <int TILES, bool CAPPED> __global__ void __launch_bounds__(TILES * kRow
     // barriers: keys there, free, values there, free (one per stage), scores there, weights there, sums (two per tile, by turns), copies there, free (one per slot, keys and values by turns)
     const unsigned k_full = bars, k_free = k_full + kStages * 8, v_full = k_free + kStages * 8, v_free = v_full + kStages * 8, s_full = v_free + kStages * 8, w_full = s_full + 32, o_done = w_full + 32, raw_full = o_done + 32, raw_free = raw_full + kSlots * 8;
     unsigned* tmem_slot = reinterpret_cast<unsigned*>(smem + (raw_free + kSlots * 8 - sq0));
+    unsigned* bad_s = tmem_slot + 4;  // [stages][1 + keys]: of tiles with hidden keys, whether and which sixteen dimensions of a value are no numbers
     if (tid == 0) {
         for (unsigned b = bars; b < raw_free + kSlots * 8; b += 8) mbar_init(b, (b >= k_full && b < k_free) || (b >= v_full && b < v_free) || b >= raw_free ? kUnpack / 32 : b >= w_full && b < o_done ? kRows / 32 : 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -80,22 +81,31 @@ template <int TILES, bool CAPPED> __global__ void __launch_bounds__(TILES * kRow
     const unsigned tmem = *tmem_slot, t_sum = tmem + TILES * 2 * kKeys;  // two turns of scores of each tile; weights take their place
     const int lowest = first_key(p, pos0), kt0 = lowest / kKeys, n = last / kKeys + 1 - kt0;
     bool ok = true;
+    const int last_low = first_key(p, last);
+    auto hides = [&](int j0) { return j0 + kKeys - 1 > pos0 || j0 < last_low; };  // whether some rows do not see some keys of the tile from j0 on
 
     if (warp >= kSoftWarps && warp < kIssues) {
         // A thread has sixteen dimensions of a key at a time.
         const int u0 = tid - kSoft;
-        auto put = [&](unsigned from, unsigned base, int i, int dim, unsigned by) {
+        auto put = [&](unsigned from, unsigned base, int i, int dim, unsigned by, unsigned* bad, auto marked) {
             const int j0 = (kt0 + i) * kKeys, blocks = dim / kPack;
             const bool whole = j0 >= lowest && j0 + kKeys - 1 <= last;
             const unsigned scales = from + kKeys * (dim / 2);
             // Sixteen dimensions of a key. (The first 64 dimensions' lanes begin with the even eighths, the next with the odd ones: eight lanes write 128 bytes in different banks.)
-            auto unit = [&](unsigned codes, unsigned scale, unsigned to0, unsigned to1, unsigned first, int key) {
+            auto unit = [&](unsigned codes, unsigned scale, unsigned to0, unsigned to1, unsigned first, int key, int b) {
                 unsigned x, y, code;
                 asm volatile("ld.shared.b32 %0, [%1];" : "=r"(x) : "r"(codes + first));
                 asm volatile("ld.shared.b32 %0, [%1];" : "=r"(y) : "r"(codes + (first ^ 4)));
                 asm volatile("ld.shared.u8 %0, [%1];" : "=r"(code) : "r"(scale));
                 // keys that are not there are 0: what was copied in their place, or not, may be no number
                 if (!whole && (j0 + key < lowest || j0 + key > last)) code = 0;
+                // Nor would a weight of 0 cancel a value that is none for the rows that do not see it: where there are such, those that see it are told instead.
+                if constexpr (marked)
+                    if ((code & 127u) == 127u) {
+                        atomicOr(bad + 1 + key, 1u << b);
+                        *bad = 1;
+                        code = 0;
+                    }
                 const __half2 s = __low2half2(scales_f16(code));
                 __half2 v[4], w[4];
                 units8(x, v);
@@ -105,17 +115,17 @@ template <int TILES, bool CAPPED> __global__ void __launch_bounds__(TILES * kRow
                 asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to1), "r"(bits(__hmul2(w[0], s))), "r"(bits(__hmul2(w[1], s))), "r"(bits(__hmul2(w[2], s))), "r"(bits(__hmul2(w[3], s)))
                              : "memory");
             };
-            if ((blocks & blocks - 1) == 0) {  // a thread's units are the same dimensions of keys that lie a multiple of eight apart
+            if (!marked && (blocks & blocks - 1) == 0) {  // a thread's units are the same dimensions of keys that lie a multiple of eight apart
                 const int b = u0 & blocks - 1, key0 = over(u0, by), keys = over(kUnpack, by);
                 const unsigned flip = b >> 2 & 1, c = (b & 3) * 2 + flip, row = base + (b >> 2) * kPanel + key0 * 128, to0 = row + ((c ^ (key0 & 7)) << 4), to1 = row + ((c ^ 1 ^ (key0 & 7)) << 4);
 #pragma unroll 4
-                for (int k = 0; k + key0 < kKeys; k += keys) unit(from + (u0 + k * blocks) * 8, scales + u0 + k * blocks, to0 + k * 128, to1 + k * 128, flip * 4, k + key0);
+                for (int k = 0; k + key0 < kKeys; k += keys) unit(from + (u0 + k * blocks) * 8, scales + u0 + k * blocks, to0 + k * 128, to1 + k * 128, flip * 4, k + key0, b);
             } else {
-#pragma unroll 2
+#pragma unroll 1
                 for (int u = u0; u < kKeys * blocks; u += kUnpack) {
                     const int key = over(u, by), b = u - key * blocks;
                     const unsigned flip = b >> 2 & 1, c = (b & 3) * 2 + flip, row = base + (b >> 2) * kPanel + key * 128;
-                    unit(from + u * 8, scales + u, row + ((c ^ (key & 7)) << 4), row + ((c ^ 1 ^ (key & 7)) << 4), flip * 4, key);
+                    unit(from + u * 8, scales + u, row + ((c ^ (key & 7)) << 4), row + ((c ^ 1 ^ (key & 7)) << 4), flip * 4, key, b);
                 }
             }
         };
@@ -131,12 +141,19 @@ template <int TILES, bool CAPPED> __global__ void __launch_bounds__(TILES * kRow
         for (int i = 0; i < n; i++) {
             if (ok && !mbar_wait(raw_full + in.s * 8, in.parity)) ok = false;
             if (i >= kStages && ok && !mbar_wait(k_free + at.s * 8, at.parity ^ 1)) ok = false;
-            put(raw + in.s * slot, sk + at.s * k_stage, i, p.dim, p.by_key);
+            put(raw + in.s * slot, sk + at.s * k_stage, i, p.dim, p.by_key, nullptr, std::false_type{});
             tell(k_full + at.s * 8, raw_free + in.s * 8);
             in.next(p.raw_slots);
             if (ok && !mbar_wait(raw_full + in.s * 8, in.parity)) ok = false;
             if (i >= kStages && ok && !mbar_wait(v_free + at.s * 8, at.parity ^ 1)) ok = false;
-            put(raw + in.s * slot, sv + at.s * v_stage, i, p.vdim, p.by_value);
+            if (hides((kt0 + i) * kKeys)) {
+                unsigned* bad = bad_s + at.s * (1 + kKeys);
+                if (u0 <= kKeys) bad[u0] = 0;
+                asm volatile("bar.sync 1, 128;" ::: "memory");
+                put(raw + in.s * slot, sv + at.s * v_stage, i, p.vdim, p.by_value, bad, std::true_type{});
+            } else {
+                put(raw + in.s * slot, sv + at.s * v_stage, i, p.vdim, p.by_value, nullptr, std::false_type{});
+            }
             tell(v_full + at.s * 8, raw_free + in.s * 8);
             in.next(p.raw_slots);
             at.next(kStages);
@@ -217,18 +234,19 @@ template <int TILES, bool CAPPED> __global__ void __launch_bounds__(TILES * kRow
     } else {
         const int tile = warp / 4, tok = over(tid, p.by_rep), head = g * rep + tid - tok * rep;
         const bool live = tok < n_tok;
-        const int pos = live ? pos0 + tok : last, low = first_key(p, pos), last_low = first_key(p, last);  // rows without a token compute something harmless
+        const int pos = live ? pos0 + tok : last, low = first_key(p, pos);  // rows without a token compute something harmless
         const float mul = live ? p.q_mul[(long long)(sq.start + first + tok) * p.heads + head] : 0.f, cap2 = p.cap2, by_cap = mul * (1.f / kTwiceLog2e), series1 = cap2 * (-1.f / 3.f), series2 = cap2 * (2.f / 15.f), series3 = cap2 * (-17.f / 315.f);
         const unsigned lanes = (unsigned)((warp & 3) * 32) << 16, sum = t_sum + lanes + tile * 128;
         float m = kNone, l = 0.f, sums[4];
         const float factor = value_factor(p, g);
+        unsigned bad = 0;  // sixteen dimensions each that are no numbers
         RingAt at;
         for (int i = 0; i < n; i++) {
             const int j0 = (kt0 + i) * kKeys;
             if (ok && !mbar_wait(s_full + (2 * tile + at.s) * 8, at.parity)) ok = false;
             after_sync();
             const unsigned place = tmem + lanes + (2 * tile + at.s) * kKeys;
-            const bool edge = j0 + kKeys - 1 > pos0 || j0 < last_low;
+            const bool edge = hides(j0);
             bool near = false;
             // In base 2. Factors are positive (a negative one is in the queries): the largest score is that of the largest product.
             auto score = [&](float d) {
@@ -319,6 +337,14 @@ template <int TILES, bool CAPPED> __global__ void __launch_bounds__(TILES * kRow
                 tmem_st16(place + c / 2, w);  // where scores were that this thread has read twice
             };
             auto plainly = [](float x, int) { return x; };
+            if (edge) {
+                if (ok && !mbar_wait(v_full + i % kStages * 8, (unsigned)(i / kStages) & 1)) ok = false;
+                const unsigned* marks = bad_s + i % kStages * (1 + kKeys);
+                if (*marks)
+#pragma unroll 1
+                    for (int j = 0; j < kKeys; j++)
+                        if (!hidden(j0 + j)) bad |= marks[1 + j];
+            }
             if (edge) each([&](int c, const unsigned (&v)[32]) { weigh(c, v, std::false_type{}, [&](float x, int j) { return hidden(j) ? -INFINITY : x; }); });
             else if (CAPPED && near) each([&](int c, const unsigned (&v)[32]) { weigh(c, v, std::true_type{}, plainly); });
             else each([&](int c, const unsigned (&v)[32]) { weigh(c, v, std::false_type{}, plainly); });
@@ -331,10 +357,10 @@ template <int TILES, bool CAPPED> __global__ void __launch_bounds__(TILES * kRow
         }
         if (ok && !mbar_wait(o_done + (2 * tile + ((n - 1) & 1)) * 8, (unsigned)((n - 1) >> 1) & 1)) ok = false;
         after_sync();
-        float f = factor / l;
+        float scale = factor / l;
         if (p.sink) {
             const float top = fmaxf(m, 0.f), keep = exp2_fast(m - top);
-            f = factor * keep / (l * keep + exp2_fast(-top));
+            scale = factor * keep / (l * keep + exp2_fast(-top));
         }
         // 64 dimensions of 32 rows at a time by way of shared memory, where the queries were, so that eight lanes write a row's 128 bytes
         unsigned char* mine = smem + tile * kp * kPanelQ + (warp & 3) * 32 * 128;
@@ -347,6 +373,7 @@ template <int TILES, bool CAPPED> __global__ void __launch_bounds__(TILES * kRow
 #pragma unroll
             for (int e = 0; e < 8; e++) {
                 const unsigned* x = v[e / 4] + e % 4 * 8;
+                const float f = bad >> (c / kPack + e / 2) & 1 ? __int_as_float(0x7FFFFFFF) : scale;
                 uint4 q;
                 q.x = pack_bf16(__uint_as_float(x[0]) * f, __uint_as_float(x[1]) * f);
                 q.y = pack_bf16(__uint_as_float(x[2]) * f, __uint_as_float(x[3]) * f);
@@ -373,7 +400,7 @@ template <int TILES, bool CAPPED> __global__ void __launch_bounds__(TILES * kRow
 // Bytes without the slots of copies
 int smem_of(int dim, int vdim, int tiles) {
     const int kp = (dim + 63) / 64, vp = (vdim + 63) / 64;
-    return 1024 + tiles * kp * (int)kPanelQ + kStages * (kp + vp) * (int)kPanel + (4 * kStages + 12 + 2 * kSlots) * 8 + 16;
+    return 1024 + tiles * kp * (int)kPanelQ + kStages * (kp + vp) * (int)kPanel + (4 * kStages + 12 + 2 * kSlots) * 8 + 16 + kStages * (1 + kKeys) * 4;
 }
 
 }  // namespace

@@ -72,7 +72,7 @@ def check(f, lengths, kind, seed=0, form="attend", **more):
 
 LAYOUTS = [Form(4, 1, 128, 256, 128), Form(16, 4, 64, 128, 64), Form(6, 2, 32, 64, 16), Form(5, 5, 48, 48, 48), Form(3, 1, 80, 160, 40), Form(20, 2, 64, 64, 0), Form(2, 1, 16, 32, 8),
            Form(3, 3, 16, 16, 6), Form(9, 1, 16, 32, 16), Form(1, 1, 256, 256, 256), Form(2, 2, 272, 144, 8), Form(8, 8, 112, 96, 112, gap=8), Form(4, 2, 64, 128, 32, gap=3), Form(34, 2, 96, 80, 96),
-           Form(4, 4, 128, 128, 128, factors=1), Form(12, 1, 192, 64, 64, factors=1)]
+           Form(4, 4, 128, 128, 128, factors=1), Form(12, 1, 192, 64, 64, factors=1), Form(130, 1, 16, 32, 16)]
 
 
 @BOTH
@@ -180,6 +180,32 @@ def test_values_that_are_no_numbers_are_stored_as_such(kind):
     got = session.download(outs["stored"]).numpy()
     assert np.array_equal(np.isnan(got), np.isnan(want)) and np.isnan(want).sum() == 32
     assert np.array_equal(got[~np.isnan(got)], rounded(kind)(want.astype(np.float32))[~np.isnan(got)])
+
+
+@BOTH
+@pytest.mark.parametrize("f", [Form(4, 2, 64, 96, 32), Form(8, 8, 128, 128, 128, window=40), Form(40, 8, 128, 64, 0, page=16), Form(2, 1, 256, 256, 256)], ids=lambda f: f"{f.heads}x{f.kv_heads}x{f.dim}x{f.vdim}")
+def test_what_is_no_number_reaches_the_rows_that_see_it(f, kind):
+    """A key that is none: the rows of its head that see it. Sixteen dimensions of a value: these of the same rows. Rows before them, behind the window, and other heads are as without."""
+    lengths = [(150, 20), (1, 130), (70, 0), (1, 20)]
+    s = util.step(f, lengths, 3, round_to=rounded(kind))
+    _, k0, v0 = f.offsets
+    g = f.kv_heads - 1
+    s.proj[60, v0 + g * f.vdim + 17] = np.nan    # token 60 of the first sequence: position 80
+    s.proj[131, k0 + g * f.dim + 3] = np.nan     # token 131: position 151
+    session, _, outs = run(f, s, kind)
+    pools = util.written(f, s, rounded(kind))
+    assert np.array_equal(session.download(outs["updated.pages.values"]).numpy(), pools[1])
+    got, live = session.download(outs["out"]).numpy().reshape(len(s.proj), f.heads, f.vdim), rows_of(s)
+    want = np.zeros(got.shape, bool)
+    rep, w = f.heads // f.kv_heads, f.window or 10 ** 6
+    want[60:min(150, 60 + w), g * rep:(g + 1) * rep, 16:32] = True
+    want[131:min(150, 131 + w), g * rep:(g + 1) * rep] = True
+    assert np.array_equal(np.isnan(got[live]), want[live])
+    s.proj[60, v0 + g * f.vdim + 17] = s.proj[131, k0 + g * f.dim + 3] = 0.0
+    other = util.reference(f, s, util.written(f, s, rounded(kind))).reshape(got.shape)
+    seen = want.any(2)[live]
+    off = np.sqrt(((got[live] - other[live]) ** 2).sum(2)) / np.sqrt((other[live] ** 2).sum(2))
+    assert off[~seen].max() <= (2 ** -8 + 3 * 2 ** -10 if kind == "bf16" else 1e-5)
 
 
 @BOTH

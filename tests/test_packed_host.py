@@ -103,7 +103,7 @@ def test_forms_that_are_refused(taken, kind, changed):
 
 @pytest.mark.parametrize("kind", ["attend", "shared", "write", "read"])
 def test_sizes_and_factors_that_are_refused(taken, kind):
-    for f in (Form(1, 1, 24, 16), Form(1, 1, 16, 40), Form(1, 1, 8208, 16), Form(1, 1, 16, 8208), Form(512, 512, 4096, 4112), Form(4, 2, 64, 64, page=8), Form(4, 2, 64, 64, page=1)):
+    for f in (Form(1, 1, 24, 16), Form(1, 1, 16, 40), Form(1, 1, 8208, 16), Form(1, 1, 16, 8208), Form(512, 512, 4096, 4112), Form(4, 2, 64, 64, page=8), Form(1, 1, 16, 2048, page=1 << 20), Form(1, 1, 16, 16, page=1 << 21), Form(4, 2, 64, 64, page=1)):
         assert taken(f, kind=kind) == 0
     f = Form(4, 2, 64, 64, factors=1)
     for bad in (0.0, -1.0, np.inf, np.nan, 1e-31, 1e31):

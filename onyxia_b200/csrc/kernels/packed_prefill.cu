@@ -24,6 +24,20 @@ __device__ __forceinline__ float exp2_fast(float x) {
     return y;
 }
 
+__device__ __forceinline__ unsigned ld_shared(unsigned at) {
+    unsigned v;
+    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+    return v;
+}
+
+__device__ __forceinline__ unsigned ld_shared_u8(unsigned at) {
+    unsigned v;
+    asm volatile("ld.shared.u8 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+    return v;
+}
+
+__device__ __forceinline__ void st_shared(unsigned at, unsigned v) { asm volatile("st.shared.b32 [%0], %1;" ::"r"(at), "r"(v) : "memory"); }
+
 template <int TILES, bool CAPPED> __global__ void __launch_bounds__(TILES * kRows + kUnpack + 64, TILES == 1 ? 2 : 1) packed_prefill(const PackP p) {
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
@@ -34,7 +48,8 @@ template <int TILES, bool CAPPED> __global__ void __launch_bounds__(TILES * kRow
     // barriers: keys there, free, values there, free (one per stage), scores there, weights there, sums (two per tile, by turns), copies there, free (one per slot, keys and values by turns)
     const unsigned k_full = bars, k_free = k_full + kStages * 8, v_full = k_free + kStages * 8, v_free = v_full + kStages * 8, s_full = v_free + kStages * 8, w_full = s_full + 32, o_done = w_full + 32, raw_full = o_done + 32, raw_free = raw_full + kSlots * 8;
     unsigned* tmem_slot = reinterpret_cast<unsigned*>(smem + (raw_free + kSlots * 8 - sq0));
-    unsigned* bad_s = tmem_slot + 4;  // [stages][1 + keys]: of tiles with hidden keys, whether and which sixteen dimensions of a value are no numbers
+    // Which sixteen dimensions are no numbers: of the rows' results, [rows]; of the values of tiles with hidden keys, [stages][1 + keys], behind whether there are any.
+    const unsigned row_bad = raw_free + kSlots * 8 + 16, value_bad = row_bad + TILES * kRows * 4;
     if (tid == 0) {
         for (unsigned b = bars; b < raw_free + kSlots * 8; b += 8) mbar_init(b, (b >= k_full && b < k_free) || (b >= v_full && b < v_free) || b >= raw_free ? kUnpack / 32 : b >= w_full && b < o_done ? kRows / 32 : 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -87,25 +102,18 @@ template <int TILES, bool CAPPED> __global__ void __launch_bounds__(TILES * kRow
     if (warp >= kSoftWarps && warp < kIssues) {
         // A thread has sixteen dimensions of a key at a time.
         const int u0 = tid - kSoft;
-        auto put = [&](unsigned from, unsigned base, int i, int dim, unsigned by, unsigned* bad, auto marked) {
+        auto put = [&](unsigned from, unsigned base, int i, int dim, unsigned by) {
             const int j0 = (kt0 + i) * kKeys, blocks = dim / kPack;
             const bool whole = j0 >= lowest && j0 + kKeys - 1 <= last;
             const unsigned scales = from + kKeys * (dim / 2);
             // Sixteen dimensions of a key. (The first 64 dimensions' lanes begin with the even eighths, the next with the odd ones: eight lanes write 128 bytes in different banks.)
-            auto unit = [&](unsigned codes, unsigned scale, unsigned to0, unsigned to1, unsigned first, int key, int b) {
+            auto unit = [&](unsigned codes, unsigned scale, unsigned to0, unsigned to1, unsigned first, int key) {
                 unsigned x, y, code;
-                asm volatile("ld.shared.b32 %0, [%1];" : "=r"(x) : "r"(codes + first));
-                asm volatile("ld.shared.b32 %0, [%1];" : "=r"(y) : "r"(codes + (first ^ 4)));
-                asm volatile("ld.shared.u8 %0, [%1];" : "=r"(code) : "r"(scale));
+                x = ld_shared(codes + first);
+                y = ld_shared(codes + (first ^ 4));
+                code = ld_shared_u8(scale);
                 // keys that are not there are 0: what was copied in their place, or not, may be no number
                 if (!whole && (j0 + key < lowest || j0 + key > last)) code = 0;
-                // Nor would a weight of 0 cancel a value that is none for the rows that do not see it: where there are such, those that see it are told instead.
-                if constexpr (marked)
-                    if ((code & 127u) == 127u) {
-                        atomicOr(bad + 1 + key, 1u << b);
-                        *bad = 1;
-                        code = 0;
-                    }
                 const __half2 s = __low2half2(scales_f16(code));
                 __half2 v[4], w[4];
                 units8(x, v);
@@ -115,19 +123,32 @@ template <int TILES, bool CAPPED> __global__ void __launch_bounds__(TILES * kRow
                 asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to1), "r"(bits(__hmul2(w[0], s))), "r"(bits(__hmul2(w[1], s))), "r"(bits(__hmul2(w[2], s))), "r"(bits(__hmul2(w[3], s)))
                              : "memory");
             };
-            if (!marked && (blocks & blocks - 1) == 0) {  // a thread's units are the same dimensions of keys that lie a multiple of eight apart
+            if ((blocks & blocks - 1) == 0) {  // a thread's units are the same dimensions of keys that lie a multiple of eight apart
                 const int b = u0 & blocks - 1, key0 = over(u0, by), keys = over(kUnpack, by);
                 const unsigned flip = b >> 2 & 1, c = (b & 3) * 2 + flip, row = base + (b >> 2) * kPanel + key0 * 128, to0 = row + ((c ^ (key0 & 7)) << 4), to1 = row + ((c ^ 1 ^ (key0 & 7)) << 4);
 #pragma unroll 4
-                for (int k = 0; k + key0 < kKeys; k += keys) unit(from + (u0 + k * blocks) * 8, scales + u0 + k * blocks, to0 + k * 128, to1 + k * 128, flip * 4, k + key0, b);
+                for (int k = 0; k + key0 < kKeys; k += keys) unit(from + (u0 + k * blocks) * 8, scales + u0 + k * blocks, to0 + k * 128, to1 + k * 128, flip * 4, k + key0);
             } else {
-#pragma unroll 1
+#pragma unroll 2
                 for (int u = u0; u < kKeys * blocks; u += kUnpack) {
                     const int key = over(u, by), b = u - key * blocks;
                     const unsigned flip = b >> 2 & 1, c = (b & 3) * 2 + flip, row = base + (b >> 2) * kPanel + key * 128;
-                    unit(from + u * 8, scales + u, row + ((c ^ (key & 7)) << 4), row + ((c ^ 1 ^ (key & 7)) << 4), flip * 4, key, b);
+                    unit(from + u * 8, scales + u, row + ((c ^ (key & 7)) << 4), row + ((c ^ 1 ^ (key & 7)) << 4), flip * 4, key);
                 }
             }
+        };
+        // A weight of 0 does not cancel a value that is no number for the rows that do not see it: where there are such, it becomes 0, and the rows that see it are told.
+        auto mark = [&](unsigned scales, unsigned bad) {
+            if (u0 <= kKeys) st_shared(bad + u0 * 4, 0);
+            asm volatile("bar.sync 1, 128;" ::: "memory");
+            for (int u = u0; u < kKeys * (p.vdim / kPack); u += kUnpack)
+                if ((ld_shared_u8(scales + u) & 127) == 127) {
+                    const int key = over(u, p.by_value);
+                    asm volatile("red.shared.or.b32 [%0], %1;" ::"r"(bad + 4 + key * 4), "r"(1u << (u - key * (p.vdim / kPack))) : "memory");
+                    st_shared(bad, 1);
+                    asm volatile("st.shared.u8 [%0], %1;" ::"r"(scales + u), "r"(0) : "memory");
+                }
+            asm volatile("bar.sync 1, 128;" ::: "memory");
         };
         auto tell = [&](unsigned there, unsigned free) {
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -141,19 +162,13 @@ template <int TILES, bool CAPPED> __global__ void __launch_bounds__(TILES * kRow
         for (int i = 0; i < n; i++) {
             if (ok && !mbar_wait(raw_full + in.s * 8, in.parity)) ok = false;
             if (i >= kStages && ok && !mbar_wait(k_free + at.s * 8, at.parity ^ 1)) ok = false;
-            put(raw + in.s * slot, sk + at.s * k_stage, i, p.dim, p.by_key, nullptr, std::false_type{});
+            put(raw + in.s * slot, sk + at.s * k_stage, i, p.dim, p.by_key);
             tell(k_full + at.s * 8, raw_free + in.s * 8);
             in.next(p.raw_slots);
             if (ok && !mbar_wait(raw_full + in.s * 8, in.parity)) ok = false;
             if (i >= kStages && ok && !mbar_wait(v_free + at.s * 8, at.parity ^ 1)) ok = false;
-            if (hides((kt0 + i) * kKeys)) {
-                unsigned* bad = bad_s + at.s * (1 + kKeys);
-                if (u0 <= kKeys) bad[u0] = 0;
-                asm volatile("bar.sync 1, 128;" ::: "memory");
-                put(raw + in.s * slot, sv + at.s * v_stage, i, p.vdim, p.by_value, bad, std::true_type{});
-            } else {
-                put(raw + in.s * slot, sv + at.s * v_stage, i, p.vdim, p.by_value, nullptr, std::false_type{});
-            }
+            if (hides((kt0 + i) * kKeys)) mark(raw + in.s * slot + kKeys * (p.vdim / 2), value_bad + at.s * (1 + kKeys) * 4);
+            put(raw + in.s * slot, sv + at.s * v_stage, i, p.vdim, p.by_value);
             tell(v_full + at.s * 8, raw_free + in.s * 8);
             in.next(p.raw_slots);
             at.next(kStages);
@@ -239,7 +254,7 @@ template <int TILES, bool CAPPED> __global__ void __launch_bounds__(TILES * kRow
         const unsigned lanes = (unsigned)((warp & 3) * 32) << 16, sum = t_sum + lanes + tile * 128;
         float m = kNone, l = 0.f, sums[4];
         const float factor = value_factor(p, g);
-        unsigned bad = 0;  // sixteen dimensions each that are no numbers
+        st_shared(row_bad + tid * 4, 0);
         RingAt at;
         for (int i = 0; i < n; i++) {
             const int j0 = (kt0 + i) * kKeys;
@@ -254,26 +269,15 @@ template <int TILES, bool CAPPED> __global__ void __launch_bounds__(TILES * kRow
                 return CAPPED ? cap2 - __fdividef(2.f * cap2, 1.f + exp2_fast(x)) : x;
             };
             auto hidden = [&](int j) { return j > pos || j < low; };
-            // 32 products at a time. Two tiles' threads have the registers to keep them all; otherwise they are read twice, the next ones on their way.
-            unsigned all[TILES == 2 ? kKeys : 64];
-            if constexpr (TILES == 2) {
-#pragma unroll
-                for (int c = 0; c < kKeys; c += 32) tmem_ld32(*reinterpret_cast<unsigned(*)[32]>(all + c), place + c);
-                tmem_ld_wait();
-            }
+            // 32 products at a time, the next ones on their way
             auto each = [&](auto&& take) {
-                if constexpr (TILES == 2) {
+                unsigned v[2][32];
+                tmem_ld32(v[0], place);
 #pragma unroll
-                    for (int c = 0; c < kKeys; c += 32) take(c, *reinterpret_cast<const unsigned(*)[32]>(all + c));
-                } else {
-                    unsigned(&v)[2][32] = *reinterpret_cast<unsigned(*)[2][32]>(all);
-                    tmem_ld32(v[0], place);
-#pragma unroll
-                    for (int c = 0; c < kKeys / 32; c++) {
-                        tmem_ld_wait();
-                        if (c + 1 < kKeys / 32) tmem_ld32(v[(c + 1) & 1], place + (c + 1) * 32);
-                        take(c * 32, v[c & 1]);
-                    }
+                for (int c = 0; c < kKeys / 32; c++) {
+                    tmem_ld_wait();
+                    if (c + 1 < kKeys / 32) tmem_ld32(v[(c + 1) & 1], place + (c + 1) * 32);
+                    take(c * 32, v[c & 1]);
                 }
             };
             float top = -INFINITY, least = INFINITY;
@@ -339,11 +343,14 @@ template <int TILES, bool CAPPED> __global__ void __launch_bounds__(TILES * kRow
             auto plainly = [](float x, int) { return x; };
             if (edge) {
                 if (ok && !mbar_wait(v_full + i % kStages * 8, (unsigned)(i / kStages) & 1)) ok = false;
-                const unsigned* marks = bad_s + i % kStages * (1 + kKeys);
-                if (*marks)
+                const unsigned marks = value_bad + i % kStages * (1 + kKeys) * 4;
+                if (ld_shared(marks)) {
+                    unsigned bad = ld_shared(row_bad + tid * 4);
 #pragma unroll 1
                     for (int j = 0; j < kKeys; j++)
-                        if (!hidden(j0 + j)) bad |= marks[1 + j];
+                        if (!hidden(j0 + j)) bad |= ld_shared(marks + 4 + j * 4);
+                    st_shared(row_bad + tid * 4, bad);
+                }
             }
             if (edge) each([&](int c, const unsigned (&v)[32]) { weigh(c, v, std::false_type{}, [&](float x, int j) { return hidden(j) ? -INFINITY : x; }); });
             else if (CAPPED && near) each([&](int c, const unsigned (&v)[32]) { weigh(c, v, std::true_type{}, plainly); });
@@ -370,15 +377,19 @@ template <int TILES, bool CAPPED> __global__ void __launch_bounds__(TILES * kRow
             tmem_ld32(v[0], sum + c);
             tmem_ld32(v[1], sum + c + 32);
             tmem_ld_wait();
+            const unsigned bad = ld_shared(row_bad + tid * 4) >> c / kPack & 15;
+            if (bad)
+#pragma unroll
+                for (int e = 0; e < 64; e++)
+                    if (bad >> e / kPack & 1) v[e / 32][e % 32] = 0x7FFFFFFF;
 #pragma unroll
             for (int e = 0; e < 8; e++) {
                 const unsigned* x = v[e / 4] + e % 4 * 8;
-                const float f = bad >> (c / kPack + e / 2) & 1 ? __int_as_float(0x7FFFFFFF) : scale;
                 uint4 q;
-                q.x = pack_bf16(__uint_as_float(x[0]) * f, __uint_as_float(x[1]) * f);
-                q.y = pack_bf16(__uint_as_float(x[2]) * f, __uint_as_float(x[3]) * f);
-                q.z = pack_bf16(__uint_as_float(x[4]) * f, __uint_as_float(x[5]) * f);
-                q.w = pack_bf16(__uint_as_float(x[6]) * f, __uint_as_float(x[7]) * f);
+                q.x = pack_bf16(__uint_as_float(x[0]) * scale, __uint_as_float(x[1]) * scale);
+                q.y = pack_bf16(__uint_as_float(x[2]) * scale, __uint_as_float(x[3]) * scale);
+                q.z = pack_bf16(__uint_as_float(x[4]) * scale, __uint_as_float(x[5]) * scale);
+                q.w = pack_bf16(__uint_as_float(x[6]) * scale, __uint_as_float(x[7]) * scale);
                 *reinterpret_cast<uint4*>(mine + lane * 128 + ((e ^ (lane & 7)) << 4)) = q;
             }
             __syncwarp();
@@ -400,7 +411,7 @@ template <int TILES, bool CAPPED> __global__ void __launch_bounds__(TILES * kRow
 // Bytes without the slots of copies
 int smem_of(int dim, int vdim, int tiles) {
     const int kp = (dim + 63) / 64, vp = (vdim + 63) / 64;
-    return 1024 + tiles * kp * (int)kPanelQ + kStages * (kp + vp) * (int)kPanel + (4 * kStages + 12 + 2 * kSlots) * 8 + 16 + kStages * (1 + kKeys) * 4;
+    return 1024 + tiles * kp * (int)kPanelQ + kStages * (kp + vp) * (int)kPanel + (4 * kStages + 12 + 2 * kSlots) * 8 + 16 + kStages * (1 + kKeys) * 4 + tiles * kRows * 4;
 }
 
 }  // namespace

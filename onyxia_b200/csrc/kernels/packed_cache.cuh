@@ -78,8 +78,8 @@ __device__ __forceinline__ float scale_value(unsigned code) { return __low2float
 // A value over its scale; 0 where that is 0 or no number.
 __device__ __forceinline__ float over_scale(float y, float scale) { return scale > 0.f ? y / scale : 0.f; }
 // The same for a value of eight significant bits (bf16), by the scale's reciprocal `by`: y / scale is halfway between two codes (a multiple of 1/4 up to 5), or 2^-10 away from it and more. The sum
-// with 3072 rounds to a multiple of 2^-12: what is halfway comes out so, the rest stays on its side.
-__device__ __forceinline__ float near_scale(float y, float by) { return __fadd_rn(__fmaf_rn(y, by, 3072.f), -3072.f); }
+// with 2560 rounds to a multiple of 2^-12: what is halfway comes out so, the rest stays on its side.
+__device__ __forceinline__ float near_scale(float y, float by) { return __fadd_rn(__fmaf_rn(y, by, 2560.f), -2560.f); }
 __device__ __forceinline__ unsigned without_signs_of_0(unsigned codes) { return codes & (0x77777777u | (((codes & 0x77777777u) + 0x77777777u) & 0x88888888u)); }
 // Eight values over their scale as codes, the first one lowest.
 __device__ __forceinline__ unsigned codes8(const float (&r)[8]) {

@@ -3,6 +3,14 @@
 // A CTA owns one or two tiles of 128 (token, head) rows of one key head and walks over their keys, 64 at a time. One warp copies what the pages hold of them, several steps ahead; four warps turn
 // codes into f16 (exactly: packed_cache.cuh), a step ahead of the products; one warp issues these; a thread per row masks and weighs scores. The next 64 keys' scores are made meanwhile: a tile has two turns of them. Two tiles share what is
 // unpacked.
+//
+// A row's softmax is taken in one pass: m, l and the sums of values against a maximum that may lie up to 8 (in base 2) behind. Queries are f16 times a power of two of their own, weights f16 (either
+// off by 2^-12 of itself), all sums f32.
+//
+// What bounds it: 4096 tokens of 32 heads of 128 over 16 take 189 us, 730 TFLOP/s of 4 · 128 operations per pair (at a plain matrix product's rate 83 us). Of a step's 2430 cycles (two tiles, 64 keys)
+// the products take 1900, since a product with 64 keys reads 128 queries from shared memory for half the columns, and the issuing warp waits for weights the other 530. Scores of 128 keys would leave
+// tensor memory no place for the next ones beside two tiles' sums. Copies, codes and conversions lie under the products, in 54 % of the issue slots. 1999 tokens behind 1000, capped and normed, of 16
+// heads of 128 over 4: 103 us (20): one tile per CTA, two of them in an SM, and the last tiles' chain over 47 steps.
 #include <type_traits>
 
 #include "packed_cache.cuh"
@@ -417,6 +425,8 @@ int smem_of(int dim, int vdim, int tiles) {
 }  // namespace
 
 PackedPrefill packed_prefill_of(int64_t dim, int64_t vdim, int64_t rows, int64_t kv_heads, int64_t rep, bool capped) {
+    // Two tiles share what is unpacked: 4096 tokens of 32 heads over 16 take 191 us, with one per CTA 229. They have to fill the device twice, or its SMs wait for the longest: 1999 behind 1000 of 16
+    // heads over 4 take 119 us with two, 112 with one.
     const int tiles = dim <= 128 && vdim <= 128 && (rows * rep + 2 * kRows - 1) / (2 * kRows) * kv_heads >= 2 * sm_count() ? 2 : 1;
     const PackKernel k = tiles == 2 ? (capped ? packed_prefill<2, true> : packed_prefill<2, false>) : capped ? packed_prefill<1, true> : packed_prefill<1, false>;
     // With 512 columns of tensor memory a CTA has its SM alone, with 256 it shares it with one other.

@@ -89,9 +89,20 @@ template <bool ALL, bool NORM> __global__ void __launch_bounds__(128, 8) packed_
     for (int i = tid; i < half; i += 128) short_angle(pos, (double)p.turns[i] + (double)p.turns[half + i], cs + i, sn + i);
     const int turned = half / 8, units = p.dim / 8 - turned, runs = p.vdim / 8, eighths = p.dim / 8;
     if (NORM)
-        for (int h = tid >> 5; h < p.heads + kv; h += 4) {
-            const double f = norm_factor(p, h < p.heads ? from_q + h * p.dim : from_k + (h - p.heads) * p.dim);
-            if ((tid & 31) == 0) (h < p.heads ? (void)(query_norm[h] = (float)f) : (void)(norms[h - p.heads] = f));
+        for (int h0 = tid >> 5; h0 < p.heads + kv; h0 += 4 * 32) {  // a warp sums up to 32 heads, then has a root and a quotient for each lane
+            const int h = h0 + 4 * (tid & 31);
+            double mine = 0.0;
+#pragma unroll 4
+            for (int j = 0; j < 32; j++) {
+                const int other = h0 + 4 * j;
+                if (other >= p.heads + kv) break;
+                const double ss = square_sum(p, other < p.heads ? from_q + other * p.dim : from_k + (other - p.heads) * p.dim);
+                if (j == (tid & 31)) mine = ss;
+            }
+            if (h < p.heads + kv) {
+                const double f = norm_of(p, mine);
+                h < p.heads ? (void)(query_norm[h] = (float)f) : (void)(norms[h - p.heads] = f);
+            }
         }
     auto wide = [](const bf16* from, float (&v)[8]) {
         const uint4 u = *reinterpret_cast<const uint4*>(from);

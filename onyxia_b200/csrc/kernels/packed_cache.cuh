@@ -173,15 +173,16 @@ template <typename T> __device__ __forceinline__ double turned(int half, const T
     if (i >= 2 * half) return v;
     return i < half ? v * cs[i] - (double)to_f(x[i + half]) * sn[i] : v * cs[i - half] + (double)to_f(x[i - half]) * sn[i - half];
 }
-// 1 / root mean square of a query or key in 64 bits, by one warp
-template <typename T> __device__ __forceinline__ double norm_factor(const PackP& p, const T* x) {
-    if (!p.norm) return 1.0;
+// The sum of squares of a query or key in 64 bits, by one warp, and 1 / root mean square
+template <typename T> __device__ __forceinline__ double square_sum(const PackP& p, const T* x) {
     double ss = 0.0;
     for (int i = threadIdx.x & 31; i < p.dim; i += 32) ss += (double)to_f(x[i]) * (double)to_f(x[i]);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    return 1.0 / sqrt(ss / p.dim + p.eps);
+    return ss;
 }
+__device__ __forceinline__ double norm_of(const PackP& p, double ss) { return 1.0 / sqrt(ss / p.dim + p.eps); }
+template <typename T> __device__ __forceinline__ double norm_factor(const PackP& p, const T* x) { return p.norm ? norm_of(p, square_sum(p, x)) : 1.0; }
 
 // The power of two that brings the largest element of a query, `top`, next to 1, as its exponent field: queries are f16 times it, so that none is too large and what is rounded is 2^-12 of an element.
 __device__ __forceinline__ int query_exponent(float top) { return min(max((int)(__float_as_uint(top) >> 23), 1), 253); }

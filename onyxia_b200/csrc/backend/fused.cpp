@@ -674,7 +674,8 @@ void differential_lower(FusedCtx& c) {
 //   SharedPackedKVAttention  the same, to what another node has put into the pools → out
 //   CacheWrite               the same without queries → keys, values
 //   CacheRead                keys, values, places, pages [, factors × 2] → keys and values side by side
-// The other attributes are those of onyxia.PagedKVAttention.
+// The other attributes are q_offset, k_offset, v_offset, rot_dims, window, scale, softcap, norm, epsilon and sink, as in onyxia.PagedKVAttention. What else that one has is refused: pairs that turn
+// side by side (interleaved), gates, learned sinks, temperatures, mixed heads.
 bool packed_sizes_fit(const Module& m, const Node& n, size_t pools) {
     const Attrs& a = n.composite.attrs;
     const int64_t G = a.int_or("kv_heads", 0), D = a.int_or("dim", 0), V = a.int_or("vdim", 0);
@@ -705,6 +706,8 @@ bool packed_fits(const Module& m, const Node& n, PackedForm form) {
     const int64_t H = a.int_or("heads", 0), G = a.int_or("kv_heads", 0), D = a.int_or("dim", 0), V = a.int_or("vdim", 0), R = a.int_or("rot_dims", 0);
     if ((queries && (H <= 0 || H > 65535 || H % G != 0 || H * std::max(D, V) > 1 << 22)) || R < 0 || R > D || R % 2 != 0) return false;
     if (a.int_or("window", 0) < 0 || a.int_or("window", 0) > INT32_MAX) return false;
+    for (const char* other : {"interleaved", "gate", "sinks", "temps", "talk"})
+        if (a.int_or(other, 0) != 0) return false;
     for (const char* f : {"softcap", "epsilon"})
         if (!(a.float_or(f, 0.0) >= 0.0) || !std::isfinite(a.float_or(f, 0.0))) return false;
     // (in f32, and in the quotient that scores are multiplied by, too)

@@ -188,6 +188,11 @@ template <typename T> __device__ __forceinline__ double norm_factor(const PackP&
 __device__ __forceinline__ int query_exponent(float top) { return min(max((int)(__float_as_uint(top) >> 23), 1), 253); }
 __device__ __forceinline__ float power_down(int e) { return __uint_as_float((unsigned)(254 - e) << 23); }
 __device__ __forceinline__ float power_up(int e) { return __uint_as_float((unsigned)e << 23); }
+// Weights of a softmax are f16 against a reference that the largest score so far lies kLeast to kMost above (in base 2): a sum of values is rescaled where it moves, which is dear. Down to
+// 2^-(14 + kLeast) of the largest weight f16 holds 11 bits of them, below it has steps of 2^-(24 + kLeast) of that: a first key that has nearly all weight, and a value that adds little, leaves the others
+// what they are. (A weight of 2^16 would be infinite: what moves the reference, and where to, is rounded so that none gets beyond 2^kMost.) A
+// closer reference costs prompts more moves: 4096 tokens of 32 heads over 16 take 187 us with 8, 194 with 11, 206 with 13.
+constexpr float kLeast = 8.f, kMost = 15.f;
 // 32 values of a head by one warp, the lane's `value` dimension c + lane: codes and scales to where they are held. Values from n on are nobody's.
 __device__ __forceinline__ void put_32(unsigned char* codes, unsigned char* scales, int c, int n, float factor, float value) {
     const int lane = threadIdx.x & 31, i = c + lane;

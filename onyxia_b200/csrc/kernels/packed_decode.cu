@@ -325,7 +325,7 @@ template <int KS, int VC, bool WHOLE, int RESIDENT> __global__ void __launch_bou
         const float mul[2] = {factor_s[2 * t4], factor_s[2 * t4 + 1]};
         const bool capped = p.cap2 > 0.f;
         const float weigh[2] = {capped ? 1.f : mul[0], capped ? 1.f : mul[1]}, back[2] = {1.f / weigh[0], 1.f / weigh[1]};
-        // `most`: what a score may be until the weights are taken against another maximum, before it is multiplied; `l`: sums of the weights, by a product with ones
+        // `top`: what weights are taken against; `most`: what a score may be until that moves, before it is multiplied; `l`: sums of the weights, by a product with ones
         float o[VC][4], l[4] = {0.f, 0.f, 0.f, 0.f}, top[2] = {kNone, kNone}, most[2] = {kNone, kNone};
 #pragma unroll
         for (int n = 0; n < VC; n++)
@@ -400,17 +400,17 @@ template <int KS, int VC, bool WHOLE, int RESIDENT> __global__ void __launch_bou
 #pragma unroll
                 for (int e = 0; e < 4; e++) above |= s[half][e] > most[e & 1];
             }
-            // Weights are taken against a maximum that the largest score is up to 8 above: f16 holds 2^8 as exactly as 1, and 2^-22 of the largest weight with all its bits.
             if (__any_sync(0xffffffffu, above)) {
 #pragma unroll
                 for (int e = 0; e < 2; e++) {
                     float now = fmaxf(fmaxf(s[0][e], s[0][e + 2]), fmaxf(s[1][e], s[1][e + 2]));
 #pragma unroll
                     for (int d = 4; d < 32; d <<= 1) now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, d));
-                    now = now > -INFINITY ? fmaxf(top[e], now * weigh[e]) : top[e];
+                    now = now > -INFINITY ? fmaxf(top[e], __fsub_ru(__fmul_ru(now, weigh[e]), kLeast)) : top[e];
                     const float keep = exp2_fast(top[e] - now);
                     top[e] = now;
-                    most[e] = now > kNone ? (now + 8.f) * back[e] : kNone;
+                    const float beyond = (now + kMost) * back[e];
+                    most[e] = now > kNone ? __fmaf_rn(fabsf(beyond), -0x1p-21f, beyond) : kNone;  // (three roundings, 2^-24 of it each)
                     l[e] *= keep;
                     l[e + 2] *= keep;
 #pragma unroll

@@ -4,8 +4,8 @@
 // codes into f16 (exactly: packed_cache.cuh), a step ahead of the products; one warp issues these; a thread per row masks and weighs scores. The next 64 keys' scores are made meanwhile: a tile has two turns of them. Two tiles share what is
 // unpacked.
 //
-// A row's softmax is taken in one pass: m, l and the sums of values against a maximum that may lie up to 8 (in base 2) behind. Queries are f16 times a power of two of their own, weights f16 (either
-// off by 2^-12 of itself), all sums f32.
+// A row's softmax is taken in one pass: m, l and the sums of values against a reference below the maximum (kLeast, kMost: packed_cache.cuh). Queries are f16 times a power of two of their own, weights f16,
+// all sums f32.
 //
 // What bounds it: 4096 tokens of 32 heads of 128 over 16 take 189 us, 730 TFLOP/s of 4 · 128 operations per pair (at a plain matrix product's rate 83 us). Of a step's 2430 cycles (two tiles, 64 keys)
 // the products take 1900, since a product with 64 keys reads 128 queries from shared memory for half the columns, and the issuing warp waits for weights the other 530. Scores of 128 keys would leave
@@ -276,6 +276,7 @@ template <int TILES, bool CAPPED> __global__ void __launch_bounds__(TILES * kRow
                 const float x = d * mul;
                 return CAPPED ? cap2 - __fdividef(2.f * cap2, 1.f + exp2_fast(x)) : x;
             };
+            auto largest = [&](float d) { return CAPPED ? score(d) : __fmul_ru(d, mul); };
             auto hidden = [&](int j) { return j > pos || j < low; };
             // 32 products at a time, the next ones on their way
             auto each = [&](auto&& take) {
@@ -294,7 +295,7 @@ template <int TILES, bool CAPPED> __global__ void __launch_bounds__(TILES * kRow
 #pragma unroll
                     for (int e = 0; e < 32; e++) top = fmaxf(top, hidden(j0 + c + e) ? -INFINITY : __uint_as_float(v[e]));
                 });
-                if (top != -INFINITY) top = score(top);
+                if (top != -INFINITY) top = largest(top);
             } else {
                 each([&](int c, const unsigned (&v)[32]) {
 #pragma unroll
@@ -305,11 +306,10 @@ template <int TILES, bool CAPPED> __global__ void __launch_bounds__(TILES * kRow
                 });
                 // tanh u = u (1 - u²/3 + 2u⁴/15 - 17u⁶/315 + 62u⁸/2835 - ...): where no score that the warp's rows see is beyond a quarter of the cap, what is left out is 4e-7 of it.
                 if (CAPPED) near = __all_sync(0xffffffffu, fmaxf(fabsf(top), fabsf(least)) * mul <= 0.25f * kTwiceLog2e);
-                top = score(top);
+                top = largest(top);
             }
-            // Weights are taken against a maximum that the largest score is up to 8 above: f16 holds 2^8 as exactly as 1.
-            if (__any_sync(0xffffffffu, top > m + 8.f)) {
-                const float now = fmaxf(m, top), keep = exp2_fast(m - now);
+            if (__any_sync(0xffffffffu, top - m > kMost)) {
+                const float now = fmaxf(m, __fsub_ru(top, kLeast)), keep = exp2_fast(m - now);
                 m = now;
                 l *= keep;
                 if (i > 0) {

@@ -1,0 +1,91 @@
+"""Keys and values in 4 bits where the kernels' number ranges end: keys that have nearly all weight. The formulas in 64 bits and the tolerances are those of test_gpu_packed.py; what these do not
+cover stands at each test."""
+import numpy as np
+import pytest
+
+import packed_util as util
+from kipizen_util import to_bf16
+from packed_util import Form
+from test_gpu_packed import BOTH, compare, rounded, rows_of, run
+
+pytestmark = pytest.mark.gpu
+
+
+def with_block(f, s, score, value):
+    """Keys whose first sixteen dimensions are `score(sequence, position)` times those of a query, and keys whose value is `value(position)` times what it was: the score of a key is that, and a normal number of
+    spread 1 from its other dimensions. Queries are neither turned nor normed: f16 holds them."""
+    assert f.rot_dims == 0 and not f.norm and f.dim > 16 and not f.factors
+    r, (q0, k0, v0) = np.random.default_rng(7), f.offsets
+    q = r.standard_normal((len(s.proj), f.heads, f.dim)) / (f.scale * (f.dim - 16) ** 0.5)
+    q[..., :16] = 1.0 / (16 * f.scale)
+    s.proj[:, q0:q0 + f.heads * f.dim] = to_bf16(q.reshape(len(q), -1).astype(np.float32))
+    pools = [[x.copy() for x in util.parts_of(pool)] for pool in (s.keys, s.values)]
+    for i, (row, n, past, _) in enumerate(s.seqs):
+        j = np.arange(past + n)
+        for part, d, of in ((pools[0], f.dim, "key"), (pools[1], f.vdim, "value")):
+            x = np.zeros((len(j), f.kv_heads, d), np.float32)
+            old = j[:past]
+            at = s.table[i, old // f.page], slice(None), old % f.page
+            new = s.proj[row:row + n, (k0 if of == "key" else v0):][:, :f.kv_heads * d].reshape(n, f.kv_heads, d)
+            assert np.shares_memory(new, s.proj)
+            x[:past], x[past:] = util.valued(part[0][at], part[1][at], np.ones(f.kv_heads)), new
+            if of == "key":
+                x[..., :16] = np.array([score(p) for p in j])[:, None, None]
+                x[..., 16:][np.array([score(p) for p in j]) != 0] *= 0.25
+            else:
+                x *= np.array([value(p) for p in j])[:, None, None]
+            x = to_bf16(x)
+            part[0][at], part[1][at] = util.packed(x[:past], np.ones(f.kv_heads))
+            new[:] = x[past:]
+    s.keys, s.values = util.bytes_of(*pools[0]), util.bytes_of(*pools[1])
+
+
+def check(f, s, kind, gap):
+    """bf16: the tolerances of `compare` at a spread of 1; a weight that is `gap` and a few units below the largest may be off by 2^-33 of that, which over a few thousand keys is 2^-33 / sqrt 3 · e^gap of the result, 6e-4
+    at 17. f32: a product's sum reaches gap / scale in its first sixteen terms, each rounded to 2^-24, the exponential's argument and its value once more."""
+    session, _, outs = run(f, s, kind)
+    got, pools = session.download(outs["out"]).numpy(), util.written(f, s, rounded(kind))
+    want, live = util.reference(f, s, pools), rows_of(s)
+    empty = ~want[live].any(1)  # rows that see nothing but a value of 0
+    assert not got[live][empty].any()
+    if kind == "bf16":
+        got[live[empty]] = want[live[empty]] = 1.0
+        compare(got, want, kind, s, 1.0)
+    else:
+        off = np.sqrt(((got[live] - want[live]) ** 2).sum(1))[~empty] / np.sqrt((want[live] ** 2).sum(1))[~empty]
+        assert off.max() <= 2.0 ** -24 * (18 * gap + 20)
+
+
+FORMS = [Form(8, 2, 64, 128), Form(4, 4, 128, 64), Form(20, 1, 256, 256)]
+STEPS = [[(150, 3000), (1, 4000), (1, 3500)], [(1, 8000), (1, 3000)], [(70, 4000)]]
+
+
+@BOTH
+@pytest.mark.parametrize("gap", [8, 12, 14, 17])
+@pytest.mark.parametrize("lengths", STEPS, ids=str)
+@pytest.mark.parametrize("f", FORMS, ids=lambda f: f"{f.heads}x{f.kv_heads}x{f.dim}x{f.vdim}")
+def test_a_first_key_that_has_nearly_all_weight(f, lengths, gap, kind):
+    """As in trained models: its value adds little, so that a row's result is that of all the others."""
+    s = util.step(f, lengths, 3, round_to=rounded(kind))
+    with_block(f, s, lambda p: gap * (p == 0), lambda p: float(p != 0))
+    check(f, s, kind, gap)
+
+
+@BOTH
+def test_a_long_prompt_behind_such_a_key(kind):
+    """Its own first key: two tiles of rows in a CTA, and rows of few keys."""
+    f = Form(16, 16, 64, 64)
+    s = util.step(f, [(4800 if kind == "bf16" else 300, 0)], 3, round_to=rounded(kind))
+    with_block(f, s, lambda p: 12 * (p == 0), lambda p: float(p != 0))
+    check(f, s, kind, 12)
+
+
+@BOTH
+@pytest.mark.parametrize("lengths", STEPS, ids=str)
+def test_scores_that_rise_and_a_key_far_above_the_ones_before(lengths, kind):
+    """What weights are taken against moves many times, by little and by much."""
+    f = Form(8, 2, 64, 128)
+    for score in (lambda p: 30.0 * p / 4000, lambda p: 9.0 * (p // 700), lambda p: 60.0 * (p == 1234), lambda p: -20.0 * (p < 2500)):
+        s = util.step(f, lengths, 3, round_to=rounded(kind))
+        with_block(f, s, score, lambda p: 1.0)
+        check(f, s, kind, 60)

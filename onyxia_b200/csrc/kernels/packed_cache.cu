@@ -453,12 +453,14 @@ void emit_packed_attention(Emitter& em, const PackedDesc& d, const TRef& proj, c
     p.append = d.append;
     p.cap2 = (float)(d.softcap * (double)kLog2e);
     p.mul2 = (float)(d.softcap > 0 ? 2.0 * (double)kLog2e * d.scale / d.softcap : (double)kLog2e * d.scale);
-    p.by_rep = by_of(d.heads ? d.heads / d.kv_heads : 1);
-    p.by_units = by_of(d.dim / 8 - d.rot_dims / 16);
-    p.by_runs = by_of(d.vdim / 8);
-    p.by_key = by_of(d.dim / kPack);
-    p.by_value = by_of(d.vdim / kPack);
-    p.by_eighths = by_of(d.dim / 8);
+    // (rows of a prompt's CTA, scales of 64 keys)
+    const int64_t most_heads = std::max(d.heads, d.kv_heads), units = d.dim / 8 - d.rot_dims / 16, cta_rows = 256, cta_keys = 64;
+    p.by_rep = by_of(d.heads ? d.heads / d.kv_heads : 1, std::max(d.heads, cta_rows));
+    p.by_units = by_of(units, most_heads * units);
+    p.by_runs = by_of(d.vdim / 8, d.kv_heads * d.vdim / 8);
+    p.by_key = by_of(d.dim / kPack, std::max(cta_keys * d.dim / kPack, cta_rows));
+    p.by_value = by_of(d.vdim / kPack, std::max(cta_keys * d.vdim / kPack, cta_rows));
+    p.by_eighths = by_of(d.dim / 8, d.heads * d.dim / 8);
     const bool bf = proj.dtype == DT_BF16, tc = out && bf && d.dim <= 256 && d.vdim <= 256 && n_seqs <= 65535 && n_seqs * d.heads <= INT32_MAX;
     p.only = tc && rows == n_seqs;
     const bool prefill = tc && !p.only && d.heads / d.kv_heads <= 128 && out->buf.off % 16 == 0 && rows * d.heads / 64 + n_seqs * d.kv_heads <= INT32_MAX;
@@ -529,11 +531,11 @@ void emit_packed_read(Emitter& em, const PackedDesc& d, const TRef& keys, const 
     p.vdim = (int)d.vdim;
     p.node = em.node;
     const int64_t blocks = d.kv_heads * (d.dim + d.vdim) / kPack;
-    p.by_all = by_of(blocks);
-    p.by_key = by_of(d.dim / kPack);
-    p.by_value = by_of(d.vdim / kPack);
     // eight blocks a thread, fewer where that leaves SMs without a CTA
     p.per = (int)std::max<int64_t>(1, std::min<int64_t>({kReadRows, 8 * kReadThreads / blocks, (rows + 2 * sm_count() - 1) / (2 * sm_count())}));
+    p.by_all = p.per > 1 ? by_of(blocks, p.per * blocks) : 1u;  // (1: the quotient is 0, however many blocks the one place has)
+    p.by_key = by_of(d.dim / kPack, d.kv_heads * d.dim / kPack);
+    p.by_value = by_of(d.vdim / kPack, d.kv_heads * d.vdim / kPack);
     const Buf none{kSlotNull, 0};
     em.launch(out.dtype == DT_BF16 ? packed_read<bf16> : packed_read<float>, dim3((unsigned)((rows + p.per - 1) / p.per)), dim3(kReadThreads), 0, p,
               {{&p.keys, keys.buf}, {&p.values, values.buf}, {&p.places, places.buf}, {&p.table, pages.buf}, {&p.out, out.buf}, {&p.key_factors, key_factors ? key_factors->buf : none},

@@ -8,6 +8,7 @@
 // scale comes out as 0 so do the codes; where one of the 16 is no number the scale is none, and all 16 read as NaN. The code of 0 has no sign.
 #pragma once
 #include "paged_util.cuh"
+#include "quotient.hpp"
 
 namespace oxk {
 
@@ -41,9 +42,8 @@ struct PackP {
     int only;                    // no rows for prompts: as many rows as sequences, none of which may have more than one new token
 };
 
-// n / d for n < 2^32 / d: `by` is by_of(d)
+// n / d for 0 ≤ n ≤ most: `by` is by_of(d, most)
 __device__ __forceinline__ int over(int n, unsigned by) { return by ? (int)__umulhi((unsigned)n, by) : n; }
-inline unsigned by_of(int64_t d) { return d > 1 ? (unsigned)(((1ull << 32) + d - 1) / d) : 0u; }
 
 __device__ __forceinline__ float key_factor(const PackP& p, int g) { return p.key_factors ? p.key_factors[g] : 1.f; }
 __device__ __forceinline__ float value_factor(const PackP& p, int g) { return p.value_factors ? p.value_factors[g] : 1.f; }

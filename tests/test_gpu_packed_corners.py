@@ -1,9 +1,10 @@
-"""Keys and values in 4 bits where the kernels' number ranges end: keys that have nearly all weight. The formulas in 64 bits and the tolerances are those of test_gpu_packed.py; what these do not
+"""Keys and values in 4 bits where the kernels' number ranges end: keys that have nearly all weight, places of very many values. The formulas in 64 bits and the tolerances are those of test_gpu_packed.py; what these do not
 cover stands at each test."""
 import numpy as np
 import pytest
 
 import packed_util as util
+import test_gpu_packed as base
 from kipizen_util import to_bf16
 from packed_util import Form
 from test_gpu_packed import BOTH, compare, rounded, rows_of, run
@@ -89,3 +90,14 @@ def test_scores_that_rise_and_a_key_far_above_the_ones_before(lengths, kind):
         s = util.step(f, lengths, 3, round_to=rounded(kind))
         with_block(f, s, score, lambda p: 1.0)
         check(f, s, kind, 60)
+
+
+@BOTH
+@pytest.mark.parametrize("f", [Form(1, 5000, 128, 128, page=16), Form(1, 65535, 16, 16, page=16), Form(1, 150, 8192, 8192, page=16), Form(1, 520, 2048, 2032, page=16)], ids=lambda f: f"{f.kv_heads}x{f.dim}x{f.vdim}")
+def test_places_of_very_many_values(f, kind):
+    """More blocks of 16 dimensions than a quotient by a product serves: written, and read back."""
+    s, got = base.check(f, [(2, 0), (1, 17)], kind, 3, "write")
+    s.keys, s.values = got["updated.pages.keys"], got["updated.pages.values"]
+    places = [(1, 17), (0, 1), (0, 0), (1, 3)]
+    session, _, outs = run(f, s, kind, "read", places)
+    assert np.array_equal(session.download(outs["stored"]).numpy(), rounded(kind)(util.read(f, [s.keys, s.values], s.table, places).astype(np.float32)))

@@ -1,10 +1,16 @@
-"""What keys and values in 4 bits refuse beside what test_packed_host.py has, asked of the backend's registry without a device."""
+"""What keys and values in 4 bits refuse beside what test_packed_host.py has, asked of the backend's registry without a device, and the quotients that their kernels take by a product."""
+import ctypes as C
+import os
+import shutil
+import subprocess
+
+import numpy as np
 import pytest
 
 import packed_util as util
 from packed_util import Form
 from onyxia_b200 import ir
-from test_packed_host import lib  # noqa: F401  (a fixture)
+from test_packed_host import ROOT, lib  # noqa: F401  (a fixture)
 
 
 @pytest.fixture
@@ -31,3 +37,39 @@ def test_attributes_that_only_the_whole_cache_has(lib, with_attrs, name, kind, d
     for value, nodes in ((0, 1), (1, 0), (2, 0)):
         m = with_attrs(f, dtype, kind, **{name: value, "gate_offset": 3})
         assert lib.taken(m.handle) == nodes
+
+
+QUOTIENT = r"""
+#include "kernels/quotient.hpp"
+// 0 where there is none
+extern "C" unsigned by_of(int64_t d, int64_t most) {
+    try {
+        return oxk::by_of(d, most);
+    } catch (const std::exception&) {
+        return 0;
+    }
+}
+"""
+
+
+def test_quotients_by_a_product(tmp_path):
+    """Every divisor up to 2^18 (the blocks of 16 dimensions that a place may have) for as many as the kernels divide, and at the ends of what it serves."""
+    if shutil.which("g++") is None:
+        pytest.skip("needs g++")
+    (tmp_path / "q.cpp").write_text(QUOTIENT)
+    subprocess.run(["g++", "-std=c++17", "-shared", "-fPIC", "-I", os.path.join(ROOT, "onyxia_b200", "csrc"), str(tmp_path / "q.cpp"), "-o", str(tmp_path / "q.so")], check=True)
+    by_of = C.CDLL(str(tmp_path / "q.so")).by_of
+    by_of.argtypes, by_of.restype = [C.c_int64, C.c_int64], C.c_uint
+    assert by_of(1, 2 ** 31 - 1) == 0
+    for d in [*range(2, 2 ** 18 + 1, 7), *range(65530, 65600), 80000, 131070, 153600, 2 ** 17, 2 ** 18]:
+        for most in (d - 1, 2048, 2 ** 19):
+            by = by_of(d, most)
+            # the ends of the last multiples of the divisor, where the product is first too large, and of the first ones
+            n = np.concatenate([np.arange(0, 3) * d + d - 1, (most + 1) // d * d - 1 - np.arange(0, 3) * d, [most]])
+            n = n[(n >= 0) & (n <= most)].astype(np.uint64)
+            right = bool(((n * np.uint64(-(-2 ** 32 // d))) >> np.uint64(32) == n // np.uint64(d)).all())
+            assert by == (-(-2 ** 32 // d) if by else 0) and (right or not by), (d, most)
+    # what every call of a kernel divides is served
+    assert all(by_of(d, most) for d, most in ((512, 2 ** 18), (1024, 2 ** 19), (65535, 65535), (2048, 2048), (16, 1024)))
+    # one place of this many blocks is not: the reading kernel has one place per block of threads there, and divides nothing
+    assert by_of(65537, 65536) == by_of(80000, 79999) == by_of(153600, 153599) == 0

@@ -489,7 +489,7 @@ void emit_packed_attention(Emitter& em, const PackedDesc& d, const TRef& proj, c
         if (!out) return;
         if (prefill) {
             const int64_t rep = d.heads / d.kv_heads;
-            const PackedPrefill pf = packed_prefill_of(d.dim, d.vdim, rows, d.kv_heads, rep, d.softcap > 0);
+            const PackedPrefill pf = packed_prefill_of(d.dim, d.vdim, rows, d.kv_heads, rep, p.cap2);
             const int64_t tq = pf.rows / rep;
             p.raw_slots = pf.slots;
             ensure_max_dynamic_smem((const void*)pf.kernel, pf.smem);

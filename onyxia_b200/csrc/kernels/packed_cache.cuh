@@ -193,6 +193,21 @@ __device__ __forceinline__ float power_up(int e) { return __uint_as_float((unsig
 // what they are. (A weight of 2^16 would be infinite: what moves the reference, and where to, is rounded so that none gets beyond 2^kMost.) A
 // closer reference costs prompts more moves: 4096 tokens of 32 heads over 16 take 187 us with 8, 194 with 11, 206 with 13.
 constexpr float kLeast = 8.f, kMost = 15.f;
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// cap2 · tanh(u), x = 2 log2 e · u. tanh u = 1 - 2 / (1 + e^2u) is off by 4e-7: for a cap2 up to kWideCap less than queries in f16 move a score. Beyond (WIDE) what lies within a quarter of the cap is a series,
+// u (1 - u²/3 + 2u⁴/15 - 17u⁶/315 + 62u⁸/2835 - ...), which leaves out 4e-7 of the score itself. (Rows of scores on both sides of the quarter have either: every element is chosen for.)
+constexpr float kWideCap = 256.f, kTwiceLog2e = 2.f * kLog2e;
+__device__ __forceinline__ float cap_series(float cap2, float z) {  // z = u²: what u is multiplied by
+    return __fmaf_rn(__fmaf_rn(__fmaf_rn(cap2 * (-17.f / 315.f), z, cap2 * (2.f / 15.f)), z, cap2 * (-1.f / 3.f)), z, cap2);
+}
+template <bool WIDE> __device__ __forceinline__ float capped_score(float cap2, float x) {
+    const float far = cap2 - __fdividef(2.f * cap2, 1.f + exp2_fast(x)), u = x * (1.f / kTwiceLog2e);
+    return WIDE && fabsf(u) <= 0.25f ? u * cap_series(cap2, u * u) : far;
+}
 // 32 values of a head by one warp, the lane's `value` dimension c + lane: codes and scales to where they are held. Values from n on are nobody's.
 __device__ __forceinline__ void put_32(unsigned char* codes, unsigned char* scales, int c, int n, float factor, float value) {
     const int lane = threadIdx.x & 31, i = c + lane;
@@ -221,6 +236,6 @@ struct PackedPrefill {
     PackKernel kernel;
     int smem, rows, threads, slots;  // bytes; (token, head) rows of a CTA; copies of 64 keys or values under way
 };
-PackedPrefill packed_prefill_of(int64_t dim, int64_t vdim, int64_t rows, int64_t kv_heads, int64_t rep, bool capped);
+PackedPrefill packed_prefill_of(int64_t dim, int64_t vdim, int64_t rows, int64_t kv_heads, int64_t rep, float cap2);
 
 }  // namespace oxk

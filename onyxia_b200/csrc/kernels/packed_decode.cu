@@ -40,12 +40,6 @@ template <int KS, int VC> struct Smem {
     static_assert(raw + (kHeads + 1) * dk * 2 + dv * 2 <= rings && angle % 16 == 0 && raw % 16 == 0, "all of it fits the last stage");
 };
 
-__device__ __forceinline__ float exp2_fast(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
 // What single tokens have to go through: blocks of 128 keys of every sequence and group of query heads (a cell), cell behind cell.
 template <class P> __device__ __forceinline__ int blocks_of(const P& p, const SeqRow& s) {
     return s.len == 1 ? s.past / (kTile * kWarps) + 1 - first_key(p, s.past) / (kTile * kWarps) : 0;
@@ -385,11 +379,15 @@ template <int KS, int VC, bool WHOLE, int RESIDENT> __global__ void __launch_bou
 #pragma unroll
                 for (int e = 0; e < 4; e++) s[half][e] += more[half][e];
             bool above = false;
+            auto cap = [&](auto wide) {
+#pragma unroll
+                for (int half = 0; half < 2; half++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) s[half][e] = capped_score<decltype(wide)::value>(p.cap2, s[half][e] * mul[e & 1]);
+            };
+            if (capped) p.cap2 > kWideCap ? cap(std::true_type{}) : cap(std::false_type{});
 #pragma unroll
             for (int half = 0; half < 2; half++) {
-                if (capped)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) s[half][e] = p.cap2 - __fdividef(2.f * p.cap2, 1.f + exp2_fast(s[half][e] * mul[e & 1]));
                 if constexpr (edge) {
 #pragma unroll
                     for (int e = 0; e < 4; e++) {

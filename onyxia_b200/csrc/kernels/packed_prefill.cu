@@ -21,16 +21,9 @@ namespace {
 
 constexpr int kRows = 128, kUnpack = 128, kStages = 2, kKeys = 64, kSlots = 8;
 constexpr unsigned kPanelQ = kRows * 128, kPanel = kKeys * 128;  // bytes: rows, or keys, × 64 dimensions
-constexpr float kTwiceLog2e = 2.f * kLog2e;
 constexpr float kNone = -1e30f;            // below every score, and finite: differences stay numbers
 
 __device__ __forceinline__ unsigned bits(__half2 v) { return *reinterpret_cast<unsigned*>(&v); }
-
-__device__ __forceinline__ float exp2_fast(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 
 __device__ __forceinline__ unsigned ld_shared(unsigned at) {
     unsigned v;
@@ -46,9 +39,11 @@ __device__ __forceinline__ unsigned ld_shared_u8(unsigned at) {
 
 __device__ __forceinline__ void st_shared(unsigned at, unsigned v) { asm volatile("st.shared.b32 [%0], %1;" ::"r"(at), "r"(v) : "memory"); }
 
-template <int TILES, bool CAPPED> __global__ void __launch_bounds__(TILES * kRows + kUnpack + 64, TILES == 1 ? 2 : 1) packed_prefill(const PackP p) {
+// CAP: 1, scores are capped; 2, by more than kWideCap
+template <int TILES, int CAP> __global__ void __launch_bounds__(TILES * kRows + kUnpack + 64, TILES == 1 ? 2 : 1) packed_prefill(const PackP p) {
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    constexpr bool CAPPED = CAP != 0;
     constexpr int kSoft = TILES * kRows, kThreads = kSoft + kUnpack + 64, kSoftWarps = kSoft / 32, kIssues = kSoftWarps + kUnpack / 32, kCopies = kIssues + 1;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, kp = (p.dim + 63) / 64, vp = (p.vdim + 63) / 64;
     const unsigned k_stage = kp * kPanel, v_stage = vp * kPanel;
@@ -258,7 +253,7 @@ template <int TILES, bool CAPPED> __global__ void __launch_bounds__(TILES * kRow
         const int tile = warp / 4, tok = over(tid, p.by_rep), head = g * rep + tid - tok * rep;
         const bool live = tok < n_tok;
         const int pos = live ? pos0 + tok : last, low = first_key(p, pos);  // rows without a token compute something harmless
-        const float mul = live ? p.q_mul[(long long)(sq.start + first + tok) * p.heads + head] : 0.f, cap2 = p.cap2, by_cap = mul * (1.f / kTwiceLog2e), series1 = cap2 * (-1.f / 3.f), series2 = cap2 * (2.f / 15.f), series3 = cap2 * (-17.f / 315.f);
+        const float mul = live ? p.q_mul[(long long)(sq.start + first + tok) * p.heads + head] : 0.f, cap2 = p.cap2, by_cap = mul * (1.f / kTwiceLog2e);
         const unsigned lanes = (unsigned)((warp & 3) * 32) << 16, sum = t_sum + lanes + tile * 128;
         float m = kNone, l = 0.f, sums[4];
         const float factor = value_factor(p, g);
@@ -274,9 +269,16 @@ template <int TILES, bool CAPPED> __global__ void __launch_bounds__(TILES * kRow
             // In base 2. Factors are positive (a negative one is in the queries): the largest score is that of the largest product.
             auto score = [&](float d) {
                 const float x = d * mul;
-                return CAPPED ? cap2 - __fdividef(2.f * cap2, 1.f + exp2_fast(x)) : x;
+                return CAPPED ? capped_score<CAP == 2>(cap2, x) : x;
             };
-            auto largest = [&](float d) { return CAPPED ? score(d) : __fmul_ru(d, mul); };
+            auto near_score = [&](float d, auto&& product) {
+                const float u = d * by_cap;
+                return product(u, cap_series(cap2, u * u));
+            };
+            auto largest = [&](float d) {
+                if (CAP == 2 && near) return near_score(d, [](float u, float s) { return __fmul_ru(u, s); });
+                return CAPPED ? score(d) : __fmul_ru(d, mul);
+            };
             auto hidden = [&](int j) { return j > pos || j < low; };
             // 32 products at a time, the next ones on their way
             auto each = [&](auto&& take) {
@@ -304,7 +306,7 @@ template <int TILES, bool CAPPED> __global__ void __launch_bounds__(TILES * kRow
                         if (CAPPED) least = fminf(fminf(least, __uint_as_float(v[e])), __uint_as_float(v[e + 1]));
                     }
                 });
-                // tanh u = u (1 - u²/3 + 2u⁴/15 - 17u⁶/315 + 62u⁸/2835 - ...): where no score that the warp's rows see is beyond a quarter of the cap, what is left out is 4e-7 of it.
+                // where no score that the warp's rows see is beyond a quarter of the cap they are a series (capped_score)
                 if (CAPPED) near = __all_sync(0xffffffffu, fmaxf(fabsf(top), fabsf(least)) * mul <= 0.25f * kTwiceLog2e);
                 top = largest(top);
             }
@@ -328,17 +330,18 @@ template <int TILES, bool CAPPED> __global__ void __launch_bounds__(TILES * kRow
             }
 #pragma unroll
             for (int e = 0; e < 4; e++) sums[e] = 0.f;
-            auto near_score = [&](float d) {
-                const float u = d * by_cap, z = u * u;
-                return __fmaf_rn(u, __fmaf_rn(__fmaf_rn(__fmaf_rn(series3, z, series2), z, series1), z, cap2), -m);
+            auto near_weight = [&](float d) { return near_score(d, [&](float u, float s) { return __fmaf_rn(u, s, -m); }); };
+            auto weight = [&](float d) {
+                const float a = score(d) - m;
+                return CAP == 2 && a > kMost ? kMost : a;  // (far above a quarter of the widest caps a score is off by more than that)
             };
             auto weigh = [&](int c, const unsigned (&v)[32], auto series, auto&& shown) {
                 unsigned w[16];
 #pragma unroll
                 for (int e = 0; e < 32; e += 2) {
                     float a, b;
-                    if constexpr (CAPPED && series) a = near_score(__uint_as_float(v[e])), b = near_score(__uint_as_float(v[e + 1]));
-                    else if (CAPPED) a = score(__uint_as_float(v[e])) - m, b = score(__uint_as_float(v[e + 1])) - m;
+                    if constexpr (CAPPED && series) a = near_weight(__uint_as_float(v[e])), b = near_weight(__uint_as_float(v[e + 1]));
+                    else if (CAPPED) a = weight(__uint_as_float(v[e])), b = weight(__uint_as_float(v[e + 1]));
                     else a = __fmaf_rn(__uint_as_float(v[e]), mul, -m), b = __fmaf_rn(__uint_as_float(v[e + 1]), mul, -m);
                     a = exp2_fast(shown(a, j0 + c + e));
                     b = exp2_fast(shown(b, j0 + c + e + 1));
@@ -424,11 +427,12 @@ int smem_of(int dim, int vdim, int tiles) {
 
 }  // namespace
 
-PackedPrefill packed_prefill_of(int64_t dim, int64_t vdim, int64_t rows, int64_t kv_heads, int64_t rep, bool capped) {
+PackedPrefill packed_prefill_of(int64_t dim, int64_t vdim, int64_t rows, int64_t kv_heads, int64_t rep, float cap2) {
     // Two tiles share what is unpacked: 4096 tokens of 32 heads over 16 take 191 us, with one per CTA 229. They have to fill the device twice, or its SMs wait for the longest: 1999 behind 1000 of 16
     // heads over 4 take 119 us with two, 112 with one.
     const int tiles = dim <= 128 && vdim <= 128 && (rows * rep + 2 * kRows - 1) / (2 * kRows) * kv_heads >= 2 * sm_count() ? 2 : 1;
-    const PackKernel k = tiles == 2 ? (capped ? packed_prefill<2, true> : packed_prefill<2, false>) : capped ? packed_prefill<1, true> : packed_prefill<1, false>;
+    const PackKernel of[2][3] = {{packed_prefill<1, 0>, packed_prefill<1, 1>, packed_prefill<1, 2>}, {packed_prefill<2, 0>, packed_prefill<2, 1>, packed_prefill<2, 2>}};
+    const PackKernel k = of[tiles - 1][cap2 > kWideCap ? 2 : cap2 > 0.f];
     // With 512 columns of tensor memory a CTA has its SM alone, with 256 it shares it with one other.
     const bool alone = tiles == 2 || vdim > 128;
     const int fixed = smem_of((int)dim, (int)vdim, tiles), slot = kKeys * (int)std::max(dim, vdim) / kPack * 9, room = (alone || fixed + 2 * slot > 112 * 1024 ? 226 : 112) * 1024;

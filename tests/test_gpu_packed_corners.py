@@ -1,4 +1,4 @@
-"""Keys and values in 4 bits where the kernels' number ranges end: keys that have nearly all weight, places of very many values. The formulas in 64 bits and the tolerances are those of test_gpu_packed.py; what these do not
+"""Keys and values in 4 bits where the kernels' number ranges end: keys that have nearly all weight, wide caps, places of very many values. The formulas in 64 bits and the tolerances are those of test_gpu_packed.py; what these do not
 cover stands at each test."""
 import numpy as np
 import pytest
@@ -101,3 +101,23 @@ def test_places_of_very_many_values(f, kind):
     places = [(1, 17), (0, 1), (0, 0), (1, 3)]
     session, _, outs = run(f, s, kind, "read", places)
     assert np.array_equal(session.download(outs["stored"]).numpy(), rounded(kind)(util.read(f, [s.keys, s.values], s.table, places).astype(np.float32)))
+
+
+@BOTH
+@pytest.mark.parametrize("cap", [1e3, 1e4, 1e6, 1e9, 1e30])
+def test_wide_caps(cap, kind):
+    """A cap far above all scores changes none of them, in prompts and single tokens, whole tiles and those with hidden keys."""
+    for f in (Form(4, 2, 64, 128, 64, softcap=cap), Form(4, 1, 128, 256, 128, softcap=cap, window=90), Form(16, 16, 64, 64, 64, softcap=cap)):
+        base.check(f, [(100, 150), (1, 90)], kind)
+        base.check(f, [(1, 700), (1, 3)], kind, seed=1)
+
+
+@BOTH
+@pytest.mark.parametrize("cap", [300.0, 4e3, 1e4, 1e6])
+@pytest.mark.parametrize("lengths", STEPS, ids=str)
+def test_scores_on_both_sides_of_a_quarter_of_a_wide_cap(lengths, cap, kind):
+    """A few keys far below the others, which have all weight."""
+    f = Form(8, 2, 64, 128, softcap=cap)
+    s = util.step(f, lengths, 3, round_to=rounded(kind))
+    with_block(f, s, lambda p: -2600.0 * (p % 97 == 5), lambda p: 1.0)
+    check(f, s, kind, 10)

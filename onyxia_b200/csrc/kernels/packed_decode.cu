@@ -17,8 +17,9 @@ namespace oxk {
 
 namespace {
 
+// Weights are those of products that are not rounded before the reference, a rounded one, is subtracted. Where that rounding may come near kLeast, all are rounded alike first.
+constexpr float kLarge = 0x1p25f;
 constexpr int kWarps = 4, kThreads = kWarps * 32, kPages = 256, kHeads = 8, kKeys = 16, kTile = 2 * kKeys, kStages = 3, kMostParts = 64;
-constexpr float kNone = -1e30f;  // below every score, and finite: differences stay numbers
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -325,6 +326,7 @@ template <int KS, int VC, bool WHOLE, int RESIDENT> __global__ void __launch_bou
         for (int n = 0; n < VC; n++)
 #pragma unroll
             for (int e = 0; e < 4; e++) o[n][e] = 0.f;
+        // Whether it is done: scores beyond kLarge are left to the form for edges.
         auto attend = [&](auto edge, int j0, const unsigned char* stage) {
             // (the two halves in turn, each in two sums: a product does not wait for the one before it)
             uint2 key[2][2][KS];
@@ -404,6 +406,7 @@ template <int KS, int VC, bool WHOLE, int RESIDENT> __global__ void __launch_bou
                     float now = fmaxf(fmaxf(s[0][e], s[0][e + 2]), fmaxf(s[1][e], s[1][e + 2]));
 #pragma unroll
                     for (int d = 4; d < 32; d <<= 1) now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, d));
+                    if (!edge && __any_sync(0xffffffffu, fabsf(now * weigh[e]) > kLarge)) return false;
                     now = now > -INFINITY ? fmaxf(top[e], __fsub_ru(__fmul_ru(now, weigh[e]), kLeast)) : top[e];
                     const float keep = exp2_fast(top[e] - now);
                     top[e] = now;
@@ -423,7 +426,8 @@ template <int KS, int VC, bool WHOLE, int RESIDENT> __global__ void __launch_bou
                 unsigned pb[2];
 #pragma unroll
                 for (int r = 0; r < 2; r++) {
-                    const float w0 = exp2_fast(__fmaf_rn(s[half][2 * r], weigh[0], -top[0])), w1 = exp2_fast(__fmaf_rn(s[half][2 * r + 1], weigh[1], -top[1]));
+                    auto weight = [&](float x, int e) { return exp2_fast(edge ? __fmul_ru(x, weigh[e]) - top[e] : __fmaf_rn(x, weigh[e], -top[e])); };
+                    const float w0 = weight(s[half][2 * r], 0), w1 = weight(s[half][2 * r + 1], 1);
                     pb[r] = transpose8x8(bits(__floats2half2_rn(w0, w1)));
                 }
                 constexpr unsigned kOnes = 0x3C003C00u;
@@ -483,16 +487,21 @@ template <int KS, int VC, bool WHOLE, int RESIDENT> __global__ void __launch_bou
                     }
                 }
             }
+            return true;
         };
         unsigned at = 0;
+        bool large = false;
 #pragma unroll 1
         for (int i = 0; i < tiles; i++) {
             if (ok && !mbar_wait(full + at * 8, rounds >> at & 1)) ok = false;
             rounds ^= 1u << at;
             const int j0 = first + i * step;
             const unsigned char* stage = smem + (at * kWarps + warp) * L::stage;
-            if (j0 + kTile > hi || j0 < low) attend(std::true_type{}, j0, stage);
-            else attend(std::false_type{}, j0, stage);
+            if (large || j0 + kTile > hi || j0 < low || !attend(std::false_type{}, j0, stage)) {
+                attend(std::true_type{}, j0, stage);
+                large |= (top[0] > kNone && fabsf(top[0]) > kLarge) || (top[1] > kNone && fabsf(top[1]) > kLarge);
+                large = __any_sync(0xffffffffu, large);
+            }
             __syncwarp();
             copy(i + kStages, at);
             __syncwarp();

@@ -21,7 +21,6 @@ namespace {
 
 constexpr int kRows = 128, kUnpack = 128, kStages = 2, kKeys = 64, kSlots = 8;
 constexpr unsigned kPanelQ = kRows * 128, kPanel = kKeys * 128;  // bytes: rows, or keys, × 64 dimensions
-constexpr float kNone = -1e30f;            // below every score, and finite: differences stay numbers
 
 __device__ __forceinline__ unsigned bits(__half2 v) { return *reinterpret_cast<unsigned*>(&v); }
 
@@ -268,8 +267,7 @@ template <int TILES, int CAP> __global__ void __launch_bounds__(TILES * kRows + 
             bool near = false;
             // In base 2. Factors are positive (a negative one is in the queries): the largest score is that of the largest product.
             auto score = [&](float d) {
-                const float x = d * mul;
-                return CAPPED ? capped_score<CAP == 2>(cap2, x) : x;
+                return CAPPED ? capped_score<CAP == 2>(cap2, d * mul) : __fmul_ru(d, mul);
             };
             auto near_score = [&](float d, auto&& product) {
                 const float u = d * by_cap;
@@ -277,7 +275,7 @@ template <int TILES, int CAP> __global__ void __launch_bounds__(TILES * kRows + 
             };
             auto largest = [&](float d) {
                 if (CAP == 2 && near) return near_score(d, [](float u, float s) { return __fmul_ru(u, s); });
-                return CAPPED ? score(d) : __fmul_ru(d, mul);
+                return score(d);
             };
             auto hidden = [&](int j) { return j > pos || j < low; };
             // 32 products at a time, the next ones on their way

@@ -121,3 +121,15 @@ def test_scores_on_both_sides_of_a_quarter_of_a_wide_cap(lengths, cap, kind):
     s = util.step(f, lengths, 3, round_to=rounded(kind))
     with_block(f, s, lambda p: -2600.0 * (p % 97 == 5), lambda p: 1.0)
     check(f, s, kind, 10)
+
+
+@BOTH
+@pytest.mark.parametrize("scale", [3e5, -3e6, 3e7, -3e8, 3e9, -3e10, 1e29, -1e29, 1e30, -1e30])
+def test_scores_of_any_size_that_f32_has(scale, kind):
+    """A row that sees one key has its value, whatever the score, far below 0 too."""
+    f = Form(4, 2, 64, 128, 64, window=1, scale=scale)
+    for lengths in ([(150, 20), (1, 200), (20, 130), (1, 0)], [(1, 200), (1, 0), (1, 63)]):
+        s = util.step(f, lengths, 1, round_to=rounded(kind))
+        session, _, outs = run(f, s, kind)
+        want = util.reference(f, s, util.written(f, s, rounded(kind)))[rows_of(s)]
+        assert np.array_equal(session.download(outs["out"]).numpy()[rows_of(s)], rounded(kind)(want.astype(np.float32)))

@@ -112,10 +112,12 @@ __device__ __forceinline__ void units8(unsigned word, __half2 (&v)[4]) {
 }
 
 // ── a batch step ──
+// Keys are counted in 32 bits, 128 at a time: a sequence ends this far in front of their end.
+constexpr long long kMostKeys = (1ll << 31) - 128;
 // Sequence r of the batch. One whose rows are not the batch's, or whose positions the page table has no place for, is reported and has no rows.
 template <class P> __device__ __forceinline__ SeqRow checked_seq(const P& p, int r) {
     SeqRow s = load_seq(p.seqs, r);
-    if (s.len != 0 && (s.start < 0 || s.len < 0 || s.past < 0 || s.start + (long long)s.len > p.rows || s.past + (long long)s.len > (long long)p.width << p.shift)) {
+    if (s.len != 0 && (s.start < 0 || s.len < 0 || s.past < 0 || s.start + (long long)s.len > p.rows || s.past + (long long)s.len > min((long long)p.width << p.shift, kMostKeys))) {
         report(p.err, ERR_BATCH_SEQ, p.node, r, s.past + (long long)s.len);
         s.len = 0;
     }

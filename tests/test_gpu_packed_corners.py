@@ -1,4 +1,4 @@
-"""Keys and values in 4 bits where the kernels' number ranges end: keys that have nearly all weight, wide caps, places of very many values. The formulas in 64 bits and the tolerances are those of test_gpu_packed.py; what these do not
+"""Keys and values in 4 bits where the kernels' number ranges end: keys that have nearly all weight, wide caps, positions next to 2^31, places of very many values. The formulas in 64 bits and the tolerances are those of test_gpu_packed.py; what these do not
 cover stands at each test."""
 import numpy as np
 import pytest
@@ -6,6 +6,7 @@ import pytest
 import packed_util as util
 import test_gpu_packed as base
 from kipizen_util import to_bf16
+from onyxia_b200 import OnyxiaError
 from packed_util import Form
 from test_gpu_packed import BOTH, compare, rounded, rows_of, run
 
@@ -133,3 +134,29 @@ def test_scores_of_any_size_that_f32_has(scale, kind):
         session, _, outs = run(f, s, kind)
         want = util.reference(f, s, util.written(f, s, rounded(kind)))[rows_of(s)]
         assert np.array_equal(session.download(outs["out"]).numpy()[rows_of(s)], rounded(kind)(want.astype(np.float32)))
+
+
+@BOTH
+@pytest.mark.parametrize("new", [1, 70])
+@pytest.mark.parametrize("form", ["attend", "write"])
+def test_the_last_positions(form, new, kind):
+    """Keys are counted in 32 bits, 128 at a time. Up to 2^31 - 128 a window's keys are those of the same page at its first place; a sequence that ends behind that is reported."""
+    f = Form(2, 1, 16, 16, page=1 << 20, window=100)
+    s = util.step(f, [(new, 500)], 3, round_to=rounded(kind), spare=0)
+    place = f.page - 128 - new  # where the new tokens go; the window's keys come from where the step has some
+    pools = [[x.copy() for x in util.parts_of(p)] for p in (s.keys, s.values)]
+    for codes, scales in pools:
+        codes[:, :, place - 500:place], scales[:, :, place - 500:place] = codes[:, :, :500].copy(), scales[:, :, :500].copy()
+    s.keys, s.values = (util.bytes_of(*p) for p in pools)
+    s.seqs[0, 2] = place
+    session, _, outs = run(f, s, kind, form)
+    want = {n: session.download(t).numpy() for n, t in outs.items()}
+    s.table = np.full((1, 2048), -1, np.int32)
+    s.table[0, -1] = 0
+    s.seqs[0, 2] = 2 ** 31 - 128 - new
+    session, dev, outs = run(f, s, kind, form)
+    assert all(np.array_equal(session.download(t).numpy(), want[n]) for n, t in outs.items()) and len(want) == (3 if form == "attend" else 2)
+    s.seqs[0, 2] += 1
+    session, _, outs = run(f, s, kind, form)
+    with pytest.raises(OnyxiaError, match="sequence 0 does not lie in"):
+        session.download(next(iter(outs.values())))

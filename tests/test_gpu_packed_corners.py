@@ -1,5 +1,7 @@
-"""Keys and values in 4 bits where the kernels' number ranges end: keys that have nearly all weight, wide caps, positions next to 2^31, places of very many values. The formulas in 64 bits and the tolerances are those of test_gpu_packed.py; what these do not
+"""Keys and values in 4 bits where the kernels' number ranges end: keys that have nearly all weight, wide caps, positions next to 2^31, norms of many heads, places of very many values. The formulas in 64 bits and the tolerances are those of test_gpu_packed.py; what these do not
 cover stands at each test."""
+import dataclasses
+
 import numpy as np
 import pytest
 
@@ -160,3 +162,13 @@ def test_the_last_positions(form, new, kind):
     session, _, outs = run(f, s, kind, form)
     with pytest.raises(OnyxiaError, match="sequence 0 does not lie in"):
         session.download(next(iter(outs.values())))
+
+
+@BOTH
+@pytest.mark.parametrize("heads,kv", [(95, 1), (126, 1), (127, 1), (128, 1), (120, 40), (96, 32), (192, 96)], ids=str)
+def test_norms_of_many_heads(heads, kv, kind):
+    """A block of threads sums the squares of up to 128 heads at a time: as many, one fewer, one more, and a second and third time; queries and keys in one turn."""
+    f = Form(heads, kv, 32, 32, 32, norm=1)
+    base.check(f, [(40, 30), (1, 70), (3, 0)], kind)
+    base.check(dataclasses.replace(f, rot_dims=0), [(5, 30)], kind, form="write")
+    base.check(f, [(1, 30), (1, 70)], kind, seed=1)

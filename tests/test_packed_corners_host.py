@@ -10,6 +10,7 @@ import pytest
 import packed_util as util
 from packed_util import Form
 from onyxia_b200 import ir
+from onyxia_b200.ir import HostTensor
 from test_packed_host import ROOT, lib  # noqa: F401  (a fixture)
 
 
@@ -73,3 +74,28 @@ def test_quotients_by_a_product(tmp_path):
     assert all(by_of(d, most) for d, most in ((512, 2 ** 18), (1024, 2 ** 19), (65535, 65535), (2048, 2048), (16, 1024)))
     # one place of this many blocks is not: the reading kernel has one place per block of threads there, and divides nothing
     assert by_of(65537, 65536) == by_of(80000, 79999) == by_of(153600, 153599) == 0
+
+
+@pytest.mark.parametrize("kind,computed,early", [(k, c, e) for k in ("attend", "shared", "write") for c, e in (("", 1), ("reshaped", 1), ("seq_info", 0), ("page_table", 0), ("turns", 0))] +
+                         [("read", "", 1), ("read", "reshaped", 1), ("read", "page_table", 0)])
+def test_what_the_module_computes_is_waited_for(lib, monkeypatch, kind, computed, early):  # noqa: F811
+    """Single tokens look at the batch description, the page table and the angles before the launches in front of theirs have ended: only where nothing of the run makes them."""
+    class Builder(ir.GraphBuilder):
+        def input(self, name, dtype, shape):
+            if name == computed:
+                return self.cast(super().input(name, ir.I64, shape), ir.I32)
+            if name == "page_table" and computed == "reshaped":
+                return self.reshape(super().input(name, dtype, [shape[0], 1, shape[1]]), shape)
+            return super().input(name, dtype, shape)
+
+        def constant(self, tensor):
+            a = tensor.numpy()
+            if computed != "turns" or a.shape != (2, 32):
+                return super().constant(tensor)
+            half = [super(Builder, self).constant(HostTensor.from_numpy(a / 2)) for _ in range(2)]
+            return self.add(*half)
+
+    with monkeypatch.context() as m:
+        m.setattr(ir, "GraphBuilder", Builder)
+        module = util.module(Form(4, 2, 64, 128, 64, factors=1), ir.BF16, kind)
+    assert lib.taken(module.handle) == 1 and lib.early(module.handle) == early

@@ -15,6 +15,17 @@ from test_gpu_packed import BOTH, compare, rounded, rows_of, run
 pytestmark = pytest.mark.gpu
 
 
+STEPS_MADE = {}
+
+
+def fresh(f, lengths, kind):
+    """util.step, made once for all that begin with the same."""
+    key = repr(f), str(lengths), kind
+    if key not in STEPS_MADE:
+        STEPS_MADE[key] = util.step(f, lengths, 3, round_to=rounded(kind))
+    return dataclasses.replace(STEPS_MADE[key], proj=STEPS_MADE[key].proj.copy())
+
+
 def with_block(f, s, score, value):
     """Keys whose first sixteen dimensions are `score(sequence, position)` times those of a query, and keys whose value is `value(position)` times what it was: the score of a key is that, and a normal number of
     spread 1 from its other dimensions. Queries are neither turned nor normed: f16 holds them."""
@@ -65,12 +76,12 @@ STEPS = [[(150, 3000), (1, 4000), (1, 3500)], [(1, 8000), (1, 3000)], [(70, 4000
 
 
 @BOTH
-@pytest.mark.parametrize("gap", [8, 12, 14, 17])
+@pytest.mark.parametrize("gap", [12, 14, 17])
 @pytest.mark.parametrize("lengths", STEPS, ids=str)
 @pytest.mark.parametrize("f", FORMS, ids=lambda f: f"{f.heads}x{f.kv_heads}x{f.dim}x{f.vdim}")
 def test_a_first_key_that_has_nearly_all_weight(f, lengths, gap, kind):
     """As in trained models: its value adds little, so that a row's result is that of all the others."""
-    s = util.step(f, lengths, 3, round_to=rounded(kind))
+    s = fresh(f, lengths, kind)
     with_block(f, s, lambda p: gap * (p == 0), lambda p: float(p != 0))
     check(f, s, kind, gap)
 
@@ -90,7 +101,7 @@ def test_scores_that_rise_and_a_key_far_above_the_ones_before(lengths, kind):
     """What weights are taken against moves many times, by little and by much."""
     f = Form(8, 2, 64, 128)
     for score in (lambda p: 30.0 * p / 4000, lambda p: 9.0 * (p // 700), lambda p: 60.0 * (p == 1234), lambda p: -20.0 * (p < 2500)):
-        s = util.step(f, lengths, 3, round_to=rounded(kind))
+        s = fresh(f, lengths, kind)
         with_block(f, s, score, lambda p: 1.0)
         check(f, s, kind, 60)
 
@@ -121,7 +132,7 @@ def test_wide_caps(cap, kind):
 def test_scores_on_both_sides_of_a_quarter_of_a_wide_cap(lengths, cap, kind):
     """A few keys far below the others, which have all weight."""
     f = Form(8, 2, 64, 128, softcap=cap)
-    s = util.step(f, lengths, 3, round_to=rounded(kind))
+    s = fresh(f, lengths, kind)
     with_block(f, s, lambda p: -2600.0 * (p % 97 == 5), lambda p: 1.0)
     check(f, s, kind, 10)
 

@@ -7,10 +7,10 @@
 // A row's softmax is taken in one pass: m, l and the sums of values against a reference below the maximum (kLeast, kMost: packed_cache.cuh). Queries are f16 times a power of two of their own, weights f16,
 // all sums f32.
 //
-// What bounds it: 4096 tokens of 32 heads of 128 over 16 take 189 us, 730 TFLOP/s of 4 · 128 operations per pair (at a plain matrix product's rate 83 us). Of a step's 2430 cycles (two tiles, 64 keys)
+// What bounds it: 4096 tokens of 32 heads of 128 over 16 take 187 us, 735 TFLOP/s of 4 · 128 operations per pair (at a plain matrix product's rate 81 us). Of a step's 2430 cycles (two tiles, 64 keys)
 // the products take 1900, since a product with 64 keys reads 128 queries from shared memory for half the columns, and the issuing warp waits for weights the other 530. Scores of 128 keys would leave
 // tensor memory no place for the next ones beside two tiles' sums. Copies, codes and conversions lie under the products, in 54 % of the issue slots. 1999 tokens behind 1000, capped and normed, of 16
-// heads of 128 over 4: 103 us (20): one tile per CTA, two of them in an SM, and the last tiles' chain over 47 steps.
+// heads of 128 over 4: 94 us (19): 128 CTAs of 17 to 47 steps, which take as long as the last of them.
 #include <type_traits>
 
 #include "packed_cache.cuh"
@@ -426,9 +426,12 @@ int smem_of(int dim, int vdim, int tiles) {
 }  // namespace
 
 PackedPrefill packed_prefill_of(int64_t dim, int64_t vdim, int64_t rows, int64_t kv_heads, int64_t rep, float cap2) {
-    // Two tiles share what is unpacked: 4096 tokens of 32 heads over 16 take 191 us, with one per CTA 229. They have to fill the device twice, or its SMs wait for the longest: 1999 behind 1000 of 16
-    // heads over 4 take 119 us with two, 112 with one.
-    const int tiles = dim <= 128 && vdim <= 128 && (rows * rep + 2 * kRows - 1) / (2 * kRows) * kv_heads >= 2 * sm_count() ? 2 : 1;
+    // Two tiles share what is unpacked, one tile has half the rows to wait for. From 96 dimensions of a key on two pay as soon as single tiles would share SMs; below, a tile's products are short, and pairs have
+    // to fill the device twice. us a launch with one, two: 4096 tokens of 32 heads over 16 225, 186, of 16 heads over 4 133, 91, of 8 heads of 96 over 4 99, 92; 1999 behind 1000 of 16 heads over 4 81, 71,
+    // capped 105, 94; 600 of 32 over 16 (160 single tiles) 24, 26, behind 2000 75, 63, 300 (80) 18, 20; of 80 dimensions and values of 64, 8 heads, 4096 (256) 88, 92, of 64 79, 85, of 12 heads over 2
+    // with values of 128 (384) 93, 91, 1999 (188) 46, 51.
+    const int64_t pairs = (rows * rep + 2 * kRows - 1) / (2 * kRows) * kv_heads;
+    const int tiles = dim <= 128 && vdim <= 128 && (dim >= 96 ? 2 * pairs > sm_count() : pairs >= 2 * sm_count()) ? 2 : 1;
     const PackKernel of[2][3] = {{packed_prefill<1, 0>, packed_prefill<1, 1>, packed_prefill<1, 2>}, {packed_prefill<2, 0>, packed_prefill<2, 1>, packed_prefill<2, 2>}};
     const PackKernel k = of[tiles - 1][cap2 > kWideCap ? 2 : cap2 > 0.f];
     // With 512 columns of tensor memory a CTA has its SM alone, with 256 it shares it with one other.

@@ -183,3 +183,17 @@ def test_norms_of_many_heads(heads, kv, kind):
     base.check(f, [(40, 30), (1, 70), (3, 0)], kind)
     base.check(dataclasses.replace(f, rot_dims=0), [(5, 30)], kind, form="write")
     base.check(f, [(1, 30), (1, 70)], kind, seed=1)
+
+
+@BOTH
+@pytest.mark.parametrize("more", [dict(), dict(softcap=5.0), dict(softcap=1e4, window=200), dict(window=90), dict(sink=1, norm=1, factors=1), dict(scale=-0.125), dict(softcap=20.0, sink=1, norm=1, window=70, factors=1)], ids=str)
+def test_two_tiles_of_rows(more, kind):
+    """As many heads as give a block of threads two tiles of rows; tiles of one sequence, of its end, and of others."""
+    f = Form(40, 40, 96, 64, 32, **more)
+    base.check(f, [(280, 50), (30, 0), (1, 200)], kind)
+    base.check(dataclasses.replace(f, heads=80, page=16), [(129, 300), (128, 0), (3, 63)], kind, seed=1)
+
+
+@BOTH
+def test_what_is_no_number_in_two_tiles_of_rows(kind):
+    base.test_what_is_no_number_reaches_the_rows_that_see_it(Form(80, 80, 96, 64, 32), kind)

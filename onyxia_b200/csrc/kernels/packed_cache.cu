@@ -63,7 +63,7 @@ template <typename T> __global__ void __launch_bounds__(128) packed_write(const 
 }
 
 // The same in bf16 eight elements at a time, where heads, rotated halves and rows allow it: a unit is eight pairs that turn (all of them, ALL) or eight elements that do not, two neighbours share their
-// scales. Angles, and keys where that says which bf16 they are, in 32 bits. 4096 tokens of 32 + 16 + 16 heads of 128: 67 MB read, 51 MB written in 42 us (2.8 TB/s); without queries (read 33.6 MB, 9.4 written) 29 us. The 1560
+// scales. Angles, and keys where that says which bf16 they are, in 32 bits. 4096 tokens of 32 + 16 + 16 heads of 128: 67 MB read, 51 MB written in 42 us (2.8 TB/s; by the device's clock, events have 45); without queries (read 33.6 MB, 9.4 written) 29 us. The 1560
 // instructions of a warp take 62 % of the issue slots, the rest is the chain from the sequence's lookup over angles to scales.
 template <bool ALL, bool NORM> __global__ void __launch_bounds__(128, 8) packed_write8(const PackP p) {
     extern __shared__ __align__(16) float cs[];  // cosines [half], sines [half], norms of keys [kv_heads] in 64 bits, of queries [heads], with queries as f16 their largest elements [heads]
@@ -206,7 +206,7 @@ template <bool ALL, bool NORM> __global__ void __launch_bounds__(128, 8) packed_
         const float factor = key_factor(p, g), short_f = (float)f;
         float a[8], b[8], second[8] = {}, size[8];
         wide(src, a);
-        // In 32 bits a key is off by less than 2^-21 of its pair; where that leaves open which bf16 it is, and for what is no number, 64 bits say. (One element of 4000.)
+        // In 32 bits a key is off by less than 2^-21 of its pair; where that leaves open which bf16 it is, or the pair is infinite, 64 bits say. (One element of 4000.)
         auto rounded = [&](float (&v)[8], auto&& exact) {
             unsigned open = 0;
 #pragma unroll
@@ -291,7 +291,8 @@ struct ReadP {
 };
 constexpr int kReadThreads = 256, kReadRows = 64;
 
-// A CTA has a run of places, a thread sixteen dimensions at a time: two stores of 16 bytes in bf16. 32768 places of 16 heads of 128 + 128: 75 MB read, 268 MB written in 66 us (5.2 TB/s); stores element by element took 791.
+// A CTA has a run of places, a thread sixteen dimensions at a time: two stores of 16 bytes in bf16. 32768 places of 16 heads of 128 + 128: 75 MB read, 268 MB written in 60 us, calls one behind the other (5.7 TB/s; a launch between events 73); stores
+// element by element took 791.
 template <typename T> __global__ void __launch_bounds__(kReadThreads) packed_read(const ReadP p) {
     __shared__ int page_s[kReadRows], pos_s[kReadRows];
     pdl_enter();
@@ -351,8 +352,9 @@ template <typename T> __global__ void __launch_bounds__(kReadThreads) packed_rea
 }
 
 // ── attention of any shape ──
-// A row's head by 128 threads: chunks of 128 keys, a thread per key, then a thread per value dimension. Nothing is shared between rows or heads: for f32, dimensions beyond 256 and lone tokens it is right first; the tensor
-// cores' f16 queries and weights would not hold f32 results.
+// A row's head by 128 threads: chunks of 128 keys, a thread per key, then a thread per value dimension. Nothing is shared between rows or heads: it is right for f32, dimensions beyond 256, more than 128 heads of a key and scales beyond
+// 1024, where the tensor cores' f16 queries and weights would not hold the results. Slow where there is much to do (us a call, beside pools in f32 with onyxia.PagedKVAttention): 2048 tokens of 16 heads of 128 over 4 in f32 7200 (5900),
+// one behind 8191 1400 (1500), 16 behind 8191 2500 (3500).
 template <typename T> __global__ void __launch_bounds__(kAnyKeys) packed_simt(const PackP p) {
     extern __shared__ float sm[];  // q[dim], acc[vdim], w[128]
     __shared__ float red[32];
@@ -506,7 +508,8 @@ void emit_packed_attention(Emitter& em, const PackedDesc& d, const TRef& proj, c
         const PackedDecode dc = packed_decode_of(d.dim, d.vdim);
         const int64_t groups = d.kv_heads * ((d.heads / d.kv_heads + dc.heads - 1) / dc.heads), cells = n_seqs * groups;
         // Pieces of the same number for every cell leave nobody a second one, which costs as much as a dozen blocks of 128 keys. With more cells than places, or places that would stay empty, CTAs share
-        // all blocks evenly, but for cells without a counter each. (64 sequences up to 8192 long, 16 cells in all places: pieces 74 us, shares 78–84; 64 behind 8191 of 16 cells each: CTAs of a cell 290, shares 267.)
+        // all blocks evenly, but for cells without a counter each. us a call with pieces, shares, one behind the other (alone): 64 sequences up to 8192 long of 4 cells 57, 62 (101, 99); behind 8191 of 16 cells
+        // each, 16 sequences 68, 71 (123, 114), 30 123, 128 (198, 175), 37 150, 150, 37 up to 8192 long 133, 140 (186, 198); 20 up to 8192 long, where this shares, 84, 83 (141, 128); 64, one CTA a cell, 290, 267.
         const int64_t places = (int64_t)dc.resident * sm_count(), blocks = ((int64_t)p.width * d.page + dc.step - 1) / dc.step + 1;
         const int64_t pieces = std::min<int64_t>({places / cells, blocks, dc.pieces});
         p.pieces = (int)(cells > (int64_t)kCounterWords ? 1 : pieces * cells * 5 >= places * 4 || pieces == blocks || pieces == dc.pieces ? pieces : 0);

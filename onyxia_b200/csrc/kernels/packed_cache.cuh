@@ -59,6 +59,7 @@ template <class P> __device__ __forceinline__ unsigned char* scales_of(const P& 
 }
 
 // ── the format ──
+__device__ __forceinline__ unsigned bits(__half2 v) { return *reinterpret_cast<unsigned*>(&v); }
 __device__ __forceinline__ float max_nan(float a, float b) {
     float r;
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
@@ -161,7 +162,7 @@ template <class P> __device__ __forceinline__ void exact_angles(const P& p, int 
         sincospi(t - 2.0 * rint(0.5 * t), sn + i, cs + i);
     }
 }
-// The same of one pair in 32 bits, for queries, which f16 holds to 2^-12. Turns are reduced to quarters in 64 bits: what is left is small and loses little as f32.
+// The same of one pair in 32 bits, for queries, which f16 holds to 2^-11. Turns are reduced to quarters in 64 bits: what is left is small and loses little as f32.
 __device__ __forceinline__ void short_angle(int pos, double turns, float* cs, float* sn) {
     const double t = (double)pos * turns * 4.0, whole = rint(t);
     const int quarter = (int)((long long)whole & 3);
@@ -187,7 +188,8 @@ template <typename T> __device__ __forceinline__ double square_sum(const PackP& 
 __device__ __forceinline__ double norm_of(const PackP& p, double ss) { return 1.0 / sqrt(ss / p.dim + p.eps); }
 template <typename T> __device__ __forceinline__ double norm_factor(const PackP& p, const T* x) { return p.norm ? norm_of(p, square_sum(p, x)) : 1.0; }
 
-// The power of two that brings the largest element of a query, `top`, next to 1, as its exponent field: queries are f16 times it, so that none is too large and what is rounded is 2^-12 of an element.
+// The power of two that brings the largest element of a query, `top`, next to 1, as its exponent field: queries are f16 times it, so that none is too large and what is rounded is 2^-11 of an element, of those
+// below 2^-14 of the largest 2^-25 of that.
 __device__ __forceinline__ int query_exponent(float top) { return min(max((int)(__float_as_uint(top) >> 23), 1), 253); }
 __device__ __forceinline__ float power_down(int e) { return __uint_as_float((unsigned)(254 - e) << 23); }
 __device__ __forceinline__ float power_up(int e) { return __uint_as_float((unsigned)e << 23); }

@@ -7,7 +7,8 @@
 // What bounds it: 9/16 of a byte per dimension comes from memory, but 16 keys and values of 128 dimensions each cost a warp 313 instructions (70 conversions of codes to f16, 64 products with scales), and
 // the four CTAs of an SM issue in 55 % of its slots: 64 sequences behind 8191, 16 heads of keys, 267 us (4.5 TB/s; memory alone 185). Eight query heads of a key at most are multiplied at a time: a wider
 // matrix instruction would multiply mostly nothing, and want values as f16 in shared memory first. Loads by registers took 393 us (too few are under way), bulk copies 348, 16 more keys under way while
-// the first are weighed 293, even shares of all blocks 267. One sequence behind 519 of a key head of 256: 19 us, a chain of lookups, rotation, keys and joining.
+// the first are weighed 293, even shares of all blocks 267. One sequence behind 519 of a key head of 256: 18 us, a chain of lookups, rotation, keys and joining.
+// Of more than eight query heads of a key every eight read and convert the keys again: 64 sequences behind 8191 of one key head of 128 take 36 us with 8 heads, 51 with 9, 53 with 16, 87 with 32.
 #include <cmath>
 #include <type_traits>
 
@@ -26,7 +27,6 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], unsigned a0, unsigned a1,
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ unsigned bits(__half2 v) { return *reinterpret_cast<unsigned*>(&v); }
 
 // KS: blocks of 16 dimensions of a key per lane (64 · KS dimensions at most); VC: bytes of codes of a value per lane (16 · VC dimensions at most)
 template <int KS, int VC> struct Smem {

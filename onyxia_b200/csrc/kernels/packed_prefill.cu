@@ -22,8 +22,6 @@ namespace {
 constexpr int kRows = 128, kUnpack = 128, kStages = 2, kKeys = 64, kSlots = 8;
 constexpr unsigned kPanelQ = kRows * 128, kPanel = kKeys * 128;  // bytes: rows, or keys, × 64 dimensions
 
-__device__ __forceinline__ unsigned bits(__half2 v) { return *reinterpret_cast<unsigned*>(&v); }
-
 __device__ __forceinline__ unsigned ld_shared(unsigned at) {
     unsigned v;
     asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");

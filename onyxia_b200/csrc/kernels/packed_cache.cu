@@ -10,6 +10,7 @@
 //   packed_decode  sequences with one new token in bf16, all of the above in one launch (packed_decode.cu)
 //   packed_prefill sequences with several new tokens in bf16 (packed_prefill.cu)
 //   packed_simt    attention of any shape, f32 and bf16
+#include <cfloat>
 #include <cmath>
 
 #include "packed_cache.cuh"
@@ -448,12 +449,14 @@ void emit_packed_attention(Emitter& em, const PackedDesc& d, const TRef& proj, c
     p.window = (int)d.window;
     p.node = em.node;
     p.scale = (float)d.scale;
-    p.cap = (float)d.softcap;
+    // (a cap that f32 does not hold is the least that it does: 0 would be none)
+    const double cap = d.softcap > 0 ? std::max(d.softcap, (double)FLT_MIN) : 0.0;
+    p.cap = (float)cap;
     p.eps = d.eps;
     p.norm = d.norm;
     p.sink = d.sink;
     p.append = d.append;
-    p.cap2 = (float)(d.softcap * (double)kLog2e);
+    p.cap2 = (float)(cap * (double)kLog2e);
     p.mul2 = (float)(d.softcap > 0 ? 2.0 * (double)kLog2e * d.scale / d.softcap : (double)kLog2e * d.scale);
     // (rows of a prompt's CTA, scales of 64 keys)
     const int64_t most_heads = std::max(d.heads, d.kv_heads), units = d.dim / 8 - d.rot_dims / 16, cta_rows = 256, cta_keys = 64;

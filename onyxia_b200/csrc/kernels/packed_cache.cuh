@@ -195,8 +195,7 @@ __device__ __forceinline__ float power_down(int e) { return __uint_as_float((uns
 __device__ __forceinline__ float power_up(int e) { return __uint_as_float((unsigned)e << 23); }
 // Weights of a softmax are f16 against a reference that the largest score so far lies kLeast to kMost above (in base 2): a sum of values is rescaled where it moves, which is dear. Down to
 // 2^-(14 + kLeast) of the largest weight f16 holds 11 bits of them, below it has steps of 2^-(24 + kLeast) of that: a first key that has nearly all weight, and a value that adds little, leaves the others
-// what they are. A
-// closer reference costs prompts more moves: 4096 tokens of 32 heads over 16 take 187 us with 8, 194 with 11, 206 with 13.
+// what they are. A closer reference costs prompts more moves: 4096 tokens of 32 heads over 16 take 187 us with 8, 194 with 11, 206 with 13.
 constexpr float kLeast = 8.f, kMost = 15.f;
 __device__ __forceinline__ float exp2_fast(float x) {
     float y;

@@ -127,6 +127,15 @@ def test_wide_caps(cap, kind):
 
 
 @BOTH
+@pytest.mark.parametrize("cap", [1e-30, 1e-38, 1e-40, 1e-46])
+def test_caps_next_to_nothing(cap, kind):
+    """Every key weighs the same, also where f32 does not hold the cap."""
+    f = Form(4, 2, 64, 128, 64, softcap=cap, scale=cap * 1e25)
+    base.check(f, [(100, 150), (1, 90)], kind)
+    base.check(f, [(1, 700), (1, 3)], kind, seed=1)
+
+
+@BOTH
 @pytest.mark.parametrize("cap", [300.0, 4e3, 1e4, 1e6])
 @pytest.mark.parametrize("lengths", STEPS, ids=str)
 def test_scores_on_both_sides_of_a_quarter_of_a_wide_cap(lengths, cap, kind):
